@@ -428,6 +428,76 @@ int pico_cross_entropy_mean_bwd(const void* logits, const int64_t* targets, cons
                                 const float* grad_out, void* dlogits, int have_unit, int64_t rows, int64_t vocab, int64_t ld,
                                 int64_t dld, int64_t ignore_index, int dtype, void* stream);
 
+/* ------------------------------------------------------------------ log-probabilities of given tokens, and losses made of them
+ * No counterpart in the reference (its training ends at the cross-entropy): what preference and policy training need next to it.
+ * Logits are rows of `vocab` contiguous elements, row (b, s) at data + b * batch_stride + s * row_stride (elements, not negative);
+ * a row may start at any element.  A value or token per row has two strides of its own, 0 among them (broadcast).
+ * A target that equals ignore_index or lies outside [0, vocab) is never used as an index: the row is not read, its results are
+ * 0 and so is its gradient row.  z = logits / temperature, p = softmax(z), q = log p_target.  batch * seq < 2^31, vocab < 2^30.
+ * dlogits: rows that do not overlap, each as far from a 16-byte boundary as its row of logits (buffers of the logits' own
+ * strides whose addresses agree modulo 16 do); it may be the logits themselves.
+ */
+typedef struct pico_logits {
+  const void* data;
+  int64_t batch, seq, vocab;
+  int64_t batch_stride, row_stride;
+  int32_t dtype;                       /* PICO_BF16 or PICO_F32 */
+  int32_t reserved;
+} pico_logits;
+typedef struct pico_tokens {
+  const int64_t* data;
+  int64_t batch_stride, row_stride;
+} pico_tokens;
+typedef struct pico_values {
+  const float* data;
+  int64_t batch_stride, row_stride;
+} pico_values;
+
+/* log_probs = q and, where entropy is given, entropy = -sum_j p_j ln p_j, both fp32 [batch, seq] contiguous.  max_sum: [batch, seq, 2]
+ * fp32, 8-byte aligned, what the gradient needs of a row; may be NULL.
+ */
+int pico_log_probs_fwd(const pico_logits* logits, const pico_tokens* targets, float* log_probs, float* entropy, float* max_sum,
+                       float temperature, int64_t ignore_index, void* stream);
+/* dlogits of sum over rows of dlog_probs * q + dentropy * H: (dlog_probs ([j = target] - p_j) - dentropy p_j (ln p_j + H)) / temperature.
+ * Either of the two (not both) may be NULL; entropy ([batch, seq], from the forward) is needed with dentropy only.  grad_out: an optional
+ * factor of both (device float).  have_unit != 0: dlogits holds the gradient for a factor of 1 already and is left as it is where
+ * grad_out[0] is 1 (decided on the device).  A row whose factors are 0 gets a gradient of 0 and is not read.
+ */
+int pico_log_probs_bwd(const pico_logits* logits, const pico_tokens* targets, const float* max_sum, const float* entropy,
+                       const pico_values* dlog_probs, const pico_values* dentropy, const float* grad_out, int have_unit,
+                       void* dlogits, int64_t dbatch_stride, int64_t drow_stride, float temperature, int64_t ignore_index, void* stream);
+
+/* The clipped policy loss: per row that counts
+ *   ratio = exp(q - old),  l = -min(ratio A, clamp(ratio, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(ref - q) - (ref - q) - 1) - entropy_coef H
+ * and loss[0] = scale * sum of weight * l, or, where weights are not given, scale * the mean of l over the rows that count (0 where none does).
+ * old_log_probs not given: the policy's own (ratio 1, gradient -A).  All but the logits are constants.  Where both sides of the minimum are equal
+ * the gradient is the first's.
+ * log_probs (q), losses (weight * l): fp32 [batch, seq].  With dlogits the gradient for an upstream gradient of 1 is written in the same call, and
+ * `saved` ([batch, seq] each, max_sum [batch, seq, 2]; entropy and dentropy with an entropy term only) is what pico_log_probs_bwd needs for another
+ * one.  inv_count: one device float, scratch.
+ */
+typedef struct pico_policy {
+  pico_values advantages, old_log_probs, ref_log_probs, weights;   /* the last three: data may be NULL */
+  float clip_low, clip_high, kl_coef, entropy_coef, scale;
+} pico_policy;
+typedef struct pico_policy_saved {
+  float *max_sum, *dlog_probs, *entropy, *dentropy;
+} pico_policy_saved;
+int pico_policy_loss_fwd(const pico_logits* logits, const pico_tokens* targets, const pico_policy* policy, float* loss, float* log_probs,
+                         float* losses, float* inv_count, const pico_policy_saved* saved, void* dlogits, int64_t dbatch_stride,
+                         int64_t drow_stride, float temperature, int64_t ignore_index, void* stream);
+
+/* The preference loss over pairs: sequence i < batch / 2 is the chosen one of pair i, sequence batch / 2 + i the rejected one.
+ *   L = sum of q over a sequence's rows that count, or with average != 0 their mean (0 where none does);
+ *   x = beta ((L_chosen - ref_chosen) - (L_rejected - ref_rejected));  loss[0] = scale * mean of (1 - label_smoothing) softplus(-x) + label_smoothing softplus(x)
+ * (0 without pairs).  ref_log_probs: [batch] fp32 or NULL (0).  sequence_log_probs: L, [batch] fp32.  slope: [batch], dloss / dq of every row of the
+ * sequence that counts: the gradient is pico_log_probs_bwd with dlog_probs = {slope, 1, 0}.  log_probs: q, [batch, seq] fp32; max_sum as
+ * above; workspace: batch doubles.  The sums over rows and pairs are in double, always in the same order.
+ */
+int pico_preference_loss_fwd(const pico_logits* logits, const pico_tokens* targets, const float* ref_log_probs, float beta,
+                             float label_smoothing, int average, float scale, float* loss, float* sequence_log_probs, float* slope,
+                             float* log_probs, float* max_sum, void* workspace, int64_t ignore_index, void* stream);
+
 /* ------------------------------------------------------------------ optimizer step
  * replaces: torch.optim.AdamW(model.parameters(), lr).step()  train.py:204-209,240  for low-precision parameters
  *           with fp32 state: the reference keeps the AdamW state in the parameter dtype; here master weights and

@@ -40,8 +40,31 @@ class KvChunks(Structure):
                 ("accumulate_mask", ctypes.c_uint32), ("reserved", ctypes.c_uint32)]
 
 
+class Logits(Structure):
+    """Mirror of ``pico_logits``."""
+    _fields_ = [("data", c_void_p), ("batch", c_int64), ("seq", c_int64), ("vocab", c_int64), ("batch_stride", c_int64), ("row_stride", c_int64),
+                ("dtype", c_int32), ("reserved", c_int32)]
+
+
+class PerRow(Structure):
+    """Mirror of ``pico_tokens`` and ``pico_values``."""
+    _fields_ = [("data", c_void_p), ("batch_stride", c_int64), ("row_stride", c_int64)]
+
+
+class Policy(Structure):
+    """Mirror of ``pico_policy``."""
+    _fields_ = [("advantages", PerRow), ("old_log_probs", PerRow), ("ref_log_probs", PerRow), ("weights", PerRow),
+                ("clip_low", c_float), ("clip_high", c_float), ("kl_coef", c_float), ("entropy_coef", c_float), ("scale", c_float)]
+
+
+class PolicySaved(Structure):
+    """Mirror of ``pico_policy_saved``."""
+    _fields_ = [("max_sum", c_void_p), ("dlog_probs", c_void_p), ("entropy", c_void_p), ("dentropy", c_void_p)]
+
+
 _P = c_void_p
 _I64 = c_int64
+_ROWS = [POINTER(Logits), POINTER(PerRow)]
 SIGNATURES = {
     "pico_version": (c_char_p, []),
     "pico_last_error": (c_char_p, []),
@@ -80,6 +103,10 @@ SIGNATURES = {
     "pico_cross_entropy_mean_fwd": (c_int, [_P] * 7 + [_I64] * 5 + [c_int, _P]),
     "pico_cross_entropy_scaled_mean_fwd": (c_int, [_P] * 7 + [c_float] + [_I64] * 5 + [c_int, _P]),
     "pico_cross_entropy_mean_bwd": (c_int, [_P] * 6 + [c_int] + [_I64] * 5 + [c_int, _P]),
+    "pico_log_probs_fwd": (c_int, _ROWS + [_P, _P, _P, c_float, _I64, _P]),
+    "pico_log_probs_bwd": (c_int, _ROWS + [_P, _P, POINTER(PerRow), POINTER(PerRow), _P, c_int, _P, _I64, _I64, c_float, _I64, _P]),
+    "pico_policy_loss_fwd": (c_int, _ROWS + [POINTER(Policy), _P, _P, _P, _P, POINTER(PolicySaved), _P, _I64, _I64, c_float, _I64, _P]),
+    "pico_preference_loss_fwd": (c_int, _ROWS + [_P, c_float, c_float, c_int, c_float, _P, _P, _P, _P, _P, _P, _I64, _P]),
     "pico_adamw": (c_int, [_P, _P, _P, c_int, _P, _P, _I64] + [ctypes.c_float] * 5 + [_I64, ctypes.c_float, _P]),
     "pico_adamw_lp": (c_int, [_P, _P, c_int, _P, _P, _I64, c_int, c_int] + [ctypes.c_float] * 5 + [_I64, ctypes.c_float, _P]),
     "pico_adamw_multi": (c_int, [c_int, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int] + [ctypes.c_float] * 5 + [_I64, ctypes.c_float, _P]),

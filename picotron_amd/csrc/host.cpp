@@ -1335,6 +1335,251 @@ Tensor cross_entropy(const Tensor& logits, const Tensor& targets, int64_t ignore
   return CrossEntropy::apply(logits, targets, ignore_index, scale);
 }
 
+// ------------------------------------------------------------------------------------------------ log-probabilities of given tokens
+// [..., V] logits as the library takes them: [batch, seq, V] of any strides but a unit one on V, one target and value per row.
+struct TokenRows {
+  Tensor logits, targets;   // [batch, seq, V], [batch, seq]
+  pico_logits z;
+  pico_tokens t;
+};
+Tensor per_row(const Tensor& t) {   // [...] -> [batch, seq]
+  return t.dim() == 2 ? t : t.dim() < 2 ? t.reshape({1, -1}) : t.flatten(0, -2);
+}
+void check_tokens(const char* fn, const Tensor& x, const Tensor& targets) {
+  on_gpu(x);
+  on_gpu(targets);
+  TORCH_CHECK(targets.scalar_type() == at::kLong, fn, ": targets must be int64 (got ", targets.scalar_type(), ")");
+  TORCH_CHECK(x.dim() >= 1 && targets.sizes() == x.sizes().slice(0, x.dim() - 1), fn, ": targets must have one entry per row (got ", targets.sizes(), " for ", x.sizes(), ")");
+  TORCH_CHECK(targets.device() == x.device(), fn, ": targets must be on ", x.device());
+}
+TokenRows token_rows(const char* fn, const Tensor& logits, const Tensor& targets) {
+  check_tokens(fn, logits, targets);
+  TORCH_CHECK(logits.size(-1) == 1 || logits.stride(-1) == 1, fn, ": logits must have a unit stride on the vocabulary");
+  TokenRows r;
+  r.logits = logits.dim() == 3 ? logits : logits.dim() == 2 ? logits.unsqueeze(0) : logits.dim() == 1 ? logits.reshape({1, 1, -1}) : logits.flatten(0, -3);
+  r.targets = per_row(targets);
+  r.z = {ptr(r.logits), r.logits.size(0), r.logits.size(1), r.logits.size(2), r.logits.stride(0), r.logits.stride(1), dtype_code(logits, "logits"), 0};
+  r.t = {r.targets.data_ptr<int64_t>(), r.targets.stride(0), r.targets.stride(1)};
+  return r;
+}
+// an fp32 value per row, broadcast to the targets' shape without a copy; the result keeps the tensor alive
+struct RowValues {
+  Tensor t;
+  pico_values v = {nullptr, 0, 0};
+};
+RowValues row_values(const char* fn, const char* what, const Tensor& v, const Tensor& targets) {
+  on_gpu(v);
+  TORCH_CHECK(v.device() == targets.device(), fn, ": ", what, " must be on ", targets.device());
+  TORCH_CHECK(v.is_floating_point(), fn, ": ", what, " must be a floating-point tensor");
+  TORCH_CHECK(at::is_expandable_to(v.sizes(), targets.sizes()), fn, ": ", what, " must have a value per target or broadcast to ", targets.sizes(), " (got ", v.sizes(), ")");
+  RowValues r;
+  r.t = per_row(v.detach().to(at::kFloat).expand(targets.sizes()));
+  r.v = {static_cast<const float*>(r.t.data_ptr()), r.t.stride(0), r.t.stride(1)};
+  return r;
+}
+RowValues row_values(const char* fn, const char* what, const OptTensor& v, const Tensor& targets) {
+  return v && v->defined() ? row_values(fn, what, *v, targets) : RowValues();
+}
+
+// A fresh gradient of the logits, every row as far from a 16-byte boundary as the row of logits (contiguous where they are).
+Tensor gradient_rows(const Tensor& z) {
+  const int64_t vec = 16 / z.element_size(), B = z.size(0), S = z.size(1), V = z.size(2);
+  auto alike = [&](int64_t least, int64_t as) { return least + ((as - least) % vec + vec) % vec; };
+  const int64_t row = S > 1 ? alike(V, z.stride(1)) : V, batch = B > 1 ? alike(S * row, z.stride(0)) : S * row;
+  const int64_t past = static_cast<int64_t>(reinterpret_cast<uintptr_t>(z.data_ptr()) % 16) / z.element_size();
+  if (z.numel() == 0) return at::empty(z.sizes(), z.options());
+  const Tensor buffer = at::empty({past + (B - 1) * batch + (S - 1) * row + V}, z.options());
+  return buffer.as_strided({B, S, V}, {batch, row, 1}, past);
+}
+Tensor per_token(const Tensor& targets, const Tensor& like, int64_t values = 1) {
+  auto sizes = targets.sizes().vec();
+  if (values > 1) sizes.push_back(values);
+  return at::empty(sizes, like.options().dtype(at::kFloat));
+}
+void refuse_second_order(const char* fn) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), fn, ": its gradient cannot be differentiated again (create_graph)");
+}
+// d(logits) of `up` times (dlp q + dh H) per row, in `d` where that holds the gradient for a factor of 1 already
+Tensor log_probs_gradient(const TokenRows& r, const Tensor& max_sum, const Tensor& entropy, const RowValues& dlp, const RowValues& dh, const Tensor& up, Tensor d,
+                          double temperature, int64_t ignore_index) {
+  const bool have_unit = d.defined();
+  if (!have_unit) d = gradient_rows(r.logits);
+  check(pico_log_probs_bwd(&r.z, &r.t, fptr(max_sum), fptr(entropy), &dlp.v, &dh.v, fptr(up), have_unit, ptr(d), d.stride(0), d.stride(1),
+                           static_cast<float>(temperature), ignore_index, stream_now()));
+  return d;
+}
+
+// log p of the targets and, if asked for, the entropy of every row's distribution
+struct LogProbs : torch::autograd::Function<LogProbs> {
+  static variable_list run(const Tensor& logits, const Tensor& targets, int64_t ignore_index, double temperature, bool entropy, Tensor* max_sum) {
+    const c10::OptionalDeviceGuard device(logits.device());
+    const TokenRows r = token_rows("log_probs", logits, targets);
+    variable_list out = {per_token(targets, logits)};
+    if (entropy) out.push_back(per_token(targets, logits));
+    if (max_sum) *max_sum = per_token(targets, logits, 2);
+    check(pico_log_probs_fwd(&r.z, &r.t, fptr(out[0]), entropy ? fptr(out[1]) : nullptr, max_sum ? fptr(*max_sum) : nullptr, static_cast<float>(temperature),
+                             ignore_index, stream_now()));
+    return out;
+  }
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& targets, int64_t ignore_index, double temperature, bool entropy) {
+    Tensor max_sum;
+    variable_list out = run(logits, targets, ignore_index, temperature, entropy, &max_sum);
+    ctx->save_for_backward({logits, targets, max_sum, entropy ? out[1] : Tensor()});
+    ctx->saved_data["ignore"] = ignore_index;
+    ctx->saved_data["temperature"] = temperature;
+    ctx->set_materialize_grads(false);
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    refuse_second_order("log_probs");
+    const auto s = ctx->get_saved_variables();
+    variable_list d(5);
+    if (!g[0].defined() && (g.size() < 2 || !g[1].defined())) return d;
+    const c10::OptionalDeviceGuard device(s[0].device());
+    const TokenRows r = token_rows("log_probs", s[0], s[1]);
+    const RowValues dlp = row_values("log_probs", "the gradient", OptTensor(g[0]), s[1]);
+    const RowValues dh = row_values("log_probs", "the gradient", g.size() > 1 ? OptTensor(g[1]) : std::nullopt, s[1]);
+    d[0] = log_probs_gradient(r, s[2], s[3], dlp, dh, Tensor(), Tensor(), ctx->saved_data["temperature"].toDouble(), ctx->saved_data["ignore"].toInt()).view(s[0].sizes());
+    return d;
+  }
+};
+variable_list log_probs(const Tensor& logits, const Tensor& targets, int64_t ignore_index, double temperature, bool entropy) {
+  if (!records({&logits})) return LogProbs::run(logits, targets, ignore_index, temperature, entropy, nullptr);
+  return LogProbs::apply(logits, targets, ignore_index, temperature, entropy);
+}
+
+// The two losses write or keep what the gradient for a unit upstream gradient needs; the kernel of the backward looks at the
+// real one on the device.
+struct PolicyOptions {
+  double clip_low, clip_high, kl_coef, entropy_coef, temperature, scale;
+  int64_t ignore_index;
+};
+struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
+  struct Saved {
+    Tensor unit, max_sum, dlp, entropy, dentropy;
+  };
+  static variable_list run(const Tensor& logits, const Tensor& targets, const Tensor& advantages, const OptTensor& old_lp, const OptTensor& ref_lp,
+                           const OptTensor& weights, const PolicyOptions& o, Saved* saved) {
+    const char* fn = "policy_loss";
+    const c10::OptionalDeviceGuard device(logits.device());
+    const TokenRows r = token_rows(fn, logits, targets);
+    const RowValues A = row_values(fn, "advantages", advantages, targets), old = row_values(fn, "old_log_probs", old_lp, targets),
+                    ref = row_values(fn, "ref_log_probs", ref_lp, targets), w = row_values(fn, "weights", weights, targets);
+    const auto f32 = logits.options().dtype(at::kFloat);
+    const Tensor loss = at::empty({}, f32), inv_count = at::empty({}, f32), lp = per_token(targets, logits), losses = per_token(targets, logits);
+    const pico_policy p = {A.v, old.v, ref.v, w.v, static_cast<float>(o.clip_low), static_cast<float>(o.clip_high), static_cast<float>(o.kl_coef),
+                           static_cast<float>(o.entropy_coef), static_cast<float>(o.scale)};
+    pico_policy_saved kept = {};
+    if (saved) {
+      saved->unit = gradient_rows(r.logits);
+      saved->max_sum = per_token(targets, logits, 2);
+      saved->dlp = per_token(targets, logits);
+      if (p.entropy_coef != 0) {
+        saved->entropy = per_token(targets, logits);
+        saved->dentropy = per_token(targets, logits);
+      }
+      kept = {fptr(saved->max_sum), fptr(saved->dlp), fptr(saved->entropy), fptr(saved->dentropy)};
+    }
+    check(pico_policy_loss_fwd(&r.z, &r.t, &p, fptr(loss), fptr(lp), fptr(losses), fptr(inv_count), &kept, saved ? ptr(saved->unit) : nullptr,
+                               saved ? saved->unit.stride(0) : 0, saved ? saved->unit.stride(1) : 0, static_cast<float>(o.temperature), o.ignore_index, stream_now()));
+    return {loss, lp};
+  }
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& targets, const Tensor& advantages, const OptTensor& old_lp,
+                               const OptTensor& ref_lp, const OptTensor& weights, double clip_low, double clip_high, double kl_coef, double entropy_coef,
+                               int64_t ignore_index, double temperature, double scale) {
+    Saved k;
+    variable_list out = run(logits, targets, advantages, old_lp, ref_lp, weights, {clip_low, clip_high, kl_coef, entropy_coef, temperature, scale, ignore_index}, &k);
+    ctx->save_for_backward({logits, targets, k.unit, k.max_sum, k.dlp, k.entropy, k.dentropy});
+    ctx->saved_data["ignore"] = ignore_index;
+    ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["spent"] = false;
+    ctx->mark_non_differentiable({out[1]});
+    ctx->set_materialize_grads(false);
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    refuse_second_order("policy_loss");
+    variable_list d(13);
+    if (!g[0].defined()) return d;
+    const auto s = ctx->get_saved_variables();
+    const c10::OptionalDeviceGuard device(s[0].device());
+    const TokenRows r = token_rows("policy_loss", s[0], s[1]);
+    const Tensor up = g[0].to(at::kFloat).contiguous();
+    // a second backward through this node (retain_graph) gets a buffer of its own
+    const bool spent = ctx->saved_data["spent"].toBool();
+    ctx->saved_data["spent"] = true;
+    const RowValues dlp = row_values("policy_loss", "the gradient", s[4], s[1]);
+    const RowValues dh = row_values("policy_loss", "the gradient", s[6].defined() ? OptTensor(s[6]) : std::nullopt, s[1]);
+    d[0] = log_probs_gradient(r, s[3], s[5], dlp, dh, up, spent ? Tensor() : s[2], ctx->saved_data["temperature"].toDouble(),
+                              ctx->saved_data["ignore"].toInt()).view(s[0].sizes());
+    return d;
+  }
+};
+std::pair<Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& targets, const Tensor& advantages, const OptTensor& old_lp, const OptTensor& ref_lp,
+                                      const OptTensor& weights, double clip_low, double clip_high, double kl_coef, double entropy_coef, int64_t ignore_index,
+                                      double temperature, double scale) {
+  const variable_list out = records({&logits})
+      ? PolicyLoss::apply(logits, targets, advantages, old_lp, ref_lp, weights, clip_low, clip_high, kl_coef, entropy_coef, ignore_index, temperature, scale)
+      : PolicyLoss::run(logits, targets, advantages, old_lp, ref_lp, weights, {clip_low, clip_high, kl_coef, entropy_coef, temperature, scale, ignore_index}, nullptr);
+  return {out[0], out[1]};
+}
+
+// logits [2 pairs, seq, V]: the chosen sequences, then the rejected ones
+struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
+  static variable_list run(const Tensor& logits, const Tensor& targets, const OptTensor& ref_lp, double beta, double smoothing, bool average, int64_t ignore_index,
+                           double scale, Tensor* max_sum, Tensor* slope_out) {
+    const char* fn = "preference_loss";
+    const c10::OptionalDeviceGuard device(logits.device());
+    TORCH_CHECK(logits.dim() == 3, fn, ": logits must be [2 pairs, seq, vocab], the chosen sequences before the rejected ones (got ", logits.sizes(), ")");
+    const TokenRows r = token_rows(fn, logits, targets);
+    const int64_t B = logits.size(0);
+    Tensor ref;
+    if (ref_lp) {
+      on_gpu(*ref_lp);
+      TORCH_CHECK(ref_lp->is_floating_point() && ref_lp->dim() == 1 && ref_lp->size(0) == B && ref_lp->device() == logits.device(), fn,
+                  ": ref_log_probs must hold one value per sequence (", B, ") on ", logits.device());
+      ref = ref_lp->detach().to(at::kFloat).contiguous();
+    }
+    const auto f32 = logits.options().dtype(at::kFloat);
+    const Tensor loss = at::empty({}, f32), sequence = at::empty({B}, f32), slope = at::empty({B}, f32), lp = per_token(targets, logits),
+                 ws = at::empty({B}, logits.options().dtype(at::kDouble));
+    if (max_sum) {
+      *max_sum = per_token(targets, logits, 2);
+      *slope_out = slope;
+    }
+    check(pico_preference_loss_fwd(&r.z, &r.t, fptr(ref), static_cast<float>(beta), static_cast<float>(smoothing), average, static_cast<float>(scale), fptr(loss),
+                                   fptr(sequence), fptr(slope), fptr(lp), max_sum ? fptr(*max_sum) : nullptr, ptr(ws), ignore_index, stream_now()));
+    return {loss, sequence};
+  }
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& targets, const OptTensor& ref_lp, double beta, double smoothing,
+                               bool average, int64_t ignore_index, double scale) {
+    Tensor max_sum, slope;
+    variable_list out = run(logits, targets, ref_lp, beta, smoothing, average, ignore_index, scale, &max_sum, &slope);
+    ctx->save_for_backward({logits, targets, max_sum, slope});
+    ctx->saved_data["ignore"] = ignore_index;
+    ctx->mark_non_differentiable({out[1]});
+    ctx->set_materialize_grads(false);
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    refuse_second_order("preference_loss");
+    variable_list d(8);
+    if (!g[0].defined()) return d;
+    const auto s = ctx->get_saved_variables();
+    const c10::OptionalDeviceGuard device(s[0].device());
+    const TokenRows r = token_rows("preference_loss", s[0], s[1]);
+    const RowValues dlp = row_values("preference_loss", "the gradient", s[3].unsqueeze(1), s[1]);
+    d[0] = log_probs_gradient(r, s[2], Tensor(), dlp, RowValues(), g[0].to(at::kFloat).contiguous(), Tensor(), 1.0, ctx->saved_data["ignore"].toInt());
+    return d;
+  }
+};
+std::pair<Tensor, Tensor> preference_loss(const Tensor& logits, const Tensor& targets, const OptTensor& ref_lp, double beta, double smoothing, bool average,
+                                          int64_t ignore_index, double scale) {
+  const variable_list out = records({&logits}) ? PreferenceLoss::apply(logits, targets, ref_lp, beta, smoothing, average, ignore_index, scale)
+                                               : PreferenceLoss::run(logits, targets, ref_lp, beta, smoothing, average, ignore_index, scale, nullptr, nullptr);
+  return {out[0], out[1]};
+}
+
 // ------------------------------------------------------------------------------------------------ AdamW
 // The step for a fixed list of tensors in as few launches as they fit.  Weights, moments and sizes are checked and their
 // pointer tables built once; a step only fills in the gradients' addresses.
@@ -1504,6 +1749,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         pybind11::arg("scale") = 1.0, nogil());
   m.def("cross_entropy_fwd", &cross_entropy_fwd, nogil());
   m.def("cross_entropy_bwd", &cross_entropy_bwd, nogil());
+  m.def("log_probs", &log_probs, nogil());
+  m.def("policy_loss", &policy_loss, nogil());
+  m.def("preference_loss", &preference_loss, nogil());
   m.def("zero_grads", &zero_grads);
   py::class_<AdamWPlan>(m, "AdamWPlan")
       .def(py::init<const std::vector<Tensor>&, const std::vector<Tensor>&, const std::vector<Tensor>&, const std::optional<OptTensors>&>())

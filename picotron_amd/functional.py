@@ -61,6 +61,16 @@ class FlashAttnFunc:
         return _lib.host().flash_attention(q, k, v, sm_scale, causal, True)
 
 
+def _check_targets(what, targets, vocab, ignore_index):
+    """F.cross_entropy asserts on the device for a target outside [0, vocab) (train.py:46-49); the kernels skip such a row
+    instead (they may not index with it), which would hide a tokenizer / vocabulary mismatch.  This opt-in check costs a
+    host synchronisation."""
+    if os.getenv("PICO_CHECK_TARGETS", "0") == "1":
+        bad = (targets != ignore_index) & ((targets < 0) | (targets >= vocab))
+        if bool(bad.any()):
+            raise RuntimeError(f"{what}: {int(bad.sum())} targets lie outside [0, {vocab}) and are not ignore_index={ignore_index}")
+
+
 class CrossEntropyFunc:
     """``apply(logits, targets, ignore_index, scale)``: `scale` times the mean cross-entropy of [rows, vocab] logits against
     int64 targets (``train.py:46-49``), fp32 loss.  The gradient leaves in the dtype of the logits; the upstream gradient and the
@@ -73,14 +83,7 @@ class CrossEntropyFunc:
 
     @staticmethod
     def apply(logits, targets, ignore_index=-100, scale=1.0):
-        if os.getenv("PICO_CHECK_TARGETS", "0") == "1":
-            # F.cross_entropy asserts on the device for a target outside [0, vocab) (train.py:46-49); the kernels skip such
-            # a row instead (they may not index with it), which would hide a tokenizer / vocabulary mismatch.  This
-            # opt-in check costs a host synchronisation.
-            bad = (targets != ignore_index) & ((targets < 0) | (targets >= logits.size(-1)))
-            if bool(bad.any()):
-                raise RuntimeError(f"cross_entropy: {int(bad.sum())} targets lie outside [0, {logits.size(-1)}) and are not "
-                                   f"ignore_index={ignore_index}")
+        _check_targets("cross_entropy", targets, logits.size(-1), ignore_index)
         return _lib.host().cross_entropy(logits, targets, ignore_index, scale)
 
 
@@ -89,6 +92,49 @@ def cross_entropy(logits, targets, ignore_index: int = -100, scale: float = 1.0)
     accumulation ``cross_entropy(logits, targets, scale=1 / steps).backward()`` is the fast form of
     ``(cross_entropy(logits, targets) / steps).backward()``: [4096, 49152] in bf16 150 us against 293."""
     return CrossEntropyFunc.apply(logits, targets, ignore_index, scale)
+
+
+def log_probs(logits, targets, ignore_index: int = -100, temperature: float = 1.0, entropy: bool = False):
+    """Log-probabilities of the tokens `targets` [...] (int64) under softmax(logits / temperature), logits [..., vocab] in bf16
+    or fp32: fp32, shaped like the targets, differentiable.  With `entropy` also the entropy of every row's distribution, which
+    is differentiable too: (log_probs, entropy).  Rows whose target is `ignore_index` give 0 and are not read.  The last axis needs
+    a unit stride, the others may have any (``logits[:, :-1]`` is taken as it is)."""
+    _check_targets("log_probs", targets, logits.size(-1), ignore_index)
+    out = _lib.host().log_probs(logits, targets, ignore_index, temperature, entropy)
+    return tuple(out) if entropy else out[0]
+
+
+def policy_loss(logits, targets, advantages, old_log_probs=None, ref_log_probs=None, weights=None, clip=(0.2, 0.2), kl_coef: float = 0.0,
+                entropy_coef: float = 0.0, ignore_index: int = -100, temperature: float = 1.0, scale: float = 1.0):
+    """The clipped policy loss over sampled tokens, from their logits: returns (loss, log_probs), the second without a gradient.
+    With q the log-probability of a token under softmax(logits / temperature) and A its advantage
+
+        ratio = exp(q - old_log_probs)                    (old_log_probs None: of this policy itself, ratio 1)
+        l = -min(ratio A, clamp(ratio, 1 - clip[0], 1 + clip[1]) A)
+            + kl_coef (exp(ref - q) - (ref - q) - 1) - entropy_coef * entropy
+
+    and loss = `scale` times the mean of l over the tokens whose target is not `ignore_index`, or times the sum of `weights` * l
+    (1 / (answers * tokens of the answer) averages each answer first).  advantages, old_log_probs, ref_log_probs and weights are
+    constants that broadcast to the targets' shape (one advantage per answer: [batch, 1]).  Where a gradient will be wanted the
+    forward already writes it for an upstream gradient of 1, as cross_entropy does: a factor known beforehand goes into `scale`."""
+    _check_targets("policy_loss", targets, logits.size(-1), ignore_index)
+    return _lib.host().policy_loss(logits, targets, advantages, old_log_probs, ref_log_probs, weights, clip[0], clip[1], kl_coef, entropy_coef,
+                                   ignore_index, temperature, scale)
+
+
+def preference_loss(logits, targets, ref_log_probs=None, beta: float = 0.1, label_smoothing: float = 0.0, average: bool = False,
+                    ignore_index: int = -100, scale: float = 1.0):
+    """The preference loss over pairs of answers: logits [2 pairs, seq, vocab] and targets [2 pairs, seq] hold the chosen answers and
+    behind them the rejected ones, in the same order.  Returns (loss, log_probs), the second [2 pairs] without a gradient:
+
+        log_probs = the sum of log softmax(logits)[target] over an answer's tokens (their mean with `average`),
+        x = beta * ((chosen - ref_chosen) - (rejected - ref_rejected))
+        loss = scale * mean over pairs of -(1 - label_smoothing) log sigmoid(x) - label_smoothing log sigmoid(-x)
+
+    with ref_log_probs [2 pairs] the same sums (means) of the frozen reference, None for 0.  Tokens whose target is `ignore_index`
+    (prompts, padding) do not count; an answer without any has a log-probability of 0."""
+    _check_targets("preference_loss", targets, logits.size(-1), ignore_index)
+    return _lib.host().preference_loss(logits, targets, ref_log_probs, beta, label_smoothing, average, ignore_index, scale)
 
 
 # ---------------------------------------------------------------------------------------------------------------

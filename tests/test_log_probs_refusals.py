@@ -1,0 +1,151 @@
+"""What the operators on log-probabilities refuse, at the C ABI and in the host path, before anything is launched (no GPU needed)."""
+import ctypes
+import os
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from picotron_amd import _lib
+    if not os.path.exists(_lib.LIB_PATH):
+        pytest.skip("library not built here")
+    return _lib.lib()
+
+
+def logits(data=4096, batch=2, seq=4, vocab=1000, dtype=0, **over):
+    from picotron_amd._lib import Logits
+    z = Logits(data, batch, seq, vocab, seq * vocab, vocab, dtype, 0)
+    for k, v in over.items():
+        setattr(z, k, v)
+    return z
+
+
+def tokens(data=4096):
+    from picotron_amd._lib import PerRow
+    return PerRow(data, 4, 1)
+
+
+BUF = ctypes.c_void_p(4096)      # never read: every call here is refused first
+R = ctypes.byref
+
+
+def message(lib):
+    return lib.pico_last_error().decode()
+
+
+@pytest.mark.parametrize("over,code", [(dict(dtype=7), -2), (dict(vocab=0), -3), (dict(vocab=1 << 30), -3), (dict(batch=-1), -3), (dict(batch=1 << 20, seq=1 << 12), -3),
+                                       (dict(data=None), -1), (dict(data=4097), -4), (dict(row_stride=-8), -5), (dict(batch_stride=-8), -5)])
+def test_logits_that_are_refused_everywhere(lib, over, code):
+    from picotron_amd._lib import PerRow, Policy, PolicySaved
+    z, t = logits(**over), tokens()
+    v = PerRow(4096, 4, 1)
+    p = Policy(v, v, v, v, 0.2, 0.2, 0.0, 0.0, 1.0)
+    saved = PolicySaved(4096, 4096, 4096, 4096)
+    assert lib.pico_log_probs_fwd(R(z), R(t), BUF, None, None, 1.0, -100, None) == code, message(lib)
+    assert lib.pico_log_probs_bwd(R(z), R(t), BUF, None, R(v), None, None, 0, BUF, 4000, 1000, 1.0, -100, None) == code, message(lib)
+    assert lib.pico_policy_loss_fwd(R(z), R(t), R(p), BUF, BUF, BUF, BUF, R(saved), None, 0, 0, 1.0, -100, None) == code, message(lib)
+    assert lib.pico_preference_loss_fwd(R(z), R(t), None, 0.1, 0.0, 0, 1.0, BUF, BUF, BUF, BUF, None, BUF, -100, None) == code, message(lib)
+
+
+@pytest.mark.parametrize("temperature", [0.0, -1.0, float("nan"), float("inf"), 1e-38])
+def test_temperatures(lib, temperature):
+    assert lib.pico_log_probs_fwd(R(logits()), R(tokens()), BUF, None, None, temperature, -100, None) == -3
+    assert "temperature" in message(lib)
+
+
+def test_missing_pointers(lib):
+    from picotron_amd._lib import PerRow, Policy, PolicySaved
+    z, t, v, none = logits(), tokens(), PerRow(4096, 4, 1), PerRow(None, 0, 0)
+    assert lib.pico_log_probs_fwd(None, R(t), BUF, None, None, 1.0, -100, None) == -1
+    assert lib.pico_log_probs_fwd(R(z), None, BUF, None, None, 1.0, -100, None) == -1
+    assert lib.pico_log_probs_fwd(R(z), R(tokens(None)), BUF, None, None, 1.0, -100, None) == -1
+    assert lib.pico_log_probs_fwd(R(z), R(t), None, None, None, 1.0, -100, None) == -1
+    assert lib.pico_log_probs_bwd(R(z), R(t), None, None, R(v), None, None, 0, BUF, 4000, 1000, 1.0, -100, None) == -1
+    assert lib.pico_log_probs_bwd(R(z), R(t), BUF, None, R(none), R(none), None, 0, BUF, 4000, 1000, 1.0, -100, None) == -1
+    assert lib.pico_log_probs_bwd(R(z), R(t), BUF, None, R(v), R(v), None, 0, BUF, 4000, 1000, 1.0, -100, None) == -1      # dentropy without entropy
+    assert lib.pico_log_probs_bwd(R(z), R(t), BUF, None, R(v), None, None, 1, BUF, 4000, 1000, 1.0, -100, None) == -1      # have_unit without grad_out
+    assert lib.pico_log_probs_bwd(R(z), R(t), BUF, None, R(v), None, None, 0, None, 4000, 1000, 1.0, -100, None) == -1
+    saved, p = PolicySaved(4096, 4096, None, None), Policy(v, none, none, none, 0.2, 0.2, 0.0, 0.0, 1.0)
+
+    def policy(p=p, saved=saved, d=None, loss=BUF):
+        return lib.pico_policy_loss_fwd(R(z), R(t), R(p) if p else None, loss, BUF, BUF, BUF, R(saved) if saved else None, d, 4000, 1000, 1.0, -100, None)
+    assert policy(p=None) == -1 and policy(loss=None) == -1
+    assert policy(p=Policy(none, none, none, none, 0.2, 0.2, 0.0, 0.0, 1.0)) == -1
+    assert policy(p=Policy(v, none, none, none, 0.2, 0.2, 0.1, 0.0, 1.0)) == -1 and "ref_log_probs" in message(lib)
+    assert policy(saved=None, d=BUF) == -1 and policy(saved=PolicySaved(), d=BUF) == -1
+    assert policy(p=Policy(v, none, none, none, 0.2, 0.2, 0.0, 0.5, 1.0), d=BUF) == -1                                     # entropy, nothing to keep it in
+    assert policy(p=Policy(v, none, none, none, -0.1, 0.2, 0.0, 0.0, 1.0)) == -3 and "clip" in message(lib)
+    assert policy(p=Policy(v, none, none, none, 0.2, float("nan"), 0.0, 0.0, 1.0)) == -3
+    assert lib.pico_preference_loss_fwd(R(z), R(t), None, 0.1, 0.0, 0, 1.0, None, BUF, BUF, BUF, None, BUF, -100, None) == -1
+    assert lib.pico_preference_loss_fwd(R(z), R(t), None, 0.1, 0.0, 0, 1.0, BUF, BUF, BUF, BUF, None, None, -100, None) == -1
+    assert lib.pico_preference_loss_fwd(R(z), R(t), None, 0.1, 1.5, 0, 1.0, BUF, BUF, BUF, BUF, None, BUF, -100, None) == -3
+    assert lib.pico_preference_loss_fwd(R(logits(batch=3)), R(t), None, 0.1, 0.0, 0, 1.0, BUF, BUF, BUF, BUF, None, BUF, -100, None) == -3 and "even" in message(lib)
+    assert lib.pico_preference_loss_fwd(R(z), R(t), None, 0.1, 0.0, 0, 1.0, BUF, BUF, BUF, BUF, None, ctypes.c_void_p(4100), -100, None) == -4
+
+
+@pytest.mark.parametrize("dtype,size", [(0, 2), (1, 4)])
+def test_gradients_that_overlap_or_lie_otherwise(lib, dtype, size):
+    from picotron_amd._lib import PerRow
+    z, t, v = logits(dtype=dtype), tokens(), PerRow(4096, 4, 1)
+
+    def bwd(d=4096, batch=4000, row=1000):
+        return lib.pico_log_probs_bwd(R(z), R(t), BUF, None, R(v), None, None, 0, ctypes.c_void_p(d), batch, row, 1.0, -100, None)
+    assert bwd(row=999) == -5 and bwd(batch=3999) == -5 and "overlap" in message(lib)
+    assert bwd(d=4096 + size) == -4 and bwd(row=1001, batch=4008) == -4 and bwd(batch=4001) == -4
+
+
+def test_host_path_refusals():
+    """Tensors on the CPU are refused, not computed, and shapes are looked at first."""
+    from picotron_amd.functional import log_probs, policy_loss, preference_loss
+    x, t = torch.zeros(2, 3, 8), torch.zeros(2, 3, dtype=torch.long)
+    for call in (lambda: log_probs(x, t), lambda: policy_loss(x, t, torch.zeros(2, 1)), lambda: preference_loss(x, t)):
+        with pytest.raises(RuntimeError, match="GPU only"):
+            call()
+
+
+@pytest.mark.gpu
+def test_host_path_refusals_on_the_gpu(device):
+    from picotron_amd.functional import log_probs, policy_loss, preference_loss
+    x = torch.zeros(2, 3, 8, device=device, dtype=torch.bfloat16)
+    t = torch.zeros(2, 3, dtype=torch.long, device=device)
+    A = torch.zeros(2, 1, device=device)
+
+    def refused(match, fn, *args, **kw):
+        with pytest.raises(RuntimeError, match=match):
+            fn(*args, **kw)
+    for fn, rest in ((log_probs, ()), (policy_loss, (A,)), (preference_loss, ())):
+        refused("one entry per row", fn, x, t[:, :2], *rest)
+        refused("int64", fn, x, t.int(), *rest)
+        refused("GPU only", fn, x, t.cpu(), *rest)
+        refused("unit stride", fn, x.transpose(1, 2).contiguous().transpose(1, 2), t, *rest)
+        refused("not supported", fn, x.half(), t, *rest)
+        y = x.clone().requires_grad_()
+        out = fn(y, t, *rest)
+        out = out if torch.is_tensor(out) else out[0]
+        refused("differentiated again", torch.autograd.grad, out.sum(), y, create_graph=True)
+    refused("temperature", log_probs, x, t, temperature=0.0)
+    refused("advantages", policy_loss, x, t, torch.zeros(3, 1, device=device))
+    refused("advantages", policy_loss, x, t, torch.zeros(2, 1, dtype=torch.long, device=device))
+    refused("GPU only", policy_loss, x, t, A.cpu())
+    refused("old_log_probs", policy_loss, x, t, A, torch.zeros(2, 2, device=device))
+    refused("ref_log_probs", policy_loss, x, t, A, kl_coef=0.1)
+    refused("weights", policy_loss, x, t, A, weights=torch.zeros(5, device=device))
+    refused("clip", policy_loss, x, t, A, clip=(-0.1, 0.2))
+    refused("even", preference_loss, x[:1], t[:1])
+    refused("2 pairs", preference_loss, x[0], t[0])
+    refused("ref_log_probs", preference_loss, x, t, torch.zeros(3, device=device))
+    refused("label_smoothing", preference_loss, x, t, label_smoothing=-0.1)
+
+
+@pytest.mark.gpu
+def test_targets_outside_the_vocabulary_can_be_checked(device, monkeypatch):
+    from picotron_amd.functional import log_probs, policy_loss, preference_loss
+    x = torch.zeros(2, 3, 8, device=device)
+    t = torch.zeros(2, 3, dtype=torch.long, device=device)
+    t[1, 1] = 8
+    monkeypatch.setenv("PICO_CHECK_TARGETS", "1")
+    for fn, rest in ((log_probs, ()), (policy_loss, (torch.zeros(2, 1, device=device),)), (preference_loss, ())):
+        with pytest.raises(RuntimeError, match="1 targets lie outside"):
+            fn(x, t, *rest)
