@@ -498,6 +498,24 @@ int pico_preference_loss_fwd(const pico_logits* logits, const pico_tokens* targe
                              float label_smoothing, int average, float scale, float* loss, float* sequence_log_probs, float* slope,
                              float* log_probs, float* max_sum, void* workspace, int64_t ignore_index, void* stream);
 
+/* Log-probabilities of given tokens straight from hidden states: z = x w^T / temperature for bf16 x [rows, hidden] (pitch ldx) and w [vocab, hidden]
+ * (pitch ldw), the vocabulary projection, without its logits in memory; log_probs [rows] fp32 = z_target - logsumexp(z) of the products' fp32
+ * sums (0 where the target does not count, as above).  max_sum: [rows, 2] fp32, what the gradient needs; may be NULL.  hidden must be a multiple of 8
+ * over 64, the pitches multiples of 8, x and w aligned to 16 bytes; targets: [rows] contiguous.
+ * workspace: pico_linear_log_probs_workspace_bytes(rows, vocab) bytes (an eighth of bf16 logits; -1: too large).
+ */
+int64_t pico_linear_log_probs_workspace_bytes(int64_t rows, int64_t vocab);
+int pico_linear_log_probs_fwd(const void* x, const void* w, const int64_t* targets, float* log_probs, float* max_sum, int64_t rows,
+                              int64_t hidden, int64_t vocab, int64_t ldx, int64_t ldw, float temperature, int64_t ignore_index,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+/* The gradient of sum over rows of dlog_probs * log_probs with respect to x w^T, bf16 [rows, vocab] with row pitch ldd = vocab rounded up to a multiple
+ * of 8 (zeros in the columns behind vocab): the products dlogits w and dlogits^T x of it are the gradients of x and w.  The logits are computed again.
+ * workspace: 16 bytes per row, 16-byte aligned.
+ */
+int pico_linear_log_probs_dlogits(const void* x, const void* w, const int64_t* targets, const float* max_sum, const float* dlog_probs,
+                                  void* dlogits, int64_t rows, int64_t hidden, int64_t vocab, int64_t ldx, int64_t ldw, int64_t ldd,
+                                  float temperature, int64_t ignore_index, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------ optimizer step
  * replaces: torch.optim.AdamW(model.parameters(), lr).step()  train.py:204-209,240  for low-precision parameters
  *           with fp32 state: the reference keeps the AdamW state in the parameter dtype; here master weights and

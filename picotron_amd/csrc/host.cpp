@@ -1580,6 +1580,66 @@ std::pair<Tensor, Tensor> preference_loss(const Tensor& logits, const Tensor& ta
   return {out[0], out[1]};
 }
 
+// log p of the targets under softmax(x w^T / temperature) without the logits in memory; the backward computes them again, as their
+// gradient, which lives until the two products with it are done.
+struct LinearLogProbs : torch::autograd::Function<LinearLogProbs> {
+  static Tensor rows(const Tensor& t) {   // as the products take them
+    const Tensor m = t.dim() == 1 ? t.unsqueeze(0) : matrix(t);
+    return m.stride(1) == 1 && m.stride(0) % 8 == 0 && m.stride(0) >= m.size(1) && reinterpret_cast<uintptr_t>(m.data_ptr()) % 16 == 0 ? m : m.contiguous();
+  }
+  static Tensor run(const Tensor& x, const Tensor& w, const Tensor& targets, int64_t ignore_index, double temperature, Tensor* max_sum) {
+    const char* fn = "linear_log_probs";
+    const c10::OptionalDeviceGuard device(x.device());
+    check_tokens(fn, x, targets);
+    on_gpu(w);
+    TORCH_CHECK(x.scalar_type() == at::kBFloat16 && w.scalar_type() == at::kBFloat16, fn, ": x and weight must be bf16 (got ", x.scalar_type(), " and ", w.scalar_type(), ")");
+    TORCH_CHECK(w.dim() == 2 && w.size(1) == x.size(-1) && w.device() == x.device(), fn, ": weight must be [vocab, ", x.size(-1), "] on ", x.device());
+    const Tensor a = rows(x), b = rows(w), t = targets.contiguous();
+    Tensor lp = per_token(targets, x);
+    if (max_sum) *max_sum = per_token(targets, x, 2);
+    const int64_t bytes = pico_linear_log_probs_workspace_bytes(a.size(0), b.size(0));
+    const Tensor ws = at::empty({std::max<int64_t>(bytes, 8)}, x.options().dtype(at::kByte));
+    check(pico_linear_log_probs_fwd(ptr(a), ptr(b), t.data_ptr<int64_t>(), fptr(lp), max_sum ? fptr(*max_sum) : nullptr, a.size(0), a.size(1), b.size(0), a.stride(0),
+                                    b.stride(0), static_cast<float>(temperature), ignore_index, ptr(ws), bytes, stream_now()));
+    return lp;
+  }
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& targets, int64_t ignore_index, double temperature) {
+    Tensor max_sum;
+    const Tensor lp = run(x, w, targets, ignore_index, temperature, &max_sum);
+    ctx->save_for_backward({x, w, targets, max_sum});
+    ctx->saved_data["ignore"] = ignore_index;
+    ctx->saved_data["temperature"] = temperature;
+    return lp;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    refuse_second_order("linear_log_probs");
+    const auto s = ctx->get_saved_variables();
+    const Tensor &x = s[0], &w = s[1];
+    const c10::OptionalDeviceGuard device(x.device());
+    const Tensor a = rows(x), b = rows(w), t = s[2].contiguous(), dlp = g[0].to(at::kFloat).contiguous();
+    const int64_t M = a.size(0), N = b.size(0), pitch = (N + 7) / 8 * 8;
+    const Tensor dz = at::empty({M, pitch}, a.options()), ws = at::empty({std::max<int64_t>(M * 16, 16)}, a.options().dtype(at::kByte));
+    check(pico_linear_log_probs_dlogits(ptr(a), ptr(b), t.data_ptr<int64_t>(), fptr(s[3]), fptr(dlp), ptr(dz), M, a.size(1), N, a.stride(0), b.stride(0), pitch,
+                                        static_cast<float>(ctx->saved_data["temperature"].toDouble()), ctx->saved_data["ignore"].toInt(), ptr(ws), M * 16, stream_now()));
+    const Tensor d = dz.narrow(1, 0, N);
+    variable_list r(5);
+    if (ctx->needs_input_grad(0) && ctx->needs_input_grad(1)) {
+      Gradients both = gradients(d, b, a);
+      r[0] = both.dx.view(x.sizes());
+      r[1] = both.dw;
+    } else if (ctx->needs_input_grad(0)) {
+      r[0] = product(d, b, Product::NN).view(x.sizes());
+    } else if (ctx->needs_input_grad(1)) {
+      r[1] = product(d, a, Product::TN);
+    }
+    return r;
+  }
+};
+Tensor linear_log_probs(const Tensor& x, const Tensor& w, const Tensor& targets, int64_t ignore_index, double temperature) {
+  if (!records({&x, &w})) return LinearLogProbs::run(x, w, targets, ignore_index, temperature, nullptr);
+  return LinearLogProbs::apply(x, w, targets, ignore_index, temperature);
+}
+
 // ------------------------------------------------------------------------------------------------ AdamW
 // The step for a fixed list of tensors in as few launches as they fit.  Weights, moments and sizes are checked and their
 // pointer tables built once; a step only fills in the gradients' addresses.
@@ -1752,6 +1812,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("log_probs", &log_probs, nogil());
   m.def("policy_loss", &policy_loss, nogil());
   m.def("preference_loss", &preference_loss, nogil());
+  m.def("linear_log_probs", &linear_log_probs, nogil());
   m.def("zero_grads", &zero_grads);
   py::class_<AdamWPlan>(m, "AdamWPlan")
       .def(py::init<const std::vector<Tensor>&, const std::vector<Tensor>&, const std::vector<Tensor>&, const std::optional<OptTensors>&>())

@@ -1,0 +1,320 @@
+// Log-probabilities of given tokens straight from hidden states x [M, K] and the vocabulary projection w [N, K]: the logits
+// z = x w^T / T are a matrix product whose tiles never leave the CU.
+//   forward : the product's epilogue reduces a tile to (max, sum of 2^D) per row and 64 columns (16 bytes of partial results
+//             for what would be 128 of bf16 logits and back), and picks the target's logit where its column passes; a second launch
+//             joins a row's partial results.
+//   backward: the product again (the logits were not kept), whose epilogue turns z into d(logits) = g ([j = t] - p_j) / T with the row's
+//             maximum and sum from the forward, bf16; the gradients of x and w are two more products.
+// The logits are the products' fp32 sums here, never rounded to bf16.
+#include "log_probs.h"
+#include "product_large.h"
+
+namespace pico {
+namespace {
+
+// of 16 columns each: a wave's share of a tile, and the width of a partial result
+constexpr int kJ = 4, kGroup = 16 * kJ;
+
+struct ScoreParams : LargeParams {
+  const int64_t* targets;   // [M]
+  f32x2* partial;           // [groups, M]
+  float* target_logit;      // [M]
+  float k;
+};
+
+// 4 bytes per lane to LDS, as request16_to
+template <int kPlus>
+__device__ __forceinline__ void request4_to(uint32_t lds_off, u32x4 window, uint32_t off) {
+  uint32_t aim;
+  asm volatile("s_add_u32 %0, %1, %2\n\ts_nop 0\n\tbuffer_load_dword %3, %4, 0 offen lds"
+               : "=&{m0}"(aim) : "s"(lds_off), "n"(kPlus), "v"(off), "s"(window) : "scc", "memory");
+}
+
+// the same value, of which the compiler does not know that it is (or it would keep what follows from it for all rows in registers)
+__device__ __forceinline__ int hidden(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+// Epilogue of the forward.  A lane holds columns 4 h ..+3 (h = lane / 16) of 16 consecutive ones, of row lane % 16 of 16: a row's 64
+// columns meet over four lanes.  128 exponentials a lane at a quarter of the vector rate are most of it.
+struct ScoreTile {
+  using Params = ScoreParams;
+  template <int I, int J> static constexpr int kStores = (I + 3) / 4;
+  template <int I> static constexpr int kBegun = I / 2;   // 256 bytes each: 32 rows
+  // the targets of the wave's rows, 8 bytes each, go to its rows region and are there long before the tile's end
+  template <int I>
+  static __device__ __forceinline__ void begin(const Params& p, const Unit& u, int wm, int lane, int wave, uint32_t lds_rows) {
+    lane = hidden(lane);
+    const int left = min(16 * I, p.M - u.m0 - wm);
+    const u32x4 window = request_window(reinterpret_cast<uint64_t>(p.targets + u.m0 + wm), left > 0 ? left * 8u : 0u);
+    wait_lds();
+    each(std::make_integer_sequence<int, kBegun<I>>(), [&](auto piece) __attribute__((always_inline)) {
+      request4_to<decltype(piece)::value * 256>(lds_rows, window, decltype(piece)::value * 256 + lane * 4);
+    });
+  }
+  template <int I, int J>
+  static __device__ __forceinline__ void tile(const Params& p, const Unit& u, int wm, int wn, int lane, const unsigned char* rows, f32x4 (&acc)[I][J]) {
+    lane = hidden(lane);
+    const int row0 = u.m0 + wm, col0 = u.n0 + wn, n = lane % 16, h = lane / 16, cols = p.N - col0;
+    const float k = p.k;
+    float top = 0.f, sum = 0.f;   // of row 64 q + lane
+    const int live = p.M - row0;
+    const u32x4 w = request_window(reinterpret_cast<uint64_t>(p.partial + static_cast<int64_t>(col0 / kGroup) * p.M + row0),
+                                   live > 0 && cols > 0 ? static_cast<uint32_t>(min(live, 16 * I)) * 8u : 0u);
+    const buffer_rsrc window = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(w[0] | static_cast<uint64_t>(w[1]) << 32), 0, static_cast<int>(w[2]), static_cast<int>(w[3]));
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      f32x4 (&v)[J] = acc[i];
+      // (a target's column passes here in one of N / 64 groups: nearly always none of the 16 rows has one)
+      const int2 t = *reinterpret_cast<const int2*>(rows + (16 * i + n) * 8);
+      const int at = t.y == 0 && t.x >= 0 && t.x < p.N ? t.x - col0 : -1, place = at - 4 * h;
+      if (__any(at >= 0 && at < kGroup)) {
+        float z = 0.f;
+        bool here = false;
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (place == 16 * j + e) { z = v[j][e]; here = true; }
+          }
+        if (here && 16 * i + n < live) p.target_logit[row0 + 16 * i + n] = z;
+      }
+      if (cols < kGroup) {   // columns past the vocabulary
+        const int left = hidden(cols - 4 * h);
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[j][e] = 16 * j + e < left ? v[j][e] : -INFINITY;
+      }
+      float m = v[0][0];
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m = fmaxf(m, v[j][e]);
+      m = group_max(m);
+      const float base = m == -INFINITY ? 0.f : m;
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s += fast_exp2((v[j][e] - base) * k);
+      s = group_sum(s);
+      if (h == i % 4) { top = m; sum = s; }
+      if (i % 4 == 3 || i == I - 1) {
+        const int r = i / 4 * 64 + lane;
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, f32x2{top, sum}), window, r < 16 * I ? r * 8 : static_cast<int>(0xfffffff0u), 0, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  // over the four lanes that have a row's columns
+  static __device__ __forceinline__ float group_max(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return half_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+  }
+};
+
+// The partial results of kJoinRows rows of one workgroup: a row's groups are dealt to kSlices threads.
+constexpr int kJoinRows = 16, kSlices = 32;
+__global__ __launch_bounds__(kJoinRows * kSlices) void join_kernel(const f32x2* __restrict__ partial, const float* __restrict__ target_logit,
+                                                                   const int64_t* __restrict__ targets, float* __restrict__ log_probs,
+                                                                   f32x2* __restrict__ max_sum, int M, int groups, int vocab, float k, float inv_t,
+                                                                   int64_t ignore_index) {
+  __shared__ f32x2 share[kSlices][kJoinRows];
+  const int r = threadIdx.x % kJoinRows, slice = threadIdx.x / kJoinRows, row = blockIdx.x * kJoinRows + r;
+  Gather<false> g;
+  if (row < M) {
+    constexpr int U = 4;   // partial results requested together
+    for (int first = slice; first < groups; first += U * kSlices) {
+      f32x2 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int at = first + u * kSlices;
+        v[u] = at < groups ? partial[static_cast<int64_t>(at) * M + row] : f32x2{-INFINITY, 0.f};
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) g.meet(v[u][0], v[u][1], k);
+    }
+  }
+  share[slice][r] = f32x2{g.zmax, g.s};
+  __syncthreads();
+  if (slice == 0 && row < M) {
+    for (int i = 1; i < kSlices; ++i) g.meet(share[i][r][0], share[i][r][1], k);
+    const int64_t t = targets[row];
+    const bool counts = t != ignore_index && t >= 0 && t < vocab;
+    log_probs[row] = counts ? (target_logit[row] - g.zmax) * inv_t - logf(g.s) : 0.f;
+    if (max_sum != nullptr) max_sum[row] = f32x2{g.m, g.s};
+  }
+}
+
+// ---- backward
+// a row as the epilogue needs it: p_j = 2^((z_j - lse) k), lse = max + T ln S in units of z; g = the gradient of its log-probability over T
+// (0 where the row does not count, whatever its logits hold); the target's column
+struct GradRow {
+  float lse, g;
+  int target, counts;
+};
+__global__ void grad_rows_kernel(const f32x2* __restrict__ max_sum, const float* __restrict__ dlog_probs, const int64_t* __restrict__ targets,
+                                 GradRow* __restrict__ out, int M, int vocab, float temperature, float inv_t, int64_t ignore_index) {
+  const int row = blockIdx.x * blockDim.x + threadIdx.x;
+  if (row >= M) return;
+  const int64_t t = targets[row];
+  const bool counts = t != ignore_index && t >= 0 && t < vocab && dlog_probs[row] != 0.f;
+  const f32x2 ms = max_sum[row];
+  out[row] = {ms[0] + temperature * logf(ms[1]), counts ? dlog_probs[row] * inv_t : 0.f, counts ? static_cast<int>(t) : -1, counts};
+}
+
+struct GradParams : LargeParams {
+  const GradRow* grad_rows;   // [M]
+  int ldc;
+  float k;
+};
+struct GradTile {
+  using Params = GradParams;
+  template <int I, int J> static constexpr int kStores = I * ((J + 3) / 4) * 2;
+  template <int I> static constexpr int kBegun = (I + 3) / 4;   // 1 KiB each: 64 rows
+  template <int I>
+  static __device__ __forceinline__ void begin(const Params& p, const Unit& u, int wm, int lane, int wave, uint32_t lds_rows) {
+    lane = hidden(lane);
+    const int left = min(16 * I, p.M - u.m0 - wm);
+    const u32x4 window = request_window(reinterpret_cast<uint64_t>(p.grad_rows + u.m0 + wm), left > 0 ? left * 16u : 0u);
+    wait_lds();
+    request16_to<0>(lds_rows, window, lane * 16);
+    if constexpr (kBegun<I> > 1) request16_to<1024>(lds_rows, window, 1024 + lane * 16);
+    static_assert(kBegun<I> <= 2);
+  }
+  template <int I, int J>
+  static __device__ __forceinline__ void tile(const Params& p, const Unit& u, int wm, int wn, int lane, unsigned char* rows, f32x4 (&acc)[I][J]) {
+    lane = hidden(lane);
+    const int col0 = u.n0 + wn, n = lane % 16, h = lane / 16, cols = p.N - col0;
+    const float k = p.k;
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      const GradRow r = *reinterpret_cast<const GradRow*>(rows + (16 * i + n) * 16);
+      const int at = r.target - col0 - 4 * h;
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float p = fast_exp2((acc[i][j][e] - r.lse) * k), d = r.g * ((at == 16 * j + e ? 1.f : 0.f) - p);
+          acc[i][j][e] = r.counts ? d : 0.f;
+        }
+      if (cols < kGroup) {   // zeros in the columns that pad a row
+        const int left = hidden(cols - 4 * h);
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = 16 * j + e < left ? acc[i][j][e] : 0.f;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    store_tile<__bf16, I, J>(static_cast<__bf16*>(p.c), 0, p.M, p.ldc, p.ldc, p.streaming, u, wm, wn, lane, rows, acc);
+  }
+};
+
+template <int I, typename Epilogue>
+int launch(typename Epilogue::Params p, const char* fn, hipStream_t s) {
+  using S = Shape<false, false, I, kJ>;
+  static LdsOnce reserved;
+  if (!reserve_lds_once(reserved, reinterpret_cast<const void*>(&product_large_kernel<false, false, I, kJ, Epilogue>), S::kLds))
+    return fail(PICO_ERR_LAUNCH, "%s: cannot reserve %d bytes of LDS", fn, S::kLds);
+  p.tiles_m = (p.M + S::TM - 1) / S::TM;
+  p.tiles_n = (p.N + S::TN - 1) / S::TN;
+  p.parts = 1;
+  const int64_t units = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
+  p.streaming = units > 256;   // (as pico_product_large)
+  hipLaunchKernelGGL((product_large_kernel<false, false, I, kJ, Epilogue>), dim3(static_cast<unsigned>(std::min<int64_t>(units, 256))), dim3(S::kThreads), S::kLds, s, p);
+  return check_launch(fn);
+}
+// The tile's rows: what costs least in rounds of 256 workgroups.
+template <typename Epilogue>
+int launch_best(const typename Epilogue::Params& p, const char* fn, hipStream_t s) {
+  const int64_t tiles_n = (p.N + 255) / 256;
+  auto cost = [&](int64_t tm) { return ((p.M + tm - 1) / tm * tiles_n + 255) / 256 * (tm + 32); };
+  int best = 256;
+  for (int tm : {192, 128})
+    if (cost(tm) < cost(best)) best = tm;
+  if (best == 256) return launch<8, Epilogue>(p, fn, s);
+  if (best == 192) return launch<6, Epilogue>(p, fn, s);
+  return launch<4, Epilogue>(p, fn, s);
+}
+
+int check_linear(const char* fn, const void* x, const void* w, const int64_t* targets, int64_t M, int64_t K, int64_t N, int64_t ldx, int64_t ldw, float temperature) {
+  if (M < 0 || N <= 0 || K % 8 != 0 || (M > 0 && !pico_product_large_takes(M, (N + 7) / 8 * 8, K, ldx, ldw, 0, 0, 1)))
+    return fail(PICO_ERR_SHAPE, "%s: rows=%lld hidden=%lld vocab=%lld row pitches %lld, %lld (hidden a multiple of 8 over 64, pitches multiples of 8, a tile's rows span less than 2 GiB)",
+                fn, static_cast<long long>(M), static_cast<long long>(K), static_cast<long long>(N), static_cast<long long>(ldx), static_cast<long long>(ldw));
+  if (!(temperature > 0.f) || !(temperature <= 1e30f) || !(1.f / temperature <= 1e30f)) return fail(PICO_ERR_SHAPE, "%s: temperature %g must be positive and finite", fn, temperature);
+  if (M == 0) return PICO_OK;
+  if (!x || !w || !targets) return fail(PICO_ERR_NULL, "%s: x, w and targets are required", fn);
+  if (!aligned16(x) || !aligned16(w) || reinterpret_cast<uintptr_t>(targets) % 8) return fail(PICO_ERR_ALIGN, "%s: x and w must be aligned to 16 bytes, targets to 8", fn);
+  return PICO_OK;
+}
+int64_t groups_of(int64_t N) { return (N + kGroup - 1) / kGroup; }
+void fill(LargeParams& p, const void* x, const void* w, int64_t M, int64_t K, int64_t N, int64_t ldx, int64_t ldw) {
+  p.a = static_cast<const __bf16*>(x);
+  p.b = static_cast<const __bf16*>(w);
+  p.M = static_cast<int>(M);
+  p.N = static_cast<int>(N);
+  p.K = static_cast<int>(K);
+  p.lda = ldx;
+  p.ldb = ldw;
+}
+
+}  // namespace
+}  // namespace pico
+
+using namespace pico;
+
+extern "C" int64_t pico_linear_log_probs_workspace_bytes(int64_t rows, int64_t vocab) {
+  if (rows < 0 || vocab < 0 || rows > 0x7fffffff || vocab > 0x7fffffff) return -1;
+  return rows * (groups_of(vocab) * 8 + 4);
+}
+
+extern "C" int pico_linear_log_probs_fwd(const void* x, const void* w, const int64_t* targets, float* log_probs, float* max_sum, int64_t rows, int64_t hidden,
+                                         int64_t vocab, int64_t ldx, int64_t ldw, float temperature, int64_t ignore_index, void* workspace,
+                                         int64_t workspace_bytes, void* stream) {
+  const char* fn = "pico_linear_log_probs_fwd";
+  if (int rc = check_linear(fn, x, w, targets, rows, hidden, vocab, ldx, ldw, temperature)) return rc;
+  if (rows == 0) return PICO_OK;
+  if (!log_probs || !workspace) return fail(PICO_ERR_NULL, "%s: log_probs and workspace are required", fn);
+  if (reinterpret_cast<uintptr_t>(workspace) % 8 || reinterpret_cast<uintptr_t>(max_sum) % 8) return fail(PICO_ERR_ALIGN, "%s: workspace and max_sum must be aligned to 8 bytes", fn);
+  if (workspace_bytes < pico_linear_log_probs_workspace_bytes(rows, vocab))
+    return fail(PICO_ERR_WORKSPACE, "%s: workspace of %lld bytes, needs %lld", fn, static_cast<long long>(workspace_bytes),
+                static_cast<long long>(pico_linear_log_probs_workspace_bytes(rows, vocab)));
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  ScoreParams p = {};
+  fill(p, x, w, rows, hidden, vocab, ldx, ldw);
+  p.targets = targets;
+  p.partial = static_cast<f32x2*>(workspace);
+  p.target_logit = reinterpret_cast<float*>(p.partial + rows * groups_of(vocab));
+  p.k = static_cast<float>(1.4426950408889634 / temperature);
+  if (int rc = launch_best<ScoreTile>(p, fn, s)) return rc;
+  hipLaunchKernelGGL(join_kernel, dim3(static_cast<unsigned>((rows + kJoinRows - 1) / kJoinRows)), dim3(kJoinRows * kSlices), 0, s, p.partial, p.target_logit, targets,
+                     log_probs, reinterpret_cast<f32x2*>(max_sum), p.M, static_cast<int>(groups_of(vocab)), p.N, p.k, 1.f / temperature, ignore_index);
+  return check_launch(fn);
+}
+
+extern "C" int pico_linear_log_probs_dlogits(const void* x, const void* w, const int64_t* targets, const float* max_sum, const float* dlog_probs, void* dlogits,
+                                             int64_t rows, int64_t hidden, int64_t vocab, int64_t ldx, int64_t ldw, int64_t ldd, float temperature,
+                                             int64_t ignore_index, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* fn = "pico_linear_log_probs_dlogits";
+  if (int rc = check_linear(fn, x, w, targets, rows, hidden, vocab, ldx, ldw, temperature)) return rc;
+  if (ldd < vocab || ldd % 8 != 0 || ldd >= vocab + 8) return fail(PICO_ERR_STRIDE, "%s: row pitch %lld of dlogits must be vocab, rounded up to a multiple of 8", fn, static_cast<long long>(ldd));
+  if (rows == 0) return PICO_OK;
+  if (!max_sum || !dlog_probs || !dlogits || !workspace) return fail(PICO_ERR_NULL, "%s: max_sum, dlog_probs, dlogits and workspace are required", fn);
+  if (!aligned16(dlogits) || !aligned16(workspace) || reinterpret_cast<uintptr_t>(max_sum) % 8)
+    return fail(PICO_ERR_ALIGN, "%s: dlogits and workspace must be aligned to 16 bytes, max_sum to 8", fn);
+  if (workspace_bytes < rows * 16) return fail(PICO_ERR_WORKSPACE, "%s: workspace of %lld bytes, needs 16 per row", fn, static_cast<long long>(workspace_bytes));
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  GradParams p = {};
+  fill(p, x, w, rows, hidden, vocab, ldx, ldw);
+  GradRow* of = static_cast<GradRow*>(workspace);
+  hipLaunchKernelGGL(grad_rows_kernel, dim3(static_cast<unsigned>((rows + 255) / 256)), dim3(256), 0, s, reinterpret_cast<const f32x2*>(max_sum), dlog_probs, targets, of,
+                     p.M, p.N, temperature, 1.f / temperature, ignore_index);
+  p.c = dlogits;
+  p.ldc = static_cast<int>(ldd);
+  p.grad_rows = of;
+  p.k = static_cast<float>(1.4426950408889634 / temperature);
+  return launch_best<GradTile>(p, fn, s);
+}

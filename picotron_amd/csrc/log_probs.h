@@ -57,6 +57,11 @@ struct Gather {
     zmax = to;
     m = to == -INFINITY ? 0.f : to;
   }
+  __device__ __forceinline__ void meet(float other_max, float other_s, float k) {   // what was gathered elsewhere (no entropy)
+    const float top = fmaxf(zmax, other_max), shift = other_max == -INFINITY ? 0.f : fmaxf((other_max - top) * k, kFloor);
+    rise(top, k);
+    s += other_s * fast_exp2(shift);
+  }
   template <int N>
   __device__ __forceinline__ void add(const float (&e)[N], float k) {
     float top = e[0];

@@ -104,6 +104,15 @@ def log_probs(logits, targets, ignore_index: int = -100, temperature: float = 1.
     return tuple(out) if entropy else out[0]
 
 
+def linear_log_probs(x, weight, targets, ignore_index: int = -100, temperature: float = 1.0):
+    """``log_probs(F.linear(x, weight), targets)`` for bf16 hidden states x [..., hidden] and vocabulary projection weight [vocab, hidden]
+    without the logits in memory: what a frozen reference or the sampling policy answers with.  Differentiable in x and weight; the
+    backward computes the logits again, so where memory does not matter ``log_probs`` on kept logits trains faster.  The logits are
+    fp32 sums that are not rounded to bf16 on the way."""
+    _check_targets("linear_log_probs", targets, weight.size(0), ignore_index)
+    return _lib.host().linear_log_probs(x, weight, targets, ignore_index, temperature)
+
+
 def policy_loss(logits, targets, advantages, old_log_probs=None, ref_log_probs=None, weights=None, clip=(0.2, 0.2), kl_coef: float = 0.0,
                 entropy_coef: float = 0.0, ignore_index: int = -100, temperature: float = 1.0, scale: float = 1.0):
     """The clipped policy loss over sampled tokens, from their logits: returns (loss, log_probs), the second without a gradient.

@@ -35,7 +35,7 @@ import torch.nn.functional as F
 import picotron_amd.process_group_manager as pgm
 from picotron_amd import _lib
 from picotron_amd.context_parallel import context_parallel
-from picotron_amd.functional import (FusedLinearFunc, QKVAttentionFunc, RMSNormFunc, RMSNormHeadFunc, RMSNormResidualFunc,
+from picotron_amd.functional import (linear_log_probs, log_probs, FusedLinearFunc, QKVAttentionFunc, RMSNormFunc, RMSNormHeadFunc, RMSNormResidualFunc,
                                      RotaryFunc, SwiGLUFunc, SwiGLUFusedFunc, _fused_rope)
 
 
@@ -292,6 +292,13 @@ class FinalProjection(nn.Module):
             return F.linear(x, self.weight, self.bias)
         return _lib.host().linear(x, self.weight)
 
+    def log_probs(self, x, targets, ignore_index=-100, temperature=1.0):
+        """Log-probabilities of the tokens `targets` under softmax(self(x) / temperature), fp32; for a bf16 projection without a
+        bias the logits stay out of memory."""
+        if self.bias is not None or self.weight.dtype != torch.bfloat16 or x.dtype != torch.bfloat16:
+            return log_probs(self(x), targets, ignore_index, temperature)
+        return linear_log_probs(x, self.weight, targets, ignore_index, temperature)
+
 
 class DecoderLayer(nn.Module):
     """RMSNorm -> Attention -> residual -> RMSNorm -> MLP -> residual."""
@@ -390,16 +397,23 @@ class Llama(nn.Module):
                                                  base=self.model_config.rope_theta)
             layer.cos, layer.sin = context_parallel.update_rope_for_context_parallel(*layer._full_tables)
 
-    def forward(self, input_ids, attention_mask=None, position_ids: torch.Tensor = None):
+    def hidden_states(self, input_ids):
+        """What the vocabulary projection reads: the residual stream behind the last layer, normalised."""
         x = self.embedding(input_ids)
         if _fused_residual() and isinstance(self.final_norm, TritonRMSNorm) and all(
                 isinstance(l.input_layernorm, TritonRMSNorm) for l in self.decoder_layers):
             residual = None
             for layer in self.decoder_layers:
                 x, residual = layer.forward_chained(x, residual)
-            x = self.final_norm(x, residual=residual)
-        else:
-            for layer in self.decoder_layers:
-                x = layer(x)
-            x = self.final_norm(x)
-        return self.final_proj(x)
+            return self.final_norm(x, residual=residual)
+        for layer in self.decoder_layers:
+            x = layer(x)
+        return self.final_norm(x)
+
+    def forward(self, input_ids, attention_mask=None, position_ids: torch.Tensor = None):
+        return self.final_proj(self.hidden_states(input_ids))
+
+    def log_probs(self, input_ids, targets, ignore_index=-100, temperature=1.0):
+        """Log-probabilities of `targets` [batch, seq] after `input_ids` [batch, seq], fp32, 0 where the target is `ignore_index`: what
+        a reference or a sampling policy answers with, without the logits in memory."""
+        return self.final_proj.log_probs(self.hidden_states(input_ids), targets, ignore_index, temperature)

@@ -96,11 +96,37 @@ def test_gradients_that_overlap_or_lie_otherwise(lib, dtype, size):
     assert bwd(d=4096 + size) == -4 and bwd(row=1001, batch=4008) == -4 and bwd(batch=4001) == -4
 
 
+def test_linear_log_probs(lib):
+    """Sizes, pitches, alignments, pointers and workspaces."""
+    assert lib.pico_linear_log_probs_workspace_bytes(100, 129) == 100 * (3 * 8 + 4)
+    assert lib.pico_linear_log_probs_workspace_bytes(-1, 8) == -1 and lib.pico_linear_log_probs_workspace_bytes(1, 1 << 40) == -1
+
+    def fwd(x=4096, w=4096, t=4096, lp=4096, ms=4096, M=10, K=128, N=1000, ldx=128, ldw=128, T=1.0, ws=4096, bytes=1 << 20):
+        P = ctypes.c_void_p
+        return lib.pico_linear_log_probs_fwd(P(x), P(w), P(t), P(lp), P(ms), M, K, N, ldx, ldw, T, -100, P(ws), bytes, None)
+
+    def bwd(x=4096, w=4096, t=4096, ms=4096, g=4096, d=4096, M=10, K=128, N=1000, ldx=128, ldw=128, ldd=1000, T=1.0, ws=4096, bytes=1 << 20):
+        P = ctypes.c_void_p
+        return lib.pico_linear_log_probs_dlogits(P(x), P(w), P(t), P(ms), P(g), P(d), M, K, N, ldx, ldw, ldd, T, -100, P(ws), bytes, None)
+    for call in (fwd, bwd):
+        for over in (dict(M=-1), dict(K=64), dict(K=100), dict(N=0), dict(ldx=120), dict(ldw=132), dict(ldx=1 << 31), dict(K=0), dict(M=1 << 31), dict(T=0.0), dict(T=float("nan"))):
+            assert call(**over) == -3, over
+        for over in (dict(x=4104), dict(w=4098), dict(t=4100), dict(ms=4100), dict(ws=4100)):
+            assert call(**over) == -4, over
+        for over in (dict(x=None), dict(w=None), dict(t=None), dict(ws=None)):
+            assert call(**over) == -1, over
+        assert call(bytes=100) == -6 and "workspace" in message(lib)
+    assert fwd(lp=None) == -1 and bwd(ms=None) == -1 and bwd(g=None) == -1 and bwd(d=None) == -1 and bwd(d=4104) == -4
+    for ldd in (992, 1004, 1008):
+        assert bwd(ldd=ldd) == -5 and "row pitch" in message(lib)
+    assert bwd(N=1001, ldd=1001) == -5
+
+
 def test_host_path_refusals():
     """Tensors on the CPU are refused, not computed, and shapes are looked at first."""
-    from picotron_amd.functional import log_probs, policy_loss, preference_loss
+    from picotron_amd.functional import linear_log_probs, log_probs, policy_loss, preference_loss
     x, t = torch.zeros(2, 3, 8), torch.zeros(2, 3, dtype=torch.long)
-    for call in (lambda: log_probs(x, t), lambda: policy_loss(x, t, torch.zeros(2, 1)), lambda: preference_loss(x, t)):
+    for call in (lambda: linear_log_probs(x, torch.zeros(4, 8), t), lambda: log_probs(x, t), lambda: policy_loss(x, t, torch.zeros(2, 1)), lambda: preference_loss(x, t)):
         with pytest.raises(RuntimeError, match="GPU only"):
             call()
 
