@@ -1373,7 +1373,13 @@ RowValues row_values(const char* fn, const char* what, const Tensor& v, const Te
   TORCH_CHECK(v.is_floating_point(), fn, ": ", what, " must be a floating-point tensor");
   TORCH_CHECK(at::is_expandable_to(v.sizes(), targets.sizes()), fn, ": ", what, " must have a value per target or broadcast to ", targets.sizes(), " (got ", v.sizes(), ")");
   RowValues r;
-  r.t = per_row(v.detach().to(at::kFloat).expand(targets.sizes()));
+  r.t = v.scalar_type() == at::kFloat ? v : v.detach().to(at::kFloat);
+  if (targets.dim() == 2 && r.t.dim() <= 2) {   // (the usual case, without a view on the way)
+    auto stride = [&](int64_t from_last) { return r.t.dim() >= from_last && r.t.size(-from_last) != 1 ? r.t.stride(-from_last) : 0; };
+    r.v = {static_cast<const float*>(r.t.data_ptr()), stride(2), stride(1)};
+    return r;
+  }
+  r.t = per_row(r.t.detach().expand(targets.sizes()));
   r.v = {static_cast<const float*>(r.t.data_ptr()), r.t.stride(0), r.t.stride(1)};
   return r;
 }
@@ -1400,11 +1406,11 @@ void refuse_second_order(const char* fn) {
   TORCH_CHECK(!at::GradMode::is_enabled(), fn, ": its gradient cannot be differentiated again (create_graph)");
 }
 // d(logits) of `up` times (dlp q + dh H) per row, in `d` where that holds the gradient for a factor of 1 already
-Tensor log_probs_gradient(const TokenRows& r, const Tensor& max_sum, const Tensor& entropy, const RowValues& dlp, const RowValues& dh, const Tensor& up, Tensor d,
+Tensor log_probs_gradient(const TokenRows& r, const float* max_sum, const float* entropy, const pico_values& dlp, const pico_values& dh, const Tensor& up, Tensor d,
                           double temperature, int64_t ignore_index) {
   const bool have_unit = d.defined();
   if (!have_unit) d = gradient_rows(r.logits);
-  check(pico_log_probs_bwd(&r.z, &r.t, fptr(max_sum), fptr(entropy), &dlp.v, &dh.v, fptr(up), have_unit, ptr(d), d.stride(0), d.stride(1),
+  check(pico_log_probs_bwd(&r.z, &r.t, max_sum, entropy, &dlp, &dh, fptr(up), have_unit, ptr(d), d.stride(0), d.stride(1),
                            static_cast<float>(temperature), ignore_index, stream_now()));
   return d;
 }
@@ -1439,7 +1445,8 @@ struct LogProbs : torch::autograd::Function<LogProbs> {
     const TokenRows r = token_rows("log_probs", s[0], s[1]);
     const RowValues dlp = row_values("log_probs", "the gradient", OptTensor(g[0]), s[1]);
     const RowValues dh = row_values("log_probs", "the gradient", g.size() > 1 ? OptTensor(g[1]) : std::nullopt, s[1]);
-    d[0] = log_probs_gradient(r, s[2], s[3], dlp, dh, Tensor(), Tensor(), ctx->saved_data["temperature"].toDouble(), ctx->saved_data["ignore"].toInt()).view(s[0].sizes());
+    d[0] = log_probs_gradient(r, fptr(s[2]), fptr(s[3]), dlp.v, dh.v, Tensor(), Tensor(), ctx->saved_data["temperature"].toDouble(), ctx->saved_data["ignore"].toInt());
+    if (s[0].dim() != 3) d[0] = d[0].view(s[0].sizes());
     return d;
   }
 };
@@ -1455,8 +1462,15 @@ struct PolicyOptions {
   int64_t ignore_index;
 };
 struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
+  // what the backward needs of the forward: the gradient for a unit upstream gradient, and per row in one buffer the maximum and sum, d loss / d log p
+  // and, with an entropy term, the entropy and d loss / d entropy
   struct Saved {
-    Tensor unit, max_sum, dlp, entropy, dentropy;
+    Tensor unit, rows;
+    static int64_t per_row(bool with_entropy) { return with_entropy ? 5 : 3; }
+    static pico_policy_saved parts(const Tensor& rows, int64_t n, bool with_entropy) {
+      float* p = fptr(rows);
+      return {p, p + 2 * n, with_entropy ? p + 3 * n : nullptr, with_entropy ? p + 4 * n : nullptr};
+    }
   };
   static variable_list run(const Tensor& logits, const Tensor& targets, const Tensor& advantages, const OptTensor& old_lp, const OptTensor& ref_lp,
                            const OptTensor& weights, const PolicyOptions& o, Saved* saved) {
@@ -1465,22 +1479,18 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     const TokenRows r = token_rows(fn, logits, targets);
     const RowValues A = row_values(fn, "advantages", advantages, targets), old = row_values(fn, "old_log_probs", old_lp, targets),
                     ref = row_values(fn, "ref_log_probs", ref_lp, targets), w = row_values(fn, "weights", weights, targets);
+    const int64_t n = targets.numel();
     const auto f32 = logits.options().dtype(at::kFloat);
-    const Tensor loss = at::empty({}, f32), inv_count = at::empty({}, f32), lp = per_token(targets, logits), losses = per_token(targets, logits);
+    const Tensor loss = at::empty({}, f32), lp = per_token(targets, logits), scratch = at::empty({n + 1}, f32);   // losses, 1 / count
     const pico_policy p = {A.v, old.v, ref.v, w.v, static_cast<float>(o.clip_low), static_cast<float>(o.clip_high), static_cast<float>(o.kl_coef),
                            static_cast<float>(o.entropy_coef), static_cast<float>(o.scale)};
     pico_policy_saved kept = {};
     if (saved) {
       saved->unit = gradient_rows(r.logits);
-      saved->max_sum = per_token(targets, logits, 2);
-      saved->dlp = per_token(targets, logits);
-      if (p.entropy_coef != 0) {
-        saved->entropy = per_token(targets, logits);
-        saved->dentropy = per_token(targets, logits);
-      }
-      kept = {fptr(saved->max_sum), fptr(saved->dlp), fptr(saved->entropy), fptr(saved->dentropy)};
+      saved->rows = at::empty({n * Saved::per_row(p.entropy_coef != 0)}, f32);
+      kept = Saved::parts(saved->rows, n, p.entropy_coef != 0);
     }
-    check(pico_policy_loss_fwd(&r.z, &r.t, &p, fptr(loss), fptr(lp), fptr(losses), fptr(inv_count), &kept, saved ? ptr(saved->unit) : nullptr,
+    check(pico_policy_loss_fwd(&r.z, &r.t, &p, fptr(loss), fptr(lp), fptr(scratch), fptr(scratch) + n, &kept, saved ? ptr(saved->unit) : nullptr,
                                saved ? saved->unit.stride(0) : 0, saved ? saved->unit.stride(1) : 0, static_cast<float>(o.temperature), o.ignore_index, stream_now()));
     return {loss, lp};
   }
@@ -1489,9 +1499,10 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
                                int64_t ignore_index, double temperature, double scale) {
     Saved k;
     variable_list out = run(logits, targets, advantages, old_lp, ref_lp, weights, {clip_low, clip_high, kl_coef, entropy_coef, temperature, scale, ignore_index}, &k);
-    ctx->save_for_backward({logits, targets, k.unit, k.max_sum, k.dlp, k.entropy, k.dentropy});
+    ctx->save_for_backward({logits, targets, k.unit, k.rows});
     ctx->saved_data["ignore"] = ignore_index;
     ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["entropy"] = static_cast<float>(entropy_coef) != 0;
     ctx->saved_data["spent"] = false;
     ctx->mark_non_differentiable({out[1]});
     ctx->set_materialize_grads(false);
@@ -1506,12 +1517,14 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     const TokenRows r = token_rows("policy_loss", s[0], s[1]);
     const Tensor up = g[0].to(at::kFloat).contiguous();
     // a second backward through this node (retain_graph) gets a buffer of its own
-    const bool spent = ctx->saved_data["spent"].toBool();
+    const bool spent = ctx->saved_data["spent"].toBool(), with_entropy = ctx->saved_data["entropy"].toBool();
     ctx->saved_data["spent"] = true;
-    const RowValues dlp = row_values("policy_loss", "the gradient", s[4], s[1]);
-    const RowValues dh = row_values("policy_loss", "the gradient", s[6].defined() ? OptTensor(s[6]) : std::nullopt, s[1]);
-    d[0] = log_probs_gradient(r, s[3], s[5], dlp, dh, up, spent ? Tensor() : s[2], ctx->saved_data["temperature"].toDouble(),
-                              ctx->saved_data["ignore"].toInt()).view(s[0].sizes());
+    const int64_t seq = r.z.seq;
+    const pico_policy_saved kept = Saved::parts(s[3], s[1].numel(), with_entropy);
+    const pico_values dlp = {kept.dlog_probs, seq, 1}, dh = {kept.dentropy, seq, 1};
+    d[0] = log_probs_gradient(r, kept.max_sum, kept.entropy, dlp, dh, up, spent ? Tensor() : s[2], ctx->saved_data["temperature"].toDouble(),
+                              ctx->saved_data["ignore"].toInt());
+    if (s[0].dim() != 3) d[0] = d[0].view(s[0].sizes());
     return d;
   }
 };
@@ -1527,7 +1540,7 @@ std::pair<Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& target
 // logits [2 pairs, seq, V]: the chosen sequences, then the rejected ones
 struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
   static variable_list run(const Tensor& logits, const Tensor& targets, const OptTensor& ref_lp, double beta, double smoothing, bool average, int64_t ignore_index,
-                           double scale, Tensor* max_sum, Tensor* slope_out) {
+                           double scale, Tensor* saved) {
     const char* fn = "preference_loss";
     const c10::OptionalDeviceGuard device(logits.device());
     TORCH_CHECK(logits.dim() == 3, fn, ": logits must be [2 pairs, seq, vocab], the chosen sequences before the rejected ones (got ", logits.sizes(), ")");
@@ -1541,21 +1554,22 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
       ref = ref_lp->detach().to(at::kFloat).contiguous();
     }
     const auto f32 = logits.options().dtype(at::kFloat);
-    const Tensor loss = at::empty({}, f32), sequence = at::empty({B}, f32), slope = at::empty({B}, f32), lp = per_token(targets, logits),
-                 ws = at::empty({B}, logits.options().dtype(at::kDouble));
-    if (max_sum) {
-      *max_sum = per_token(targets, logits, 2);
-      *slope_out = slope;
+    const int64_t n = targets.numel();
+    const Tensor loss = at::empty({}, f32), sequence = at::empty({B}, f32), scratch = at::empty({3 * B + n}, f32);   // doubles first: sums, slopes, log-probabilities
+    float* slope = fptr(scratch) + 2 * B;
+    if (saved) {   // maxima and sums, slopes
+      *saved = at::empty({2 * n + B}, f32);
+      slope = fptr(*saved) + 2 * n;
     }
     check(pico_preference_loss_fwd(&r.z, &r.t, fptr(ref), static_cast<float>(beta), static_cast<float>(smoothing), average, static_cast<float>(scale), fptr(loss),
-                                   fptr(sequence), fptr(slope), fptr(lp), max_sum ? fptr(*max_sum) : nullptr, ptr(ws), ignore_index, stream_now()));
+                                   fptr(sequence), slope, fptr(scratch) + 3 * B, saved ? fptr(*saved) : nullptr, ptr(scratch), ignore_index, stream_now()));
     return {loss, sequence};
   }
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& targets, const OptTensor& ref_lp, double beta, double smoothing,
                                bool average, int64_t ignore_index, double scale) {
-    Tensor max_sum, slope;
-    variable_list out = run(logits, targets, ref_lp, beta, smoothing, average, ignore_index, scale, &max_sum, &slope);
-    ctx->save_for_backward({logits, targets, max_sum, slope});
+    Tensor saved;
+    variable_list out = run(logits, targets, ref_lp, beta, smoothing, average, ignore_index, scale, &saved);
+    ctx->save_for_backward({logits, targets, saved});
     ctx->saved_data["ignore"] = ignore_index;
     ctx->mark_non_differentiable({out[1]});
     ctx->set_materialize_grads(false);
@@ -1568,15 +1582,15 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
     const auto s = ctx->get_saved_variables();
     const c10::OptionalDeviceGuard device(s[0].device());
     const TokenRows r = token_rows("preference_loss", s[0], s[1]);
-    const RowValues dlp = row_values("preference_loss", "the gradient", s[3].unsqueeze(1), s[1]);
-    d[0] = log_probs_gradient(r, s[2], Tensor(), dlp, RowValues(), g[0].to(at::kFloat).contiguous(), Tensor(), 1.0, ctx->saved_data["ignore"].toInt());
+    const pico_values dlp = {fptr(s[2]) + 2 * s[1].numel(), 1, 0};   // (one for all of a sequence)
+    d[0] = log_probs_gradient(r, fptr(s[2]), nullptr, dlp, {nullptr, 0, 0}, g[0].to(at::kFloat).contiguous(), Tensor(), 1.0, ctx->saved_data["ignore"].toInt());
     return d;
   }
 };
 std::pair<Tensor, Tensor> preference_loss(const Tensor& logits, const Tensor& targets, const OptTensor& ref_lp, double beta, double smoothing, bool average,
                                           int64_t ignore_index, double scale) {
   const variable_list out = records({&logits}) ? PreferenceLoss::apply(logits, targets, ref_lp, beta, smoothing, average, ignore_index, scale)
-                                               : PreferenceLoss::run(logits, targets, ref_lp, beta, smoothing, average, ignore_index, scale, nullptr, nullptr);
+                                               : PreferenceLoss::run(logits, targets, ref_lp, beta, smoothing, average, ignore_index, scale, nullptr);
   return {out[0], out[1]};
 }
 

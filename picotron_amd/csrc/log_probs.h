@@ -35,14 +35,23 @@ struct Row {
   const T* x;      // the row
   const T* body;   // its first whole piece
   int head, nvec, edge;   // edge: this thread's element of head or tail, -1: none
+  int inside;             // pieces between the line of 128 bytes that `body` lies in and body
   __device__ __forceinline__ Row(const void* data, int64_t offset, int vocab) {
     x = static_cast<const T*>(data) + offset;
     const int past = static_cast<int>(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));
     head = min(past ? V - past : 0, vocab);
     nvec = (vocab - head) / V;
     body = x + head;
+    inside = static_cast<int>(reinterpret_cast<uintptr_t>(body) % 128 / 16);
     const int tail = vocab - head - nvec * V, i = threadIdx.x;
     edge = i < head ? i : i >= 8 && i - 8 < tail ? vocab - tail + i - 8 : -1;
+  }
+  // The thread's first piece; the others follow NT apart.  A wave's accesses are whole lines: stores of parts of lines past the caches are slow ([3, 777,
+  // 32001] fp32 backward 119 -> 107 us).  (The first lanes of a row that starts inside a line come a round later.)
+  template <int NT>
+  __device__ __forceinline__ int first() const {
+    const int v = static_cast<int>(threadIdx.x) - inside;
+    return v < 0 ? v + NT : v;
   }
 };
 
@@ -50,7 +59,9 @@ struct Row {
 template <bool kEntropy>
 struct Gather {
   float zmax = -INFINITY, m = 0.f, s = 0.f, w = 0.f;   // m: zmax, or 0 where nothing but -inf was there
-  __device__ __forceinline__ void rise(float to, float k) {   // to another maximum, no smaller than this one
+  // to another maximum, no smaller than this one (no product here is taken into a sum unrounded: where lanes exchange sums, each would have another)
+  __device__ __forceinline__ void rise(float to, float k) {
+#pragma clang fp contract(off)
     const float shift = zmax == -INFINITY ? 0.f : fmaxf((zmax - to) * k, kFloor), c = fast_exp2(shift);
     if constexpr (kEntropy) w = c * (w + shift * s);
     s *= c;
@@ -68,6 +79,10 @@ struct Gather {
 #pragma unroll
     for (int i = 1; i < N; ++i) top = fmaxf(top, e[i]);
     if (top > zmax) rise(top, k);
+    take(e, k);
+  }
+  template <int N>
+  __device__ __forceinline__ void take(const float (&e)[N], float k) {   // none over the maximum
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const float d = (e[i] - m) * k, p = fast_exp2(d);
@@ -83,7 +98,8 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
-// A workgroup's gathered shares as one, for every thread.  `share`: 3 floats a wave of LDS.
+// A workgroup's gathered shares as one, for every thread.  `share`: 3 floats a wave of LDS.  A lane reads one wave's share and the lanes exchange them: read
+// whole by every lane they would take three registers a wave, beside a row that is held in registers too many.
 template <int NT, bool kEntropy>
 __device__ __forceinline__ void join(Gather<kEntropy>& g, float k, float (*share)[3]) {
   constexpr int W = NT / kWave;
@@ -91,26 +107,21 @@ __device__ __forceinline__ void join(Gather<kEntropy>& g, float k, float (*share
   g.s = wave_sum(g.s);
   if constexpr (kEntropy) g.w = wave_sum(g.w);
   if constexpr (W > 1) {
-    const int wave = threadIdx.x / kWave;
+    const int wave = threadIdx.x / kWave, of = threadIdx.x % W;
     if (threadIdx.x % kWave == 0) { share[wave][0] = g.zmax; share[wave][1] = g.s; share[wave][2] = g.w; }
     __syncthreads();
-    float top = share[0][0];
+    g.zmax = share[of][0];
+    g.s = share[of][1];
+    if constexpr (kEntropy) g.w = share[of][2];
+    float top = g.zmax;
 #pragma unroll
-    for (int i = 1; i < W; ++i) top = fmaxf(top, share[i][0]);
-    float s = 0.f, w = 0.f;
-    Gather<kEntropy> one;
+    for (int off = W / 2; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
+    g.rise(top, k);
 #pragma unroll
-    for (int i = 0; i < W; ++i) {
-      one.zmax = share[i][0];
-      one.s = share[i][1];
-      one.w = share[i][2];
-      one.rise(top, k);
-      s += one.s;
-      w += one.w;
+    for (int off = W / 2; off > 0; off >>= 1) {
+      g.s += __shfl_xor(g.s, off, kWave);
+      if constexpr (kEntropy) g.w += __shfl_xor(g.w, off, kWave);
     }
-    g = one;
-    g.s = s;
-    g.w = w;
   }
 }
 

@@ -12,29 +12,61 @@ constexpr int kUnroll = 4;   // pieces of a row that a thread requests before it
 
 __device__ __forceinline__ bool is_token(int64_t t, int64_t ignore_index, int vocab) { return t != ignore_index && t >= 0 && t < vocab; }
 
+// (32-bit offsets from the row's address, which is the same for all lanes: a register per access instead of two)
+// kKeep: what is loaded is to stay in the caches, to be read again; otherwise it passes them.
+template <bool kKeep = false, typename T>
+__device__ __forceinline__ u32x4 load_piece(const T* body, uint32_t v) {
+  const u32x4* at = reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(body) + v * 16u);
+  if constexpr (kKeep) return *at;
+  else return __builtin_nontemporal_load(at);
+}
+template <typename T>
+__device__ __forceinline__ void store_piece(T* body, uint32_t v, const float (&e)[io<T>::kVec]) {
+  io<T>::store_stream(reinterpret_cast<char*>(body) + v * 16u, e);
+}
+template <typename T>
+__device__ __forceinline__ void unpack(const u32x4& raw, float (&out)[io<T>::kVec]) {
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      out[2 * i] = __uint_as_float(raw[i] << 16);
+      out[2 * i + 1] = __uint_as_float(raw[i] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = __uint_as_float(raw[i]);
+  }
+}
+
 // fn(piece's elements, its first index) for every piece of a row that this thread has
-template <typename T, int NT, typename Fn>
+template <typename T, int NT, bool kKeep, typename Fn>
 __device__ __forceinline__ void each_piece(const Row<T>& r, const Fn& fn) {
   constexpr int V = Row<T>::V, U = kUnroll;
-  int v = threadIdx.x;
+  int v = r.template first<NT>();
   for (; v + (U - 1) * NT < r.nvec; v += U * NT) {
-    float e[U][V];
+    u32x4 raw[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) io<T>::load_stream(r.body + static_cast<int64_t>(v + u * NT) * V, e[u]);
+    for (int u = 0; u < U; ++u) raw[u] = load_piece<kKeep>(r.body, v + u * NT);
 #pragma unroll
-    for (int u = 0; u < U; ++u) fn(e[u], v + u * NT);
+    for (int u = 0; u < U; ++u) {
+      float e[V];
+      unpack<T>(raw[u], e);
+      fn(e, v + u * NT);
+    }
   }
   for (; v < r.nvec; v += NT) {
     float e[V];
-    io<T>::load_stream(r.body + static_cast<int64_t>(v) * V, e);
+    unpack<T>(load_piece<kKeep>(r.body, v), e);
     fn(e, v);
   }
 }
 
 template <typename T, int NT, bool kEntropy>
-__device__ __forceinline__ Gather<kEntropy> gather_row(const Row<T>& r, float k, float (*share)[3]) {
+__device__ __forceinline__ Gather<kEntropy> gather_row(const Row<T>& r, float k, bool keep, float (*share)[3]) {
   Gather<kEntropy> g;
-  each_piece<T, NT>(r, [&](const float (&e)[Row<T>::V], int) { g.add(e, k); });
+  auto add = [&](const float (&e)[Row<T>::V], int) { g.add(e, k); };
+  if (keep) each_piece<T, NT, true>(r, add);
+  else each_piece<T, NT, false>(r, add);
   if (r.edge >= 0) {
     const float e[1] = {static_cast<float>(r.x[r.edge])};
     g.add(e, k);
@@ -45,11 +77,11 @@ __device__ __forceinline__ Gather<kEntropy> gather_row(const Row<T>& r, float k,
 
 // the gradient of a row at d; d and r.x lie alike modulo 16 bytes
 template <typename T, int NT, bool kEntropy>
-__device__ __forceinline__ void write_gradient(const Row<T>& r, T* d, const Slope& slope, float k, float m, int t) {
+__device__ __forceinline__ void write_gradient(const Row<T>& r, T* d, const Slope& slope, float k, float m, int t, bool kept) {
   constexpr int V = Row<T>::V;
   T* body = d + r.head;
   const int t_piece = t >= r.head ? (t - r.head) / V : -1, t_elem = t >= r.head ? (t - r.head) % V : 0;
-  each_piece<T, NT>(r, [&](const float (&e)[V], int v) {
+  auto write = [&](const float (&e)[V], int v) {
     float o[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) o[i] = along<kEntropy>(slope, e[i], k, m);
@@ -57,15 +89,17 @@ __device__ __forceinline__ void write_gradient(const Row<T>& r, T* d, const Slop
 #pragma unroll
       for (int i = 0; i < V; ++i) o[i] += i == t_elem ? slope.hot : 0.f;
     }
-    io<T>::store_stream(body + static_cast<int64_t>(v) * V, o);
-  });
+    store_piece(body, v, o);
+  };
+  if (kept) each_piece<T, NT, true>(r, write);
+  else each_piece<T, NT, false>(r, write);
   if (r.edge >= 0)
     d[r.edge] = static_cast<T>(along<kEntropy>(slope, static_cast<float>(r.x[r.edge]), k, m) + (r.edge == t ? slope.hot : 0.f));
 }
 template <typename T, int NT>
 __device__ __forceinline__ void write_zeros(const Row<T>& r, T* d) {
   const u32x4 zero = {0u, 0u, 0u, 0u};
-  for (int v = threadIdx.x; v < r.nvec; v += NT) __builtin_nontemporal_store(zero, reinterpret_cast<u32x4*>(d + r.head + static_cast<int64_t>(v) * Row<T>::V));
+  for (int v = r.template first<NT>(); v < r.nvec; v += NT) __builtin_nontemporal_store(zero, reinterpret_cast<u32x4*>(reinterpret_cast<char*>(d + r.head) + static_cast<uint32_t>(v) * 16u));
   if (r.edge >= 0) d[r.edge] = static_cast<T>(0.f);
 }
 
@@ -73,7 +107,7 @@ __device__ __forceinline__ void write_zeros(const Row<T>& r, T* d) {
 // log_probs, entropy [rows]; max_sum [rows, 2]: what the gradient needs of a row (the maximum and the sum)
 template <typename T, int NT, bool kEntropy>
 __global__ __launch_bounds__(NT) void log_probs_kernel(const LogitsArgs z, const TokenArgs targets, float* __restrict__ log_probs,
-                                                       float* __restrict__ entropy, f32x2* __restrict__ max_sum, int64_t ignore_index) {
+                                                       float* __restrict__ entropy, f32x2* __restrict__ max_sum, int64_t kept_from, int64_t ignore_index) {
   __shared__ float share[NT / kWave][3];
   const int64_t row = blockIdx.x, b = row / z.seq, s = row - b * z.seq;
   const int64_t t = targets.at(b, s);
@@ -87,7 +121,7 @@ __global__ __launch_bounds__(NT) void log_probs_kernel(const LogitsArgs z, const
   }
   const Row<T> r(z.data, b * z.batch_stride + s * z.row_stride, z.vocab);
   const float xt = static_cast<float>(r.x[t]);
-  const Gather<kEntropy> g = gather_row<T, NT, kEntropy>(r, z.k, share);
+  const Gather<kEntropy> g = gather_row<T, NT, kEntropy>(r, z.k, row >= kept_from, share);
   if (threadIdx.x == 0) {
     log_probs[row] = (xt - g.zmax) * z.inv_t - logf(g.s);
     if constexpr (kEntropy) entropy[row] = logf(g.s) - kLn2 * g.w / g.s;
@@ -96,14 +130,20 @@ __global__ __launch_bounds__(NT) void log_probs_kernel(const LogitsArgs z, const
 }
 
 // ---- their gradient: one read, one write.  d = up (dlp d log p_t + dh dH); up: a device scalar or NULL (1).
+// The rows are walked from the last to the first: a loss is usually differentiated as soon as it is there, and what the forward read last lies
+// in the 256 MB behind the L2s.  The forward reads the rows from kept_from on such that they stay there, the others past the caches; dlogits leaves
+// past them too, or it would push the rows out.  Forward and backward, us: [4, 1024, 49152] bf16 187 -> 173, [3, 777, 32001] fp32 146 -> 132 (128 MB
+// kept 178 and 137, 256 MB 174 and 130, but the forward alone 58 instead of 52), [14, 333, 32001] bf16 142 -> 131; everything kept and stores that stay 205,
+// 158 and 154.
 template <typename T, int NT, bool kEntropy>
 __global__ __launch_bounds__(NT) void log_probs_grad_kernel(const LogitsArgs z, const TokenArgs targets, const f32x2* __restrict__ max_sum,
                                                             const float* __restrict__ entropy, const ValueArgs dlp, const ValueArgs dh,
                                                             const float* __restrict__ upstream, int skip_unit, T* __restrict__ dlogits,
-                                                            int64_t dbatch_stride, int64_t drow_stride, int64_t rows, int64_t ignore_index) {
+                                                            int64_t dbatch_stride, int64_t drow_stride, int64_t rows, int64_t kept_from,
+                                                            int64_t ignore_index) {
   const float up = upstream != nullptr ? *upstream : 1.f;
   if (skip_unit && up == 1.f) return;   // dlogits holds the gradient for a unit upstream gradient already
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+  for (int64_t row = rows - 1 - blockIdx.x; row >= 0; row -= gridDim.x) {
     const int64_t b = row / z.seq, s = row - b * z.seq;
     const int64_t t = targets.at(b, s);
     const Row<T> r(z.data, b * z.batch_stride + s * z.row_stride, z.vocab);
@@ -118,7 +158,7 @@ __global__ __launch_bounds__(NT) void log_probs_grad_kernel(const LogitsArgs z, 
       continue;
     }
     const f32x2 ms = max_sum[row];
-    write_gradient<T, NT, kEntropy>(r, d, slope<kEntropy>(a, h, ms[1], kEntropy ? entropy[row] : 0.f, z.inv_t), z.k, ms[0], static_cast<int>(t));
+    write_gradient<T, NT, kEntropy>(r, d, slope<kEntropy>(a, h, ms[1], kEntropy ? entropy[row] : 0.f, z.inv_t), z.k, ms[0], static_cast<int>(t), row >= kept_from);
   }
 }
 
@@ -136,16 +176,25 @@ struct PolicyArgs {
 struct PolicyRow {
   float loss, a, b;   // weighted
 };
-__device__ __forceinline__ PolicyRow policy_row(const PolicyArgs& p, int64_t b, int64_t s, float q, float H, float w) {
-  const float A = p.advantages.at(b, s);
-  const float ratio = p.old_lp.data != nullptr ? expf(q - p.old_lp.at(b, s)) : 1.f;
+struct PolicyInputs {   // of a row, requested with its logits
+  float A, old, ref, w;
+  __device__ __forceinline__ PolicyInputs(const PolicyArgs& p, int64_t b, int64_t s, bool counted) {
+    A = p.advantages.at(b, s);
+    old = p.old_lp.data != nullptr ? p.old_lp.at(b, s) : 0.f;
+    ref = p.ref_lp.data != nullptr ? p.ref_lp.at(b, s) : 0.f;
+    w = p.weights.data != nullptr ? p.weights.at(b, s) * p.scale : counted ? *p.inv_count : 1.f;
+  }
+};
+__device__ __forceinline__ PolicyRow policy_row(const PolicyArgs& p, const PolicyInputs& in, float q, float H) {
+  const float A = in.A, w = in.w;
+  const float ratio = p.old_lp.data != nullptr ? fast_exp2((q - in.old) * kLog2e) : 1.f;
   const float held = fminf(fmaxf(ratio, p.low), p.high), free = ratio * A, bound = held * A;
   PolicyRow r;
   // (written such that a NaN anywhere comes out)
   r.loss = bound < free ? -bound : -free;
   r.a = bound < free ? 0.f : -free;
   if (p.ref_lp.data != nullptr && p.kl_coef != 0.f) {
-    const float diff = p.ref_lp.at(b, s) - q, grow = expm1f(diff);
+    const float diff = in.ref - q, grow = fast_exp2(diff * kLog2e) - 1.f;
     r.loss += p.kl_coef * (grow - diff);
     r.a -= p.kl_coef * grow;
   }
@@ -180,10 +229,12 @@ __global__ __launch_bounds__(NT) void policy_kernel(const LogitsArgs z, const To
     return;
   }
   const float xt = static_cast<float>(r.x[t]);
-  const float w = p.weights.data != nullptr ? p.weights.at(b, s) * p.scale : kGrad ? *p.inv_count : 1.f;
-  const Gather<kEntropy> g = gather_row<T, NT, kEntropy>(r, z.k, share);
-  const float q = (xt - g.zmax) * z.inv_t - logf(g.s), H = kEntropy ? logf(g.s) - kLn2 * g.w / g.s : 0.f;
-  const PolicyRow l = policy_row(p, b, s, q, H, w);
+  const PolicyInputs in(p, b, s, kGrad);
+  const Gather<kEntropy> g = gather_row<T, NT, kEntropy>(r, z.k, kGrad, share);   // (with a gradient the row is read again below)
+  float q = (xt - g.zmax) * z.inv_t - logf(g.s);
+  asm volatile("" : "+v"(q));   // (rounded as it is stored, or its difference from `old` is taken before the rounding: where they are equal the ratio is 1)
+  const float H = kEntropy ? logf(g.s) - kLn2 * g.w / g.s : 0.f;
+  const PolicyRow l = policy_row(p, in, q, H);
   if (threadIdx.x == 0) {
     p.log_probs[row] = q;
     p.losses[row] = l.loss;
@@ -193,7 +244,114 @@ __global__ __launch_bounds__(NT) void policy_kernel(const LogitsArgs z, const To
       p.max_sum[row] = f32x2{g.m, g.s};
     }
   }
-  if constexpr (kGrad) write_gradient<T, NT, kEntropy>(r, d, slope<kEntropy>(l.a, l.b, g.s, H, z.inv_t), z.k, g.m, static_cast<int>(t));
+  if constexpr (kGrad) write_gradient<T, NT, kEntropy>(r, d, slope<kEntropy>(l.a, l.b, g.s, H, z.inv_t), z.k, g.m, static_cast<int>(t), true);
+}
+
+// The same with the row in registers between its statistics and its gradient: the logits are read once.  NT threads hold NV pieces of 16 bytes each, packed as
+// they came; each phase unpacks them again (the empty asm hides that it is the same value, or the compiler would keep the unpacked row).
+// count_rows > 0 (at most NT; targets without gaps): every workgroup counts the rows that count for itself, behind the requests for its row, instead of a
+// launch in front.
+template <typename T, int NT, int NV, bool kEntropy>
+__global__ __launch_bounds__(NT, NV <= 6 ? 8 : NV <= 8 ? 6 : NV <= 12 ? 5 : 4) void policy_held_kernel(const LogitsArgs z, const TokenArgs targets, const PolicyArgs p, T* __restrict__ dlogits,
+                                                                         int64_t dbatch_stride, int64_t drow_stride, int64_t ignore_index, int count_rows) {
+  constexpr int V = Row<T>::V, W = NT / kWave;
+  __shared__ float share[W][3];
+  __shared__ int counted[W];
+  const int64_t row = blockIdx.x, b = row / z.seq, s = row - b * z.seq;
+  const int64_t t = targets.at(b, s);
+  const Row<T> r(z.data, b * z.batch_stride + s * z.row_stride, z.vocab);
+  T* d = dlogits + b * dbatch_stride + s * drow_stride;
+  if (!is_token(t, ignore_index, z.vocab)) {
+    write_zeros<T, NT>(r, d);
+    if (threadIdx.x == 0) {
+      p.log_probs[row] = p.losses[row] = p.dlp[row] = 0.f;
+      if constexpr (kEntropy) p.dentropy[row] = p.entropy[row] = 0.f;
+      p.max_sum[row] = f32x2{0.f, 1.f};
+    }
+    return;
+  }
+  constexpr uint32_t kNegInf = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;   // past the end of the row: its exponential is 0
+  const int first = r.template first<NT>();
+  u32x4 raw[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int v = first + j * NT;
+    raw[j] = u32x4{kNegInf, kNegInf, kNegInf, kNegInf};
+    if (v < r.nvec) raw[j] = load_piece(r.body, v);
+  }
+  auto hide = [&]() {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) asm volatile("" : "+v"(raw[j]));
+  };
+  const float xt = static_cast<float>(r.x[t]), xe = r.edge >= 0 ? static_cast<float>(r.x[r.edge]) : -INFINITY;
+  PolicyInputs in(p, b, s, count_rows == 0);
+  if (count_rows > 0) {
+    const int64_t other = static_cast<int>(threadIdx.x) < count_rows ? targets.data[threadIdx.x] : ignore_index;
+    const int n = __popcll(__ballot(is_token(other, ignore_index, z.vocab)));
+    if (threadIdx.x % kWave == 0) counted[threadIdx.x / kWave] = n;
+    if constexpr (W == 1) __syncthreads();   // (otherwise the one in join)
+  }
+  Gather<kEntropy> g;
+  float top = xe;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    float e[V];
+    unpack<T>(raw[j], e);
+#pragma unroll
+    for (int i = 0; i < V; ++i) top = fmaxf(top, e[i]);
+  }
+  hide();
+  g.rise(top, z.k);
+  {
+    const float e[1] = {xe};
+    g.take(e, z.k);
+  }
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    float e[V];
+    unpack<T>(raw[j], e);
+    g.take(e, z.k);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  hide();
+  join<NT>(g, z.k, share);
+  if (count_rows > 0) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) n += counted[i];
+    in.w = p.scale / static_cast<float>(n);   // (this row is one of them)
+  }
+  float q = (xt - g.zmax) * z.inv_t - logf(g.s);
+  asm volatile("" : "+v"(q));   // (rounded as it is stored, or its difference from `old` is taken before the rounding: where they are equal the ratio is 1)
+  const float H = kEntropy ? logf(g.s) - kLn2 * g.w / g.s : 0.f;
+  const PolicyRow l = policy_row(p, in, q, H);
+  if (threadIdx.x == 0) {
+    p.log_probs[row] = q;
+    p.losses[row] = l.loss;
+    p.dlp[row] = l.a;
+    if constexpr (kEntropy) { p.dentropy[row] = l.b; p.entropy[row] = H; }
+    p.max_sum[row] = f32x2{g.m, g.s};
+  }
+  const Slope along_row = slope<kEntropy>(l.a, l.b, g.s, H, z.inv_t);
+  T* body = d + r.head;
+  const int ti = static_cast<int>(t), t_piece = ti >= r.head ? (ti - r.head) / V : -1, t_elem = ti >= r.head ? (ti - r.head) % V : 0;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int v = first + j * NT;
+    if (v < r.nvec) {
+      float e[V];
+      unpack<T>(raw[j], e);
+#pragma unroll
+      for (int i = 0; i < V; ++i) e[i] = along<kEntropy>(along_row, e[i], z.k, g.m);
+      if (v == t_piece) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) e[i] += i == t_elem ? along_row.hot : 0.f;
+      }
+      store_piece(body, v, e);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  if (r.edge >= 0) d[r.edge] = static_cast<T>(along<kEntropy>(along_row, xe, z.k, g.m) + (r.edge == ti ? along_row.hot : 0.f));
 }
 
 // ---- sums over rows: one workgroup, in double and in a fixed order
@@ -302,14 +460,33 @@ __global__ __launch_bounds__(kSumThreads) void preference_kernel(const TokenArgs
 }
 
 // ---- launches
-// the narrowest workgroup that has a row in eight pieces a thread: in a wider one most lanes of a short row would idle
+template <int n> using Int = std::integral_constant<int, n>;
+// the narrowest workgroup that has a row in four pieces a thread, eight from 256 threads on: in a wider one most lanes of a short row would idle
 template <typename Fn>
 void with_threads(int64_t vocab, int vec, const Fn& fn) {
   const int64_t pieces = (vocab + vec - 1) / vec;
-  if (pieces <= 64 * 4) fn(std::integral_constant<int, 64>());
-  else if (pieces <= 128 * 4) fn(std::integral_constant<int, 128>());
-  else if (pieces <= 256 * 8) fn(std::integral_constant<int, 256>());
-  else fn(std::integral_constant<int, 512>());
+  if (pieces <= 64 * 4) fn(Int<64>());
+  else if (pieces <= 128 * 4) fn(Int<128>());
+  else if (pieces <= 256 * 8) fn(Int<256>());
+  else fn(Int<512>());
+}
+// Threads and pieces per thread of the kernel that holds a row of so many pieces; (0, 0): none does.  As few threads as can hold the row in four or eight pieces: a
+// barrier over fewer waves, and more rows on a CU.  6144 pieces in 1024 x 6, where two rows share a CU, [8, 1024, 49152] bf16 256 us, in 512 x 12 262; with an entropy
+// term the former has no registers left (12 bytes of scratch).
+template <bool kEntropy, typename Fn>
+void with_pieces(int64_t vocab, int vec, const Fn& fn) {
+  const int64_t pieces = vocab / vec;
+  if (pieces <= 64 * 4) fn(Int<64>(), Int<4>());
+  else if (pieces <= 128 * 4) fn(Int<128>(), Int<4>());
+  else if (pieces <= 256 * 4) fn(Int<256>(), Int<4>());
+  else if (pieces <= 256 * 8) fn(Int<256>(), Int<8>());
+  else if (pieces <= 512 * 8) fn(Int<512>(), Int<8>());
+  else if (pieces <= 1024 * 6) {
+    if constexpr (kEntropy) fn(Int<512>(), Int<12>());
+    else fn(Int<1024>(), Int<6>());
+  } else if (pieces <= 512 * 16) fn(Int<512>(), Int<16>());
+  else if (pieces <= 1024 * 16) fn(Int<1024>(), Int<16>());
+  else fn(Int<0>(), Int<0>());
 }
 template <typename Fn>
 void with_type(const pico_logits& z, const Fn& fn) {
@@ -353,6 +530,12 @@ LogitsArgs args(const pico_logits& z, float temperature) {
   const float inv_t = 1.f / temperature;
   return {z.data, z.batch_stride, z.row_stride, static_cast<int>(z.seq), static_cast<int>(z.vocab), static_cast<float>(1.4426950408889634 / temperature), inv_t};
 }
+// the first row that the forward keeps in the caches for the backward
+constexpr int64_t kKeptBytes = int64_t{160} << 20;
+int64_t kept_from(const pico_logits& z) {
+  const int64_t rows = z.batch * z.seq, most = kKeptBytes / (z.vocab * (z.dtype == PICO_BF16 ? 2 : 4));
+  return std::max<int64_t>(rows - most, 0);
+}
 TokenArgs args(const pico_tokens& t) { return {t.data, t.batch_stride, t.row_stride}; }
 ValueArgs args(const pico_values* v) { return v ? ValueArgs{v->data, v->batch_stride, v->row_stride} : ValueArgs{nullptr, 0, 0}; }
 
@@ -362,7 +545,7 @@ int run_log_probs(const char* fn, const pico_logits& z, const pico_tokens& targe
   with_type(z, [&](auto type, auto nt) {
     with_flag(entropy != nullptr, [&](auto with) {
       hipLaunchKernelGGL((log_probs_kernel<decltype(type), decltype(nt)::value, decltype(with)::value>), grid, dim3(decltype(nt)::value), 0, s, args(z, temperature),
-                         args(targets), log_probs, entropy, reinterpret_cast<f32x2*>(max_sum), ignore_index);
+                         args(targets), log_probs, entropy, reinterpret_cast<f32x2*>(max_sum), max_sum ? kept_from(z) : z.batch * z.seq, ignore_index);
     });
   });
   return check_launch(fn);
@@ -401,7 +584,7 @@ extern "C" int pico_log_probs_bwd(const pico_logits* logits, const pico_tokens* 
     with_flag(with_entropy, [&](auto with) {
       hipLaunchKernelGGL((log_probs_grad_kernel<decltype(type), decltype(nt)::value, decltype(with)::value>), grid, dim3(decltype(nt)::value), 0, static_cast<hipStream_t>(stream),
                          args(*logits, temperature), args(*targets), reinterpret_cast<const f32x2*>(max_sum), entropy, args(dlog_probs), args(dentropy),
-                         grad_out, have_unit, static_cast<decltype(type)*>(dlogits), dbatch_stride, drow_stride, rows, ignore_index);
+                         grad_out, have_unit, static_cast<decltype(type)*>(dlogits), dbatch_stride, drow_stride, rows, kept_from(*logits), ignore_index);
     });
   });
   return check_launch(fn);
@@ -428,11 +611,10 @@ extern "C" int pico_policy_loss_fwd(const pico_logits* logits, const pico_tokens
     }
   }
   auto sum = [&](float* to) {
-    hipLaunchKernelGGL(policy_sum_kernel, dim3(1), dim3(kSumThreads), 0, s, args(*targets), losses, to, inv_count, policy->scale, !weighted,
+    hipLaunchKernelGGL(policy_sum_kernel, dim3(1), dim3(kSumThreads), 0, s, args(*targets), losses, to, inv_count, policy->scale, !weighted && (!to || !dlogits),
                        !weighted && !dlogits, rows, static_cast<int>(std::max<int64_t>(logits->seq, 1)), static_cast<int>(logits->vocab), ignore_index);
   };
   if (rows > 0) {
-    if (dlogits && !weighted) sum(nullptr);   // the gradient needs scale / count
     PolicyArgs p = {args(&policy->advantages), args(&policy->old_log_probs), args(&policy->ref_log_probs), args(&policy->weights),
                     1.f - policy->clip_low, 1.f + policy->clip_high, policy->kl_coef, policy->entropy_coef, policy->scale, inv_count, log_probs, losses,
                     nullptr, nullptr, nullptr, nullptr};
@@ -443,13 +625,28 @@ extern "C" int pico_policy_loss_fwd(const pico_logits* logits, const pico_tokens
       p.max_sum = reinterpret_cast<f32x2*>(saved->max_sum);
     }
     const dim3 grid(static_cast<unsigned>(rows));
-    with_type(*logits, [&](auto type, auto nt) {
-      with_flag(with_entropy, [&](auto with) {
-        with_flag(dlogits != nullptr, [&](auto grad) {
-          hipLaunchKernelGGL((policy_kernel<decltype(type), decltype(nt)::value, decltype(with)::value, decltype(grad)::value>), grid, dim3(decltype(nt)::value), 0, s,
-                             args(*logits, temperature), args(*targets), p, static_cast<decltype(type)*>(dlogits), dbatch_stride, drow_stride, ignore_index);
-        });
+    auto stream_row = [&](auto type, auto nt, auto with, auto grad) {
+      using T = decltype(type);
+      constexpr int NT = decltype(nt)::value;
+      hipLaunchKernelGGL((policy_kernel<T, NT, decltype(with)::value, decltype(grad)::value>), grid, dim3(NT), 0, s, args(*logits, temperature), args(*targets), p,
+                         static_cast<T*>(dlogits), dbatch_stride, drow_stride, ignore_index);
+    };
+    auto with_gradient = [&](auto type, auto with) {
+      using T = decltype(type);
+      with_pieces<decltype(with)::value>(logits->vocab, io<T>::kVec, [&](auto nt, auto nv) {
+        constexpr int NT = decltype(nt)::value, NV = decltype(nv)::value;
+        const bool itself = rows <= NT && targets->row_stride == 1 && (logits->batch == 1 || targets->batch_stride == logits->seq);
+        if (!weighted && !itself) sum(nullptr);   // the gradient needs scale / count
+        if constexpr (NT == 0) stream_row(type, Int<512>(), with, std::true_type());
+        else
+          hipLaunchKernelGGL((policy_held_kernel<T, NT, NV, decltype(with)::value>), grid, dim3(NT), 0, s, args(*logits, temperature), args(*targets), p,
+                             static_cast<T*>(dlogits), dbatch_stride, drow_stride, ignore_index, !weighted && itself ? static_cast<int>(rows) : 0);
       });
+    };
+    with_flag(with_entropy, [&](auto with) {
+      if (!dlogits) with_type(*logits, [&](auto type, auto nt) { stream_row(type, nt, with, std::false_type()); });
+      else if (logits->dtype == PICO_BF16) with_gradient(__bf16(), with);
+      else with_gradient(float(), with);
     });
   }
   sum(loss);
