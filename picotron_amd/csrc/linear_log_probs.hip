@@ -15,12 +15,66 @@ namespace {
 // of 16 columns each: a wave's share of a tile, and the width of a partial result
 constexpr int kJ = 4, kGroup = 16 * kJ;
 
+// Partial results: (max, sum) of row r and group g at [r / 64][g][r % 64], so that a wave writes whole lines and a workgroup that joins reads neighbouring ones.
 struct ScoreParams : LargeParams {
   const int64_t* targets;   // [M]
-  f32x2* partial;           // [groups, M]
+  f32x2* partial;
   float* target_logit;      // [M]
+  int groups;
   float k;
 };
+// the same value, of which the compiler does not know that it is (or it would keep what follows from it for all rows in registers)
+__device__ __forceinline__ int hidden(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+__device__ __forceinline__ float group_max(float v) {   // over the four lanes that have a row's columns
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return half_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+// (max, sum of 2^D) of 64 columns of a row, 16 of them in this lane: columns 16 j + 4 h + e, of which the first `cols` are there
+template <int J>
+__device__ __forceinline__ f32x2 score(f32x4 (&v)[J], int h, int cols, float k) {
+  if (cols < kGroup) {   // columns past the vocabulary
+    const int left = hidden(cols - 4 * h);
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[j][e] = 16 * j + e < left ? v[j][e] : -INFINITY;
+  }
+  float m = v[0][0];
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m = fmaxf(m, v[j][e]);
+  m = group_max(m);
+  // D as logits k - max k, an instruction less than the difference first (exponentials and what leads to them are the tile's end): all D are off by the rounding of
+  // max k, which the sum is multiplied free of (2^-r = 1 - r ln2, r under 2^-16)
+  const float mk = m == -INFINITY ? 0.f : m * k, r = m == -INFINITY ? 0.f : fmaf(m, k, -mk);
+  float s = 0.f;
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s += fast_exp2(fmaf(v[j][e], k, -mk));
+  s = group_sum(s);
+  return {m, fmaf(-r * kLn2, s, s)};
+}
+// the target's logit to `to`, where its column is one of these 64 (nearly always none of 16 rows' is); t: the target, two words
+template <int J>
+__device__ __forceinline__ void pick(const f32x4 (&v)[J], int2 t, int h, int col0, int vocab, bool live, float* to) {
+  const int at = t.y == 0 && t.x >= 0 && t.x < vocab ? t.x - col0 : -1, place = at - 4 * h;
+  if (__any(at >= 0 && at < kGroup)) {
+    float z = 0.f;
+    bool here = false;
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (place == 16 * j + e) { z = v[j][e]; here = true; }
+      }
+    if (here && live) *to = z;
+  }
+}
 
 // 4 bytes per lane to LDS, as request16_to
 template <int kPlus>
@@ -28,12 +82,6 @@ __device__ __forceinline__ void request4_to(uint32_t lds_off, u32x4 window, uint
   uint32_t aim;
   asm volatile("s_add_u32 %0, %1, %2\n\ts_nop 0\n\tbuffer_load_dword %3, %4, 0 offen lds"
                : "=&{m0}"(aim) : "s"(lds_off), "n"(kPlus), "v"(off), "s"(window) : "scc", "memory");
-}
-
-// the same value, of which the compiler does not know that it is (or it would keep what follows from it for all rows in registers)
-__device__ __forceinline__ int hidden(int v) {
-  asm volatile("" : "+v"(v));
-  return v;
 }
 
 // Epilogue of the forward.  A lane holds columns 4 h ..+3 (h = lane / 16) of 16 consecutive ones, of row lane % 16 of 16: a row's 64
@@ -58,89 +106,151 @@ struct ScoreTile {
     lane = hidden(lane);
     const int row0 = u.m0 + wm, col0 = u.n0 + wn, n = lane % 16, h = lane / 16, cols = p.N - col0;
     const float k = p.k;
-    float top = 0.f, sum = 0.f;   // of row 64 q + lane
+    f32x2 mine = {0.f, 0.f};   // of row 64 q + lane
     const int live = p.M - row0;
-    const u32x4 w = request_window(reinterpret_cast<uint64_t>(p.partial + static_cast<int64_t>(col0 / kGroup) * p.M + row0),
-                                   live > 0 && cols > 0 ? static_cast<uint32_t>(min(live, 16 * I)) * 8u : 0u);
+    const u32x4 w = request_window(reinterpret_cast<uint64_t>(p.partial + (static_cast<int64_t>(row0 / 64) * p.groups + col0 / kGroup) * 64), 0x7ffffff0u);
     const buffer_rsrc window = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(w[0] | static_cast<uint64_t>(w[1]) << 32), 0, static_cast<int>(w[2]), static_cast<int>(w[3]));
 #pragma unroll
     for (int i = 0; i < I; ++i) {
-      f32x4 (&v)[J] = acc[i];
-      // (a target's column passes here in one of N / 64 groups: nearly always none of the 16 rows has one)
-      const int2 t = *reinterpret_cast<const int2*>(rows + (16 * i + n) * 8);
-      const int at = t.y == 0 && t.x >= 0 && t.x < p.N ? t.x - col0 : -1, place = at - 4 * h;
-      if (__any(at >= 0 && at < kGroup)) {
-        float z = 0.f;
-        bool here = false;
-#pragma unroll
-        for (int j = 0; j < J; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (place == 16 * j + e) { z = v[j][e]; here = true; }
-          }
-        if (here && 16 * i + n < live) p.target_logit[row0 + 16 * i + n] = z;
-      }
-      if (cols < kGroup) {   // columns past the vocabulary
-        const int left = hidden(cols - 4 * h);
-#pragma unroll
-        for (int j = 0; j < J; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[j][e] = 16 * j + e < left ? v[j][e] : -INFINITY;
-      }
-      float m = v[0][0];
-#pragma unroll
-      for (int j = 0; j < J; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) m = fmaxf(m, v[j][e]);
-      m = group_max(m);
-      const float base = m == -INFINITY ? 0.f : m;
-      float s = 0.f;
-#pragma unroll
-      for (int j = 0; j < J; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s += fast_exp2((v[j][e] - base) * k);
-      s = group_sum(s);
-      if (h == i % 4) { top = m; sum = s; }
+      const int row = 16 * i + n;
+      pick(acc[i], *reinterpret_cast<const int2*>(rows + row * 8), h, col0, p.N, row < live, p.target_logit + row0 + row);
+      const f32x2 ms = score(acc[i], h, cols, k);
+      if (h == i % 4) mine = ms;
       if (i % 4 == 3 || i == I - 1) {
-        const int r = i / 4 * 64 + lane;
-        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, f32x2{top, sum}), window, r < 16 * I ? r * 8 : static_cast<int>(0xfffffff0u), 0, 0);
+        const int r = i / 4 * 64 + lane, past = row0 % 64 + r;   // (the first row may lie inside a block of 64)
+        const bool there = r < min(16 * I, live) && cols > 0;
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, mine), window, there ? (past / 64 * p.groups * 64 + past % 64) * 8 : static_cast<int>(0xfffffff0u), 0, 0);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
   }
-  // over the four lanes that have a row's columns
-  static __device__ __forceinline__ float group_max(float v) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return half_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
-  }
 };
 
-// The partial results of kJoinRows rows of one workgroup: a row's groups are dealt to kSlices threads.
-constexpr int kJoinRows = 16, kSlices = 32;
+// Few rows (16 RB at most): what bounds them is reading w once.  A workgroup has 64 entries of the vocabulary, and its four waves a quarter of the contraction
+// each, 128 bytes of a row at a time; operands come straight from memory in the layout of the products (x from the caches), a step's loads ahead of the step
+// before's products, and the waves' sums meet in LDS.  Whole calls, us, in the product's tiles and here: 1 x 2048 against 49152 59.7, 47.0 (4.3 TB/s), 16 rows 56.5,
+// 50.4, 32 rows 59.9, 54.8, 24 x 576 21.6, 17.9.  For 64 rows x is read as often as w: 58.9, 66.3; they stay with the product.
+template <int RB>
+__global__ __launch_bounds__(256, 3) void score_few_kernel(const ScoreParams p) {
+  __shared__ f32x4 sums[4][RB][kJ][kWave];
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), n = lane % 16, h = lane / 16;
+  const int col0 = blockIdx.x * kGroup, cols = p.N - col0;
+  const char* w = reinterpret_cast<const char*>(p.b + static_cast<int64_t>(col0) * p.ldb);
+  const char* x = reinterpret_cast<const char*>(p.a);
+  uint32_t wo[kJ], xo[RB];   // (rows past the end read the last one)
+#pragma unroll
+  for (int j = 0; j < kJ; ++j) wo[j] = static_cast<uint32_t>(min(16 * j + n, cols - 1) * p.ldb * 2 + 16 * h);
+#pragma unroll
+  for (int b = 0; b < RB; ++b) xo[b] = static_cast<uint32_t>(min(16 * b + n, p.M - 1) * p.lda * 2 + 16 * h);
+  struct Step {
+    bf16x8 w[2][kJ], x[2][RB];
+  };
+  auto load = [&](Step& f, int step) __attribute__((always_inline)) {
+    const char *wk = w + step * 128, *xk = x + step * 128;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int j = 0; j < kJ; ++j) f.w[s][j] = *reinterpret_cast<const bf16x8*>(wk + (wo[j] + 64u * s));
+#pragma unroll
+      for (int b = 0; b < RB; ++b) f.x[s][b] = *reinterpret_cast<const bf16x8*>(xk + (xo[b] + 64u * s));
+    }
+  };
+  f32x4 acc[RB][kJ];
+#pragma unroll
+  for (int b = 0; b < RB; ++b)
+#pragma unroll
+    for (int j = 0; j < kJ; ++j) acc[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto multiply = [&](const Step& f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) acc[b][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.w[s][j], f.x[s][b], acc[b][j], 0, 0, 0);
+  };
+  const int whole = p.K / 64;
+  Step one, two;
+  int step = wave;
+  if (step < whole) load(one, step);
+  for (; step + 4 < whole; step += 8) {
+    load(two, step + 4);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(one);
+    if (step + 8 < whole) load(one, step + 8);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(two);
+  }
+  if (step < whole) multiply(one);
+  if (p.K % 64 != 0 && wave == whole % 4) {   // the contraction's last piece, with zeros behind its end
+    const char *wk = w + whole * 128, *xk = x + whole * 128;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const bool in = whole * 64 + 32 * s + 8 * h < p.K;
+#pragma unroll
+      for (int j = 0; j < kJ; ++j) {
+        one.w[s][j] = bf16x8{};
+        if (in) one.w[s][j] = *reinterpret_cast<const bf16x8*>(wk + (wo[j] + 64u * s));
+      }
+#pragma unroll
+      for (int b = 0; b < RB; ++b) {
+        one.x[s][b] = bf16x8{};
+        if (in) one.x[s][b] = *reinterpret_cast<const bf16x8*>(xk + (xo[b] + 64u * s));
+      }
+    }
+    multiply(one);
+  }
+#pragma unroll
+  for (int b = 0; b < RB; ++b)
+#pragma unroll
+    for (int j = 0; j < kJ; ++j) sums[wave][b][j][lane] = acc[b][j];
+  __syncthreads();
+  for (int b = wave; b < RB; b += 4) {
+    f32x4 v[kJ];
+#pragma unroll
+    for (int j = 0; j < kJ; ++j) v[j] = (sums[0][b][j][lane] + sums[1][b][j][lane]) + (sums[2][b][j][lane] + sums[3][b][j][lane]);
+    const int row = 16 * b + n;
+    const bool live = row < p.M;
+    const int2 t = live ? *reinterpret_cast<const int2*>(p.targets + row) : int2{-1, -1};
+    pick(v, t, h, col0, p.N, live, p.target_logit + row);
+    const f32x2 ms = score(v, h, cols, p.k);
+    if (h == 0 && live) p.partial[static_cast<int64_t>(blockIdx.x) * 64 + row] = ms;
+  }
+}
+constexpr int kFewRows = 32;
+
+// A workgroup joins the partial results of kJoinRows rows: a row's groups are dealt to kSlices threads.
+constexpr int kJoinRows = 16, kSlices = 64;
 __global__ __launch_bounds__(kJoinRows * kSlices) void join_kernel(const f32x2* __restrict__ partial, const float* __restrict__ target_logit,
                                                                    const int64_t* __restrict__ targets, float* __restrict__ log_probs,
                                                                    f32x2* __restrict__ max_sum, int M, int groups, int vocab, float k, float inv_t,
                                                                    int64_t ignore_index) {
-  __shared__ f32x2 share[kSlices][kJoinRows];
+  __shared__ f32x2 share[kSlices * kJoinRows / kWave][kJoinRows];
   const int r = threadIdx.x % kJoinRows, slice = threadIdx.x / kJoinRows, row = blockIdx.x * kJoinRows + r;
   Gather<false> g;
   if (row < M) {
-    constexpr int U = 4;   // partial results requested together
+    constexpr int U = 6;   // partial results requested together
+    const f32x2* of = partial + static_cast<int64_t>(row / 64) * groups * 64 + row % 64;
     for (int first = slice; first < groups; first += U * kSlices) {
       f32x2 v[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int at = first + u * kSlices;
-        v[u] = at < groups ? partial[static_cast<int64_t>(at) * M + row] : f32x2{-INFINITY, 0.f};
+        v[u] = at < groups ? of[at * 64] : f32x2{-INFINITY, 0.f};
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) g.meet(v[u][0], v[u][1], k);
     }
   }
-  share[slice][r] = f32x2{g.zmax, g.s};
+  // a wave has four slices of 16 rows, and 16 waves meet in LDS
+#pragma unroll
+  for (int off = 16; off < kWave; off *= 2) {
+    const float other_max = __shfl_xor(g.zmax, off, kWave), other_s = __shfl_xor(g.s, off, kWave);
+    g.meet(other_max, other_s, k);
+  }
+  if (threadIdx.x % kWave < kJoinRows) share[threadIdx.x / kWave][r] = f32x2{g.zmax, g.s};
   __syncthreads();
   if (slice == 0 && row < M) {
-    for (int i = 1; i < kSlices; ++i) g.meet(share[i][r][0], share[i][r][1], k);
+    for (int i = 1; i < kSlices * kJoinRows / kWave; ++i) g.meet(share[i][r][0], share[i][r][1], k);
     const int64_t t = targets[row];
     const bool counts = t != ignore_index && t >= 0 && t < vocab;
     log_probs[row] = counts ? (target_logit[row] - g.zmax) * inv_t - logf(g.s) : 0.f;
@@ -149,20 +259,20 @@ __global__ __launch_bounds__(kJoinRows * kSlices) void join_kernel(const f32x2* 
 }
 
 // ---- backward
-// a row as the epilogue needs it: p_j = 2^((z_j - lse) k), lse = max + T ln S in units of z; g = the gradient of its log-probability over T
+// a row as the epilogue needs it: p_j = 2^(k z_j - lse2), lse2 = k max + log2 S; g = the gradient of its log-probability over T
 // (0 where the row does not count, whatever its logits hold); the target's column
 struct GradRow {
-  float lse, g;
+  float lse2, g;
   int target, counts;
 };
 __global__ void grad_rows_kernel(const f32x2* __restrict__ max_sum, const float* __restrict__ dlog_probs, const int64_t* __restrict__ targets,
-                                 GradRow* __restrict__ out, int M, int vocab, float temperature, float inv_t, int64_t ignore_index) {
+                                 GradRow* __restrict__ out, int M, int vocab, float k, float inv_t, int64_t ignore_index) {
   const int row = blockIdx.x * blockDim.x + threadIdx.x;
   if (row >= M) return;
   const int64_t t = targets[row];
   const bool counts = t != ignore_index && t >= 0 && t < vocab && dlog_probs[row] != 0.f;
   const f32x2 ms = max_sum[row];
-  out[row] = {ms[0] + temperature * logf(ms[1]), counts ? dlog_probs[row] * inv_t : 0.f, counts ? static_cast<int>(t) : -1, counts};
+  out[row] = {fmaf(ms[0], k, log2f(ms[1])), counts ? dlog_probs[row] * inv_t : 0.f, counts ? static_cast<int>(t) : -1, counts};
 }
 
 struct GradParams : LargeParams {
@@ -197,7 +307,7 @@ struct GradTile {
       for (int j = 0; j < J; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float p = fast_exp2((acc[i][j][e] - r.lse) * k), d = r.g * ((at == 16 * j + e ? 1.f : 0.f) - p);
+          const float p = fast_exp2(fmaf(acc[i][j][e], k, -r.lse2)), d = r.g * ((at == 16 * j + e ? 1.f : 0.f) - p);
           acc[i][j][e] = r.counts ? d : 0.f;
         }
       if (cols < kGroup) {   // zeros in the columns that pad a row
@@ -268,7 +378,7 @@ using namespace pico;
 
 extern "C" int64_t pico_linear_log_probs_workspace_bytes(int64_t rows, int64_t vocab) {
   if (rows < 0 || vocab < 0 || rows > 0x7fffffff || vocab > 0x7fffffff) return -1;
-  return rows * (groups_of(vocab) * 8 + 4);
+  return (rows + 63) / 64 * 64 * groups_of(vocab) * 8 + rows * 4;
 }
 
 extern "C" int pico_linear_log_probs_fwd(const void* x, const void* w, const int64_t* targets, float* log_probs, float* max_sum, int64_t rows, int64_t hidden,
@@ -287,11 +397,18 @@ extern "C" int pico_linear_log_probs_fwd(const void* x, const void* w, const int
   fill(p, x, w, rows, hidden, vocab, ldx, ldw);
   p.targets = targets;
   p.partial = static_cast<f32x2*>(workspace);
-  p.target_logit = reinterpret_cast<float*>(p.partial + rows * groups_of(vocab));
+  p.groups = static_cast<int>(groups_of(vocab));
+  p.target_logit = reinterpret_cast<float*>(p.partial + (rows + 63) / 64 * 64 * p.groups);
   p.k = static_cast<float>(1.4426950408889634 / temperature);
-  if (int rc = launch_best<ScoreTile>(p, fn, s)) return rc;
+  if (rows <= kFewRows) {
+    const dim3 grid(static_cast<unsigned>(p.groups)), threads(256);
+    if (rows <= 16) hipLaunchKernelGGL(score_few_kernel<1>, grid, threads, 0, s, p);
+    else hipLaunchKernelGGL(score_few_kernel<2>, grid, threads, 0, s, p);
+  } else if (int rc = launch_best<ScoreTile>(p, fn, s)) {
+    return rc;
+  }
   hipLaunchKernelGGL(join_kernel, dim3(static_cast<unsigned>((rows + kJoinRows - 1) / kJoinRows)), dim3(kJoinRows * kSlices), 0, s, p.partial, p.target_logit, targets,
-                     log_probs, reinterpret_cast<f32x2*>(max_sum), p.M, static_cast<int>(groups_of(vocab)), p.N, p.k, 1.f / temperature, ignore_index);
+                     log_probs, reinterpret_cast<f32x2*>(max_sum), p.M, p.groups, p.N, p.k, 1.f / temperature, ignore_index);
   return check_launch(fn);
 }
 
@@ -309,12 +426,12 @@ extern "C" int pico_linear_log_probs_dlogits(const void* x, const void* w, const
   hipStream_t s = static_cast<hipStream_t>(stream);
   GradParams p = {};
   fill(p, x, w, rows, hidden, vocab, ldx, ldw);
+  p.k = static_cast<float>(1.4426950408889634 / temperature);
   GradRow* of = static_cast<GradRow*>(workspace);
   hipLaunchKernelGGL(grad_rows_kernel, dim3(static_cast<unsigned>((rows + 255) / 256)), dim3(256), 0, s, reinterpret_cast<const f32x2*>(max_sum), dlog_probs, targets, of,
-                     p.M, p.N, temperature, 1.f / temperature, ignore_index);
+                     p.M, p.N, p.k, 1.f / temperature, ignore_index);
   p.c = dlogits;
   p.ldc = static_cast<int>(ldd);
   p.grad_rows = of;
-  p.k = static_cast<float>(1.4426950408889634 / temperature);
   return launch_best<GradTile>(p, fn, s);
 }

@@ -43,7 +43,7 @@ template <typename T, int NT, bool kKeep, typename Fn>
 __device__ __forceinline__ void each_piece(const Row<T>& r, const Fn& fn) {
   constexpr int V = Row<T>::V, U = kUnroll;
   int v = r.template first<NT>();
-  for (; v + (U - 1) * NT < r.nvec; v += U * NT) {
+  for (int whole = r.nvec / (U * NT); whole > 0; --whole, v += U * NT) {
     u32x4 raw[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) raw[u] = load_piece<kKeep>(r.body, v + u * NT);
@@ -54,11 +54,18 @@ __device__ __forceinline__ void each_piece(const Row<T>& r, const Fn& fn) {
       fn(e, v + u * NT);
     }
   }
-  for (; v < r.nvec; v += NT) {
-    float e[V];
-    unpack<T>(load_piece<kKeep>(r.body, v), e);
-    fn(e, v);
-  }
+  // the last ones, requested together too ([1, 64, 32000] 6.4 -> 6.1 us, [16, 1024, 2000] 16.1 -> 11.9)
+  u32x4 raw[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (v + u * NT < r.nvec) raw[u] = load_piece<kKeep>(r.body, v + u * NT);
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (v + u * NT < r.nvec) {
+      float e[V];
+      unpack<T>(raw[u], e);
+      fn(e, v + u * NT);
+    }
 }
 
 template <typename T, int NT, bool kEntropy>
@@ -461,14 +468,16 @@ __global__ __launch_bounds__(kSumThreads) void preference_kernel(const TokenArgs
 
 // ---- launches
 template <int n> using Int = std::integral_constant<int, n>;
-// the narrowest workgroup that has a row in four pieces a thread, eight from 256 threads on: in a wider one most lanes of a short row would idle
-template <typename Fn>
+// the narrowest workgroup that has a row in four pieces a thread, eight from 256 threads on: in a wider one most lanes of a short row would idle.
+// Long rows of the gradient in 1024: [4, 1024, 49152] bf16 124 -> 120 us ([14, 333, 32001], 4000 pieces, 79 -> 92; the forward 52 -> 56).
+template <bool kGrad, typename Fn>
 void with_threads(int64_t vocab, int vec, const Fn& fn) {
   const int64_t pieces = (vocab + vec - 1) / vec;
   if (pieces <= 64 * 4) fn(Int<64>());
   else if (pieces <= 128 * 4) fn(Int<128>());
   else if (pieces <= 256 * 8) fn(Int<256>());
-  else fn(Int<512>());
+  else if (!kGrad || pieces < 1024 * 5) fn(Int<512>());
+  else if constexpr (kGrad) fn(Int<1024>());
 }
 // Threads and pieces per thread of the kernel that holds a row of so many pieces; (0, 0): none does.  As few threads as can hold the row in four or eight pieces: a
 // barrier over fewer waves, and more rows on a CU.  6144 pieces in 1024 x 6, where two rows share a CU, [8, 1024, 49152] bf16 256 us, in 512 x 12 262; with an entropy
@@ -488,10 +497,10 @@ void with_pieces(int64_t vocab, int vec, const Fn& fn) {
   else if (pieces <= 1024 * 16) fn(Int<1024>(), Int<16>());
   else fn(Int<0>(), Int<0>());
 }
-template <typename Fn>
+template <bool kGrad, typename Fn>
 void with_type(const pico_logits& z, const Fn& fn) {
-  if (z.dtype == PICO_BF16) with_threads(z.vocab, 8, [&](auto nt) { fn(__bf16(), nt); });
-  else with_threads(z.vocab, 4, [&](auto nt) { fn(float(), nt); });
+  if (z.dtype == PICO_BF16) with_threads<kGrad>(z.vocab, 8, [&](auto nt) { fn(__bf16(), nt); });
+  else with_threads<kGrad>(z.vocab, 4, [&](auto nt) { fn(float(), nt); });
 }
 template <typename Fn>
 void with_flag(bool v, const Fn& fn) {
@@ -542,7 +551,7 @@ ValueArgs args(const pico_values* v) { return v ? ValueArgs{v->data, v->batch_st
 int run_log_probs(const char* fn, const pico_logits& z, const pico_tokens& targets, float* log_probs, float* entropy, float* max_sum,
                   float temperature, int64_t ignore_index, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(z.batch * z.seq));
-  with_type(z, [&](auto type, auto nt) {
+  with_type<false>(z, [&](auto type, auto nt) {
     with_flag(entropy != nullptr, [&](auto with) {
       hipLaunchKernelGGL((log_probs_kernel<decltype(type), decltype(nt)::value, decltype(with)::value>), grid, dim3(decltype(nt)::value), 0, s, args(z, temperature),
                          args(targets), log_probs, entropy, reinterpret_cast<f32x2*>(max_sum), max_sum ? kept_from(z) : z.batch * z.seq, ignore_index);
@@ -580,7 +589,7 @@ extern "C" int pico_log_probs_bwd(const pico_logits* logits, const pico_tokens* 
   if (int rc = check_gradient(fn, *logits, dlogits, dbatch_stride, drow_stride)) return rc;
   // (with the gradient at hand the launch usually only looks at grad_out: few workgroups, which walk the rows if they must)
   const dim3 grid(static_cast<unsigned>(have_unit ? std::min<int64_t>(rows, 1024) : rows));
-  with_type(*logits, [&](auto type, auto nt) {
+  with_type<true>(*logits, [&](auto type, auto nt) {
     with_flag(with_entropy, [&](auto with) {
       hipLaunchKernelGGL((log_probs_grad_kernel<decltype(type), decltype(nt)::value, decltype(with)::value>), grid, dim3(decltype(nt)::value), 0, static_cast<hipStream_t>(stream),
                          args(*logits, temperature), args(*targets), reinterpret_cast<const f32x2*>(max_sum), entropy, args(dlog_probs), args(dentropy),
@@ -644,7 +653,7 @@ extern "C" int pico_policy_loss_fwd(const pico_logits* logits, const pico_tokens
       });
     };
     with_flag(with_entropy, [&](auto with) {
-      if (!dlogits) with_type(*logits, [&](auto type, auto nt) { stream_row(type, nt, with, std::false_type()); });
+      if (!dlogits) with_type<false>(*logits, [&](auto type, auto nt) { stream_row(type, nt, with, std::false_type()); });
       else if (logits->dtype == PICO_BF16) with_gradient(__bf16(), with);
       else with_gradient(float(), with);
     });

@@ -67,7 +67,8 @@ def check(x, w, t, T=1.0, ignore=IGNORE, seed=0, grads=True):
 
 @pytest.mark.parametrize("rows,hidden,vocab", [(1, 72, 1), (1, 72, 8), (1, 128, 1000), (2, 96, 63), (3, 128, 64), (5, 128, 65), (7, 576, 49152), (64, 72, 257), (65, 200, 511),
                                                (128, 576, 1000), (129, 264, 1003), (257, 2048, 4099), (300, 1000, 32001), (513, 72, 66), (1000, 128, 777), (700, 136, 20000),
-                                               (2049, 192, 4096), (90, 4096, 2500)])
+                                               (2049, 192, 4096), (90, 4096, 2500), (15, 584, 64), (16, 136, 1000), (17, 2048, 999), (32, 320, 4000), (33, 1096, 3000), (48, 264, 640),
+                                               (49, 200, 127), (64, 4096, 2049)])
 def test_over_sizes(device, rows, hidden, vocab):
     x, w, t = inputs(rows + hidden + vocab, rows, hidden, vocab)
     t[0], t[-1] = 0, vocab - 1
@@ -75,7 +76,7 @@ def test_over_sizes(device, rows, hidden, vocab):
     check(x, w, t, T=0.7)
 
 
-@pytest.mark.parametrize("rows", [1, 127, 128, 129, 255, 256, 257, 383, 385, 511, 640, 1023])
+@pytest.mark.parametrize("rows", [1, 16, 17, 32, 33, 64, 65, 127, 128, 129, 255, 256, 257, 383, 385, 511, 640, 1023])
 def test_rows_at_the_ends_of_tiles(device, rows):
     """Every row's target in turn at the ends of the groups of 64 columns and of the tiles."""
     x, w, t = inputs(rows, rows, 128, 1029, kept=1.0)
