@@ -53,9 +53,12 @@ __device__ __forceinline__ f32x2 score(f32x4 (&v)[J], int h, int cols, float k) 
   const float mk = m == -INFINITY ? 0.f : m * k, r = m == -INFINITY ? 0.f : fmaf(m, k, -mk);
   float s = 0.f;
 #pragma unroll
-  for (int j = 0; j < J; ++j)
+  for (int j = 0; j < J; ++j) {
+    float part = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s += fast_exp2(fmaf(v[j][e], k, -mk));
+    for (int e = 0; e < 4; ++e) part += fast_exp2(fmaf(v[j][e], k, -mk));
+    s += part;
+  }
   s = group_sum(s);
   return {m, fmaf(-r * kLn2, s, s)};
 }

@@ -81,16 +81,31 @@ struct Gather {
     if (top > zmax) rise(top, k);
     take(e, k);
   }
+  // none over the maximum.  A piece's sum first: beside a certain token's 1 the others are added one by one with an error of 2^-24 each, and ln S is what they sum to.
   template <int N>
-  __device__ __forceinline__ void take(const float (&e)[N], float k) {   // none over the maximum
+  __device__ __forceinline__ void take(const float (&e)[N], float k) {
+    float ps = 0.f, pw = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const float d = (e[i] - m) * k, p = fast_exp2(d);
-      s += p;
-      if constexpr (kEntropy) w = fmaf(p, fmaxf(d, kFloor), w);
+      ps += p;
+      if constexpr (kEntropy) pw = fmaf(p, fmaxf(d, kFloor), pw);
     }
+    s += ps;
+    if constexpr (kEntropy) w += pw;
   }
 };
+
+// The target's logit joins what was gathered of the others, and its log-probability.  Where it is the largest that is -ln(1 + the others), which keeps its relative
+// accuracy however certain the token is; a sum that held the 1 from the beginning would have lost it.
+template <bool kEntropy>
+__device__ __forceinline__ float with_target(Gather<kEntropy>& g, float xt, float k, float inv_t) {
+  g.rise(fmaxf(g.zmax, xt), k);
+  const float d = (xt - g.m) * k, p = fast_exp2(d), others = g.s;
+  g.s = others + p;
+  if constexpr (kEntropy) g.w = fmaf(p, fmaxf(d, kFloor), g.w);
+  return xt == g.m ? -log1pf(others) : (xt - g.m) * inv_t - logf(g.s);
+}
 
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll

@@ -38,15 +38,17 @@ __device__ __forceinline__ void unpack(const u32x4& raw, float (&out)[io<T>::kVe
   }
 }
 
-// fn(piece's elements, its first index) for every piece of a row that this thread has
-template <typename T, int NT, bool kKeep, typename Fn>
-__device__ __forceinline__ void each_piece(const Row<T>& r, const Fn& fn) {
+// fn(piece's elements, its index) for every piece of a row that this thread has, NT apart; before(pieces as they were loaded, the first one's index) for kUnroll of
+// them at a time
+template <typename T, int NT, bool kKeep, typename Fn, typename Before>
+__device__ __forceinline__ void each_piece(const Row<T>& r, const Fn& fn, const Before& before) {
   constexpr int V = Row<T>::V, U = kUnroll;
   int v = r.template first<NT>();
   for (int whole = r.nvec / (U * NT); whole > 0; --whole, v += U * NT) {
     u32x4 raw[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) raw[u] = load_piece<kKeep>(r.body, v + u * NT);
+    before(raw, v);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       float e[V];
@@ -54,11 +56,12 @@ __device__ __forceinline__ void each_piece(const Row<T>& r, const Fn& fn) {
       fn(e, v + u * NT);
     }
   }
-  // the last ones, requested together too ([1, 64, 32000] 6.4 -> 6.1 us, [16, 1024, 2000] 16.1 -> 11.9)
+  // the last ones, requested together too ([1, 64, 32000] 6.5 -> 5.7 us, [16, 1024, 2000] 16.1 -> 12.0)
   u32x4 raw[U];
 #pragma unroll
   for (int u = 0; u < U; ++u)
     if (v + u * NT < r.nvec) raw[u] = load_piece<kKeep>(r.body, v + u * NT);
+  before(raw, v);
 #pragma unroll
   for (int u = 0; u < U; ++u)
     if (v + u * NT < r.nvec) {
@@ -68,13 +71,40 @@ __device__ __forceinline__ void each_piece(const Row<T>& r, const Fn& fn) {
     }
 }
 
+// where a column lies among a row's pieces (piece -1: in the head; one past the last: in the tail)
+template <typename T>
+struct Place {
+  int piece, elem;
+  __device__ __forceinline__ Place(const Row<T>& r, int t) : piece(t >= r.head ? (t - r.head) / Row<T>::V : -1), elem(t >= r.head ? (t - r.head) % Row<T>::V : 0) {}
+  __device__ __forceinline__ void mask(u32x4& raw) const {   // -inf there, in a piece as it was loaded
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) raw[i] = i == elem ? 0xff800000u : raw[i];
+      else raw[i] = i != elem / 2 ? raw[i] : elem % 2 ? (raw[i] & 0xffffu) | 0xff800000u : (raw[i] & 0xffff0000u) | 0xff80u;
+    }
+  }
+  __device__ __forceinline__ void add(float (&e)[Row<T>::V], float v) const {
+#pragma unroll
+    for (int i = 0; i < Row<T>::V; ++i) e[i] += i == elem ? v : 0.f;
+  }
+};
+
 template <typename T, int NT, bool kEntropy>
-__device__ __forceinline__ Gather<kEntropy> gather_row(const Row<T>& r, float k, bool keep, float (*share)[3]) {
+__device__ __forceinline__ Gather<kEntropy> gather_row(const Row<T>& r, int t, float k, bool keep, float (*share)[3]) {   // all but the target
   Gather<kEntropy> g;
+  const Place<T> target(r, t);
+  const int mine = (target.piece - r.template first<NT>()) % NT == 0 ? target.piece : -1;   // (looked for once in four pieces, by one thread)
   auto add = [&](const float (&e)[Row<T>::V], int) { g.add(e, k); };
-  if (keep) each_piece<T, NT, true>(r, add);
-  else each_piece<T, NT, false>(r, add);
-  if (r.edge >= 0) {
+  auto without_target = [&](u32x4 (&raw)[kUnroll], int v) {
+    if (mine >= v && mine < v + kUnroll * NT) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (mine == v + u * NT) target.mask(raw[u]);
+    }
+  };
+  if (keep) each_piece<T, NT, true>(r, add, without_target);
+  else each_piece<T, NT, false>(r, add, without_target);
+  if (r.edge >= 0 && r.edge != t) {
     const float e[1] = {static_cast<float>(r.x[r.edge])};
     g.add(e, k);
   }
@@ -87,19 +117,17 @@ template <typename T, int NT, bool kEntropy>
 __device__ __forceinline__ void write_gradient(const Row<T>& r, T* d, const Slope& slope, float k, float m, int t, bool kept) {
   constexpr int V = Row<T>::V;
   T* body = d + r.head;
-  const int t_piece = t >= r.head ? (t - r.head) / V : -1, t_elem = t >= r.head ? (t - r.head) % V : 0;
+  const Place<T> target(r, t);
   auto write = [&](const float (&e)[V], int v) {
     float o[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) o[i] = along<kEntropy>(slope, e[i], k, m);
-    if (v == t_piece) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) o[i] += i == t_elem ? slope.hot : 0.f;
-    }
+    if (v == target.piece) target.add(o, slope.hot);
     store_piece(body, v, o);
   };
-  if (kept) each_piece<T, NT, true>(r, write);
-  else each_piece<T, NT, false>(r, write);
+  auto nothing = [](u32x4 (&)[kUnroll], int) {};
+  if (kept) each_piece<T, NT, true>(r, write, nothing);
+  else each_piece<T, NT, false>(r, write, nothing);
   if (r.edge >= 0)
     d[r.edge] = static_cast<T>(along<kEntropy>(slope, static_cast<float>(r.x[r.edge]), k, m) + (r.edge == t ? slope.hot : 0.f));
 }
@@ -128,9 +156,9 @@ __global__ __launch_bounds__(NT) void log_probs_kernel(const LogitsArgs z, const
   }
   const Row<T> r(z.data, b * z.batch_stride + s * z.row_stride, z.vocab);
   const float xt = static_cast<float>(r.x[t]);
-  const Gather<kEntropy> g = gather_row<T, NT, kEntropy>(r, z.k, row >= kept_from, share);
+  Gather<kEntropy> g = gather_row<T, NT, kEntropy>(r, static_cast<int>(t), z.k, row >= kept_from, share);
   if (threadIdx.x == 0) {
-    log_probs[row] = (xt - g.zmax) * z.inv_t - logf(g.s);
+    log_probs[row] = with_target(g, xt, z.k, z.inv_t);
     if constexpr (kEntropy) entropy[row] = logf(g.s) - kLn2 * g.w / g.s;
     if (max_sum != nullptr) max_sum[row] = f32x2{g.m, g.s};
   }
@@ -237,8 +265,8 @@ __global__ __launch_bounds__(NT) void policy_kernel(const LogitsArgs z, const To
   }
   const float xt = static_cast<float>(r.x[t]);
   const PolicyInputs in(p, b, s, kGrad);
-  const Gather<kEntropy> g = gather_row<T, NT, kEntropy>(r, z.k, kGrad, share);   // (with a gradient the row is read again below)
-  float q = (xt - g.zmax) * z.inv_t - logf(g.s);
+  Gather<kEntropy> g = gather_row<T, NT, kEntropy>(r, static_cast<int>(t), z.k, kGrad, share);   // (with a gradient the row is read again below)
+  float q = with_target(g, xt, z.k, z.inv_t);
   asm volatile("" : "+v"(q));   // (rounded as it is stored, or its difference from `old` is taken before the rounding: where they are equal the ratio is 1)
   const float H = kEntropy ? logf(g.s) - kLn2 * g.w / g.s : 0.f;
   const PolicyRow l = policy_row(p, in, q, H);
@@ -307,8 +335,10 @@ __global__ __launch_bounds__(NT, NV <= 6 ? 8 : NV <= 8 ? 6 : NV <= 12 ? 5 : 4) v
 #pragma unroll
     for (int i = 0; i < V; ++i) top = fmaxf(top, e[i]);
   }
-  hide();
   g.rise(top, z.k);
+  const int ti = static_cast<int>(t);
+  const Place<T> target(r, ti);
+  hide();
   {
     const float e[1] = {xe};
     g.take(e, z.k);
@@ -328,7 +358,7 @@ __global__ __launch_bounds__(NT, NV <= 6 ? 8 : NV <= 8 ? 6 : NV <= 12 ? 5 : 4) v
     for (int i = 0; i < W; ++i) n += counted[i];
     in.w = p.scale / static_cast<float>(n);   // (this row is one of them)
   }
-  float q = (xt - g.zmax) * z.inv_t - logf(g.s);
+  float q = (xt - g.zmax) * z.inv_t - logf(g.s);   // (the target among the others: taking it out of a row that is held costs registers that are not there)
   asm volatile("" : "+v"(q));   // (rounded as it is stored, or its difference from `old` is taken before the rounding: where they are equal the ratio is 1)
   const float H = kEntropy ? logf(g.s) - kLn2 * g.w / g.s : 0.f;
   const PolicyRow l = policy_row(p, in, q, H);
@@ -341,7 +371,6 @@ __global__ __launch_bounds__(NT, NV <= 6 ? 8 : NV <= 8 ? 6 : NV <= 12 ? 5 : 4) v
   }
   const Slope along_row = slope<kEntropy>(l.a, l.b, g.s, H, z.inv_t);
   T* body = d + r.head;
-  const int ti = static_cast<int>(t), t_piece = ti >= r.head ? (ti - r.head) / V : -1, t_elem = ti >= r.head ? (ti - r.head) % V : 0;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int v = first + j * NT;
@@ -350,10 +379,7 @@ __global__ __launch_bounds__(NT, NV <= 6 ? 8 : NV <= 8 ? 6 : NV <= 12 ? 5 : 4) v
       unpack<T>(raw[j], e);
 #pragma unroll
       for (int i = 0; i < V; ++i) e[i] = along<kEntropy>(along_row, e[i], z.k, g.m);
-      if (v == t_piece) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) e[i] += i == t_elem ? along_row.hot : 0.f;
-      }
+      if (v == target.piece) target.add(e, along_row.hot);
       store_piece(body, v, e);
     }
     __builtin_amdgcn_sched_barrier(0);

@@ -206,6 +206,25 @@ def test_log_probs_of_the_lowest_values(device, dtype):
     check_policy(x, t, torch.ones(1, 3, device="cuda"), ent=0.01)
 
 
+@pytest.mark.parametrize("vocab", [100, 2001, 49152])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_log_probs_of_nearly_certain_tokens(device, dtype, vocab):
+    """-ln(1 + r) with a small r = the sum of the others' exponentials keeps the relative accuracy of r (2^-16, as above, and twice the roundings of its
+    terms' arguments, |D| u ln2 each with |D| up to 60: 2^-16 again), where 1 + r would be off by 2^-24 / r."""
+    from picotron_amd.functional import log_probs
+    g = gen(vocab)
+    x = logits_of(g, 1, 12, vocab, dtype=dtype, scale=1.0)
+    t = torch.randint(0, vocab, (1, 12), generator=g, device="cuda")
+    t[0, 0], t[0, 1] = 0, vocab - 1
+    up = torch.linspace(12, 38, 12, device="cuda").to(dtype)
+    x.scatter_(2, t[..., None], up[None, :, None])
+    lp = reference(x, t, 1.0)[0]
+    rest = x.double().scatter(2, t[..., None], -float("inf"))
+    want = -torch.log1p((rest - up.double()[None, :, None]).exp().sum(-1))
+    assert (want - lp).abs().max().item() < 1e-9 and want.abs().max().item() < 0.1
+    assert ((log_probs(x, t).double() - want).abs() <= 2 ** -15 * want.abs()).all()
+
+
 def test_log_probs_past_32_bits(device):
     """A batch whose second sequence starts more than 2^31 elements behind the first."""
     from picotron_amd.functional import log_probs
