@@ -221,7 +221,7 @@ def test_log_probs_of_nearly_certain_tokens(device, dtype, vocab):
     lp = reference(x, t, 1.0)[0]
     rest = x.double().scatter(2, t[..., None], -float("inf"))
     want = -torch.log1p((rest - up.double()[None, :, None]).exp().sum(-1))
-    assert (want - lp).abs().max().item() < 1e-9 and want.abs().max().item() < 0.1
+    assert (want - lp).abs().max().item() < 1e-9 and want.abs().max().item() < 0.7      # (49152 e^0.5 e^-12 is 0.5)
     assert ((log_probs(x, t).double() - want).abs() <= 2 ** -15 * want.abs()).all()
 
 
