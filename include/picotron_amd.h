@@ -433,9 +433,10 @@ int pico_cross_entropy_mean_bwd(const void* logits, const int64_t* targets, cons
  * Logits are rows of `vocab` contiguous elements, row (b, s) at data + b * batch_stride + s * row_stride (elements, not negative);
  * a row may start at any element.  A value or token per row has two strides of its own, 0 among them (broadcast).
  * A target that equals ignore_index or lies outside [0, vocab) is never used as an index: the row is not read, its results are
- * 0 and so is its gradient row.  z = logits / temperature, p = softmax(z), q = log p_target.  batch * seq < 2^31, vocab < 2^30.
- * dlogits: rows that do not overlap, each as far from a 16-byte boundary as its row of logits (buffers of the logits' own
- * strides whose addresses agree modulo 16 do); it may be the logits themselves.
+ * 0 and so is its gradient row.  z = logits / temperature, p = softmax(z), q = log p_target.  batch * seq < 2^22 (more for short
+ * rows: a launch has fewer than 2^32 threads), vocab < 2^29.
+ * dlogits: memory of its own, rows that do not overlap, each as far from a 16-byte boundary as its row of logits (buffers of the
+ * logits' own strides whose addresses agree modulo 16 do).
  */
 typedef struct pico_logits {
   const void* data;

@@ -1499,11 +1499,12 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
                                int64_t ignore_index, double temperature, double scale) {
     Saved k;
     variable_list out = run(logits, targets, advantages, old_lp, ref_lp, weights, {clip_low, clip_high, kl_coef, entropy_coef, temperature, scale, ignore_index}, &k);
-    ctx->save_for_backward({logits, targets, k.unit, k.rows});
+    ctx->save_for_backward({logits, targets, k.rows});
+    // (not among the saved variables: it is handed over as the gradient, whose owner may change it in place between two backward passes)
+    ctx->saved_data["unit"] = k.unit;
     ctx->saved_data["ignore"] = ignore_index;
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["entropy"] = static_cast<float>(entropy_coef) != 0;
-    ctx->saved_data["spent"] = false;
     ctx->mark_non_differentiable({out[1]});
     ctx->set_materialize_grads(false);
     return out;
@@ -1517,12 +1518,16 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     const TokenRows r = token_rows("policy_loss", s[0], s[1]);
     const Tensor up = g[0].to(at::kFloat).contiguous();
     // a second backward through this node (retain_graph) gets a buffer of its own
-    const bool spent = ctx->saved_data["spent"].toBool(), with_entropy = ctx->saved_data["entropy"].toBool();
-    ctx->saved_data["spent"] = true;
+    Tensor unit;
+    if (const auto it = ctx->saved_data.find("unit"); it != ctx->saved_data.end()) {
+      unit = it->second.toTensor();
+      ctx->saved_data.erase(it);
+    }
+    const bool with_entropy = ctx->saved_data["entropy"].toBool();
     const int64_t seq = r.z.seq;
-    const pico_policy_saved kept = Saved::parts(s[3], s[1].numel(), with_entropy);
+    const pico_policy_saved kept = Saved::parts(s[2], s[1].numel(), with_entropy);
     const pico_values dlp = {kept.dlog_probs, seq, 1}, dh = {kept.dentropy, seq, 1};
-    d[0] = log_probs_gradient(r, kept.max_sum, kept.entropy, dlp, dh, up, spent ? Tensor() : s[2], ctx->saved_data["temperature"].toDouble(),
+    d[0] = log_probs_gradient(r, kept.max_sum, kept.entropy, dlp, dh, up, unit, ctx->saved_data["temperature"].toDouble(),
                               ctx->saved_data["ignore"].toInt());
     if (s[0].dim() != 3) d[0] = d[0].view(s[0].sizes());
     return d;
@@ -1597,9 +1602,11 @@ std::pair<Tensor, Tensor> preference_loss(const Tensor& logits, const Tensor& ta
 // log p of the targets under softmax(x w^T / temperature) without the logits in memory; the backward computes them again, as their
 // gradient, which lives until the two products with it are done.
 struct LinearLogProbs : torch::autograd::Function<LinearLogProbs> {
+  static int64_t pitch(const Tensor& m) { return m.size(0) > 1 ? m.stride(0) : m.size(1); }
   static Tensor rows(const Tensor& t) {   // as the products take them
     const Tensor m = t.dim() == 1 ? t.unsqueeze(0) : matrix(t);
-    return m.stride(1) == 1 && m.stride(0) % 8 == 0 && m.stride(0) >= m.size(1) && reinterpret_cast<uintptr_t>(m.data_ptr()) % 16 == 0 ? m : m.contiguous();
+    const bool fits = (m.size(1) == 1 || m.stride(1) == 1) && pitch(m) % 8 == 0 && pitch(m) >= m.size(1) && reinterpret_cast<uintptr_t>(m.data_ptr()) % 16 == 0;
+    return fits ? m : m.clone(at::MemoryFormat::Contiguous);
   }
   static Tensor run(const Tensor& x, const Tensor& w, const Tensor& targets, int64_t ignore_index, double temperature, Tensor* max_sum) {
     const char* fn = "linear_log_probs";
@@ -1613,8 +1620,8 @@ struct LinearLogProbs : torch::autograd::Function<LinearLogProbs> {
     if (max_sum) *max_sum = per_token(targets, x, 2);
     const int64_t bytes = pico_linear_log_probs_workspace_bytes(a.size(0), b.size(0));
     const Tensor ws = at::empty({std::max<int64_t>(bytes, 8)}, x.options().dtype(at::kByte));
-    check(pico_linear_log_probs_fwd(ptr(a), ptr(b), t.data_ptr<int64_t>(), fptr(lp), max_sum ? fptr(*max_sum) : nullptr, a.size(0), a.size(1), b.size(0), a.stride(0),
-                                    b.stride(0), static_cast<float>(temperature), ignore_index, ptr(ws), bytes, stream_now()));
+    check(pico_linear_log_probs_fwd(ptr(a), ptr(b), t.data_ptr<int64_t>(), fptr(lp), max_sum ? fptr(*max_sum) : nullptr, a.size(0), a.size(1), b.size(0), pitch(a),
+                                    pitch(b), static_cast<float>(temperature), ignore_index, ptr(ws), bytes, stream_now()));
     return lp;
   }
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& targets, int64_t ignore_index, double temperature) {
@@ -1631,9 +1638,9 @@ struct LinearLogProbs : torch::autograd::Function<LinearLogProbs> {
     const Tensor &x = s[0], &w = s[1];
     const c10::OptionalDeviceGuard device(x.device());
     const Tensor a = rows(x), b = rows(w), t = s[2].contiguous(), dlp = g[0].to(at::kFloat).contiguous();
-    const int64_t M = a.size(0), N = b.size(0), pitch = (N + 7) / 8 * 8;
-    const Tensor dz = at::empty({M, pitch}, a.options()), ws = at::empty({std::max<int64_t>(M * 16, 16)}, a.options().dtype(at::kByte));
-    check(pico_linear_log_probs_dlogits(ptr(a), ptr(b), t.data_ptr<int64_t>(), fptr(s[3]), fptr(dlp), ptr(dz), M, a.size(1), N, a.stride(0), b.stride(0), pitch,
+    const int64_t M = a.size(0), N = b.size(0), ldd = (N + 7) / 8 * 8;
+    const Tensor dz = at::empty({M, ldd}, a.options()), ws = at::empty({std::max<int64_t>(M * 16, 16)}, a.options().dtype(at::kByte));
+    check(pico_linear_log_probs_dlogits(ptr(a), ptr(b), t.data_ptr<int64_t>(), fptr(s[3]), fptr(dlp), ptr(dz), M, a.size(1), N, pitch(a), pitch(b), ldd,
                                         static_cast<float>(ctx->saved_data["temperature"].toDouble()), ctx->saved_data["ignore"].toInt(), ptr(ws), M * 16, stream_now()));
     const Tensor d = dz.narrow(1, 0, N);
     variable_list r(5);

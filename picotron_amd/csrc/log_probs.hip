@@ -403,12 +403,22 @@ __global__ __launch_bounds__(kSumThreads) void policy_sum_kernel(const TokenArgs
   __shared__ int red_n[kSumWaves];
   double sum = 0;
   int n = 0;
-  for (int64_t row = threadIdx.x; row < rows; row += kSumThreads) {
-    if (count) {
-      const int64_t b = row / seq;
-      n += is_token(targets.at(b, row - b * seq), ignore_index, vocab);
+  constexpr int U = 8;   // rows requested together
+  for (int64_t first = threadIdx.x; first < rows; first += U * kSumThreads) {
+    float l[U];
+    int64_t t[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = first + u * kSumThreads, b = row / seq;
+      const bool in = row < rows;
+      t[u] = in && count ? targets.at(b, row - b * seq) : ignore_index;
+      l[u] = in && loss != nullptr ? losses[row] : 0.f;
     }
-    if (loss != nullptr) sum += losses[row];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      n += is_token(t[u], ignore_index, vocab);
+      sum += l[u];
+    }
   }
   sum = wave_sum64(sum);
 #pragma unroll
@@ -449,9 +459,22 @@ __global__ __launch_bounds__(kSumThreads) void preference_kernel(const TokenArgs
     double sum = 0;
     int n = 0;
     if (b < sequences) {
-      for (int s = wave % team * kWave + lane; s < seq; s += team * kWave) {
-        sum += p.log_probs[static_cast<int64_t>(b) * seq + s];
-        if (p.average) n += is_token(targets.at(b, s), ignore_index, vocab);
+      constexpr int U = 4;   // tokens requested together
+      const int step = team * kWave;
+      for (int64_t first = wave % team * kWave + lane; first < seq; first += U * step) {
+        float q[U];
+        int64_t t[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int64_t s = first + u * step;
+          q[u] = s < seq ? p.log_probs[static_cast<int64_t>(b) * seq + s] : 0.f;
+          t[u] = s < seq && p.average ? targets.at(b, s) : ignore_index;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          sum += q[u];
+          n += is_token(t[u], ignore_index, vocab);
+        }
       }
     }
     sum = wave_sum64(sum);
@@ -539,9 +562,13 @@ int check_logits(const char* fn, const pico_logits* z, const pico_tokens* target
   if (z->dtype != PICO_BF16 && z->dtype != PICO_F32) return fail(PICO_ERR_DTYPE, "%s: dtype code %d not supported", fn, z->dtype);
   constexpr int64_t kMost = 0x7fffffff;
   // (one workgroup per row; vocab: a row's index fits 32 bits with room for the pieces of an unrolled step)
-  if (z->batch < 0 || z->seq < 0 || z->vocab <= 0 || z->vocab > kMost / 2 || z->seq > kMost || z->batch > kMost || z->batch * z->seq > kMost)
+  if (z->batch < 0 || z->seq < 0 || z->vocab <= 0 || z->vocab > kMost / 4 || z->seq > kMost || z->batch > kMost || z->batch * z->seq > kMost)
     return fail(PICO_ERR_SHAPE, "%s: batch=%lld seq=%lld vocab=%lld", fn, static_cast<long long>(z->batch), static_cast<long long>(z->seq),
                 static_cast<long long>(z->vocab));
+  // (a launch has fewer than 2^32 threads)
+  const int64_t threads = z->vocab <= 2048 ? 128 : z->vocab <= 8192 ? 256 : 1024;
+  if (z->batch * z->seq > 0xffffffffll / threads)
+    return fail(PICO_ERR_SHAPE, "%s: %lld rows of %lld, at most %lld", fn, static_cast<long long>(z->batch * z->seq), static_cast<long long>(z->vocab), 0xffffffffll / threads);
   if (!(temperature > 0.f) || !(temperature <= 1e30f) || !(1.f / temperature <= 1e30f)) return fail(PICO_ERR_SHAPE, "%s: temperature %g must be positive and finite", fn, temperature);
   if (z->batch * z->seq > 0) {
     if (!z->data || !targets->data) return fail(PICO_ERR_NULL, "%s: logits and targets are required", fn);
@@ -613,8 +640,8 @@ extern "C" int pico_log_probs_bwd(const pico_logits* logits, const pico_tokens* 
     return fail(PICO_ERR_NULL, "%s: max_sum, dlogits, one of dlog_probs and dentropy, entropy with the latter and grad_out with have_unit are required", fn);
   if (reinterpret_cast<uintptr_t>(max_sum) % 8) return fail(PICO_ERR_ALIGN, "%s: max_sum must be aligned to 8 bytes", fn);
   if (int rc = check_gradient(fn, *logits, dlogits, dbatch_stride, drow_stride)) return rc;
-  // (with the gradient at hand the launch usually only looks at grad_out: few workgroups, which walk the rows if they must)
-  const dim3 grid(static_cast<unsigned>(have_unit ? std::min<int64_t>(rows, 1024) : rows));
+  // (with the gradient at hand the launch usually only looks at grad_out: as many workgroups as the GPU holds at once, which walk the rows if they must)
+  const dim3 grid(static_cast<unsigned>(have_unit ? std::min<int64_t>(rows, 512) : rows));
   with_type<true>(*logits, [&](auto type, auto nt) {
     with_flag(with_entropy, [&](auto with) {
       hipLaunchKernelGGL((log_probs_grad_kernel<decltype(type), decltype(nt)::value, decltype(with)::value>), grid, dim3(decltype(nt)::value), 0, static_cast<hipStream_t>(stream),

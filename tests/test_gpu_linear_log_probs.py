@@ -103,6 +103,11 @@ def test_strides(device):
     check(wide[..., 3:203], big[:, 5:205], ids[:, 1:])
     check(wide.view(2, 3, 50, 400)[..., :200], big[:, :200], ids[:, 1:].reshape(2, 3, 50))
     check(wide[2, 3, :200], big[:, :200], ids[2, 3])
+    flat = torch.randn(1 + 7 * 200, generator=g, device="cuda").to(BF16)
+    check(flat[1:].view(7, 200), big[:, :200], ids[0, :7])          # rows without gaps that start beside a 16-byte boundary
+    odd = torch.randn(5, 403, generator=g, device="cuda").to(BF16)
+    check(odd[2:3, :200], big[:, :200], ids[0, :1])                  # one row, whose pitch does not matter
+    check(odd[:, :200], big[4:5, :200], torch.zeros_like(ids[0, :5]))
 
 
 def test_tokens_that_do_not_count(device):

@@ -381,6 +381,23 @@ def test_policy_loss_at_and_around_the_borders(device):
     assert abs(loss.item() + 1.2 * (A.abs() + 0.1).mean().item()) <= 1e-5 and not d.any()
 
 
+def test_policy_loss_without_rows_and_backward_several_times(device):
+    from picotron_amd.functional import policy_loss
+    e = torch.empty(0, 5, 8, dtype=BF16, device="cuda").requires_grad_()
+    none = torch.empty(0, 5, device="cuda")
+    for w in (None, none):
+        loss, q = policy_loss(e, none.long(), none, weights=w, kl_coef=0.1, ref_log_probs=none)
+        assert loss.item() == 0.0 and q.shape == (0, 5) and torch.autograd.grad(loss, e)[0].shape == e.shape
+    # a leaf's .grad is the buffer that the forward wrote, and later passes add to it in place
+    x, t, A, old, ref, w = policy_inputs(41, 2, 6, 777, F32)
+    y = x.clone().requires_grad_()
+    loss, _ = policy_loss(y, t, A, old, ref, w, kl_coef=0.1)
+    for _ in range(3):
+        loss.backward(retain_graph=True)
+    (once,) = torch.autograd.grad(loss, y)
+    assert (y.grad - 3 * once).abs().max().item() <= 2 ** -22 * once.abs().max().item() * 3
+
+
 def test_policy_loss_ignores_what_does_not_count(device):
     """NaN in the logits, advantages and log-probabilities of tokens that do not count, targets outside the vocabulary."""
     x, t, A, old, ref, w = policy_inputs(31, 3, 8, 1003, BF16, kept=1.0)

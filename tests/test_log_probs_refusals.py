@@ -35,7 +35,7 @@ def message(lib):
     return lib.pico_last_error().decode()
 
 
-@pytest.mark.parametrize("over,code", [(dict(dtype=7), -2), (dict(vocab=0), -3), (dict(vocab=1 << 30), -3), (dict(batch=-1), -3), (dict(batch=1 << 20, seq=1 << 12), -3),
+@pytest.mark.parametrize("over,code", [(dict(dtype=7), -2), (dict(vocab=0), -3), (dict(vocab=1 << 29), -3), (dict(batch=-1), -3), (dict(batch=1 << 20, seq=1 << 12), -3), (dict(batch=1 << 20, seq=5, vocab=40000), -3), (dict(batch=1 << 20, seq=40), -3),
                                        (dict(data=None), -1), (dict(data=4097), -4), (dict(row_stride=-8), -5), (dict(batch_stride=-8), -5)])
 def test_logits_that_are_refused_everywhere(lib, over, code):
     from picotron_amd._lib import PerRow, Policy, PolicySaved
