@@ -1,7 +1,7 @@
 // Log-probabilities of given tokens straight from hidden states x [M, K] and the vocabulary projection w [N, K]: the logits
 // z = x w^T / T are a matrix product whose tiles never leave the CU.
-//   forward : the product's epilogue reduces a tile to (max, sum of 2^D) per row and 64 columns (16 bytes of partial results
-//             for what would be 128 of bf16 logits and back), and picks the target's logit where its column passes; a second launch
+//   forward : the product's epilogue reduces a tile to (max, sum of 2^D) per row and 48 or 64 columns (16 bytes of partial
+//             results, there and back, for what would be 256 of bf16 logits), and picks the target's logit where its column passes; a second launch
 //             joins a row's partial results.
 //   backward: the product again (the logits were not kept), whose epilogue turns z into d(logits) = g ([j = t] - p_j) / T with the row's
 //             maximum and sum from the forward, bf16; the gradients of x and w are two more products.
@@ -12,8 +12,9 @@
 namespace pico {
 namespace {
 
-// of 16 columns each: a wave's share of a tile, and the width of a partial result
-constexpr int kJ = 4, kGroup = 16 * kJ;
+// A wave has 16 J columns of a tile, which are a group: the width of a partial result.
+constexpr int kFewJ = 4, kFewGroup = 16 * kFewJ, kLeastGroup = 48;
+int groups_of(int64_t N, int width) { return static_cast<int>((N + width - 1) / width); }
 
 // Partial results: (max, sum) of row r and group g at [r / 64][g][r % 64], so that a wave writes whole lines and a workgroup that joins reads neighbouring ones.
 struct ScoreParams : LargeParams {
@@ -32,10 +33,10 @@ __device__ __forceinline__ float group_max(float v) {   // over the four lanes t
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return half_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
 }
-// (max, sum of 2^D) of 64 columns of a row, 16 of them in this lane: columns 16 j + 4 h + e, of which the first `cols` are there
+// (max, sum of 2^D) of 16 J columns of a row, 4 J of them in this lane: columns 16 j + 4 h + e, of which the first `cols` are there
 template <int J>
 __device__ __forceinline__ f32x2 score(f32x4 (&v)[J], int h, int cols, float k) {
-  if (cols < kGroup) {   // columns past the vocabulary
+  if (cols < 16 * J) {   // columns past the vocabulary
     const int left = hidden(cols - 4 * h);
 #pragma unroll
     for (int j = 0; j < J; ++j)
@@ -62,11 +63,11 @@ __device__ __forceinline__ f32x2 score(f32x4 (&v)[J], int h, int cols, float k) 
   s = group_sum(s);
   return {m, fmaf(-r * kLn2, s, s)};
 }
-// the target's logit to `to`, where its column is one of these 64 (nearly always none of 16 rows' is); t: the target, two words
+// the target's logit to `to`, where its column is one of these (nearly always none of 16 rows' is); t: the target, two words
 template <int J>
 __device__ __forceinline__ void pick(const f32x4 (&v)[J], int2 t, int h, int col0, int vocab, bool live, float* to) {
   const int at = t.y == 0 && t.x >= 0 && t.x < vocab ? t.x - col0 : -1, place = at - 4 * h;
-  if (__any(at >= 0 && at < kGroup)) {
+  if (__any(at >= 0 && at < 16 * J)) {
     float z = 0.f;
     bool here = false;
 #pragma unroll
@@ -87,7 +88,7 @@ __device__ __forceinline__ void request4_to(uint32_t lds_off, u32x4 window, uint
                : "=&{m0}"(aim) : "s"(lds_off), "n"(kPlus), "v"(off), "s"(window) : "scc", "memory");
 }
 
-// Epilogue of the forward.  A lane holds columns 4 h ..+3 (h = lane / 16) of 16 consecutive ones, of row lane % 16 of 16: a row's 64
+// Epilogue of the forward.  A lane holds columns 4 h ..+3 (h = lane / 16) of 16 consecutive ones, of row lane % 16 of 16: a row's
 // columns meet over four lanes.  128 exponentials a lane at a quarter of the vector rate are most of it.
 struct ScoreTile {
   using Params = ScoreParams;
@@ -111,7 +112,7 @@ struct ScoreTile {
     const float k = p.k;
     f32x2 mine = {0.f, 0.f};   // of row 64 q + lane
     const int live = p.M - row0;
-    const u32x4 w = request_window(reinterpret_cast<uint64_t>(p.partial + (static_cast<int64_t>(row0 / 64) * p.groups + col0 / kGroup) * 64), 0x7ffffff0u);
+    const u32x4 w = request_window(reinterpret_cast<uint64_t>(p.partial + (static_cast<int64_t>(row0 / 64) * p.groups + col0 / (16 * J)) * 64), 0x7ffffff0u);
     const buffer_rsrc window = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(w[0] | static_cast<uint64_t>(w[1]) << 32), 0, static_cast<int>(w[2]), static_cast<int>(w[3]));
 #pragma unroll
     for (int i = 0; i < I; ++i) {
@@ -135,41 +136,41 @@ struct ScoreTile {
 // 50.4, 32 rows 59.9, 54.8, 24 x 576 21.6, 17.9.  For 64 rows x is read as often as w: 58.9, 66.3; they stay with the product.
 template <int RB>
 __global__ __launch_bounds__(256, 3) void score_few_kernel(const ScoreParams p) {
-  __shared__ f32x4 sums[4][RB][kJ][kWave];
+  __shared__ f32x4 sums[4][RB][kFewJ][kWave];
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), n = lane % 16, h = lane / 16;
-  const int col0 = blockIdx.x * kGroup, cols = p.N - col0;
+  const int col0 = blockIdx.x * kFewGroup, cols = p.N - col0;
   const char* w = reinterpret_cast<const char*>(p.b + static_cast<int64_t>(col0) * p.ldb);
   const char* x = reinterpret_cast<const char*>(p.a);
-  uint32_t wo[kJ], xo[RB];   // (rows past the end read the last one)
+  uint32_t wo[kFewJ], xo[RB];   // (rows past the end read the last one)
 #pragma unroll
-  for (int j = 0; j < kJ; ++j) wo[j] = static_cast<uint32_t>(min(16 * j + n, cols - 1) * p.ldb * 2 + 16 * h);
+  for (int j = 0; j < kFewJ; ++j) wo[j] = static_cast<uint32_t>(min(16 * j + n, cols - 1) * p.ldb * 2 + 16 * h);
 #pragma unroll
   for (int b = 0; b < RB; ++b) xo[b] = static_cast<uint32_t>(min(16 * b + n, p.M - 1) * p.lda * 2 + 16 * h);
   struct Step {
-    bf16x8 w[2][kJ], x[2][RB];
+    bf16x8 w[2][kFewJ], x[2][RB];
   };
   auto load = [&](Step& f, int step) __attribute__((always_inline)) {
     const char *wk = w + step * 128, *xk = x + step * 128;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
 #pragma unroll
-      for (int j = 0; j < kJ; ++j) f.w[s][j] = *reinterpret_cast<const bf16x8*>(wk + (wo[j] + 64u * s));
+      for (int j = 0; j < kFewJ; ++j) f.w[s][j] = *reinterpret_cast<const bf16x8*>(wk + (wo[j] + 64u * s));
 #pragma unroll
       for (int b = 0; b < RB; ++b) f.x[s][b] = *reinterpret_cast<const bf16x8*>(xk + (xo[b] + 64u * s));
     }
   };
-  f32x4 acc[RB][kJ];
+  f32x4 acc[RB][kFewJ];
 #pragma unroll
   for (int b = 0; b < RB; ++b)
 #pragma unroll
-    for (int j = 0; j < kJ; ++j) acc[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < kFewJ; ++j) acc[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   auto multiply = [&](const Step& f) __attribute__((always_inline)) {
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int b = 0; b < RB; ++b)
 #pragma unroll
-        for (int j = 0; j < kJ; ++j) acc[b][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.w[s][j], f.x[s][b], acc[b][j], 0, 0, 0);
+        for (int j = 0; j < kFewJ; ++j) acc[b][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.w[s][j], f.x[s][b], acc[b][j], 0, 0, 0);
   };
   const int whole = p.K / 64;
   Step one, two;
@@ -190,7 +191,7 @@ __global__ __launch_bounds__(256, 3) void score_few_kernel(const ScoreParams p) 
     for (int s = 0; s < 2; ++s) {
       const bool in = whole * 64 + 32 * s + 8 * h < p.K;
 #pragma unroll
-      for (int j = 0; j < kJ; ++j) {
+      for (int j = 0; j < kFewJ; ++j) {
         one.w[s][j] = bf16x8{};
         if (in) one.w[s][j] = *reinterpret_cast<const bf16x8*>(wk + (wo[j] + 64u * s));
       }
@@ -205,12 +206,12 @@ __global__ __launch_bounds__(256, 3) void score_few_kernel(const ScoreParams p) 
 #pragma unroll
   for (int b = 0; b < RB; ++b)
 #pragma unroll
-    for (int j = 0; j < kJ; ++j) sums[wave][b][j][lane] = acc[b][j];
+    for (int j = 0; j < kFewJ; ++j) sums[wave][b][j][lane] = acc[b][j];
   __syncthreads();
   for (int b = wave; b < RB; b += 4) {
-    f32x4 v[kJ];
+    f32x4 v[kFewJ];
 #pragma unroll
-    for (int j = 0; j < kJ; ++j) v[j] = (sums[0][b][j][lane] + sums[1][b][j][lane]) + (sums[2][b][j][lane] + sums[3][b][j][lane]);
+    for (int j = 0; j < kFewJ; ++j) v[j] = (sums[0][b][j][lane] + sums[1][b][j][lane]) + (sums[2][b][j][lane] + sums[3][b][j][lane]);
     const int row = 16 * b + n;
     const bool live = row < p.M;
     const int2 t = live ? *reinterpret_cast<const int2*>(p.targets + row) : int2{-1, -1};
@@ -313,7 +314,7 @@ struct GradTile {
           const float p = fast_exp2(fmaf(acc[i][j][e], k, -r.lse2)), d = r.g * ((at == 16 * j + e ? 1.f : 0.f) - p);
           acc[i][j][e] = r.counts ? d : 0.f;
         }
-      if (cols < kGroup) {   // zeros in the columns that pad a row
+      if (cols < 16 * J) {   // zeros in the columns that pad a row
         const int left = hidden(cols - 4 * h);
 #pragma unroll
         for (int j = 0; j < J; ++j)
@@ -326,31 +327,47 @@ struct GradTile {
   }
 };
 
-template <int I, typename Epilogue>
+template <int I, int J, typename Epilogue>
 int launch(typename Epilogue::Params p, const char* fn, hipStream_t s) {
-  using S = Shape<false, false, I, kJ>;
+  using S = Shape<false, false, I, J>;
   static LdsOnce reserved;
-  if (!reserve_lds_once(reserved, reinterpret_cast<const void*>(&product_large_kernel<false, false, I, kJ, Epilogue>), S::kLds))
+  if (!reserve_lds_once(reserved, reinterpret_cast<const void*>(&product_large_kernel<false, false, I, J, Epilogue>), S::kLds))
     return fail(PICO_ERR_LAUNCH, "%s: cannot reserve %d bytes of LDS", fn, S::kLds);
   p.tiles_m = (p.M + S::TM - 1) / S::TM;
   p.tiles_n = (p.N + S::TN - 1) / S::TN;
   p.parts = 1;
   const int64_t units = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
   p.streaming = units > 256;   // (as pico_product_large)
-  hipLaunchKernelGGL((product_large_kernel<false, false, I, kJ, Epilogue>), dim3(static_cast<unsigned>(std::min<int64_t>(units, 256))), dim3(S::kThreads), S::kLds, s, p);
+  hipLaunchKernelGGL((product_large_kernel<false, false, I, J, Epilogue>), dim3(static_cast<unsigned>(std::min<int64_t>(units, 256))), dim3(S::kThreads), S::kLds, s, p);
   return check_launch(fn);
 }
-// The tile's rows: what costs least in rounds of 256 workgroups.
-template <typename Epilogue>
-int launch_best(const typename Epilogue::Params& p, const char* fn, hipStream_t s) {
-  const int64_t tiles_n = (p.N + 255) / 256;
-  auto cost = [&](int64_t tm) { return ((p.M + tm - 1) / tm * tiles_n + 255) / 256 * (tm + 32); };
-  int best = 256;
-  for (int tm : {192, 128})
-    if (cost(tm) < cost(best)) best = tm;
-  if (best == 256) return launch<8, Epilogue>(p, fn, s);
-  if (best == 192) return launch<6, Epilogue>(p, fn, s);
-  return launch<4, Epilogue>(p, fn, s);
+// fn(rows / 32, columns / 64) of the tile whose rounds of 256 workgroups take the least time.  A round's time relative to 256 x 256, at [3000 x 2048] @
+// [49152 x 2048]^T: 51.8 us, 192 x 256 41.5, 256 x 192 42.5, 128 x 256 32.9, 128 x 192 28.1 (256 x 128 was never the best).  Over 60 shapes of 40 .. 3000 rows,
+// hidden sizes 232 .. 4008 and vocabularies 2392 .. 120696 the rule is within 2 % of the best tile; with one of 256 columns throughout it lost up to 19 %: us at
+// [rows x 2048] @ [49152 x 2048]^T, 256 x 256 | 192 x 256 | 128 x 256 | 256 x 192 | 128 x 192:
+//    128 rows  61.8 |  59.7 |  58.9 |  59.7 |  54.9
+//    256 rows  69.0 |  91.6 |  89.7 |  64.9 |  80.6
+//    300 rows 100.9 |  93.6 | 116.4 |  96.2 | 108.5
+//    512 rows 109.9 | 129.6 | 120.4 | 100.8 | 139.5
+//   1000 rows 165.9 | 206.7 | 221.0 | 180.6 | 261.1
+template <typename Fn>
+int with_tile(int64_t M, int64_t N, const Fn& fn) {
+  static constexpr struct { int i, j; double round; } kTiles[] = {{8, 4, 1.}, {6, 4, 0.84}, {8, 3, 0.84}, {4, 4, 0.64}, {4, 3, 0.56}};
+  int best = 0;
+  double least = INFINITY;
+  for (int t = 0; t < 5; ++t) {
+    const int64_t tm = 32 * kTiles[t].i, tn = 64 * kTiles[t].j;
+    const double cost = kTiles[t].round * static_cast<double>(((M + tm - 1) / tm * ((N + tn - 1) / tn) + 255) / 256);
+    if (cost < least) least = cost, best = t;
+  }
+  using std::integral_constant;
+  switch (best) {
+    case 0: return fn(integral_constant<int, 8>(), integral_constant<int, 4>());
+    case 1: return fn(integral_constant<int, 6>(), integral_constant<int, 4>());
+    case 2: return fn(integral_constant<int, 8>(), integral_constant<int, 3>());
+    case 3: return fn(integral_constant<int, 4>(), integral_constant<int, 4>());
+    default: return fn(integral_constant<int, 4>(), integral_constant<int, 3>());
+  }
 }
 
 int check_linear(const char* fn, const void* x, const void* w, const int64_t* targets, int64_t M, int64_t K, int64_t N, int64_t ldx, int64_t ldw, float temperature) {
@@ -363,7 +380,6 @@ int check_linear(const char* fn, const void* x, const void* w, const int64_t* ta
   if (!aligned16(x) || !aligned16(w) || reinterpret_cast<uintptr_t>(targets) % 8) return fail(PICO_ERR_ALIGN, "%s: x and w must be aligned to 16 bytes, targets to 8", fn);
   return PICO_OK;
 }
-int64_t groups_of(int64_t N) { return (N + kGroup - 1) / kGroup; }
 void fill(LargeParams& p, const void* x, const void* w, int64_t M, int64_t K, int64_t N, int64_t ldx, int64_t ldw) {
   p.a = static_cast<const __bf16*>(x);
   p.b = static_cast<const __bf16*>(w);
@@ -381,7 +397,7 @@ using namespace pico;
 
 extern "C" int64_t pico_linear_log_probs_workspace_bytes(int64_t rows, int64_t vocab) {
   if (rows < 0 || vocab < 0 || rows > 0x7fffffff || vocab > 0x7fffffff) return -1;
-  return (rows + 63) / 64 * 64 * groups_of(vocab) * 8 + rows * 4;
+  return (rows + 63) / 64 * 64 * groups_of(vocab, kLeastGroup) * 8 + rows * 4;
 }
 
 extern "C" int pico_linear_log_probs_fwd(const void* x, const void* w, const int64_t* targets, float* log_probs, float* max_sum, int64_t rows, int64_t hidden,
@@ -400,15 +416,20 @@ extern "C" int pico_linear_log_probs_fwd(const void* x, const void* w, const int
   fill(p, x, w, rows, hidden, vocab, ldx, ldw);
   p.targets = targets;
   p.partial = static_cast<f32x2*>(workspace);
-  p.groups = static_cast<int>(groups_of(vocab));
-  p.target_logit = reinterpret_cast<float*>(p.partial + (rows + 63) / 64 * 64 * p.groups);
+  p.target_logit = reinterpret_cast<float*>(p.partial + (rows + 63) / 64 * 64 * groups_of(vocab, kLeastGroup));
   p.k = static_cast<float>(1.4426950408889634 / temperature);
   if (rows <= kFewRows) {
+    p.groups = groups_of(vocab, kFewGroup);
     const dim3 grid(static_cast<unsigned>(p.groups)), threads(256);
     if (rows <= 16) hipLaunchKernelGGL(score_few_kernel<1>, grid, threads, 0, s, p);
     else hipLaunchKernelGGL(score_few_kernel<2>, grid, threads, 0, s, p);
-  } else if (int rc = launch_best<ScoreTile>(p, fn, s)) {
-    return rc;
+  } else {
+    const int rc = with_tile(rows, vocab, [&](auto i, auto j) {
+      constexpr int I = decltype(i)::value, J = decltype(j)::value;
+      p.groups = groups_of(vocab, 16 * J);
+      return launch<I, J, ScoreTile>(p, fn, s);
+    });
+    if (rc) return rc;
   }
   hipLaunchKernelGGL(join_kernel, dim3(static_cast<unsigned>((rows + kJoinRows - 1) / kJoinRows)), dim3(kJoinRows * kSlices), 0, s, p.partial, p.target_logit, targets,
                      log_probs, reinterpret_cast<f32x2*>(max_sum), p.M, p.groups, p.N, p.k, 1.f / temperature, ignore_index);
@@ -436,5 +457,5 @@ extern "C" int pico_linear_log_probs_dlogits(const void* x, const void* w, const
   p.c = dlogits;
   p.ldc = static_cast<int>(ldd);
   p.grad_rows = of;
-  return launch_best<GradTile>(p, fn, s);
+  return with_tile(rows, vocab, [&](auto i, auto j) { return launch<decltype(i)::value, decltype(j)::value, GradTile>(p, fn, s); });
 }

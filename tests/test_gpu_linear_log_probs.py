@@ -92,6 +92,17 @@ def test_many_rounds_of_tiles(device):
         check(x, w, t)
 
 
+@pytest.mark.parametrize("rows,vocab", [(1001, 16010), (190, 65001), (255, 49001), (510, 24501), (127, 65001), (130, 32003), (127, 48003)])
+def test_every_shape_of_tile(device, rows, vocab):
+    """Sizes that take 256 x 256, 192 x 256, 256 x 192, 128 x 256 and 128 x 192, whose waves have
+    48 columns: targets at the ends of both widths, in the first and the last tile."""
+    x, w, t = inputs(rows + vocab, rows, 96, vocab, kept=0.9)
+    at = [k * n + d for n in (48, 64, 192, 256) for k in (0, 1, 2, 3, 4, (vocab - 1) // n) for d in (-1, 0, 1)] + [vocab - 1, vocab // 2]
+    at = torch.tensor(sorted({c for c in at if 0 <= c < vocab}), device="cuda")
+    t[::2] = at[torch.arange(t[::2].numel(), device="cuda") % at.numel()]
+    check(x, w, t)
+
+
 def test_strides(device):
     """Hidden states and weights with a row pitch, halves of wider buffers, rows that are no multiple of 16 bytes (copied), more axes, slices of tokens."""
     g = gen(1)
