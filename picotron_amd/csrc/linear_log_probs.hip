@@ -228,8 +228,12 @@ __global__ __launch_bounds__(kJoinRows * kSlices) void join_kernel(const f32x2* 
                                                                    const int64_t* __restrict__ targets, float* __restrict__ log_probs,
                                                                    f32x2* __restrict__ max_sum, int M, int groups, int vocab, float k, float inv_t,
                                                                    int64_t ignore_index) {
-  __shared__ f32x2 share[kSlices * kJoinRows / kWave][kJoinRows];
+  constexpr int kWaves = kSlices * kJoinRows / kWave, kOf = kWave / kJoinRows;   // a wave has kOf slices of kJoinRows rows
+  __shared__ f32x2 share[kWaves][kJoinRows];
   const int r = threadIdx.x % kJoinRows, slice = threadIdx.x / kJoinRows, row = blockIdx.x * kJoinRows + r;
+  const bool writes = slice == 0 && row < M;
+  const int64_t t = writes ? targets[row] : 0;
+  const float z = writes ? target_logit[row] : 0.f;
   Gather<false> g;
   if (row < M) {
     constexpr int U = 6;   // partial results requested together
@@ -241,23 +245,30 @@ __global__ __launch_bounds__(kJoinRows * kSlices) void join_kernel(const f32x2* 
         const int at = first + u * kSlices;
         v[u] = at < groups ? of[at * 64] : f32x2{-INFINITY, 0.f};
       }
-#pragma unroll
-      for (int u = 0; u < U; ++u) g.meet(v[u][0], v[u][1], k);
+      g.meet(v, k);
     }
   }
-  // a wave has four slices of 16 rows, and 16 waves meet in LDS
+  // a row's slices meet over lanes, waves (in LDS) and lanes
+  auto over_lanes = [&] {
 #pragma unroll
-  for (int off = 16; off < kWave; off *= 2) {
-    const float other_max = __shfl_xor(g.zmax, off, kWave), other_s = __shfl_xor(g.s, off, kWave);
-    g.meet(other_max, other_s, k);
-  }
+    for (int off = kJoinRows; off < kWave; off *= 2) {
+      const f32x2 other[1] = {{__shfl_xor(g.zmax, off, kWave), __shfl_xor(g.s, off, kWave)}};
+      g.meet(other, k);
+    }
+  };
+  over_lanes();
   if (threadIdx.x % kWave < kJoinRows) share[threadIdx.x / kWave][r] = f32x2{g.zmax, g.s};
   __syncthreads();
-  if (slice == 0 && row < M) {
-    for (int i = 1; i < kSlices * kJoinRows / kWave; ++i) g.meet(share[i][r][0], share[i][r][1], k);
-    const int64_t t = targets[row];
+  if (threadIdx.x >= kWave) return;
+  f32x2 waves[kWaves / kOf];
+#pragma unroll
+  for (int i = 0; i < kWaves / kOf; ++i) waves[i] = share[slice * (kWaves / kOf) + i][r];
+  g = {};
+  g.meet(waves, k);
+  over_lanes();
+  if (writes) {
     const bool counts = t != ignore_index && t >= 0 && t < vocab;
-    log_probs[row] = counts ? (target_logit[row] - g.zmax) * inv_t - logf(g.s) : 0.f;
+    log_probs[row] = counts ? (z - g.zmax) * inv_t - logf(g.s) : 0.f;
     if (max_sum != nullptr) max_sum[row] = f32x2{g.m, g.s};
   }
 }

@@ -68,10 +68,14 @@ struct Gather {
     zmax = to;
     m = to == -INFINITY ? 0.f : to;
   }
-  __device__ __forceinline__ void meet(float other_max, float other_s, float k) {   // what was gathered elsewhere (no entropy)
-    const float top = fmaxf(zmax, other_max), shift = other_max == -INFINITY ? 0.f : fmaxf((other_max - top) * k, kFloor);
+  template <int N>
+  __device__ __forceinline__ void meet(const f32x2 (&others)[N], float k) {   // (max, sum) gathered elsewhere (no entropy)
+    float top = zmax;
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = fmaxf(top, others[i][0]);
     rise(top, k);
-    s += other_s * fast_exp2(shift);
+#pragma unroll
+    for (int i = 0; i < N; ++i) s += others[i][1] * fast_exp2(others[i][0] == -INFINITY ? 0.f : fmaxf((others[i][0] - top) * k, kFloor));
   }
   template <int N>
   __device__ __forceinline__ void add(const float (&e)[N], float k) {
