@@ -222,7 +222,8 @@ __global__ __launch_bounds__(256, 3) void score_few_kernel(const ScoreParams p) 
 }
 constexpr int kFewRows = 32;
 
-// A workgroup joins the partial results of kJoinRows rows: a row's groups are dealt to kSlices threads.
+// A workgroup joins the partial results of kJoinRows rows: a row's groups are dealt to kSlices threads.  3.3 us at 24 rows of 49152 (one partial result after the
+// other: 4.8), 7 at 4096; 8 rows of 128 slices take 0.4 us less at up to 32 rows, 3 more from 3000 on.
 constexpr int kJoinRows = 16, kSlices = 64;
 __global__ __launch_bounds__(kJoinRows * kSlices) void join_kernel(const f32x2* __restrict__ partial, const float* __restrict__ target_logit,
                                                                    const int64_t* __restrict__ targets, float* __restrict__ log_probs,
