@@ -47,6 +47,15 @@ int dtype_code(const Tensor& t, const char* what) {
 }
 
 void* stream_now() { return c10::hip::getCurrentHIPStream().stream(); }
+// which graph capture the current stream is in (0: none)
+int64_t capture_now() {
+  const hipStream_t s = c10::hip::getCurrentHIPStream().stream();
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (s == nullptr) return 0;   // (the legacy stream cannot be captured, and may not be asked while another one is)
+  TORCH_CHECK(hipStreamGetCaptureInfo(s, &status, &id) == hipSuccess, "hipStreamGetCaptureInfo");
+  return status == hipStreamCaptureStatusActive ? static_cast<int64_t>(id) : 0;
+}
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 void* ptr(const OptTensor& t) { return t ? ptr(*t) : nullptr; }
 float* fptr(const Tensor& t) { return static_cast<float*>(ptr(t)); }
@@ -1502,6 +1511,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     ctx->save_for_backward({logits, targets, k.rows});
     // (not among the saved variables: it is handed over as the gradient, whose owner may change it in place between two backward passes)
     ctx->saved_data["unit"] = k.unit;
+    ctx->saved_data["capture"] = capture_now();
     ctx->saved_data["ignore"] = ignore_index;
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["entropy"] = static_cast<float>(entropy_coef) != 0;
@@ -1517,9 +1527,10 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     const c10::OptionalDeviceGuard device(s[0].device());
     const TokenRows r = token_rows("policy_loss", s[0], s[1]);
     const Tensor up = g[0].to(at::kFloat).contiguous();
-    // a second backward through this node (retain_graph) gets a buffer of its own
+    // a second backward through this node (retain_graph) gets a buffer of its own, and so does one that is captured without its forward: its replays would find
+    // there what the one before left
     Tensor unit;
-    if (const auto it = ctx->saved_data.find("unit"); it != ctx->saved_data.end()) {
+    if (const auto it = ctx->saved_data.find("unit"); it != ctx->saved_data.end() && ctx->saved_data["capture"].toInt() == capture_now()) {
       unit = it->second.toTensor();
       ctx->saved_data.erase(it);
     }

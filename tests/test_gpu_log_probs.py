@@ -607,6 +607,32 @@ def test_recorded_into_graphs(device):
                 assert torch.equal(a, b), (i, k, j)
 
 
+def test_a_backward_recorded_without_its_forward(device):
+    """Its replays start from the logits, whatever the upstream gradient of the one before was and whatever became of the result."""
+    from picotron_amd.functional import policy_loss
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        x = torch.randn(3, 20, 1001, generator=gen(1), device="cuda").to(BF16).requires_grad_()
+        t = torch.randint(0, 1001, (3, 20), generator=gen(2), device="cuda")
+        A, up = torch.randn(3, 1, generator=gen(3), device="cuda"), torch.ones((), device="cuda")
+        other = policy_loss(x, t, A)[0]
+        torch.autograd.grad(other, x, retain_graph=True)
+        want = {v: torch.autograd.grad(other, x, torch.full_like(other, v), retain_graph=True)[0] for v in (2.0, 1.0, 0.5)}
+        loss = policy_loss(x, t, A)[0]
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        (d,) = torch.autograd.grad(loss, x, up)
+    for v in (2.0, 1.0, 0.5, 1.0):
+        up.fill_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(d, want[v]), v
+        d.mul_(3)
+        torch.cuda.synchronize()
+
+
 def test_a_model_learns_from_them_like_from_the_definitions(device):
     """Gradients of a small Llama's parameters through each loss, against the same losses in torch on the same logits' graph."""
     import picotron_amd.process_group_manager as pgm
