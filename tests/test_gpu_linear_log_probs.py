@@ -267,3 +267,7 @@ def test_a_model_scores_its_tokens(device):
     with_bias = type(model.final_proj)(128, 1000, bias=True).to("cuda", BF16)
     h = model.hidden_states(ids[:, :-1])
     assert torch.equal(with_bias.log_probs(h, t), log_probs(with_bias(h), t))
+    for hidden in (64, 100):      # what the kernels for hidden states do not take
+        small = type(model.final_proj)(hidden, 1000, bias=False).to("cuda", BF16)
+        h = torch.randn(4, 64, hidden, generator=gen(3), device="cuda").to(BF16)
+        assert torch.equal(small.log_probs(h, t), log_probs(small(h), t))
