@@ -503,9 +503,10 @@ int pico_preference_loss_fwd(const pico_logits* logits, const pico_tokens* targe
  * (pitch ldw), the vocabulary projection, without its logits in memory; log_probs [rows] fp32 = z_target - logsumexp(z) of the products' fp32
  * sums (0 where the target does not count, as above).  max_sum: [rows, 2] fp32, what the gradient needs; may be NULL.  hidden must be a multiple of 8
  * over 64, the pitches multiples of 8, x and w aligned to 16 bytes; targets: [rows] contiguous.
- * workspace: pico_linear_log_probs_workspace_bytes(rows, vocab) bytes (a twelfth of bf16 logits; -1: too large).
+ * workspace: pico_linear_log_probs_workspace_bytes(rows, hidden, vocab) bytes, 16-byte aligned (a twelfth of bf16 logits and as much as x; -1: too large).
+ * Rows that do not count are left out of the product where that saves rounds of its tiles and x has no gaps between its rows.
  */
-int64_t pico_linear_log_probs_workspace_bytes(int64_t rows, int64_t vocab);
+int64_t pico_linear_log_probs_workspace_bytes(int64_t rows, int64_t hidden, int64_t vocab);
 int pico_linear_log_probs_fwd(const void* x, const void* w, const int64_t* targets, float* log_probs, float* max_sum, int64_t rows,
                               int64_t hidden, int64_t vocab, int64_t ldx, int64_t ldw, float temperature, int64_t ignore_index,
                               void* workspace, int64_t workspace_bytes, void* stream);

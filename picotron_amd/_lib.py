@@ -107,7 +107,7 @@ SIGNATURES = {
     "pico_log_probs_bwd": (c_int, _ROWS + [_P, _P, POINTER(PerRow), POINTER(PerRow), _P, c_int, _P, _I64, _I64, c_float, _I64, _P]),
     "pico_policy_loss_fwd": (c_int, _ROWS + [POINTER(Policy), _P, _P, _P, _P, POINTER(PolicySaved), _P, _I64, _I64, c_float, _I64, _P]),
     "pico_preference_loss_fwd": (c_int, _ROWS + [_P, c_float, c_float, c_int, c_float, _P, _P, _P, _P, _P, _P, _I64, _P]),
-    "pico_linear_log_probs_workspace_bytes": (_I64, [_I64, _I64]),
+    "pico_linear_log_probs_workspace_bytes": (_I64, [_I64] * 3),
     "pico_linear_log_probs_fwd": (c_int, [_P] * 5 + [_I64] * 5 + [c_float, _I64, _P, _I64, _P]),
     "pico_linear_log_probs_dlogits": (c_int, [_P] * 6 + [_I64] * 6 + [c_float, _I64, _P, _I64, _P]),
     "pico_adamw": (c_int, [_P, _P, _P, c_int, _P, _P, _I64] + [ctypes.c_float] * 5 + [_I64, ctypes.c_float, _P]),

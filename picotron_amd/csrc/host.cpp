@@ -1629,7 +1629,7 @@ struct LinearLogProbs : torch::autograd::Function<LinearLogProbs> {
     const Tensor a = rows(x), b = rows(w), t = targets.contiguous();
     Tensor lp = per_token(targets, x);
     if (max_sum) *max_sum = per_token(targets, x, 2);
-    const int64_t bytes = pico_linear_log_probs_workspace_bytes(a.size(0), b.size(0));
+    const int64_t bytes = pico_linear_log_probs_workspace_bytes(a.size(0), a.size(1), b.size(0));
     const Tensor ws = at::empty({std::max<int64_t>(bytes, 8)}, x.options().dtype(at::kByte));
     check(pico_linear_log_probs_fwd(ptr(a), ptr(b), t.data_ptr<int64_t>(), fptr(lp), max_sum ? fptr(*max_sum) : nullptr, a.size(0), a.size(1), b.size(0), pitch(a),
                                     pitch(b), static_cast<float>(temperature), ignore_index, ptr(ws), bytes, stream_now()));

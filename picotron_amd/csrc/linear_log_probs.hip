@@ -1,11 +1,12 @@
 // Log-probabilities of given tokens straight from hidden states x [M, K] and the vocabulary projection w [N, K]: the logits
 // z = x w^T / T are a matrix product whose tiles never leave the CU.
-//   forward : the product's epilogue reduces a tile to (max, sum of 2^D) per row and 48 or 64 columns (16 bytes of partial
+//   forward : where it saves rounds of tiles the rows that count are put together first; the product's epilogue reduces a tile to (max, sum of 2^D) per row and 48 or 64 columns (16 bytes of partial
 //             results, there and back, for what would be 256 of bf16 logits), and picks the target's logit where its column passes; a second launch
 //             joins a row's partial results.
 //   backward: the product again (the logits were not kept), whose epilogue turns z into d(logits) = g ([j = t] - p_j) / T with the row's
 //             maximum and sum from the forward, bf16; the gradients of x and w are two more products.
 // The logits are the products' fp32 sums here, never rounded to bf16.
+#include <type_traits>
 #include "log_probs.h"
 #include "product_large.h"
 
@@ -23,6 +24,8 @@ struct ScoreParams : LargeParams {
   float* target_logit;      // [M]
   int groups;
   float k;
+  const int* count;       // rows that count, or NULL: all are taken as they lie
+  const __bf16* packed;   // these rows put together, where some do not count
 };
 // the same value, of which the compiler does not know that it is (or it would keep what follows from it for all rows in registers)
 __device__ __forceinline__ int hidden(int v) {
@@ -92,6 +95,13 @@ __device__ __forceinline__ void request4_to(uint32_t lds_off, u32x4 window, uint
 // columns meet over four lanes.  128 exponentials a lane at a quarter of the vector rate are most of it.
 struct ScoreTile {
   using Params = ScoreParams;
+  static constexpr bool kCounted = true;
+  static __device__ __forceinline__ void count(Params& p) {
+    if (p.count == nullptr) return;
+    const int n = *p.count;
+    if (n < p.M) p.a = p.packed;
+    p.M = n;
+  }
   template <int I, int J> static constexpr int kStores = (I + 3) / 4;
   template <int I> static constexpr int kBegun = I / 2;   // 256 bytes each: 32 rows
   // the targets of the wave's rows, 8 bytes each, go to its rows region and are there long before the tile's end
@@ -222,29 +232,103 @@ __global__ __launch_bounds__(256, 3) void score_few_kernel(const ScoreParams p) 
 }
 constexpr int kFewRows = 32;
 
+// ---- the rows that count, put together.  A prompt's and a padding's rows need no product; how many there are is known on the device only, so the product's
+// workgroups look at the count and those past its tiles end.  position[row]: where a row went, -1 where it does not count.  Where all count x stays where it is.
+// Every workgroup counts the rows in front of its own for itself (32 KB of targets for 4096 rows, from the caches): one launch, 3 - 4 us where all count.  Whole calls, us, all
+// rows taken as they lie and put together, with all, 90 % and half of them counting: [4096 x 2048] against 49152 609, 611, 599, 324; [2000 x 4096] against 32000 391,
+// 394, 394, 212; [3000 x 576] against 49152 155, 157, 154, 91.  In one or two rounds of tiles too few are saved: [1000 x 4096] against 32000 205, 208, 214, 161, [512 x 2048]
+// against 49152 99, 102, 108, 103.
+constexpr int kPackThreads = 1024;
+int pack_rows_of(int64_t M) { return static_cast<int>(std::max<int64_t>(16, (M + 255) / 256)); }   // a workgroup's (all workgroups' counting grows with M only)
+__global__ __launch_bounds__(kPackThreads) void pack_rows_kernel(const __bf16* __restrict__ x, const int64_t* __restrict__ targets, int* __restrict__ position,
+                                                                 int* __restrict__ count, int64_t* __restrict__ packed_targets, __bf16* __restrict__ packed, int M,
+                                                                 int K, int vocab, int per, int64_t ignore_index) {
+  constexpr int W = kPackThreads / kWave;
+  __shared__ int all_of[W], before_of[W], to[kWave];
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, row0 = blockIdx.x * per;
+  auto counts = [&](int64_t t) { return t != ignore_index && t >= 0 && t < vocab; };
+  int all = 0, before = 0;
+  constexpr int U = 4;   // targets requested together
+  for (int first = threadIdx.x; first < M; first += U * kPackThreads) {
+    int64_t t[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) t[u] = first < M - u * kPackThreads ? targets[first + u * kPackThreads] : ignore_index;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = counts(t[u]);
+      all += in;
+      before += in && first + u * kPackThreads < row0;
+    }
+  }
+#pragma unroll
+  for (int off = kWave / 2; off > 0; off /= 2) {
+    all += __shfl_xor(all, off, kWave);
+    before += __shfl_xor(before, off, kWave);
+  }
+  if (lane == 0) { all_of[wave] = all; before_of[wave] = before; }
+  __syncthreads();
+  all = before = 0;
+#pragma unroll
+  for (int i = 0; i < W; ++i) { all += all_of[i]; before += before_of[i]; }
+  if (blockIdx.x == 0 && threadIdx.x == 0) *count = all;
+  const int last = min(row0 + per, M);
+  for (int first = row0; first < last; first += kWave) {   // 64 rows at a time
+    if (wave == 0) {
+      const int row = first + lane;
+      const int64_t t = row < last ? targets[row] : ignore_index;
+      const bool in = counts(t);
+      const auto which = __ballot(in);
+      const int at = in ? before + __popcll(which & ((1ull << lane) - 1)) : -1;
+      before += __popcll(which);
+      to[lane] = at;
+      if (row < last) position[row] = at;
+      if (in) packed_targets[at] = t;
+    }
+    __syncthreads();
+    if (all != M)
+      for (int r = wave; r < kWave; r += W) {
+        if (to[r] < 0) continue;
+        const u32x4* from = reinterpret_cast<const u32x4*>(x + static_cast<int64_t>(first + r) * K);
+        u32x4* there = reinterpret_cast<u32x4*>(packed + static_cast<int64_t>(to[r]) * K);
+        constexpr int P = 4;   // pieces requested together
+        for (int piece = lane; piece < K / 8; piece += P * kWave) {
+          u32x4 v[P];
+#pragma unroll
+          for (int i = 0; i < P; ++i)
+            if (piece + i * kWave < K / 8) v[i] = from[piece + i * kWave];
+#pragma unroll
+          for (int i = 0; i < P; ++i)
+            if (piece + i * kWave < K / 8) there[piece + i * kWave] = v[i];
+        }
+      }
+    __syncthreads();
+  }
+}
+
 // A workgroup joins the partial results of kJoinRows rows: a row's groups are dealt to kSlices threads.  3.3 us at 24 rows of 49152 (one partial result after the
 // other: 4.8), 7 at 4096; 8 rows of 128 slices take 0.4 us less at up to 32 rows, 3 more from 3000 on.
 constexpr int kJoinRows = 16, kSlices = 64;
 __global__ __launch_bounds__(kJoinRows * kSlices) void join_kernel(const f32x2* __restrict__ partial, const float* __restrict__ target_logit,
                                                                    const int64_t* __restrict__ targets, float* __restrict__ log_probs,
-                                                                   f32x2* __restrict__ max_sum, int M, int groups, int vocab, float k, float inv_t,
+                                                                   f32x2* __restrict__ max_sum, const int* __restrict__ position, int M, int groups, int vocab, float k, float inv_t,
                                                                    int64_t ignore_index) {
   constexpr int kWaves = kSlices * kJoinRows / kWave, kOf = kWave / kJoinRows;   // a wave has kOf slices of kJoinRows rows
   __shared__ f32x2 share[kWaves][kJoinRows];
   const int r = threadIdx.x % kJoinRows, slice = threadIdx.x / kJoinRows, row = blockIdx.x * kJoinRows + r;
   const bool writes = slice == 0 && row < M;
+  const int at = row >= M ? -1 : position != nullptr ? position[row] : row;   // (-1: it does not count and was left out)
   const int64_t t = writes ? targets[row] : 0;
-  const float z = writes ? target_logit[row] : 0.f;
+  const float z = writes && at >= 0 ? target_logit[at] : 0.f;
   Gather<false> g;
-  if (row < M) {
+  if (at >= 0) {
     constexpr int U = 6;   // partial results requested together
-    const f32x2* of = partial + static_cast<int64_t>(row / 64) * groups * 64 + row % 64;
+    const f32x2* of = partial + static_cast<int64_t>(at / 64) * groups * 64 + at % 64;
     for (int first = slice; first < groups; first += U * kSlices) {
       f32x2 v[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int at = first + u * kSlices;
-        v[u] = at < groups ? of[at * 64] : f32x2{-INFINITY, 0.f};
+        const int group = first + u * kSlices;
+        v[u] = group < groups ? of[group * 64] : f32x2{-INFINITY, 0.f};
       }
       g.meet(v, k);
     }
@@ -270,7 +354,7 @@ __global__ __launch_bounds__(kJoinRows * kSlices) void join_kernel(const f32x2* 
   if (writes) {
     const bool counts = t != ignore_index && t >= 0 && t < vocab;
     log_probs[row] = counts ? (z - g.zmax) * inv_t - logf(g.s) : 0.f;
-    if (max_sum != nullptr) max_sum[row] = f32x2{g.m, g.s};
+    if (max_sum != nullptr) max_sum[row] = at >= 0 ? f32x2{g.m, g.s} : f32x2{0.f, 1.f};
   }
 }
 
@@ -298,6 +382,7 @@ struct GradParams : LargeParams {
 };
 struct GradTile {
   using Params = GradParams;
+  static constexpr bool kCounted = false;
   template <int I, int J> static constexpr int kStores = I * ((J + 3) / 4) * 2;
   template <int I> static constexpr int kBegun = (I + 3) / 4;   // 1 KiB each: 64 rows
   template <int I>
@@ -382,6 +467,30 @@ int with_tile(int64_t M, int64_t N, const Fn& fn) {
   }
 }
 
+// what the forward keeps beside its results
+struct Workspace {
+  __bf16* packed;        // [rows, hidden]
+  f32x2* partial;        // [rows / 64][groups][64]
+  int64_t* targets;      // [rows], of the packed ones
+  float* target_logit;   // [rows]
+  int *position, *count; // [rows], [1]
+  int64_t bytes;
+  Workspace(void* at, int64_t rows, int64_t hidden, int64_t vocab) {
+    char* next = static_cast<char*>(at);
+    auto take = [&](auto*& part, int64_t n) {
+      part = reinterpret_cast<std::remove_reference_t<decltype(part)>>(next);
+      next += (n * static_cast<int64_t>(sizeof(*part)) + 15) / 16 * 16;
+    };
+    take(packed, rows > kFewRows ? rows * hidden : 0);
+    take(partial, (rows + 63) / 64 * 64 * groups_of(vocab, kLeastGroup));
+    take(targets, rows);
+    take(target_logit, rows);
+    take(position, rows);
+    take(count, 1);
+    bytes = next - static_cast<char*>(at);
+  }
+};
+
 int check_linear(const char* fn, const void* x, const void* w, const int64_t* targets, int64_t M, int64_t K, int64_t N, int64_t ldx, int64_t ldw, float temperature) {
   if (M < 0 || N <= 0 || K % 8 != 0 || (M > 0 && !pico_product_large_takes(M, (N + 7) / 8 * 8, K, ldx, ldw, 0, 0, 1)))
     return fail(PICO_ERR_SHAPE, "%s: rows=%lld hidden=%lld vocab=%lld row pitches %lld, %lld (hidden a multiple of 8 over 64, pitches multiples of 8, a tile's rows span less than 2 GiB)",
@@ -407,9 +516,9 @@ void fill(LargeParams& p, const void* x, const void* w, int64_t M, int64_t K, in
 
 using namespace pico;
 
-extern "C" int64_t pico_linear_log_probs_workspace_bytes(int64_t rows, int64_t vocab) {
-  if (rows < 0 || vocab < 0 || rows > 0x7fffffff || vocab > 0x7fffffff) return -1;
-  return (rows + 63) / 64 * 64 * groups_of(vocab, kLeastGroup) * 8 + rows * 4;
+extern "C" int64_t pico_linear_log_probs_workspace_bytes(int64_t rows, int64_t hidden, int64_t vocab) {
+  if (rows < 0 || hidden < 0 || vocab < 0 || rows > 0x7fffffff || hidden > 0x7fffffff || vocab > 0x7fffffff) return -1;
+  return Workspace(nullptr, rows, hidden, vocab).bytes;
 }
 
 extern "C" int pico_linear_log_probs_fwd(const void* x, const void* w, const int64_t* targets, float* log_probs, float* max_sum, int64_t rows, int64_t hidden,
@@ -419,16 +528,16 @@ extern "C" int pico_linear_log_probs_fwd(const void* x, const void* w, const int
   if (int rc = check_linear(fn, x, w, targets, rows, hidden, vocab, ldx, ldw, temperature)) return rc;
   if (rows == 0) return PICO_OK;
   if (!log_probs || !workspace) return fail(PICO_ERR_NULL, "%s: log_probs and workspace are required", fn);
-  if (reinterpret_cast<uintptr_t>(workspace) % 8 || reinterpret_cast<uintptr_t>(max_sum) % 8) return fail(PICO_ERR_ALIGN, "%s: workspace and max_sum must be aligned to 8 bytes", fn);
-  if (workspace_bytes < pico_linear_log_probs_workspace_bytes(rows, vocab))
-    return fail(PICO_ERR_WORKSPACE, "%s: workspace of %lld bytes, needs %lld", fn, static_cast<long long>(workspace_bytes),
-                static_cast<long long>(pico_linear_log_probs_workspace_bytes(rows, vocab)));
+  if (!aligned16(workspace) || reinterpret_cast<uintptr_t>(max_sum) % 8) return fail(PICO_ERR_ALIGN, "%s: workspace must be aligned to 16 bytes, max_sum to 8", fn);
+  const Workspace of(workspace, rows, hidden, vocab);
+  if (workspace_bytes < of.bytes)
+    return fail(PICO_ERR_WORKSPACE, "%s: workspace of %lld bytes, needs %lld", fn, static_cast<long long>(workspace_bytes), static_cast<long long>(of.bytes));
   hipStream_t s = static_cast<hipStream_t>(stream);
   ScoreParams p = {};
   fill(p, x, w, rows, hidden, vocab, ldx, ldw);
   p.targets = targets;
-  p.partial = static_cast<f32x2*>(workspace);
-  p.target_logit = reinterpret_cast<float*>(p.partial + (rows + 63) / 64 * 64 * groups_of(vocab, kLeastGroup));
+  p.partial = of.partial;
+  p.target_logit = of.target_logit;
   p.k = static_cast<float>(1.4426950408889634 / temperature);
   if (rows <= kFewRows) {
     p.groups = groups_of(vocab, kFewGroup);
@@ -439,12 +548,21 @@ extern "C" int pico_linear_log_probs_fwd(const void* x, const void* w, const int
     const int rc = with_tile(rows, vocab, [&](auto i, auto j) {
       constexpr int I = decltype(i)::value, J = decltype(j)::value;
       p.groups = groups_of(vocab, 16 * J);
+      // (rows with gaps between them are left to the product.  hidden x vocab: a row's product takes 40 times as long as its part of the packing, or longer)
+      if (vocab * hidden >= (1 << 23) && (rows + 32 * I - 1) / (32 * I) * ((vocab + 64 * J - 1) / (64 * J)) > 2 * 256 && ldx == hidden) {
+        const int per = pack_rows_of(rows);
+        hipLaunchKernelGGL(pack_rows_kernel, dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(kPackThreads), 0, s, p.a, targets, of.position, of.count,
+                           of.targets, of.packed, p.M, p.K, p.N, per, ignore_index);
+        p.count = of.count;
+        p.packed = of.packed;
+        p.targets = of.targets;
+      }
       return launch<I, J, ScoreTile>(p, fn, s);
     });
     if (rc) return rc;
   }
   hipLaunchKernelGGL(join_kernel, dim3(static_cast<unsigned>((rows + kJoinRows - 1) / kJoinRows)), dim3(kJoinRows * kSlices), 0, s, p.partial, p.target_logit, targets,
-                     log_probs, reinterpret_cast<f32x2*>(max_sum), p.M, p.groups, p.N, p.k, 1.f / temperature, ignore_index);
+                     log_probs, reinterpret_cast<f32x2*>(max_sum), p.count ? of.position : nullptr, p.M, p.groups, p.N, p.k, 1.f / temperature, ignore_index);
   return check_launch(fn);
 }
 

@@ -119,6 +119,7 @@ struct StoreTile {
   using Params = LargeParams;
   template <int I, int J> static constexpr int kStores = I * (kParts ? (J + 1) / 2 : (J + 3) / 4) * 2;
   template <int I> static constexpr int kBegun = 0;
+  static constexpr bool kCounted = false;
   template <int I> static __device__ __forceinline__ void begin(const Params&, const Unit&, int, int, int, uint32_t) {}
   template <int I, int J>
   static __device__ __forceinline__ void tile(const Params& p, const Unit& u, int wm, int wn, int lane, unsigned char* rows, f32x4 (&acc)[I][J]) {
@@ -128,9 +129,9 @@ struct StoreTile {
 };
 
 // What becomes of a tile's sums is the epilogue's: Epilogue::Params (LargeParams and what it needs beside), begin(), called once the tile before
-// has left, with kBegun vector memory operations, and tile(), with kStores of them.
+// has left, with kBegun vector memory operations, and tile(), with kStores of them.  Where kCounted count(), first of all, may set another, smaller M and another a.
 template <bool kSlowA, bool kSlowB, int I, int J, typename Epilogue>
-__global__ __launch_bounds__(512, 2) void product_large_kernel(const typename Epilogue::Params p) {
+__global__ __launch_bounds__(512, 2) void product_large_kernel(const typename Epilogue::Params given) {
   using S = Shape<kSlowA, kSlowB, I, J>;
   using A = typename S::A;
   using B = typename S::B;
@@ -138,6 +139,13 @@ __global__ __launch_bounds__(512, 2) void product_large_kernel(const typename Ep
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int wm = wave / 4 * 16 * I, wn = wave % 4 * 16 * J;
+
+  typename Epilogue::Params p = given;
+  if constexpr (Epilogue::kCounted) {
+    Epilogue::count(p);
+    p.tiles_m = (p.M + TM - 1) / TM;
+    if (static_cast<int>(blockIdx.x) >= p.tiles_m * p.tiles_n) return;
+  }
 
   // ---- requests
   uint32_t oa[kPA], ob[kPB];
@@ -150,7 +158,7 @@ __global__ __launch_bounds__(512, 2) void product_large_kernel(const typename Ep
   const uint32_t step_a = static_cast<uint32_t>(kSlowA ? kStep * p.lda * 2 : kStep * 2), step_b = static_cast<uint32_t>(kSlowB ? kStep * p.ldb * 2 : kStep * 2);
   Unit load;   // where the requests stand
   int load_round = 0, load_step = 0;
-  unit_at<TM, TN>(p, 0, load);   // (the grid is no larger than the work)
+  unit_at<TM, TN>(p, 0, load);   // (the grid, or what is left of it, is no larger than the work)
   Window wa = open_window<kSlowA>(p.a, p.lda, load.m0, TM, p.M, load.first * kStep, p.K);
   Window wb = open_window<kSlowB>(p.b, p.ldb, load.n0, TN, p.N, load.first * kStep, p.K);
   u32x4 ra = resource(wa), rb = resource(wb);

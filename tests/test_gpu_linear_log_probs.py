@@ -145,6 +145,50 @@ def test_tokens_that_do_not_count(device):
     assert q.shape == (0, 7) and dx.shape == e.shape and dw.shape == w.shape and not dw.any()
 
 
+@pytest.mark.parametrize("rows,hidden,vocab", [(1100, 264, 33001), (4096, 704, 12001), (511, 264, 49001), (17001, 4096, 2051)])
+def test_rows_that_do_not_count_change_nothing(device, rows, hidden, vocab):
+    """Several rounds of tiles, where the rows that count are put together: the others hold NaN, and what counts gets the same bits whichever they are."""
+    from picotron_amd.functional import linear_log_probs
+    x, w, t = inputs(rows, rows, hidden, vocab, kept=1.0)
+    every = linear_log_probs(x, w, t)
+    check(x, w, t, grads=False)
+    kept = torch.rand(rows, generator=gen(8), device="cuda")
+    r = torch.arange(rows, device="cuda")
+    for i, counts in enumerate((kept < 0.3, kept < 0.9, r >= rows // 2, r < rows // 2, (r // 100) % 3 == 1, r == 0, r == rows - 1, r < 0, r != 77, r > -1)):
+        u = torch.where(counts, t, torch.where(r % 3 == 0, IGNORE, torch.where(r % 3 == 1, vocab, -1 - r)))
+        y = torch.where(counts[:, None], x, float("nan"))
+        assert torch.equal(linear_log_probs(y, w, u), torch.where(counts, every, 0.0)), i
+    u, x = torch.where(kept < 0.3, t, IGNORE), x.requires_grad_()
+    v = w.clone().requires_grad_()
+    a = torch.randn(rows, generator=gen(9), device="cuda")
+    dx, dw = torch.autograd.grad(linear_log_probs(x, v, u), (x, v), a)
+    ex, ew = torch.autograd.grad(linear_log_probs(x, v, t), (x, v), torch.where(kept < 0.3, a, 0.0))
+    assert torch.equal(dx, ex) and torch.equal(dw, ew) and not dx[kept >= 0.3].any()
+
+
+def test_a_recorded_call_takes_other_rows_on_every_replay(device):
+    from picotron_amd.functional import linear_log_probs
+    x, w, t = inputs(5, 1100, 264, 33001, kept=1.0)
+    kept = torch.rand(1100, generator=gen(6), device="cuda")
+    masked = [torch.where(kept < share, t, IGNORE) for share in (0.0, 0.5, 1.0, 0.2)]
+    want = [linear_log_probs(x, w, u) for u in masked]
+    still = t.clone()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        side.wait_stream(torch.cuda.default_stream())
+        linear_log_probs(x, w, still)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        q = linear_log_probs(x, w, still)
+    for i in (2, 0, 1, 3, 2, 1):
+        still.copy_(masked[i])
+        graph.replay()
+        linear_log_probs(x, w, masked[(i + 1) % 4])
+        torch.cuda.synchronize()
+        assert torch.equal(q, want[i]), i
+
+
 def test_large_and_certain_logits(device):
     """Logits of several hundred, one token nearly certain in every row."""
     x, w, t = inputs(3, 200, 256, 3001, kept=1.0, size=30.0)

@@ -98,8 +98,10 @@ def test_gradients_that_overlap_or_lie_otherwise(lib, dtype, size):
 
 def test_linear_log_probs(lib):
     """Sizes, pitches, alignments, pointers and workspaces."""
-    assert lib.pico_linear_log_probs_workspace_bytes(100, 129) == 128 * 3 * 8 + 100 * 4      # (three groups of 48 columns)
-    assert lib.pico_linear_log_probs_workspace_bytes(-1, 8) == -1 and lib.pico_linear_log_probs_workspace_bytes(1, 1 << 40) == -1
+    # x, partial results of three groups of 48 columns, three numbers a row and one more, each from a 16-byte boundary
+    assert lib.pico_linear_log_probs_workspace_bytes(100, 72, 129) == 100 * 72 * 2 + 128 * 3 * 8 + 100 * 8 + 100 * 4 + 100 * 4 + 16
+    for sizes in ((-1, 8, 8), (1, -8, 8), (1, 8, 1 << 40), (1 << 40, 8, 8)):
+        assert lib.pico_linear_log_probs_workspace_bytes(*sizes) == -1
 
     def fwd(x=4096, w=4096, t=4096, lp=4096, ms=4096, M=10, K=128, N=1000, ldx=128, ldw=128, T=1.0, ws=4096, bytes=1 << 20):
         P = ctypes.c_void_p
