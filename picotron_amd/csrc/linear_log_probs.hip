@@ -142,8 +142,9 @@ struct ScoreTile {
 
 // Few rows (16 RB at most): what bounds them is reading w once.  A workgroup has 64 entries of the vocabulary, and its four waves a quarter of the contraction
 // each, 128 bytes of a row at a time; operands come straight from memory in the layout of the products (x from the caches), a step's loads ahead of the step
-// before's products, and the waves' sums meet in LDS.  Whole calls, us, in the product's tiles and here: 1 x 2048 against 49152 59.7, 47.0 (4.3 TB/s), 16 rows 56.5,
-// 50.4, 32 rows 59.9, 54.8, 24 x 576 21.6, 17.9.  For 64 rows x is read as often as w: 58.9, 66.3; they stay with the product.
+// before's products, and the waves' sums meet in LDS.  Whole calls, us, in the product's tiles and here: 1 row of 2048 against 49152 52.5, 45.9 (4.4 TB/s), 16 rows 56.2,
+// 48.4, 32 rows 52.3, 53.0; 24 x 576 18.5, 17.1; 32 x 4096 against 32000 79.0, 68.2.  Of 18 sizes the product's tiles took 0.87 to 1.84 of the time at 32 rows and
+// 0.92 to 1.94 at 24; with 64 rows x would be read as often as w: they stay with the product.
 template <int RB>
 __global__ __launch_bounds__(256, 3) void score_few_kernel(const ScoreParams p) {
   __shared__ f32x4 sums[4][RB][kFewJ][kWave];
