@@ -1649,13 +1649,24 @@ struct LinearLogProbs : torch::autograd::Function<LinearLogProbs> {
     const Tensor &x = s[0], &w = s[1];
     const c10::OptionalDeviceGuard device(x.device());
     const Tensor a = rows(x), b = rows(w), t = s[2].contiguous(), dlp = g[0].to(at::kFloat).contiguous();
-    const int64_t M = a.size(0), N = b.size(0), ldd = (N + 7) / 8 * 8;
+    const int64_t M = a.size(0), K = a.size(1), N = b.size(0), ldd = (N + 7) / 8 * 8;
+    const auto temperature = static_cast<float>(ctx->saved_data["temperature"].toDouble());
+    const int64_t ignore = ctx->saved_data["ignore"].toInt();
+    variable_list r(5);
+    const bool both_wanted = ctx->needs_input_grad(0) && ctx->needs_input_grad(1);
+    if (const int64_t bytes = both_wanted && pitch(a) == K && pitch(b) == K ? pico_linear_log_probs_bwd_workspace_bytes(M, K, N) : 0) {
+      const Tensor dx = at::empty({M, K}, a.options()), dw = at::empty({N, K}, a.options()), ws = at::empty({bytes}, a.options().dtype(at::kByte));
+      check(pico_linear_log_probs_bwd(ptr(a), ptr(b), t.data_ptr<int64_t>(), fptr(s[3]), fptr(dlp), ptr(dx), ptr(dw), M, K, N, K, temperature, ignore, ptr(ws), bytes,
+                                      stream_now()));
+      r[0] = dx.view(x.sizes());
+      r[1] = dw;
+      return r;
+    }
     const Tensor dz = at::empty({M, ldd}, a.options()), ws = at::empty({std::max<int64_t>(M * 16, 16)}, a.options().dtype(at::kByte));
     check(pico_linear_log_probs_dlogits(ptr(a), ptr(b), t.data_ptr<int64_t>(), fptr(s[3]), fptr(dlp), ptr(dz), M, a.size(1), N, pitch(a), pitch(b), ldd,
-                                        static_cast<float>(ctx->saved_data["temperature"].toDouble()), ctx->saved_data["ignore"].toInt(), ptr(ws), M * 16, stream_now()));
+                                        temperature, ignore, ptr(ws), M * 16, stream_now()));
     const Tensor d = dz.narrow(1, 0, N);
-    variable_list r(5);
-    if (ctx->needs_input_grad(0) && ctx->needs_input_grad(1)) {
+    if (both_wanted) {
       Gradients both = gradients(d, b, a);
       r[0] = both.dx.view(x.sizes());
       r[1] = both.dw;

@@ -4,7 +4,7 @@
 //             results, there and back, for what would be 256 of bf16 logits), and picks the target's logit where its column passes; a second launch
 //             joins a row's partial results.
 //   backward: the product again (the logits were not kept), whose epilogue turns z into d(logits) = g ([j = t] - p_j) / T with the row's
-//             maximum and sum from the forward, bf16; the gradients of x and w are two more products.
+//             maximum and sum from the forward, bf16; the gradients of x and w are two more products, large ones over the rows that count only.
 // The logits are the products' fp32 sums here, never rounded to bf16.
 #include <type_traits>
 #include "log_probs.h"
@@ -96,11 +96,13 @@ __device__ __forceinline__ void request4_to(uint32_t lds_off, u32x4 window, uint
 struct ScoreTile {
   using Params = ScoreParams;
   static constexpr bool kCounted = true;
+  template <int TM>
   static __device__ __forceinline__ void count(Params& p) {
     if (p.count == nullptr) return;
     const int n = *p.count;
     if (n < p.M) p.a = p.packed;
     p.M = n;
+    p.tiles_m = (n + TM - 1) / TM;
   }
   template <int I, int J> static constexpr int kStores = (I + 3) / 4;
   template <int I> static constexpr int kBegun = I / 2;   // 256 bytes each: 32 rows
@@ -239,7 +241,7 @@ constexpr int kFewRows = 32;
 // rows taken as they lie and put together, with all, 90 % and half of them counting: [4096 x 2048] against 49152 609, 611, 599, 324; [2000 x 4096] against 32000 391,
 // 394, 394, 212; [3000 x 576] against 49152 155, 157, 154, 91.  In one or two rounds of tiles too few are saved: [1000 x 4096] against 32000 205, 208, 214, 161, [512 x 2048]
 // against 49152 99, 102, 108, 103.
-constexpr int kPackThreads = 1024;
+constexpr int kPackThreads = 1024, kLeastRows = 2 * kStep;
 int pack_rows_of(int64_t M) { return static_cast<int>(std::max<int64_t>(16, (M + 255) / 256)); }   // a workgroup's (all workgroups' counting grows with M only)
 __global__ __launch_bounds__(kPackThreads) void pack_rows_kernel(const __bf16* __restrict__ x, const int64_t* __restrict__ targets, int* __restrict__ position,
                                                                  int* __restrict__ count, int64_t* __restrict__ packed_targets, __bf16* __restrict__ packed, int M,
@@ -272,6 +274,9 @@ __global__ __launch_bounds__(kPackThreads) void pack_rows_kernel(const __bf16* _
 #pragma unroll
   for (int i = 0; i < W; ++i) { all += all_of[i]; before += before_of[i]; }
   if (blockIdx.x == 0 && threadIdx.x == 0) *count = all;
+  if (blockIdx.x == 0 && all < M)   // zeros up to the least contraction of the gradient of w
+    for (int r = all + wave; r < min(kLeastRows, M); r += W)
+      for (int piece = lane; piece < K / 8; piece += kWave) reinterpret_cast<u32x4*>(packed + static_cast<int64_t>(r) * K)[piece] = u32x4{0u, 0u, 0u, 0u};
   const int last = min(row0 + per, M);
   for (int first = row0; first < last; first += kWave) {   // 64 rows at a time
     if (wave == 0) {
@@ -367,23 +372,37 @@ struct GradRow {
   int target, counts;
 };
 __global__ void grad_rows_kernel(const f32x2* __restrict__ max_sum, const float* __restrict__ dlog_probs, const int64_t* __restrict__ targets,
-                                 GradRow* __restrict__ out, int M, int vocab, float k, float inv_t, int64_t ignore_index) {
+                                 GradRow* __restrict__ out, const int* __restrict__ position, const int* __restrict__ count, int M, int vocab, float k, float inv_t,
+                                 int64_t ignore_index) {
   const int row = blockIdx.x * blockDim.x + threadIdx.x;
   if (row >= M) return;
+  const int at = position != nullptr ? position[row] : row;
+  if (count != nullptr && row >= *count && row < kLeastRows) out[row] = {0.f, 0.f, -1, 0};   // (behind the rows that are put together)
+  if (at < 0) return;
   const int64_t t = targets[row];
   const bool counts = t != ignore_index && t >= 0 && t < vocab && dlog_probs[row] != 0.f;
   const f32x2 ms = max_sum[row];
-  out[row] = {fmaf(ms[0], k, log2f(ms[1])), counts ? dlog_probs[row] * inv_t : 0.f, counts ? static_cast<int>(t) : -1, counts};
+  out[at] = {fmaf(ms[0], k, log2f(ms[1])), counts ? dlog_probs[row] * inv_t : 0.f, counts ? static_cast<int>(t) : -1, counts};
 }
 
 struct GradParams : LargeParams {
   const GradRow* grad_rows;   // [M]
   int ldc;
   float k;
+  const int* count;           // (as in ScoreParams)
+  const __bf16* packed;
 };
 struct GradTile {
   using Params = GradParams;
-  static constexpr bool kCounted = false;
+  static constexpr bool kCounted = true;
+  template <int TM>
+  static __device__ __forceinline__ void count(Params& p) {
+    if (p.count == nullptr) return;
+    const int n = *p.count;
+    if (n < p.M) p.a = p.packed;
+    p.M = max(n, kLeastRows);
+    p.tiles_m = (p.M + TM - 1) / TM;
+  }
   template <int I, int J> static constexpr int kStores = I * ((J + 3) / 4) * 2;
   template <int I> static constexpr int kBegun = (I + 3) / 4;   // 1 KiB each: 64 rows
   template <int I>
@@ -425,18 +444,85 @@ struct GradTile {
   }
 };
 
-template <int I, int J, typename Epilogue>
+// ---- the two products with d(logits) of the rows that count, put together.  Both operands' rows that do not count are missing: the gradient of w is a shorter
+// contraction, that of x has fewer rows.  The latter's contraction (the vocabulary) is cut into parts such that its tiles fill the GPU, which depends on the
+// number of rows and is found where that is known; the parts' sums go to the rows' places in a launch of their own.  Forward and backward, us, with all rows in the
+// backward's products and with those that count, all, 90 %, 60 % and 30 % of them: [2000 x 4096] against 32000 1609, 1594, 1456, 1318 and 1607, 1552, 1106, 675; [2800 x
+// 576] against 49152 714, 703, 664, 613 and 704, 655, 490, 341; [512 x 4096] against 32000 485, 482, 482, 470 and 500, 485, 421, 363; [2048 x 1024] against 49152 705,
+// 700, 640, 596 and 725, 699, 521, 393.
+struct CountedParams : LargeParams {
+  const int* count;
+  const __bf16* packed;
+  int rows;   // all
+};
+constexpr int kMostParts = 32;
+constexpr int64_t kMostPartial = 1 << 25;   // fp32 sums in parts: two rounds of tiles
+__device__ __forceinline__ int parts_of(int tiles, int n, int hidden) {
+  int best = 1;
+  float least = static_cast<float>((tiles + 255) / 256);
+  for (int q = 2; q <= kMostParts && static_cast<int64_t>(q) * n * hidden <= kMostPartial; ++q) {
+    const float cost = static_cast<float>((tiles * q + 255) / 256) / static_cast<float>(q) + 0.02f * static_cast<float>(q - 1);   // (a part's sums written and read)
+    if (cost < least) least = cost, best = q;
+  }
+  return best;
+}
+struct InputGradTile : StoreTile<true> {   // a: d(logits), b: w; fp32 [parts, rows that count, hidden]
+  using Params = CountedParams;
+  static constexpr bool kCounted = true;
+  template <int TM>
+  static __device__ __forceinline__ void count(Params& p) {
+    p.M = *p.count;
+    p.tiles_m = (p.M + TM - 1) / TM;
+    p.parts = parts_of(p.tiles_m * p.tiles_n, p.M, p.N);
+  }
+};
+struct WeightGradTile : StoreTile<false> {   // a: d(logits), b: x
+  using Params = CountedParams;
+  static constexpr bool kCounted = true;
+  template <int TM>
+  static __device__ __forceinline__ void count(Params& p) {
+    const int n = *p.count;
+    if (n < p.rows) p.b = p.packed;
+    p.K = max(n, kLeastRows);
+  }
+};
+constexpr int kUnpackThreads = 256;
+__global__ __launch_bounds__(kUnpackThreads) void unpack_rows_kernel(const float* __restrict__ partial, const int* __restrict__ position, const int* __restrict__ count,
+                                                                     __bf16* __restrict__ dx, int rows, int K, int tile_rows, int tiles_n) {
+  const int pieces = K / 8, n = *count, parts = parts_of((n + tile_rows - 1) / tile_rows * tiles_n, n, K);
+  const int64_t all = static_cast<int64_t>(rows) * pieces, id = static_cast<int64_t>(blockIdx.x) * kUnpackThreads + threadIdx.x;
+  if (id >= all) return;
+  const int64_t row = id / pieces, at = position[row], piece = id - row * pieces;
+  f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+  if (at >= 0)
+    for (int q = 0; q < parts; ++q) {
+      const f32x4* from = reinterpret_cast<const f32x4*>(partial + ((static_cast<int64_t>(q) * n + at) * pieces + piece) * 8);
+      lo += from[0];
+      hi += from[1];
+    }
+  bf16x8 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    v[e] = static_cast<__bf16>(lo[e]);
+    v[4 + e] = static_cast<__bf16>(hi[e]);
+  }
+  reinterpret_cast<bf16x8*>(dx)[id] = v;
+}
+
+template <int I, int J, typename Epilogue, bool kSlowA = false, bool kSlowB = false>
 int launch(typename Epilogue::Params p, const char* fn, hipStream_t s) {
-  using S = Shape<false, false, I, J>;
+  using S = Shape<kSlowA, kSlowB, I, J>;
   static LdsOnce reserved;
-  if (!reserve_lds_once(reserved, reinterpret_cast<const void*>(&product_large_kernel<false, false, I, J, Epilogue>), S::kLds))
+  if (!reserve_lds_once(reserved, reinterpret_cast<const void*>(&product_large_kernel<kSlowA, kSlowB, I, J, Epilogue>), S::kLds))
     return fail(PICO_ERR_LAUNCH, "%s: cannot reserve %d bytes of LDS", fn, S::kLds);
   p.tiles_m = (p.M + S::TM - 1) / S::TM;
   p.tiles_n = (p.N + S::TN - 1) / S::TN;
   p.parts = 1;
   const int64_t units = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
   p.streaming = units > 256;   // (as pico_product_large)
-  hipLaunchKernelGGL((product_large_kernel<false, false, I, J, Epilogue>), dim3(static_cast<unsigned>(std::min<int64_t>(units, 256))), dim3(S::kThreads), S::kLds, s, p);
+  // (the input gradient's parts are not known here)
+  const unsigned grid = std::is_same_v<Epilogue, InputGradTile> ? 256u : static_cast<unsigned>(std::min<int64_t>(units, 256));
+  hipLaunchKernelGGL((product_large_kernel<kSlowA, kSlowB, I, J, Epilogue>), dim3(grid), dim3(S::kThreads), S::kLds, s, p);
   return check_launch(fn);
 }
 // fn(rows / 32, columns / 64) of the tile whose rounds of 256 workgroups take the least time.  A round's time relative to 256 x 256, at [3000 x 2048] @
@@ -468,6 +554,11 @@ int with_tile(int64_t M, int64_t N, const Fn& fn) {
   }
 }
 
+template <typename T>
+void take(char*& next, T*& part, int64_t n) {   // n of them, from a 16-byte boundary
+  part = reinterpret_cast<T*>(next);
+  next += (n * static_cast<int64_t>(sizeof(T)) + 15) / 16 * 16;
+}
 // what the forward keeps beside its results
 struct Workspace {
   __bf16* packed;        // [rows, hidden]
@@ -478,16 +569,32 @@ struct Workspace {
   int64_t bytes;
   Workspace(void* at, int64_t rows, int64_t hidden, int64_t vocab) {
     char* next = static_cast<char*>(at);
-    auto take = [&](auto*& part, int64_t n) {
-      part = reinterpret_cast<std::remove_reference_t<decltype(part)>>(next);
-      next += (n * static_cast<int64_t>(sizeof(*part)) + 15) / 16 * 16;
-    };
-    take(packed, rows > kFewRows ? rows * hidden : 0);
-    take(partial, (rows + 63) / 64 * 64 * groups_of(vocab, kLeastGroup));
-    take(targets, rows);
-    take(target_logit, rows);
-    take(position, rows);
-    take(count, 1);
+    take(next, packed, rows > kFewRows ? rows * hidden : 0);
+    take(next, partial, (rows + 63) / 64 * 64 * groups_of(vocab, kLeastGroup));
+    take(next, targets, rows);
+    take(next, target_logit, rows);
+    take(next, position, rows);
+    take(next, count, 1);
+    bytes = next - static_cast<char*>(at);
+  }
+};
+
+struct BackwardWorkspace {
+  __bf16 *dlogits, *packed;   // [rows, vocab], [rows, hidden]: of those that count
+  float* partial;             // [parts][rows that count][hidden]
+  GradRow* grad_rows;         // [rows]
+  int64_t* targets;           // [rows]
+  int *position, *count;      // [rows], [1]
+  int64_t bytes;
+  BackwardWorkspace(void* at, int64_t rows, int64_t hidden, int64_t vocab) {
+    char* next = static_cast<char*>(at);
+    take(next, dlogits, rows * vocab);
+    take(next, packed, rows * hidden);
+    take(next, partial, std::max(rows * hidden, kMostPartial));
+    take(next, grad_rows, rows);
+    take(next, targets, rows);
+    take(next, position, rows);
+    take(next, count, 1);
     bytes = next - static_cast<char*>(at);
   }
 };
@@ -584,9 +691,72 @@ extern "C" int pico_linear_log_probs_dlogits(const void* x, const void* w, const
   p.k = static_cast<float>(1.4426950408889634 / temperature);
   GradRow* of = static_cast<GradRow*>(workspace);
   hipLaunchKernelGGL(grad_rows_kernel, dim3(static_cast<unsigned>((rows + 255) / 256)), dim3(256), 0, s, reinterpret_cast<const f32x2*>(max_sum), dlog_probs, targets, of,
-                     p.M, p.N, p.k, 1.f / temperature, ignore_index);
+                     nullptr, nullptr, p.M, p.N, p.k, 1.f / temperature, ignore_index);
   p.c = dlogits;
   p.ldc = static_cast<int>(ldd);
   p.grad_rows = of;
   return with_tile(rows, vocab, [&](auto i, auto j) { return launch<decltype(i)::value, decltype(j)::value, GradTile>(p, fn, s); });
+}
+
+// The whole backward, of the rows that count, where it is worth it: two rows of tiles, tiles of the gradient of w that fill the GPU twice, and of that of x enough that
+// 32 parts of them fill it when few rows count (9 tiles, [600 x 576], took 391 us instead of 200 with a quarter of the parts).
+extern "C" int64_t pico_linear_log_probs_bwd_workspace_bytes(int64_t rows, int64_t hidden, int64_t vocab) {
+  const int64_t tiles_n = (hidden + 255) / 256;
+  if (rows < 512 || hidden <= 0 || vocab % 8 != 0 || vocab < 64 * 2 * kMostParts || vocab * hidden < (1 << 23) || (vocab + 255) / 256 * tiles_n < 512 ||
+      (rows + 255) / 256 * tiles_n < 32 ||
+      !pico_product_large_takes(rows, vocab, hidden, hidden, hidden, 0, 0, 1) || !pico_product_large_takes(rows, hidden, vocab, vocab, hidden, 0, 1, kMostParts) ||
+      !pico_product_large_takes(vocab, hidden, rows, vocab, hidden, 1, 1, 1) || rows * hidden > (int64_t{1} << 31))
+    return 0;
+  return BackwardWorkspace(nullptr, rows, hidden, vocab).bytes;
+}
+
+extern "C" int pico_linear_log_probs_bwd(const void* x, const void* w, const int64_t* targets, const float* max_sum, const float* dlog_probs, void* dx, void* dw,
+                                         int64_t rows, int64_t hidden, int64_t vocab, int64_t ldw, float temperature, int64_t ignore_index, void* workspace,
+                                         int64_t workspace_bytes, void* stream) {
+  const char* fn = "pico_linear_log_probs_bwd";
+  if (int rc = check_linear(fn, x, w, targets, rows, hidden, vocab, hidden, ldw, temperature)) return rc;
+  const int64_t bytes = pico_linear_log_probs_bwd_workspace_bytes(rows, hidden, vocab);
+  if (bytes <= 0 || !pico_product_large_takes(rows, hidden, vocab, vocab, ldw, 0, 1, kMostParts))
+    return fail(PICO_ERR_SHAPE, "%s: rows=%lld hidden=%lld vocab=%lld (pitch of w %lld): pico_linear_log_probs_dlogits and two products take these", fn,
+                static_cast<long long>(rows), static_cast<long long>(hidden), static_cast<long long>(vocab), static_cast<long long>(ldw));
+  if (!max_sum || !dlog_probs || !dx || !dw || !workspace) return fail(PICO_ERR_NULL, "%s: max_sum, dlog_probs, dx, dw and workspace are required", fn);
+  if (!aligned16(dx) || !aligned16(dw) || !aligned16(workspace) || reinterpret_cast<uintptr_t>(max_sum) % 8)
+    return fail(PICO_ERR_ALIGN, "%s: dx, dw and workspace must be aligned to 16 bytes, max_sum to 8", fn);
+  if (workspace_bytes < bytes) return fail(PICO_ERR_WORKSPACE, "%s: workspace of %lld bytes, needs %lld", fn, static_cast<long long>(workspace_bytes), static_cast<long long>(bytes));
+  const BackwardWorkspace of(workspace, rows, hidden, vocab);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const float inv_t = 1.f / temperature;
+  GradParams g = {};
+  fill(g, x, w, rows, hidden, vocab, hidden, ldw);
+  g.k = static_cast<float>(1.4426950408889634 / temperature);
+  const int per = pack_rows_of(rows);
+  hipLaunchKernelGGL(pack_rows_kernel, dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(kPackThreads), 0, s, g.a, targets, of.position, of.count, of.targets,
+                     of.packed, g.M, g.K, g.N, per, ignore_index);
+  hipLaunchKernelGGL(grad_rows_kernel, dim3(static_cast<unsigned>((rows + 255) / 256)), dim3(256), 0, s, reinterpret_cast<const f32x2*>(max_sum), dlog_probs, targets,
+                     of.grad_rows, of.position, of.count, g.M, g.N, g.k, inv_t, ignore_index);
+  g.c = of.dlogits;
+  g.ldc = static_cast<int>(vocab);
+  g.grad_rows = of.grad_rows;
+  g.count = of.count;
+  g.packed = of.packed;
+  if (int rc = with_tile(rows, vocab, [&](auto i, auto j) { return launch<decltype(i)::value, decltype(j)::value, GradTile>(g, fn, s); })) return rc;
+  // gradient of x: [rows that count, vocab] @ [vocab, hidden]; of w: [vocab, rows that count] @ [rows that count, hidden]
+  CountedParams p = {};
+  fill(p, of.dlogits, w, rows, vocab, hidden, vocab, ldw);
+  p.c = of.partial;
+  p.count = of.count;
+  p.rows = static_cast<int>(rows);
+  CountedParams q = {};
+  fill(q, of.dlogits, x, vocab, rows, hidden, vocab, hidden);
+  q.c = dw;
+  q.count = of.count;
+  q.packed = of.packed;
+  q.rows = p.rows;
+  // (columns of 192 where they leave less over: hidden 576)
+  const bool narrow = (hidden + 191) / 192 * 84 < (hidden + 255) / 256 * 100;
+  if (int rc = narrow ? launch<8, 3, InputGradTile, false, true>(p, fn, s) : launch<8, 4, InputGradTile, false, true>(p, fn, s)) return rc;
+  const int tn = narrow ? 192 : 256;
+  hipLaunchKernelGGL(unpack_rows_kernel, dim3(static_cast<unsigned>((rows * (hidden / 8) + kUnpackThreads - 1) / kUnpackThreads)), dim3(kUnpackThreads), 0, s, of.partial,
+                     of.position, of.count, static_cast<__bf16*>(dx), p.rows, static_cast<int>(hidden), 256, static_cast<int>((hidden + tn - 1) / tn));
+  return narrow ? launch<8, 3, WeightGradTile, true, true>(q, fn, s) : launch<8, 4, WeightGradTile, true, true>(q, fn, s);
 }

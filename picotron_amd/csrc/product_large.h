@@ -129,7 +129,8 @@ struct StoreTile {
 };
 
 // What becomes of a tile's sums is the epilogue's: Epilogue::Params (LargeParams and what it needs beside), begin(), called once the tile before
-// has left, with kBegun vector memory operations, and tile(), with kStores of them.  Where kCounted count(), first of all, may set another, smaller M and another a.
+// has left, with kBegun vector memory operations, and tile(), with kStores of them.  Where kCounted count(), first of all, may set other, smaller
+// sizes and other operands.
 template <bool kSlowA, bool kSlowB, int I, int J, typename Epilogue>
 __global__ __launch_bounds__(512, 2) void product_large_kernel(const typename Epilogue::Params given) {
   using S = Shape<kSlowA, kSlowB, I, J>;
@@ -142,9 +143,8 @@ __global__ __launch_bounds__(512, 2) void product_large_kernel(const typename Ep
 
   typename Epilogue::Params p = given;
   if constexpr (Epilogue::kCounted) {
-    Epilogue::count(p);
-    p.tiles_m = (p.M + TM - 1) / TM;
-    if (static_cast<int>(blockIdx.x) >= p.tiles_m * p.tiles_n) return;
+    Epilogue::template count<TM>(p);
+    if (static_cast<int>(blockIdx.x) >= p.tiles_m * p.tiles_n * p.parts) return;
   }
 
   // ---- requests

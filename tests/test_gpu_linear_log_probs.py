@@ -166,6 +166,56 @@ def test_rows_that_do_not_count_change_nothing(device, rows, hidden, vocab):
     assert torch.equal(dx, ex) and torch.equal(dw, ew) and not dx[kept >= 0.3].any()
 
 
+@pytest.mark.parametrize("rows,hidden,vocab", [(2800, 576, 49152), (2000, 4096, 8192), (1503, 2048, 16392), (2049, 1000, 32776), (4100, 264, 65544), (512, 4096, 8200)])
+def test_gradients_of_the_rows_that_count(device, rows, hidden, vocab):
+    """Sizes whose backward leaves out what does not count: against the definition, and the same bits whatever the other rows hold."""
+    from picotron_amd import _lib
+    from picotron_amd.functional import linear_log_probs
+    assert _lib.lib().pico_linear_log_probs_bwd_workspace_bytes(rows, hidden, vocab) > 0
+    x, w, t = inputs(rows, rows, hidden, vocab, kept=1.0)
+    kept, r = torch.rand(rows, generator=gen(8), device="cuda"), torch.arange(rows, device="cuda")
+    a = torch.randn(rows, generator=gen(9), device="cuda")
+    for i, counts in enumerate((kept < 0.3, r < 0, r == rows - 3, r < 127, r >= rows - 129, (r // 100) % 3 == 1, kept < 0.9, r > -1)):
+        u = torch.where(counts, t, IGNORE)
+        if i in (0, 2, 3, 6, 7):
+            check(x, w, u, seed=i)
+        got = []
+        for y in (x, torch.where(counts[:, None], x, float("nan"))):
+            y, v = y.detach().clone().requires_grad_(), w.clone().requires_grad_()
+            got.append(torch.autograd.grad(linear_log_probs(y, v, u), (y, v), torch.where(counts, a, float("inf"))))
+        (dx, dw), (ex, ew) = got
+        assert torch.equal(dx, ex) and torch.equal(dw, ew) and not dw.isnan().any() and not dx[~counts].any(), i
+        assert dx[counts].any(1).all() and bool(dw.any()) == bool(counts.any()), i
+
+
+def test_a_recorded_step_takes_other_rows_on_every_replay(device):
+    from picotron_amd.functional import linear_log_probs
+    x, w, t = inputs(5, 2049, 1000, 32776, kept=1.0)
+    kept = torch.rand(2049, generator=gen(6), device="cuda")
+    masked = [torch.where(kept < share, t, IGNORE) for share in (0.0, 0.5, 1.0, 0.04)]
+    a = torch.randn(2049, generator=gen(7), device="cuda")
+
+    def step(u):
+        y, v = x.detach().requires_grad_(), w.detach().requires_grad_()
+        return torch.autograd.grad(linear_log_probs(y, v, u), (y, v), a)
+    want = [step(u) for u in masked]
+    still = t.clone()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        side.wait_stream(torch.cuda.default_stream())
+        step(still)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(still)
+    for i in (2, 0, 1, 3, 2, 1):
+        still.copy_(masked[i])
+        graph.replay()
+        step(masked[(i + 1) % 4])
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[i][0]) and torch.equal(got[1], want[i][1]), i
+
+
 def test_a_recorded_call_takes_other_rows_on_every_replay(device):
     from picotron_amd.functional import linear_log_probs
     x, w, t = inputs(5, 1100, 264, 33001, kept=1.0)

@@ -18,7 +18,7 @@ def test_products_with_an_epilogue_of_their_own():
     from picotron_amd import build
     kernels, assembly = compiled(csrc("linear_log_probs.hip"))
     looked_at = {name for name in kernels if re.search(build.REQUESTING["linear_log_probs.hip"], name)}
-    assert len(looked_at) == 10
+    assert len(looked_at) == 14
     for name, r in kernels.items():
         body = assembly[assembly.index(f"\n{name}:"):]
         assert (" lds\n" in body[:body.index(".Lfunc_end")]) == (name in looked_at), name
