@@ -517,6 +517,9 @@ int pico_linear_log_probs_fwd(const void* x, const void* w, const int64_t* targe
 int pico_linear_log_probs_dlogits(const void* x, const void* w, const int64_t* targets, const float* max_sum, const float* dlog_probs,
                                   void* dlogits, int64_t rows, int64_t hidden, int64_t vocab, int64_t ldx, int64_t ldw, int64_t ldd,
                                   float temperature, int64_t ignore_index, void* workspace, int64_t workspace_bytes, void* stream);
+/* dw = d^T x of few rows (1 .. 32): d [rows, out] (pitch ldd) and x [rows, in] (pitch ldx) bf16, dw [out, in] bf16, contiguous and aligned to 16 bytes; in a
+ * multiple of 8. */
+int pico_weight_grad_few(const void* d, const void* x, void* dw, int64_t rows, int64_t out, int64_t in, int64_t ldd, int64_t ldx, void* stream);
 /* The gradients of x and w as one call, over the rows that count: what does not count takes no part in any of the three products.  dx [rows, hidden] and
  * dw [vocab, hidden]: bf16, contiguous (dx 0 in rows that do not count); x contiguous.  workspace: pico_linear_log_probs_bwd_workspace_bytes bytes, 16-byte
  * aligned (d(logits) in bf16, x, x in fp32 or 128 MiB); that is 0 for sizes that this call does not take (vocab no multiple of 8, under 512 rows, few tiles).

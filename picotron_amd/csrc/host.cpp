@@ -1666,12 +1666,19 @@ struct LinearLogProbs : torch::autograd::Function<LinearLogProbs> {
     check(pico_linear_log_probs_dlogits(ptr(a), ptr(b), t.data_ptr<int64_t>(), fptr(s[3]), fptr(dlp), ptr(dz), M, a.size(1), N, pitch(a), pitch(b), ldd,
                                         temperature, ignore, ptr(ws), M * 16, stream_now()));
     const Tensor d = dz.narrow(1, 0, N);
-    if (both_wanted) {
+    // (few rows' gradient of w where no other kernel of the package takes it)
+    const bool few = M > 0 && M <= 32 && ctx->needs_input_grad(1) && !stays_with_torch(d, a) &&
+                     product_route(Product::TN, product_sizes(d, a, Product::TN)).kernel == ProductRoute::Library;
+    if (both_wanted && !few) {
       Gradients both = gradients(d, b, a);
       r[0] = both.dx.view(x.sizes());
       r[1] = both.dw;
-    } else if (ctx->needs_input_grad(0)) {
-      r[0] = product(d, b, Product::NN).view(x.sizes());
+      return r;
+    }
+    if (ctx->needs_input_grad(0)) r[0] = product(d, b, Product::NN).view(x.sizes());
+    if (few) {
+      r[1] = at::empty({N, K}, a.options());
+      check(pico_weight_grad_few(ptr(d), ptr(a), ptr(r[1]), M, N, K, ldd, pitch(a), stream_now()));
     } else if (ctx->needs_input_grad(1)) {
       r[1] = product(d, a, Product::TN);
     }

@@ -509,6 +509,51 @@ __global__ __launch_bounds__(kUnpackThreads) void unpack_rows_kernel(const float
   reinterpret_cast<bf16x8*>(dx)[id] = v;
 }
 
+// ---- the gradient of w from few rows (32 at most): d(logits)^T x has a contraction of one product, and what bounds it is writing dw once.  A wave keeps x's
+// 128 columns in registers as operands and walks 16 rows of dw at a time, whose d(logits) it requests one step ahead.  Tile j's column c is column
+// 32 (j / 2) + 8 (c / 4) + 4 (j % 2) + c % 4 of the 128, so that two tiles give a lane 16 bytes and four lanes 64 of a row.  us, the GEMM library and here: 16 rows of
+// 2048 against 49152 66, 34 (5.9 TB/s), 32 rows 44, 36, 4 of 2112 182, 42, 32 of 1024 against 120000 94, 44.  (Where the package's other products take it, up to
+// 576 or 1024 columns, they are 2 .. 10 us faster; 64 rows, two products, took 0.85 to 1.04 of the library's time.)
+constexpr int kFewGradRows = 32, kGradJ = 8, kGradColumns = 16 * kGradJ, kGradWalk = 16;   // kGradWalk steps of 16 rows of dw
+__global__ __launch_bounds__(256) void weight_grad_few_kernel(const __bf16* __restrict__ d, const __bf16* __restrict__ x, __bf16* __restrict__ dw, int M, int N, int K,
+                                                              int64_t ldd, int64_t ldx) {
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, n = lane % 16, h = lane / 16;
+  const int col0 = (blockIdx.x * 4 + wave) * kGradColumns, row0 = blockIdx.y * 16 * kGradWalk;
+  if (col0 >= K) return;
+  bf16x8 fx[kGradJ];
+#pragma unroll
+  for (int j = 0; j < kGradJ; ++j) {
+    const int col = col0 + 32 * (j / 2) + 8 * (n / 4) + 4 * (j % 2) + n % 4;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int r = 8 * h + e;
+      const __bf16 v = x[min(r, M - 1) * ldx + min(col, K - 1)];   // (no load hangs on a condition: they are requested together, 58 -> 35 us)
+      fx[j][e] = r < M ? v : static_cast<__bf16>(0.f);
+    }
+  }
+  auto load = [&](bf16x8& f, int row) __attribute__((always_inline)) {   // d(logits) of rows row .. row + 15 of dw (past M: beside zeros of x)
+    const __bf16* from = d + min(row + n, N - 1);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = from[min(8 * h + e, M - 1) * ldd];
+  };
+  bf16x8 now, next;
+  load(now, row0);
+  const int last = min(row0 + 16 * kGradWalk, N);
+  for (int row = row0; row < last; row += 16, now = next) {
+    if (row + 16 < last) load(next, row + 16);
+#pragma unroll
+    for (int j = 0; j < kGradJ; j += 2) {
+      const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+      const f32x4 v[2] = {__builtin_amdgcn_mfma_f32_16x16x32_bf16(fx[j], now, zero, 0, 0, 0), __builtin_amdgcn_mfma_f32_16x16x32_bf16(fx[j + 1], now, zero, 0, 0, 0)};
+      bf16x8 out;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) out[e] = static_cast<__bf16>(v[e / 4][e % 4]);
+      const int col = col0 + 16 * j + 8 * h;
+      if (row + n < last && col < K) *reinterpret_cast<bf16x8*>(dw + static_cast<int64_t>(row + n) * K + col) = out;
+    }
+  }
+}
+
 template <int I, int J, typename Epilogue, bool kSlowA = false, bool kSlowB = false>
 int launch(typename Epilogue::Params p, const char* fn, hipStream_t s) {
   using S = Shape<kSlowA, kSlowB, I, J>;
@@ -759,4 +804,18 @@ extern "C" int pico_linear_log_probs_bwd(const void* x, const void* w, const int
   hipLaunchKernelGGL(unpack_rows_kernel, dim3(static_cast<unsigned>((rows * (hidden / 8) + kUnpackThreads - 1) / kUnpackThreads)), dim3(kUnpackThreads), 0, s, of.partial,
                      of.position, of.count, static_cast<__bf16*>(dx), p.rows, static_cast<int>(hidden), 256, static_cast<int>((hidden + tn - 1) / tn));
   return narrow ? launch<8, 3, WeightGradTile, true, true>(q, fn, s) : launch<8, 4, WeightGradTile, true, true>(q, fn, s);
+}
+
+extern "C" int pico_weight_grad_few(const void* d, const void* x, void* dw, int64_t rows, int64_t out, int64_t in, int64_t ldd, int64_t ldx, void* stream) {
+  const char* fn = "pico_weight_grad_few";
+  if (rows < 1 || rows > kFewGradRows || out < 1 || out > 0x7fffffff / 256 || in < 8 || in % 8 != 0 || in > 0x7fffffff / 256)
+    return fail(PICO_ERR_SHAPE, "%s: rows=%lld (1 .. %d) out=%lld in=%lld (a multiple of 8)", fn, static_cast<long long>(rows), kFewGradRows, static_cast<long long>(out),
+                static_cast<long long>(in));
+  if (ldd < out || ldx < in) return fail(PICO_ERR_STRIDE, "%s: row pitches %lld, %lld are less than the rows", fn, static_cast<long long>(ldd), static_cast<long long>(ldx));
+  if (!d || !x || !dw) return fail(PICO_ERR_NULL, "%s: d, x and dw are required", fn);
+  if (reinterpret_cast<uintptr_t>(d) % 2 || reinterpret_cast<uintptr_t>(x) % 2 || !aligned16(dw)) return fail(PICO_ERR_ALIGN, "%s: dw must be aligned to 16 bytes, d and x to their elements", fn);
+  const dim3 grid(static_cast<unsigned>((in + 4 * kGradColumns - 1) / (4 * kGradColumns)), static_cast<unsigned>((out + 16 * kGradWalk - 1) / (16 * kGradWalk)));
+  hipLaunchKernelGGL(weight_grad_few_kernel, grid, dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<const __bf16*>(d), static_cast<const __bf16*>(x),
+                     static_cast<__bf16*>(dw), static_cast<int>(rows), static_cast<int>(out), static_cast<int>(in), ldd, ldx);
+  return check_launch(fn);
 }

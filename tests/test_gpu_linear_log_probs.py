@@ -216,6 +216,32 @@ def test_a_recorded_step_takes_other_rows_on_every_replay(device):
         assert torch.equal(got[0], want[i][0]) and torch.equal(got[1], want[i][1]), i
 
 
+@pytest.mark.parametrize("rows,hidden,vocab", [(1, 2048, 49152), (4, 2112, 49152), (16, 2048, 32000), (31, 1032, 60001), (32, 2048, 49151), (17, 4096, 20003)])
+def test_gradients_of_few_rows(device, rows, hidden, vocab):
+    x, w, t = inputs(rows, rows, hidden, vocab, kept=1.0)
+    check(x, w, t)
+    t[rows // 2] = IGNORE
+    check(x, w, t, T=0.8)
+
+
+def test_weight_gradient_of_few_rows(device):
+    """pico_weight_grad_few over rows, edges of its tiles and pitches: a sum of 32 exact products in fp32 (32 half steps of 2^-24 of their magnitudes) and one
+    rounding, and not a byte behind dw."""
+    import ctypes
+    from picotron_amd import _lib
+    lib, P = _lib.lib(), lambda v: ctypes.c_void_p(v.data_ptr())
+    for rows, out, inn in ((1, 1, 8), (2, 15, 16), (7, 16, 24), (8, 17, 120), (9, 255, 128), (15, 256, 136), (16, 257, 512), (17, 300, 520), (31, 1000, 1032), (32, 513, 640), (32, 16, 2048)):
+        g = gen(rows)
+        d = torch.randn(rows, out + 3, generator=g, device="cuda").to(BF16)[:, :out]
+        x = torch.randn(rows, inn + 5, generator=g, device="cuda").to(BF16)[:, 2:2 + inn]
+        dw = torch.full((out * inn + 64,), 7.0, dtype=BF16, device="cuda")
+        assert lib.pico_weight_grad_few(P(d), P(x), P(dw), rows, out, inn, d.stride(0), x.stride(0), None) == 0
+        torch.cuda.synchronize()
+        got, want = dw[:out * inn].view(out, inn).double(), d.double().t() @ x.double()
+        over = (got - want).abs() - 2 ** -8 * want.abs() - 2 ** -18 * (d.double().abs().t() @ x.double().abs())
+        assert (over <= 0).all() and (dw[out * inn:] == 7).all(), (rows, out, inn, over.max().item())
+
+
 def test_a_recorded_call_takes_other_rows_on_every_replay(device):
     from picotron_amd.functional import linear_log_probs
     x, w, t = inputs(5, 1100, 264, 33001, kept=1.0)

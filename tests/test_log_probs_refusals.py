@@ -146,6 +146,20 @@ def test_linear_log_probs_backward_of_the_rows_that_count(lib):
     assert bwd(bytes=size(2800, 576, 49152) - 1) == -6 and "workspace" in message(lib)
 
 
+def test_weight_gradient_of_few_rows(lib):
+    def call(d=4096, x=4096, dw=4096, rows=8, out=100, inn=64, ldd=100, ldx=64):
+        P = ctypes.c_void_p
+        return lib.pico_weight_grad_few(P(d), P(x), P(dw), rows, out, inn, ldd, ldx, None)
+    for over in (dict(rows=0), dict(rows=33), dict(out=0), dict(inn=0), dict(inn=60), dict(out=1 << 30), dict(inn=1 << 30)):
+        assert call(**over) == -3, over
+    for over in (dict(ldd=99), dict(ldx=63)):
+        assert call(**over) == -5, over
+    for over in (dict(d=None), dict(x=None), dict(dw=None)):
+        assert call(**over) == -1, over
+    for over in (dict(d=4097), dict(x=4097), dict(dw=4104)):
+        assert call(**over) == -4, over
+
+
 def test_host_path_refusals():
     """Tensors on the CPU are refused, not computed, and shapes are looked at first."""
     from picotron_amd.functional import linear_log_probs, log_probs, policy_loss, preference_loss
