@@ -1666,10 +1666,12 @@ struct LinearLogProbs : torch::autograd::Function<LinearLogProbs> {
     check(pico_linear_log_probs_dlogits(ptr(a), ptr(b), t.data_ptr<int64_t>(), fptr(s[3]), fptr(dlp), ptr(dz), M, a.size(1), N, pitch(a), pitch(b), ldd,
                                         temperature, ignore, ptr(ws), M * 16, stream_now()));
     const Tensor d = dz.narrow(1, 0, N);
-    // (few rows' gradient of w where no other kernel of the package takes it)
-    const bool few = M > 0 && M <= 32 && ctx->needs_input_grad(1) && !stays_with_torch(d, a) &&
-                     product_route(Product::TN, product_sizes(d, a, Product::TN)).kernel == ProductRoute::Library;
-    if (both_wanted && !few) {
+    // The gradient of w from few rows, a short contraction that writes much, where the rules for products would leave it to the GEMM library.  us, there and here: up
+    // to 32 rows see the kernel; [32000 x 4096] from 72 rows 99, 62, from 104 103, 58, [49152 x 2112] from 96 175, 57; from 128 on the rules choose that kernel.
+    const bool short_walk = M > 0 && M < 128 && ctx->needs_input_grad(1) && !stays_with_torch(d, a) &&
+                            product_route(Product::TN, product_sizes(d, a, Product::TN)).kernel == ProductRoute::Library;
+    const bool few = short_walk && M <= 32, large = short_walk && M > 64 && N * K >= 1 << 25 && pico_product_large_takes(N, K, M, ldd, pitch(a), 1, 1, 1);
+    if (both_wanted && !few && !large) {
       Gradients both = gradients(d, b, a);
       r[0] = both.dx.view(x.sizes());
       r[1] = both.dw;
@@ -1679,6 +1681,8 @@ struct LinearLogProbs : torch::autograd::Function<LinearLogProbs> {
     if (few) {
       r[1] = at::empty({N, K}, a.options());
       check(pico_weight_grad_few(ptr(d), ptr(a), ptr(r[1]), M, N, K, ldd, pitch(a), stream_now()));
+    } else if (large) {
+      r[1] = product(d, a, Product::TN, product_sizes(d, a, Product::TN), {ProductRoute::Large, 256, 256, 0, 1, 0});
     } else if (ctx->needs_input_grad(1)) {
       r[1] = product(d, a, Product::TN);
     }

@@ -216,7 +216,8 @@ def test_a_recorded_step_takes_other_rows_on_every_replay(device):
         assert torch.equal(got[0], want[i][0]) and torch.equal(got[1], want[i][1]), i
 
 
-@pytest.mark.parametrize("rows,hidden,vocab", [(1, 2048, 49152), (4, 2112, 49152), (16, 2048, 32000), (31, 1032, 60001), (32, 2048, 49151), (17, 4096, 20003)])
+@pytest.mark.parametrize("rows,hidden,vocab", [(1, 2048, 49152), (4, 2112, 49152), (16, 2048, 32000), (31, 1032, 60001), (32, 2048, 49151), (17, 4096, 20003),
+                                               (33, 2112, 32000), (65, 4096, 10000), (100, 2112, 49152), (127, 4096, 32000), (127, 4096, 32001)])
 def test_gradients_of_few_rows(device, rows, hidden, vocab):
     x, w, t = inputs(rows, rows, hidden, vocab, kept=1.0)
     check(x, w, t)
