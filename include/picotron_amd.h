@@ -521,8 +521,9 @@ int pico_linear_log_probs_dlogits(const void* x, const void* w, const int64_t* t
  * multiple of 8. */
 int pico_weight_grad_few(const void* d, const void* x, void* dw, int64_t rows, int64_t out, int64_t in, int64_t ldd, int64_t ldx, void* stream);
 /* The gradients of x and w as one call, over the rows that count: what does not count takes no part in any of the three products.  dx [rows, hidden] and
- * dw [vocab, hidden]: bf16, contiguous (dx 0 in rows that do not count); x contiguous.  workspace: pico_linear_log_probs_bwd_workspace_bytes bytes, 16-byte
- * aligned (d(logits) in bf16, x, x in fp32 or 128 MiB); that is 0 for sizes that this call does not take (vocab no multiple of 8, under 512 rows, few tiles).
+ * dw [vocab rounded up to a multiple of 8, hidden]: bf16, contiguous (dx 0 in rows that do not count, dw 0 in rows from vocab on); x contiguous.  workspace:
+ * pico_linear_log_probs_bwd_workspace_bytes bytes, 16-byte aligned (d(logits) in bf16, x, x in fp32 or 128 MiB); that is 0 for sizes that this call does not
+ * take (under 512 rows, few tiles).
  */
 int64_t pico_linear_log_probs_bwd_workspace_bytes(int64_t rows, int64_t hidden, int64_t vocab);
 int pico_linear_log_probs_bwd(const void* x, const void* w, const int64_t* targets, const float* max_sum, const float* dlog_probs,

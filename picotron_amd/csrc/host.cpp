@@ -1655,11 +1655,11 @@ struct LinearLogProbs : torch::autograd::Function<LinearLogProbs> {
     variable_list r(5);
     const bool both_wanted = ctx->needs_input_grad(0) && ctx->needs_input_grad(1);
     if (const int64_t bytes = both_wanted && pitch(a) == K && pitch(b) == K ? pico_linear_log_probs_bwd_workspace_bytes(M, K, N) : 0) {
-      const Tensor dx = at::empty({M, K}, a.options()), dw = at::empty({N, K}, a.options()), ws = at::empty({bytes}, a.options().dtype(at::kByte));
+      const Tensor dx = at::empty({M, K}, a.options()), dw = at::empty({ldd, K}, a.options()), ws = at::empty({bytes}, a.options().dtype(at::kByte));
       check(pico_linear_log_probs_bwd(ptr(a), ptr(b), t.data_ptr<int64_t>(), fptr(s[3]), fptr(dlp), ptr(dx), ptr(dw), M, K, N, K, temperature, ignore, ptr(ws), bytes,
                                       stream_now()));
       r[0] = dx.view(x.sizes());
-      r[1] = dw;
+      r[1] = dw.narrow(0, 0, N);
       return r;
     }
     const Tensor dz = at::empty({M, ldd}, a.options()), ws = at::empty({std::max<int64_t>(M * 16, 16)}, a.options().dtype(at::kByte));

@@ -488,7 +488,9 @@ struct WeightGradTile : StoreTile<false> {   // a: d(logits), b: x
 };
 constexpr int kUnpackThreads = 256;
 __global__ __launch_bounds__(kUnpackThreads) void unpack_rows_kernel(const float* __restrict__ partial, const int* __restrict__ position, const int* __restrict__ count,
-                                                                     __bf16* __restrict__ dx, int rows, int K, int tile_rows, int tiles_n) {
+                                                                     __bf16* __restrict__ dx, int rows, int K, int tile_rows, int tiles_n,
+                                                                     const __bf16* __restrict__ dlogits, const __bf16* __restrict__ w, int ldd, int64_t ldw, int from_entry,
+                                                                     int vocab) {
   const int pieces = K / 8, n = *count, parts = parts_of((n + tile_rows - 1) / tile_rows * tiles_n, n, K);
   const int64_t all = static_cast<int64_t>(rows) * pieces, id = static_cast<int64_t>(blockIdx.x) * kUnpackThreads + threadIdx.x;
   if (id >= all) return;
@@ -499,6 +501,16 @@ __global__ __launch_bounds__(kUnpackThreads) void unpack_rows_kernel(const float
       const f32x4* from = reinterpret_cast<const f32x4*>(partial + ((static_cast<int64_t>(q) * n + at) * pieces + piece) * 8);
       lo += from[0];
       hi += from[1];
+    }
+  if (at >= 0)   // the vocabulary's last entries, of which no whole piece of 16 bytes is left
+    for (int entry = from_entry; entry < vocab; ++entry) {
+      const float g = static_cast<float>(dlogits[at * ldd + entry]);
+      const bf16x8 of = *reinterpret_cast<const bf16x8*>(w + entry * ldw + piece * 8);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        lo[e] = fmaf(g, static_cast<float>(of[e]), lo[e]);
+        hi[e] = fmaf(g, static_cast<float>(of[4 + e]), hi[e]);
+      }
     }
   bf16x8 v;
 #pragma unroll
@@ -633,7 +645,7 @@ struct BackwardWorkspace {
   int64_t bytes;
   BackwardWorkspace(void* at, int64_t rows, int64_t hidden, int64_t vocab) {
     char* next = static_cast<char*>(at);
-    take(next, dlogits, rows * vocab);
+    take(next, dlogits, rows * ((vocab + 7) / 8 * 8));
     take(next, packed, rows * hidden);
     take(next, partial, std::max(rows * hidden, kMostPartial));
     take(next, grad_rows, rows);
@@ -746,11 +758,11 @@ extern "C" int pico_linear_log_probs_dlogits(const void* x, const void* w, const
 // The whole backward, of the rows that count, where it is worth it: two rows of tiles, tiles of the gradient of w that fill the GPU twice, and of that of x enough that
 // 32 parts of them fill it when few rows count (9 tiles, [600 x 576], took 391 us instead of 200 with a quarter of the parts).
 extern "C" int64_t pico_linear_log_probs_bwd_workspace_bytes(int64_t rows, int64_t hidden, int64_t vocab) {
-  const int64_t tiles_n = (hidden + 255) / 256;
-  if (rows < 512 || hidden <= 0 || vocab % 8 != 0 || vocab < 64 * 2 * kMostParts || vocab * hidden < (1 << 23) || (vocab + 255) / 256 * tiles_n < 512 ||
+  const int64_t tiles_n = (hidden + 255) / 256, pitch = (vocab + 7) / 8 * 8, whole = vocab / 8 * 8;
+  if (rows < 512 || hidden <= 0 || whole < 64 * 2 * kMostParts || vocab * hidden < (1 << 23) || (vocab + 255) / 256 * tiles_n < 512 ||
       (rows + 255) / 256 * tiles_n < 32 ||
-      !pico_product_large_takes(rows, vocab, hidden, hidden, hidden, 0, 0, 1) || !pico_product_large_takes(rows, hidden, vocab, vocab, hidden, 0, 1, kMostParts) ||
-      !pico_product_large_takes(vocab, hidden, rows, vocab, hidden, 1, 1, 1) || rows * hidden > (int64_t{1} << 31))
+      !pico_product_large_takes(rows, pitch, hidden, hidden, hidden, 0, 0, 1) || !pico_product_large_takes(rows, hidden, whole, pitch, hidden, 0, 1, kMostParts) ||
+      !pico_product_large_takes(pitch, hidden, rows, pitch, hidden, 1, 1, 1) || rows * hidden > (int64_t{1} << 31))
     return 0;
   return BackwardWorkspace(nullptr, rows, hidden, vocab).bytes;
 }
@@ -761,7 +773,8 @@ extern "C" int pico_linear_log_probs_bwd(const void* x, const void* w, const int
   const char* fn = "pico_linear_log_probs_bwd";
   if (int rc = check_linear(fn, x, w, targets, rows, hidden, vocab, hidden, ldw, temperature)) return rc;
   const int64_t bytes = pico_linear_log_probs_bwd_workspace_bytes(rows, hidden, vocab);
-  if (bytes <= 0 || !pico_product_large_takes(rows, hidden, vocab, vocab, ldw, 0, 1, kMostParts))
+  const int64_t pitch = (vocab + 7) / 8 * 8, whole = vocab / 8 * 8;   // d(logits)' rows end in zeros up to pitch; whole pieces of 16 bytes
+  if (bytes <= 0 || !pico_product_large_takes(rows, hidden, whole, pitch, ldw, 0, 1, kMostParts))
     return fail(PICO_ERR_SHAPE, "%s: rows=%lld hidden=%lld vocab=%lld (pitch of w %lld): pico_linear_log_probs_dlogits and two products take these", fn,
                 static_cast<long long>(rows), static_cast<long long>(hidden), static_cast<long long>(vocab), static_cast<long long>(ldw));
   if (!max_sum || !dlog_probs || !dx || !dw || !workspace) return fail(PICO_ERR_NULL, "%s: max_sum, dlog_probs, dx, dw and workspace are required", fn);
@@ -780,19 +793,19 @@ extern "C" int pico_linear_log_probs_bwd(const void* x, const void* w, const int
   hipLaunchKernelGGL(grad_rows_kernel, dim3(static_cast<unsigned>((rows + 255) / 256)), dim3(256), 0, s, reinterpret_cast<const f32x2*>(max_sum), dlog_probs, targets,
                      of.grad_rows, of.position, of.count, g.M, g.N, g.k, inv_t, ignore_index);
   g.c = of.dlogits;
-  g.ldc = static_cast<int>(vocab);
+  g.ldc = static_cast<int>(pitch);
   g.grad_rows = of.grad_rows;
   g.count = of.count;
   g.packed = of.packed;
   if (int rc = with_tile(rows, vocab, [&](auto i, auto j) { return launch<decltype(i)::value, decltype(j)::value, GradTile>(g, fn, s); })) return rc;
   // gradient of x: [rows that count, vocab] @ [vocab, hidden]; of w: [vocab, rows that count] @ [rows that count, hidden]
   CountedParams p = {};
-  fill(p, of.dlogits, w, rows, vocab, hidden, vocab, ldw);
+  fill(p, of.dlogits, w, rows, whole, hidden, pitch, ldw);
   p.c = of.partial;
   p.count = of.count;
   p.rows = static_cast<int>(rows);
   CountedParams q = {};
-  fill(q, of.dlogits, x, vocab, rows, hidden, vocab, hidden);
+  fill(q, of.dlogits, x, pitch, rows, hidden, pitch, hidden);
   q.c = dw;
   q.count = of.count;
   q.packed = of.packed;
@@ -802,7 +815,8 @@ extern "C" int pico_linear_log_probs_bwd(const void* x, const void* w, const int
   if (int rc = narrow ? launch<8, 3, InputGradTile, false, true>(p, fn, s) : launch<8, 4, InputGradTile, false, true>(p, fn, s)) return rc;
   const int tn = narrow ? 192 : 256;
   hipLaunchKernelGGL(unpack_rows_kernel, dim3(static_cast<unsigned>((rows * (hidden / 8) + kUnpackThreads - 1) / kUnpackThreads)), dim3(kUnpackThreads), 0, s, of.partial,
-                     of.position, of.count, static_cast<__bf16*>(dx), p.rows, static_cast<int>(hidden), 256, static_cast<int>((hidden + tn - 1) / tn));
+                     of.position, of.count, static_cast<__bf16*>(dx), p.rows, static_cast<int>(hidden), 256, static_cast<int>((hidden + tn - 1) / tn), of.dlogits, p.b, g.ldc, ldw,
+                     static_cast<int>(whole), static_cast<int>(vocab));
   return narrow ? launch<8, 3, WeightGradTile, true, true>(q, fn, s) : launch<8, 4, WeightGradTile, true, true>(q, fn, s);
 }
 

@@ -129,15 +129,16 @@ def test_linear_log_probs_backward_of_the_rows_that_count(lib):
     size = lib.pico_linear_log_probs_bwd_workspace_bytes
     # d(logits), x, partial sums, four numbers a row, targets and positions, one number
     assert size(2000, 4096, 32000) == 2000 * 32000 * 2 + 2000 * 4096 * 2 + 2 ** 27 + 2000 * 16 + 2000 * 8 + 2000 * 4 + 16
+    assert size(2000, 4096, 32001) == size(2000, 4096, 32008) > size(2000, 4096, 32000)
     assert size(2800, 576, 49152) > 0 and size(9000, 4096, 32000) > 9000 * (32000 * 2 + 4096 * 6)
-    for sizes in ((511, 4096, 32000), (2000, 4096, 32001), (2000, 4096, 4088), (2000, 576, 32000), (600, 576, 49152), (700, 2048, 32768), (2000, 64, 1 << 20), (40000, 4096, 32000), (-1, 4096, 32000), (2000, -8, 32000),
+    for sizes in ((511, 4096, 32000), (2000, 4096, 4095), (2000, 4096, 4088), (2000, 576, 32000), (600, 576, 49152), (700, 2048, 32768), (2000, 64, 1 << 20), (40000, 4096, 32000), (-1, 4096, 32000), (2000, -8, 32000),
                   (2000, 4096, -8), (1 << 31, 4096, 32000)):
         assert size(*sizes) == 0, sizes
 
     def bwd(x=4096, w=4096, t=4096, ms=4096, g=4096, dx=4096, dw=4096, M=2800, K=576, N=49152, ldw=576, T=1.0, ws=4096, bytes=1 << 30):
         P = ctypes.c_void_p
         return lib.pico_linear_log_probs_bwd(P(x), P(w), P(t), P(ms), P(g), P(dx), P(dw), M, K, N, ldw, T, -100, P(ws), bytes, None)
-    for over in (dict(M=100), dict(M=0), dict(K=64), dict(N=49153), dict(N=4096), dict(ldw=568), dict(ldw=1 << 30), dict(T=0.0)):
+    for over in (dict(M=100), dict(M=0), dict(K=64), dict(N=4096), dict(ldw=568), dict(ldw=1 << 30), dict(T=0.0)):
         assert bwd(**over) == -3, over
     for over in (dict(x=4104), dict(w=4098), dict(t=4100), dict(ms=4100), dict(ws=4104), dict(dx=4104), dict(dw=4098)):
         assert bwd(**over) == -4, over
