@@ -1668,10 +1668,10 @@ struct LinearLogProbs : torch::autograd::Function<LinearLogProbs> {
     const Tensor d = dz.narrow(1, 0, N);
     // The gradient of w from few rows, a short contraction that writes much, where the rules for products would leave it to the GEMM library.  us, there and here: up
     // to 32 rows see the kernel; [32000 x 4096] from 72 rows 99, 62, from 104 103, 58, [49152 x 2112] from 96 175, 57; from 128 on the rules choose that kernel.
-    const bool short_walk = M > 0 && M < 128 && ctx->needs_input_grad(1) && !stays_with_torch(d, a) &&
-                            product_route(Product::TN, product_sizes(d, a, Product::TN)).kernel == ProductRoute::Library;
-    const bool few = short_walk && M <= 32, large = short_walk && M > 64 && N * K >= 1 << 25 && pico_product_large_takes(N, K, M, ldd, pitch(a), 1, 1, 1);
-    if (both_wanted && !few && !large) {
+    const bool wants_w = ctx->needs_input_grad(1), short_walk = M > 0 && M < 128 && wants_w && !stays_with_torch(dz, a) &&
+                                                                product_route(Product::TN, product_sizes(dz, a, Product::TN)).kernel == ProductRoute::Library;
+    const bool few = short_walk && M <= 32, large = short_walk && M > 64 && ldd * K >= 1 << 25 && pico_product_large_takes(ldd, K, M, ldd, pitch(a), 1, 1, 1);
+    if (both_wanted && !few && !large && ldd == N) {
       Gradients both = gradients(d, b, a);
       r[0] = both.dx.view(x.sizes());
       r[1] = both.dw;
@@ -1681,10 +1681,8 @@ struct LinearLogProbs : torch::autograd::Function<LinearLogProbs> {
     if (few) {
       r[1] = at::empty({N, K}, a.options());
       check(pico_weight_grad_few(ptr(d), ptr(a), ptr(r[1]), M, N, K, ldd, pitch(a), stream_now()));
-    } else if (large) {
-      r[1] = product(d, a, Product::TN, product_sizes(d, a, Product::TN), {ProductRoute::Large, 256, 256, 0, 1, 0});
-    } else if (ctx->needs_input_grad(1)) {
-      r[1] = product(d, a, Product::TN);
+    } else if (wants_w) {   // (with the zeros behind the vocabulary the rows are whole pieces of 16 bytes, and the rows of dw that they make are left out)
+      r[1] = (large ? product(dz, a, Product::TN, product_sizes(dz, a, Product::TN), {ProductRoute::Large, 256, 256, 0, 1, 0}) : product(dz, a, Product::TN)).narrow(0, 0, N);
     }
     return r;
   }
