@@ -106,7 +106,7 @@ def log_probs(logits, targets, ignore_index: int = -100, temperature: float = 1.
 
 def linear_log_probs(x, weight, targets, ignore_index: int = -100, temperature: float = 1.0):
     """``log_probs(F.linear(x, weight), targets)`` for bf16 hidden states x [..., hidden] and vocabulary projection weight [vocab, hidden]
-    without the logits in memory: what a frozen reference or the sampling policy answers with.  Differentiable in x and weight; the
+    (hidden a multiple of 8 over 64) without the logits in memory: what a frozen reference or the sampling policy answers with.  Differentiable in x and weight; the
     backward computes the logits again, so where memory does not matter and most rows count ``log_probs`` on kept logits trains faster.
     Large products leave out the rows that do not count (prompts, padding).  The logits are fp32 sums that are not rounded to bf16
     on the way."""

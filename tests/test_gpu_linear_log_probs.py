@@ -303,10 +303,11 @@ def test_only_one_gradient_wanted_and_refusals(device):
         torch.autograd.grad(q.sum(), xs, create_graph=True)
 
 
-def test_streams_threads_and_graphs(device):
+@pytest.mark.parametrize("rows,hidden,vocab", [(200, 256, 5000), (700, 1000, 32777), (5, 2112, 20000)])
+def test_streams_threads_and_graphs(device, rows, hidden, vocab):
     from picotron_amd.functional import linear_log_probs
-    ready = [inputs(s, (3, 200), 256, 5000) for s in range(3)]
-    up = torch.randn(3, 200, generator=gen(9), device="cuda")
+    ready = [inputs(s, (3, rows), hidden, vocab, kept=(0.8, 1.0, 0.3)[s]) for s in range(3)]
+    up = torch.randn(3, rows, generator=gen(9), device="cuda")
 
     def run(x, w, t):
         x, w = x.detach().requires_grad_(), w.detach().requires_grad_()
