@@ -101,14 +101,14 @@ struct Gather {
 };
 
 // The target's logit joins what was gathered of the others, and its log-probability.  Where it is the largest that is -ln(1 + the others), which keeps its relative
-// accuracy however certain the token is; a sum that held the 1 from the beginning would have lost it.
+// accuracy however certain the token is; a sum that held the 1 from the beginning would have lost it.  (p - 1 there is 0, or not a number where the target is +inf.)
 template <bool kEntropy>
 __device__ __forceinline__ float with_target(Gather<kEntropy>& g, float xt, float k, float inv_t) {
   g.rise(fmaxf(g.zmax, xt), k);
   const float d = (xt - g.m) * k, p = fast_exp2(d), others = g.s;
   g.s = others + p;
   if constexpr (kEntropy) g.w = fmaf(p, fmaxf(d, kFloor), g.w);
-  return xt == g.m ? -log1pf(others) : (xt - g.m) * inv_t - logf(g.s);
+  return xt == g.m ? -log1pf(others + (p - 1.f)) : (xt - g.m) * inv_t - logf(g.s);
 }
 
 __device__ __forceinline__ float wave_max(float v) {

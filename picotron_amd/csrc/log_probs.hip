@@ -222,7 +222,7 @@ struct PolicyInputs {   // of a row, requested with its logits
 };
 __device__ __forceinline__ PolicyRow policy_row(const PolicyArgs& p, const PolicyInputs& in, float q, float H) {
   const float A = in.A, w = in.w;
-  const float ratio = p.old_lp.data != nullptr ? fast_exp2((q - in.old) * kLog2e) : 1.f;
+  const float ratio = p.old_lp.data != nullptr ? fast_exp2((q - in.old) * kLog2e) : q != q ? q : 1.f;   // (no finite loss beside a gradient of NaN)
   const float held = fminf(fmaxf(ratio, p.low), p.high), free = ratio * A, bound = held * A;
   PolicyRow r;
   // (written such that a NaN anywhere comes out)

@@ -1,0 +1,57 @@
+"""Log-probabilities of given tokens and their losses at the limits of what they take.  u = 2^-24."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32 = torch.bfloat16, torch.float32
+IGNORE = -100
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("vocab", [1, 9, 700, 49153, 140003])
+def test_a_target_of_plus_infinity_is_not_a_number(device, dtype, vocab):
+    """inf - inf has no value, in every form and however the others look; the other rows do not notice."""
+    from picotron_amd.functional import log_probs, policy_loss, preference_loss
+    g = gen(vocab)
+    clean = (torch.randn(2, 4, vocab, generator=g, device="cuda") * 2).to(dtype)
+    t = torch.randint(0, vocab, (2, 4), generator=g, device="cuda")
+    x = clean.clone()
+    x[0, 1, t[0, 1]] = float("inf")                                     # the target alone
+    x[0, 2] = -float("inf")
+    x[0, 2, t[0, 2]] = float("inf")                                     # beside nothing
+    x[1, 3] = float("inf")                                              # among others of its kind
+    bad = torch.zeros(2, 4, dtype=torch.bool, device="cuda")
+    bad[0, 1] = bad[0, 2] = bad[1, 3] = True
+    A = torch.randn(2, 4, generator=g, device="cuda")
+    want = log_probs(clean, t)
+
+    def rows(q, what):      # (each form is within 2^-16 + 4 u of the definition)
+        assert torch.equal(q.isnan(), bad), what
+        assert ((q - want)[~bad].abs() <= 2 ** -15 + 2 ** -21 * want[~bad].abs()).all(), what
+    for entropy in (False, True):
+        y = x.clone().requires_grad_()
+        out = log_probs(y, t, entropy=entropy)
+        out = out if entropy else (out,)
+        rows(out[0], "log_probs")
+        assert not entropy or torch.equal(out[1].isnan(), bad)
+        (d,) = torch.autograd.grad(out, y, [torch.ones_like(o) for o in out])
+        assert torch.equal(d.isnan().any(-1), bad)
+    for ent in (0.0, 0.01):
+        with torch.no_grad():
+            loss, q = policy_loss(x, t, A, entropy_coef=ent)
+        rows(q, "policy_loss without a gradient")
+        y = x.clone().requires_grad_()
+        again, q = policy_loss(y, t, A, entropy_coef=ent)
+        assert loss.isnan() and again.isnan()
+        rows(q, "policy_loss")
+        (d,) = torch.autograd.grad(again, y)
+        assert torch.equal(d.isnan().any(-1), bad)
+    loss, seq = preference_loss(x, t)
+    assert loss.isnan() and seq.isnan().all()
+    loss, seq = preference_loss(torch.cat([clean[:1], x[:1]]), torch.cat([t[:1], t[:1]]))
+    assert loss.isnan() and seq.isnan().tolist() == [False, True]
