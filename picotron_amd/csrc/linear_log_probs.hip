@@ -52,19 +52,17 @@ __device__ __forceinline__ f32x2 score(f32x4 (&v)[J], int h, int cols, float k) 
 #pragma unroll
     for (int e = 0; e < 4; ++e) m = fmaxf(m, v[j][e]);
   m = group_max(m);
-  // D as logits k - max k, an instruction less than the difference first (exponentials and what leads to them are the tile's end): all D are off by the rounding of
-  // max k, which the sum is multiplied free of (2^-r = 1 - r ln2, r under 2^-16)
-  const float mk = m == -INFINITY ? 0.f : m * k, r = m == -INFINITY ? 0.f : fmaf(m, k, -mk);
+  // (the difference first: max k is off by up to its last bit, and so would all D be, which at a low temperature is more than a whole one)
+  const float base = m == -INFINITY ? 0.f : m;
   float s = 0.f;
 #pragma unroll
   for (int j = 0; j < J; ++j) {
     float part = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) part += fast_exp2(fmaf(v[j][e], k, -mk));
+    for (int e = 0; e < 4; ++e) part += fast_exp2((v[j][e] - base) * k);
     s += part;
   }
-  s = group_sum(s);
-  return {m, fmaf(-r * kLn2, s, s)};
+  return {m, group_sum(s)};
 }
 // the target's logit to `to`, where its column is one of these (nearly always none of 16 rows' is); t: the target, two words
 template <int J>
@@ -365,11 +363,11 @@ __global__ __launch_bounds__(kJoinRows * kSlices) void join_kernel(const f32x2* 
 }
 
 // ---- backward
-// a row as the epilogue needs it: p_j = 2^(k z_j - lse2), lse2 = k max + log2 S; g = the gradient of its log-probability over T
-// (0 where the row does not count, whatever its logits hold); the target's column
+// a row as the epilogue needs it: p_j = 2^(k (z_j - max) - log2 S) (k max + log2 S as one number would be off by up to its last bit, and so would all p be); g = the
+// gradient of its log-probability over T; the target's column, -1 where the row does not count (its gradient is 0, whatever its logits hold)
 struct GradRow {
-  float lse2, g;
-  int target, counts;
+  float max, log2_s, g;
+  int target;
 };
 __global__ void grad_rows_kernel(const f32x2* __restrict__ max_sum, const float* __restrict__ dlog_probs, const int64_t* __restrict__ targets,
                                  GradRow* __restrict__ out, const int* __restrict__ position, const int* __restrict__ count, int M, int vocab, float k, float inv_t,
@@ -377,12 +375,12 @@ __global__ void grad_rows_kernel(const f32x2* __restrict__ max_sum, const float*
   const int row = blockIdx.x * blockDim.x + threadIdx.x;
   if (row >= M) return;
   const int at = position != nullptr ? position[row] : row;
-  if (count != nullptr && row >= *count && row < kLeastRows) out[row] = {0.f, 0.f, -1, 0};   // (behind the rows that are put together)
+  if (count != nullptr && row >= *count && row < kLeastRows) out[row] = {0.f, 0.f, 0.f, -1};   // (behind the rows that are put together)
   if (at < 0) return;
   const int64_t t = targets[row];
   const bool counts = t != ignore_index && t >= 0 && t < vocab && dlog_probs[row] != 0.f;
   const f32x2 ms = max_sum[row];
-  out[at] = {fmaf(ms[0], k, log2f(ms[1])), counts ? dlog_probs[row] * inv_t : 0.f, counts ? static_cast<int>(t) : -1, counts};
+  out[at] = {ms[0], log2f(ms[1]), counts ? dlog_probs[row] * inv_t : 0.f, counts ? static_cast<int>(t) : -1};
 }
 
 struct GradParams : LargeParams {
@@ -428,8 +426,8 @@ struct GradTile {
       for (int j = 0; j < J; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float p = fast_exp2(fmaf(acc[i][j][e], k, -r.lse2)), d = r.g * ((at == 16 * j + e ? 1.f : 0.f) - p);
-          acc[i][j][e] = r.counts ? d : 0.f;
+          const float p = fast_exp2(fmaf(acc[i][j][e] - r.max, k, -r.log2_s)), d = fmaf(-r.g, p, at == 16 * j + e ? r.g : 0.f);
+          acc[i][j][e] = r.target >= 0 ? d : 0.f;
         }
       if (cols < 16 * J) {   // zeros in the columns that pad a row
         const int left = hidden(cols - 4 * h);
