@@ -511,12 +511,16 @@ int pico_linear_log_probs_fwd(const void* x, const void* w, const int64_t* targe
                               int64_t hidden, int64_t vocab, int64_t ldx, int64_t ldw, float temperature, int64_t ignore_index,
                               void* workspace, int64_t workspace_bytes, void* stream);
 /* The gradient of sum over rows of dlog_probs * log_probs with respect to x w^T, bf16 [rows, vocab] with row pitch ldd = vocab rounded up to a multiple
- * of 8 (zeros in the columns behind vocab): the products dlogits w and dlogits^T x of it are the gradients of x and w.  The logits are computed again.
+ * of 8 (zeros in the columns behind vocab): the products dlogits w and dlogits^T x of it are the gradients of x and w.  The logits are computed again.  Rows that
+ * do not count are 0, whatever x holds there; the product with x itself wants them to be finite (pico_linear_log_probs_counted).
  * workspace: 16 bytes per row, 16-byte aligned.
  */
 int pico_linear_log_probs_dlogits(const void* x, const void* w, const int64_t* targets, const float* max_sum, const float* dlog_probs,
                                   void* dlogits, int64_t rows, int64_t hidden, int64_t vocab, int64_t ldx, int64_t ldw, int64_t ldd,
                                   float temperature, int64_t ignore_index, void* workspace, int64_t workspace_bytes, void* stream);
+/* out = x with zeros in the rows whose target does not count: bf16 [rows, hidden], out contiguous, both aligned to 16 bytes; hidden and the pitch ldx multiples of 8. */
+int pico_linear_log_probs_counted(const void* x, const int64_t* targets, void* out, int64_t rows, int64_t hidden, int64_t vocab, int64_t ldx,
+                                  int64_t ignore_index, void* stream);
 /* dw = d^T x of few rows (1 .. 32): d [rows, out] (pitch ldd) and x [rows, in] (pitch ldx) bf16, dw [out, in] bf16, contiguous and aligned to 16 bytes; in a
  * multiple of 8. */
 int pico_weight_grad_few(const void* d, const void* x, void* dw, int64_t rows, int64_t out, int64_t in, int64_t ldd, int64_t ldx, void* stream);

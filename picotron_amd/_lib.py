@@ -109,6 +109,7 @@ SIGNATURES = {
     "pico_preference_loss_fwd": (c_int, _ROWS + [_P, c_float, c_float, c_int, c_float, _P, _P, _P, _P, _P, _P, _I64, _P]),
     "pico_linear_log_probs_workspace_bytes": (_I64, [_I64] * 3),
     "pico_linear_log_probs_fwd": (c_int, [_P] * 5 + [_I64] * 5 + [c_float, _I64, _P, _I64, _P]),
+    "pico_linear_log_probs_counted": (c_int, [_P] * 3 + [_I64] * 5 + [_P]),
     "pico_weight_grad_few": (c_int, [_P] * 3 + [_I64] * 5 + [_P]),
     "pico_linear_log_probs_bwd_workspace_bytes": (_I64, [_I64] * 3),
     "pico_linear_log_probs_bwd": (c_int, [_P] * 7 + [_I64] * 4 + [c_float, _I64, _P, _I64, _P]),

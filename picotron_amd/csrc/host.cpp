@@ -1666,13 +1666,19 @@ struct LinearLogProbs : torch::autograd::Function<LinearLogProbs> {
     check(pico_linear_log_probs_dlogits(ptr(a), ptr(b), t.data_ptr<int64_t>(), fptr(s[3]), fptr(dlp), ptr(dz), M, a.size(1), N, pitch(a), pitch(b), ldd,
                                         temperature, ignore, ptr(ws), M * 16, stream_now()));
     const Tensor d = dz.narrow(1, 0, N);
+    const bool wants_w = ctx->needs_input_grad(1);
+    Tensor counted;   // (0 times what a row that does not count holds need not be 0)
+    if (wants_w) {
+      counted = at::empty({M, K}, a.options());
+      check(pico_linear_log_probs_counted(ptr(a), t.data_ptr<int64_t>(), ptr(counted), M, K, N, pitch(a), ignore, stream_now()));
+    }
     // The gradient of w from few rows, a short contraction that writes much, where the rules for products would leave it to the GEMM library.  us, there and here: up
     // to 32 rows see the kernel; [32000 x 4096] from 72 rows 99, 62, from 104 103, 58, [49152 x 2112] from 96 175, 57; from 128 on the rules choose that kernel.
-    const bool wants_w = ctx->needs_input_grad(1), short_walk = M > 0 && M < 128 && wants_w && !stays_with_torch(dz, a) &&
-                                                                product_route(Product::TN, product_sizes(dz, a, Product::TN)).kernel == ProductRoute::Library;
-    const bool few = short_walk && M <= 32, large = short_walk && M > 64 && ldd * K >= 1 << 25 && pico_product_large_takes(ldd, K, M, ldd, pitch(a), 1, 1, 1);
+    const bool short_walk = M > 0 && M < 128 && wants_w && !stays_with_torch(dz, counted) &&
+                            product_route(Product::TN, product_sizes(dz, counted, Product::TN)).kernel == ProductRoute::Library;
+    const bool few = short_walk && M <= 32, large = short_walk && M > 64 && ldd * K >= 1 << 25 && pico_product_large_takes(ldd, K, M, ldd, K, 1, 1, 1);
     if (both_wanted && !few && !large && ldd == N) {
-      Gradients both = gradients(d, b, a);
+      Gradients both = gradients(d, b, counted);
       r[0] = both.dx.view(x.sizes());
       r[1] = both.dw;
       return r;
@@ -1680,9 +1686,9 @@ struct LinearLogProbs : torch::autograd::Function<LinearLogProbs> {
     if (ctx->needs_input_grad(0)) r[0] = product(d, b, Product::NN).view(x.sizes());
     if (few) {
       r[1] = at::empty({N, K}, a.options());
-      check(pico_weight_grad_few(ptr(d), ptr(a), ptr(r[1]), M, N, K, ldd, pitch(a), stream_now()));
+      check(pico_weight_grad_few(ptr(d), ptr(counted), ptr(r[1]), M, N, K, ldd, K, stream_now()));
     } else if (wants_w) {   // (with the zeros behind the vocabulary the rows are whole pieces of 16 bytes, and the rows of dw that they make are left out)
-      r[1] = (large ? product(dz, a, Product::TN, product_sizes(dz, a, Product::TN), {ProductRoute::Large, 256, 256, 0, 1, 0}) : product(dz, a, Product::TN)).narrow(0, 0, N);
+      r[1] = (large ? product(dz, counted, Product::TN, product_sizes(dz, counted, Product::TN), {ProductRoute::Large, 256, 256, 0, 1, 0}) : product(dz, counted, Product::TN)).narrow(0, 0, N);
     }
     return r;
   }

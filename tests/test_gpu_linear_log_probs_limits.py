@@ -50,3 +50,29 @@ def test_temperatures_that_leave_the_largest_logits_only(device, rows, hidden, v
     for got, want, bound in ((dx, d @ wd, dd @ wd.abs() + 2 ** -10 * (d.abs() @ wd.abs())), (dw, d.t() @ xd, dd.t() @ xd.abs() + 2 ** -10 * (d.abs().t() @ xd.abs()))):
         over = (got.double() - want).abs() - bound - 2 ** -8 * want.abs() - 1e-37
         assert not got.isnan().any() and (over <= 0).all(), over.max().item()
+
+
+@pytest.mark.parametrize("rows,hidden,vocab", [(2, 128, 1000), (4, 2112, 20000), (32, 2048, 16001), (40, 128, 600), (64, 4096, 2049), (100, 2112, 49152), (127, 4096, 32001), (300, 576, 1003),
+                                               (600, 576, 2000), (2000, 4096, 8192), (1503, 2048, 16385)])
+@pytest.mark.parametrize("wanted", ["both", "weight", "x"])
+def test_rows_that_do_not_count_may_hold_anything(device, rows, hidden, vocab, wanted):
+    """NaN and infinities in hidden states whose target does not count: the same bits of both gradients as beside ordinary ones, in every product that may take them."""
+    from picotron_amd.functional import linear_log_probs
+    g = gen(rows)
+    x = torch.randn(rows, hidden, generator=g, device="cuda").to(BF16)
+    w = (torch.randn(vocab, hidden, generator=g, device="cuda") * 0.1).to(BF16)
+    t = torch.randint(0, vocab, (rows,), generator=g, device="cuda")
+    r = torch.arange(rows, device="cuda")
+    t = torch.where(r % 4 == 1, IGNORE, torch.where(r % 4 == 3, vocab + r, t))
+    a = torch.randn(rows, generator=g, device="cuda")
+    out = []
+    for fill in (None, float("nan"), float("inf")):
+        y = x if fill is None else torch.where((r % 2 == 1)[:, None], fill, x)
+        y, v = y.detach().clone().requires_grad_(wanted != "weight"), w.clone().requires_grad_(wanted != "x")
+        out.append(torch.autograd.grad(linear_log_probs(y, v, t), [p for p in (y, v) if p.requires_grad], a))
+    for clean, *others in zip(*out):
+        assert bool(clean.any()) and not clean.isnan().any()
+        for other in others:
+            assert torch.equal(clean, other)
+    if wanted != "weight":
+        assert not out[1][0][r % 2 == 1].any()
