@@ -55,3 +55,38 @@ def test_a_target_of_plus_infinity_is_not_a_number(device, dtype, vocab):
     assert loss.isnan() and seq.isnan().all()
     loss, seq = preference_loss(torch.cat([clean[:1], x[:1]]), torch.cat([t[:1], t[:1]]))
     assert loss.isnan() and seq.isnan().tolist() == [False, True]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("vocab", [700, 49152, 140003])
+def test_the_kl_term_next_to_the_reference(device, dtype, vocab):
+    """exp(d) - 1 - d, d = ref - q, keeps its relative accuracy however near the policy is to its reference, and so does its slope.  Near 0: some roundings of a sum whose first term
+    is the largest.  From |d| = 1/2 on: exp(d) is off by (|d| + 2) u of itself, which is under 64 u of exp(d) - 1 - d.  With the factors: 2^-17.  (The kernels' own q, which ref - q is
+    taken with without a rounding.)  The gradient: the same of a, and the usual 2^-15 |a| p + 2^-21 |a| at the target, and one rounding."""
+    from picotron_amd.functional import policy_loss
+    g = gen(vocab)
+    d = torch.tensor([0.0, 1e-6, -1e-6, 1e-5, -1e-5, 1e-4, -1e-4, 3e-4, 1e-3, -1e-3, 0.01, -0.01, 0.1, -0.1, 0.3, -0.3, 0.49, -0.49, 0.51, -0.51, 1.0, -1.0, 5.0, -5.0], device="cuda")[None]
+    S = d.size(1)
+    x = (torch.randn(1, S, vocab, generator=g, device="cuda") * 2).to(dtype)
+    t = torch.randint(0, vocab, (1, S), generator=g, device="cuda")
+    x.scatter_(2, t[..., None], 6.0)
+    none = torch.zeros(1, S, device="cuda")
+    p = torch.softmax(x.double(), -1)
+    hot = torch.zeros_like(p).scatter_(-1, t[..., None], 1.0)
+    for grad in (False, True):
+        y = x.clone().requires_grad_(grad)
+        q = policy_loss(y, t, none)[1]
+        ref = q + d
+        far = ref.double() - q.double()
+        grow = torch.expm1(far)
+        want = 0.25 * (grow - far)
+        for i in range(S):
+            w = none.clone()
+            w[0, i] = 1.0
+            loss, again = policy_loss(y, t, none, ref_log_probs=ref, weights=w, kl_coef=0.25)
+            assert torch.equal(again, q) and loss.item() >= 0.0
+            assert abs(loss.item() - want[0, i].item()) <= 2 ** -17 * want[0, i].item() + 1e-37, (grad, i, loss.item(), want[0, i].item())
+    (dx,) = torch.autograd.grad(policy_loss(y, t, none, ref_log_probs=ref, weights=torch.ones(1, 1, device="cuda"), kl_coef=0.25)[0], y)
+    a = (-0.25 * grow)[..., None]
+    over = (dx.double() - a * (hot - p)).abs() - (torch.finfo(dtype).eps / 2 + 2 ** -17) * (a * (hot - p)).abs() - a.abs() * (2 ** -15 * p + 2 ** -21 * hot) - 1e-37
+    assert (over <= 0).all(), over.max().item()
