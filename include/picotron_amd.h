@@ -473,7 +473,7 @@ int pico_log_probs_bwd(const pico_logits* logits, const pico_tokens* targets, co
  * and loss[0] = scale * sum of weight * l, or, where weights are not given, scale * the mean of l over the rows that count (0 where none does).
  * old_log_probs not given: the policy's own (ratio 1, gradient -A).  All but the logits are constants.  Where both sides of the minimum are equal
  * the gradient is the first's.
- * log_probs (q), losses (weight * l): fp32 [batch, seq].  With dlogits the gradient for an upstream gradient of 1 is written in the same call, and
+ * log_probs (q), losses (what a row adds to loss[0]): fp32 [batch, seq].  With dlogits the gradient for an upstream gradient of 1 is written in the same call, and
  * `saved` ([batch, seq] each, max_sum [batch, seq, 2]; entropy and dentropy with an entropy term only) is what pico_log_probs_bwd needs for another
  * one.  inv_count: one device float, scratch.
  */

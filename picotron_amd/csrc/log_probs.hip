@@ -410,12 +410,13 @@ __device__ __forceinline__ double wave_sum64(double v) {
   return v;
 }
 
-// count: inv_count = scale / max(rows that count, 1); with `loss`: the sum of the losses, times that where they are not weighted yet
-__global__ __launch_bounds__(kSumThreads) void policy_sum_kernel(const TokenArgs targets, const float* __restrict__ losses, float* __restrict__ loss,
+// count: inv_count = scale / max(rows that count, 1); with `loss`: the sum of the losses, times that where they are not weighted yet, and so are they then
+__global__ __launch_bounds__(kSumThreads) void policy_sum_kernel(const TokenArgs targets, float* __restrict__ losses, float* __restrict__ loss,
                                                                  float* __restrict__ inv_count, float scale, int count, int unweighted,
                                                                  int64_t rows, int seq, int vocab, int64_t ignore_index) {
   __shared__ double red_s[kSumWaves];
   __shared__ int red_n[kSumWaves];
+  __shared__ float factor;
   double sum = 0;
   int n = 0;
   constexpr int U = 8;   // rows requested together
@@ -447,6 +448,18 @@ __global__ __launch_bounds__(kSumThreads) void policy_sum_kernel(const TokenArgs
     const float inv = scale / static_cast<float>(all > 0 ? all : 1);
     if (count) *inv_count = inv;
     if (loss != nullptr) *loss = static_cast<float>(unweighted ? total * inv : total);
+    factor = inv;
+  }
+  if (loss == nullptr || !unweighted) return;
+  __syncthreads();
+  const float by = factor;
+  for (int64_t first = threadIdx.x; first < rows; first += U * kSumThreads) {
+    float l[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) l[u] = first + u * kSumThreads < rows ? losses[first + u * kSumThreads] : 0.f;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (first + u * kSumThreads < rows) losses[first + u * kSumThreads] = l[u] * by;
   }
 }
 

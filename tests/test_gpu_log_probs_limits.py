@@ -90,3 +90,42 @@ def test_the_kl_term_next_to_the_reference(device, dtype, vocab):
     a = (-0.25 * grow)[..., None]
     over = (dx.double() - a * (hot - p)).abs() - (torch.finfo(dtype).eps / 2 + 2 ** -17) * (a * (hot - p)).abs() - a.abs() * (2 ** -15 * p + 2 ** -21 * hot) - 1e-37
     assert (over <= 0).all(), over.max().item()
+
+
+@pytest.mark.parametrize("rows", [(1, 1), (3, 5), (2, 1025), (5, 2000)])
+@pytest.mark.parametrize("weighted", [False, True])
+def test_losses_are_what_the_rows_add_to_the_loss(device, rows, weighted):
+    """pico_policy_loss_fwd with and without a gradient: the same numbers per row (a logits' statistics in another order: 2^-14 of each, as for the loss), whose sum the loss is
+    (rounded once more each: 2^-22)."""
+    import ctypes
+    from picotron_amd import _lib
+    lib, g, V = _lib.lib(), gen(7), 700
+    B, S = rows
+    x = (torch.randn(B, S, V, generator=g, device="cuda") * 2).to(BF16)
+    t = torch.randint(0, V, rows, generator=g, device="cuda")
+    t[0, ::3] = IGNORE if B * S > 1 else 5
+    A, old, w = (torch.rand(rows, generator=g, device="cuda") + 0.5 for _ in range(3))
+    q = torch.log_softmax(x.double(), -1).gather(-1, t.clamp(min=0)[..., None])[..., 0]
+    old = (q + old - 1.0).float()
+    n = t != IGNORE
+    ratio = (q - old.double()).exp()
+    want = -torch.minimum(ratio * A, ratio.clamp(0.8, 1.2) * A) * (w.double() * 1.5 if weighted else 1.5 / max(int(n.sum()), 1))
+    want = torch.where(n, want, 0.0)
+
+    def P(v):
+        return ctypes.c_void_p(v.data_ptr())
+
+    def per_row(v):
+        return _lib.PerRow(v.data_ptr(), S, 1)
+    none = _lib.PerRow(None, 0, 0)
+    z = _lib.Logits(x.data_ptr(), B, S, V, S * V, V, _lib.PICO_BF16, 0)
+    p = _lib.Policy(per_row(A), per_row(old), none, per_row(w) if weighted else none, 0.2, 0.2, 0.0, 0.0, 1.5)
+    for grad in (False, True):
+        loss, lp, losses, count = (torch.full((m,), 7.0, device="cuda") for m in (1, B * S, B * S, 1))
+        ms, dlp, d = torch.empty(2 * B * S, device="cuda"), torch.empty(B * S, device="cuda"), torch.empty_like(x)
+        saved = _lib.PolicySaved(ms.data_ptr(), dlp.data_ptr(), None, None)
+        assert lib.pico_policy_loss_fwd(ctypes.byref(z), ctypes.byref(per_row(t)), ctypes.byref(p), P(loss), P(lp), P(losses), P(count), ctypes.byref(saved) if grad else None,
+                                        P(d) if grad else None, S * V, V, 1.0, IGNORE, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0, lib.pico_last_error()
+        got = losses.view(rows).double()
+        assert ((got - want).abs() <= 2 ** -14 * want.abs()).all(), grad
+        assert abs(got.sum().item() - loss.item()) <= 2 ** -22 * want.abs().sum().item() + 2 ** -24 * abs(loss.item())
