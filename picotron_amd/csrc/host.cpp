@@ -1414,6 +1414,10 @@ Tensor per_token(const Tensor& targets, const Tensor& like, int64_t values = 1) 
 void refuse_second_order(const char* fn) {
   TORCH_CHECK(!at::GradMode::is_enabled(), fn, ": its gradient cannot be differentiated again (create_graph)");
 }
+// (none of these operators has a counterpart in torch to go to, and a tangent would be lost without a sign)
+void refuse_tangents(const char* fn, std::initializer_list<const Tensor*> inputs) {
+  for (const Tensor* t : inputs) TORCH_CHECK(!t->_fw_grad(0).defined(), fn, ": has no forward-mode derivative");
+}
 // d(logits) of `up` times (dlp q + dh H) per row, in `d` where that holds the gradient for a factor of 1 already
 Tensor log_probs_gradient(const TokenRows& r, const float* max_sum, const float* entropy, const pico_values& dlp, const pico_values& dh, const Tensor& up, Tensor d,
                           double temperature, int64_t ignore_index) {
@@ -1460,6 +1464,7 @@ struct LogProbs : torch::autograd::Function<LogProbs> {
   }
 };
 variable_list log_probs(const Tensor& logits, const Tensor& targets, int64_t ignore_index, double temperature, bool entropy) {
+  refuse_tangents("log_probs", {&logits});
   if (!records({&logits})) return LogProbs::run(logits, targets, ignore_index, temperature, entropy, nullptr);
   return LogProbs::apply(logits, targets, ignore_index, temperature, entropy);
 }
@@ -1547,6 +1552,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
 std::pair<Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& targets, const Tensor& advantages, const OptTensor& old_lp, const OptTensor& ref_lp,
                                       const OptTensor& weights, double clip_low, double clip_high, double kl_coef, double entropy_coef, int64_t ignore_index,
                                       double temperature, double scale) {
+  refuse_tangents("policy_loss", {&logits});
   const variable_list out = records({&logits})
       ? PolicyLoss::apply(logits, targets, advantages, old_lp, ref_lp, weights, clip_low, clip_high, kl_coef, entropy_coef, ignore_index, temperature, scale)
       : PolicyLoss::run(logits, targets, advantages, old_lp, ref_lp, weights, {clip_low, clip_high, kl_coef, entropy_coef, temperature, scale, ignore_index}, nullptr);
@@ -1605,6 +1611,7 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
 };
 std::pair<Tensor, Tensor> preference_loss(const Tensor& logits, const Tensor& targets, const OptTensor& ref_lp, double beta, double smoothing, bool average,
                                           int64_t ignore_index, double scale) {
+  refuse_tangents("preference_loss", {&logits});
   const variable_list out = records({&logits}) ? PreferenceLoss::apply(logits, targets, ref_lp, beta, smoothing, average, ignore_index, scale)
                                                : PreferenceLoss::run(logits, targets, ref_lp, beta, smoothing, average, ignore_index, scale, nullptr);
   return {out[0], out[1]};
@@ -1694,6 +1701,7 @@ struct LinearLogProbs : torch::autograd::Function<LinearLogProbs> {
   }
 };
 Tensor linear_log_probs(const Tensor& x, const Tensor& w, const Tensor& targets, int64_t ignore_index, double temperature) {
+  refuse_tangents("linear_log_probs", {&x, &w});
   if (!records({&x, &w})) return LinearLogProbs::run(x, w, targets, ignore_index, temperature, nullptr);
   return LinearLogProbs::apply(x, w, targets, ignore_index, temperature);
 }

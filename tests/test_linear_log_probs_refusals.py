@@ -1,8 +1,9 @@
-"""What the copy of the hidden states that count refuses, before anything is launched (no GPU needed)."""
+"""What the copy of the hidden states that count refuses, and forward-mode tangents, before anything is launched (no GPU needed)."""
 import ctypes
 import os
 
 import pytest
+import torch
 
 
 @pytest.fixture(scope="module")
@@ -27,3 +28,29 @@ def test_rows_that_count(lib):
     for over in (dict(x=4104), dict(t=4100), dict(out=4098)):
         assert call(**over) == -4, over
     assert call(rows=0, x=None, t=None, out=None) == 0
+
+
+def forward_mode(device):
+    from torch.autograd import forward_ad
+
+    from picotron_amd.functional import linear_log_probs, log_probs, policy_loss, preference_loss
+    t = torch.zeros(2, 3, dtype=torch.long, device=device)
+    A = torch.zeros(2, 1, device=device)
+    with forward_ad.dual_level():
+        for grad in (False, True):
+            x, w = torch.zeros(2, 3, 128, dtype=torch.bfloat16, device=device), torch.zeros(40, 128, dtype=torch.bfloat16, device=device)
+            dual, wdual = (forward_ad.make_dual(v.requires_grad_(grad), torch.ones_like(v)) for v in (x, w))
+            for call in (lambda: log_probs(dual, t), lambda: log_probs(dual, t, entropy=True), lambda: policy_loss(dual, t, A), lambda: preference_loss(dual, t),
+                         lambda: linear_log_probs(dual, w, t), lambda: linear_log_probs(x, wdual, t)):
+                with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                    call()
+
+
+def test_forward_mode_tangents():
+    """They would be lost without a sign."""
+    forward_mode("cpu")
+
+
+@pytest.mark.gpu
+def test_forward_mode_tangents_on_the_gpu(device):
+    forward_mode(device)
