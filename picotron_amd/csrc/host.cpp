@@ -1361,8 +1361,10 @@ void check_tokens(const char* fn, const Tensor& x, const Tensor& targets) {
   TORCH_CHECK(x.dim() >= 1 && targets.sizes() == x.sizes().slice(0, x.dim() - 1), fn, ": targets must have one entry per row (got ", targets.sizes(), " for ", x.sizes(), ")");
   TORCH_CHECK(targets.device() == x.device(), fn, ": targets must be on ", x.device());
 }
-TokenRows token_rows(const char* fn, const Tensor& logits, const Tensor& targets) {
-  check_tokens(fn, logits, targets);
+Tensor as_it_is(const Tensor& t) { return t.is_neg() ? t.detach().resolve_neg() : t; }   // (not what torch negates when it reads it)
+TokenRows token_rows(const char* fn, const Tensor& given, const Tensor& targets) {
+  check_tokens(fn, given, targets);
+  const Tensor logits = as_it_is(given);
   TORCH_CHECK(logits.size(-1) == 1 || logits.stride(-1) == 1, fn, ": logits must have a unit stride on the vocabulary");
   TokenRows r;
   r.logits = logits.dim() == 3 ? logits : logits.dim() == 2 ? logits.unsqueeze(0) : logits.dim() == 1 ? logits.reshape({1, 1, -1}) : logits.flatten(0, -3);
@@ -1382,7 +1384,7 @@ RowValues row_values(const char* fn, const char* what, const Tensor& v, const Te
   TORCH_CHECK(v.is_floating_point(), fn, ": ", what, " must be a floating-point tensor");
   TORCH_CHECK(at::is_expandable_to(v.sizes(), targets.sizes()), fn, ": ", what, " must have a value per target or broadcast to ", targets.sizes(), " (got ", v.sizes(), ")");
   RowValues r;
-  r.t = v.scalar_type() == at::kFloat ? v : v.detach().to(at::kFloat);
+  r.t = as_it_is(v.scalar_type() == at::kFloat ? v : v.detach().to(at::kFloat));
   if (targets.dim() == 2 && r.t.dim() <= 2) {   // (the usual case, without a view on the way)
     auto stride = [&](int64_t from_last) { return r.t.dim() >= from_last && r.t.size(-from_last) != 1 ? r.t.stride(-from_last) : 0; };
     r.v = {static_cast<const float*>(r.t.data_ptr()), stride(2), stride(1)};
@@ -1531,7 +1533,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     const auto s = ctx->get_saved_variables();
     const c10::OptionalDeviceGuard device(s[0].device());
     const TokenRows r = token_rows("policy_loss", s[0], s[1]);
-    const Tensor up = g[0].to(at::kFloat).contiguous();
+    const Tensor up = as_it_is(g[0].to(at::kFloat)).contiguous();
     // a second backward through this node (retain_graph) gets a buffer of its own, and so does one that is captured without its forward: its replays would find
     // there what the one before left
     Tensor unit;
@@ -1573,7 +1575,7 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
       on_gpu(*ref_lp);
       TORCH_CHECK(ref_lp->is_floating_point() && ref_lp->dim() == 1 && ref_lp->size(0) == B && ref_lp->device() == logits.device(), fn,
                   ": ref_log_probs must hold one value per sequence (", B, ") on ", logits.device());
-      ref = ref_lp->detach().to(at::kFloat).contiguous();
+      ref = as_it_is(ref_lp->detach().to(at::kFloat)).contiguous();
     }
     const auto f32 = logits.options().dtype(at::kFloat);
     const int64_t n = targets.numel();
@@ -1605,7 +1607,7 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
     const c10::OptionalDeviceGuard device(s[0].device());
     const TokenRows r = token_rows("preference_loss", s[0], s[1]);
     const pico_values dlp = {fptr(s[2]) + 2 * s[1].numel(), 1, 0};   // (one for all of a sequence)
-    d[0] = log_probs_gradient(r, fptr(s[2]), nullptr, dlp, {nullptr, 0, 0}, g[0].to(at::kFloat).contiguous(), Tensor(), 1.0, ctx->saved_data["ignore"].toInt());
+    d[0] = log_probs_gradient(r, fptr(s[2]), nullptr, dlp, {nullptr, 0, 0}, as_it_is(g[0].to(at::kFloat)).contiguous(), Tensor(), 1.0, ctx->saved_data["ignore"].toInt());
     return d;
   }
 };
@@ -1621,8 +1623,8 @@ std::pair<Tensor, Tensor> preference_loss(const Tensor& logits, const Tensor& ta
 // gradient, which lives until the two products with it are done.
 struct LinearLogProbs : torch::autograd::Function<LinearLogProbs> {
   static int64_t pitch(const Tensor& m) { return m.size(0) > 1 ? m.stride(0) : m.size(1); }
-  static Tensor rows(const Tensor& t) {   // as the products take them
-    const Tensor m = t.dim() == 1 ? t.unsqueeze(0) : matrix(t);
+  static Tensor rows(const Tensor& given) {   // as the products take them
+    const Tensor t = as_it_is(given), m = t.dim() == 1 ? t.unsqueeze(0) : matrix(t);
     const bool fits = (m.size(1) == 1 || m.stride(1) == 1) && pitch(m) % 8 == 0 && pitch(m) >= m.size(1) && reinterpret_cast<uintptr_t>(m.data_ptr()) % 16 == 0;
     return fits ? m : m.clone(at::MemoryFormat::Contiguous);
   }
@@ -1655,7 +1657,7 @@ struct LinearLogProbs : torch::autograd::Function<LinearLogProbs> {
     const auto s = ctx->get_saved_variables();
     const Tensor &x = s[0], &w = s[1];
     const c10::OptionalDeviceGuard device(x.device());
-    const Tensor a = rows(x), b = rows(w), t = s[2].contiguous(), dlp = g[0].to(at::kFloat).contiguous();
+    const Tensor a = rows(x), b = rows(w), t = s[2].contiguous(), dlp = as_it_is(g[0].to(at::kFloat)).contiguous();
     const int64_t M = a.size(0), K = a.size(1), N = b.size(0), ldd = (N + 7) / 8 * 8;
     const auto temperature = static_cast<float>(ctx->saved_data["temperature"].toDouble());
     const int64_t ignore = ctx->saved_data["ignore"].toInt();

@@ -129,3 +129,35 @@ def test_losses_are_what_the_rows_add_to_the_loss(device, rows, weighted):
         got = losses.view(rows).double()
         assert ((got - want).abs() <= 2 ** -14 * want.abs()).all(), grad
         assert abs(got.sum().item() - loss.item()) <= 2 ** -22 * want.abs().sum().item() + 2 ** -24 * abs(loss.item())
+
+
+def test_lazily_negated_tensors(device):
+    """A view that torch negates when it is read (an imaginary part of a conjugate) gives what its values give."""
+    from picotron_amd.functional import linear_log_probs, log_probs, policy_loss, preference_loss
+    g = gen(12)
+
+    def negated(v):
+        return torch._neg_view(-v)
+
+    def value(v):
+        return torch.complex(v, -v).conj().imag          # strides of 2 on every axis
+    x = torch.randn(4, 6, 501, generator=g, device="cuda")
+    t = torch.randint(0, 501, (4, 6), generator=g, device="cuda")
+    A, old, ref, w, sums = (torch.randn(*s, generator=g, device="cuda") for s in ((4, 1), (4, 6), (4, 6), (6,), (4,)))
+    assert negated(x).is_neg() and value(A).is_neg() and torch.equal(value(A), A)
+    h, v = (torch.randn(*s, generator=g, device="cuda").to(BF16) for s in ((4, 6, 128), (501, 128)))
+    for turn in (negated, value):
+        want = [log_probs(x, t), *policy_loss(x, t, A, old, ref, w, kl_coef=0.1), *preference_loss(x, t, sums), linear_log_probs(h, v, t)]
+        z = negated(x)
+        got = [log_probs(z, t), *policy_loss(z, t, turn(A), turn(old), turn(ref), turn(w), kl_coef=0.1), *preference_loss(z, t, turn(sums)), linear_log_probs(negated(h), negated(v), t)]
+        for a, b in zip(want, got):
+            assert torch.equal(a, b)
+    y, z = x.clone().requires_grad_(), x.clone().requires_grad_()
+    for fn in (lambda s, n: log_probs(s, t), lambda s, n: policy_loss(s, t, n(A), n(old), n(ref), n(w), kl_coef=0.1)[0], lambda s, n: preference_loss(s, t, n(sums))[0]):
+        a, b = fn(y, lambda q: q), fn(torch._neg_view(-z), negated)
+        (da,), (db,) = (torch.autograd.grad(o.sum(), leaf) for o, leaf in ((a, y), (b, z)))
+        assert torch.equal(da, db)
+    hs, vs = h.clone().requires_grad_(), v.clone().requires_grad_()
+    want = torch.autograd.grad(linear_log_probs(hs, vs, t), (hs, vs), A.expand(4, 6))
+    got = torch.autograd.grad(linear_log_probs(negated(hs), negated(vs), t), (hs, vs), A.expand(4, 6))
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
