@@ -504,7 +504,8 @@ int pico_preference_loss_fwd(const pico_logits* logits, const pico_tokens* targe
  * sums (0 where the target does not count, as above).  max_sum: [rows, 2] fp32, what the gradient needs; may be NULL.  hidden must be a multiple of 8
  * over 64, the pitches multiples of 8, x and w aligned to 16 bytes; targets: [rows] contiguous.
  * workspace: pico_linear_log_probs_workspace_bytes(rows, hidden, vocab) bytes, 16-byte aligned (a twelfth of bf16 logits and as much as x; -1: too large).
- * Rows that do not count are left out of the product where that saves rounds of its tiles and x has no gaps between its rows.
+ * Rows that do not count are left out of the product where that saves rounds of its tiles and x has no gaps between its rows.  (The gradient of the logits, rows x vocab
+ * in bf16, is in memory in the backward, whichever of the calls below it is made of.)
  */
 int64_t pico_linear_log_probs_workspace_bytes(int64_t rows, int64_t hidden, int64_t vocab);
 int pico_linear_log_probs_fwd(const void* x, const void* w, const int64_t* targets, float* log_probs, float* max_sum, int64_t rows,

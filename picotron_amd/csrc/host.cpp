@@ -1682,7 +1682,9 @@ struct LinearLogProbs : torch::autograd::Function<LinearLogProbs> {
       check(pico_linear_log_probs_counted(ptr(a), t.data_ptr<int64_t>(), ptr(counted), M, K, N, pitch(a), ignore, stream_now()));
     }
     // The gradient of w from few rows, a short contraction that writes much, where the rules for products would leave it to the GEMM library.  us, there and here: up
-    // to 32 rows see the kernel; [32000 x 4096] from 72 rows 99, 62, from 104 103, 58, [49152 x 2112] from 96 175, 57; from 128 on the rules choose that kernel.
+    // to 32 rows see the kernel; [32000 x 4096] from 72 rows 99, 62, from 104 103, 58, [49152 x 2112] from 96 175, 57; from 128 on the rules choose that kernel, and up to 64
+    // its contraction is too short.  dw of 2^26 entries on, 65 to 127 rows: [32000 x 2048] 38 .. 63, 31 .. 34, [120000 x 1024] 117 .. 179, 58; of 2^23 to 2^25 entries the rules took none of 40
+    // sizes to the library ([32000 x 1032] 24 in the kernel that they choose, 40 in this one).
     const bool short_walk = M > 0 && M < 128 && wants_w && !stays_with_torch(dz, counted) &&
                             product_route(Product::TN, product_sizes(dz, counted, Product::TN)).kernel == ProductRoute::Library;
     const bool few = short_walk && M <= 32, large = short_walk && M > 64 && ldd * K >= 1 << 25 && pico_product_large_takes(ldd, K, M, ldd, K, 1, 1, 1);

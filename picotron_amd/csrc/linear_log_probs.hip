@@ -4,7 +4,9 @@
 //             results, there and back, for what would be 256 of bf16 logits), and picks the target's logit where its column passes; a second launch
 //             joins a row's partial results.
 //   backward: the product again (the logits were not kept), whose epilogue turns z into d(logits) = g ([j = t] - p_j) / T with the row's
-//             maximum and sum from the forward, bf16; the gradients of x and w are two more products, large ones over the rows that count only.
+//             maximum and sum from the forward; the gradients of x and w are two more products, where both are wanted large ones over the rows that count only.
+//             d(logits) lies in memory until they are done, rounded to bf16 (2^-8 of each entry, as the gradient of bf16 logits is): the matrix instructions take bf16, and an fp32
+//             entry would be two of them, each with products of its own.
 // The logits are the products' fp32 sums here, never rounded to bf16.
 #include <type_traits>
 #include "log_probs.h"
@@ -309,6 +311,8 @@ __global__ __launch_bounds__(kPackThreads) void pack_rows_kernel(const __bf16* _
   }
 }
 
+// (log S as a whole, with the target's own 1 in it: a nearly certain token's log-probability is off by 2^-24, not by 2^-16 of itself.  The target is not left out of a group's sum, where
+// its column would have to be told from 48 or 64 others.)
 // A workgroup joins the partial results of kJoinRows rows: a row's groups are dealt to kSlices threads.  3.3 us at 24 rows of 49152 (one partial result after the
 // other: 4.8), 7 at 4096; 8 rows of 128 slices take 0.4 us less at up to 32 rows, 3 more from 3000 on.
 constexpr int kJoinRows = 16, kSlices = 64;
@@ -455,6 +459,8 @@ struct CountedParams : LargeParams {
 };
 constexpr int kMostParts = 32;
 constexpr int64_t kMostPartial = 1 << 25;   // fp32 sums in parts: two rounds of tiles
+// (The product and the launch that sums the parts each find it for themselves, and find the same: over all numbers of tiles and bounds on q that can occur, cost rounded after each
+// operation, contracted and exact choose alike.)
 __device__ __forceinline__ int parts_of(int tiles, int n, int hidden) {
   int best = 1;
   float least = static_cast<float>((tiles + 255) / 256);

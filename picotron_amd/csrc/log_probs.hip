@@ -558,7 +558,15 @@ void with_threads(int64_t vocab, int vec, const Fn& fn) {
 }
 // Threads and pieces per thread of the kernel that holds a row of so many pieces; (0, 0): none does.  As few threads as can hold the row in four or eight pieces: a
 // barrier over fewer waves, and more rows on a CU.  6144 pieces in 1024 x 6, where two rows share a CU, [8, 1024, 49152] bf16 256 us, in 512 x 12 262; with an entropy
-// term the former has no registers left (12 bytes of scratch).
+// term the former has no registers left (12 bytes of scratch).  The long rows, us of 400 MB of logits (a copy: 162), without and with an entropy term, held here, in 1024
+// threads up to 8192 pieces (12288 for the last rung), and read twice:
+//   bf16  49160   147, 159 | 180, 195 | 181, 182      bf16 131072   160, 173 |    -     | 187, 189
+//   bf16  65536   151, 156 | 162, 176 | 179, 180      fp32  25000   144, 143 | 149, 157 | 179, 180
+//   bf16  65544   188, 221 | 187, 201 | 179, 180      fp32  32772   155, 161 | 160, 164 | 178, 179
+//   bf16  80000   179, 201 | 180, 191 | 180, 181      fp32  50000   152, 156 |    -     | 182, 183
+//   bf16 100000   168, 190 |    -     | 182, 185      fp32  65536   152, 152 |    -     | 182, 183
+// (1024 x 16 leaves one row on a CU, whose phases nothing overlaps: just past 8192 pieces of bf16 it loses 5 to 23 %.  Past 16384, read twice, 131080 bf16 187, 190, 128256 fp32
+// 227, 230.)
 template <bool kEntropy, typename Fn>
 void with_pieces(int64_t vocab, int vec, const Fn& fn) {
   const int64_t pieces = vocab / vec;

@@ -106,10 +106,12 @@ def log_probs(logits, targets, ignore_index: int = -100, temperature: float = 1.
 
 def linear_log_probs(x, weight, targets, ignore_index: int = -100, temperature: float = 1.0):
     """``log_probs(F.linear(x, weight), targets)`` for bf16 hidden states x [..., hidden] and vocabulary projection weight [vocab, hidden]
-    (hidden a multiple of 8 over 64) without the logits in memory: what a frozen reference or the sampling policy answers with.  Differentiable in x and weight; the
-    backward computes the logits again, so where memory does not matter and most rows count ``log_probs`` on kept logits trains faster.
-    Large products leave out the rows that do not count (prompts, padding).  The logits are fp32 sums that are not rounded to bf16
-    on the way."""
+    (hidden a multiple of 8 over 64) without the logits in memory: what a frozen reference or the sampling policy answers with.  The logits are fp32 sums that are
+    not rounded to bf16 on the way.  Large products leave out the rows that do not count (prompts, padding), whose hidden states may hold anything.
+
+    Differentiable in x and weight.  Nothing of the size of the logits lives between forward and backward, but the backward computes them again and holds their gradient while
+    it runs: rows * vocab * 2 bytes, rounded to bf16, as the gradient of bf16 logits is (and up to x in bf16 and fp32, or 128 MiB).  So where memory does not matter and most rows
+    count ``log_probs`` on kept logits trains faster.  The backward leaves out rows only where both gradients are wanted."""
     _check_targets("linear_log_probs", targets, weight.size(0), ignore_index)
     return _lib.host().linear_log_probs(x, weight, targets, ignore_index, temperature)
 

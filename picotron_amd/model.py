@@ -294,7 +294,7 @@ class FinalProjection(nn.Module):
 
     def log_probs(self, x, targets, ignore_index=-100, temperature=1.0):
         """Log-probabilities of the tokens `targets` under softmax(self(x) / temperature), fp32; for a bf16 projection without a
-        bias the logits stay out of memory (a hidden size that is a multiple of 8 over 64)."""
+        bias the logits stay out of the forward's memory (a hidden size that is a multiple of 8 over 64)."""
         if self.bias is not None or self.weight.dtype != torch.bfloat16 or x.dtype != torch.bfloat16 or x.size(-1) % 8 or x.size(-1) <= 64:
             return log_probs(self(x), targets, ignore_index, temperature)
         return linear_log_probs(x, self.weight, targets, ignore_index, temperature)
