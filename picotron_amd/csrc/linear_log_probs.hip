@@ -384,7 +384,8 @@ __global__ void grad_rows_kernel(const f32x2* __restrict__ max_sum, const float*
   const int64_t t = targets[row];
   const bool counts = t != ignore_index && t >= 0 && t < vocab && dlog_probs[row] != 0.f;
   const f32x2 ms = max_sum[row];
-  out[at] = {ms[0], log2f(ms[1]), counts ? dlog_probs[row] * inv_t : 0.f, counts ? static_cast<int>(t) : -1};
+  const float g = ms[1] > 0.f ? dlog_probs[row] * inv_t : NAN;   // (a row whose logits are no numbers: p is held to 0 .. 1 below)
+  out[at] = {ms[0], log2f(ms[1]), counts ? g : 0.f, counts ? static_cast<int>(t) : -1};
 }
 
 struct GradParams : LargeParams {
@@ -430,7 +431,8 @@ struct GradTile {
       for (int j = 0; j < J; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float p = fast_exp2(fmaf(acc[i][j][e] - r.max, k, -r.log2_s)), d = fmaf(-r.g, p, at == 16 * j + e ? r.g : 0.f);
+          // (p is 1 at most also where the forward, up to 32 rows, added a logit up in another order and the temperature makes much of the difference; a modifier of the exponential)
+          const float p = __builtin_amdgcn_fmed3f(fast_exp2(fmaf(acc[i][j][e] - r.max, k, -r.log2_s)), 0.f, 1.f), d = fmaf(-r.g, p, at == 16 * j + e ? r.g : 0.f);
           acc[i][j][e] = r.target >= 0 ? d : 0.f;
         }
       if (cols < 16 * J) {   // zeros in the columns that pad a row

@@ -76,3 +76,29 @@ def test_rows_that_do_not_count_may_hold_anything(device, rows, hidden, vocab, w
             assert torch.equal(clean, other)
     if wanted != "weight":
         assert not out[1][0][r % 2 == 1].any()
+
+
+@pytest.mark.parametrize("T", [1e-7, 1e-8, 1e-10, 1e-20])
+@pytest.mark.parametrize("rows,hidden,vocab", [(1, 4096, 3000), (7, 264, 1001), (32, 2048, 8192), (70, 128, 5003), (512, 4096, 8200)])
+def test_gradients_at_temperatures_under_the_logits_roundings(device, rows, hidden, vocab, T):
+    """A logit's rounding over T is more than any exponent holds, and the backward may add logits up in another order: probabilities stay under 1 and gradients finite.
+    (|d(logits)| <= |a| / T (1 + 2^-8), and with |w| <= 1 no sum of them leaves bf16.)  A row that is no number stays one."""
+    from picotron_amd.functional import linear_log_probs
+    g = gen(rows + hidden)
+    x = torch.randn(rows, hidden, generator=g, device="cuda").to(BF16)
+    w = (torch.randn(vocab, hidden, generator=g, device="cuda") * (2 / hidden ** 0.5)).clamp(-1, 1).to(BF16)
+    t = torch.randint(0, vocab, (rows,), generator=g, device="cuda")
+    a = torch.randn(rows, generator=g, device="cuda")
+    y, v = x.clone().requires_grad_(), w.clone().requires_grad_()
+    q = linear_log_probs(y, v, t, temperature=T)
+    assert q.isfinite().all() and (q <= 0).all()
+    dx, dw = torch.autograd.grad(q, (y, v), a)
+    assert dx.isfinite().all() and dw.isfinite().all()
+    bad = x.clone()
+    bad[rows // 2, 3] = float("nan")
+    y = bad.requires_grad_()
+    for temperature in (1.0, T):
+        q = linear_log_probs(y, v, t, temperature=temperature)
+        dx, dw = torch.autograd.grad(q, (y, v), a)
+        r = torch.arange(rows, device="cuda") == rows // 2
+        assert torch.equal(q.isnan(), r) and dx[r].isnan().all() and not dx[~r].isnan().any() and dw.isnan().all()
