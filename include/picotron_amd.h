@@ -535,6 +535,38 @@ int pico_linear_log_probs_bwd(const void* x, const void* w, const int64_t* targe
                               void* dx, void* dw, int64_t rows, int64_t hidden, int64_t vocab, int64_t ldw, float temperature,
                               int64_t ignore_index, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------ activations and weights in 8 bits
+ * No counterpart in the reference.  A row's values as e4m3, every 32 of them under one power-of-two scale:
+ *   data    e4m3 [rows, cols], contiguous, 16-byte aligned; cols a multiple of 32
+ *   scales  bytes [ceil(cols / 128), rows, 4], 4-byte aligned: byte (t, r, q) is that of columns 128 t + 32 q .. + 31 of row r and stands for
+ *           2^(byte - 127); 255: the block is NaN.  Bytes past the last column are written as 0.
+ * A block's scale is the smallest 2^e, e >= -127, for which its largest |value| / 2^e is at most 448; values are rounded to the nearest, ties to even.  A block
+ * with an infinity or a NaN becomes NaN as a whole.  rows * ceil(cols / 128) stays under 2^31.
+ */
+typedef struct pico_mx8 {
+  void* data;
+  void* scales;
+} pico_mx8;
+/* y = x in 8 bits: x [rows, cols] of `dtype` with row pitch x_ld (a multiple of 8 (bf16) / 4 (fp32), as all pitches here), 16-byte aligned. */
+int pico_mx8_quantize(const void* x, const pico_mx8* y, int64_t rows, int64_t cols, int64_t x_ld, int dtype, void* stream);
+/* The values that x stands for, in `dtype` (both hold them exactly from 2^-126 on; what was rounded up to 2^128 is infinite), with row pitch y_ld. */
+int pico_mx8_dequantize(const pico_mx8* x, void* y, int64_t rows, int64_t cols, int64_t y_ld, int dtype, void* stream);
+/* pico_rmsnorm_fwd (cast_then_scale = 0) whose output is written in 8 bits, from fp32, and in no other form: y [rows, hidden], hidden a multiple of 32
+ * up to 16384.  The backward is pico_rmsnorm_bwd, with the gradient of the values that y stands for. */
+int pico_rmsnorm_mx8_fwd(const void* x, const void* weight, const pico_mx8* y, float* rstd, const void* residual_in, void* residual_out,
+                         int64_t rows, int64_t hidden, float eps, int dtype, void* stream);
+/* silu(gate) * up into y (contiguous, `dtype`), y8, or both; gate8 and up8 (both or neither) take what pico_swiglu_mx8_bwd reads. */
+int pico_swiglu_mx8_fwd(const void* gate, const void* up, void* y, const pico_mx8* y8, const pico_mx8* gate8, const pico_mx8* up8,
+                        int64_t rows, int64_t cols, int64_t gate_ld, int64_t up_ld, int dtype, void* stream);
+/* Gradients of silu(gate) * up at the values that gate8 and up8 stand for; y (contiguous, may be NULL): silu(gate) * up of these values, for the
+ * gradient of the weight that it met. */
+int pico_swiglu_mx8_bwd(const void* dy, const pico_mx8* gate8, const pico_mx8* up8, void* dgate, void* dup, void* y, int64_t rows, int64_t cols,
+                        int64_t dy_ld, int64_t dgate_ld, int64_t dup_ld, int dtype, void* stream);
+/* c = a b^T, bf16 [M, N rounded up to a multiple of 8] (the columns from N on are written as 0), contiguous, 16-byte aligned, for a [M, K] and b
+ * [N, K].  workspace: pico_mx8_product_workspace_bytes bytes, 16-byte aligned (NULL where that is 0). */
+int64_t pico_mx8_product_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int pico_mx8_product(const pico_mx8* a, const pico_mx8* b, void* c, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------ optimizer step
  * replaces: torch.optim.AdamW(model.parameters(), lr).step()  train.py:204-209,240  for low-precision parameters
  *           with fp32 state: the reference keeps the AdamW state in the parameter dtype; here master weights and

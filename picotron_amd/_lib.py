@@ -62,8 +62,14 @@ class PolicySaved(Structure):
     _fields_ = [("max_sum", c_void_p), ("dlog_probs", c_void_p), ("entropy", c_void_p), ("dentropy", c_void_p)]
 
 
+class Mx8(Structure):
+    """Mirror of ``pico_mx8``."""
+    _fields_ = [("data", c_void_p), ("scales", c_void_p)]
+
+
 _P = c_void_p
 _I64 = c_int64
+_MX8 = POINTER(Mx8)
 _ROWS = [POINTER(Logits), POINTER(PerRow)]
 SIGNATURES = {
     "pico_version": (c_char_p, []),
@@ -114,6 +120,13 @@ SIGNATURES = {
     "pico_linear_log_probs_bwd_workspace_bytes": (_I64, [_I64] * 3),
     "pico_linear_log_probs_bwd": (c_int, [_P] * 7 + [_I64] * 4 + [c_float, _I64, _P, _I64, _P]),
     "pico_linear_log_probs_dlogits": (c_int, [_P] * 6 + [_I64] * 6 + [c_float, _I64, _P, _I64, _P]),
+    "pico_mx8_quantize": (c_int, [_P, _MX8, _I64, _I64, _I64, c_int, _P]),
+    "pico_mx8_dequantize": (c_int, [_MX8, _P, _I64, _I64, _I64, c_int, _P]),
+    "pico_rmsnorm_mx8_fwd": (c_int, [_P, _P, _MX8, _P, _P, _P, _I64, _I64, c_float, c_int, _P]),
+    "pico_swiglu_mx8_fwd": (c_int, [_P, _P, _P, _MX8, _MX8, _MX8] + [_I64] * 4 + [c_int, _P]),
+    "pico_swiglu_mx8_bwd": (c_int, [_P, _MX8, _MX8, _P, _P, _P] + [_I64] * 5 + [c_int, _P]),
+    "pico_mx8_product_workspace_bytes": (_I64, [_I64] * 3),
+    "pico_mx8_product": (c_int, [_MX8, _MX8, _P] + [_I64] * 3 + [_P, _I64, _P]),
     "pico_adamw": (c_int, [_P, _P, _P, c_int, _P, _P, _I64] + [ctypes.c_float] * 5 + [_I64, ctypes.c_float, _P]),
     "pico_adamw_lp": (c_int, [_P, _P, c_int, _P, _P, _I64, c_int, c_int] + [ctypes.c_float] * 5 + [_I64, ctypes.c_float, _P]),
     "pico_adamw_multi": (c_int, [c_int, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int] + [ctypes.c_float] * 5 + [_I64, ctypes.c_float, _P]),

@@ -14,6 +14,7 @@
 
 #include <array>
 #include <cstdlib>
+#include <functional>
 #include <mutex>
 #include <optional>
 #include <unordered_map>
@@ -1710,6 +1711,387 @@ Tensor linear_log_probs(const Tensor& x, const Tensor& w, const Tensor& targets,
   return LinearLogProbs::apply(x, w, targets, ignore_index, temperature);
 }
 
+// ------------------------------------------------------------------------------------------------ activations and weights in 8 bits
+// e4m3 [..., cols] and its scales [ceil(cols / 128), rows, 4] (pico_mx8)
+struct Mx8 {
+  Tensor data, scales;
+  bool defined() const { return data.defined(); }
+  pico_mx8 c() const { return {data.data_ptr(), scales.data_ptr()}; }
+  int64_t cols() const { return data.size(-1); }
+  int64_t rows() const { return scales.size(1); }
+};
+using Mx8Pair = std::pair<Tensor, Tensor>;
+using OptMx8 = std::optional<Mx8Pair>;
+
+void check_columns(const char* fn, const Tensor& t) {
+  TORCH_CHECK(t.dim() >= 1 && t.size(-1) >= 32 && t.size(-1) % 32 == 0, fn, ": the last axis must be a multiple of 32 (got ", t.sizes(), ")");
+}
+Mx8 mx8_empty(at::IntArrayRef sizes, const Tensor& like) {
+  const int64_t cols = sizes.back(), rows = c10::multiply_integers(sizes.slice(0, sizes.size() - 1));
+  return {at::empty(sizes, like.options().dtype(at::kFloat8_e4m3fn)), at::empty({(cols + 127) / 128, rows, 4}, like.options().dtype(at::kByte))};
+}
+Mx8 mx8_given(const char* fn, const Mx8Pair& p) {
+  const auto& [d, s] = p;
+  on_gpu(d);
+  TORCH_CHECK(d.scalar_type() == at::kFloat8_e4m3fn && d.is_contiguous(), fn, ": 8-bit data must be contiguous float8_e4m3fn (got ", d.scalar_type(), ")");
+  check_columns(fn, d);
+  const int64_t cols = d.size(-1), rows = d.numel() / cols;
+  TORCH_CHECK(s.scalar_type() == at::kByte && s.is_contiguous() && s.device() == d.device() && s.sizes() == at::IntArrayRef({(cols + 127) / 128, rows, 4}), fn,
+              ": the scales of ", d.sizes(), " must be contiguous uint8 [", (cols + 127) / 128, ", ", rows, ", 4] on ", d.device(), " (got ", s.sizes(), " on ", s.device(), ")");
+  return {d, s};
+}
+// [..., cols] as rows that the kernels take: one pitch, 16-byte aligned (a copy where that is not so)
+Rows mx8_rows(const Tensor& given) {
+  const Tensor t = as_it_is(given);
+  const int64_t vec = 16 / t.element_size();
+  if (one_pitch(t) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0) {
+    const Rows r = as_rows(t);
+    bool whole = r.rows <= 1;   // (one row; else its pitch is a stride, and an expanded axis has none)
+    for (int64_t i = t.dim() - 2; i >= 0 && !whole; --i)
+      if (t.size(i) != 1) {
+        whole = t.stride(i) >= r.cols && t.stride(i) % vec == 0;
+        break;
+      }
+    if (whole) return r.rows <= 1 ? Rows{r.t, r.rows, r.cols, r.cols} : r;
+  }
+  return as_rows(t.clone(at::MemoryFormat::Contiguous));
+}
+
+Mx8 mx8_quantized(const char* fn, const Tensor& x) {
+  on_gpu(x);
+  check_columns(fn, x);
+  const int dt = dtype_code(x, fn);
+  const c10::OptionalDeviceGuard device(x.device());
+  const Rows r = mx8_rows(x);
+  const Mx8 y = mx8_empty(x.sizes(), x);
+  const pico_mx8 c = y.c();
+  check(pico_mx8_quantize(ptr(r.t), &c, r.rows, r.cols, r.pitch, dt, stream_now()));
+  return y;
+}
+Tensor mx8_values(const Mx8& x, at::ScalarType dtype) {
+  const c10::OptionalDeviceGuard device(x.data.device());
+  const Tensor y = at::empty(x.data.sizes(), x.data.options().dtype(dtype));
+  const pico_mx8 c = x.c();
+  check(pico_mx8_dequantize(&c, ptr(y), x.rows(), x.cols(), x.cols(), dtype_code(y, "mx8_dequantize"), stream_now()));
+  return y;
+}
+// a [..., K] times b [N, K]^T, bf16
+Tensor mx8_product(const char* fn, const Mx8& a, const Mx8& b) {
+  TORCH_CHECK(b.data.dim() == 2 && a.cols() == b.cols() && a.data.device() == b.data.device(), fn, ": a weight of [out, ", a.cols(), "] on ", a.data.device(), " is wanted (got ", b.data.sizes(),
+              " on ", b.data.device(), ")");
+  const c10::OptionalDeviceGuard device(a.data.device());
+  const int64_t M = a.rows(), N = b.rows(), K = a.cols(), bytes = pico_mx8_product_workspace_bytes(M, N, K);
+  const auto bf16 = a.data.options().dtype(at::kBFloat16);
+  auto sizes = a.data.sizes().vec();
+  sizes.back() = N;
+  const Tensor y = at::empty(sizes, bf16), rounded_up = N % 8 == 0 ? y : at::empty({M, (N + 7) / 8 * 8}, bf16);
+  const Tensor ws = bytes > 0 ? at::empty({bytes}, bf16.dtype(at::kByte)) : Tensor();
+  const pico_mx8 ca = a.c(), cb = b.c();
+  check(pico_mx8_product(&ca, &cb, ptr(rounded_up), M, N, K, ptr(ws), bytes, stream_now()));
+  if (N % 8 != 0) y.view({M, N}).copy_(rounded_up.narrow(1, 0, N));
+  return y;
+}
+
+struct NormMx8Out {
+  Mx8 y;
+  Tensor rstd, sum;
+};
+NormMx8Out rmsnorm_mx8(const char* fn, const Tensor& x, const Tensor& weight, double eps, const OptTensor& residual, bool want_rstd) {
+  on_gpu(x);
+  on_gpu(weight);
+  on_gpu(residual);
+  check_columns(fn, x);
+  const int dt = dtype_code(x, fn);
+  const int64_t hidden = x.size(-1);
+  TORCH_CHECK(weight.dim() == 1 && weight.size(0) == hidden && weight.device() == x.device(), fn, ": the norm's weight must be [", hidden, "] on ", x.device(), " (got ", weight.sizes(), " on ",
+              weight.device(), ")");
+  const c10::OptionalDeviceGuard device(x.device());
+  const Tensor xc = as_it_is(x).contiguous(), w = as_it_is(weight).to(x.scalar_type()).contiguous();
+  Tensor res;
+  if (residual) {
+    TORCH_CHECK(residual->scalar_type() == x.scalar_type() && residual->sizes() == x.sizes() && residual->device() == x.device(), fn, ": residual must match x in dtype, shape and device");
+    res = as_it_is(*residual).contiguous();
+  }
+  NormMx8Out o;
+  o.y = mx8_empty(xc.sizes(), xc);
+  const int64_t rows = o.y.rows();
+  if (want_rstd) o.rstd = at::empty({rows}, xc.options().dtype(at::kFloat));
+  if (res.defined()) o.sum = at::empty(xc.sizes(), xc.options());
+  const pico_mx8 c = o.y.c();
+  check(pico_rmsnorm_mx8_fwd(ptr(xc), ptr(w), &c, fptr(o.rstd), ptr(res), ptr(o.sum), rows, hidden, static_cast<float>(eps), dt, stream_now()));
+  return o;
+}
+
+struct SwiGLUMx8Out {
+  Tensor y;
+  Mx8 y8, gate8, up8;
+};
+SwiGLUMx8Out swiglu_mx8(const char* fn, const Tensor& gate_up, bool packed, bool keep) {
+  on_gpu(gate_up);
+  TORCH_CHECK(gate_up.dim() >= 1 && gate_up.size(-1) >= 64 && gate_up.size(-1) % 64 == 0, fn, ": gate and up must each be a multiple of 32 wide (got ", gate_up.sizes(), ")");
+  const int dt = dtype_code(gate_up, fn);
+  const c10::OptionalDeviceGuard device(gate_up.device());
+  const int64_t half = gate_up.size(-1) / 2;
+  const Rows whole = mx8_rows(gate_up);
+  auto sizes = gate_up.sizes().vec();
+  sizes.back() = half;
+  SwiGLUMx8Out o;
+  if (packed) o.y8 = mx8_empty(sizes, gate_up);
+  else o.y = at::empty(sizes, gate_up.options());
+  if (keep) {
+    o.gate8 = mx8_empty(sizes, gate_up);
+    o.up8 = mx8_empty(sizes, gate_up);
+  }
+  const pico_mx8 none = {}, y8 = packed ? o.y8.c() : none, g8 = keep ? o.gate8.c() : none, u8 = keep ? o.up8.c() : none;
+  const char* first = static_cast<const char*>(ptr(whole.t));
+  check(pico_swiglu_mx8_fwd(first, first + half * gate_up.element_size(), ptr(o.y), packed ? &y8 : nullptr, keep ? &g8 : nullptr, keep ? &u8 : nullptr, whole.rows, half, whole.pitch,
+                            whole.pitch, dt, stream_now()));
+  return o;
+}
+// d(gate_up) and, where it is wanted, silu(gate) * up of what was kept
+std::pair<Tensor, Tensor> swiglu_mx8_backward(const Tensor& dy, const Mx8& gate8, const Mx8& up8, at::ScalarType dtype, bool want_y) {
+  const c10::OptionalDeviceGuard device(gate8.data.device());
+  const Rows d = mx8_rows(dy.to(dtype));
+  const int64_t half = gate8.cols();
+  auto sizes = gate8.data.sizes().vec();
+  const auto o = gate8.data.options().dtype(dtype);
+  const Tensor y = want_y ? at::empty(sizes, o) : Tensor();
+  sizes.back() = 2 * half;
+  const Tensor dx = at::empty(sizes, o);
+  const pico_mx8 g = gate8.c(), u = up8.c();
+  char* first = static_cast<char*>(ptr(dx));
+  check(pico_swiglu_mx8_bwd(ptr(d.t), &g, &u, first, first + half * dx.element_size(), ptr(y), gate8.rows(), half, d.pitch, 2 * half, 2 * half, dtype_code(dx, "swiglu_8bit"), stream_now()));
+  return {dx, y};
+}
+
+// What the layers below share.  Their gradients are those of the layer with its 8-bit values in the place of the activations (a rounding counts as the identity), and
+// with the weight itself, not its 8-bit form, in the product that gives the input's.
+void check_weight(const char* fn, const Tensor& like, int64_t in, const Tensor& w) {
+  on_gpu(like);
+  on_gpu(w);
+  TORCH_CHECK(like.scalar_type() == at::kBFloat16 && w.scalar_type() == at::kBFloat16, fn, ": activations and weight must be bf16 (got ", like.scalar_type(), " and ", w.scalar_type(), ")");
+  TORCH_CHECK(w.dim() == 2 && w.size(1) == in && w.device() == like.device(), fn, ": weight must be [out, ", in, "] on ", like.device(), " (got ", w.sizes(), " on ", w.device(), ")");
+}
+Mx8 packed_weight(const char* fn, const Tensor& w, const OptMx8& given) {
+  if (!given) return mx8_quantized(fn, w);
+  const Mx8 p = mx8_given(fn, *given);
+  TORCH_CHECK(p.data.sizes() == w.sizes() && p.data.device() == w.device(), fn, ": packed must be the weight's 8-bit form, ", w.sizes(), " on ", w.device(), " (got ", p.data.sizes(), " on ",
+              p.data.device(), ")");
+  return p;
+}
+bool needs_any(const AutogradContext* ctx, size_t from, size_t count) {
+  for (size_t i = 0; i < count; ++i)
+    if (ctx->needs_input_grad(from + i)) return true;
+  return false;
+}
+// an upstream gradient as the products take it, whatever its layout (a bias of one layout's sums against another's would be none of the caller's)
+Tensor upstream(const Tensor& given) {
+  const Tensor g = as_it_is(given), m = g.dim() == 1 ? g.unsqueeze(0) : matrix(g);
+  return plain(m) && m.stride(0) % 8 == 0 ? m : m.contiguous();
+}
+// the gradients of x [rows, in] (as wanted) and of the weight, rows of which may be parameters of their own
+struct WeightGradients {
+  Tensor dx;
+  variable_list dw;
+};
+WeightGradients weight_gradients(const Tensor& dy, const Tensor& w, bool want_x, bool want_w, const std::function<Tensor()>& x, const std::vector<int64_t>& rows) {
+  WeightGradients r;
+  Tensor dw;
+  if (want_x && want_w) {
+    Gradients both = gradients(dy, w, x());
+    r.dx = both.dx;
+    dw = both.dw;
+  } else if (want_w) {
+    dw = product(dy, x(), Product::TN);
+  } else if (want_x) {
+    r.dx = product(dy, w, Product::NN);
+  }
+  if (rows.empty()) r.dw.push_back(dw);
+  int64_t at_row = 0;
+  for (int64_t n : rows) {
+    r.dw.push_back(dw.defined() ? dw.narrow(0, at_row, n) : Tensor());
+    at_row += n;
+  }
+  return r;
+}
+std::vector<int64_t> part_rows(const char* fn, const Tensor& w, at::TensorList parts) {
+  std::vector<int64_t> rows;
+  int64_t sum = 0;
+  for (const Tensor& p : parts) {
+    TORCH_CHECK(p.dim() == 2 && p.size(1) == w.size(1), fn, ": a part of the weight ", w.sizes(), " cannot be ", p.sizes());
+    rows.push_back(p.size(0));
+    sum += p.size(0);
+  }
+  TORCH_CHECK(parts.empty() || sum == w.size(0), fn, ": the parts of the weight have ", sum, " rows, it has ", w.size(0));
+  return rows;
+}
+
+// y = x w^T with both in 8 bits; what is kept of x is its 8-bit form
+struct Linear8 : torch::autograd::Function<Linear8> {
+  static Tensor run(const Tensor& x, const Tensor& w, const OptMx8& packed, Mx8* kept) {
+    const char* fn = "linear_8bit";
+    TORCH_CHECK(x.dim() >= 1, fn, ": x must have an axis");
+    check_weight(fn, x, x.size(-1), w);
+    const c10::OptionalDeviceGuard device(x.device());
+    const Mx8 x8 = mx8_quantized(fn, x);
+    if (kept) *kept = x8;
+    return mx8_product(fn, x8, packed_weight(fn, w, packed));
+  }
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptMx8& packed) {
+    Mx8 x8;
+    const Tensor y = run(x, w, packed, &x8);
+    const bool keep = w.requires_grad();
+    ctx->save_for_backward({x.requires_grad() ? w : Tensor(), keep ? x8.data : Tensor(), keep ? x8.scales : Tensor()});
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    refuse_second_order("linear_8bit");
+    const auto s = ctx->get_saved_variables();
+    const c10::OptionalDeviceGuard device(g[0].device());
+    auto sizes = g[0].sizes().vec();
+    const Tensor dy = upstream(g[0]);
+    WeightGradients r = weight_gradients(dy, s[0], ctx->needs_input_grad(0), ctx->needs_input_grad(1), [&] { return matrix8(s[1], s[2]); }, {});
+    if (r.dx.defined()) {
+      sizes.back() = r.dx.size(1);
+      r.dx = r.dx.view(sizes);
+    }
+    return {r.dx, r.dw[0], Tensor()};
+  }
+  static Tensor matrix8(const Tensor& data, const Tensor& scales) {   // the values of a kept operand, [rows, cols]
+    return mx8_values({data.view({scales.size(1), data.size(-1)}), scales}, at::kBFloat16);
+  }
+};
+Tensor linear_8bit(const Tensor& x, const Tensor& w, const OptMx8& packed) {
+  refuse_tangents("linear_8bit", {&x, &w});
+  if (!records({&x, &w})) return Linear8::run(x, w, packed, nullptr);
+  return Linear8::apply(x, w, packed);
+}
+
+// h = x + residual (x where there is none); returns (rmsnorm(h) * norm_weight, in 8 bits, times w^T, h).  Where w is a buffer that the parameters `parts` alias, row
+// block by row block, they get its gradient.
+struct NormLinear8 : torch::autograd::Function<NormLinear8> {
+  static constexpr const char* fn = "rms_norm_linear_8bit";
+  static variable_list run(const Tensor& x, const OptTensor& residual, const Tensor& norm_weight, double eps, const Tensor& w, const OptMx8& packed, NormMx8Out* kept) {
+    TORCH_CHECK(x.dim() >= 1, fn, ": x must have an axis");
+    check_weight(fn, x, x.size(-1), w);
+    const c10::OptionalDeviceGuard device(x.device());
+    NormMx8Out o = rmsnorm_mx8(fn, x, norm_weight, eps, residual, kept != nullptr);
+    const Tensor y = mx8_product(fn, o.y, packed_weight(fn, w, packed));
+    if (kept) *kept = o;
+    return {y, residual ? o.sum : x};
+  }
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& residual, const Tensor& norm_weight, double eps, const Tensor& w, const OptMx8& packed,
+                               at::TensorList parts) {
+    ctx->saved_data["rows"] = part_rows(fn, w, parts);
+    NormMx8Out kept;
+    variable_list out = run(x, residual, norm_weight, eps, w, packed, &kept);
+    bool keep = w.requires_grad();
+    for (const Tensor& p : parts) keep |= p.requires_grad();
+    ctx->save_for_backward({residual ? out[1] : x, norm_weight, kept.rstd, w, keep ? kept.y.data : Tensor(), keep ? kept.y.scales : Tensor()});
+    ctx->saved_data["residual"] = residual.has_value();
+    ctx->set_materialize_grads(false);   // (the stream's h may have no other reader)
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    refuse_second_order(fn);
+    const auto rows = ctx->saved_data["rows"].toIntVector();
+    variable_list r(6 + rows.size());
+    const bool has_residual = ctx->saved_data["residual"].toBool();
+    if (!g[0].defined()) {   // only the residual stream carried a gradient
+      r[0] = g[1];
+      if (has_residual) r[1] = g[1];
+      return r;
+    }
+    const auto s = ctx->get_saved_variables();
+    const c10::OptionalDeviceGuard device(g[0].device());
+    const Tensor dy = upstream(g[0]);
+    const size_t at_gamma = has_residual ? 2 : 1;   // (among the tensors: eps, packed and a residual that is none do not count)
+    const bool wants_norm = needs_any(ctx, 0, at_gamma + 1), wants_w = rows.empty() ? ctx->needs_input_grad(at_gamma + 1) : needs_any(ctx, at_gamma + 2, rows.size());
+    WeightGradients d = weight_gradients(dy, s[3], wants_norm, wants_w, [&] { return Linear8::matrix8(s[4], s[5]); }, rows);
+    if (wants_norm) {
+      auto [dx, dgamma] = rmsnorm_backward(d.dx.view(s[0].sizes()), as_it_is(s[0]), as_it_is(s[1]), s[2], g[1].defined() ? OptTensor(as_it_is(g[1])) : std::nullopt, s[1].scalar_type());
+      r[0] = dx;
+      if (has_residual) r[1] = dx;
+      r[2] = dgamma;
+    }
+    if (rows.empty()) r[4] = d.dw[0];
+    for (size_t i = 0; i < rows.size(); ++i) r[6 + i] = d.dw[i];
+    return r;
+  }
+};
+std::pair<Tensor, Tensor> rms_norm_linear_8bit(const Tensor& x, const OptTensor& residual, const Tensor& norm_weight, double eps, const Tensor& w, const OptMx8& packed,
+                                               const std::vector<Tensor>& parts) {
+  refuse_tangents(NormLinear8::fn, {&x, &norm_weight, &w});
+  if (residual) refuse_tangents(NormLinear8::fn, {&*residual});
+  bool recorded = records({&x, &norm_weight, &w}) || (residual && records({&*residual}));
+  for (const Tensor& p : parts) recorded |= records({&p});
+  if (!recorded) {
+    part_rows(NormLinear8::fn, w, parts);
+    auto o = NormLinear8::run(x, residual, norm_weight, eps, w, packed, nullptr);
+    return {o[0], o[1]};
+  }
+  auto o = NormLinear8::apply(x, residual, norm_weight, eps, w, packed, at::TensorList(parts));
+  return {o[0], residual || x.requires_grad() ? o[1] : x};   // (x without a gradient passes as it is)
+}
+
+// silu(gate) * up of the two halves of gate_up; gate and up are kept in 8 bits and the gradient is taken at the values that these stand for
+struct SwiGLU8 : torch::autograd::Function<SwiGLU8> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& gate_up) {
+    SwiGLUMx8Out o = swiglu_mx8("swiglu_8bit", gate_up, false, true);
+    ctx->save_for_backward({o.gate8.data, o.gate8.scales, o.up8.data, o.up8.scales});
+    ctx->saved_data["dtype"] = static_cast<int64_t>(gate_up.scalar_type());
+    return o.y;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    refuse_second_order("swiglu_8bit");
+    const auto s = ctx->get_saved_variables();
+    return {swiglu_mx8_backward(g[0], {s[0], s[1]}, {s[2], s[3]}, static_cast<at::ScalarType>(ctx->saved_data["dtype"].toInt()), false).first};
+  }
+};
+Tensor swiglu_8bit(const Tensor& gate_up) {
+  refuse_tangents("swiglu_8bit", {&gate_up});
+  if (!records({&gate_up})) return swiglu_mx8("swiglu_8bit", gate_up, false, false).y;
+  return SwiGLU8::apply(gate_up);
+}
+
+// The same, in 8 bits, times w^T.  The weight's gradient takes silu(gate) * up of what was kept, which the kernel of gate's and up's gradients writes beside them.
+struct SwiGLULinear8 : torch::autograd::Function<SwiGLULinear8> {
+  static constexpr const char* fn = "swiglu_linear_8bit";
+  static Tensor run(const Tensor& gate_up, const Tensor& w, const OptMx8& packed, SwiGLUMx8Out* kept) {
+    TORCH_CHECK(gate_up.dim() >= 1 && gate_up.size(-1) % 2 == 0, fn, ": gate_up must hold two halves (got ", gate_up.sizes(), ")");
+    check_weight(fn, gate_up, gate_up.size(-1) / 2, w);
+    const c10::OptionalDeviceGuard device(gate_up.device());
+    SwiGLUMx8Out o = swiglu_mx8(fn, gate_up, true, kept != nullptr);
+    const Tensor y = mx8_product(fn, o.y8, packed_weight(fn, w, packed));
+    if (kept) *kept = o;
+    return y;
+  }
+  static Tensor forward(AutogradContext* ctx, const Tensor& gate_up, const Tensor& w, const OptMx8& packed) {
+    SwiGLUMx8Out kept;
+    const Tensor y = run(gate_up, w, packed, &kept);
+    ctx->save_for_backward({w, kept.gate8.data, kept.gate8.scales, kept.up8.data, kept.up8.scales});
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    refuse_second_order(fn);
+    const auto s = ctx->get_saved_variables();
+    const c10::OptionalDeviceGuard device(g[0].device());
+    const Tensor dy = upstream(g[0]);
+    variable_list r(3);
+    const bool wants_w = ctx->needs_input_grad(1);
+    const Tensor dh = product(dy, s[0], Product::NN);
+    auto [dx, h] = swiglu_mx8_backward(dh, {s[1], s[2]}, {s[3], s[4]}, at::kBFloat16, wants_w);
+    if (ctx->needs_input_grad(0)) r[0] = dx;
+    if (wants_w) r[1] = product(dy, h.view({dy.size(0), s[0].size(1)}), Product::TN);
+    return r;
+  }
+};
+Tensor swiglu_linear_8bit(const Tensor& gate_up, const Tensor& w, const OptMx8& packed) {
+  refuse_tangents(SwiGLULinear8::fn, {&gate_up, &w});
+  if (!records({&gate_up, &w})) return SwiGLULinear8::run(gate_up, w, packed, nullptr);
+  return SwiGLULinear8::apply(gate_up, w, packed);
+}
+
 // ------------------------------------------------------------------------------------------------ AdamW
 // The step for a fixed list of tensors in as few launches as they fit.  Weights, moments and sizes are checked and their
 // pointer tables built once; a step only fills in the gradients' addresses.
@@ -1883,6 +2265,20 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("policy_loss", &policy_loss, nogil());
   m.def("preference_loss", &preference_loss, nogil());
   m.def("linear_log_probs", &linear_log_probs, nogil());
+  m.def("mx8_quantize", [](const Tensor& x) {
+    const Mx8 y = mx8_quantized("mx8_quantize", x);
+    return Mx8Pair{y.data, y.scales};
+  }, nogil());
+  m.def("mx8_dequantize", [](const Mx8Pair& x, at::ScalarType dtype) { return mx8_values(mx8_given("mx8_dequantize", x), dtype); }, nogil());
+  m.def("mx8_product", [](const Mx8Pair& a, const Mx8Pair& b) { return mx8_product("mx8_product", mx8_given("mx8_product", a), mx8_given("mx8_product", b)); }, nogil());
+  m.def("rmsnorm_mx8_fwd", [](const Tensor& x, const Tensor& w, double eps, const OptTensor& residual) {
+    NormMx8Out o = rmsnorm_mx8("rmsnorm_mx8_fwd", x, w, eps, residual, true);
+    return std::make_tuple(o.y.data, o.y.scales, o.rstd, o.sum.defined() ? OptTensor(o.sum) : std::nullopt);
+  }, nogil());
+  m.def("linear_8bit", &linear_8bit, nogil());
+  m.def("rms_norm_linear_8bit", &rms_norm_linear_8bit, nogil());
+  m.def("swiglu_8bit", &swiglu_8bit, nogil());
+  m.def("swiglu_linear_8bit", &swiglu_linear_8bit, nogil());
   m.def("zero_grads", &zero_grads);
   py::class_<AdamWPlan>(m, "AdamWPlan")
       .def(py::init<const std::vector<Tensor>&, const std::vector<Tensor>&, const std::vector<Tensor>&, const std::optional<OptTensors>&>())

@@ -1,0 +1,357 @@
+// What makes the 8-bit form (mx8.h) and reads it back beside the products: rows of a tensor, RMSNorm (with the residual's addition) that writes nothing
+// else, SwiGLU whose output or checkpoint is held that way and its gradient from that checkpoint.
+//
+// All of them are bound by memory; each value passes the registers once, and a block's largest value is found among the 4 (bf16) or 8
+// (fp32) lanes that hold it.
+#include "mx8.h"
+
+namespace pico {
+namespace {
+
+constexpr int kThreads = 256;
+
+__device__ __forceinline__ float sigmoid_fast(float x) { return __builtin_amdgcn_rcpf(1.f + fast_exp2(-x * kLog2e)); }
+
+// n / d for n under 2^31: (high half of n m + n) >> s
+struct Divide {
+  uint32_t m, s, d;
+};
+Divide divide_by(uint32_t d) {
+  uint32_t s = 0;
+  while ((uint64_t{1} << s) < d) ++s;
+  return {static_cast<uint32_t>((uint64_t{1} << 32) * ((uint64_t{1} << s) - d) / d + 1), s, d};
+}
+__device__ __forceinline__ uint32_t quotient(uint32_t n, Divide by) { return (__umulhi(n, by.m) + n) >> by.s; }
+
+// Where a thread of the kernels that walk groups of 128 columns stands.  128 / V neighbouring lanes hold a group; the last of a row may be cut short, its
+// lanes past the row stay on.
+struct Place {
+  int64_t row;
+  int col, t;      // t: the group in its row
+  bool live;
+};
+template <int V>
+__device__ __forceinline__ bool place(Place& p, int64_t groups, Divide per_row, int cols) {
+  constexpr int kLanes = kGroup / V;
+  const int64_t g = static_cast<int64_t>(blockIdx.x) * (kThreads / kLanes) + threadIdx.x / kLanes;
+  if (g >= groups) return false;
+  const uint32_t row = quotient(static_cast<uint32_t>(g), per_row);
+  p.row = row;
+  p.t = static_cast<int>(static_cast<uint32_t>(g) - row * per_row.d);
+  p.col = p.t * kGroup + static_cast<int>(threadIdx.x % kLanes) * V;
+  p.live = p.col < cols;
+  return true;
+}
+template <int V>
+__device__ __forceinline__ void store_block(const pico_mx8& y, const Place& p, int64_t rows, int cols, const float (&v)[V]) {
+  const Codes<V> c = encode<V>(v);
+  const uint32_t scales = four_scales<V>(c.scale, threadIdx.x);
+  if (!p.live) return;
+  store_codes<V>(static_cast<uint8_t*>(y.data) + p.row * cols + p.col, c.word);
+  if (threadIdx.x % (kGroup / V) == 0) static_cast<uint32_t*>(y.scales)[p.t * rows + p.row] = scales;
+}
+template <int V>
+__device__ __forceinline__ void load_block(const pico_mx8& x, const Place& p, int64_t rows, int cols, float (&v)[V]) {
+  uint32_t word[V / 4];
+  load_codes<V>(static_cast<const uint8_t*>(x.data) + p.row * cols + p.col, word);
+  decode<V>(word, static_cast<const uint8_t*>(x.scales)[(p.t * rows + p.row) * 4 + p.col % kGroup / kBlock], v);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void quantize_kernel(const T* __restrict__ x, const pico_mx8 y, int64_t rows, int cols, int64_t ld, int64_t groups, Divide per_row) {
+  constexpr int V = io<T>::kVec;
+  Place p;
+  if (!place<V>(p, groups, per_row, cols)) return;
+  float v[V] = {};
+  if (p.live) io<T>::load(x + p.row * ld + p.col, v);
+  store_block<V>(y, p, rows, cols, v);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void dequantize_kernel(const pico_mx8 x, T* __restrict__ y, int64_t rows, int cols, int64_t ld, int64_t groups, Divide per_row) {
+  constexpr int V = io<T>::kVec;
+  Place p;
+  if (!place<V>(p, groups, per_row, cols) || !p.live) return;
+  float v[V];
+  load_block<V>(x, p, rows, cols, v);
+  io<T>::store(y + p.row * ld + p.col, v);
+}
+
+// silu(gate) * up; y and y8, either or both, and the checkpoint where it is wanted
+template <typename T>
+__global__ __launch_bounds__(kThreads) void swiglu_mx8_fwd_kernel(const T* __restrict__ gate, const T* __restrict__ up, T* __restrict__ y, const pico_mx8 y8,
+                                                                  const pico_mx8 gate8, const pico_mx8 up8, int64_t rows, int cols, int64_t gate_ld, int64_t up_ld,
+                                                                  int64_t groups, Divide per_row) {
+  constexpr int V = io<T>::kVec;
+  Place p;
+  if (!place<V>(p, groups, per_row, cols)) return;
+  float g[V] = {}, u[V] = {}, o[V];
+  if (p.live) {
+    io<T>::load(gate + p.row * gate_ld + p.col, g);
+    io<T>::load(up + p.row * up_ld + p.col, u);
+  }
+#pragma unroll
+  for (int e = 0; e < V; ++e) o[e] = g[e] * sigmoid_fast(g[e]) * u[e];
+  if (gate8.data != nullptr) {
+    store_block<V>(gate8, p, rows, cols, g);
+    store_block<V>(up8, p, rows, cols, u);
+  }
+  if (y8.data != nullptr) store_block<V>(y8, p, rows, cols, o);
+  if (y != nullptr && p.live) io<T>::store(y + p.row * cols + p.col, o);
+}
+
+// With g, u what the checkpoint stands for and s = sigmoid(g): dgate = dy u s (1 + g (1 - s)), dup = dy g s; y = g s u again where it is wanted
+template <typename T>
+__global__ __launch_bounds__(kThreads) void swiglu_mx8_bwd_kernel(const T* __restrict__ dy, const pico_mx8 gate8, const pico_mx8 up8, T* __restrict__ dgate, T* __restrict__ dup,
+                                                                  T* __restrict__ y, int64_t rows, int cols, int64_t dy_ld, int64_t dgate_ld, int64_t dup_ld, int64_t groups,
+                                                                  Divide per_row) {
+  constexpr int V = io<T>::kVec;
+  Place p;
+  if (!place<V>(p, groups, per_row, cols) || !p.live) return;
+  float d[V], g[V], u[V], dg[V], du[V], o[V];
+  load_block<V>(gate8, p, rows, cols, g);
+  load_block<V>(up8, p, rows, cols, u);
+  io<T>::load(dy + p.row * dy_ld + p.col, d);
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    const float s = sigmoid_fast(g[e]), gs = g[e] * s;
+    dg[e] = d[e] * u[e] * s * (1.f + g[e] * (1.f - s));
+    du[e] = d[e] * gs;
+    o[e] = gs * u[e];
+  }
+  io<T>::store(dgate + p.row * dgate_ld + p.col, dg);
+  io<T>::store(dup + p.row * dup_ld + p.col, du);
+  if (y != nullptr) io<T>::store(y + p.row * cols + p.col, o);
+}
+
+// ---- RMSNorm: y = (x + residual) rstd w in the 8-bit form only
+template <int G>
+__device__ __forceinline__ float group_sum(float v, float* smem) {
+  v = wave_sum(v);
+  if constexpr (G == kWave) {
+    return v;
+  } else {
+    if (threadIdx.x % kWave == 0) smem[threadIdx.x / kWave] = v;
+    __syncthreads();
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < G / kWave; ++i) t += smem[i];
+    return t;
+  }
+}
+
+// A row to a wave (G 64) or to the workgroup (G 256), NV pieces of 16 bytes to a thread, which stay in registers between the sum of squares and the
+// output.
+template <typename T, int G, int NV>
+__global__ __launch_bounds__(kThreads) void rmsnorm_mx8_kernel(const T* __restrict__ x, const T* __restrict__ w, const pico_mx8 y, float* __restrict__ rstd,
+                                                               const T* __restrict__ res_in, T* __restrict__ res_out, int64_t rows, int hidden, float eps) {
+  Arguments<0, 64>().arrive();
+  constexpr int V = io<T>::kVec;
+  __shared__ float smem[kThreads / kWave];
+  const int t = threadIdx.x % G, nvec = hidden / V;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / G) + threadIdx.x / G;
+  if (row >= rows) return;   // (G 256: uniform over the workgroup, which meets at a barrier below)
+  const int64_t at = row * hidden;
+  // everything that the row needs is requested before the first of it is used; pieces past the row re-read its first
+  constexpr bool kEarly = NV <= 4;
+  auto piece = [&](int j) { return (t + j * G < nvec ? t + j * G : 0) * V; };
+  u32x4 x_raw[kEarly ? NV : 1], r_raw[kEarly ? NV : 1], w_raw[kEarly ? NV : 1];
+  if constexpr (kEarly) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) x_raw[j] = *reinterpret_cast<const u32x4*>(x + at + piece(j));
+    if (res_in != nullptr) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) r_raw[j] = *reinterpret_cast<const u32x4*>(res_in + at + piece(j));
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) w_raw[j] = *reinterpret_cast<const u32x4*>(w + piece(j));
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  float vals[NV][V], ss = 0.f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    if constexpr (kEarly) io<T>::load(&x_raw[j], vals[j]);
+    else io<T>::load(x + at + piece(j), vals[j]);
+    if (res_in != nullptr) {
+      float r[V];
+      if constexpr (kEarly) io<T>::load(&r_raw[j], r);
+      else io<T>::load(res_in + at + piece(j), r);
+#pragma unroll
+      for (int e = 0; e < V; ++e) vals[j][e] += r[e];
+      if (res_out != nullptr && t + j * G < nvec) store_as<T, true>(res_out + at + piece(j), vals[j]);
+    }
+    if (t + j * G < nvec) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) ss += vals[j][e] * vals[j][e];
+    }
+  }
+  ss = group_sum<G>(ss, smem);
+  const float r = rsqrtf(ss / static_cast<float>(hidden) + eps);
+  if (rstd != nullptr && t == 0) rstd[row] = r;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int v = t + j * G;
+    if (__builtin_amdgcn_readfirstlane(v) >= nvec) break;   // (uniform: whole waves of pieces past the row)
+    float wv[V], o[V];
+    if constexpr (kEarly) io<T>::load(&w_raw[j], wv);
+    else io<T>::load(w + piece(j), wv);
+#pragma unroll
+    for (int e = 0; e < V; ++e) o[e] = v < nvec ? vals[j][e] * r * wv[e] : 0.f;
+    const Codes<V> c = encode<V>(o);
+    const uint32_t scales = four_scales<V>(c.scale, t);
+    if (v < nvec) {
+      store_codes<V>(static_cast<uint8_t*>(y.data) + at + static_cast<int64_t>(v) * V, c.word);
+      if (v % (kGroup / V) == 0) static_cast<uint32_t*>(y.scales)[static_cast<int64_t>(v / (kGroup / V)) * rows + row] = scales;
+    }
+  }
+}
+
+template <typename T, int G, int NV>
+void launch_norm(const void* x, const void* w, const pico_mx8& y, float* rstd, const void* ri, void* ro, int64_t rows, int hidden, float eps, hipStream_t s) {
+  constexpr int kRows = kThreads / G;
+  hipLaunchKernelGGL((rmsnorm_mx8_kernel<T, G, NV>), dim3(static_cast<unsigned>((rows + kRows - 1) / kRows)), dim3(kThreads), 0, s, static_cast<const T*>(x),
+                     static_cast<const T*>(w), y, rstd, static_cast<const T*>(ri), static_cast<T*>(ro), rows, hidden, eps);
+}
+template <typename T>
+void dispatch_norm(const void* x, const void* w, const pico_mx8& y, float* rstd, const void* ri, void* ro, int64_t rows, int hidden, float eps, hipStream_t s) {
+  const int nvec = hidden / io<T>::kVec;
+  if (nvec <= 64) return launch_norm<T, 64, 1>(x, w, y, rstd, ri, ro, rows, hidden, eps, s);
+  if (nvec <= 128) return launch_norm<T, 64, 2>(x, w, y, rstd, ri, ro, rows, hidden, eps, s);
+  if (nvec <= 256) return launch_norm<T, 64, 4>(x, w, y, rstd, ri, ro, rows, hidden, eps, s);
+  if (nvec <= 512) return launch_norm<T, 256, 2>(x, w, y, rstd, ri, ro, rows, hidden, eps, s);
+  if (nvec <= 1024) return launch_norm<T, 256, 4>(x, w, y, rstd, ri, ro, rows, hidden, eps, s);
+  if (nvec <= 2048) return launch_norm<T, 256, 8>(x, w, y, rstd, ri, ro, rows, hidden, eps, s);
+  launch_norm<T, 256, 16>(x, w, y, rstd, ri, ro, rows, hidden, eps, s);
+}
+
+int vec_of(int dtype) { return dtype == PICO_BF16 ? 8 : 4; }
+int check_dtype(const char* fn, int dtype) {
+  return dtype == PICO_BF16 || dtype == PICO_F32 ? PICO_OK : fail(PICO_ERR_DTYPE, "%s: dtype code %d not supported", fn, dtype);
+}
+// a tensor of rows of pitch ld beside the 8-bit operands
+int check_rows(const char* fn, const char* what, const void* p, int64_t cols, int64_t ld, int dtype) {
+  if (!p) return fail(PICO_ERR_NULL, "%s: %s is required", fn, what);
+  if (ld < cols) return fail(PICO_ERR_STRIDE, "%s: %s has a row pitch under its columns", fn, what);
+  if (!aligned16(p) || ld % vec_of(dtype) != 0) return fail(PICO_ERR_ALIGN, "%s: %s must be 16-byte aligned, its row pitch a multiple of %d", fn, what, vec_of(dtype));
+  return PICO_OK;
+}
+struct Walk {
+  int64_t groups;
+  Divide per_row;
+  dim3 grid;
+};
+Walk walk(int64_t rows, int64_t cols, int dtype) {
+  const int64_t per_row = (cols + kGroup - 1) / kGroup, groups = rows * per_row, per_block = kThreads / (kGroup / vec_of(dtype));
+  return {groups, divide_by(static_cast<uint32_t>(per_row)), dim3(static_cast<unsigned>((groups + per_block - 1) / per_block))};
+}
+
+}  // namespace
+}  // namespace pico
+
+using namespace pico;
+
+#define PICO_TRY(call) \
+  if (int rc = (call)) return rc
+
+extern "C" int pico_mx8_quantize(const void* x, const pico_mx8* y, int64_t rows, int64_t cols, int64_t x_ld, int dtype, void* stream) {
+  const char* fn = "pico_mx8_quantize";
+  PICO_TRY(check_dtype(fn, dtype));
+  PICO_TRY(check_mx8_shape(fn, rows, cols));
+  if (rows == 0) return PICO_OK;
+  PICO_TRY(check_rows(fn, "x", x, cols, x_ld, dtype));
+  PICO_TRY(check_mx8(fn, "y", y));
+  const Walk w = walk(rows, cols, dtype);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == PICO_BF16)
+    hipLaunchKernelGGL(quantize_kernel<__bf16>, w.grid, dim3(kThreads), 0, s, static_cast<const __bf16*>(x), *y, rows, static_cast<int>(cols), x_ld, w.groups, w.per_row);
+  else
+    hipLaunchKernelGGL(quantize_kernel<float>, w.grid, dim3(kThreads), 0, s, static_cast<const float*>(x), *y, rows, static_cast<int>(cols), x_ld, w.groups, w.per_row);
+  return check_launch(fn);
+}
+
+extern "C" int pico_mx8_dequantize(const pico_mx8* x, void* y, int64_t rows, int64_t cols, int64_t y_ld, int dtype, void* stream) {
+  const char* fn = "pico_mx8_dequantize";
+  PICO_TRY(check_dtype(fn, dtype));
+  PICO_TRY(check_mx8_shape(fn, rows, cols));
+  if (rows == 0) return PICO_OK;
+  PICO_TRY(check_mx8(fn, "x", x));
+  PICO_TRY(check_rows(fn, "y", y, cols, y_ld, dtype));
+  const Walk w = walk(rows, cols, dtype);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == PICO_BF16)
+    hipLaunchKernelGGL(dequantize_kernel<__bf16>, w.grid, dim3(kThreads), 0, s, *x, static_cast<__bf16*>(y), rows, static_cast<int>(cols), y_ld, w.groups, w.per_row);
+  else
+    hipLaunchKernelGGL(dequantize_kernel<float>, w.grid, dim3(kThreads), 0, s, *x, static_cast<float*>(y), rows, static_cast<int>(cols), y_ld, w.groups, w.per_row);
+  return check_launch(fn);
+}
+
+extern "C" int pico_rmsnorm_mx8_fwd(const void* x, const void* weight, const pico_mx8* y, float* rstd, const void* residual_in, void* residual_out, int64_t rows, int64_t hidden,
+                                    float eps, int dtype, void* stream) {
+  const char* fn = "pico_rmsnorm_mx8_fwd";
+  PICO_TRY(check_dtype(fn, dtype));
+  PICO_TRY(check_mx8_shape(fn, rows, hidden));
+  if (hidden > 16384) return fail(PICO_ERR_SHAPE, "%s: hidden=%lld (16384 at most)", fn, (long long)hidden);
+  if (rows == 0) return PICO_OK;
+  PICO_TRY(check_rows(fn, "x", x, hidden, hidden, dtype));
+  PICO_TRY(check_rows(fn, "weight", weight, hidden, hidden, dtype));
+  PICO_TRY(check_mx8(fn, "y", y));
+  if (residual_out && !residual_in) return fail(PICO_ERR_NULL, "%s: residual_out without residual_in", fn);
+  if (!aligned16(residual_in) || !aligned16(residual_out)) return fail(PICO_ERR_ALIGN, "%s: pointers must be 16-byte aligned", fn);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == PICO_BF16) dispatch_norm<__bf16>(x, weight, *y, rstd, residual_in, residual_out, rows, static_cast<int>(hidden), eps, s);
+  else dispatch_norm<float>(x, weight, *y, rstd, residual_in, residual_out, rows, static_cast<int>(hidden), eps, s);
+  return check_launch(fn);
+}
+
+extern "C" int pico_swiglu_mx8_fwd(const void* gate, const void* up, void* y, const pico_mx8* y8, const pico_mx8* gate8, const pico_mx8* up8, int64_t rows, int64_t cols,
+                                   int64_t gate_ld, int64_t up_ld, int dtype, void* stream) {
+  const char* fn = "pico_swiglu_mx8_fwd";
+  PICO_TRY(check_dtype(fn, dtype));
+  PICO_TRY(check_mx8_shape(fn, rows, cols));
+  if (rows == 0) return PICO_OK;
+  if (!y && !y8) return fail(PICO_ERR_NULL, "%s: y or y8 is required", fn);
+  if (!gate8 != !up8) return fail(PICO_ERR_NULL, "%s: gate8 and up8 come together", fn);
+  PICO_TRY(check_rows(fn, "gate", gate, cols, gate_ld, dtype));
+  PICO_TRY(check_rows(fn, "up", up, cols, up_ld, dtype));
+  if (y) PICO_TRY(check_rows(fn, "y", y, cols, cols, dtype));
+  if (y8) PICO_TRY(check_mx8(fn, "y8", y8));
+  if (gate8) {
+    PICO_TRY(check_mx8(fn, "gate8", gate8));
+    PICO_TRY(check_mx8(fn, "up8", up8));
+  }
+  const Walk w = walk(rows, cols, dtype);
+  const pico_mx8 none = {nullptr, nullptr};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  auto go = [&](auto kernel, auto zero) {
+    using T = decltype(zero);
+    hipLaunchKernelGGL(kernel, w.grid, dim3(kThreads), 0, s, static_cast<const T*>(gate), static_cast<const T*>(up), static_cast<T*>(y), y8 ? *y8 : none, gate8 ? *gate8 : none,
+                       up8 ? *up8 : none, rows, static_cast<int>(cols), gate_ld, up_ld, w.groups, w.per_row);
+  };
+  if (dtype == PICO_BF16) go(swiglu_mx8_fwd_kernel<__bf16>, __bf16());
+  else go(swiglu_mx8_fwd_kernel<float>, float());
+  return check_launch(fn);
+}
+
+extern "C" int pico_swiglu_mx8_bwd(const void* dy, const pico_mx8* gate8, const pico_mx8* up8, void* dgate, void* dup, void* y, int64_t rows, int64_t cols, int64_t dy_ld,
+                                   int64_t dgate_ld, int64_t dup_ld, int dtype, void* stream) {
+  const char* fn = "pico_swiglu_mx8_bwd";
+  PICO_TRY(check_dtype(fn, dtype));
+  PICO_TRY(check_mx8_shape(fn, rows, cols));
+  if (rows == 0) return PICO_OK;
+  PICO_TRY(check_rows(fn, "dy", dy, cols, dy_ld, dtype));
+  PICO_TRY(check_mx8(fn, "gate8", gate8));
+  PICO_TRY(check_mx8(fn, "up8", up8));
+  PICO_TRY(check_rows(fn, "dgate", dgate, cols, dgate_ld, dtype));
+  PICO_TRY(check_rows(fn, "dup", dup, cols, dup_ld, dtype));
+  if (y) PICO_TRY(check_rows(fn, "y", y, cols, cols, dtype));
+  const Walk w = walk(rows, cols, dtype);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  auto go = [&](auto kernel, auto zero) {
+    using T = decltype(zero);
+    hipLaunchKernelGGL(kernel, w.grid, dim3(kThreads), 0, s, static_cast<const T*>(dy), *gate8, *up8, static_cast<T*>(dgate), static_cast<T*>(dup), static_cast<T*>(y), rows,
+                       static_cast<int>(cols), dy_ld, dgate_ld, dup_ld, w.groups, w.per_row);
+  };
+  if (dtype == PICO_BF16) go(swiglu_mx8_bwd_kernel<__bf16>, __bf16());
+  else go(swiglu_mx8_bwd_kernel<float>, float());
+  return check_launch(fn);
+}

@@ -150,6 +150,41 @@ def preference_loss(logits, targets, ref_log_probs=None, beta: float = 0.1, labe
 
 
 # ---------------------------------------------------------------------------------------------------------------
+# Layers whose activations are held in 8 bits (ops.Mx8: e4m3, one power-of-two scale for every 32 values of a row).  They multiply
+# at the 8-bit rate of the matrix instructions and keep 8-bit values for the backward.  Their gradients are those of the layer with these values in the
+# place of the activations, a rounding counting as the identity; the input's gradient goes through the weight itself.  All of them need
+# bf16 (swiglu_8bit: or fp32) and an inner size that is a multiple of 32; gradients cannot be differentiated again.
+
+def _packed(packed):
+    return None if packed is None else packed.pair
+
+
+def linear_8bit(x, weight, packed=None):
+    """x [..., in] times weight [out, in]^T with both in 8 bits, bf16.  Of x its 8-bit form is kept, a byte a value.  `packed`: ops.mx8_quantize(weight) made
+    beforehand, where the weight stays the same for several calls (frozen, or the micro-batches of a step)."""
+    return _lib.host().linear_8bit(x, weight, _packed(packed))
+
+
+def rms_norm_linear_8bit(x, residual, norm_weight, eps, weight, packed=None, parts=()):
+    """h = x + residual (x where residual is None); returns (rmsnorm(h) * norm_weight times weight^T, h): a norm and the projection behind it, between which the
+    activations exist in 8 bits only, for the forward and the backward.  `packed` as in linear_8bit.  `parts`: Parameters that alias `weight`, row block by row
+    block, and take its gradient (q, k and v, or gate and up)."""
+    return _lib.host().rms_norm_linear_8bit(x, residual, norm_weight, eps, weight, _packed(packed), list(parts))
+
+
+def swiglu_8bit(gate_up):
+    """silu(gate) * up of the two halves of gate_up [..., 2 I] in its dtype; for the backward gate and up are kept in 8 bits and the
+    gradient is taken at the values that these stand for."""
+    return _lib.host().swiglu_8bit(gate_up)
+
+
+def swiglu_linear_8bit(gate_up, weight, packed=None):
+    """silu(gate) * up, in 8 bits, times weight [out, I]^T: bf16 [..., out].  What is kept are gate and up in 8 bits, 2 I bytes a row (swiglu and a
+    projection keep 6 I); the gradients of gate_up and of weight are taken at the values that these stand for.  `packed` as in linear_8bit."""
+    return _lib.host().swiglu_linear_8bit(gate_up, weight, _packed(packed))
+
+
+# ---------------------------------------------------------------------------------------------------------------
 # Fused projections.  The reference's q_proj / k_proj / v_proj (and gate_proj / up_proj) read the same activation;
 # their weights are kept as separate Parameters but laid out back to back in one buffer, so one GEMM produces all
 # outputs, one GEMM all weight gradients and one GEMM the (already summed) input gradient.  The pieces below hand

@@ -35,8 +35,8 @@ import torch.nn.functional as F
 import picotron_amd.process_group_manager as pgm
 from picotron_amd import _lib
 from picotron_amd.context_parallel import context_parallel
-from picotron_amd.functional import (linear_log_probs, log_probs, FusedLinearFunc, QKVAttentionFunc, RMSNormFunc, RMSNormHeadFunc, RMSNormResidualFunc,
-                                     RotaryFunc, SwiGLUFunc, SwiGLUFusedFunc, _fused_rope)
+from picotron_amd.functional import (linear_log_probs, log_probs, rms_norm_linear_8bit, swiglu_linear_8bit, FusedLinearFunc, QKVAttentionFunc, RMSNormFunc,
+                                     RMSNormHeadFunc, RMSNormResidualFunc, RotaryFunc, SwiGLUFunc, SwiGLUFusedFunc, _fused_rope)
 
 
 def apply_rotary_pos_emb(x, cos, sin):
@@ -139,6 +139,13 @@ def _fused_residual() -> bool:
     return os.getenv("PICO_FUSED_RESIDUAL", "1") != "0"
 
 
+def _linear_8bit() -> bool:
+    """PICO_LINEAR_8BIT=1: the projections behind the layers' norms (q, k and v; gate and up) and behind SwiGLU multiply in 8 bits, and the activations that
+    their backward reads are kept in 8 bits.  Weights, gradients and the residual stream stay as they are.  Needs the residual adds inside the norms and the fused
+    projections (both the default), bf16, and sizes that are multiples of 32."""
+    return os.getenv("PICO_LINEAR_8BIT", "0") == "1"
+
+
 def _fused_weight(owner, name, linears):
     """The [sum(out_i), in] buffer that the weights of `linears` alias, row block by row block.  Built on first use
     and rebuilt whenever the Parameters were moved or cast since (``model.to(...)`` gives them fresh storage); the
@@ -205,32 +212,40 @@ class Attention(nn.Module):
         for proj in (self.q_proj, self.k_proj, self.v_proj, self.out_proj):
             _fan_in_uniform_(proj.weight)
 
+    def qkv_weights(self):
+        """(buffer, its parts): the weights of q, k and v as one."""
+        linears = (self.q_proj, self.k_proj, self.v_proj)
+        return _fused_weight(self, "_qkv_weight", linears), [m.weight for m in linears]
+
+    def from_qkv(self, qkv, cos, sin):
+        """What follows the fused projection [batch, seq, q, k and v beside one another]."""
+        batch_size, seq_length, _ = qkv.size()
+        if os.getenv("CONTEXT_PARALLEL", "0") != "1":
+            out = QKVAttentionFunc.apply(qkv, cos, sin, self.num_local_heads, self.num_local_kv_heads, self.head_dim, True)
+            return self.out_proj(out)
+        nq, nkv = self.num_local_heads * self.head_dim, self.num_local_kv_heads * self.head_dim
+        q = qkv[..., :nq].view(batch_size, seq_length, self.num_local_heads, self.head_dim).transpose(1, 2)
+        k = qkv[..., nq:nq + nkv].view(batch_size, seq_length, self.num_local_kv_heads, self.head_dim).transpose(1, 2)
+        v = qkv[..., nq + nkv:].view(batch_size, seq_length, self.num_local_kv_heads, self.head_dim).transpose(1, 2)
+        sm_scale = 1.0 / (self.head_dim ** 0.5)
+        whole_cos, whole_sin = getattr(cos, "whole_table", None), getattr(sin, "whole_table", None)
+        rank_pos = pgm.process_group_manager.cp_rank * seq_length
+        if (_fused_rope() and whole_cos is not None and whole_sin is not None
+                and whole_cos[1] == rank_pos and whole_sin[1] == rank_pos):
+            # RoPE inside the ring: q rotated in the attention forward at the rank's absolute positions, k by one
+            # launch before its chunk is published, dq / dk un-rotated in the backward kernels' epilogues
+            out = context_parallel.ring_attention(q, k, v, sm_scale, True, rope=(whole_cos[0], whole_sin[0]))
+        else:
+            out = context_parallel.ring_attention(apply_rotary_pos_emb(q, cos, sin), apply_rotary_pos_emb(k, cos, sin), v,
+                                                  sm_scale, True)
+        return self.out_proj(out.transpose(1, 2).reshape(batch_size, seq_length, nq))
+
     def forward(self, x, cos, sin, attention_mask=None, position_ids=None):
         batch_size, seq_length, _ = x.size()
-        context = os.getenv("CONTEXT_PARALLEL", "0") == "1"
         if _fused_projections() and cos.size(0) >= seq_length:
             # one GEMM for q, k and v; RoPE, attention and their backward work on strided views of the fused buffers
-            w = _fused_weight(self, "_qkv_weight", (self.q_proj, self.k_proj, self.v_proj))
-            qkv = FusedLinearFunc.apply(x, w, self.q_proj.weight, self.k_proj.weight, self.v_proj.weight)
-            if not context:
-                out = QKVAttentionFunc.apply(qkv, cos, sin, self.num_local_heads, self.num_local_kv_heads, self.head_dim, True)
-                return self.out_proj(out)
-            nq, nkv = self.num_local_heads * self.head_dim, self.num_local_kv_heads * self.head_dim
-            q = qkv[..., :nq].view(batch_size, seq_length, self.num_local_heads, self.head_dim).transpose(1, 2)
-            k = qkv[..., nq:nq + nkv].view(batch_size, seq_length, self.num_local_kv_heads, self.head_dim).transpose(1, 2)
-            v = qkv[..., nq + nkv:].view(batch_size, seq_length, self.num_local_kv_heads, self.head_dim).transpose(1, 2)
-            sm_scale = 1.0 / (self.head_dim ** 0.5)
-            whole_cos, whole_sin = getattr(cos, "whole_table", None), getattr(sin, "whole_table", None)
-            rank_pos = pgm.process_group_manager.cp_rank * seq_length
-            if (_fused_rope() and whole_cos is not None and whole_sin is not None
-                    and whole_cos[1] == rank_pos and whole_sin[1] == rank_pos):
-                # RoPE inside the ring: q rotated in the attention forward at the rank's absolute positions, k by one
-                # launch before its chunk is published, dq / dk un-rotated in the backward kernels' epilogues
-                out = context_parallel.ring_attention(q, k, v, sm_scale, True, rope=(whole_cos[0], whole_sin[0]))
-            else:
-                out = context_parallel.ring_attention(apply_rotary_pos_emb(q, cos, sin), apply_rotary_pos_emb(k, cos, sin), v,
-                                                      sm_scale, True)
-            return self.out_proj(out.transpose(1, 2).reshape(batch_size, seq_length, nq))
+            w, parts = self.qkv_weights()
+            return self.from_qkv(FusedLinearFunc.apply(x, w, *parts), cos, sin)
         # [B,S,H*D] -> [B,H,S,D] views over [B,S,H,D] memory; the kernels take the strides as they are
         q = self.q_proj(x).view(batch_size, seq_length, self.num_local_heads, self.head_dim).transpose(1, 2)
         k = self.k_proj(x).view(batch_size, seq_length, self.num_local_kv_heads, self.head_dim).transpose(1, 2)
@@ -263,11 +278,15 @@ class MLP(nn.Module):
         for proj in (self.up_proj, self.gate_proj, self.down_proj):
             _fan_in_uniform_(proj.weight)
 
+    def gate_up_weights(self):
+        """(buffer, its parts): the weights of gate and up as one."""
+        linears = (self.gate_proj, self.up_proj)
+        return _fused_weight(self, "_gate_up_weight", linears), [m.weight for m in linears]
+
     def forward(self, x):
         if _fused_projections():
-            w = _fused_weight(self, "_gate_up_weight", (self.gate_proj, self.up_proj))
-            gate_up = FusedLinearFunc.apply(x, w, self.gate_proj.weight, self.up_proj.weight)
-            return self.down_proj(SwiGLUFusedFunc.apply(gate_up))
+            w, parts = self.gate_up_weights()
+            return self.down_proj(SwiGLUFusedFunc.apply(FusedLinearFunc.apply(x, w, *parts)))
         return self.down_proj(SwiGLUFunc.apply(self.gate_proj(x), self.up_proj(x)))
 
 
@@ -329,10 +348,24 @@ class DecoderLayer(nn.Module):
         returns (mlp output, residual stream before it) for the next norm to add.  Forward values are those of
         forward(); in the backward the gradient of the residual stream enters the norm's backward kernel, so no
         separate add runs on either pass."""
+        if _linear_8bit():
+            return self.forward_chained_8bit(branch, residual)
         y, residual = self.input_layernorm(branch, residual=residual, prenorm=True)
         a = self.attention(y, self.cos, self.sin, attention_mask, position_ids)
         y, residual = self.post_attention_layernorm(a, residual=residual, prenorm=True)
         return self.mlp(y), residual
+
+    def forward_chained_8bit(self, branch, residual):
+        """forward_chained where the activations between each norm and its projection, and between SwiGLU and the down projection, exist in 8 bits only, and gate and up are
+        kept for the backward that way."""
+        if not _fused_projections() or self.cos.size(0) < branch.size(1):
+            raise RuntimeError("PICO_LINEAR_8BIT=1 needs the fused projections (PICO_FUSED_PROJ) and RoPE tables as long as the sequence")
+        norm, (w, parts) = self.input_layernorm, self.attention.qkv_weights()
+        qkv, residual = rms_norm_linear_8bit(branch, residual, norm.weight, norm.eps, w, parts=parts)
+        a = self.attention.from_qkv(qkv, self.cos, self.sin)
+        norm, (w, parts) = self.post_attention_layernorm, self.mlp.gate_up_weights()
+        gate_up, residual = rms_norm_linear_8bit(a, residual, norm.weight, norm.eps, w, parts=parts)
+        return swiglu_linear_8bit(gate_up, self.mlp.down_proj.weight), residual
 
 
 class Embedding(nn.Module):
@@ -406,6 +439,8 @@ class Llama(nn.Module):
             for layer in self.decoder_layers:
                 x, residual = layer.forward_chained(x, residual)
             return self.final_norm(x, residual=residual)
+        if _linear_8bit():
+            raise RuntimeError("PICO_LINEAR_8BIT=1 needs the residual adds inside the norms (PICO_FUSED_RESIDUAL, FLASH_ATTEN)")
         for layer in self.decoder_layers:
             x = layer(x)
         return self.final_norm(x)

@@ -409,3 +409,43 @@ def cross_entropy_bwd(logits: torch.Tensor, targets: torch.Tensor, lse: torch.Te
                       ignore_index: int = -100, inplace: bool = False) -> torch.Tensor:
     """dlogits = (softmax(logits) - onehot(targets)) * scale, scale a one-element fp32 tensor on the device."""
     return _lib.host().cross_entropy_bwd(logits, targets, lse, scale, ignore_index, inplace)
+
+
+# ------------------------------------------------------------------------------- activations and weights in 8 bits
+class Mx8:
+    """A tensor held in 8 bits: ``data`` float8_e4m3fn [..., cols] and ``scales`` uint8 [ceil(cols / 128), rows, 4], byte (t, r, q) the power of
+    two, 2^(byte - 127), of columns 128 t + 32 q .. + 31 of row r.  The scale of 32 values is the smallest power of two under which they fit e4m3
+    (448), so nothing saturates and a value is off by at most 2^-4 of itself (2^-10 of the scale where it is under 2^-6 of it); a block that holds an infinity or
+    a NaN is NaN as a whole.  Made by mx8_quantize and rmsnorm_mx8_fwd."""
+
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor):
+        self.data, self.scales = data, scales
+
+    @property
+    def shape(self):
+        return self.data.shape
+
+    @property
+    def pair(self):
+        return self.data, self.scales
+
+    def dequantize(self, dtype=torch.bfloat16) -> torch.Tensor:
+        """The values it stands for, in bf16 or fp32 (both hold them exactly from 2^-126 on)."""
+        return _lib.host().mx8_dequantize(self.pair, dtype)
+
+
+def mx8_quantize(x: torch.Tensor) -> Mx8:
+    """x [..., cols] (bf16 or fp32, cols a multiple of 32) in 8 bits.  No gradient passes."""
+    return Mx8(*_lib.host().mx8_quantize(x))
+
+
+def mx8_product(a: Mx8, b: Mx8) -> torch.Tensor:
+    """a [..., K] b [N, K]^T in bf16, from fp32 sums.  No gradient passes (functional.linear_8bit has one)."""
+    return _lib.host().mx8_product(a.pair, b.pair)
+
+
+def rmsnorm_mx8_fwd(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: Optional[torch.Tensor] = None):
+    """rmsnorm(h) * weight for h = x + residual (bf16 or fp32, hidden a multiple of 32 up to 16384), written in 8 bits only: returns (Mx8, rstd fp32 [rows], h or
+    None without a residual).  The sum that is normalised is not rounded to x's dtype on the way, h is."""
+    data, scales, rstd, h = _lib.host().rmsnorm_mx8_fwd(x, weight, eps, residual)
+    return Mx8(data, scales), rstd, h

@@ -1,0 +1,275 @@
+"""Activations and weights in 8 bits against float64: the form itself, what writes it, the product of two such operands.
+
+Rounding to bf16 is off by at most 2^-8 of the value, to e4m3 by 2^-4 of it (by 2^-10 of the scale where it is under 2^-6 of that).
+"""
+import ctypes
+
+import pytest
+import torch
+
+from oracle import mx8 as O
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32, F64 = torch.bfloat16, torch.float32, torch.float64
+SIZES = [(1, 32), (1, 2048), (2, 96), (3, 128), (5, 160), (33, 576), (64, 4096), (257, 1056), (7, 11008)]
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def wide(rows, cols, g, dtype=F32):
+    """Normal values whose rows and channels differ by many powers of two."""
+    x = torch.randn(rows, cols, generator=g, device="cuda") * torch.exp2(torch.randint(-12, 13, (rows, 1), generator=g, device="cuda").float())
+    return (x * torch.exp2(torch.randint(-4, 5, (1, cols), generator=g, device="cuda").float())).to(dtype)
+
+
+def agrees(packed, v):
+    """packed is exactly the oracle's 8-bit form of v (float64 [rows, cols])."""
+    q, e = O.quantize(v)
+    assert torch.equal(O.exponents_of(packed.scales, v.size(1)), e)
+    pad = packed.scales.permute(1, 0, 2).reshape(v.size(0), 4 * packed.scales.size(0))[:, v.size(1) // 32:]
+    assert (pad == 0).all()
+    for dtype in (F32, BF16):
+        got, want = packed.dequantize(dtype).view(v.shape), q.to(dtype)      # (which holds them, but for 2^128, the largest finite values rounded up)
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got[~got.isnan()], want[~want.isnan()])
+
+
+# ------------------------------------------------------------------------------------------------- the form
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,cols", SIZES)
+def test_quantize_is_exact(device, rows, cols, dtype):
+    from picotron_amd import ops
+    x = wide(rows, cols, gen(rows + cols), dtype)
+    agrees(ops.mx8_quantize(x), x.double())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_borders_of_the_form(device, dtype):
+    """Every code and every middle between two, at scales over the whole range; blocks of zeros, of the smallest values, and of the largest."""
+    from picotron_amd import ops
+    codes = torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    v = torch.cat((codes, (codes[1:] + codes[:-1]) / 2)).cuda()
+    v = torch.cat((v, -v))
+    rows = []
+    for k in (-110, -30, 0, 1, 30, 100):
+        block = torch.zeros(len(v), 32, dtype=F64, device="cuda")
+        block[:, 7], block[:, 8] = 448, v
+        rows.append(block * 2.0 ** k)
+    odd = torch.zeros(12, 32, dtype=F64, device="cuda")
+    largest = torch.finfo(dtype).max
+    odd[1, 3], odd[2, 3], odd[3, 31], odd[4, 0] = 2.0 ** -126, -2.0 ** -133, largest, -largest
+    odd[5] = 1e-20
+    odd[6, :] = 2.0 ** -118 * 1.75
+    odd[7, 9], odd[7, 10] = 2.0 ** -118 * 1.875, 2.0 ** -130
+    odd[8] = -0.0
+    odd[9, 4], odd[9, 5] = 448 * 2.0 ** -127, 2.0 ** -133
+    odd[10, 1], odd[11, 30] = 464, 480
+    x = torch.cat(rows + [odd]).to(dtype)
+    agrees(ops.mx8_quantize(x), x.double())
+    x3 = x[: x.size(0) // 3 * 3].view(-1, 96)       # the same blocks beside one another
+    agrees(ops.mx8_quantize(x3), x3.double())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_infinities_and_nans_take_their_block(device, dtype):
+    from picotron_amd import ops
+    x = wide(9, 320, gen(1), dtype)
+    x[1, 40], x[2, 319], x[4, 0], x[4, 100] = float("inf"), -float("inf"), float("nan"), 1
+    packed = ops.mx8_quantize(x)
+    agrees(packed, x.double())
+    bad = torch.zeros(9, 10, dtype=torch.bool, device="cuda")
+    bad[1, 1] = bad[2, 9] = bad[4, 0] = True
+    assert torch.equal(packed.dequantize().view(9, 10, 32).isnan().all(-1), bad) and torch.equal(packed.dequantize().view(9, 10, 32).isnan().any(-1), bad)
+
+
+def test_views_and_shapes(device):
+    """Column slices, rows that start anywhere, steps between rows, expanded and transposed tensors, more axes, none."""
+    from picotron_amd import ops
+    g = gen(2)
+    base = wide(40, 520, g, BF16)
+    views = [base[:, 128:288], base[:, 1:161], base[::3, 8:72], base[:, :512].t()[:, :32], base[:, :64].expand(3, 40, 64), base[:1, :64].expand(7, 64), base[0, 32:64],
+             base[:, :512].reshape(4, 10, 512)[:, 2:5], base[:, :320].reshape(8, 5, 320).transpose(0, 1), base[:0, :64], torch.randn(2, 0, 64, device="cuda")]
+    for v in views:
+        packed = ops.mx8_quantize(v)
+        assert packed.shape == v.shape and packed.dequantize().shape == v.shape
+        agrees(packed, v.double().reshape(-1, v.size(-1)))
+    z = torch.complex(base[:, :64].float(), -base[:, :64].float()).conj().imag       # lazily negated
+    agrees(ops.mx8_quantize(z), z.double().resolve_neg())
+
+
+def test_nothing_around_the_outputs_is_written(device):
+    """Through the C ABI, into the middle of larger buffers, with pitches."""
+    from picotron_amd import _lib
+    lib, g = _lib.lib(), gen(4)
+    rows, cols, ld = 5, 160, 168
+    x = wide(rows, ld, g, BF16)
+    p = lambda t, off=0: ctypes.c_void_p(t.data_ptr() + off)      # noqa: E731
+    data, scales = torch.full((rows * cols + 64,), 77, dtype=torch.uint8, device="cuda"), torch.full((2 * rows * 4 + 32,), 77, dtype=torch.uint8, device="cuda")
+    y8 = _lib.Mx8(data.data_ptr() + 32, scales.data_ptr() + 16)
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    _lib.check(lib.pico_mx8_quantize(p(x), ctypes.byref(y8), rows, cols, ld, 0, stream))
+    assert (data[:32] == 77).all() and (data[-32:] == 77).all() and (scales[:16] == 77).all() and (scales[-16:] == 77).all()
+    out = torch.full((rows + 2, ld), 5.0, dtype=BF16, device="cuda")
+    _lib.check(lib.pico_mx8_dequantize(ctypes.byref(y8), p(out[1:]), rows, cols, ld, 0, stream))
+    q, _ = O.quantize(x[:, :cols].double())
+    assert torch.equal(out[1:-1, :cols].double(), q) and (out[:, cols:] == 5).all() and (out[0] == 5).all() and (out[-1] == 5).all()
+    dy, dg, du = wide(rows, ld, g, BF16), torch.full((rows + 1, ld), 5.0, dtype=BF16, device="cuda"), torch.full((rows + 1, ld), 5.0, dtype=BF16, device="cuda")
+    _lib.check(lib.pico_swiglu_mx8_bwd(p(dy), ctypes.byref(y8), ctypes.byref(y8), p(dg), p(du), None, rows, cols, ld, ld, ld, 0, stream))
+    assert (dg[:, cols:] == 5).all() and (dg[-1] == 5).all() and (du[:, cols:] == 5).all() and (du[-1] == 5).all() and not (dg[:-1, :cols] == 5).all()
+
+
+# ------------------------------------------------------------------------------------------------- RMSNorm
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("rows,cols", SIZES + [(3, 16384), (4, 8192), (6, 5152), (1021, 192)])
+def test_norm(device, rows, cols, residual, dtype):
+    from picotron_amd import ops
+    g = gen(rows * 7 + cols)
+    x = wide(rows, cols, g, dtype)
+    res = wide(rows, cols, g, dtype) if residual else None
+    w = (1 + 0.3 * torch.randn(cols, generator=g, device="cuda")).to(dtype)
+    packed, rstd, h = ops.rmsnorm_mx8_fwd(x, w, 1e-5, residual=res)
+    exact = (x.float() + res.float()).double() if residual else x.double()      # (the sum is fp32)
+    if residual:
+        assert torch.equal(h, (x.float() + res.float()).to(dtype))
+    else:
+        assert h is None
+    want_rstd = (exact.pow(2).mean(-1) + 1e-5).rsqrt()
+    # a sum of cols squares in fp32, 64 lanes or more side by side: (cols / 64 + 10) roundings of at most 2^-24 each, and a few for the root and the products
+    delta = (cols / 64 + 24) * 2.0 ** -24
+    assert ((rstd.double() - want_rstd).abs() <= delta * want_rstd).all()
+    y = exact * want_rstd[:, None] * w.double()
+    got, s = packed.dequantize(F32).double(), O.power(O.exponents_of(packed.scales, cols)).repeat_interleave(32, 1)
+    assert ((got - y).abs() <= (2.0 ** -4 * (1 + delta) + delta) * y.abs() + 2.0 ** -10 * s).all()
+    # a value that is delta off rounds differently only within delta of a middle, and those lie 2^-4 of the value apart at least: 2^5 delta of all, and the block's
+    # scale (with it what lies under 2^-6 of it) where its largest is that near to 448 times a power of two
+    q, e = O.quantize(y)
+    differ = (got != q).sum().item()
+    assert differ <= 2.0 ** 6 * delta * y.numel() + 40, differ
+    assert (O.exponents_of(packed.scales, cols) != e).sum().item() <= 2
+
+
+def test_norm_rows_of_zeros_infinities_and_far_scales(device):
+    from picotron_amd import ops
+    x = torch.randn(6, 256, device="cuda")
+    x[1], x[2, 5], x[3, 200] = 0, float("inf"), float("nan")
+    x[4] *= 1e-30
+    x[5] *= 1e15
+    packed, rstd, _ = ops.rmsnorm_mx8_fwd(x, torch.ones(256, device="cuda"), 1e-5)
+    v = packed.dequantize(F32)
+    assert (v[1] == 0).all() and v[3].isnan().all() and v[2].view(8, 32)[0].isnan().all() and not v[[0, 4, 5]].isnan().any()
+    assert (v[5].double().pow(2).mean().sqrt() - 1).abs() < 2.0 ** -4      # every value is off by at most 2^-4 of itself
+
+
+# ------------------------------------------------------------------------------------------------- the product
+
+PRODUCTS = [(1, 1, 32), (1, 8, 64), (1, 2048, 2048), (2, 49, 96), (5, 1000, 160), (16, 64, 128), (17, 33, 224), (24, 2048, 8192), (33, 576, 576), (64, 100, 4096), (65, 256, 288),
+            (100, 7, 1056), (128, 128, 256), (130, 264, 384), (256, 256, 512), (257, 513, 576), (333, 1728, 576), (512, 640, 2080), (1003, 520, 1376), (700, 4096, 320),
+            (1024, 1024, 4096), (2049, 2056, 1056), (4100, 300, 544)]
+
+
+@pytest.mark.parametrize("M,N,K", PRODUCTS)
+def test_product(device, M, N, K):
+    from picotron_amd import ops
+    g = gen(M + N + K)
+    a, b = ops.mx8_quantize(wide(M, K, g)), ops.mx8_quantize(wide(N, K, g))
+    va, vb = a.dequantize(F32).double(), b.dequantize(F32).double()
+    got = ops.mx8_product(a, b)
+    assert got.shape == (M, N) and got.dtype == BF16 and got.is_contiguous()
+    ref = va @ vb.t()
+    # Rounding to bf16; fp32 sums over the instructions; within one of them the products of eight neighbours lose what lies 2^-13 below the largest of the eight
+    # (2^16 and 2^e added: 2^3 stays, 2^2 is lost), so 28 * 2^-13 of the largest in a block of 32, which is bounded by the operands' largest.  (Rows and channels differ by
+    # powers of two: block by block.)
+    blocks = lambda v: v.abs().view(v.size(0), -1, 32).amax(-1)      # noqa: E731
+    steps = (K + 127) // 128
+    cut = 28 * 2.0 ** -13 * (blocks(va) @ blocks(vb).t()) + (steps + 8) * 2.0 ** -24 * (va.abs() @ vb.abs().t())
+    assert ((got.double() - ref).abs() <= 2.0 ** -8 * ref.abs() + cut).all()
+    assert (got.double() - ref).norm() <= (2.0 ** -8 + 2.0 ** -12) * ref.norm() + (cut.norm() if M * N < 64 else 0)
+    assert torch.equal(got, ops.mx8_product(a, b))
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 64, 128), (20, 40, 288), (300, 520, 416), (600, 300, 2048)])
+def test_product_of_exact_sums(device, M, N, K):
+    """Small whole numbers under different scales: every sum is exact, so a value at the wrong place, or under another block's scale, shows."""
+    from picotron_amd import ops
+    g = gen(K)
+    def rows(n):
+        v = torch.randint(-3, 4, (n, K), generator=g, device="cuda").float().view(n, -1, 32)
+        v[..., 0] = 3       # (so that a block's scale is known)
+        return (v * torch.exp2(torch.randint(-1, 2, (n, K // 32, 1), generator=g, device="cuda").float())).view(n, K)
+    x, w = rows(M), rows(N)
+    a, b = ops.mx8_quantize(x), ops.mx8_quantize(w)
+    assert torch.equal(a.dequantize(F32), x)
+    ref = x.double() @ w.double().t()
+    assert torch.equal(ops.mx8_product(a, b), ref.to(BF16))
+
+
+@pytest.mark.parametrize("M,N,K", [(3, 40, 160), (300, 300, 416), (600, 520, 1056)])
+def test_a_nan_reaches_its_row_or_column_only(device, M, N, K):
+    from picotron_amd import ops
+    x, w = wide(M, K, gen(1)), wide(N, K, gen(2))
+    x[M // 2, K - 1], w[N // 3, 0] = float("nan"), float("inf")
+    got = ops.mx8_product(ops.mx8_quantize(x), ops.mx8_quantize(w))
+    bad = torch.zeros(M, N, dtype=torch.bool, device="cuda")
+    bad[M // 2] = True
+    bad[:, N // 3] = True
+    assert torch.equal(got.isnan(), bad)
+
+
+def test_product_of_more_axes_and_of_nothing(device):
+    from picotron_amd import ops
+    g = gen(5)
+    x, w = torch.randn(2, 3, 5, 64, generator=g, device="cuda"), torch.randn(9, 64, generator=g, device="cuda")
+    b = ops.mx8_quantize(w)
+    y = ops.mx8_product(ops.mx8_quantize(x), b)
+    assert y.shape == (2, 3, 5, 9) and torch.equal(y.view(30, 9), ops.mx8_product(ops.mx8_quantize(x.view(30, 64)), b))
+    assert ops.mx8_product(ops.mx8_quantize(x[:, :0]), b).shape == (2, 0, 5, 9)
+    assert ops.mx8_product(ops.mx8_quantize(x[0, 0, 0]), b).shape == (9,)
+    assert ops.mx8_product(ops.mx8_quantize(x), ops.mx8_quantize(w[:0])).shape == (2, 3, 5, 0)
+
+
+def test_the_product_writes_its_columns_only(device):
+    """Through the C ABI: nothing before or behind c, zeros in the columns that round its rows up."""
+    from picotron_amd import _lib, ops
+    lib = _lib.lib()
+    for M, N, K in [(3, 13, 64), (50, 100, 256), (300, 261, 512), (520, 1001, 1056)]:
+        a, b = ops.mx8_quantize(wide(M, K, gen(1))), ops.mx8_quantize(wide(N, K, gen(2)))
+        ldc = (N + 7) // 8 * 8
+        buf = torch.full((M * ldc + 128,), 3.0, dtype=BF16, device="cuda")
+        bytes_ = lib.pico_mx8_product_workspace_bytes(M, N, K)
+        ws = torch.full((bytes_ + 64,), 9, dtype=torch.uint8, device="cuda")
+        ca, cb = (_lib.Mx8(t.data.data_ptr(), t.scales.data_ptr()) for t in (a, b))
+        _lib.check(lib.pico_mx8_product(ctypes.byref(ca), ctypes.byref(cb), ctypes.c_void_p(buf.data_ptr() + 128), M, N, K, ctypes.c_void_p(ws.data_ptr()), bytes_,
+                                        ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))
+        c = buf[64:-64].view(M, ldc)
+        assert (buf[:64] == 3).all() and (buf[-64:] == 3).all() and (ws[bytes_:] == 9).all()
+        assert (c[:, N:] == 0).all() and torch.equal(c[:, :N].contiguous(), ops.mx8_product(a, b))
+
+
+def test_operands_that_do_not_fit(device):
+    from picotron_amd import ops
+    a, b = ops.mx8_quantize(torch.ones(4, 64, device="cuda")), ops.mx8_quantize(torch.ones(8, 96, device="cuda"))
+    with pytest.raises(RuntimeError, match="weight of"):
+        ops.mx8_product(a, b)
+    with pytest.raises(RuntimeError, match="weight of"):
+        ops.mx8_product(a, ops.mx8_quantize(torch.ones(2, 8, 64, device="cuda")))
+    with pytest.raises(RuntimeError, match="multiple of 32"):
+        ops.mx8_quantize(torch.ones(4, 40, device="cuda"))
+    with pytest.raises(RuntimeError, match="multiple of 32"):
+        ops.mx8_quantize(torch.tensor(1.0, device="cuda"))
+    with pytest.raises(RuntimeError, match="not supported"):
+        ops.mx8_quantize(torch.ones(4, 64, device="cuda", dtype=torch.float16))
+    with pytest.raises(RuntimeError, match="not supported"):
+        a.dequantize(torch.float16)
+    with pytest.raises(RuntimeError, match="scales"):
+        ops.Mx8(a.data, b.scales).dequantize()
+    with pytest.raises(RuntimeError, match="float8_e4m3fn"):
+        ops.Mx8(a.data.float(), a.scales).dequantize()
+    with pytest.raises(RuntimeError, match="float8_e4m3fn"):
+        ops.Mx8(a.data.t(), a.scales).dequantize()
+    with pytest.raises(RuntimeError, match="residual"):
+        ops.rmsnorm_mx8_fwd(torch.ones(4, 64, device="cuda"), torch.ones(64, device="cuda"), 1e-5, residual=torch.ones(3, 64, device="cuda"))
+    with pytest.raises(RuntimeError, match="norm's weight"):
+        ops.rmsnorm_mx8_fwd(torch.ones(4, 64, device="cuda"), torch.ones(32, device="cuda"), 1e-5)
