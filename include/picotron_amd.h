@@ -566,6 +566,10 @@ int pico_swiglu_mx8_bwd(const void* dy, const pico_mx8* gate8, const pico_mx8* u
  * [N, K].  workspace: pico_mx8_product_workspace_bytes bytes, 16-byte aligned (NULL where that is 0). */
 int64_t pico_mx8_product_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int pico_mx8_product(const pico_mx8* a, const pico_mx8* b, void* c, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
+/* The same in given tiles, each side 128 or 256, the contraction in `parts` pieces of two steps of 128 at least (parts > 1: workspace of parts * M * (N rounded
+ * up) * 4 bytes), or, tile_m = 0, in the kernel of few rows.  What pico_mx8_product goes to by its rules. */
+int pico_mx8_product_tiled(const pico_mx8* a, const pico_mx8* b, void* c, int64_t M, int64_t N, int64_t K, int tile_m, int tile_n, int parts,
+                           void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------ optimizer step
  * replaces: torch.optim.AdamW(model.parameters(), lr).step()  train.py:204-209,240  for low-precision parameters

@@ -47,7 +47,6 @@ __global__ __launch_bounds__(W * kWave) void product_mx8_few_kernel(const Mx8Par
     const u32x4 low = k + 16 * h < p.K ? *reinterpret_cast<const u32x4*>(at) : zero, high = k + 64 + 16 * h < p.K ? *reinterpret_cast<const u32x4*>(at + 64) : zero;
     return both(low, high);
   };
-#pragma unroll 2
   for (int t = wave; t < steps; t += W) {
     i32x8 fa[MT], fb[NT];
     int sa[MT], sb[NT];
@@ -91,13 +90,333 @@ void launch_few(const Mx8Params& p, hipStream_t s) {
   hipLaunchKernelGGL((product_mx8_few_kernel<MT, NT, W>), dim3((p.N + 16 * NT - 1) / (16 * NT), (p.M + 16 * MT - 1) / (16 * MT)), dim3(W * kWave), 0, s, p);
 }
 
+// ---- many rows: the large products' workgroups (product_large.h) with 128 of contraction a step
+//
+// An e4m3 matrix [rows, K] is staged as a bf16 one [rows, K / 2] would be: a step is 128 bytes of every row of the tiles.  2 x 4 waves of 32 I x 32 J;
+// each half of a step is one 32 x 32 x 64 product per pair of fragments.  The scales of a step's rows, four bytes a row, take one request more: 64 rows by each wave.
+struct Mx8Large : LargeParams {   // (a, b, K and the pitches in pairs of values; N without the columns that round the output up)
+  const uint8_t *sa, *sb;
+  int cols;                       // of c
+};
+// wait_requests<N> where `but` is not 0, wait_requests<0> where it is.  The branch is inside: products ahead of one that the compiler sees would be moved behind it.
+template <int N>
+__device__ __forceinline__ void wait_requests_but(int but) {
+  asm volatile("s_cmp_lg_u32 %0, 0\n\ts_cbranch_scc1 pico_but_%=\n\ts_waitcnt vmcnt(0)\npico_but_%=:\n\ts_waitcnt vmcnt(%1)" ::"s"(but), "n"(N) : "scc", "memory");
+}
+// unit_at of product_large.h in 32 bits and scalar registers: pieces times steps stay under 2^21 here, and a division of 64 bits takes the sizes, and with them the loops' counts and the
+// windows, through vector registers.
+template <int TM, int TN>
+__device__ __forceinline__ bool mx8_unit_at(const Mx8Large& p, int round, Unit& u) {
+  const int tiles = p.tiles_m * p.tiles_n, grid = gridDim.x, start = round * grid, count = min(grid, tiles * p.parts - start);
+  if (static_cast<int>(blockIdx.x) >= count) return false;
+  const int xcd = blockIdx.x % 8, id = start + xcd * (count / 8) + min(xcd, count % 8) + blockIdx.x / 8;
+  constexpr int kDeep = 8;
+  u.part = __builtin_amdgcn_readfirstlane(id / tiles);
+  const int t = id - u.part * tiles, block = __builtin_amdgcn_readfirstlane(t / (kDeep * p.tiles_n)), in = t - block * kDeep * p.tiles_n, deep = min(kDeep, p.tiles_m - block * kDeep);
+  const int column = __builtin_amdgcn_readfirstlane(in / deep);
+  u.m0 = (block * kDeep + in - column * deep) * TM;
+  u.n0 = column * TN;
+  const int steps = (p.K + kStep - 1) / kStep;
+  u.first = __builtin_amdgcn_readfirstlane(u.part * steps / p.parts);
+  u.steps = __builtin_amdgcn_readfirstlane((u.part + 1) * steps / p.parts) - u.first;
+  return true;
+}
+template <int I, int J>
+struct Mx8Shape {
+  static constexpr int kThreads = 512, TM = 64 * I, TN = 128 * J;
+  using A = Tile<false, TM, kThreads>;
+  using B = Tile<false, TN, kThreads>;
+  static constexpr int kBuffer = A::kBytes + B::kBytes, kScaleBytes = 2 * 256 * 4;   // (of up to 256 rows of a, and of b)
+  static constexpr int kScales = 2 * kBuffer, kRows = kScales + 2 * kScaleBytes, kRowRegion = 16 * 128;
+  static constexpr int kCounts = kRows + 8 * kRowRegion, kLds = kCounts + 16;
+  static_assert(kLds <= 160 * 1024);
+};
+template <int kPlus>
+__device__ __forceinline__ void request4_to(uint32_t lds_off, u32x4 window, uint32_t off) {   // request16_to of 4 bytes per lane
+  uint32_t aim;
+  asm volatile("s_add_u32 %0, %1, %2\n\ts_nop 0\n\tbuffer_load_dword %3, %4, 0 offen lds" : "=&{m0}"(aim) : "s"(lds_off), "n"(kPlus), "v"(off), "s"(window) : "scc", "memory");
+}
+
+// The tile leaves as in product_large.h, 16 rows and 128 bytes of columns at a time through LDS.  A lane holds, of row lane % 32 of a 32 x 32 block, columns 8 q + 4 h .. + 3:
+// two q change places between the two 16 rows, so that all lanes write each time (branches on lanes would cost the kernel its scalar registers).
+template <typename Out, int I, int J>
+__device__ __forceinline__ void store_tile32(Out* c, int64_t first_row, int M, int cols, bool streaming, int row0, int col0, int lane, unsigned char* rows, const f32x16 (&acc)[I][J]) {
+  constexpr int kBlocks = 128 / 32 / static_cast<int>(sizeof(Out)) < J ? 128 / 32 / static_cast<int>(sizeof(Out)) : J;   // of 32 columns at a time
+  constexpr int kWords = sizeof(Out);   // of four columns
+  const int n = lane % 16, odd = lane / 16 % 2, h = lane / 32, left = cols - col0;
+  const uint32_t pitch = static_cast<uint32_t>(cols) * sizeof(Out), back = lane / 8 * pitch + lane % 8 * 16;
+#pragma unroll
+  for (int i = 0; i < I; ++i) {
+#pragma unroll
+    for (int j0 = 0; j0 < J; j0 += kBlocks) {
+      uint32_t word[2][kBlocks][2][kWords];   // of the first and the second 16 rows: column blocks 2 k + odd
+#pragma unroll
+      for (int j = 0; j < kBlocks; ++j)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int w = 0; w < kWords; ++w) {
+            auto packed = [&](int q) {
+              if constexpr (sizeof(Out) == 4) return __float_as_uint(acc[i][j0 + j][4 * q + w]);
+              else return pack_bf16x2(acc[i][j0 + j][4 * q + 2 * w], acc[i][j0 + j][4 * q + 2 * w + 1]);
+            };
+            const auto swapped = __builtin_amdgcn_permlane16_swap(packed(2 * k), packed(2 * k + 1), false, false);
+            word[0][j][k][w] = swapped[0];
+            word[1][j][k][w] = swapped[1];
+          }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int j = 0; j < kBlocks; ++j)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            unsigned char* to = rows + n * 128;
+            const int q = 2 * k + odd;
+            if constexpr (sizeof(Out) == 4)
+              *reinterpret_cast<u32x4*>(to + ((j * 8 + 2 * q + h) ^ (n / 2)) * 16) = u32x4{word[half][j][k][0], word[half][j][k][1], word[half][j][k][2], word[half][j][k][3]};
+            else
+              *reinterpret_cast<u32x2*>(to + ((j * 4 + q) ^ (n / 2)) * 16 + h * 8) = u32x2{word[half][j][k][0], word[half][j][k][1]};
+          }
+        const int first = row0 + 32 * i + 16 * half, live = min(16, M - first);
+        const u32x4 r = request_window(reinterpret_cast<uint64_t>(c + (first_row + first) * cols + col0),
+                                       live > 0 && left > 0 ? static_cast<uint32_t>(((live - 1) * static_cast<int64_t>(cols) + left) * sizeof(Out)) : 0u);
+        const buffer_rsrc window = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(r[0] | static_cast<uint64_t>(r[1]) << 32), 0, static_cast<int>(r[2]), static_cast<int>(r[3]));
+        const int col = lane % 8 * (16 / static_cast<int>(sizeof(Out)));
+        const bool in = col < kBlocks * 32 && 32 * j0 + col < left;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int row = 8 * q + lane / 8;
+          const u32x4 v = *reinterpret_cast<const u32x4*>(rows + row * 128 + ((lane % 8) ^ (row / 2)) * 16);
+          const int to = in ? static_cast<int>(back + 8 * q * pitch + 32 * j0 * sizeof(Out)) : static_cast<int>(0xfffffff0u);
+          constexpr int kStreaming = 2;
+          if (streaming) __builtin_amdgcn_raw_buffer_store_b128(v, window, to, 0, kStreaming);
+          else __builtin_amdgcn_raw_buffer_store_b128(v, window, to, 0, 0);
+        }
+      }
+    }
+  }
+}
+
+template <int I, int J, bool kParts>
+__global__ __launch_bounds__(512, 2) void product_mx8_kernel(const Mx8Large p) {
+  using S = Mx8Shape<I, J>;
+  using A = typename S::A;
+  using B = typename S::B;
+  constexpr int TM = S::TM, TN = S::TN, kPA = A::kPieces, kPB = B::kPieces, kPieces = kPA + kPB;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+  const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int wm = wave / 4 * 32 * I, wn = wave % 4 * 32 * J, n = lane % 32, h = lane / 32;
+
+  // ---- requests (as in product_large_kernel; both operands have one pitch, and a thread's pieces lie 64 rows apart)
+  const uint32_t piece_bytes = static_cast<uint32_t>(p.lda) * (64 * 2);
+  uint32_t first_piece = A::offset(p.lda, tid, 0);
+  const int k_piece = (tid % 8 ^ (tid / 16 & 7)) * 8;
+  const bool ragged = p.K % kStep != 0;
+  Unit load;   // where the requests stand
+  int load_round = 0, load_step = 0;
+  mx8_unit_at<TM, TN>(p, 0, load);
+  Window wa, wb, ws;
+  // the scales of this wave's 64 rows: of a for the first four waves, of b for the others
+  const int s_rows = wave < 4 ? p.M : p.N, s_first = wave % 4 * 64;
+  const uint8_t* s_base = wave < 4 ? p.sa : p.sb;
+  auto open = [&]() __attribute__((always_inline)) {
+    wa = open_window<false>(p.a, p.lda, load.m0, TM, p.M, load.first * kStep, p.K);
+    wb = open_window<false>(p.b, p.ldb, load.n0, TN, p.N, load.first * kStep, p.K);
+    const int first = (wave < 4 ? load.m0 : load.n0) + s_first;
+    ws = {reinterpret_cast<uint64_t>(s_base) + (static_cast<int64_t>(load.first) * s_rows + first) * 4, first < s_rows ? static_cast<uint32_t>(min(s_rows - first, 64)) * 4 : 0u};
+  };
+  open();
+  u32x4 ra = resource(wa), rb = resource(wb), rs = resource(ws);
+  auto go_on = [&](int part) __attribute__((always_inline)) {
+    if (part == 0) {
+      ++load_step;
+      advance(wa, kStep * 2);
+    }
+    if (part == 1) {
+      advance(wb, kStep * 2);
+      ws.base += static_cast<uint32_t>(s_rows) * 4u;
+    }
+    if (part == 2 && load_step >= load.steps - 1) {
+      if (load_step == load.steps) {
+        load_step = 0;
+        const bool more = mx8_unit_at<TM, TN>(p, ++load_round, load);
+        open();
+        if (!more) wa.bytes = wb.bytes = ws.bytes = 0;   // requests past the work's end read no memory
+      }
+      if (ragged) {   // pieces past the contraction's end read as zeros (their scales are bytes of 0, no NaN)
+        // (a window is under 2^31 bytes, and so are three times piece_bytes)
+        first_piece = k_piece < p.K - (load.first + load_step) * kStep ? A::offset(p.lda, tid, 0) : 0x80000000u;
+      }
+    }
+    if (part == 3) {
+      ra = resource(wa);
+      rb = resource(wb);
+      rs = resource(ws);
+    }
+  };
+  const uint32_t lds_wave = wave * 1024, lds_scales = S::kScales + wave * 256;   // (dynamic LDS starts at 0: the build looks)
+  auto request = [&](auto piece, uint32_t buffer) __attribute__((always_inline)) {
+    constexpr int i = decltype(piece)::value;
+    if constexpr (i < kPA) request16_to<i * S::kThreads * 16>(lds_wave + buffer, ra, first_piece + i * piece_bytes);
+    else if constexpr (i < kPieces) request16_to<A::kBytes + (i - kPA) * S::kThreads * 16>(lds_wave + buffer, rb, first_piece + (i - kPA) * piece_bytes);
+    else request4_to<0>(lds_scales + (buffer != 0 ? S::kScaleBytes : 0), rs, static_cast<uint32_t>(lane) * 4);
+  };
+  constexpr int kRequests = kPieces + 1;
+  using Out = std::conditional_t<kParts, float, __bf16>;
+  constexpr int kAtOnce = 128 / 32 / static_cast<int>(sizeof(Out)), kStores = 2 * I * ((J + kAtOnce - 1) / kAtOnce) * 2;   // of a wave, at a tile's end
+
+  // ---- half a step: its products, row by row of the wave's tile.  A fragment of a is read anew, for the half step that follows, as soon as its row is done, those of b are
+  // held twice.  The workgroup meets once a step: a wave arrives behind the first product of the second half, when its reads of the buffer in use and its requests for the other
+  // one are complete, and waits a quarter of the half later; from there on it reads the other buffer and requests into the one in use.
+  constexpr int kProducts = I * J, kWait = kProducts / 4 > 1 ? kProducts / 4 : 1;
+  i32x8 fa[I], fb[2][J];
+  int sca[I], scb[2][J];
+  f32x16 acc[I][J];
+  // row `first` + n, bytes 64 s + 16 h and 32 further, and the scale of bytes 64 s + 32 h .. + 31
+  auto fragment = [&](const unsigned char* tile, int first, int s) __attribute__((always_inline)) {
+    const unsigned char* row = tile + first * 128 + n * 128;
+    return both(*reinterpret_cast<const u32x4*>(row + ((4 * s + h) ^ (n / 2 & 7)) * 16), *reinterpret_cast<const u32x4*>(row + ((4 * s + 2 + h) ^ (n / 2 & 7)) * 16));
+  };
+  auto scale = [&](uint32_t buffer, int first, int s) __attribute__((always_inline)) { return lds[S::kScales + (buffer != 0 ? S::kScaleBytes : 0) + (first + n) * 4 + 2 * s + h]; };
+  auto fetch_a = [&](uint32_t buffer, int s, int i) __attribute__((always_inline)) {
+    fa[i] = fragment(lds + buffer, wm + 32 * i, s);
+    sca[i] = scale(buffer, wm + 32 * i, s);
+  };
+  auto fetch_b = [&](uint32_t buffer, int s, int j) __attribute__((always_inline)) {
+    fb[s][j] = fragment(lds + buffer + A::kBytes, wn + 32 * j, s);
+    scb[s][j] = scale(buffer, 256 + wn + 32 * j, s);
+  };
+  int arrivals = 0;
+  auto half_step = [&](auto half, uint32_t next, uint32_t free, int stores) __attribute__((always_inline)) {
+    constexpr int s = decltype(half)::value, kFrom = s == 0 ? 0 : kWait;
+    each(std::make_integer_sequence<int, kProducts>(), [&](auto product) __attribute__((always_inline)) {
+      constexpr int m = decltype(product)::value, i = m / J, j = i % 2 ? J - 1 - m % J : m % J;
+      __builtin_amdgcn_sched_barrier(0);
+      // C^T: a lane holds columns of a row of C
+      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[s][j], fa[i], acc[i][j], 0, 0, 0, scb[s][j], 0, sca[i]);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (s == 1 && m == 0) {
+        // everything requested but the stores of the tile before, which were issued behind its requests
+        wait_requests_but<kStores>(stores);
+        wait_lds();
+        arrive(S::kCounts);
+      }
+      if constexpr (s == 1 && m == kWait) wait_for(S::kCounts, arrivals);
+#pragma unroll
+      for (int f = 0; f < J; ++f)
+        if ((kFrom + f < kProducts ? kFrom + f : kProducts - 1) == m) fetch_b(next, 1 - s, f);
+#pragma unroll
+      for (int f = 0; f < I; ++f)
+        if ((f * J + J - 1 > kFrom ? f * J + J - 1 : kFrom) == m) fetch_a(next, 1 - s, f);
+      if constexpr (s == 1)
+        each(std::make_integer_sequence<int, kRequests>(), [&](auto piece) __attribute__((always_inline)) {
+          if constexpr (kFrom + decltype(piece)::value * (kProducts - kFrom) / kRequests == m) request(piece, free);
+        });
+      if constexpr (s == 0 && m == kProducts / 2) go_on(3);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+
+  auto all_requests = [&](uint32_t buffer) __attribute__((always_inline)) {
+    each(std::make_integer_sequence<int, kRequests>(), [&](auto piece) __attribute__((always_inline)) { request(piece, buffer); });
+  };
+  all_requests(0);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) go_on(i);
+  all_requests(S::kBuffer);
+  *reinterpret_cast<uint32_t*>(lds + S::kCounts) = 0;
+  wait_lds();
+  wait_requests<kRequests>();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < I; ++i) fetch_a(0, 0, i);
+#pragma unroll
+  for (int j = 0; j < J; ++j) fetch_b(0, 0, j);
+
+  unsigned char* rows = lds + S::kRows + wave * S::kRowRegion;
+  uint32_t now = 0;   // the buffer of this step
+  Unit u;
+  for (int round = 0; mx8_unit_at<TM, TN>(p, round, u); ++round) {
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+#pragma unroll 1
+    for (int t = 0; t < u.steps; ++t) {
+      const uint32_t then = S::kBuffer - now;
+      arrivals = __builtin_amdgcn_readfirstlane(arrivals + 8);
+      __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+      for (int part = 0; part < 3; ++part) go_on(part);   // (its branch ahead of the products: the compiler would move those before a branch behind it)
+      half_step(std::integral_constant<int, 0>(), now, 0, 0);
+      __builtin_amdgcn_s_setprio(1);
+      half_step(std::integral_constant<int, 1>(), then, now, t == 0 ? round : 0);   // (requests the step after the next into `now`)
+      now = then;
+    }
+    store_tile32<Out, I, J>(static_cast<Out*>(p.c), static_cast<int64_t>(u.part) * p.M, p.M, p.cols, p.streaming, u.m0 + wm, u.n0 + wn, lane, rows, acc);
+  }
+  wait_requests<0>();   // (requests past the work's end still write zeros to LDS)
+}
+
+template <int I, int J, bool kParts>
+int launch_large(const Mx8Params& q, void* c, int parts, hipStream_t s) {
+  using S = Mx8Shape<I, J>;
+  static LdsOnce reserved;
+  if (!reserve_lds_once(reserved, reinterpret_cast<const void*>(&product_mx8_kernel<I, J, kParts>), S::kLds))
+    return fail(PICO_ERR_LAUNCH, "pico_mx8_product: cannot reserve %d bytes of LDS", S::kLds);
+  Mx8Large p;
+  p.a = reinterpret_cast<const __bf16*>(q.a);
+  p.b = reinterpret_cast<const __bf16*>(q.b);
+  p.c = c;
+  p.M = q.M;
+  p.N = q.N;
+  p.K = q.K / 2;
+  p.lda = p.ldb = p.K;
+  p.tiles_m = (q.M + S::TM - 1) / S::TM;
+  p.tiles_n = (q.N + S::TN - 1) / S::TN;
+  p.parts = parts;
+  p.sa = q.sa;
+  p.sb = q.sb;
+  p.cols = (q.N + 7) / 8 * 8;
+  const int64_t units = static_cast<int64_t>(p.tiles_m) * p.tiles_n * parts;
+  p.streaming = !kParts && units > 256;   // (as for the large products in bf16)
+  hipLaunchKernelGGL((product_mx8_kernel<I, J, kParts>), dim3(static_cast<unsigned>(std::min<int64_t>(units, 256))), dim3(S::kThreads), S::kLds, s, p);
+  return check_launch("pico_mx8_product");
+}
+template <bool kParts>
+int launch_shape(const Mx8Params& p, void* c, int tile_m, int tile_n, int parts, hipStream_t s) {
+  if (tile_m == 256 && tile_n == 256) return launch_large<4, 2, kParts>(p, c, parts, s);
+  if (tile_m == 128 && tile_n == 256) return launch_large<2, 2, kParts>(p, c, parts, s);
+  if (tile_m == 256 && tile_n == 128) return launch_large<4, 1, kParts>(p, c, parts, s);
+  if (tile_m == 128 && tile_n == 128) return launch_large<2, 1, kParts>(p, c, parts, s);
+  return fail(PICO_ERR_SHAPE, "pico_mx8_product: tiles of %d x %d (sides of 128 or 256)", tile_m, tile_n);
+}
+
+// Which kernel, tiles and pieces of the contraction a product of these sizes goes to.  tile_m 0: the kernel of few rows.
+struct Route {
+  int tile_m, tile_n, parts;
+};
+bool large_takes(int64_t M, int64_t N, int64_t K, int parts) {
+  return parts >= 1 && parts <= 64 && (K + 127) / 128 >= 2 * parts && K <= (1 << 22) && ((M + 127) / 128) * ((N + 127) / 128) * parts <= 0x7fffffff / 256 && N <= 0x7fffffff / 256 && M <= 0x7fffffff / 2;
+}
+Route route(int64_t M, int64_t N, int64_t K) {
+  if (M <= 64 || !large_takes(M, N, K, 1)) return {0, 0, 1};
+  auto units = [&](int64_t tm, int64_t tn) { return ((M + tm - 1) / tm) * ((N + tn - 1) / tn); };
+  if (units(256, 256) >= 192) return {256, 256, 1};
+  if (units(128, 256) >= 192) return {128, 256, 1};
+  return {128, 128, 1};
+}
+
 }  // namespace
 }  // namespace pico
 
 using namespace pico;
 
-extern "C" int pico_mx8_product(const pico_mx8* a, const pico_mx8* b, void* c, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream) {
-  const char* fn = "pico_mx8_product";
+namespace {
+int check_product(const char* fn, const pico_mx8* a, const pico_mx8* b, const void* c, int64_t M, int64_t N, int64_t K) {
   if (int rc = check_mx8_shape(fn, M, K)) return rc;
   if (int rc = check_mx8_shape(fn, N, K)) return rc;
   if (M == 0 || N == 0) return PICO_OK;
@@ -105,12 +424,42 @@ extern "C" int pico_mx8_product(const pico_mx8* a, const pico_mx8* b, void* c, i
   if (int rc = check_mx8(fn, "b", b)) return rc;
   if (!c) return fail(PICO_ERR_NULL, "%s: c is required", fn);
   if (!aligned16(c)) return fail(PICO_ERR_ALIGN, "%s: c must be 16-byte aligned", fn);
+  return PICO_OK;
+}
+int64_t parts_bytes(int64_t M, int64_t N, int parts) { return parts > 1 ? parts * M * ((N + 7) / 8 * 8) * 4 : 0; }
+}  // namespace
+
+extern "C" int64_t pico_mx8_product_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  if (M < 1 || N < 1 || K < 1) return 0;
+  return parts_bytes(M, N, route(M, N, K).parts);
+}
+
+extern "C" int pico_mx8_product_tiled(const pico_mx8* a, const pico_mx8* b, void* c, int64_t M, int64_t N, int64_t K, int tile_m, int tile_n, int parts, void* workspace,
+                                      int64_t workspace_bytes, void* stream) {
+  const char* fn = "pico_mx8_product";
+  if (int rc = check_product(fn, a, b, c, M, N, K)) return rc;
+  if (M == 0 || N == 0) return PICO_OK;
   const Mx8Params p = {static_cast<const uint8_t*>(a->data), static_cast<const uint8_t*>(b->data), static_cast<const uint8_t*>(a->scales), static_cast<const uint8_t*>(b->scales),
                        static_cast<__bf16*>(c), (int)M, (int)N, (int)K};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (M <= 16) launch_few<1, 1, 4>(p, s);
-  else launch_few<2, 2, 4>(p, s);
-  return check_launch(fn);
+  if (tile_m == 0) {
+    if (M <= 16) launch_few<1, 1, 4>(p, s);
+    else launch_few<2, 2, 4>(p, s);
+    return check_launch(fn);
+  }
+  if (!large_takes(M, N, K, parts))
+    return fail(PICO_ERR_SHAPE, "%s: M=%lld N=%lld K=%lld in %d pieces (two steps of 128 a piece at least)", fn, (long long)M, (long long)N, (long long)K, parts);
+  if (parts == 1) return launch_shape<false>(p, c, tile_m, tile_n, 1, s);
+  if (!workspace || workspace_bytes < parts_bytes(M, N, parts))
+    return fail(PICO_ERR_WORKSPACE, "%s: the workspace has %lld bytes, needs %lld", fn, (long long)workspace_bytes, (long long)parts_bytes(M, N, parts));
+  if (!aligned16(workspace)) return fail(PICO_ERR_ALIGN, "%s: the workspace must be 16-byte aligned", fn);
+  if (int rc = launch_shape<true>(p, workspace, tile_m, tile_n, parts, s)) return rc;
+  return pico_sum_parts(static_cast<const float*>(workspace), c, parts, M * ((N + 7) / 8 * 8), PICO_BF16, stream);
 }
 
-extern "C" int64_t pico_mx8_product_workspace_bytes(int64_t M, int64_t N, int64_t K) { return 0; }
+extern "C" int pico_mx8_product(const pico_mx8* a, const pico_mx8* b, void* c, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (int rc = check_product("pico_mx8_product", a, b, c, M, N, K)) return rc;
+  if (M == 0 || N == 0) return PICO_OK;
+  const Route r = route(M, N, K);
+  return pico_mx8_product_tiled(a, b, c, M, N, K, r.tile_m, r.tile_n, r.parts, workspace, workspace_bytes, stream);
+}

@@ -248,6 +248,34 @@ def test_the_product_writes_its_columns_only(device):
         assert (c[:, N:] == 0).all() and torch.equal(c[:, :N].contiguous(), ops.mx8_product(a, b))
 
 
+def tiled(a, b, tile_m, tile_n, parts):
+    from picotron_amd import _lib
+    (M, K), N = a.shape, b.shape[0]
+    ldc = (N + 7) // 8 * 8
+    c = torch.full((M, ldc), 3.0, dtype=BF16, device="cuda")
+    ws = torch.empty(max(parts * M * ldc, 1) if parts > 1 else 1, device="cuda")
+    ca, cb = (_lib.Mx8(t.data.data_ptr(), t.scales.data_ptr()) for t in (a, b))
+    _lib.check(_lib.lib().pico_mx8_product_tiled(ctypes.byref(ca), ctypes.byref(cb), ctypes.c_void_p(c.data_ptr()), M, N, K, tile_m, tile_n, parts, ctypes.c_void_p(ws.data_ptr()),
+                                                 ws.numel() * 4, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))
+    return c[:, :N]
+
+
+@pytest.mark.parametrize("M,N,K,parts", [(1, 1, 256, 1), (255, 257, 288, 1), (256, 512, 384, 1), (130, 1000, 544, 2), (700, 264, 2080, 3), (1, 8, 4096, 8), (520, 530, 1024, 4), (6000, 5000, 352, 1),
+                                         (3000, 2900, 1056, 4)])
+@pytest.mark.parametrize("tile", [(0, 0), (128, 128), (128, 256), (256, 128), (256, 256)])
+def test_every_tile_of_the_product(device, M, N, K, parts, tile):
+    """Exact sums, as above: more tiles than workgroups, fewer, cut at every side; contractions that end inside a step, in pieces of unequal lengths."""
+    from picotron_amd import ops
+    g = gen(K)
+    def rows(n):
+        v = torch.randint(-3, 4, (n, K), generator=g, device="cuda").float().view(n, -1, 32)
+        v[..., 0] = 3
+        return (v * torch.exp2(torch.randint(-1, 2, (n, K // 32, 1), generator=g, device="cuda").float())).view(n, K)
+    x, w = rows(M), rows(N)
+    got = tiled(ops.mx8_quantize(x), ops.mx8_quantize(w), *tile, 1 if tile[0] == 0 else parts)
+    assert torch.equal(got.float(), (x @ w.t()).to(BF16).float())      # (whole numbers of at most 36 K over 4: exact in fp32)
+
+
 def test_operands_that_do_not_fit(device):
     from picotron_amd import ops
     a, b = ops.mx8_quantize(torch.ones(4, 64, device="cuda")), ops.mx8_quantize(torch.ones(8, 96, device="cuda"))

@@ -73,6 +73,16 @@ def test_products(lib):
     assert product(c=None) == -1 and product(c=ctypes.c_void_p(BUF + 8)) == -4
 
 
+def test_tiles_pieces_and_workspaces(lib):
+    def tiled(tile_m=256, tile_n=256, parts=1, ws=None, bytes_=0, K=1024):
+        return lib.pico_mx8_product_tiled(packed(), packed(), P, 512, 512, K, tile_m, tile_n, parts, ws, bytes_, None)
+    assert tiled(tile_m=64) == -3 and tiled(tile_n=192) == -3 and tiled(parts=0) == -3 and tiled(parts=5) == -3 and tiled(parts=65, K=1 << 20) == -3 and tiled(K=128) == -3
+    assert tiled(parts=2) == -6 and tiled(parts=2, ws=P, bytes_=2 * 512 * 512 * 4 - 1) == -6 and tiled(parts=2, ws=ctypes.c_void_p(BUF + 8), bytes_=1 << 30) == -4
+    bytes_ = lib.pico_mx8_product_workspace_bytes(512, 512, 65536)
+    if bytes_:
+        assert lib.pico_mx8_product(packed(), packed(), P, 512, 512, 65536, P, bytes_ - 1, None) == -6
+
+
 def test_nothing_to_do_is_no_error(lib):
     assert set(calls(lib, x=None, y8=packed(data=None), rows=0).values()) == {0}
     assert lib.pico_mx8_product(packed(data=None), packed(), None, 0, 4, 64, None, 0, None) == 0
