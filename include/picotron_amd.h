@@ -566,9 +566,9 @@ int pico_swiglu_mx8_bwd(const void* dy, const pico_mx8* gate8, const pico_mx8* u
  * [N, K].  workspace: pico_mx8_product_workspace_bytes bytes, 16-byte aligned (NULL where that is 0). */
 int64_t pico_mx8_product_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int pico_mx8_product(const pico_mx8* a, const pico_mx8* b, void* c, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
-/* The same in given tiles, each side 128 or 256, the contraction in `parts` pieces of two steps of 128 at least (parts > 1: workspace of parts * M * (N rounded
- * up) * 4 bytes), or, tile_m = 0, in the kernel of few rows.  What pico_mx8_product goes to by its rules. */
-int pico_mx8_product_tiled(const pico_mx8* a, const pico_mx8* b, void* c, int64_t M, int64_t N, int64_t K, int tile_m, int tile_n, int parts,
+/* The same in given tiles, 64 x 128 or each side 128 or 256, by per_cu workgroups to a CU (1; 2 for 128 x 128), the contraction in `parts` pieces of two steps of 128 at least (parts > 1: workspace of parts * M * (N rounded
+ * up) * 4 bytes), or, tile_m = 0, in form tile_n (0 .. 12) of the kernel of few rows.  What pico_mx8_product goes to by its rules. */
+int pico_mx8_product_tiled(const pico_mx8* a, const pico_mx8* b, void* c, int64_t M, int64_t N, int64_t K, int tile_m, int tile_n, int per_cu, int parts,
                            void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------ optimizer step

@@ -5,6 +5,7 @@
 // (half) of the wave; its scale is that of block h.  The sums are fp32 registers, but within an instruction the products are added with about 17 bits behind the
 // largest: over normal values 1.5e-5 of the result's root mean square (7e-5 with outliers of 20), without a bias and without growth from a contraction
 // of 128 to one of 8192.  The rounding of the result to bf16 is 1.7e-3, so the result is bf16 only.
+#include <iterator>
 #include "mx8.h"
 #include "product_large.h"
 
@@ -24,12 +25,15 @@ __device__ __forceinline__ i32x8 both(u32x4 low, u32x4 high) {
   return __builtin_bit_cast(i32x8, __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-// ---- few rows: MT x NT tiles of 16 x 16 to a workgroup, whose W waves take every W-th 128 of the contraction straight from memory and join their sums in LDS.
-template <int MT, int NT, int W>
+// ---- few rows: MT x NT tiles of 16 x 16 to a workgroup, whose W waves take every W-th 128 of the contraction straight from memory and join their sums in LDS.  Bound by the weight's
+// bytes, so what counts is how much is on its way: a wave requests U steps before it uses the first.
+template <int MT, int NT, int W, int U>
 __global__ __launch_bounds__(W * kWave) void product_mx8_few_kernel(const Mx8Params p) {
+  Arguments<0>().arrive();
   __shared__ f32x4 sums[W][MT * NT][kWave];
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, n = lane % 16, h = lane / 16;
-  const int m0 = blockIdx.y * 16 * MT, n0 = blockIdx.x * 16 * NT, steps = (p.K + kGroup - 1) / kGroup;
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), n = lane % 16, h = lane / 16;
+  const int across = (p.N + 16 * NT - 1) / (16 * NT), m0 = static_cast<int>(blockIdx.x) / across * 16 * MT, n0 = static_cast<int>(blockIdx.x) % across * 16 * NT;
+  const int steps = (p.K + kGroup - 1) / kGroup;
   // rows past the matrix read its last one, and what they give is not written
   int64_t ra[MT], rb[NT];
 #pragma unroll
@@ -41,30 +45,41 @@ __global__ __launch_bounds__(W * kWave) void product_mx8_few_kernel(const Mx8Par
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto fragment = [&](const uint8_t* m, int64_t row, int k) __attribute__((always_inline)) {   // (zeros past the contraction, in pieces of 16)
-    const uint8_t* at = m + row * p.K + k + 16 * h;
-    const u32x4 zero = {0, 0, 0, 0};
-    const u32x4 low = k + 16 * h < p.K ? *reinterpret_cast<const u32x4*>(at) : zero, high = k + 64 + 16 * h < p.K ? *reinterpret_cast<const u32x4*>(at + 64) : zero;
-    return both(low, high);
-  };
-  for (int t = wave; t < steps; t += W) {
-    i32x8 fa[MT], fb[NT];
-    int sa[MT], sb[NT];
+  for (int t0 = wave; t0 < steps; t0 += U * W) {
+    u32x4 a[U][MT][2], b[U][NT][2];
+    int sa[U][MT], sb[U][NT];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      fb[j] = fragment(p.b, rb[j], t * kGroup);
-      sb[j] = p.sb[(static_cast<int64_t>(t) * p.N + rb[j]) * 4 + h];
+    for (int u = 0; u < U; ++u) {
+      // pieces past the contraction read their row's first ones; b's are made 0 below (a's row is NaN as a whole or finite)
+      const int t = min(t0 + u * W, steps - 1), k = (t0 + u * W) * kGroup + 16 * h;
+      const int64_t low = k < p.K ? k : 0, high = k + 64 < p.K ? k + 64 : 0;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        b[u][j][0] = *reinterpret_cast<const u32x4*>(p.b + rb[j] * p.K + low);
+        b[u][j][1] = *reinterpret_cast<const u32x4*>(p.b + rb[j] * p.K + high);
+        sb[u][j] = p.sb[(static_cast<int64_t>(t) * p.N + rb[j]) * 4 + h];
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        a[u][i][0] = *reinterpret_cast<const u32x4*>(p.a + ra[i] * p.K + low);
+        a[u][i][1] = *reinterpret_cast<const u32x4*>(p.a + ra[i] * p.K + high);
+        sa[u][i] = p.sa[(static_cast<int64_t>(t) * p.M + ra[i]) * 4 + h];
+      }
     }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      fa[i] = fragment(p.a, ra[i], t * kGroup);
-      sa[i] = p.sa[(static_cast<int64_t>(t) * p.M + ra[i]) * 4 + h];
+    for (int u = 0; u < U; ++u) {
+      const int k = (t0 + u * W) * kGroup + 16 * h;
+      const u32x4 zero = {0, 0, 0, 0};
+      i32x8 fb[NT];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) fb[j] = both(k < p.K ? b[u][j][0] : zero, k + 64 < p.K ? b[u][j][1] : zero);
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)   // C^T: a lane holds four columns of a row of C
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], both(a[u][i][0], a[u][i][1]), acc[i][j], 0, 0, 0, sb[u][j], 0, sa[u][i]);
     }
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int j = 0; j < NT; ++j)   // C^T: a lane holds four columns of a row of C
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], fa[i], acc[i][j], 0, 0, 0, sb[j], 0, sa[i]);
   }
 #pragma unroll
   for (int i = 0; i < MT; ++i)
@@ -85,9 +100,23 @@ __global__ __launch_bounds__(W * kWave) void product_mx8_few_kernel(const Mx8Par
   }
 }
 
-template <int MT, int NT, int W>
-void launch_few(const Mx8Params& p, hipStream_t s) {
-  hipLaunchKernelGGL((product_mx8_few_kernel<MT, NT, W>), dim3((p.N + 16 * NT - 1) / (16 * NT), (p.M + 16 * MT - 1) / (16 * MT)), dim3(W * kWave), 0, s, p);
+template <int MT, int NT, int W, int U>
+int launch_few(const Mx8Params& p, hipStream_t s) {
+  const int64_t tiles = ((p.N + INT64_C(16) * NT - 1) / (16 * NT)) * ((p.M + INT64_C(16) * MT - 1) / (16 * MT));
+  if (tiles > 0x7fffffff) return fail(PICO_ERR_SHAPE, "pico_mx8_product: M=%d N=%d with K=%d has too many tiles", p.M, p.N, p.K);
+  hipLaunchKernelGGL((product_mx8_few_kernel<MT, NT, W, U>), dim3(static_cast<unsigned>(tiles)), dim3(W * kWave), 0, s, p);
+  return check_launch("pico_mx8_product");
+}
+// What can be asked for: tiles of 16 x 16 to a workgroup, its waves, steps that a wave requests at once.
+struct Few {
+  int mt, nt, waves, ahead;
+};
+constexpr Few kFew[] = {{1, 1, 4, 2}, {1, 1, 8, 2}, {1, 1, 16, 2}, {1, 2, 4, 2}, {1, 2, 8, 2}, {1, 2, 16, 2}, {2, 1, 4, 2}, {2, 1, 8, 2}, {2, 1, 16, 2}, {2, 2, 4, 2}, {2, 2, 8, 2}, {2, 4, 4, 1}, {4, 2, 8, 1}};
+template <int... v>
+int dispatch_few(const Mx8Params& p, int form, hipStream_t s, std::integer_sequence<int, v...>) {
+  int rc = PICO_ERR_SHAPE;
+  ((form == v ? static_cast<void>(rc = launch_few<kFew[v].mt, kFew[v].nt, kFew[v].waves, kFew[v].ahead>(p, s)) : void()), ...);
+  return rc;
 }
 
 // ---- many rows: the large products' workgroups (product_large.h) with 128 of contraction a step
@@ -98,10 +127,11 @@ struct Mx8Large : LargeParams {   // (a, b, K and the pitches in pairs of values
   const uint8_t *sa, *sb;
   int cols;                       // of c
 };
-// wait_requests<N> where `but` is not 0, wait_requests<0> where it is.  The branch is inside: products ahead of one that the compiler sees would be moved behind it.
-template <int N>
+// wait_requests<kMore> where `but` is not 0, wait_requests<kLess> where it is.  The branch is inside: products ahead of one that the compiler sees would be moved behind it.
+template <int kLess, int kMore>
 __device__ __forceinline__ void wait_requests_but(int but) {
-  asm volatile("s_cmp_lg_u32 %0, 0\n\ts_cbranch_scc1 pico_but_%=\n\ts_waitcnt vmcnt(0)\npico_but_%=:\n\ts_waitcnt vmcnt(%1)" ::"s"(but), "n"(N) : "scc", "memory");
+  static_assert(kLess <= kMore && kMore < 64);
+  asm volatile("s_cmp_lg_u32 %0, 0\n\ts_cbranch_scc1 pico_but_%=\n\ts_waitcnt vmcnt(%1)\npico_but_%=:\n\ts_waitcnt vmcnt(%2)" ::"s"(but), "n"(kLess), "n"(kMore) : "scc", "memory");
 }
 // unit_at of product_large.h in 32 bits and scalar registers: pieces times steps stay under 2^21 here, and a division of 64 bits takes the sizes, and with them the loops' counts and the
 // windows, through vector registers.
@@ -121,16 +151,26 @@ __device__ __forceinline__ bool mx8_unit_at(const Mx8Large& p, int round, Unit& 
   u.steps = __builtin_amdgcn_readfirstlane((u.part + 1) * steps / p.parts) - u.first;
   return true;
 }
-template <int I, int J>
+// kWavesM x kWavesN waves of 32 I x 32 J, and as many buffers as kPerCu workgroups find place for in a CU's LDS (two of tiles of 256 x 256; four of 128 x 128, or two where two
+// workgroups share a CU; six of 64 x 128).  Where there are fewer tiles than CUs nothing else hides what a request takes, about 0.5 us: us with two buffers and with four or six,
+// [1003 x 11008] @ [4096 x 11008]^T in tiles of 128 x 128 70.3, 52.2; [512 x 2048] @ [2048 x 2048]^T in 64 x 128 11.6, 10.2.  Where there are more, a second workgroup does
+// better: [4096 x 2048] @ [2048 x 2048]^T 19.3, and 23.5 with four buffers and one workgroup.
+template <int kWavesM, int kWavesN, int I, int J, int kPerCu>
 struct Mx8Shape {
-  static constexpr int kThreads = 512, TM = 64 * I, TN = 128 * J;
+  static constexpr int kWaves = kWavesM * kWavesN, kThreads = kWaves * kWave, TM = 32 * I * kWavesM, TN = 32 * J * kWavesN;
   using A = Tile<false, TM, kThreads>;
   using B = Tile<false, TN, kThreads>;
-  static constexpr int kBuffer = A::kBytes + B::kBytes, kScaleBytes = 2 * 256 * 4;   // (of up to 256 rows of a, and of b)
-  static constexpr int kScales = 2 * kBuffer, kRows = kScales + 2 * kScaleBytes, kRowRegion = 16 * 128;
-  static constexpr int kCounts = kRows + 8 * kRowRegion, kLds = kCounts + 16;
-  static_assert(kLds <= 160 * 1024);
+  static constexpr int kScales = A::kBytes + B::kBytes, kBuffer = kScales + kWaves * 256;   // (the scales of 64 rows by each wave)
+  static constexpr int kRowRegion = 16 * 128, kMost = 160 * 1024 / kPerCu, kBuffers = (kMost - kWaves * kRowRegion) / kBuffer;   // (rows: per wave, where a tile's rows are put together)
+  static constexpr int kRows = kBuffers * kBuffer, kLds = kRows + kWaves * kRowRegion;
+  static_assert(kBuffers >= 2 && kLds <= kMost && (TM + TN) / 64 <= kWaves && TM % 64 == 0);
 };
+template <int kPlus>
+__device__ __forceinline__ void request16_along(uint32_t lds_off, u32x4 window, uint32_t off, uint32_t along) {   // request16_to with a scalar offset
+  uint32_t aim;
+  asm volatile("s_add_u32 %0, %1, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %4, %5 offen lds"
+               : "=&{m0}"(aim) : "s"(lds_off), "n"(kPlus), "v"(off), "s"(window), "s"(along) : "scc", "memory");
+}
 template <int kPlus>
 __device__ __forceinline__ void request4_to(uint32_t lds_off, u32x4 window, uint32_t off) {   // request16_to of 4 bytes per lane
   uint32_t aim;
@@ -197,78 +237,81 @@ __device__ __forceinline__ void store_tile32(Out* c, int64_t first_row, int M, i
   }
 }
 
-template <int I, int J, bool kParts>
-__global__ __launch_bounds__(512, 2) void product_mx8_kernel(const Mx8Large p) {
-  using S = Mx8Shape<I, J>;
+template <int kWavesM, int kWavesN, int I, int J, int kPerCu, bool kParts>
+__global__ __launch_bounds__(kWavesM * kWavesN * kWave, 2) void product_mx8_kernel(const Mx8Large p) {
+  using S = Mx8Shape<kWavesM, kWavesN, I, J, kPerCu>;
   using A = typename S::A;
   using B = typename S::B;
   constexpr int TM = S::TM, TN = S::TN, kPA = A::kPieces, kPB = B::kPieces, kPieces = kPA + kPB;
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const int wm = wave / 4 * 32 * I, wn = wave % 4 * 32 * J, n = lane % 32, h = lane / 32;
+  const int wm = wave / kWavesN * 32 * I, wn = wave % kWavesN * 32 * J, n = lane % 32, h = lane / 32;
 
-  // ---- requests (as in product_large_kernel; both operands have one pitch, and a thread's pieces lie 64 rows apart)
-  const uint32_t piece_bytes = static_cast<uint32_t>(p.lda) * (64 * 2);
+  // ---- requests (as in product_large_kernel; both operands have one pitch, and a thread's pieces lie kThreads / 8 rows apart)
+  const uint32_t piece_bytes = static_cast<uint32_t>(p.lda) * (S::kThreads / 8 * 2);
   uint32_t first_piece = A::offset(p.lda, tid, 0);
   const int k_piece = (tid % 8 ^ (tid / 16 & 7)) * 8;
   const bool ragged = p.K % kStep != 0;
   Unit load;   // where the requests stand
   int load_round = 0, load_step = 0;
   mx8_unit_at<TM, TN>(p, 0, load);
-  Window wa, wb, ws;
-  // the scales of this wave's 64 rows: of a for the first four waves, of b for the others
-  const int s_rows = wave < 4 ? p.M : p.N, s_first = wave % 4 * 64;
-  const uint8_t* s_base = wave < 4 ? p.sa : p.sb;
-  auto open = [&]() __attribute__((always_inline)) {
-    wa = open_window<false>(p.a, p.lda, load.m0, TM, p.M, load.first * kStep, p.K);
-    wb = open_window<false>(p.b, p.ldb, load.n0, TN, p.N, load.first * kStep, p.K);
-    const int first = (wave < 4 ? load.m0 : load.n0) + s_first;
-    ws = {reinterpret_cast<uint64_t>(s_base) + (static_cast<int64_t>(load.first) * s_rows + first) * 4, first < s_rows ? static_cast<uint32_t>(min(s_rows - first, 64)) * 4 : 0u};
+  // A tile's windows stay where they are and the contraction goes on in the requests' scalar offset, with which a piece in the window stays in its row (a piece of a row past the
+  // matrix lies past the window without it).  The scales of the steps lie as far apart as the matrix has rows: their window moves.
+  u32x4 ra, rb, rs;
+  uint32_t along = 0;
+  uint64_t s_base;
+  // the scales of this wave's 64 rows: of a for the first TM / 64 waves, of b for the others
+  constexpr int kOfA = TM / 64;
+  const bool of_a = wave < kOfA;
+  const int s_rows = of_a ? p.M : p.N, s_first = (of_a ? wave : wave - kOfA) * 64;
+  auto open = [&](uint32_t whole) __attribute__((always_inline)) {   // (whole 0: requests past the work's end read no memory)
+    const Window wa = open_window<false>(p.a, p.lda, load.m0, TM, p.M, load.first * kStep, p.K), wb = open_window<false>(p.b, p.ldb, load.n0, TN, p.N, load.first * kStep, p.K);
+    const int first = (of_a ? load.m0 : load.n0) + s_first;
+    s_base = reinterpret_cast<uint64_t>(of_a ? p.sa : p.sb) + (static_cast<int64_t>(load.first) * s_rows + first) * 4;
+    ra = request_window(wa.base, wa.bytes * whole);
+    rb = request_window(wb.base, wb.bytes * whole);
+    rs = request_window(s_base, first < s_rows ? static_cast<uint32_t>(min(s_rows - first, 64)) * 4 * whole : 0u);
+    along = 0;
   };
-  open();
-  u32x4 ra = resource(wa), rb = resource(wb), rs = resource(ws);
-  auto go_on = [&](int part) __attribute__((always_inline)) {
-    if (part == 0) {
-      ++load_step;
-      advance(wa, kStep * 2);
-    }
-    if (part == 1) {
-      advance(wb, kStep * 2);
-      ws.base += static_cast<uint32_t>(s_rows) * 4u;
-    }
-    if (part == 2 && load_step >= load.steps - 1) {
+  open(1);
+  auto go_on = [&]() __attribute__((always_inline)) {
+    ++load_step;
+    along += kStep * 2;
+    s_base += static_cast<uint32_t>(s_rows) * 4u;
+    rs[0] = static_cast<uint32_t>(s_base);
+    rs[1] = static_cast<uint32_t>(s_base >> 32);
+    if (load_step >= load.steps - 1) {
       if (load_step == load.steps) {
         load_step = 0;
-        const bool more = mx8_unit_at<TM, TN>(p, ++load_round, load);
-        open();
-        if (!more) wa.bytes = wb.bytes = ws.bytes = 0;   // requests past the work's end read no memory
+        open(mx8_unit_at<TM, TN>(p, ++load_round, load) ? 1 : 0);
       }
-      if (ragged) {   // pieces past the contraction's end read as zeros (their scales are bytes of 0, no NaN)
-        // (a window is under 2^31 bytes, and so are three times piece_bytes)
+      if (ragged)   // pieces past the contraction's end read as zeros (their scales are bytes of 0, no NaN); a window is under 2^31 bytes, and so is a row's end past this
         first_piece = k_piece < p.K - (load.first + load_step) * kStep ? A::offset(p.lda, tid, 0) : 0x80000000u;
-      }
     }
-    if (part == 3) {
-      ra = resource(wa);
-      rb = resource(wb);
-      rs = resource(ws);
+    along = __builtin_amdgcn_readfirstlane(along);   // (they are scalars; the compiler does not see it behind the branch)
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      ra[i] = __builtin_amdgcn_readfirstlane(ra[i]);
+      rb[i] = __builtin_amdgcn_readfirstlane(rb[i]);
+      rs[i] = __builtin_amdgcn_readfirstlane(rs[i]);
     }
   };
   const uint32_t lds_wave = wave * 1024, lds_scales = S::kScales + wave * 256;   // (dynamic LDS starts at 0: the build looks)
   auto request = [&](auto piece, uint32_t buffer) __attribute__((always_inline)) {
     constexpr int i = decltype(piece)::value;
-    if constexpr (i < kPA) request16_to<i * S::kThreads * 16>(lds_wave + buffer, ra, first_piece + i * piece_bytes);
-    else if constexpr (i < kPieces) request16_to<A::kBytes + (i - kPA) * S::kThreads * 16>(lds_wave + buffer, rb, first_piece + (i - kPA) * piece_bytes);
-    else request4_to<0>(lds_scales + (buffer != 0 ? S::kScaleBytes : 0), rs, static_cast<uint32_t>(lane) * 4);
+    if constexpr (i < kPA) request16_along<i * S::kThreads * 16>(lds_wave + buffer, ra, first_piece + i * piece_bytes, along);
+    else if constexpr (i < kPieces) request16_along<A::kBytes + (i - kPA) * S::kThreads * 16>(lds_wave + buffer, rb, first_piece + (i - kPA) * piece_bytes, along);
+    else request4_to<0>(lds_scales + buffer, rs, static_cast<uint32_t>(lane) * 4);
   };
-  constexpr int kRequests = kPieces + 1;
+  constexpr int kRequests = kPieces + 1, kAhead = (S::kBuffers - 2) * kRequests;   // of a step; of the steps behind the one that is waited for
   using Out = std::conditional_t<kParts, float, __bf16>;
   constexpr int kAtOnce = 128 / 32 / static_cast<int>(sizeof(Out)), kStores = 2 * I * ((J + kAtOnce - 1) / kAtOnce) * 2;   // of a wave, at a tile's end
 
   // ---- half a step: its products, row by row of the wave's tile.  A fragment of a is read anew, for the half step that follows, as soon as its row is done, those of b are
-  // held twice.  The workgroup meets once a step: a wave arrives behind the first product of the second half, when its reads of the buffer in use and its requests for the other
-  // one are complete, and waits a quarter of the half later; from there on it reads the other buffer and requests into the one in use.
-  constexpr int kProducts = I * J, kWait = kProducts / 4 > 1 ? kProducts / 4 : 1;
+  // held twice.  The workgroup meets once a step, behind the first product of the second half: a wave's reads of the buffer in use are complete there, and so are its
+  // requests for the next; from there on it reads the next buffer and requests into the one that was in use.  (A barrier in two halves over a count in LDS, as product_large.h
+  // has it, is slower here: [4096 x 2048] @ [16384 x 2048]^T 119.7 us against 116.4, tiles of 128 x 128 27.4 against 23.8 at [1024 x 4096] @ [4096 x 4096]^T.)
+  constexpr int kProducts = I * J;
   i32x8 fa[I], fb[2][J];
   int sca[I], scb[2][J];
   f32x16 acc[I][J];
@@ -277,18 +320,17 @@ __global__ __launch_bounds__(512, 2) void product_mx8_kernel(const Mx8Large p) {
     const unsigned char* row = tile + first * 128 + n * 128;
     return both(*reinterpret_cast<const u32x4*>(row + ((4 * s + h) ^ (n / 2 & 7)) * 16), *reinterpret_cast<const u32x4*>(row + ((4 * s + 2 + h) ^ (n / 2 & 7)) * 16));
   };
-  auto scale = [&](uint32_t buffer, int first, int s) __attribute__((always_inline)) { return lds[S::kScales + (buffer != 0 ? S::kScaleBytes : 0) + (first + n) * 4 + 2 * s + h]; };
+  auto scale = [&](uint32_t buffer, int first, int s) __attribute__((always_inline)) { return lds[S::kScales + buffer + (first + n) * 4 + 2 * s + h]; };
   auto fetch_a = [&](uint32_t buffer, int s, int i) __attribute__((always_inline)) {
     fa[i] = fragment(lds + buffer, wm + 32 * i, s);
     sca[i] = scale(buffer, wm + 32 * i, s);
   };
   auto fetch_b = [&](uint32_t buffer, int s, int j) __attribute__((always_inline)) {
     fb[s][j] = fragment(lds + buffer + A::kBytes, wn + 32 * j, s);
-    scb[s][j] = scale(buffer, 256 + wn + 32 * j, s);
+    scb[s][j] = scale(buffer, TM + wn + 32 * j, s);
   };
-  int arrivals = 0;
   auto half_step = [&](auto half, uint32_t next, uint32_t free, int stores) __attribute__((always_inline)) {
-    constexpr int s = decltype(half)::value, kFrom = s == 0 ? 0 : kWait;
+    constexpr int s = decltype(half)::value;
     each(std::make_integer_sequence<int, kProducts>(), [&](auto product) __attribute__((always_inline)) {
       constexpr int m = decltype(product)::value, i = m / J, j = i % 2 ? J - 1 - m % J : m % J;
       __builtin_amdgcn_sched_barrier(0);
@@ -296,23 +338,21 @@ __global__ __launch_bounds__(512, 2) void product_mx8_kernel(const Mx8Large p) {
       acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[s][j], fa[i], acc[i][j], 0, 0, 0, scb[s][j], 0, sca[i]);
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (s == 1 && m == 0) {
-        // everything requested but the stores of the tile before, which were issued behind its requests
-        wait_requests_but<kStores>(stores);
+        // the next step's requests, behind which lie those of kBuffers - 2 steps more and, in a tile's first steps, the stores of the tile before
+        wait_requests_but<kAhead, kAhead + kStores>(stores);
         wait_lds();
-        arrive(S::kCounts);
+        __builtin_amdgcn_s_barrier();
       }
-      if constexpr (s == 1 && m == kWait) wait_for(S::kCounts, arrivals);
 #pragma unroll
       for (int f = 0; f < J; ++f)
-        if ((kFrom + f < kProducts ? kFrom + f : kProducts - 1) == m) fetch_b(next, 1 - s, f);
+        if ((f < kProducts ? f : kProducts - 1) == m) fetch_b(next, 1 - s, f);
 #pragma unroll
       for (int f = 0; f < I; ++f)
-        if ((f * J + J - 1 > kFrom ? f * J + J - 1 : kFrom) == m) fetch_a(next, 1 - s, f);
+        if (f * J + J - 1 == m) fetch_a(next, 1 - s, f);
       if constexpr (s == 1)
         each(std::make_integer_sequence<int, kRequests>(), [&](auto piece) __attribute__((always_inline)) {
-          if constexpr (kFrom + decltype(piece)::value * (kProducts - kFrom) / kRequests == m) request(piece, free);
+          if constexpr (decltype(piece)::value * kProducts / kRequests == m) request(piece, free);
         });
-      if constexpr (s == 0 && m == kProducts / 2) go_on(3);
       __builtin_amdgcn_sched_barrier(0);
     });
   };
@@ -320,13 +360,12 @@ __global__ __launch_bounds__(512, 2) void product_mx8_kernel(const Mx8Large p) {
   auto all_requests = [&](uint32_t buffer) __attribute__((always_inline)) {
     each(std::make_integer_sequence<int, kRequests>(), [&](auto piece) __attribute__((always_inline)) { request(piece, buffer); });
   };
-  all_requests(0);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) go_on(i);
-  all_requests(S::kBuffer);
-  *reinterpret_cast<uint32_t*>(lds + S::kCounts) = 0;
-  wait_lds();
-  wait_requests<kRequests>();
+  for (int b = 0; b < S::kBuffers; ++b) {
+    if (b > 0) go_on();
+    all_requests(b * S::kBuffer);
+  }
+  wait_requests<kAhead + kRequests>();
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 #pragma unroll
@@ -346,14 +385,12 @@ __global__ __launch_bounds__(512, 2) void product_mx8_kernel(const Mx8Large p) {
         for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 #pragma unroll 1
     for (int t = 0; t < u.steps; ++t) {
-      const uint32_t then = S::kBuffer - now;
-      arrivals = __builtin_amdgcn_readfirstlane(arrivals + 8);
+      const uint32_t then = now == (S::kBuffers - 1) * S::kBuffer ? 0 : now + S::kBuffer;
       __builtin_amdgcn_s_setprio(0);
-#pragma unroll
-      for (int part = 0; part < 3; ++part) go_on(part);   // (its branch ahead of the products: the compiler would move those before a branch behind it)
+      go_on();   // (its branch ahead of the products: the compiler would move those before a branch behind it)
       half_step(std::integral_constant<int, 0>(), now, 0, 0);
       __builtin_amdgcn_s_setprio(1);
-      half_step(std::integral_constant<int, 1>(), then, now, t == 0 ? round : 0);   // (requests the step after the next into `now`)
+      half_step(std::integral_constant<int, 1>(), then, now, t < S::kBuffers - 1 ? round : 0);   // (requests a step that comes kBuffers later into `now`)
       now = then;
     }
     store_tile32<Out, I, J>(static_cast<Out*>(p.c), static_cast<int64_t>(u.part) * p.M, p.M, p.cols, p.streaming, u.m0 + wm, u.n0 + wn, lane, rows, acc);
@@ -361,11 +398,11 @@ __global__ __launch_bounds__(512, 2) void product_mx8_kernel(const Mx8Large p) {
   wait_requests<0>();   // (requests past the work's end still write zeros to LDS)
 }
 
-template <int I, int J, bool kParts>
+template <int kWavesM, int kWavesN, int I, int J, int kPerCu, bool kParts>
 int launch_large(const Mx8Params& q, void* c, int parts, hipStream_t s) {
-  using S = Mx8Shape<I, J>;
+  using S = Mx8Shape<kWavesM, kWavesN, I, J, kPerCu>;
   static LdsOnce reserved;
-  if (!reserve_lds_once(reserved, reinterpret_cast<const void*>(&product_mx8_kernel<I, J, kParts>), S::kLds))
+  if (!reserve_lds_once(reserved, reinterpret_cast<const void*>(&product_mx8_kernel<kWavesM, kWavesN, I, J, kPerCu, kParts>), S::kLds))
     return fail(PICO_ERR_LAUNCH, "pico_mx8_product: cannot reserve %d bytes of LDS", S::kLds);
   Mx8Large p;
   p.a = reinterpret_cast<const __bf16*>(q.a);
@@ -382,32 +419,63 @@ int launch_large(const Mx8Params& q, void* c, int parts, hipStream_t s) {
   p.sb = q.sb;
   p.cols = (q.N + 7) / 8 * 8;
   const int64_t units = static_cast<int64_t>(p.tiles_m) * p.tiles_n * parts;
-  p.streaming = !kParts && units > 256;   // (as for the large products in bf16)
-  hipLaunchKernelGGL((product_mx8_kernel<I, J, kParts>), dim3(static_cast<unsigned>(std::min<int64_t>(units, 256))), dim3(S::kThreads), S::kLds, s, p);
+  constexpr int kGrid = 256 * kPerCu;
+  p.streaming = !kParts && units > kGrid;   // (as for the large products in bf16)
+  hipLaunchKernelGGL((product_mx8_kernel<kWavesM, kWavesN, I, J, kPerCu, kParts>), dim3(static_cast<unsigned>(std::min<int64_t>(units, kGrid))), dim3(S::kThreads), S::kLds, s, p);
   return check_launch("pico_mx8_product");
 }
+// What can be asked for: the sides of a tile, workgroups to a CU.
+struct Tiling {
+  int tile_m, tile_n, per_cu;
+  float step, step_full, end;   // us a step with few tiles and with every CU taken, us a tile beside them (for route)
+};
+constexpr Tiling kTilings[] = {{256, 256, 1, 1.03f, 1.60f, 2.0f}, {128, 256, 1, 0.72f, 0.93f, 1.5f}, {256, 128, 1, 0.72f, 0.93f, 1.5f}, {128, 128, 2, 0.55f, 0.93f, 1.5f}, {128, 128, 1, 0.44f, 0.53f, 1.2f},
+                               {64, 128, 1, 0.35f, 0.38f, 1.0f}};
 template <bool kParts>
-int launch_shape(const Mx8Params& p, void* c, int tile_m, int tile_n, int parts, hipStream_t s) {
-  if (tile_m == 256 && tile_n == 256) return launch_large<4, 2, kParts>(p, c, parts, s);
-  if (tile_m == 128 && tile_n == 256) return launch_large<2, 2, kParts>(p, c, parts, s);
-  if (tile_m == 256 && tile_n == 128) return launch_large<4, 1, kParts>(p, c, parts, s);
-  if (tile_m == 128 && tile_n == 128) return launch_large<2, 1, kParts>(p, c, parts, s);
-  return fail(PICO_ERR_SHAPE, "pico_mx8_product: tiles of %d x %d (sides of 128 or 256)", tile_m, tile_n);
+int launch_shape(const Mx8Params& p, void* c, int tile_m, int tile_n, int per_cu, int parts, hipStream_t s) {
+  if (tile_m == 256 && tile_n == 256 && per_cu == 1) return launch_large<2, 4, 4, 2, 1, kParts>(p, c, parts, s);
+  if (tile_m == 128 && tile_n == 256 && per_cu == 1) return launch_large<2, 4, 2, 2, 1, kParts>(p, c, parts, s);
+  if (tile_m == 256 && tile_n == 128 && per_cu == 1) return launch_large<4, 2, 2, 2, 1, kParts>(p, c, parts, s);
+  if (tile_m == 128 && tile_n == 128 && per_cu == 2) return launch_large<2, 2, 2, 2, 2, kParts>(p, c, parts, s);
+  if (tile_m == 128 && tile_n == 128 && per_cu == 1) return launch_large<2, 2, 2, 2, 1, kParts>(p, c, parts, s);
+  if (tile_m == 64 && tile_n == 128 && per_cu == 1) return launch_large<2, 2, 1, 2, 1, kParts>(p, c, parts, s);
+  return fail(PICO_ERR_SHAPE, "pico_mx8_product: tiles of %d x %d, %d workgroups to a CU (64 x 128, or sides of 128 or 256; 2 for 128 x 128)", tile_m, tile_n, per_cu);
 }
 
-// Which kernel, tiles and pieces of the contraction a product of these sizes goes to.  tile_m 0: the kernel of few rows.
+// Which kernel, tiles and pieces of the contraction a product of these sizes goes to.  tile_m 0: the kernel of few rows, in form tile_n.
 struct Route {
-  int tile_m, tile_n, parts;
+  int tile_m, tile_n, per_cu, parts;
 };
 bool large_takes(int64_t M, int64_t N, int64_t K, int parts) {
-  return parts >= 1 && parts <= 64 && (K + 127) / 128 >= 2 * parts && K <= (1 << 22) && ((M + 127) / 128) * ((N + 127) / 128) * parts <= 0x7fffffff / 256 && N <= 0x7fffffff / 256 && M <= 0x7fffffff / 2;
+  return parts >= 1 && parts <= 64 && (K + 127) / 128 >= 2 * parts && K <= (1 << 22) && ((M + 63) / 64) * ((N + 127) / 128) * parts <= 0x7fffffff / 256 && N <= 0x7fffffff / 256 && M <= 0x7fffffff / 2;
 }
 Route route(int64_t M, int64_t N, int64_t K) {
-  if (M <= 64 || !large_takes(M, N, K, 1)) return {0, 0, 1};
-  auto units = [&](int64_t tm, int64_t tn) { return ((M + tm - 1) / tm) * ((N + tn - 1) / tn); };
-  if (units(256, 256) >= 192) return {256, 256, 1};
-  if (units(128, 256) >= 192) return {128, 256, 1};
-  return {128, 128, 1};
+  const int64_t steps = (K + 127) / 128, cols = (N + 7) / 8 * 8;
+  Route best = {0, 0, 1, 1};
+  float least = 1e30f;
+  for (int v = 0; v < static_cast<int>(std::size(kFew)); ++v) {
+    const Few& f = kFew[v];
+    const int64_t blocks = (M + 16 * f.mt - 1) / (16 * f.mt), tiles = blocks * ((N + 16 * f.nt - 1) / (16 * f.nt)), per_cu = (tiles + 255) / 256, turns = (steps + f.waves * f.ahead - 1) / (f.waves * f.ahead);
+    const float rows = static_cast<float>(M) / (16 * blocks);   // (rows past the matrix cost no memory)
+    const float us = 2.f + std::max(0.066f * per_cu * steps * (f.nt + rows), 1.55e-7f * N * K) + 0.9f * (turns - 1) / per_cu;
+    if (us < least) {
+      least = us;
+      best = {0, v, 1, 1};
+    }
+  }
+  if (!large_takes(M, N, K, 1)) return best;
+  for (const Tiling& t : kTilings)
+    for (int parts = 1; parts <= 16 && large_takes(M, N, K, parts); parts *= 2) {
+      const int64_t units = ((M + t.tile_m - 1) / t.tile_m) * ((N + t.tile_n - 1) / t.tile_n) * parts, slots = 256 * t.per_cu, rounds = (units + slots - 1) / slots;
+      const float taken = static_cast<float>(units < slots ? units : slots) / slots, step = std::max(t.step, t.step_full * taken);
+      float us = 3.5f + rounds * ((steps + parts - 1) / parts * step + t.end);
+      if (parts > 1) us += 2.f + (4.f * parts + 2.f) * M * cols * 2.5e-7f;   // (the sums again, at 4 TB/s)
+      if (us < least) {
+        least = us;
+        best = {t.tile_m, t.tile_n, t.per_cu, parts};
+      }
+    }
+  return best;
 }
 
 }  // namespace
@@ -434,7 +502,7 @@ extern "C" int64_t pico_mx8_product_workspace_bytes(int64_t M, int64_t N, int64_
   return parts_bytes(M, N, route(M, N, K).parts);
 }
 
-extern "C" int pico_mx8_product_tiled(const pico_mx8* a, const pico_mx8* b, void* c, int64_t M, int64_t N, int64_t K, int tile_m, int tile_n, int parts, void* workspace,
+extern "C" int pico_mx8_product_tiled(const pico_mx8* a, const pico_mx8* b, void* c, int64_t M, int64_t N, int64_t K, int tile_m, int tile_n, int per_cu, int parts, void* workspace,
                                       int64_t workspace_bytes, void* stream) {
   const char* fn = "pico_mx8_product";
   if (int rc = check_product(fn, a, b, c, M, N, K)) return rc;
@@ -443,17 +511,17 @@ extern "C" int pico_mx8_product_tiled(const pico_mx8* a, const pico_mx8* b, void
                        static_cast<__bf16*>(c), (int)M, (int)N, (int)K};
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (tile_m == 0) {
-    if (M <= 16) launch_few<1, 1, 4>(p, s);
-    else launch_few<2, 2, 4>(p, s);
-    return check_launch(fn);
+    constexpr int kForms = static_cast<int>(std::size(kFew));
+    if (tile_n < 0 || tile_n >= kForms) return fail(PICO_ERR_SHAPE, "%s: no form %d of the kernel of few rows", fn, tile_n);
+    return dispatch_few(p, tile_n, s, std::make_integer_sequence<int, kForms>());
   }
   if (!large_takes(M, N, K, parts))
     return fail(PICO_ERR_SHAPE, "%s: M=%lld N=%lld K=%lld in %d pieces (two steps of 128 a piece at least)", fn, (long long)M, (long long)N, (long long)K, parts);
-  if (parts == 1) return launch_shape<false>(p, c, tile_m, tile_n, 1, s);
+  if (parts == 1) return launch_shape<false>(p, c, tile_m, tile_n, per_cu, 1, s);
   if (!workspace || workspace_bytes < parts_bytes(M, N, parts))
     return fail(PICO_ERR_WORKSPACE, "%s: the workspace has %lld bytes, needs %lld", fn, (long long)workspace_bytes, (long long)parts_bytes(M, N, parts));
   if (!aligned16(workspace)) return fail(PICO_ERR_ALIGN, "%s: the workspace must be 16-byte aligned", fn);
-  if (int rc = launch_shape<true>(p, workspace, tile_m, tile_n, parts, s)) return rc;
+  if (int rc = launch_shape<true>(p, workspace, tile_m, tile_n, per_cu, parts, s)) return rc;
   return pico_sum_parts(static_cast<const float*>(workspace), c, parts, M * ((N + 7) / 8 * 8), PICO_BF16, stream);
 }
 
@@ -461,5 +529,5 @@ extern "C" int pico_mx8_product(const pico_mx8* a, const pico_mx8* b, void* c, i
   if (int rc = check_product("pico_mx8_product", a, b, c, M, N, K)) return rc;
   if (M == 0 || N == 0) return PICO_OK;
   const Route r = route(M, N, K);
-  return pico_mx8_product_tiled(a, b, c, M, N, K, r.tile_m, r.tile_n, r.parts, workspace, workspace_bytes, stream);
+  return pico_mx8_product_tiled(a, b, c, M, N, K, r.tile_m, r.tile_n, r.per_cu, r.parts, workspace, workspace_bytes, stream);
 }

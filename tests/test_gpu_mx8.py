@@ -248,21 +248,21 @@ def test_the_product_writes_its_columns_only(device):
         assert (c[:, N:] == 0).all() and torch.equal(c[:, :N].contiguous(), ops.mx8_product(a, b))
 
 
-def tiled(a, b, tile_m, tile_n, parts):
+def tiled(a, b, tile_m, tile_n, per_cu, parts):
     from picotron_amd import _lib
     (M, K), N = a.shape, b.shape[0]
     ldc = (N + 7) // 8 * 8
     c = torch.full((M, ldc), 3.0, dtype=BF16, device="cuda")
     ws = torch.empty(max(parts * M * ldc, 1) if parts > 1 else 1, device="cuda")
     ca, cb = (_lib.Mx8(t.data.data_ptr(), t.scales.data_ptr()) for t in (a, b))
-    _lib.check(_lib.lib().pico_mx8_product_tiled(ctypes.byref(ca), ctypes.byref(cb), ctypes.c_void_p(c.data_ptr()), M, N, K, tile_m, tile_n, parts, ctypes.c_void_p(ws.data_ptr()),
+    _lib.check(_lib.lib().pico_mx8_product_tiled(ctypes.byref(ca), ctypes.byref(cb), ctypes.c_void_p(c.data_ptr()), M, N, K, tile_m, tile_n, per_cu, parts, ctypes.c_void_p(ws.data_ptr()),
                                                  ws.numel() * 4, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))
     return c[:, :N]
 
 
 @pytest.mark.parametrize("M,N,K,parts", [(1, 1, 256, 1), (255, 257, 288, 1), (256, 512, 384, 1), (130, 1000, 544, 2), (700, 264, 2080, 3), (1, 8, 4096, 8), (520, 530, 1024, 4), (6000, 5000, 352, 1),
                                          (3000, 2900, 1056, 4)])
-@pytest.mark.parametrize("tile", [(0, 0), (128, 128), (128, 256), (256, 128), (256, 256)])
+@pytest.mark.parametrize("tile", [(0, form, 1) for form in range(13)] + [(64, 128, 1), (128, 128, 1), (128, 128, 2), (128, 256, 1), (256, 128, 1), (256, 256, 1)])
 def test_every_tile_of_the_product(device, M, N, K, parts, tile):
     """Exact sums, as above: more tiles than workgroups, fewer, cut at every side; contractions that end inside a step, in pieces of unequal lengths."""
     from picotron_amd import ops
