@@ -1712,33 +1712,44 @@ Tensor linear_log_probs(const Tensor& x, const Tensor& w, const Tensor& targets,
 }
 
 // ------------------------------------------------------------------------------------------------ activations and weights in 8 bits
-// e4m3 [..., cols] and its scales [ceil(cols / 128), rows, 4] (pico_mx8)
+// e4m3 [rows, cols] and its scales (pico_mx8)
 struct Mx8 {
-  Tensor data, scales;
-  bool defined() const { return data.defined(); }
-  pico_mx8 c() const { return {data.data_ptr(), scales.data_ptr()}; }
-  int64_t cols() const { return data.size(-1); }
-  int64_t rows() const { return scales.size(1); }
+  pico_mx8 c;
+  int64_t rows, cols;
 };
+// A tensor [..., cols] in that form as the caller has it: e4m3 data of its shape and scales [ceil(cols / 128), rows, 4].
 using Mx8Pair = std::pair<Tensor, Tensor>;
 using OptMx8 = std::optional<Mx8Pair>;
+// `count` operands of one size in one buffer, the scales behind the data: what lives within a call or is kept for the backward
+struct Held {
+  Tensor bytes;
+  int64_t rows, cols, count;
+  Mx8 at(int64_t i) const {
+    char* first = static_cast<char*>(bytes.data_ptr());
+    return {{first + i * rows * cols, first + count * rows * cols + i * ((cols + 127) / 128 * rows * 4)}, rows, cols};
+  }
+};
 
+int64_t mx8_rows_of(const Tensor& t) { return t.numel() / t.size(-1); }
 void check_columns(const char* fn, const Tensor& t) {
   TORCH_CHECK(t.dim() >= 1 && t.size(-1) >= 32 && t.size(-1) % 32 == 0, fn, ": the last axis must be a multiple of 32 (got ", t.sizes(), ")");
 }
-Mx8 mx8_empty(at::IntArrayRef sizes, const Tensor& like) {
-  const int64_t cols = sizes.back(), rows = c10::multiply_integers(sizes.slice(0, sizes.size() - 1));
-  return {at::empty(sizes, like.options().dtype(at::kFloat8_e4m3fn)), at::empty({(cols + 127) / 128, rows, 4}, like.options().dtype(at::kByte))};
+Held held(int64_t rows, int64_t cols, int64_t count, const Tensor& like) {
+  return {at::empty({count * rows * (cols + (cols + 127) / 128 * 4)}, like.options().dtype(at::kByte)), rows, cols, count};
 }
+Mx8Pair mx8_empty(at::IntArrayRef sizes, int64_t rows, const Tensor& like) {
+  return {at::empty(sizes, like.options().dtype(at::kFloat8_e4m3fn)), at::empty({(sizes.back() + 127) / 128, rows, 4}, like.options().dtype(at::kByte))};
+}
+Mx8 mx8_of(const Mx8Pair& p) { return {{p.first.data_ptr(), p.second.data_ptr()}, p.second.size(1), p.first.size(-1)}; }
 Mx8 mx8_given(const char* fn, const Mx8Pair& p) {
   const auto& [d, s] = p;
   on_gpu(d);
   TORCH_CHECK(d.scalar_type() == at::kFloat8_e4m3fn && d.is_contiguous(), fn, ": 8-bit data must be contiguous float8_e4m3fn (got ", d.scalar_type(), ")");
   check_columns(fn, d);
-  const int64_t cols = d.size(-1), rows = d.numel() / cols;
+  const int64_t cols = d.size(-1), rows = mx8_rows_of(d);
   TORCH_CHECK(s.scalar_type() == at::kByte && s.is_contiguous() && s.device() == d.device() && s.sizes() == at::IntArrayRef({(cols + 127) / 128, rows, 4}), fn,
               ": the scales of ", d.sizes(), " must be contiguous uint8 [", (cols + 127) / 128, ", ", rows, ", 4] on ", d.device(), " (got ", s.sizes(), " on ", s.device(), ")");
-  return {d, s};
+  return mx8_of(p);
 }
 // [..., cols] as rows that the kernels take: one pitch, 16-byte aligned (a copy where that is not so)
 Rows mx8_rows(const Tensor& given) {
@@ -1757,110 +1768,94 @@ Rows mx8_rows(const Tensor& given) {
   return as_rows(t.clone(at::MemoryFormat::Contiguous));
 }
 
-Mx8 mx8_quantized(const char* fn, const Tensor& x) {
+// contiguous and 16-byte aligned
+Tensor mx8_dense(const Tensor& given) {
+  const Tensor t = as_it_is(given).contiguous();
+  return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t : t.clone();
+}
+
+// x, whose last axis has been checked, into y; the caller has set the device
+void mx8_quantize(const char* fn, const Tensor& x, const Mx8& y) {
+  const int dt = dtype_code(x, fn);
+  const Rows r = mx8_rows(x);
+  check(pico_mx8_quantize(ptr(r.t), &y.c, r.rows, r.cols, r.pitch, dt, stream_now()));
+}
+Held mx8_held(const char* fn, const Tensor& x) {
   on_gpu(x);
   check_columns(fn, x);
-  const int dt = dtype_code(x, fn);
-  const c10::OptionalDeviceGuard device(x.device());
-  const Rows r = mx8_rows(x);
-  const Mx8 y = mx8_empty(x.sizes(), x);
-  const pico_mx8 c = y.c();
-  check(pico_mx8_quantize(ptr(r.t), &c, r.rows, r.cols, r.pitch, dt, stream_now()));
+  const Held y = held(mx8_rows_of(x), x.size(-1), 1, x);
+  mx8_quantize(fn, x, y.at(0));
   return y;
 }
-Tensor mx8_values(const Mx8& x, at::ScalarType dtype) {
-  const c10::OptionalDeviceGuard device(x.data.device());
-  const Tensor y = at::empty(x.data.sizes(), x.data.options().dtype(dtype));
-  const pico_mx8 c = x.c();
-  check(pico_mx8_dequantize(&c, ptr(y), x.rows(), x.cols(), x.cols(), dtype_code(y, "mx8_dequantize"), stream_now()));
+Tensor mx8_values(const Mx8& x, at::IntArrayRef sizes, const at::TensorOptions& o) {
+  const Tensor y = at::empty(sizes, o);
+  check(pico_mx8_dequantize(&x.c, ptr(y), x.rows, x.cols, x.cols, dtype_code(y, "mx8_dequantize"), stream_now()));
   return y;
 }
-// a [..., K] times b [N, K]^T, bf16
-Tensor mx8_product(const char* fn, const Mx8& a, const Mx8& b) {
-  TORCH_CHECK(b.data.dim() == 2 && a.cols() == b.cols() && a.data.device() == b.data.device(), fn, ": a weight of [out, ", a.cols(), "] on ", a.data.device(), " is wanted (got ", b.data.sizes(),
-              " on ", b.data.device(), ")");
-  const c10::OptionalDeviceGuard device(a.data.device());
-  const int64_t M = a.rows(), N = b.rows(), K = a.cols(), bytes = pico_mx8_product_workspace_bytes(M, N, K);
-  const auto bf16 = a.data.options().dtype(at::kBFloat16);
-  auto sizes = a.data.sizes().vec();
+// a b^T in bf16, shaped like `like` [..., K] but for the last axis; the caller has checked that K and the devices agree, and set the device
+Tensor mx8_product(const Mx8& a, const Mx8& b, const Tensor& like) {
+  const int64_t M = a.rows, N = b.rows, K = a.cols, bytes = pico_mx8_product_workspace_bytes(M, N, K);
+  const auto bf16 = like.options().dtype(at::kBFloat16);
+  auto sizes = like.sizes().vec();
   sizes.back() = N;
   const Tensor y = at::empty(sizes, bf16), rounded_up = N % 8 == 0 ? y : at::empty({M, (N + 7) / 8 * 8}, bf16);
   const Tensor ws = bytes > 0 ? at::empty({bytes}, bf16.dtype(at::kByte)) : Tensor();
-  const pico_mx8 ca = a.c(), cb = b.c();
-  check(pico_mx8_product(&ca, &cb, ptr(rounded_up), M, N, K, ptr(ws), bytes, stream_now()));
+  check(pico_mx8_product(&a.c, &b.c, ptr(rounded_up), M, N, K, ptr(ws), bytes, stream_now()));
   if (N % 8 != 0) y.view({M, N}).copy_(rounded_up.narrow(1, 0, N));
   return y;
 }
 
 struct NormMx8Out {
-  Mx8 y;
   Tensor rstd, sum;
 };
-NormMx8Out rmsnorm_mx8(const char* fn, const Tensor& x, const Tensor& weight, double eps, const OptTensor& residual, bool want_rstd) {
-  on_gpu(x);
-  on_gpu(weight);
-  on_gpu(residual);
-  check_columns(fn, x);
+// rmsnorm(x + residual) * weight into y, [rows, hidden] as x; the caller has set the device
+NormMx8Out rmsnorm_mx8(const char* fn, const Tensor& x, const Tensor& weight, double eps, const OptTensor& residual, bool want_rstd, const Mx8& y) {
   const int dt = dtype_code(x, fn);
   const int64_t hidden = x.size(-1);
   TORCH_CHECK(weight.dim() == 1 && weight.size(0) == hidden && weight.device() == x.device(), fn, ": the norm's weight must be [", hidden, "] on ", x.device(), " (got ", weight.sizes(), " on ",
               weight.device(), ")");
-  const c10::OptionalDeviceGuard device(x.device());
-  const Tensor xc = as_it_is(x).contiguous(), w = as_it_is(weight).to(x.scalar_type()).contiguous();
+  const Tensor xc = mx8_dense(x), w = mx8_dense(weight.scalar_type() == x.scalar_type() ? weight : weight.to(x.scalar_type()));
   Tensor res;
   if (residual) {
     TORCH_CHECK(residual->scalar_type() == x.scalar_type() && residual->sizes() == x.sizes() && residual->device() == x.device(), fn, ": residual must match x in dtype, shape and device");
-    res = as_it_is(*residual).contiguous();
+    res = mx8_dense(*residual);
   }
   NormMx8Out o;
-  o.y = mx8_empty(xc.sizes(), xc);
-  const int64_t rows = o.y.rows();
-  if (want_rstd) o.rstd = at::empty({rows}, xc.options().dtype(at::kFloat));
+  if (want_rstd) o.rstd = at::empty({y.rows}, xc.options().dtype(at::kFloat));
   if (res.defined()) o.sum = at::empty(xc.sizes(), xc.options());
-  const pico_mx8 c = o.y.c();
-  check(pico_rmsnorm_mx8_fwd(ptr(xc), ptr(w), &c, fptr(o.rstd), ptr(res), ptr(o.sum), rows, hidden, static_cast<float>(eps), dt, stream_now()));
+  check(pico_rmsnorm_mx8_fwd(ptr(xc), ptr(w), &y.c, fptr(o.rstd), ptr(res), ptr(o.sum), y.rows, hidden, static_cast<float>(eps), dt, stream_now()));
   return o;
 }
 
-struct SwiGLUMx8Out {
-  Tensor y;
-  Mx8 y8, gate8, up8;
-};
-SwiGLUMx8Out swiglu_mx8(const char* fn, const Tensor& gate_up, bool packed, bool keep) {
+// silu(gate) * up of the halves of gate_up into y (its dtype) or y8, and gate and up into `kept` (two operands) where that is given; the caller has set the device
+int64_t swiglu_half(const char* fn, const Tensor& gate_up) {
   on_gpu(gate_up);
   TORCH_CHECK(gate_up.dim() >= 1 && gate_up.size(-1) >= 64 && gate_up.size(-1) % 64 == 0, fn, ": gate and up must each be a multiple of 32 wide (got ", gate_up.sizes(), ")");
+  return gate_up.size(-1) / 2;
+}
+void swiglu_mx8(const char* fn, const Tensor& gate_up, const Tensor& y, const Held* y8, const Held* kept) {
   const int dt = dtype_code(gate_up, fn);
-  const c10::OptionalDeviceGuard device(gate_up.device());
   const int64_t half = gate_up.size(-1) / 2;
   const Rows whole = mx8_rows(gate_up);
-  auto sizes = gate_up.sizes().vec();
-  sizes.back() = half;
-  SwiGLUMx8Out o;
-  if (packed) o.y8 = mx8_empty(sizes, gate_up);
-  else o.y = at::empty(sizes, gate_up.options());
-  if (keep) {
-    o.gate8 = mx8_empty(sizes, gate_up);
-    o.up8 = mx8_empty(sizes, gate_up);
-  }
-  const pico_mx8 none = {}, y8 = packed ? o.y8.c() : none, g8 = keep ? o.gate8.c() : none, u8 = keep ? o.up8.c() : none;
+  const Mx8 none = {}, out = y8 ? y8->at(0) : none, gate8 = kept ? kept->at(0) : none, up8 = kept ? kept->at(1) : none;
   const char* first = static_cast<const char*>(ptr(whole.t));
-  check(pico_swiglu_mx8_fwd(first, first + half * gate_up.element_size(), ptr(o.y), packed ? &y8 : nullptr, keep ? &g8 : nullptr, keep ? &u8 : nullptr, whole.rows, half, whole.pitch,
+  check(pico_swiglu_mx8_fwd(first, first + half * gate_up.element_size(), ptr(y), y8 ? &out.c : nullptr, kept ? &gate8.c : nullptr, kept ? &up8.c : nullptr, whole.rows, half, whole.pitch,
                             whole.pitch, dt, stream_now()));
-  return o;
 }
-// d(gate_up) and, where it is wanted, silu(gate) * up of what was kept
-std::pair<Tensor, Tensor> swiglu_mx8_backward(const Tensor& dy, const Mx8& gate8, const Mx8& up8, at::ScalarType dtype, bool want_y) {
-  const c10::OptionalDeviceGuard device(gate8.data.device());
+Tensor half_of(const Tensor& gate_up) {
+  auto sizes = gate_up.sizes().vec();
+  sizes.back() /= 2;
+  return at::empty(sizes, gate_up.options());
+}
+// d(gate_up) of shape `sizes` and, where it is wanted, silu(gate) * up of what was kept, [rows, half]
+std::pair<Tensor, Tensor> swiglu_mx8_backward(const Tensor& dy, const Held& kept, at::IntArrayRef sizes, at::ScalarType dtype, bool want_y) {
   const Rows d = mx8_rows(dy.to(dtype));
-  const int64_t half = gate8.cols();
-  auto sizes = gate8.data.sizes().vec();
-  const auto o = gate8.data.options().dtype(dtype);
-  const Tensor y = want_y ? at::empty(sizes, o) : Tensor();
-  sizes.back() = 2 * half;
-  const Tensor dx = at::empty(sizes, o);
-  const pico_mx8 g = gate8.c(), u = up8.c();
+  const int64_t half = kept.cols;
+  const auto o = kept.bytes.options().dtype(dtype);
+  const Tensor dx = at::empty(sizes, o), y = want_y ? at::empty({kept.rows, half}, o) : Tensor();
+  const Mx8 gate8 = kept.at(0), up8 = kept.at(1);
   char* first = static_cast<char*>(ptr(dx));
-  check(pico_swiglu_mx8_bwd(ptr(d.t), &g, &u, first, first + half * dx.element_size(), ptr(y), gate8.rows(), half, d.pitch, 2 * half, 2 * half, dtype_code(dx, "swiglu_8bit"), stream_now()));
+  check(pico_swiglu_mx8_bwd(ptr(d.t), &gate8.c, &up8.c, first, first + half * dx.element_size(), ptr(y), kept.rows, half, d.pitch, 2 * half, 2 * half, dtype_code(dx, "swiglu_8bit"), stream_now()));
   return {dx, y};
 }
 
@@ -1872,11 +1867,15 @@ void check_weight(const char* fn, const Tensor& like, int64_t in, const Tensor& 
   TORCH_CHECK(like.scalar_type() == at::kBFloat16 && w.scalar_type() == at::kBFloat16, fn, ": activations and weight must be bf16 (got ", like.scalar_type(), " and ", w.scalar_type(), ")");
   TORCH_CHECK(w.dim() == 2 && w.size(1) == in && w.device() == like.device(), fn, ": weight must be [out, ", in, "] on ", like.device(), " (got ", w.sizes(), " on ", w.device(), ")");
 }
-Mx8 packed_weight(const char* fn, const Tensor& w, const OptMx8& given) {
-  if (!given) return mx8_quantized(fn, w);
+// the weight in 8 bits: what the caller has, or made now in `made`
+Mx8 packed_weight(const char* fn, const Tensor& w, const OptMx8& given, Held& made) {
+  if (!given) {
+    made = mx8_held(fn, w);
+    return made.at(0);
+  }
   const Mx8 p = mx8_given(fn, *given);
-  TORCH_CHECK(p.data.sizes() == w.sizes() && p.data.device() == w.device(), fn, ": packed must be the weight's 8-bit form, ", w.sizes(), " on ", w.device(), " (got ", p.data.sizes(), " on ",
-              p.data.device(), ")");
+  TORCH_CHECK(given->first.sizes() == w.sizes() && given->first.device() == w.device(), fn, ": packed must be the weight's 8-bit form, ", w.sizes(), " on ", w.device(), " (got ",
+              given->first.sizes(), " on ", given->first.device(), ")");
   return p;
 }
 bool needs_any(const AutogradContext* ctx, size_t from, size_t count) {
@@ -1887,16 +1886,18 @@ bool needs_any(const AutogradContext* ctx, size_t from, size_t count) {
 // an upstream gradient as the products take it, whatever its layout (a bias of one layout's sums against another's would be none of the caller's)
 Tensor upstream(const Tensor& given) {
   const Tensor g = as_it_is(given), m = g.dim() == 1 ? g.unsqueeze(0) : matrix(g);
-  return plain(m) && m.stride(0) % 8 == 0 ? m : m.contiguous();
+  return plain(m) && m.stride(0) % 8 == 0 ? m : mx8_dense(m);
 }
 // the gradients of x [rows, in] (as wanted) and of the weight, rows of which may be parameters of their own
 struct WeightGradients {
   Tensor dx;
   variable_list dw;
 };
-WeightGradients weight_gradients(const Tensor& dy, const Tensor& w, bool want_x, bool want_w, const std::function<Tensor()>& x, const std::vector<int64_t>& rows) {
+Tensor weight_rows(const Tensor& w) { return plain(w) ? w : mx8_dense(w); }   // (as upstream)
+WeightGradients weight_gradients(const Tensor& dy, const Tensor& given, bool want_x, bool want_w, const std::function<Tensor()>& x, const std::vector<int64_t>& rows) {
   WeightGradients r;
   Tensor dw;
+  const Tensor w = want_x ? weight_rows(given) : Tensor();
   if (want_x && want_w) {
     Gradients both = gradients(dy, w, x());
     r.dx = both.dx;
@@ -1928,41 +1929,37 @@ std::vector<int64_t> part_rows(const char* fn, const Tensor& w, at::TensorList p
 
 // y = x w^T with both in 8 bits; what is kept of x is its 8-bit form
 struct Linear8 : torch::autograd::Function<Linear8> {
-  static Tensor run(const Tensor& x, const Tensor& w, const OptMx8& packed, Mx8* kept) {
-    const char* fn = "linear_8bit";
+  static constexpr const char* fn = "linear_8bit";
+  static Tensor run(const Tensor& x, const Tensor& w, const OptMx8& packed, Held* kept) {
     TORCH_CHECK(x.dim() >= 1, fn, ": x must have an axis");
     check_weight(fn, x, x.size(-1), w);
     const c10::OptionalDeviceGuard device(x.device());
-    const Mx8 x8 = mx8_quantized(fn, x);
+    const Held x8 = mx8_held(fn, x);
     if (kept) *kept = x8;
-    return mx8_product(fn, x8, packed_weight(fn, w, packed));
+    Held made;
+    return mx8_product(x8.at(0), packed_weight(fn, w, packed, made), x);
   }
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptMx8& packed) {
-    Mx8 x8;
+    Held x8;
     const Tensor y = run(x, w, packed, &x8);
-    const bool keep = w.requires_grad();
-    ctx->save_for_backward({x.requires_grad() ? w : Tensor(), keep ? x8.data : Tensor(), keep ? x8.scales : Tensor()});
+    ctx->save_for_backward({x.requires_grad() ? w : Tensor(), w.requires_grad() ? x8.bytes : Tensor()});
+    ctx->saved_data["sizes"] = x.sizes().vec();
     return y;
   }
+  // the values of an operand that was kept, [rows, cols]
+  static Tensor values(const Tensor& bytes, int64_t rows, int64_t cols) { return mx8_values(Held{bytes, rows, cols, 1}.at(0), {rows, cols}, bytes.options().dtype(at::kBFloat16)); }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
-    refuse_second_order("linear_8bit");
+    refuse_second_order(fn);
     const auto s = ctx->get_saved_variables();
+    const auto sizes = ctx->saved_data["sizes"].toIntVector();
     const c10::OptionalDeviceGuard device(g[0].device());
-    auto sizes = g[0].sizes().vec();
     const Tensor dy = upstream(g[0]);
-    WeightGradients r = weight_gradients(dy, s[0], ctx->needs_input_grad(0), ctx->needs_input_grad(1), [&] { return matrix8(s[1], s[2]); }, {});
-    if (r.dx.defined()) {
-      sizes.back() = r.dx.size(1);
-      r.dx = r.dx.view(sizes);
-    }
-    return {r.dx, r.dw[0], Tensor()};
-  }
-  static Tensor matrix8(const Tensor& data, const Tensor& scales) {   // the values of a kept operand, [rows, cols]
-    return mx8_values({data.view({scales.size(1), data.size(-1)}), scales}, at::kBFloat16);
+    WeightGradients r = weight_gradients(dy, s[0], ctx->needs_input_grad(0), ctx->needs_input_grad(1), [&] { return values(s[1], dy.size(0), sizes.back()); }, {});
+    return {r.dx.defined() ? r.dx.view(sizes) : Tensor(), r.dw[0], Tensor()};
   }
 };
 Tensor linear_8bit(const Tensor& x, const Tensor& w, const OptMx8& packed) {
-  refuse_tangents("linear_8bit", {&x, &w});
+  refuse_tangents(Linear8::fn, {&x, &w});
   if (!records({&x, &w})) return Linear8::run(x, w, packed, nullptr);
   return Linear8::apply(x, w, packed);
 }
@@ -1971,23 +1968,31 @@ Tensor linear_8bit(const Tensor& x, const Tensor& w, const OptMx8& packed) {
 // block by row block, they get its gradient.
 struct NormLinear8 : torch::autograd::Function<NormLinear8> {
   static constexpr const char* fn = "rms_norm_linear_8bit";
-  static variable_list run(const Tensor& x, const OptTensor& residual, const Tensor& norm_weight, double eps, const Tensor& w, const OptMx8& packed, NormMx8Out* kept) {
+  struct Kept {
+    Held y;
+    NormMx8Out norm;
+  };
+  static variable_list run(const Tensor& x, const OptTensor& residual, const Tensor& norm_weight, double eps, const Tensor& w, const OptMx8& packed, Kept* kept) {
     TORCH_CHECK(x.dim() >= 1, fn, ": x must have an axis");
     check_weight(fn, x, x.size(-1), w);
+    on_gpu(norm_weight);
+    on_gpu(residual);
+    check_columns(fn, x);
     const c10::OptionalDeviceGuard device(x.device());
-    NormMx8Out o = rmsnorm_mx8(fn, x, norm_weight, eps, residual, kept != nullptr);
-    const Tensor y = mx8_product(fn, o.y, packed_weight(fn, w, packed));
-    if (kept) *kept = o;
-    return {y, residual ? o.sum : x};
+    const Held y8 = held(mx8_rows_of(x), x.size(-1), 1, x);
+    const NormMx8Out norm = rmsnorm_mx8(fn, x, norm_weight, eps, residual, kept != nullptr, y8.at(0));
+    if (kept) *kept = {y8, norm};
+    Held made;
+    return {mx8_product(y8.at(0), packed_weight(fn, w, packed, made), x), residual ? norm.sum : x};
   }
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& residual, const Tensor& norm_weight, double eps, const Tensor& w, const OptMx8& packed,
                                at::TensorList parts) {
     ctx->saved_data["rows"] = part_rows(fn, w, parts);
-    NormMx8Out kept;
+    Kept kept;
     variable_list out = run(x, residual, norm_weight, eps, w, packed, &kept);
     bool keep = w.requires_grad();
     for (const Tensor& p : parts) keep |= p.requires_grad();
-    ctx->save_for_backward({residual ? out[1] : x, norm_weight, kept.rstd, w, keep ? kept.y.data : Tensor(), keep ? kept.y.scales : Tensor()});
+    ctx->save_for_backward({residual ? out[1] : x, norm_weight, kept.norm.rstd, w, keep ? kept.y.bytes : Tensor()});
     ctx->saved_data["residual"] = residual.has_value();
     ctx->set_materialize_grads(false);   // (the stream's h may have no other reader)
     return out;
@@ -2007,9 +2012,9 @@ struct NormLinear8 : torch::autograd::Function<NormLinear8> {
     const Tensor dy = upstream(g[0]);
     const size_t at_gamma = has_residual ? 2 : 1;   // (among the tensors: eps, packed and a residual that is none do not count)
     const bool wants_norm = needs_any(ctx, 0, at_gamma + 1), wants_w = rows.empty() ? ctx->needs_input_grad(at_gamma + 1) : needs_any(ctx, at_gamma + 2, rows.size());
-    WeightGradients d = weight_gradients(dy, s[3], wants_norm, wants_w, [&] { return Linear8::matrix8(s[4], s[5]); }, rows);
+    WeightGradients d = weight_gradients(dy, s[3], wants_norm, wants_w, [&] { return Linear8::values(s[4], dy.size(0), s[3].size(1)); }, rows);
     if (wants_norm) {
-      auto [dx, dgamma] = rmsnorm_backward(d.dx.view(s[0].sizes()), as_it_is(s[0]), as_it_is(s[1]), s[2], g[1].defined() ? OptTensor(as_it_is(g[1])) : std::nullopt, s[1].scalar_type());
+      auto [dx, dgamma] = rmsnorm_backward(d.dx.view(s[0].sizes()), mx8_dense(s[0]), mx8_dense(s[1]), s[2], g[1].defined() ? OptTensor(mx8_dense(g[1])) : std::nullopt, s[1].scalar_type());
       r[0] = dx;
       if (has_residual) r[1] = dx;
       r[2] = dgamma;
@@ -2036,53 +2041,69 @@ std::pair<Tensor, Tensor> rms_norm_linear_8bit(const Tensor& x, const OptTensor&
 
 // silu(gate) * up of the two halves of gate_up; gate and up are kept in 8 bits and the gradient is taken at the values that these stand for
 struct SwiGLU8 : torch::autograd::Function<SwiGLU8> {
+  static constexpr const char* fn = "swiglu_8bit";
+  static Tensor run(const Tensor& gate_up, Held* kept) {
+    const int64_t half = swiglu_half(fn, gate_up);
+    const c10::OptionalDeviceGuard device(gate_up.device());
+    const Tensor y = half_of(gate_up);
+    if (kept) *kept = held(mx8_rows_of(gate_up), half, 2, gate_up);
+    swiglu_mx8(fn, gate_up, y, nullptr, kept);
+    return y;
+  }
   static Tensor forward(AutogradContext* ctx, const Tensor& gate_up) {
-    SwiGLUMx8Out o = swiglu_mx8("swiglu_8bit", gate_up, false, true);
-    ctx->save_for_backward({o.gate8.data, o.gate8.scales, o.up8.data, o.up8.scales});
+    Held kept;
+    const Tensor y = run(gate_up, &kept);
+    ctx->save_for_backward({kept.bytes});
+    ctx->saved_data["sizes"] = gate_up.sizes().vec();
     ctx->saved_data["dtype"] = static_cast<int64_t>(gate_up.scalar_type());
-    return o.y;
+    return y;
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
-    refuse_second_order("swiglu_8bit");
-    const auto s = ctx->get_saved_variables();
-    return {swiglu_mx8_backward(g[0], {s[0], s[1]}, {s[2], s[3]}, static_cast<at::ScalarType>(ctx->saved_data["dtype"].toInt()), false).first};
+    refuse_second_order(fn);
+    const Tensor bytes = ctx->get_saved_variables()[0];
+    const auto sizes = ctx->saved_data["sizes"].toIntVector();
+    const c10::OptionalDeviceGuard device(bytes.device());
+    const int64_t half = sizes.back() / 2;
+    return {swiglu_mx8_backward(g[0], {bytes, g[0].numel() / half, half, 2}, sizes, static_cast<at::ScalarType>(ctx->saved_data["dtype"].toInt()), false).first};
   }
 };
 Tensor swiglu_8bit(const Tensor& gate_up) {
-  refuse_tangents("swiglu_8bit", {&gate_up});
-  if (!records({&gate_up})) return swiglu_mx8("swiglu_8bit", gate_up, false, false).y;
+  refuse_tangents(SwiGLU8::fn, {&gate_up});
+  if (!records({&gate_up})) return SwiGLU8::run(gate_up, nullptr);
   return SwiGLU8::apply(gate_up);
 }
 
 // The same, in 8 bits, times w^T.  The weight's gradient takes silu(gate) * up of what was kept, which the kernel of gate's and up's gradients writes beside them.
 struct SwiGLULinear8 : torch::autograd::Function<SwiGLULinear8> {
   static constexpr const char* fn = "swiglu_linear_8bit";
-  static Tensor run(const Tensor& gate_up, const Tensor& w, const OptMx8& packed, SwiGLUMx8Out* kept) {
+  static Tensor run(const Tensor& gate_up, const Tensor& w, const OptMx8& packed, Held* kept) {
     TORCH_CHECK(gate_up.dim() >= 1 && gate_up.size(-1) % 2 == 0, fn, ": gate_up must hold two halves (got ", gate_up.sizes(), ")");
     check_weight(fn, gate_up, gate_up.size(-1) / 2, w);
+    const int64_t half = swiglu_half(fn, gate_up), rows = mx8_rows_of(gate_up);
     const c10::OptionalDeviceGuard device(gate_up.device());
-    SwiGLUMx8Out o = swiglu_mx8(fn, gate_up, true, kept != nullptr);
-    const Tensor y = mx8_product(fn, o.y8, packed_weight(fn, w, packed));
-    if (kept) *kept = o;
-    return y;
+    const Held y8 = held(rows, half, 1, gate_up);
+    if (kept) *kept = held(rows, half, 2, gate_up);
+    swiglu_mx8(fn, gate_up, Tensor(), &y8, kept);
+    Held made;
+    return mx8_product(y8.at(0), packed_weight(fn, w, packed, made), gate_up);
   }
   static Tensor forward(AutogradContext* ctx, const Tensor& gate_up, const Tensor& w, const OptMx8& packed) {
-    SwiGLUMx8Out kept;
+    Held kept;
     const Tensor y = run(gate_up, w, packed, &kept);
-    ctx->save_for_backward({w, kept.gate8.data, kept.gate8.scales, kept.up8.data, kept.up8.scales});
+    ctx->save_for_backward({w, kept.bytes});
+    ctx->saved_data["sizes"] = gate_up.sizes().vec();
     return y;
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
     refuse_second_order(fn);
     const auto s = ctx->get_saved_variables();
     const c10::OptionalDeviceGuard device(g[0].device());
-    const Tensor dy = upstream(g[0]);
+    const Tensor dy = upstream(g[0]), w = weight_rows(s[0]);
     variable_list r(3);
     const bool wants_w = ctx->needs_input_grad(1);
-    const Tensor dh = product(dy, s[0], Product::NN);
-    auto [dx, h] = swiglu_mx8_backward(dh, {s[1], s[2]}, {s[3], s[4]}, at::kBFloat16, wants_w);
+    auto [dx, h] = swiglu_mx8_backward(product(dy, w, Product::NN), {s[1], dy.size(0), w.size(1), 2}, ctx->saved_data["sizes"].toIntVector(), at::kBFloat16, wants_w);
     if (ctx->needs_input_grad(0)) r[0] = dx;
-    if (wants_w) r[1] = product(dy, h.view({dy.size(0), s[0].size(1)}), Product::TN);
+    if (wants_w) r[1] = product(dy, h, Product::TN);
     return r;
   }
 };
@@ -2266,14 +2287,34 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("preference_loss", &preference_loss, nogil());
   m.def("linear_log_probs", &linear_log_probs, nogil());
   m.def("mx8_quantize", [](const Tensor& x) {
-    const Mx8 y = mx8_quantized("mx8_quantize", x);
-    return Mx8Pair{y.data, y.scales};
+    on_gpu(x);
+    check_columns("mx8_quantize", x);
+    const c10::OptionalDeviceGuard device(x.device());
+    const Mx8Pair y = mx8_empty(x.sizes(), mx8_rows_of(x), x);
+    mx8_quantize("mx8_quantize", x, mx8_of(y));
+    return y;
   }, nogil());
-  m.def("mx8_dequantize", [](const Mx8Pair& x, at::ScalarType dtype) { return mx8_values(mx8_given("mx8_dequantize", x), dtype); }, nogil());
-  m.def("mx8_product", [](const Mx8Pair& a, const Mx8Pair& b) { return mx8_product("mx8_product", mx8_given("mx8_product", a), mx8_given("mx8_product", b)); }, nogil());
+  m.def("mx8_dequantize", [](const Mx8Pair& x, at::ScalarType dtype) {
+    const Mx8 c = mx8_given("mx8_dequantize", x);
+    const c10::OptionalDeviceGuard device(x.first.device());
+    return mx8_values(c, x.first.sizes(), x.first.options().dtype(dtype));
+  }, nogil());
+  m.def("mx8_product", [](const Mx8Pair& a, const Mx8Pair& b) {
+    const Mx8 ca = mx8_given("mx8_product", a), cb = mx8_given("mx8_product", b);
+    TORCH_CHECK(b.first.dim() == 2 && ca.cols == cb.cols && a.first.device() == b.first.device(), "mx8_product: a weight of [out, ", ca.cols, "] on ", a.first.device(), " is wanted (got ",
+                b.first.sizes(), " on ", b.first.device(), ")");
+    const c10::OptionalDeviceGuard device(a.first.device());
+    return mx8_product(ca, cb, a.first);
+  }, nogil());
   m.def("rmsnorm_mx8_fwd", [](const Tensor& x, const Tensor& w, double eps, const OptTensor& residual) {
-    NormMx8Out o = rmsnorm_mx8("rmsnorm_mx8_fwd", x, w, eps, residual, true);
-    return std::make_tuple(o.y.data, o.y.scales, o.rstd, o.sum.defined() ? OptTensor(o.sum) : std::nullopt);
+    on_gpu(x);
+    on_gpu(w);
+    on_gpu(residual);
+    check_columns("rmsnorm_mx8_fwd", x);
+    const c10::OptionalDeviceGuard device(x.device());
+    const Mx8Pair y = mx8_empty(x.sizes(), mx8_rows_of(x), x);
+    NormMx8Out o = rmsnorm_mx8("rmsnorm_mx8_fwd", x, w, eps, residual, true, mx8_of(y));
+    return std::make_tuple(y.first, y.second, o.rstd, o.sum.defined() ? OptTensor(o.sum) : std::nullopt);
   }, nogil());
   m.def("linear_8bit", &linear_8bit, nogil());
   m.def("rms_norm_linear_8bit", &rms_norm_linear_8bit, nogil());

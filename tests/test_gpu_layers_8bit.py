@@ -315,6 +315,27 @@ def test_inputs_of_any_layout(device):
         assert torch.equal(functional.swiglu_linear_8bit(a, w[:, :64]), functional.swiglu_linear_8bit(b, w[:, :64].contiguous()))
 
 
+def test_tensors_that_start_anywhere(device):
+    """Contiguous, but 2 bytes behind a 16-byte boundary: every input and every upstream gradient."""
+    leaves, dy, dh = layer_inputs()
+    def moved(t):
+        flat = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")
+        flat[1:] = t.detach().reshape(-1)
+        return flat[1:].view(t.shape)
+    for residual in (True, False):
+        args = [t if residual or i != 1 else None for i, t in enumerate(leaves)]
+        away = [None if t is None else moved(t).requires_grad_() for t in args]
+        (y, h), (ya, ha) = layer(*args), layer(*away)
+        want = torch.autograd.grad((y, h), [t for t in args if t is not None], (dy, dh))
+        got = torch.autograd.grad((ya, ha), [t for t in away if t is not None], (moved(dy), moved(dh)))
+        assert torch.equal(y, ya) and torch.equal(h, ha) and all(torch.equal(a, b) for a, b in zip(want, got))
+    from picotron_amd import functional
+    a, b = leaves[3], moved(leaves[3]).requires_grad_()
+    d = randn(a.size(0), a.size(1) // 2, g=gen(1))
+    pair = [torch.autograd.grad(functional.swiglu_8bit(t[:, :128]), t, g[:, :64])[0] for t, g in ((a, d), (b, moved(d)))]
+    assert torch.equal(*pair)
+
+
 def test_empty_batches_train(device):
     leaves, dy, dh = layer_inputs(M=0)
     y, h = layer(*leaves)
