@@ -370,6 +370,13 @@ int pico_product_large_takes(int64_t M, int64_t N, int64_t K, int64_t lda, int64
 int pico_product_large(const void* a, const void* b, void* c, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int a_slow,
                        int b_slow, int tile_m, int tile_n, int parts, void* stream);
 
+/* The same as pico_product_large and pico_product_mid (of the latter the tiles that it takes in parts), with the fp32 sums themselves as the result, [parts, M, N], also
+ * for one piece. */
+int pico_product_large_sums(const void* a, const void* b, float* sums, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int a_slow,
+                            int b_slow, int tile_m, int tile_n, int parts, void* stream);
+int pico_product_mid_sums(const void* a, const void* b, float* sums, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int a_slow,
+                          int b_slow, int tile_m, int tile_n, int parts, void* stream);
+
 /* y[c][r] = x[r][c] for bf16 x [rows, cols] with row pitch x_pitch and y [cols, rows] with row pitch y_pitch (elements).  cols
  * and both pitches must be multiples of 8, pointers 16-byte aligned; where rows is no multiple of 8, zeros follow a row of y
  * up to the next multiple.  Lays an operand of a weight gradient out as the GEMM library reads it faster.
@@ -555,6 +562,10 @@ int pico_mx8_dequantize(const pico_mx8* x, void* y, int64_t rows, int64_t cols, 
  * up to 16384.  The backward is pico_rmsnorm_bwd, with the gradient of the values that y stands for. */
 int pico_rmsnorm_mx8_fwd(const void* x, const void* weight, const pico_mx8* y, float* rstd, const void* residual_in, void* residual_out,
                          int64_t rows, int64_t hidden, float eps, int dtype, void* stream);
+/* pico_rmsnorm_bwd for a gradient that a product left in fp32, in `parts` (1 .. 64) pieces to be added: dy [parts, rows, hidden]; x, weight, dresidual (may be NULL) and dx
+ * bf16, dx in no input's place.  workspace: pico_rmsnorm_bwd_workspace_bytes bytes. */
+int pico_rmsnorm_bwd_sums(const float* dy, int parts, const void* x, const void* weight, const float* rstd, const void* dresidual, void* dx,
+                          void* dweight, int dweight_dtype, void* workspace, int64_t workspace_bytes, int64_t rows, int64_t hidden, void* stream);
 /* silu(gate) * up into y (contiguous, `dtype`), y8, or both; gate8 and up8 (both or neither) take what pico_swiglu_mx8_bwd reads. */
 int pico_swiglu_mx8_fwd(const void* gate, const void* up, void* y, const pico_mx8* y8, const pico_mx8* gate8, const pico_mx8* up8,
                         int64_t rows, int64_t cols, int64_t gate_ld, int64_t up_ld, int dtype, void* stream);

@@ -1888,32 +1888,67 @@ Tensor upstream(const Tensor& given) {
   const Tensor g = as_it_is(given), m = g.dim() == 1 ? g.unsqueeze(0) : matrix(g);
   return plain(m) && m.stride(0) % 8 == 0 ? m : mx8_dense(m);
 }
-// the gradients of x [rows, in] (as wanted) and of the weight, rows of which may be parameters of their own
-struct WeightGradients {
-  Tensor dx;
-  variable_list dw;
-};
 Tensor weight_rows(const Tensor& w) { return plain(w) ? w : mx8_dense(w); }   // (as upstream)
-WeightGradients weight_gradients(const Tensor& dy, const Tensor& given, bool want_x, bool want_w, const std::function<Tensor()>& x, const std::vector<int64_t>& rows) {
-  WeightGradients r;
-  Tensor dw;
+// dy [rows, out] and w [out, in] with zeros up to a multiple of 8 outputs, as the kernels that leave fp32 sums take them.  (The library takes them as they are: there the copies do not pay, us
+// for both gradients without and with them, [4096 x 5003] and [5003 x 2048] 191, 222; [4096 x 15001] and [15001 x 4096] 920, 886.)
+struct Rounded {
+  Tensor dy, w;
+};
+Rounded rounded_up(const Tensor& dy, const Tensor& w) {
+  const int64_t out = dy.size(1), more = (8 - out % 8) % 8;
+  if (more == 0 || dy.size(0) == 0) return {dy, w};
+  return {at::constant_pad_nd(dy, {0, more}), at::constant_pad_nd(w, {0, 0, 0, more})};
+}
+// the gradients of x [rows, in] and of the weight, as wanted
+struct WeightGradients {
+  Tensor dx, dw;
+};
+WeightGradients weight_gradients(const Tensor& dy, const Tensor& given, bool want_x, bool want_w, const std::function<Tensor()>& x) {
   const Tensor w = want_x ? weight_rows(given) : Tensor();
   if (want_x && want_w) {
-    Gradients both = gradients(dy, w, x());
-    r.dx = both.dx;
-    dw = both.dw;
-  } else if (want_w) {
-    dw = product(dy, x(), Product::TN);
-  } else if (want_x) {
-    r.dx = product(dy, w, Product::NN);
+    const Gradients both = gradients(dy, w, x());
+    return {both.dx, both.dw};
   }
-  if (rows.empty()) r.dw.push_back(dw);
-  int64_t at_row = 0;
-  for (int64_t n : rows) {
-    r.dw.push_back(dw.defined() ? dw.narrow(0, at_row, n) : Tensor());
-    at_row += n;
+  return {want_x ? product(dy, w, Product::NN) : Tensor(), want_w ? product(dy, x(), Product::TN) : Tensor()};
+}
+// dy w in fp32, in pieces to be added, as pico_rmsnorm_bwd_sums takes it; `parts` 0 where no kernel gives that (torch settings ask for another route)
+struct Sums {
+  Tensor t;
+  int parts;
+};
+Sums input_sums(const Tensor& dy, const Tensor& w) {
+  if (dy.size(0) == 0 || stays_with_torch(dy, w)) return {Tensor(), 0};
+  const ProductSizes n = product_sizes(dy, w, Product::NN);
+  if (!pico_product_mid_takes(n.M, n.N, n.K, n.lda, n.ldb, 0, 1)) return {Tensor(), 0};
+  const ProductRoute r = product_route(Product::NN, n);
+  int tile_m = static_cast<int>(r.tile_m), tile_n = static_cast<int>(r.tile_n), parts = static_cast<int>(r.parts);
+  bool large = r.kernel == ProductRoute::Large;
+  if (r.kernel == ProductRoute::Mid) {   // (tiles under 64 x 96 have no form in fp32)
+    if (tile_m * tile_n <= 64 * 64) tile_m = 64, tile_n = 96;
+    else if (tile_m * tile_n == 96 * 64) tile_m = tile_n = 96;
+    else if (tile_m == 128 && tile_n < 128) tile_n = 128;
+  } else if (!large) {   // what goes to the library, or to the kernel of few rows
+    large = n.M >= 256 && n.N >= 256 && pico_product_large_takes(n.M, n.N, n.K, n.lda, n.ldb, 0, 1, 1);
+    tile_m = large ? 256 : 64;
+    tile_n = large ? 256 : 128;
+    // pieces where the tiles leave CUs idle, 256 of contraction each at least
+    const int64_t tiles = ((n.M + tile_m - 1) / tile_m) * ((n.N + tile_n - 1) / tile_n);
+    parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({256 / tiles, n.K / 256, 8})));
   }
-  return r;
+  const Sums s = {at::empty({parts, n.M, n.N}, dy.options().dtype(at::kFloat)), parts};
+  check((large ? pico_product_large_sums : pico_product_mid_sums)(ptr(dy), ptr(w), fptr(s.t), n.M, n.N, n.K, n.lda, n.ldb, 0, 1, tile_m, tile_n, parts, stream_now()));
+  return s;
+}
+// The gradients of a norm [rows, hidden] in front of a weight, from that of the product, all bf16.
+std::pair<Tensor, Tensor> norm_gradients(const Tensor& dy, const Tensor& w, const Tensor& x, const Tensor& norm_weight, const Tensor& rstd, const OptTensor& dresidual) {
+  const Sums s = input_sums(dy, w);
+  if (s.parts == 0) return rmsnorm_backward(product(dy, w, Product::NN).view(x.sizes()), x, norm_weight, rstd, dresidual, norm_weight.scalar_type());
+  const int64_t hidden = x.size(-1), rows = dy.size(0), bytes = pico_rmsnorm_bwd_workspace_bytes(rows, hidden);
+  const Tensor weight = norm_weight.to(at::kBFloat16), dres = dresidual ? dresidual->to(at::kBFloat16) : Tensor();
+  const Tensor dx = at::empty(x.sizes(), x.options()), dw = at::empty({hidden}, norm_weight.options()), ws = at::empty({bytes}, x.options().dtype(at::kByte));
+  check(pico_rmsnorm_bwd_sums(fptr(s.t), s.parts, ptr(x), ptr(weight), fptr(rstd), ptr(dres), ptr(dx), ptr(dw), dtype_code(dw, "rms_norm_linear_8bit: norm_weight"), ptr(ws), bytes, rows, hidden,
+                              stream_now()));
+  return {dx, dw};
 }
 std::vector<int64_t> part_rows(const char* fn, const Tensor& w, at::TensorList parts) {
   std::vector<int64_t> rows;
@@ -1954,8 +1989,8 @@ struct Linear8 : torch::autograd::Function<Linear8> {
     const auto sizes = ctx->saved_data["sizes"].toIntVector();
     const c10::OptionalDeviceGuard device(g[0].device());
     const Tensor dy = upstream(g[0]);
-    WeightGradients r = weight_gradients(dy, s[0], ctx->needs_input_grad(0), ctx->needs_input_grad(1), [&] { return values(s[1], dy.size(0), sizes.back()); }, {});
-    return {r.dx.defined() ? r.dx.view(sizes) : Tensor(), r.dw[0], Tensor()};
+    WeightGradients r = weight_gradients(dy, s[0], ctx->needs_input_grad(0), ctx->needs_input_grad(1), [&] { return values(s[1], dy.size(0), sizes.back()); });
+    return {r.dx.defined() ? r.dx.view(sizes) : Tensor(), r.dw, Tensor()};
   }
 };
 Tensor linear_8bit(const Tensor& x, const Tensor& w, const OptMx8& packed) {
@@ -2009,18 +2044,22 @@ struct NormLinear8 : torch::autograd::Function<NormLinear8> {
     }
     const auto s = ctx->get_saved_variables();
     const c10::OptionalDeviceGuard device(g[0].device());
-    const Tensor dy = upstream(g[0]);
     const size_t at_gamma = has_residual ? 2 : 1;   // (among the tensors: eps, packed and a residual that is none do not count)
     const bool wants_norm = needs_any(ctx, 0, at_gamma + 1), wants_w = rows.empty() ? ctx->needs_input_grad(at_gamma + 1) : needs_any(ctx, at_gamma + 2, rows.size());
-    WeightGradients d = weight_gradients(dy, s[3], wants_norm, wants_w, [&] { return Linear8::values(s[4], dy.size(0), s[3].size(1)); }, rows);
+    const Tensor dy = upstream(g[0]);
     if (wants_norm) {
-      auto [dx, dgamma] = rmsnorm_backward(d.dx.view(s[0].sizes()), mx8_dense(s[0]), mx8_dense(s[1]), s[2], g[1].defined() ? OptTensor(mx8_dense(g[1])) : std::nullopt, s[1].scalar_type());
+      const Rounded whole = rounded_up(dy, weight_rows(s[3]));
+      auto [dx, dgamma] = norm_gradients(whole.dy, whole.w, mx8_dense(s[0]), mx8_dense(s[1]), s[2], g[1].defined() ? OptTensor(mx8_dense(g[1])) : std::nullopt);
       r[0] = dx;
       if (has_residual) r[1] = dx;
       r[2] = dgamma;
     }
-    if (rows.empty()) r[4] = d.dw[0];
-    for (size_t i = 0; i < rows.size(); ++i) r[6 + i] = d.dw[i];
+    if (wants_w) {
+      const Tensor dw = product(dy, Linear8::values(s[4], dy.size(0), s[3].size(1)), Product::TN);
+      if (rows.empty()) r[4] = dw;
+      int64_t at_row = 0;
+      for (size_t i = 0; i < rows.size(); ++i, at_row += rows[i - 1]) r[6 + i] = dw.narrow(0, at_row, rows[i]);
+    }
     return r;
   }
 };

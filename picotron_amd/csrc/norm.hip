@@ -355,6 +355,111 @@ __global__ __launch_bounds__(NWAVE * kWave) void rmsnorm_bwd_wave_kernel(
   }
 }
 
+// The backward from fp32 gradients that lie in pieces, as a product leaves them: dy = sum over `parts` of sums [parts, rows, hidden].  A dy that was rounded to bf16 on its way, an x that
+// was rounded (the residual stream) and a rounded dweight are three errors of one size in dweight; here the first is left out.  bf16 x, w, dres and dx.  Rows to a wave (G 64) or to the
+// workgroup (G 256), dweight's share in registers over all rows of a group.  Bound by memory: 4 parts + 6 bytes an element.
+constexpr int kSumsThreads = 256;
+template <int G, int NV, bool kRes>
+__global__ __launch_bounds__(kSumsThreads) void rmsnorm_bwd_sums_kernel(const float* __restrict__ sums, int parts, const __bf16* __restrict__ x, const __bf16* __restrict__ w,
+                                                                        const float* __restrict__ rstd, const __bf16* __restrict__ dres, __bf16* __restrict__ dx,
+                                                                        float* __restrict__ partial, int64_t rows, int hidden) {
+  Arguments<0, 64>().arrive();
+  constexpr int V = 8, kGroups = kSumsThreads / G;
+  __shared__ float smem[kSumsThreads / kWave];
+  extern __shared__ __attribute__((aligned(16))) float dw_lds[];   // [hidden] where there are several groups
+  const int t = threadIdx.x % G, nvec = hidden / V;
+  const int gid = G == kWave ? __builtin_amdgcn_readfirstlane(threadIdx.x / G) : 0;
+  const float inv_h = 1.f / static_cast<float>(hidden);
+  float dw[NV][V];
+  u32x4 wp[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int v = t + j * G < nvec ? t + j * G : 0;
+    wp[j] = *reinterpret_cast<const u32x4*>(w + v * V);
+#pragma unroll
+    for (int e = 0; e < V; ++e) dw[j][e] = 0.f;
+  }
+  // (G 256: one row to the workgroup, whose trips are uniform over it)
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + gid; row < rows; row += static_cast<int64_t>(gridDim.x) * kGroups) {
+    f32x4 d[NV][2];
+    u32x4 xr[NV], rr[kRes ? NV : 1];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int64_t at = row * hidden + (t + j * G < nvec ? t + j * G : 0) * V;
+      d[j][0] = *reinterpret_cast<const f32x4*>(sums + at);
+      d[j][1] = *reinterpret_cast<const f32x4*>(sums + at + 4);
+      xr[j] = *reinterpret_cast<const u32x4*>(x + at);
+      if constexpr (kRes) rr[j] = *reinterpret_cast<const u32x4*>(dres + at);
+    }
+    for (int q = 1; q < parts; ++q) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const float* more = sums + (q * rows + row) * hidden + (t + j * G < nvec ? t + j * G : 0) * V;
+        d[j][0] += *reinterpret_cast<const f32x4*>(more);
+        d[j][1] += *reinterpret_cast<const f32x4*>(more + 4);
+      }
+    }
+    const float r = rstd[row];
+    float c = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (t + j * G < nvec) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const uint32_t xb = xr[j][e / 2], wb = wp[j][e / 2];
+          const float xh = __uint_as_float(e % 2 ? xb & 0xffff0000u : xb << 16) * r, wv = __uint_as_float(e % 2 ? wb & 0xffff0000u : wb << 16), dv = d[j][e / 4][e % 4];
+          c += dv * wv * xh;
+          dw[j][e] += dv * xh;
+        }
+      }
+    }
+    c = wave_sum(c);
+    if constexpr (G > kWave) {
+      __syncthreads();
+      if (threadIdx.x % kWave == 0) smem[threadIdx.x / kWave] = c;
+      __syncthreads();
+      c = smem[0];
+#pragma unroll
+      for (int i = 1; i < G / kWave; ++i) c += smem[i];
+    }
+    c *= inv_h;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (t + j * G < nvec) {
+        float o[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const uint32_t xb = xr[j][e / 2], wb = wp[j][e / 2];
+          const float xv = __uint_as_float(e % 2 ? xb & 0xffff0000u : xb << 16), wv = __uint_as_float(e % 2 ? wb & 0xffff0000u : wb << 16);
+          o[e] = r * (d[j][e / 4][e % 4] * wv - xv * r * c);
+          if constexpr (kRes) o[e] += __uint_as_float(e % 2 ? rr[j][e / 2] & 0xffff0000u : rr[j][e / 2] << 16);
+        }
+        io<__bf16>::store(dx + row * hidden + static_cast<int64_t>(t + j * G) * V, o);
+      }
+    }
+  }
+  float* out = partial + static_cast<int64_t>(blockIdx.x) * hidden;
+  // the groups add their shares one after the other: the same sum on every run
+  for (int turn = 0; turn < kGroups; ++turn) {
+    if (gid == turn) {
+      float* to = turn == kGroups - 1 ? out : dw_lds;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int v = t + j * G;
+        if (v < nvec) {
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            f32x4 sum = {dw[j][4 * q], dw[j][4 * q + 1], dw[j][4 * q + 2], dw[j][4 * q + 3]};
+            if (turn > 0) sum += *reinterpret_cast<const f32x4*>(dw_lds + v * V + 4 * q);
+            *reinterpret_cast<f32x4*>(to + v * V + 4 * q) = sum;
+          }
+        }
+      }
+    }
+    if constexpr (kGroups > 1) __syncthreads();
+  }
+}
+
 // dweight[c] = sum_p partial[p][c]; 32 columns x 32 slices per block, every thread's loads issued together.
 constexpr int kReduceCols = 32;
 constexpr int kReduceSlices = 1024 / kReduceCols;
@@ -670,6 +775,25 @@ int64_t bwd_partial_bytes(int64_t rows, int64_t hidden, int dtype) {
   return static_cast<int64_t>(bwd_blocks(rows, kBwdThreads / 256, static_cast<int>(hidden))) * hidden * static_cast<int64_t>(sizeof(float));
 }
 
+// Launches rmsnorm_bwd_sums_kernel: the blocks that it takes.
+int launch_bwd_sums(const float* sums, int parts, const void* x, const void* w, const float* rstd, const void* dres, void* dx, float* partial, int64_t rows, int hidden, hipStream_t s) {
+  const int nvec = hidden / 8;
+  auto go = [&](auto plain, auto with_residual, int groups) {
+    const int blocks = bwd_blocks(rows, groups, hidden);
+    hipLaunchKernelGGL(dres ? with_residual : plain, dim3(blocks), dim3(kSumsThreads), groups > 1 ? hidden * sizeof(float) : 0, s, sums, parts, static_cast<const __bf16*>(x),
+                       static_cast<const __bf16*>(w), rstd, static_cast<const __bf16*>(dres), static_cast<__bf16*>(dx), partial, rows, hidden);
+    return blocks;
+  };
+#define PICO_SUMS(G, NV) return go(rmsnorm_bwd_sums_kernel<G, NV, false>, rmsnorm_bwd_sums_kernel<G, NV, true>, kSumsThreads / G)
+  if (nvec <= 64) PICO_SUMS(64, 1);
+  if (nvec <= 128) PICO_SUMS(64, 2);
+  if (nvec <= 256) PICO_SUMS(64, 4);
+  if (nvec <= 512) PICO_SUMS(64, 8);
+  if (nvec <= 1024) PICO_SUMS(256, 4);
+  PICO_SUMS(256, 8);
+#undef PICO_SUMS
+}
+
 int check_common(const char* fn, int64_t rows, int64_t hidden, int dtype) {
   if (dtype != PICO_BF16 && dtype != PICO_F32) return fail(PICO_ERR_DTYPE, "%s: dtype code %d not supported", fn, dtype);
   const int vec = dtype == PICO_BF16 ? 8 : 4;
@@ -798,4 +922,28 @@ extern "C" int pico_rmsnorm_bwd_static(const void* dy, const void* x, const void
   if (int rc = static_scratch(fn, &partial)) return rc;
   return rmsnorm_bwd_impl(fn, dy, x, weight, rstd, dresidual, dx, dweight, dweight_dtype, partial,
                           pico_rmsnorm_bwd_static_max_bytes(), rows, hidden, dtype, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int pico_rmsnorm_bwd_sums(const float* dy, int parts, const void* x, const void* weight, const float* rstd, const void* dresidual, void* dx, void* dweight, int dweight_dtype,
+                                     void* workspace, int64_t workspace_bytes, int64_t rows, int64_t hidden, void* stream) {
+  const char* fn = "pico_rmsnorm_bwd_sums";
+  if (int rc = check_common(fn, rows, hidden, PICO_BF16)) return rc;
+  if (parts < 1 || parts > 64) return fail(PICO_ERR_SHAPE, "%s: %d pieces (1 .. 64)", fn, parts);
+  if (dweight_dtype != PICO_BF16 && dweight_dtype != PICO_F32) return fail(PICO_ERR_DTYPE, "%s: dweight dtype code %d not supported", fn, dweight_dtype);
+  if (!dweight) return fail(PICO_ERR_NULL, "%s: dweight is required", fn);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (rows == 0) {
+    launch_dw_reduce(nullptr, dweight, dweight_dtype, 0, static_cast<int>(hidden), s);
+    return check_launch(fn);
+  }
+  if (!dy || !x || !weight || !rstd || !dx || !workspace) return fail(PICO_ERR_NULL, "%s: dy, x, weight, rstd, dx and the workspace are required", fn);
+  if (workspace_bytes < pico_rmsnorm_bwd_workspace_bytes(rows, hidden))
+    return fail(PICO_ERR_WORKSPACE, "%s: the workspace has %lld bytes, needs %lld", fn, static_cast<long long>(workspace_bytes), static_cast<long long>(pico_rmsnorm_bwd_workspace_bytes(rows, hidden)));
+  if (!aligned16(dy) || !aligned16(x) || !aligned16(weight) || !aligned16(dx) || !aligned16(workspace) || !aligned16(dresidual))
+    return fail(PICO_ERR_ALIGN, "%s: pointers must be 16-byte aligned", fn);
+  if (dx == x || dx == dresidual) return fail(PICO_ERR_NULL, "%s: dx cannot take an input's place", fn);
+  const int blocks = launch_bwd_sums(dy, parts, x, weight, rstd, dresidual, dx, static_cast<float*>(workspace), rows, static_cast<int>(hidden), s);
+  if (int rc = check_launch(fn)) return rc;
+  launch_dw_reduce(static_cast<float*>(workspace), dweight, dweight_dtype, blocks, static_cast<int>(hidden), s);
+  return check_launch(fn);
 }

@@ -66,8 +66,9 @@ extern "C" int pico_product_large_takes(int64_t M, int64_t N, int64_t K, int64_t
   return ((M + 127) / 128) * ((N + 127) / 128) * parts <= kMost / 256;
 }
 
-extern "C" int pico_product_large(const void* a, const void* b, void* c, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int a_slow,
-                                  int b_slow, int tile_m, int tile_n, int parts, void* stream) {
+namespace {
+int product_large(const void* a, const void* b, void* c, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int a_slow, int b_slow, int tile_m, int tile_n, int parts, bool sums,
+                  void* stream) {
   if (!pico_product_large_takes(M, N, K, lda, ldb, a_slow, b_slow, parts))
     return fail(PICO_ERR_SHAPE, "pico_product_large: M=%lld N=%lld K=%lld row pitches %lld, %lld, %d pieces (rows of a, b and c and the pitches must be multiples of 8 elements, two steps of 64 per piece, a tile's rows span less than 2 GiB, no a^T b^T)",
                 (long long)M, (long long)N, (long long)K, (long long)lda, (long long)ldb, parts);
@@ -75,7 +76,17 @@ extern "C" int pico_product_large(const void* a, const void* b, void* c, int64_t
   if (!aligned16(a) || !aligned16(b) || !aligned16(c)) return fail(PICO_ERR_ALIGN, "pico_product_large: pointers must be 16-byte aligned");
   const LargeParams p = {static_cast<const __bf16*>(a), static_cast<const __bf16*>(b), c, (int)M, (int)N, (int)K, lda, ldb, 0, 0, parts, false};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (a_slow) return parts > 1 ? launch_shape<true, true, true>(p, tile_m, tile_n, s) : launch_shape<true, true, false>(p, tile_m, tile_n, s);
-  if (b_slow) return parts > 1 ? launch_shape<false, true, true>(p, tile_m, tile_n, s) : launch_shape<false, true, false>(p, tile_m, tile_n, s);
-  return parts > 1 ? launch_shape<false, false, true>(p, tile_m, tile_n, s) : launch_shape<false, false, false>(p, tile_m, tile_n, s);
+  if (a_slow) return sums ? launch_shape<true, true, true>(p, tile_m, tile_n, s) : launch_shape<true, true, false>(p, tile_m, tile_n, s);
+  if (b_slow) return sums ? launch_shape<false, true, true>(p, tile_m, tile_n, s) : launch_shape<false, true, false>(p, tile_m, tile_n, s);
+  return sums ? launch_shape<false, false, true>(p, tile_m, tile_n, s) : launch_shape<false, false, false>(p, tile_m, tile_n, s);
+}
+}  // namespace
+
+extern "C" int pico_product_large(const void* a, const void* b, void* c, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int a_slow,
+                                  int b_slow, int tile_m, int tile_n, int parts, void* stream) {
+  return product_large(a, b, c, M, N, K, lda, ldb, a_slow, b_slow, tile_m, tile_n, parts, parts > 1, stream);
+}
+extern "C" int pico_product_large_sums(const void* a, const void* b, float* sums, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int a_slow,
+                                       int b_slow, int tile_m, int tile_n, int parts, void* stream) {
+  return product_large(a, b, sums, M, N, K, lda, ldb, a_slow, b_slow, tile_m, tile_n, parts, true, stream);
 }

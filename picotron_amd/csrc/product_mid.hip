@@ -315,8 +315,8 @@ extern "C" int pico_product_mid_takes(int64_t M, int64_t N, int64_t K, int64_t l
   return ((M + 31) / 32) * ((N + 31) / 32) <= kMost / 256;
 }
 
-extern "C" int pico_product_mid(const void* a, const void* b, void* c, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int a_slow,
-                                int b_slow, int tile_m, int tile_n, int parts, void* stream) {
+namespace {
+int product_mid(const void* a, const void* b, void* c, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int a_slow, int b_slow, int tile_m, int tile_n, int parts, bool sums, void* stream) {
   if (!pico_product_mid_takes(M, N, K, lda, ldb, a_slow, b_slow))
     return fail(PICO_ERR_SHAPE, "pico_product_mid: M=%lld N=%lld K=%lld row pitches %lld, %lld (rows of a, b and c and the pitches must be multiples of 8 elements, a tile's rows span less than 2 GiB, no a^T b^T)",
                 (long long)M, (long long)N, (long long)K, (long long)lda, (long long)ldb);
@@ -326,10 +326,20 @@ extern "C" int pico_product_mid(const void* a, const void* b, void* c, int64_t M
   if (parts < 1 || parts > 64 || (K + kStep - 1) / kStep < parts)
     return fail(PICO_ERR_SHAPE, "pico_product_mid: %d parts (1 .. 64, a step of 64 each)", parts);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (parts > 1)
+  if (sums)
     return a_slow ? launch_parts<true, true>(p, tile_m, tile_n, s) : b_slow ? launch_parts<false, true>(p, tile_m, tile_n, s) : launch_parts<false, false>(p, tile_m, tile_n, s);
   if (a_slow) return launch_form<true, true>(p, tile_m, tile_n, s);
   return b_slow ? launch_form<false, true>(p, tile_m, tile_n, s) : launch_form<false, false>(p, tile_m, tile_n, s);
+}
+}  // namespace
+
+extern "C" int pico_product_mid(const void* a, const void* b, void* c, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int a_slow,
+                                int b_slow, int tile_m, int tile_n, int parts, void* stream) {
+  return product_mid(a, b, c, M, N, K, lda, ldb, a_slow, b_slow, tile_m, tile_n, parts, parts > 1, stream);
+}
+extern "C" int pico_product_mid_sums(const void* a, const void* b, float* sums, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int a_slow,
+                                     int b_slow, int tile_m, int tile_n, int parts, void* stream) {
+  return product_mid(a, b, sums, M, N, K, lda, ldb, a_slow, b_slow, tile_m, tile_n, parts, true, stream);
 }
 
 extern "C" int pico_product_pair(const void* dy, const void* w, const void* x, void* dx, void* dw, int64_t rows, int64_t out, int64_t in,

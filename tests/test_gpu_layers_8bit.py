@@ -229,6 +229,52 @@ def test_swiglu_linear(device, M, N, K):
     assert torch.equal(torch.autograd.grad(alone, w, dy)[0], dw)
 
 
+# ------------------------------------------------------------------------------------------------- the norm's gradient from fp32 pieces
+@pytest.mark.parametrize("dw_dtype", [BF16, F32])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("rows,hidden,parts", [(1, 8, 1), (3, 96, 2), (33, 576, 1), (257, 2048, 3), (70, 4096, 1), (9, 4104, 2), (5, 8192, 1), (4, 16384, 2), (4500, 264, 1)])
+def test_norm_gradient_of_sums(device, rows, hidden, parts, residual, dw_dtype):
+    import ctypes
+    from picotron_amd import _lib
+    lib, g = _lib.lib(), gen(rows + hidden)
+    dy = torch.randn(parts, rows, hidden, generator=g, device="cuda")
+    x, gamma = randn(rows, hidden, g=g), (1 + 0.2 * torch.randn(hidden, generator=g, device="cuda")).to(BF16)
+    rstd = (x.double().pow(2).mean(-1) + EPS).rsqrt().float()
+    dres = randn(rows, hidden, g=g) if residual else None
+    dx, dw = torch.empty_like(x), torch.full((hidden + 8,), 3.0, dtype=dw_dtype, device="cuda")
+    ws = torch.empty(lib.pico_rmsnorm_bwd_workspace_bytes(rows, hidden), dtype=torch.uint8, device="cuda")
+    p = lambda t: ctypes.c_void_p(t.data_ptr()) if t is not None else None      # noqa: E731
+    _lib.check(lib.pico_rmsnorm_bwd_sums(p(dy), parts, p(x), p(gamma), p(rstd), p(dres), p(dx), p(dw), _lib.PICO_BF16 if dw_dtype == BF16 else _lib.PICO_F32, p(ws), ws.numel(), rows, hidden,
+                                         ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))
+    d, n, w = dy.double().sum(0), x.double() * rstd.double()[:, None], gamma.double()
+    q = d * w
+    want = rstd.double()[:, None] * (q - n * (q * n).mean(-1, keepdim=True)) + (dres.double() if residual else 0)
+    # sums of `rows` (dweight) and `hidden` (the row's mean) products in fp32, 64 side by side at least; one rounding to bf16
+    u = 2.0 ** -24
+    mean = rstd.double()[:, None] * n.abs() * (q * n).abs().mean(-1, keepdim=True)
+    slack = (hidden / 64 + 20) * u * mean + 16 * u * (rstd.double()[:, None] * q.abs() + want.abs() + (dres.double().abs() if residual else 0))
+    assert ((dx.double() - want).abs() <= E * want.abs() + slack).all()
+    want_w = (d * n).sum(0)
+    unit = E if dw_dtype == BF16 else 0.0
+    assert ((dw[:hidden].double() - want_w).abs() <= unit * want_w.abs() + (rows / 4 + 600) * u * (d * n).abs().sum(0) / max(1.0, rows ** 0.5) + 8 * u * (d * n).abs().sum(0)).all()
+    assert (dw[hidden:] == 3).all()
+
+
+@pytest.mark.parametrize("kind,M,N,K,tile,parts", [("mid", 33, 96, 64, (64, 96), 1), ("mid", 200, 136, 576, (64, 128), 3), ("mid", 130, 264, 1000, (96, 96), 1), ("mid", 500, 200, 320, (128, 128), 1),
+                                                   ("large", 300, 264, 512, (256, 256), 1), ("large", 300, 264, 512, (128, 256), 2)])
+def test_products_that_leave_their_sums(device, kind, M, N, K, tile, parts):
+    """fp32 sums of whole numbers are exact; nothing behind them is written."""
+    import ctypes
+    from picotron_amd import _lib
+    g = gen(M)
+    a, b = (torch.randint(-8, 9, s, generator=g, device="cuda").to(BF16) for s in ((M, K), (K, N)))
+    sums = torch.full((parts * M * N + 64,), 7.0, device="cuda")
+    p = lambda t: ctypes.c_void_p(t.data_ptr())      # noqa: E731
+    f = _lib.lib().pico_product_mid_sums if kind == "mid" else _lib.lib().pico_product_large_sums
+    _lib.check(f(p(a), p(b), p(sums), M, N, K, K, N, 0, 1, *tile, parts, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))
+    assert torch.equal(sums[:-64].view(parts, M, N).sum(0), a.float() @ b.float()) and (sums[-64:] == 7).all()
+
+
 # ------------------------------------------------------------------------------------------------- how they are called
 def layer(x, residual, gamma, gate_up_w, down_w):
     from picotron_amd import functional

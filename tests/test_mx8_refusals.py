@@ -83,6 +83,13 @@ def test_tiles_pieces_and_workspaces(lib):
         assert lib.pico_mx8_product(packed(), packed(), P, 512, 512, 65536, P, bytes_ - 1, None) == -6
 
 
+def test_the_norms_gradient_from_sums(lib):
+    def call(parts=1, hidden=64, dw=P, dw_dtype=0, dx=P, x=ctypes.c_void_p(BUF + 64), ws=P, bytes_=1 << 30, rows=4):
+        return lib.pico_rmsnorm_bwd_sums(P, parts, x, P, P, None, dx, dw, dw_dtype, ws, bytes_, rows, hidden, None)
+    assert call(hidden=12) == -3 and call(hidden=16384 + 8) == -3 and call(rows=-1) == -3 and call(parts=0) == -3 and call(parts=65) == -3
+    assert call(dw=None) == -1 and call(ws=None) == -1 and call(x=P) == -1 and call(dw_dtype=4) == -2 and call(bytes_=64) == -6 and call(dx=ctypes.c_void_p(BUF + 8)) == -4
+
+
 def test_nothing_to_do_is_no_error(lib):
     assert set(calls(lib, x=None, y8=packed(data=None), rows=0).values()) == {0}
     assert lib.pico_mx8_product(packed(data=None), packed(), None, 0, 4, 64, None, 0, None) == 0
