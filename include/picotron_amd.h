@@ -581,6 +581,10 @@ int pico_mx8_product(const pico_mx8* a, const pico_mx8* b, void* c, int64_t M, i
  * up) * 4 bytes), or, tile_m = 0, in form tile_n (0 .. 12) of the kernel of few rows.  What pico_mx8_product goes to by its rules. */
 int pico_mx8_product_tiled(const pico_mx8* a, const pico_mx8* b, void* c, int64_t M, int64_t N, int64_t K, int tile_m, int tile_n, int per_cu, int parts,
                            void* workspace, int64_t workspace_bytes, void* stream);
+/* c = x b^T for bf16 x [M, K] (row pitch x_ld, a multiple of 8) that is rounded to 8 bits on its way, without a launch of its own: to the bit what pico_mx8_quantize and
+ * pico_mx8_product give.  For the few rows for which .._pays gives 1 (16 at most), where it is the faster way. */
+int pico_mx8_product_rounding_pays(int64_t M, int64_t N, int64_t K);
+int pico_mx8_product_rounding(const void* x, const pico_mx8* b, void* c, int64_t M, int64_t N, int64_t K, int64_t x_ld, void* stream);
 
 /* ------------------------------------------------------------------ optimizer step
  * replaces: torch.optim.AdamW(model.parameters(), lr).step()  train.py:204-209,240  for low-precision parameters

@@ -131,6 +131,8 @@ SIGNATURES = {
     "pico_mx8_product_workspace_bytes": (_I64, [_I64] * 3),
     "pico_mx8_product": (c_int, [_MX8, _MX8, _P] + [_I64] * 3 + [_P, _I64, _P]),
     "pico_mx8_product_tiled": (c_int, [_MX8, _MX8, _P] + [_I64] * 3 + [c_int] * 4 + [_P, _I64, _P]),
+    "pico_mx8_product_rounding_pays": (c_int, [_I64] * 3),
+    "pico_mx8_product_rounding": (c_int, [_P, _MX8, _P] + [_I64] * 4 + [_P]),
     "pico_adamw": (c_int, [_P, _P, _P, c_int, _P, _P, _I64] + [ctypes.c_float] * 5 + [_I64, ctypes.c_float, _P]),
     "pico_adamw_lp": (c_int, [_P, _P, c_int, _P, _P, _I64, c_int, c_int] + [ctypes.c_float] * 5 + [_I64, ctypes.c_float, _P]),
     "pico_adamw_multi": (c_int, [c_int, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int] + [ctypes.c_float] * 5 + [_I64, ctypes.c_float, _P]),

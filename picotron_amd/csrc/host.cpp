@@ -1968,10 +1968,21 @@ struct Linear8 : torch::autograd::Function<Linear8> {
   static Tensor run(const Tensor& x, const Tensor& w, const OptMx8& packed, Held* kept) {
     TORCH_CHECK(x.dim() >= 1, fn, ": x must have an axis");
     check_weight(fn, x, x.size(-1), w);
+    check_columns(fn, x);
     const c10::OptionalDeviceGuard device(x.device());
+    Held made;
+    const int64_t M = mx8_rows_of(x), N = w.size(0), K = x.size(-1);
+    if (!kept && N % 8 == 0 && pico_mx8_product_rounding_pays(M, N, K)) {   // a few tokens, of which nothing is kept
+      const Mx8 b = packed_weight(fn, w, packed, made);
+      const Rows r = mx8_rows(x);
+      auto sizes = x.sizes().vec();
+      sizes.back() = N;
+      const Tensor y = at::empty(sizes, x.options());
+      check(pico_mx8_product_rounding(ptr(r.t), &b.c, ptr(y), M, N, K, r.pitch, stream_now()));
+      return y;
+    }
     const Held x8 = mx8_held(fn, x);
     if (kept) *kept = x8;
-    Held made;
     return mx8_product(x8.at(0), packed_weight(fn, w, packed, made), x);
   }
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptMx8& packed) {

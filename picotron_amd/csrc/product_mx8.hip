@@ -17,6 +17,8 @@ typedef __attribute__((ext_vector_type(8))) int i32x8;
 struct Mx8Params {
   const uint8_t *a, *b;        // [M, K], [N, K]
   const uint8_t *sa, *sb;      // their scales
+  const __bf16* x;             // or a before it is rounded to 8 bits, with its pitch
+  int64_t x_ld;
   __bf16* c;                   // [M, N rounded up to 8]
   int M, N, K;
 };
@@ -25,9 +27,39 @@ __device__ __forceinline__ i32x8 both(u32x4 low, u32x4 high) {
   return __builtin_bit_cast(i32x8, __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
+// 16 values of each half of a row's 128, rounded to 8 bits as mx8.h has it, and the scale of block h of the four: a block lies in two lanes 16 apart, its scale goes to the lanes
+// whose h it has.
+__device__ __forceinline__ i32x8 encode_fragment(const u32x4 (&raw)[2][2], int lane, int& scale) {
+  u32x4 code[2];
+  uint32_t byte[2];
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    float v[16];
+    uint32_t largest = 0;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const uint32_t pair = raw[half][e / 8][e % 8 / 2];
+      v[e] = __uint_as_float(e % 2 ? pair & 0xffff0000u : pair << 16);
+      largest = max(largest, __float_as_uint(v[e]) & 0x7fffffffu);
+    }
+    largest = max(largest, static_cast<uint32_t>(__shfl_xor(static_cast<int>(largest), 16, kWave)));
+    byte[half] = scale_byte(largest);
+    const float inverse = inverse_scale(byte[half]);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int low = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * w] * inverse, v[4 * w + 1] * inverse, 0, false);
+      code[half][w] = static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * w + 2] * inverse, v[4 * w + 3] * inverse, low, true));
+    }
+  }
+  const int from = lane % 16 + lane / 16 % 2 * 32, first = __shfl(static_cast<int>(byte[0]), from, kWave), second = __shfl(static_cast<int>(byte[1]), from, kWave);
+  scale = lane < 32 ? first : second;
+  return both(code[0], code[1]);
+}
+
 // ---- few rows: MT x NT tiles of 16 x 16 to a workgroup, whose W waves take every W-th 128 of the contraction straight from memory and join their sums in LDS.  Bound by the weight's
 // bytes, so what counts is how much is on its way: a wave requests U steps before it uses the first.
-template <int MT, int NT, int W, int U>
+// kRound: a is bf16 and every workgroup rounds it anew (MT 1): a launch less, 9.6 -> 7.5 us for [1 x 2048] @ [16384 x 2048]^T.
+template <int MT, int NT, int W, int U, bool kRound>
 __global__ __launch_bounds__(W * kWave) void product_mx8_few_kernel(const Mx8Params p) {
   Arguments<0>().arrive();
   __shared__ f32x4 sums[W][MT * NT][kWave];
@@ -46,7 +78,7 @@ __global__ __launch_bounds__(W * kWave) void product_mx8_few_kernel(const Mx8Par
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int t0 = wave; t0 < steps; t0 += U * W) {
-    u32x4 a[U][MT][2], b[U][NT][2];
+    u32x4 a[kRound ? 1 : U][MT][2], b[U][NT][2], x[kRound ? U : 1][2][2];
     int sa[U][MT], sb[U][NT];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -59,8 +91,16 @@ __global__ __launch_bounds__(W * kWave) void product_mx8_few_kernel(const Mx8Par
         b[u][j][1] = *reinterpret_cast<const u32x4*>(p.b + rb[j] * p.K + high);
         sb[u][j] = p.sb[(static_cast<int64_t>(t) * p.N + rb[j]) * 4 + h];
       }
+      if constexpr (kRound) {
+        const __bf16* row = p.x + ra[0] * p.x_ld;
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
+        for (int q = 0; q < 2; ++q) {
+          x[u][0][q] = *reinterpret_cast<const u32x4*>(row + low + 8 * q);
+          x[u][1][q] = *reinterpret_cast<const u32x4*>(row + high + 8 * q);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < (kRound ? 0 : MT); ++i) {
         a[u][i][0] = *reinterpret_cast<const u32x4*>(p.a + ra[i] * p.K + low);
         a[u][i][1] = *reinterpret_cast<const u32x4*>(p.a + ra[i] * p.K + high);
         sa[u][i] = p.sa[(static_cast<int64_t>(t) * p.M + ra[i]) * 4 + h];
@@ -75,10 +115,14 @@ __global__ __launch_bounds__(W * kWave) void product_mx8_few_kernel(const Mx8Par
 #pragma unroll
       for (int j = 0; j < NT; ++j) fb[j] = both(k < p.K ? b[u][j][0] : zero, k + 64 < p.K ? b[u][j][1] : zero);
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+      for (int i = 0; i < MT; ++i) {
+        i32x8 fa;
+        if constexpr (kRound) fa = encode_fragment(x[u], lane, sa[u][i]);   // (past the contraction: whatever its first values give, times b's zeros)
+        else fa = both(a[u][i][0], a[u][i][1]);
 #pragma unroll
         for (int j = 0; j < NT; ++j)   // C^T: a lane holds four columns of a row of C
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], both(a[u][i][0], a[u][i][1]), acc[i][j], 0, 0, 0, sb[u][j], 0, sa[u][i]);
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], fa, acc[i][j], 0, 0, 0, sb[u][j], 0, sa[u][i]);
+      }
     }
   }
 #pragma unroll
@@ -100,11 +144,11 @@ __global__ __launch_bounds__(W * kWave) void product_mx8_few_kernel(const Mx8Par
   }
 }
 
-template <int MT, int NT, int W, int U>
+template <int MT, int NT, int W, int U, bool kRound>
 int launch_few(const Mx8Params& p, hipStream_t s) {
   const int64_t tiles = ((p.N + INT64_C(16) * NT - 1) / (16 * NT)) * ((p.M + INT64_C(16) * MT - 1) / (16 * MT));
   if (tiles > 0x7fffffff) return fail(PICO_ERR_SHAPE, "pico_mx8_product: M=%d N=%d with K=%d has too many tiles", p.M, p.N, p.K);
-  hipLaunchKernelGGL((product_mx8_few_kernel<MT, NT, W, U>), dim3(static_cast<unsigned>(tiles)), dim3(W * kWave), 0, s, p);
+  hipLaunchKernelGGL((product_mx8_few_kernel<MT, NT, W, U, kRound>), dim3(static_cast<unsigned>(tiles)), dim3(W * kWave), 0, s, p);
   return check_launch("pico_mx8_product");
 }
 // What can be asked for: tiles of 16 x 16 to a workgroup, its waves, steps that a wave requests at once.
@@ -112,10 +156,12 @@ struct Few {
   int mt, nt, waves, ahead;
 };
 constexpr Few kFew[] = {{1, 1, 4, 2}, {1, 1, 8, 2}, {1, 1, 16, 2}, {1, 2, 4, 2}, {1, 2, 8, 2}, {1, 2, 16, 2}, {2, 1, 4, 2}, {2, 1, 8, 2}, {2, 1, 16, 2}, {2, 2, 4, 2}, {2, 2, 8, 2}, {2, 4, 4, 1}, {4, 2, 8, 1}};
-template <int... v>
+constexpr int kForms = static_cast<int>(std::size(kFew)), kRoundForms = 6;   // (the first ones have one tile of rows)
+static_assert(kFew[kRoundForms - 1].mt == 1 && kFew[kRoundForms].mt > 1);
+template <bool kRound, int... v>
 int dispatch_few(const Mx8Params& p, int form, hipStream_t s, std::integer_sequence<int, v...>) {
   int rc = PICO_ERR_SHAPE;
-  ((form == v ? static_cast<void>(rc = launch_few<kFew[v].mt, kFew[v].nt, kFew[v].waves, kFew[v].ahead>(p, s)) : void()), ...);
+  ((form == v ? static_cast<void>(rc = launch_few<kFew[v].mt, kFew[v].nt, kFew[v].waves, kFew[v].ahead, kRound>(p, s)) : void()), ...);
   return rc;
 }
 
@@ -449,27 +495,36 @@ struct Route {
 bool large_takes(int64_t M, int64_t N, int64_t K, int parts) {
   return parts >= 1 && parts <= 64 && (K + 127) / 128 >= 2 * parts && K <= (1 << 22) && ((M + 63) / 64) * ((N + 127) / 128) * parts <= 0x7fffffff / 256 && N <= 0x7fffffff / 256 && M <= 0x7fffffff / 2;
 }
-Route route(int64_t M, int64_t N, int64_t K) {
-  const int64_t steps = (K + 127) / 128, cols = (N + 7) / 8 * 8;
-  Route best = {0, 0, 1, 1};
-  float least = 1e30f;
-  for (int v = 0; v < static_cast<int>(std::size(kFew)); ++v) {
+// The form of the kernel of few rows, and its time.  `waves` not 0: of the forms that round, among those whose sums go over as many waves.
+int few_form(int64_t M, int64_t N, int64_t K, int waves, float& least) {
+  const bool rounding = waves != 0;
+  const int64_t steps = (K + 127) / 128;
+  int best = 0;
+  least = 1e30f;
+  for (int v = 0; v < (rounding ? kRoundForms : kForms); ++v) {
     const Few& f = kFew[v];
+    if (rounding && f.waves != waves) continue;
     const int64_t blocks = (M + 16 * f.mt - 1) / (16 * f.mt), tiles = blocks * ((N + 16 * f.nt - 1) / (16 * f.nt)), per_cu = (tiles + 255) / 256, turns = (steps + f.waves * f.ahead - 1) / (f.waves * f.ahead);
     const float rows = static_cast<float>(M) / (16 * blocks);   // (rows past the matrix cost no memory)
-    const float us = 2.f + std::max(0.066f * per_cu * steps * (f.nt + rows), 1.55e-7f * N * K) + 0.9f * (turns - 1) / per_cu;
+    const float a = rounding ? 1.5f * rows + 0.4f : rows;   // (bf16, and the rounding)
+    const float us = 2.f + std::max(0.066f * per_cu * steps * (f.nt + a), 1.55e-7f * N * K) + 0.9f * (turns - 1) / per_cu;
     if (us < least) {
       least = us;
-      best = {0, v, 1, 1};
+      best = v;
     }
   }
-  if (!large_takes(M, N, K, 1)) return best;
+  return best;
+}
+Route route(int64_t M, int64_t N, int64_t K, float& least) {
+  const int64_t steps = (K + 127) / 128, cols = (N + 7) / 8 * 8;
+  Route best = {0, few_form(M, N, K, 0, least), 1, 1};
+  if (M <= 8 || !large_takes(M, N, K, 1)) return best;
   for (const Tiling& t : kTilings)
     for (int parts = 1; parts <= 16 && large_takes(M, N, K, parts); parts *= 2) {
       const int64_t units = ((M + t.tile_m - 1) / t.tile_m) * ((N + t.tile_n - 1) / t.tile_n) * parts, slots = 256 * t.per_cu, rounds = (units + slots - 1) / slots;
       const float taken = static_cast<float>(units < slots ? units : slots) / slots, step = std::max(t.step, t.step_full * taken);
       float us = 3.5f + rounds * ((steps + parts - 1) / parts * step + t.end);
-      if (parts > 1) us += 2.f + (4.f * parts + 2.f) * M * cols * 2.5e-7f;   // (the sums again, at 4 TB/s)
+      if (parts > 1) us += 4.f + (4.f * parts + 2.f) * M * cols * 2.5e-7f;   // (the sums again, at 4 TB/s)
       if (us < least) {
         least = us;
         best = {t.tile_m, t.tile_n, t.per_cu, parts};
@@ -499,7 +554,8 @@ int64_t parts_bytes(int64_t M, int64_t N, int parts) { return parts > 1 ? parts 
 
 extern "C" int64_t pico_mx8_product_workspace_bytes(int64_t M, int64_t N, int64_t K) {
   if (M < 1 || N < 1 || K < 1) return 0;
-  return parts_bytes(M, N, route(M, N, K).parts);
+  float us;
+  return parts_bytes(M, N, route(M, N, K, us).parts);
 }
 
 extern "C" int pico_mx8_product_tiled(const pico_mx8* a, const pico_mx8* b, void* c, int64_t M, int64_t N, int64_t K, int tile_m, int tile_n, int per_cu, int parts, void* workspace,
@@ -508,12 +564,11 @@ extern "C" int pico_mx8_product_tiled(const pico_mx8* a, const pico_mx8* b, void
   if (int rc = check_product(fn, a, b, c, M, N, K)) return rc;
   if (M == 0 || N == 0) return PICO_OK;
   const Mx8Params p = {static_cast<const uint8_t*>(a->data), static_cast<const uint8_t*>(b->data), static_cast<const uint8_t*>(a->scales), static_cast<const uint8_t*>(b->scales),
-                       static_cast<__bf16*>(c), (int)M, (int)N, (int)K};
+                       nullptr, 0, static_cast<__bf16*>(c), (int)M, (int)N, (int)K};
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (tile_m == 0) {
-    constexpr int kForms = static_cast<int>(std::size(kFew));
     if (tile_n < 0 || tile_n >= kForms) return fail(PICO_ERR_SHAPE, "%s: no form %d of the kernel of few rows", fn, tile_n);
-    return dispatch_few(p, tile_n, s, std::make_integer_sequence<int, kForms>());
+    return dispatch_few<false>(p, tile_n, s, std::make_integer_sequence<int, kForms>());
   }
   if (!large_takes(M, N, K, parts))
     return fail(PICO_ERR_SHAPE, "%s: M=%lld N=%lld K=%lld in %d pieces (two steps of 128 a piece at least)", fn, (long long)M, (long long)N, (long long)K, parts);
@@ -528,6 +583,33 @@ extern "C" int pico_mx8_product_tiled(const pico_mx8* a, const pico_mx8* b, void
 extern "C" int pico_mx8_product(const pico_mx8* a, const pico_mx8* b, void* c, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream) {
   if (int rc = check_product("pico_mx8_product", a, b, c, M, N, K)) return rc;
   if (M == 0 || N == 0) return PICO_OK;
-  const Route r = route(M, N, K);
+  float us;
+  const Route r = route(M, N, K, us);
   return pico_mx8_product_tiled(a, b, c, M, N, K, r.tile_m, r.tile_n, r.per_cu, r.parts, workspace, workspace_bytes, stream);
+}
+
+namespace {
+// The form in which a's rounding costs less than a launch of its own, or -1.  It adds in the order of the form that pico_mx8_product goes to, so the results are the same to the bit.
+int rounding_form(int64_t M, int64_t N, int64_t K) {
+  float one, two;
+  const Route r = route(M, N, K, two);
+  if (M > 16 || r.tile_m != 0) return -1;
+  const int form = few_form(M, N, K, kFew[r.tile_n].waves, one);
+  return one < two + 2.f ? form : -1;
+}
+}  // namespace
+
+extern "C" int pico_mx8_product_rounding_pays(int64_t M, int64_t N, int64_t K) { return M >= 1 && N >= 1 && K >= 1 && rounding_form(M, N, K) >= 0; }
+
+extern "C" int pico_mx8_product_rounding(const void* x, const pico_mx8* b, void* c, int64_t M, int64_t N, int64_t K, int64_t x_ld, void* stream) {
+  const char* fn = "pico_mx8_product_rounding";
+  const pico_mx8 a = {const_cast<void*>(x), const_cast<void*>(x)};
+  if (int rc = check_product(fn, &a, b, c, M, N, K)) return rc;
+  if (M == 0 || N == 0) return PICO_OK;
+  if (x_ld < K) return fail(PICO_ERR_STRIDE, "%s: x has a row pitch under its columns", fn);
+  if (x_ld % 8 != 0) return fail(PICO_ERR_ALIGN, "%s: the row pitch of x must be a multiple of 8", fn);
+  Mx8Params p = {nullptr, static_cast<const uint8_t*>(b->data), nullptr, static_cast<const uint8_t*>(b->scales), static_cast<const __bf16*>(x), x_ld, static_cast<__bf16*>(c), (int)M, (int)N, (int)K};
+  const int form = rounding_form(M, N, K);
+  if (form < 0) return fail(PICO_ERR_SHAPE, "%s: M=%lld N=%lld K=%lld (sizes for which pico_mx8_product_rounding_pays)", fn, (long long)M, (long long)N, (long long)K);
+  return dispatch_few<true>(p, form, static_cast<hipStream_t>(stream), std::make_integer_sequence<int, kRoundForms>());
 }

@@ -276,6 +276,26 @@ def test_every_tile_of_the_product(device, M, N, K, parts, tile):
     assert torch.equal(got.float(), (x @ w.t()).to(BF16).float())      # (whole numbers of at most 36 K over 4: exact in fp32)
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 8, 32), (1, 2048, 2048), (2, 49, 96), (5, 1000, 160), (16, 64, 128), (7, 520, 1376), (16, 2100, 1024), (3, 17000, 288), (1, 2000, 4096), (1, 49152, 2048)])
+def test_product_that_rounds_on_its_way(device, M, N, K):
+    """What rounding and multiplying apart give, to the bit: rows with a pitch, infinities and NaN, zeros in the columns that round up."""
+    from picotron_amd import _lib, ops
+    lib, g = _lib.lib(), gen(M + N + K)
+    x, w = wide(M, K + 40, g, BF16), wide(N, K, g)
+    x[0, :32] = 0
+    if M > 2:
+        x[1, K - 1], x[2, 5] = float("nan"), float("inf")
+    b, ldc = ops.mx8_quantize(w), (N + 7) // 8 * 8
+    want = ops.mx8_product(ops.mx8_quantize(x[:, :K]), b)
+    buf = torch.full((M * ldc + 128,), 3.0, dtype=BF16, device="cuda")
+    cb = _lib.Mx8(b.data.data_ptr(), b.scales.data_ptr())
+    _lib.check(lib.pico_mx8_product_rounding(ctypes.c_void_p(x.data_ptr()), ctypes.byref(cb), ctypes.c_void_p(buf.data_ptr() + 128), M, N, K, K + 40, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))
+    c = buf[64:-64].view(M, ldc)
+    assert (buf[:64] == 3).all() and (buf[-64:] == 3).all() and (c[:, N:] == 0).all()
+    got = c[:, :N]
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got[~got.isnan()], want[~want.isnan()])
+
+
 def test_operands_that_do_not_fit(device):
     from picotron_amd import ops
     a, b = ops.mx8_quantize(torch.ones(4, 64, device="cuda")), ops.mx8_quantize(torch.ones(8, 96, device="cuda"))

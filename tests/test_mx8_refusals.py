@@ -83,6 +83,14 @@ def test_tiles_pieces_and_workspaces(lib):
         assert lib.pico_mx8_product(packed(), packed(), P, 512, 512, 65536, P, bytes_ - 1, None) == -6
 
 
+def test_the_product_that_rounds(lib):
+    def call(M=4, N=8, K=64, x=P, ld=64, c=P, b=None):
+        return lib.pico_mx8_product_rounding(x, b or packed(), c, M, N, K, ld, None)
+    assert call(M=17) == -3 and call(M=-1) == -3 and call(K=40, ld=40) == -3 and call(ld=56) == -5 and call(ld=68) == -4 and call(x=None) == -1 and call(c=None) == -1
+    assert call(x=ctypes.c_void_p(BUF + 8)) == -4 and call(b=packed(scales=None)) == -1 and call(M=0, x=None) == 0 and call(M=16, N=4096, K=11008, ld=11008) == -3
+    assert [lib.pico_mx8_product_rounding_pays(*s) for s in ((0, 64, 64), (17, 64, 64), (1, 0, 64), (1, 2048, 2048))] == [0, 0, 0, 1]
+
+
 def test_the_norms_gradient_from_sums(lib):
     def call(parts=1, hidden=64, dw=P, dw_dtype=0, dx=P, x=ctypes.c_void_p(BUF + 64), ws=P, bytes_=1 << 30, rows=4):
         return lib.pico_rmsnorm_bwd_sums(P, parts, x, P, P, None, dx, dw, dw_dtype, ws, bytes_, rows, hidden, None)
