@@ -39,7 +39,7 @@ def calls(lib, x=P, y8=None, rows=4, cols=64, ld=None, dtype=0):
 
 @pytest.mark.parametrize("over,code", [
     (dict(dtype=5), -2), (dict(cols=0), -3), (dict(cols=31), -3), (dict(cols=48), -3), (dict(rows=-1), -3), (dict(rows=1 << 31), -3),
-    (dict(rows=1 << 26, cols=4096 + 32), -3), (dict(x=None), -1), (dict(x=ctypes.c_void_p(BUF + 8)), -4)])
+    (dict(rows=1 << 26, cols=4096 + 32), -3), (dict(rows=1 << 27), -3), (dict(rows=1 << 27, dtype=1), -3), (dict(rows=1 << 20, cols=128 * 128), -3), (dict(x=None), -1), (dict(x=ctypes.c_void_p(BUF + 8)), -4)])
 def test_sizes_types_and_pointers(lib, over, code):
     assert set(calls(lib, **over).values()) == {code}, lib.pico_last_error()
 
@@ -63,6 +63,7 @@ def test_what_belongs_together(lib):
     assert lib.pico_swiglu_mx8_fwd(P, P, P, None, packed(), None, 4, 64, 64, 64, 0, None) == -1              # half a checkpoint
     assert lib.pico_rmsnorm_mx8_fwd(P, P, packed(), None, None, P, 4, 64, 1e-5, 0, None) == -1               # a sum without a residual
     assert lib.pico_rmsnorm_mx8_fwd(P, P, packed(), None, None, None, 4, 16384 + 32, 1e-5, 0, None) == -3
+    assert lib.pico_rmsnorm_mx8_fwd(P, P, packed(), None, None, None, 1 << 26, 64, 1e-5, 0, None) == -3     # threads of one launch
     assert lib.pico_rmsnorm_mx8_fwd(P, P, packed(), None, ctypes.c_void_p(BUF + 4), None, 4, 64, 1e-5, 0, None) == -4
 
 
@@ -70,6 +71,7 @@ def test_products(lib):
     def product(M=4, N=4, K=64, c=P):
         return lib.pico_mx8_product(packed(), packed(), c, M, N, K, None, 0, None)
     assert product(K=40) == -3 and product(K=0) == -3 and product(M=-1) == -3 and product(N=-1) == -3 and product(M=1 << 31) == -3
+    assert product(M=1 << 22, N=1 << 22) == -3                        # threads of one launch
     assert product(c=None) == -1 and product(c=ctypes.c_void_p(BUF + 8)) == -4
 
 
