@@ -20,6 +20,7 @@ Parity status of each oracle function (what pins it, see ``tests/test_oracle_*.p
 * ``layers.cross_entropy*``   pinned: ``F.cross_entropy`` (library), autograd
 * ``optim.adamw_step`` / ``master_step`` pinned: ``torch.optim.AdamW`` step by step
 * ``optim.lp_step``           pinned: torch's fused AdamW on bf16 parameters (rounding points of the stored values)
+* ``mx8.*``                    pinned: torch's cast to ``float8_e4m3fn``, the definition of the scale (``tests/test_mx8_refusals.py``)
 * ``model.OracleLlama`` / ``model.train_step``  pinned: transformers' ``LlamaForCausalLM`` with the same weights (logits,
                               loss, every gradient, one AdamW step), MHA and GQA, with and without the ring
                               (``tests/test_oracle_model.py``)
