@@ -271,6 +271,8 @@ bool one_pitch(const Tensor& t) {
   if (t.dim() == 0 || t.stride(-1) != 1) return false;
   for (int64_t i = t.dim() - 3; i >= 0; --i)
     if (t.size(i) != 1 && t.stride(i) != t.stride(i + 1) * t.size(i + 1)) return false;
+  for (int64_t i = t.dim() - 2; i >= 0; --i)   // rows that share memory (an expanded axis, the gradient of a sum) have no pitch that a kernel takes
+    if (t.size(i) != 1) return t.stride(i) >= t.size(-1);
   return true;
 }
 Rows as_rows(const Tensor& t_in) {
@@ -1757,13 +1759,8 @@ Rows mx8_rows(const Tensor& given) {
   const int64_t vec = 16 / t.element_size();
   if (one_pitch(t) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0) {
     const Rows r = as_rows(t);
-    bool whole = r.rows <= 1;   // (one row; else its pitch is a stride, and an expanded axis has none)
-    for (int64_t i = t.dim() - 2; i >= 0 && !whole; --i)
-      if (t.size(i) != 1) {
-        whole = t.stride(i) >= r.cols && t.stride(i) % vec == 0;
-        break;
-      }
-    if (whole) return r.rows <= 1 ? Rows{r.t, r.rows, r.cols, r.cols} : r;
+    if (r.rows <= 1) return {r.t, r.rows, r.cols, r.cols};
+    if (r.pitch % vec == 0) return r;
   }
   return as_rows(t.clone(at::MemoryFormat::Contiguous));
 }
