@@ -578,7 +578,7 @@ int pico_swiglu_mx8_bwd(const void* dy, const pico_mx8* gate8, const pico_mx8* u
 int64_t pico_mx8_product_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int pico_mx8_product(const pico_mx8* a, const pico_mx8* b, void* c, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
 /* The same in given tiles, 64 x 128 or each side 128 or 256, by per_cu workgroups to a CU (1; 2 for 128 x 128), the contraction in `parts` pieces of two steps of 128 at least (parts > 1: workspace of parts * M * (N rounded
- * up) * 4 bytes), or, tile_m = 0, in form tile_n (0 .. 12) of the kernel of few rows.  What pico_mx8_product goes to by its rules. */
+ * up) * 4 bytes), or, tile_m = 0, in form tile_n (0 .. 8; parts: 3 and 5) of the kernel of few rows.  What pico_mx8_product goes to by its rules. */
 int pico_mx8_product_tiled(const pico_mx8* a, const pico_mx8* b, void* c, int64_t M, int64_t N, int64_t K, int tile_m, int tile_n, int per_cu, int parts,
                            void* workspace, int64_t workspace_bytes, void* stream);
 /* c = x b^T for bf16 x [M, K] (row pitch x_ld, a multiple of 8) that is rounded to 8 bits on its way, without a launch of its own: to the bit what pico_mx8_quantize and

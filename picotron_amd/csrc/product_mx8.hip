@@ -6,7 +6,7 @@
 // the largest of the eight (measured: 2^16 + 2^3 is whole, 2^16 + 2^2 is 2^16), others are added with 24 bits: over normal values 1.5e-5 of the result's root mean square
 // (7e-5 with outliers of 20), without a bias and without growth from a contraction of 128 to one of 8192.  The rounding of the result to bf16 is 1.7e-3, so the result is bf16 only.
 //
-// What bounds it: few rows the weight's bytes, 1.03 of them a value and half of what bf16 takes ([1 x 2048] @ [16384 x 2048]^T 7.5 us, 4.6 TB/s, with its launch); many rows the matrix
+// What bounds it: few rows the weight's bytes, 1.03 of them a value and half of what bf16 takes ([1 x 2048] @ [16384 x 2048]^T 7.2 us, 4.8 TB/s, with its launch); many rows the matrix
 // pipe and the power that it draws: [16384 x 4096] @ [4096 x 4096]^T 213 us (2.6 PFLOP/s), where the pipe is busy 69 % of the time at a clock of 1.8 GHz (as the large products in bf16
 // are, at half the rate); [8192 x 8192] @ [8192 x 8192]^T 2.7, and 3.2 if all values are 0, which draw less.  A library's e4m3 product without block scales reaches 2.5 and 2.8.
 #include <iterator>
@@ -23,8 +23,8 @@ struct Mx8Params {
   const uint8_t *sa, *sb;      // their scales
   const __bf16* x;             // or a before it is rounded to 8 bits, with its pitch
   int64_t x_ld;
-  __bf16* c;                   // [M, N rounded up to 8]
-  int M, N, K;
+  void* c;                     // bf16 [M, N rounded up to 8]; fp32 [parts, M, N rounded up to 8] where the contraction goes in pieces
+  int M, N, K, parts;
 };
 
 __device__ __forceinline__ i32x8 both(u32x4 low, u32x4 high) {
@@ -60,17 +60,21 @@ __device__ __forceinline__ i32x8 encode_fragment(const u32x4 (&raw)[2][2], int l
   return both(code[0], code[1]);
 }
 
-// ---- few rows: MT x NT tiles of 16 x 16 to a workgroup, whose W waves take every W-th 128 of the contraction straight from memory and join their sums in LDS.  Bound by the weight's
-// bytes, so what counts is how much is on its way: a wave requests U steps before it uses the first.
-// kRound: a is bf16 and every workgroup rounds it anew (MT 1): a launch less, us for rounding and product by two launches and by one, [1 x 2048] @ [16384 x 2048]^T 9.5, 8.0;
-// [1 x 2048] @ [2048 x 2048]^T 6.7, 4.0; [1 x 11008] @ [4096 x 11008]^T 12.7, 13.5 (the same values rounded by 256 workgroups: rounding_form decides).
-template <int MT, int NT, int W, int U, bool kRound>
+// ---- few rows, and contractions under two steps: MT x NT tiles of 16 x 16 to a workgroup, whose W waves take every W-th 128 of the contraction straight from memory and join their sums in LDS.
+// Bound by the weight's bytes or, where the tiles are few and long, by what one CU takes, 25 to 35 bytes a ns however much is on its way (four steps requested ahead instead of two: the same).
+// A wave requests U steps before it uses the first.
+// kRound: a is bf16 and every workgroup rounds it anew (MT 1): a launch less, us for rounding and product by two launches and by one, [1 x 2048] @ [16384 x 2048]^T 9.2, 8.0;
+// [1 x 2048] @ [2048 x 2048]^T 7.1, 4.0; [1 x 11008] @ [4096 x 11008]^T 12.7, 13.5 (the same values rounded by 256 workgroups: rounding_form decides).
+// kParts: the contraction goes in pieces over workgroups that leave fp32 sums, with larger tiles: [24 x 8192] @ [2048 x 8192]^T 10.1 us by 256 tiles of 16 x 16, of which each reads 256 KB, 8.8 by
+// 64 tiles of 32 x 32 in four pieces, the sum's launch included.
+template <int MT, int NT, int W, int U, bool kRound, bool kParts>
 __global__ __launch_bounds__(W * kWave) void product_mx8_few_kernel(const Mx8Params p) {
   Arguments<0>().arrive();
   __shared__ f32x4 sums[W][MT * NT][kWave];
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), n = lane % 16, h = lane / 16;
-  const int across = (p.N + 16 * NT - 1) / (16 * NT), m0 = static_cast<int>(blockIdx.x) / across * 16 * MT, n0 = static_cast<int>(blockIdx.x) % across * 16 * NT;
-  const int steps = (p.K + kGroup - 1) / kGroup;
+  const int across = (p.N + 16 * NT - 1) / (16 * NT), tiles = across * ((p.M + 16 * MT - 1) / (16 * MT)), part = kParts ? static_cast<int>(blockIdx.x) / tiles : 0;
+  const int tile_of = static_cast<int>(blockIdx.x) - part * tiles, m0 = tile_of / across * 16 * MT, n0 = tile_of % across * 16 * NT;
+  const int steps = (p.K + kGroup - 1) / kGroup, first = kParts ? part * steps / p.parts : 0, end = kParts ? (part + 1) * steps / p.parts : steps;
   // rows past the matrix read its last one, and what they give is not written
   int64_t ra[MT], rb[NT];
 #pragma unroll
@@ -82,12 +86,12 @@ __global__ __launch_bounds__(W * kWave) void product_mx8_few_kernel(const Mx8Par
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int t0 = wave; t0 < steps; t0 += U * W) {
+  for (int t0 = first + wave; t0 < end; t0 += U * W) {
     u32x4 a[kRound ? 1 : U][MT][2], b[U][NT][2], x[kRound ? U : 1][2][2];
     int sa[U][MT], sb[U][NT];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      // pieces past the contraction read their row's first ones; b's are made 0 below (a's row is NaN as a whole or finite)
+      // pieces past the contraction read their row's first ones, steps past this piece of it the next one's; b's are made 0 below (a's row is NaN as a whole or finite)
       const int t = min(t0 + u * W, steps - 1), k = (t0 + u * W) * kGroup + 16 * h;
       const int64_t low = k < p.K ? k : 0, high = k + 64 < p.K ? k + 64 : 0;
 #pragma unroll
@@ -114,7 +118,7 @@ __global__ __launch_bounds__(W * kWave) void product_mx8_few_kernel(const Mx8Par
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int k = (t0 + u * W) * kGroup + 16 * h;
+      const int k = (t0 + u * W < end ? t0 + u * W : steps) * kGroup + 16 * h;
       const u32x4 zero = {0, 0, 0, 0};
       i32x8 fb[NT];
 #pragma unroll
@@ -142,31 +146,47 @@ __global__ __launch_bounds__(W * kWave) void product_mx8_few_kernel(const Mx8Par
     for (int w = 1; w < W; ++w) v += sums[w][tile][lane];
     const int row = m0 + 16 * (tile / NT) + n, col = n0 + 16 * (tile % NT) + 4 * h;
     if (row >= p.M || col >= ldc) continue;
-    bf16x4 o;   // (columns from N on are 0)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = static_cast<__bf16>(col + e < p.N ? v[e] : 0.f);
-    *reinterpret_cast<bf16x4*>(p.c + static_cast<int64_t>(row) * ldc + col) = o;
+    for (int e = 0; e < 4; ++e) v[e] = col + e < p.N ? v[e] : 0.f;
+    if constexpr (kParts) {
+      *reinterpret_cast<f32x4*>(static_cast<float*>(p.c) + (static_cast<int64_t>(part) * p.M + row) * ldc + col) = v;
+    } else {
+      bf16x4 o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = static_cast<__bf16>(v[e]);
+      *reinterpret_cast<bf16x4*>(static_cast<__bf16*>(p.c) + static_cast<int64_t>(row) * ldc + col) = o;
+    }
   }
 }
 
-template <int MT, int NT, int W, int U, bool kRound>
+template <int MT, int NT, int W, int U, bool kRound, bool kParts>
 int launch_few(const Mx8Params& p, hipStream_t s) {
-  const int64_t tiles = ((p.N + INT64_C(16) * NT - 1) / (16 * NT)) * ((p.M + INT64_C(16) * MT - 1) / (16 * MT));
+  const int64_t tiles = ((p.N + INT64_C(16) * NT - 1) / (16 * NT)) * ((p.M + INT64_C(16) * MT - 1) / (16 * MT)) * p.parts;
   if (tiles * W * kWave > 0xffffffff) return fail(PICO_ERR_SHAPE, "pico_mx8_product: M=%d N=%d with K=%d has too many tiles (a launch has under 2^32 threads)", p.M, p.N, p.K);
-  hipLaunchKernelGGL((product_mx8_few_kernel<MT, NT, W, U, kRound>), dim3(static_cast<unsigned>(tiles)), dim3(W * kWave), 0, s, p);
+  hipLaunchKernelGGL((product_mx8_few_kernel<MT, NT, W, U, kRound, kParts>), dim3(static_cast<unsigned>(tiles)), dim3(W * kWave), 0, s, p);
   return check_launch("pico_mx8_product");
 }
-// What can be asked for: tiles of 16 x 16 to a workgroup, its waves, steps that a wave requests at once.
+// What can be asked for: tiles of 16 x 16 to a workgroup, its waves, steps that a wave requests at once (of the forms that round, two), and whether the contraction can go in pieces.  us of the
+// best of the others and of each where it serves: 2048 columns and a contraction of 2048, 24 rows, 4.0 by the first, 4.6; [4096 x 4096], one row, 5.3 by the third (16 waves), 6.4;
+// [16384 x 1280], 16 rows, 6.4 by the fourth, 7.1; [16384 x 2048], 24 rows, 9.3 by {2, 4}, 9.8; [4096 x 128], 4096 rows, 20.5 by the last, 39.5 by eight waves.
 struct Few {
   int mt, nt, waves, ahead;
+  bool parts;
 };
-constexpr Few kFew[] = {{1, 1, 4, 2}, {1, 1, 8, 2}, {1, 1, 16, 2}, {1, 2, 4, 2}, {1, 2, 8, 2}, {1, 2, 16, 2}, {2, 1, 4, 2}, {2, 1, 8, 2}, {2, 1, 16, 2}, {2, 2, 4, 2}, {2, 2, 8, 2}, {2, 4, 4, 1}, {4, 2, 8, 1}};
-constexpr int kForms = static_cast<int>(std::size(kFew)), kRoundForms = 6;   // (the first ones have one tile of rows)
+constexpr Few kFew[] = {{1, 1, 4, 2, false}, {1, 1, 8, 2, false}, {1, 1, 16, 2, false}, {1, 2, 8, 1, true}, {2, 1, 8, 2, false}, {2, 2, 8, 2, true}, {2, 4, 8, 1, false}, {4, 4, 8, 1, false}, {4, 2, 2, 1, false}};
+constexpr int kForms = static_cast<int>(std::size(kFew)), kRoundForms = 4;   // (the first ones have one tile of rows)
 static_assert(kFew[kRoundForms - 1].mt == 1 && kFew[kRoundForms].mt > 1);
 template <bool kRound, int... v>
 int dispatch_few(const Mx8Params& p, int form, hipStream_t s, std::integer_sequence<int, v...>) {
   int rc = PICO_ERR_SHAPE;
-  ((form == v ? static_cast<void>(rc = launch_few<kFew[v].mt, kFew[v].nt, kFew[v].waves, kFew[v].ahead, kRound>(p, s)) : void()), ...);
+  auto launch = [&](auto of) {
+    constexpr Few f = kFew[decltype(of)::value];
+    if constexpr (f.parts && !kRound) {
+      if (p.parts > 1) return launch_few<f.mt, f.nt, f.waves, f.ahead, false, true>(p, s);
+    }
+    return launch_few<f.mt, f.nt, f.waves, kRound ? 2 : f.ahead, kRound, false>(p, s);
+  };
+  ((form == v ? static_cast<void>(rc = launch(std::integral_constant<int, v>())) : void()), ...);
   return rc;
 }
 
@@ -500,36 +520,46 @@ struct Route {
 bool large_takes(int64_t M, int64_t N, int64_t K, int parts) {
   return parts >= 1 && parts <= 64 && (K + 127) / 128 >= 2 * parts && K <= (1 << 22) && ((M + 63) / 64) * ((N + 127) / 128) * parts <= 0x7fffffff / 256 && N <= 0x7fffffff / 256 && M <= 0x7fffffff / 2;
 }
-// The form of the kernel of few rows, and its time.  `waves` not 0: of the forms that round, among those whose sums go over as many waves.
-int few_form(int64_t M, int64_t N, int64_t K, int waves, float& least) {
+// us that the sum of the pieces takes: a launch, and the sums again at 4 TB/s
+float join_us(int64_t M, int64_t N, int parts) { return parts > 1 ? 3.3f + 0.2f * parts + (4.f * parts + 2.f) * M * ((N + 7) / 8 * 8) * 2.5e-7f : 0.f; }
+// A form of the kernel of few rows, its pieces, and its time: the longer of what a CU takes from memory and the caches (about 25 bytes a ns) and the weight's bytes, and the waits for one
+// request after the other.
+struct FewRoute {
+  int form, parts;
+  float us;
+};
+// `waves` not 0: of the forms that round, among those whose sums go over as many waves
+FewRoute few_route(int64_t M, int64_t N, int64_t K, int waves) {
   const bool rounding = waves != 0;
-  const int64_t steps = (K + 127) / 128;
-  int best = 0;
-  least = 1e30f;
+  FewRoute best = {0, 1, 1e30f};
   for (int v = 0; v < (rounding ? kRoundForms : kForms); ++v) {
     const Few& f = kFew[v];
-    if (rounding && f.waves != waves) continue;
-    const int64_t blocks = (M + 16 * f.mt - 1) / (16 * f.mt), tiles = blocks * ((N + 16 * f.nt - 1) / (16 * f.nt)), per_cu = (tiles + 255) / 256, turns = (steps + f.waves * f.ahead - 1) / (f.waves * f.ahead);
-    const float rows = static_cast<float>(M) / (16 * blocks);   // (rows past the matrix cost no memory)
-    const float a = rounding ? 1.5f * rows + 0.4f : rows;   // (bf16, and the rounding)
-    const float us = 2.f + std::max(0.066f * per_cu * steps * (f.nt + a), 1.55e-7f * N * K) + 0.9f * (turns - 1) / per_cu;
-    if (us < least) {
-      least = us;
-      best = v;
+    if ((rounding && f.waves != waves) || (f.mt > 1 && M <= 8 * f.mt)) continue;   // (half a tile of rows would be empty)
+    const int ahead = rounding ? 2 : f.ahead;
+    for (int parts : {1, 4, 8}) {
+      const int64_t steps = ((K + 127) / 128 + parts - 1) / parts;
+      if (parts > 1 && (rounding || !f.parts || (K + 127) / 128 < parts)) break;
+      const int64_t blocks = (M + 16 * f.mt - 1) / (16 * f.mt), per_cu = (blocks * ((N + 16 * f.nt - 1) / (16 * f.nt)) * parts + 255) / 256, turns = (steps + f.waves * ahead - 1) / (f.waves * ahead);
+      const float rows = static_cast<float>(M) / (16 * blocks);   // (rows past the matrix cost no memory)
+      const float a = rounding ? 1.1f * rows + 0.18f : 0.7f * rows;   // (bf16, and the rounding)
+      const float asked = steps + 0.5f * (turns * f.waves * ahead - steps);   // (steps past the end are requested too)
+      const float us = 2.6f + std::max(0.09f * per_cu * asked * (f.nt + a), 1.3e-7f * N * K) + 0.17f * (turns - 1) / per_cu + join_us(M, N, parts);
+      if (us < best.us) best = {v, parts, us};
     }
   }
   return best;
 }
 Route route(int64_t M, int64_t N, int64_t K, float& least) {
-  const int64_t steps = (K + 127) / 128, cols = (N + 7) / 8 * 8;
-  Route best = {0, few_form(M, N, K, 0, least), 1, 1};
+  const int64_t steps = (K + 127) / 128;
+  const FewRoute few = few_route(M, N, K, 0);
+  Route best = {0, few.form, 1, few.parts};
+  least = few.us;
   if (M <= 8 || !large_takes(M, N, K, 1)) return best;
   for (const Tiling& t : kTilings)
     for (int parts = 1; parts <= 16 && large_takes(M, N, K, parts); parts *= 2) {
       const int64_t units = ((M + t.tile_m - 1) / t.tile_m) * ((N + t.tile_n - 1) / t.tile_n) * parts, slots = 256 * t.per_cu, rounds = (units + slots - 1) / slots;
       const float taken = static_cast<float>(units < slots ? units : slots) / slots, step = std::max(t.step, t.step_full * taken);
-      float us = 3.5f + rounds * ((steps + parts - 1) / parts * step + t.end);
-      if (parts > 1) us += 4.f + (4.f * parts + 2.f) * M * cols * 2.5e-7f;   // (the sums again, at 4 TB/s)
+      const float us = 5.4f + rounds * ((steps + parts - 1) / parts * step + t.end) + join_us(M, N, parts);
       if (us < least) {
         least = us;
         best = {t.tile_m, t.tile_n, t.per_cu, parts};
@@ -568,20 +598,26 @@ extern "C" int pico_mx8_product_tiled(const pico_mx8* a, const pico_mx8* b, void
   const char* fn = "pico_mx8_product";
   if (int rc = check_product(fn, a, b, c, M, N, K)) return rc;
   if (M == 0 || N == 0) return PICO_OK;
-  const Mx8Params p = {static_cast<const uint8_t*>(a->data), static_cast<const uint8_t*>(b->data), static_cast<const uint8_t*>(a->scales), static_cast<const uint8_t*>(b->scales),
-                       nullptr, 0, static_cast<__bf16*>(c), (int)M, (int)N, (int)K};
+  Mx8Params p = {static_cast<const uint8_t*>(a->data), static_cast<const uint8_t*>(b->data), static_cast<const uint8_t*>(a->scales), static_cast<const uint8_t*>(b->scales),
+                       nullptr, 0, c, (int)M, (int)N, (int)K, parts};
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (tile_m == 0) {
     if (tile_n < 0 || tile_n >= kForms) return fail(PICO_ERR_SHAPE, "%s: no form %d of the kernel of few rows", fn, tile_n);
-    return dispatch_few<false>(p, tile_n, s, std::make_integer_sequence<int, kForms>());
-  }
-  if (!large_takes(M, N, K, parts))
+    if (parts < 1 || parts > 64 || (parts > 1 && (!kFew[tile_n].parts || (K + 127) / 128 < parts)))
+      return fail(PICO_ERR_SHAPE, "%s: K=%lld in %d pieces by form %d of the kernel of few rows (a step of 128 a piece at least)", fn, (long long)K, parts, tile_n);
+  } else if (!large_takes(M, N, K, parts)) {
     return fail(PICO_ERR_SHAPE, "%s: M=%lld N=%lld K=%lld in %d pieces (two steps of 128 a piece at least)", fn, (long long)M, (long long)N, (long long)K, parts);
-  if (parts == 1) return launch_shape<false>(p, c, tile_m, tile_n, per_cu, 1, s);
-  if (!workspace || workspace_bytes < parts_bytes(M, N, parts))
-    return fail(PICO_ERR_WORKSPACE, "%s: the workspace has %lld bytes, needs %lld", fn, (long long)workspace_bytes, (long long)parts_bytes(M, N, parts));
-  if (!aligned16(workspace)) return fail(PICO_ERR_ALIGN, "%s: the workspace must be 16-byte aligned", fn);
-  if (int rc = launch_shape<true>(p, workspace, tile_m, tile_n, per_cu, parts, s)) return rc;
+  }
+  if (parts > 1) {
+    if (!workspace || workspace_bytes < parts_bytes(M, N, parts))
+      return fail(PICO_ERR_WORKSPACE, "%s: the workspace has %lld bytes, needs %lld", fn, (long long)workspace_bytes, (long long)parts_bytes(M, N, parts));
+    if (!aligned16(workspace)) return fail(PICO_ERR_ALIGN, "%s: the workspace must be 16-byte aligned", fn);
+    p.c = workspace;
+  }
+  int rc;
+  if (tile_m == 0) rc = dispatch_few<false>(p, tile_n, s, std::make_integer_sequence<int, kForms>());
+  else rc = parts > 1 ? launch_shape<true>(p, workspace, tile_m, tile_n, per_cu, parts, s) : launch_shape<false>(p, c, tile_m, tile_n, per_cu, 1, s);
+  if (rc || parts == 1) return rc;
   return pico_sum_parts(static_cast<const float*>(workspace), c, parts, M * ((N + 7) / 8 * 8), PICO_BF16, stream);
 }
 
@@ -596,11 +632,11 @@ extern "C" int pico_mx8_product(const pico_mx8* a, const pico_mx8* b, void* c, i
 namespace {
 // The form in which a's rounding costs less than a launch of its own, or -1.  It adds in the order of the form that pico_mx8_product goes to, so the results are the same to the bit.
 int rounding_form(int64_t M, int64_t N, int64_t K) {
-  float one, two;
+  float two;
   const Route r = route(M, N, K, two);
-  if (M > 16 || r.tile_m != 0) return -1;
-  const int form = few_form(M, N, K, kFew[r.tile_n].waves, one);
-  return one < two + 2.f ? form : -1;
+  if (M > 16 || r.tile_m != 0 || r.parts > 1) return -1;
+  const FewRoute one = few_route(M, N, K, kFew[r.tile_n].waves);
+  return one.us < two + 2.f ? one.form : -1;
 }
 }  // namespace
 
@@ -613,7 +649,7 @@ extern "C" int pico_mx8_product_rounding(const void* x, const pico_mx8* b, void*
   if (M == 0 || N == 0) return PICO_OK;
   if (x_ld < K) return fail(PICO_ERR_STRIDE, "%s: x has a row pitch under its columns", fn);
   if (x_ld % 8 != 0) return fail(PICO_ERR_ALIGN, "%s: the row pitch of x must be a multiple of 8", fn);
-  Mx8Params p = {nullptr, static_cast<const uint8_t*>(b->data), nullptr, static_cast<const uint8_t*>(b->scales), static_cast<const __bf16*>(x), x_ld, static_cast<__bf16*>(c), (int)M, (int)N, (int)K};
+  Mx8Params p = {nullptr, static_cast<const uint8_t*>(b->data), nullptr, static_cast<const uint8_t*>(b->scales), static_cast<const __bf16*>(x), x_ld, c, (int)M, (int)N, (int)K, 1};
   const int form = rounding_form(M, N, K);
   if (form < 0) return fail(PICO_ERR_SHAPE, "%s: M=%lld N=%lld K=%lld (sizes for which pico_mx8_product_rounding_pays)", fn, (long long)M, (long long)N, (long long)K);
   return dispatch_few<true>(p, form, static_cast<hipStream_t>(stream), std::make_integer_sequence<int, kRoundForms>());

@@ -261,8 +261,8 @@ def tiled(a, b, tile_m, tile_n, per_cu, parts):
 
 
 @pytest.mark.parametrize("M,N,K,parts", [(1, 1, 256, 1), (255, 257, 288, 1), (256, 512, 384, 1), (130, 1000, 544, 2), (700, 264, 2080, 3), (1, 8, 4096, 8), (520, 530, 1024, 4), (6000, 5000, 352, 1),
-                                         (3000, 2900, 1056, 4)])
-@pytest.mark.parametrize("tile", [(0, form, 1) for form in range(13)] + [(64, 128, 1), (128, 128, 1), (128, 128, 2), (128, 256, 1), (256, 128, 1), (256, 256, 1)])
+                                         (3000, 2900, 1056, 4), (24, 200, 1184, 4), (19, 36, 2080, 8), (33, 2048, 8192, 8)])
+@pytest.mark.parametrize("tile", [(0, form, 1) for form in range(9)] + [(64, 128, 1), (128, 128, 1), (128, 128, 2), (128, 256, 1), (256, 128, 1), (256, 256, 1)])
 def test_every_tile_of_the_product(device, M, N, K, parts, tile):
     """Exact sums, as above: more tiles than workgroups, fewer, cut at every side; contractions that end inside a step, in pieces of unequal lengths."""
     from picotron_amd import ops
@@ -272,7 +272,7 @@ def test_every_tile_of_the_product(device, M, N, K, parts, tile):
         v[..., 0] = 3
         return (v * torch.exp2(torch.randint(-1, 2, (n, K // 32, 1), generator=g, device="cuda").float())).view(n, K)
     x, w = rows(M), rows(N)
-    got = tiled(ops.mx8_quantize(x), ops.mx8_quantize(w), *tile, 1 if tile[0] == 0 else parts)
+    got = tiled(ops.mx8_quantize(x), ops.mx8_quantize(w), *tile, 1 if tile[0] == 0 and tile[1] not in (3, 5) else parts)      # (the forms of few rows that go in pieces)
     assert torch.equal(got.float(), (x @ w.t()).to(BF16).float())      # (whole numbers of at most 36 K over 4: exact in fp32)
 
 

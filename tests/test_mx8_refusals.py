@@ -78,7 +78,8 @@ def test_products(lib):
 def test_tiles_pieces_and_workspaces(lib):
     def tiled(tile_m=256, tile_n=256, per_cu=1, parts=1, ws=None, bytes_=0, K=1024):
         return lib.pico_mx8_product_tiled(packed(), packed(), P, 512, 512, K, tile_m, tile_n, per_cu, parts, ws, bytes_, None)
-    assert tiled(tile_m=64) == -3 and tiled(tile_n=192) == -3 and tiled(per_cu=2) == -3 and tiled(per_cu=0) == -3 and tiled(tile_m=0, tile_n=13) == -3 and tiled(tile_m=0, tile_n=-1) == -3 and tiled(parts=0) == -3 and tiled(parts=5) == -3 and tiled(parts=65, K=1 << 20) == -3 and tiled(K=128) == -3
+    assert tiled(tile_m=64) == -3 and tiled(tile_n=192) == -3 and tiled(per_cu=2) == -3 and tiled(per_cu=0) == -3 and tiled(tile_m=0, tile_n=9) == -3 and tiled(tile_m=0, tile_n=-1) == -3 and tiled(parts=0) == -3 and tiled(parts=5) == -3 and tiled(parts=65, K=1 << 20) == -3 and tiled(K=128) == -3
+    assert tiled(tile_m=0, tile_n=0, parts=2) == -3 and tiled(tile_m=0, tile_n=3, parts=9) == -3 and tiled(tile_m=0, tile_n=3, parts=0) == -3 and tiled(tile_m=0, tile_n=3, parts=2) == -6
     assert tiled(parts=2) == -6 and tiled(parts=2, ws=P, bytes_=2 * 512 * 512 * 4 - 1) == -6 and tiled(parts=2, ws=ctypes.c_void_p(BUF + 8), bytes_=1 << 30) == -4
     bytes_ = lib.pico_mx8_product_workspace_bytes(512, 512, 65536)
     if bytes_:
