@@ -3,7 +3,7 @@
 //
 // All of them are bound by memory; each value passes the registers once, and a block's largest value is found among the 4 (bf16) or 8
 // (fp32) lanes that hold it.  Measured in bf16, beside 5.1 - 5.4 TB/s of a large copy: rows [16384, 4096] made 37 us (5.5 TB/s), read back 33 (6.1);
-// RMSNorm with the residual [16384, 2048] 40 - 45 (5.2 - 5.8); SwiGLU [16384, 8192] with its checkpoint 183 (5.9), its gradient 185 (5.8).  More
+// RMSNorm with the residual [16384, 2048] 42 (5.6); SwiGLU [16384, 8192] with its checkpoint 183 (5.9), its gradient 185 (5.8).  More
 // groups to a thread, 16 values to a lane and loads past the caches all measured the same.
 #include "mx8.h"
 
@@ -128,28 +128,47 @@ __global__ __launch_bounds__(kThreads) void swiglu_mx8_bwd_kernel(const T* __res
 
 // ---- RMSNorm: y = (x + residual) rstd w in the 8-bit form only
 template <int G>
-__device__ __forceinline__ float group_sum(float v, float* smem) {
-  v = wave_sum(v);
+__device__ __forceinline__ double group_sum(double v, double* smem) {
+#pragma unroll
+  for (int off = kWave / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
   if constexpr (G == kWave) {
     return v;
   } else {
     if (threadIdx.x % kWave == 0) smem[threadIdx.x / kWave] = v;
     __syncthreads();
-    float t = 0.f;
+    double t = 0.;
 #pragma unroll
     for (int i = 0; i < G / kWave; ++i) t += smem[i];
     return t;
   }
 }
 
+// a + b less its rounding
+__device__ __forceinline__ float sum_left(float a, float b) {
+#pragma clang fp contract(off)
+  const float s = a + b, of_b = s - a;
+  return (a - (s - of_b)) + (b - of_b);
+}
+// Whether what this fp32 value stands for, up to 4 of its last places away (three roundings, and that of h in fp32), may lie in the middle of two codes: its last 19 bits are 0 there.
+__device__ __forceinline__ bool may_be_a_middle(float v) { return (__float_as_uint(v) << 13) + (4u << 13) <= 8u << 13; }
+// (v + low) (r + left) w, its last bit 1 where fp32 does not hold it: no such value lies in the middle of two codes
+__device__ __forceinline__ float scaled(float v, float low, float r, float left, float w) {
+#pragma clang fp contract(off)
+  const float n = v * r, n_left = fmaf(low, r, fmaf(v, left, fmaf(v, r, -n))), y = n * w, y_left = fmaf(n_left, w, fmaf(n, w, -y)), s = y + y_left, s_left = y_left - (s - y);
+  const int bits = __float_as_int(s), away = ((__float_as_int(s_left) ^ bits) >> 31) | 1;
+  return __int_as_float(fabsf(s_left) > 0.f && bits % 2 == 0 ? bits + away : bits);
+}
+
 // A row to a wave (G 64) or to the workgroup (G 256), NV pieces of 16 bytes to a thread, which stay in registers between the sum of squares and the
-// output.
+// output.  A value in the middle of two codes, or nearly so, takes the other one by an error of 2^-24: the row's sum goes over the lanes in 64 bits, and pieces with such a value are made anew
+// with what the roundings leave.  Of 16 M values 1 then differs from the exact one's code, plainly 12; that costs 4 % ([16384, 2048] 40 -> 42 us).
 template <typename T, int G, int NV>
 __global__ __launch_bounds__(kThreads) void rmsnorm_mx8_kernel(const T* __restrict__ x, const T* __restrict__ w, const pico_mx8 y, float* __restrict__ rstd,
-                                                               const T* __restrict__ res_in, T* __restrict__ res_out, int64_t rows, int hidden, float eps) {
+                                                               const T* __restrict__ res_in, T* __restrict__ res_out, int64_t rows, int hidden, float eps, double inv_hidden) {
   Arguments<0, 64>().arrive();
   constexpr int V = io<T>::kVec;
-  __shared__ float smem[kThreads / kWave];
+  constexpr bool kLow = std::is_same_v<T, float>;
+  __shared__ double smem[kThreads / kWave];
   const int t = threadIdx.x % G, nvec = hidden / V;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / G) + threadIdx.x / G;
   if (row >= rows) return;   // (G 256: uniform over the workgroup, which meets at a barrier below)
@@ -169,26 +188,41 @@ __global__ __launch_bounds__(kThreads) void rmsnorm_mx8_kernel(const T* __restri
     for (int j = 0; j < NV; ++j) w_raw[j] = *reinterpret_cast<const u32x4*>(w + piece(j));
     __builtin_amdgcn_sched_barrier(0);
   }
-  float vals[NV][V], ss = 0.f;
+  float vals[NV][V], low[kLow ? NV : 1][V];   // (the second: what a sum in fp32 leaves)
+  double ss = 0.;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     if constexpr (kEarly) io<T>::load(&x_raw[j], vals[j]);
     else io<T>::load(x + at + piece(j), vals[j]);
+    if constexpr (kLow) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) low[j][e] = 0.f;
+    }
     if (res_in != nullptr) {
       float r[V];
       if constexpr (kEarly) io<T>::load(&r_raw[j], r);
       else io<T>::load(res_in + at + piece(j), r);
 #pragma unroll
-      for (int e = 0; e < V; ++e) vals[j][e] += r[e];
+      for (int e = 0; e < V; ++e) {
+        if constexpr (kLow) low[j][e] = sum_left(vals[j][e], r[e]);
+        vals[j][e] += r[e];
+      }
       if (res_out != nullptr && t + j * G < nvec) store_as<T, true>(res_out + at + piece(j), vals[j]);
     }
     if (t + j * G < nvec) {
+      float piece_ss = 0.f;
 #pragma unroll
-      for (int e = 0; e < V; ++e) ss += vals[j][e] * vals[j][e];
+      for (int e = 0; e < V; ++e) piece_ss += vals[j][e] * vals[j][e];
+      ss += piece_ss;
     }
   }
-  ss = group_sum<G>(ss, smem);
-  const float r = rsqrtf(ss / static_cast<float>(hidden) + eps);
+  const double mean = group_sum<G>(ss, smem) * inv_hidden + eps;
+  float r = rsqrtf(static_cast<float>(mean)), left = 0.f;
+  if (r > 0.f && r < __builtin_huge_valf()) {   // (0: a row with an infinity)
+    const double whole = r + 0.5 * r * (1. - mean * r * r);
+    r = static_cast<float>(whole);
+    left = static_cast<float>(whole - r);
+  }
   if (rstd != nullptr && t == 0) rstd[row] = r;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
@@ -199,6 +233,13 @@ __global__ __launch_bounds__(kThreads) void rmsnorm_mx8_kernel(const T* __restri
     else io<T>::load(w + piece(j), wv);
 #pragma unroll
     for (int e = 0; e < V; ++e) o[e] = v < nvec ? vals[j][e] * r * wv[e] : 0.f;
+    bool near = false;
+#pragma unroll
+    for (int e = 0; e < V; ++e) near |= may_be_a_middle(o[e]);
+    if (__any(near && v < nvec)) {   // (one in a hundred, or two, of a wave's pieces)
+#pragma unroll
+      for (int e = 0; e < V; ++e) o[e] = v < nvec ? scaled(vals[j][e], kLow ? low[j][e] : 0.f, r, left, wv[e]) : 0.f;
+    }
     const Codes<V> c = encode<V>(o);
     const uint32_t scales = four_scales<V>(c.scale, t);
     if (v < nvec) {
@@ -212,7 +253,7 @@ template <typename T, int G, int NV>
 void launch_norm(const void* x, const void* w, const pico_mx8& y, float* rstd, const void* ri, void* ro, int64_t rows, int hidden, float eps, hipStream_t s) {
   constexpr int kRows = kThreads / G;
   hipLaunchKernelGGL((rmsnorm_mx8_kernel<T, G, NV>), dim3(static_cast<unsigned>((rows + kRows - 1) / kRows)), dim3(kThreads), 0, s, static_cast<const T*>(x),
-                     static_cast<const T*>(w), y, rstd, static_cast<const T*>(ri), static_cast<T*>(ro), rows, hidden, eps);
+                     static_cast<const T*>(w), y, rstd, static_cast<const T*>(ri), static_cast<T*>(ro), rows, hidden, eps, 1. / hidden);
 }
 template <typename T>
 void dispatch_norm(const void* x, const void* w, const pico_mx8& y, float* rstd, const void* ri, void* ro, int64_t rows, int hidden, float eps, hipStream_t s) {

@@ -151,6 +151,22 @@ def test_norm(device, rows, cols, residual, dtype):
     assert (O.exponents_of(packed.scales, cols) != e).sum().item() <= 2
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,cols", [(4096, 1024), (900, 4128)])
+def test_norm_rounds_the_exact_value(device, rows, cols, dtype):
+    """Whole numbers, whose squares add up exactly in any order: 1 / rms and the products are off by less than 2^-44, so every code is the exact value's, also beside the middle of two
+    (fp32 alone takes the other one for about one in a million)."""
+    from picotron_amd import ops
+    g = gen(cols)
+    x, res = (torch.randint(-7, 8, (rows, cols), generator=g, device="cuda").to(dtype) for _ in range(2))
+    w = (1 + 0.3 * torch.randn(cols, generator=g, device="cuda")).to(dtype)
+    packed, _, _ = ops.rmsnorm_mx8_fwd(x, w, 1e-5, residual=res)
+    h = x.double() + res.double()
+    eps = torch.tensor(1e-5, dtype=F32).double().item()
+    q, e = O.quantize(h * (h.pow(2).mean(-1, keepdim=True) + eps).rsqrt() * w.double())
+    assert torch.equal(O.exponents_of(packed.scales, cols), e) and torch.equal(packed.dequantize(F32).double(), q)
+
+
 def test_norm_rows_of_zeros_infinities_and_far_scales(device):
     from picotron_amd import ops
     x = torch.randn(6, 256, device="cuda")
