@@ -559,12 +559,13 @@ int pico_mx8_quantize(const void* x, const pico_mx8* y, int64_t rows, int64_t co
 /* The values that x stands for, in `dtype` (both hold them exactly from 2^-126 on; what was rounded up to 2^128 is infinite), with row pitch y_ld. */
 int pico_mx8_dequantize(const pico_mx8* x, void* y, int64_t rows, int64_t cols, int64_t y_ld, int dtype, void* stream);
 /* pico_rmsnorm_fwd (cast_then_scale = 0) whose output is written in 8 bits, from fp32, and in no other form: y [rows, hidden], hidden a multiple of 32
- * up to 16384.  The backward is pico_rmsnorm_bwd, with the gradient of the values that y stands for. */
+ * up to 16384.  The backward is pico_rmsnorm_bwd, with the gradient of the values that y stands for.  residual_left (bf16, may be NULL): what the rounding of
+ * residual_out leaves, [rows, hidden / 8] words of eight times four bits, sixteenths of the last place, -8 .. 7, the first value's lowest. */
 int pico_rmsnorm_mx8_fwd(const void* x, const void* weight, const pico_mx8* y, float* rstd, const void* residual_in, void* residual_out,
-                         int64_t rows, int64_t hidden, float eps, int dtype, void* stream);
+                         void* residual_left, int64_t rows, int64_t hidden, float eps, int dtype, void* stream);
 /* pico_rmsnorm_bwd for a gradient that a product left in fp32, in `parts` (1 .. 64) pieces to be added: dy [parts, rows, hidden]; x, weight, dresidual (may be NULL) and dx
- * bf16, dx in no input's place.  workspace: pico_rmsnorm_bwd_workspace_bytes bytes. */
-int pico_rmsnorm_bwd_sums(const float* dy, int parts, const void* x, const void* weight, const float* rstd, const void* dresidual, void* dx,
+ * bf16, dx in no input's place; x_left (may be NULL): residual_left of the x that pico_rmsnorm_mx8_fwd left.  workspace: pico_rmsnorm_bwd_workspace_bytes bytes. */
+int pico_rmsnorm_bwd_sums(const float* dy, int parts, const void* x, const void* x_left, const void* weight, const float* rstd, const void* dresidual, void* dx,
                           void* dweight, int dweight_dtype, void* workspace, int64_t workspace_bytes, int64_t rows, int64_t hidden, void* stream);
 /* silu(gate) * up into y (contiguous, `dtype`), y8, or both; gate8 and up8 (both or neither) take what pico_swiglu_mx8_bwd reads. */
 int pico_swiglu_mx8_fwd(const void* gate, const void* up, void* y, const pico_mx8* y8, const pico_mx8* gate8, const pico_mx8* up8,

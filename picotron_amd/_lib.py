@@ -122,10 +122,10 @@ SIGNATURES = {
     "pico_linear_log_probs_dlogits": (c_int, [_P] * 6 + [_I64] * 6 + [c_float, _I64, _P, _I64, _P]),
     "pico_product_large_sums": (c_int, [_P, _P, _P] + [_I64] * 5 + [c_int] * 5 + [_P]),
     "pico_product_mid_sums": (c_int, [_P, _P, _P] + [_I64] * 5 + [c_int] * 5 + [_P]),
-    "pico_rmsnorm_bwd_sums": (c_int, [_P, c_int] + [_P] * 6 + [c_int, _P, _I64, _I64, _I64, _P]),
+    "pico_rmsnorm_bwd_sums": (c_int, [_P, c_int] + [_P] * 7 + [c_int, _P, _I64, _I64, _I64, _P]),
     "pico_mx8_quantize": (c_int, [_P, _MX8, _I64, _I64, _I64, c_int, _P]),
     "pico_mx8_dequantize": (c_int, [_MX8, _P, _I64, _I64, _I64, c_int, _P]),
-    "pico_rmsnorm_mx8_fwd": (c_int, [_P, _P, _MX8, _P, _P, _P, _I64, _I64, c_float, c_int, _P]),
+    "pico_rmsnorm_mx8_fwd": (c_int, [_P, _P, _MX8, _P, _P, _P, _P, _I64, _I64, c_float, c_int, _P]),
     "pico_swiglu_mx8_fwd": (c_int, [_P, _P, _P, _MX8, _MX8, _MX8] + [_I64] * 4 + [c_int, _P]),
     "pico_swiglu_mx8_bwd": (c_int, [_P, _MX8, _MX8, _P, _P, _P] + [_I64] * 5 + [c_int, _P]),
     "pico_mx8_product_workspace_bytes": (_I64, [_I64] * 3),

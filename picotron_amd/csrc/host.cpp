@@ -1803,10 +1803,10 @@ Tensor mx8_product(const Mx8& a, const Mx8& b, const Tensor& like) {
 }
 
 struct NormMx8Out {
-  Tensor rstd, sum;
+  Tensor rstd, sum, left;
 };
 // rmsnorm(x + residual) * weight into y, [rows, hidden] as x; the caller has set the device
-NormMx8Out rmsnorm_mx8(const char* fn, const Tensor& x, const Tensor& weight, double eps, const OptTensor& residual, bool want_rstd, const Mx8& y) {
+NormMx8Out rmsnorm_mx8(const char* fn, const Tensor& x, const Tensor& weight, double eps, const OptTensor& residual, bool want_rstd, bool want_left, const Mx8& y) {
   const int dt = dtype_code(x, fn);
   const int64_t hidden = x.size(-1);
   TORCH_CHECK(weight.dim() == 1 && weight.size(0) == hidden && weight.device() == x.device(), fn, ": the norm's weight must be [", hidden, "] on ", x.device(), " (got ", weight.sizes(), " on ",
@@ -1819,8 +1819,9 @@ NormMx8Out rmsnorm_mx8(const char* fn, const Tensor& x, const Tensor& weight, do
   }
   NormMx8Out o;
   if (want_rstd) o.rstd = at::empty({y.rows}, xc.options().dtype(at::kFloat));
+  if (want_left && res.defined()) o.left = at::empty({y.rows, hidden / 8}, xc.options().dtype(at::kInt));
   if (res.defined()) o.sum = at::empty(xc.sizes(), xc.options());
-  check(pico_rmsnorm_mx8_fwd(ptr(xc), ptr(w), &y.c, fptr(o.rstd), ptr(res), ptr(o.sum), y.rows, hidden, static_cast<float>(eps), dt, stream_now()));
+  check(pico_rmsnorm_mx8_fwd(ptr(xc), ptr(w), &y.c, fptr(o.rstd), ptr(res), ptr(o.sum), ptr(o.left), y.rows, hidden, static_cast<float>(eps), dt, stream_now()));
   return o;
 }
 
@@ -1937,13 +1938,13 @@ Sums input_sums(const Tensor& dy, const Tensor& w) {
   return s;
 }
 // The gradients of a norm [rows, hidden] in front of a weight, from that of the product, all bf16.
-std::pair<Tensor, Tensor> norm_gradients(const Tensor& dy, const Tensor& w, const Tensor& x, const Tensor& norm_weight, const Tensor& rstd, const OptTensor& dresidual) {
+std::pair<Tensor, Tensor> norm_gradients(const Tensor& dy, const Tensor& w, const Tensor& x, const Tensor& left, const Tensor& norm_weight, const Tensor& rstd, const OptTensor& dresidual) {
   const Sums s = input_sums(dy, w);
   if (s.parts == 0) return rmsnorm_backward(product(dy, w, Product::NN).view(x.sizes()), x, norm_weight, rstd, dresidual, norm_weight.scalar_type());
   const int64_t hidden = x.size(-1), rows = dy.size(0), bytes = pico_rmsnorm_bwd_workspace_bytes(rows, hidden);
   const Tensor weight = norm_weight.to(at::kBFloat16), dres = dresidual ? dresidual->to(at::kBFloat16) : Tensor();
   const Tensor dx = at::empty(x.sizes(), x.options()), dw = at::empty({hidden}, norm_weight.options()), ws = at::empty({bytes}, x.options().dtype(at::kByte));
-  check(pico_rmsnorm_bwd_sums(fptr(s.t), s.parts, ptr(x), ptr(weight), fptr(rstd), ptr(dres), ptr(dx), ptr(dw), dtype_code(dw, "rms_norm_linear_8bit: norm_weight"), ptr(ws), bytes, rows, hidden,
+  check(pico_rmsnorm_bwd_sums(fptr(s.t), s.parts, ptr(x), ptr(left), ptr(weight), fptr(rstd), ptr(dres), ptr(dx), ptr(dw), dtype_code(dw, "rms_norm_linear_8bit: norm_weight"), ptr(ws), bytes, rows, hidden,
                               stream_now()));
   return {dx, dw};
 }
@@ -2023,7 +2024,7 @@ struct NormLinear8 : torch::autograd::Function<NormLinear8> {
     check_columns(fn, x);
     const c10::OptionalDeviceGuard device(x.device());
     const Held y8 = held(mx8_rows_of(x), x.size(-1), 1, x);
-    const NormMx8Out norm = rmsnorm_mx8(fn, x, norm_weight, eps, residual, kept != nullptr, y8.at(0));
+    const NormMx8Out norm = rmsnorm_mx8(fn, x, norm_weight, eps, residual, kept != nullptr, kept != nullptr, y8.at(0));
     if (kept) *kept = {y8, norm};
     Held made;
     return {mx8_product(y8.at(0), packed_weight(fn, w, packed, made), x), residual ? norm.sum : x};
@@ -2035,7 +2036,7 @@ struct NormLinear8 : torch::autograd::Function<NormLinear8> {
     variable_list out = run(x, residual, norm_weight, eps, w, packed, &kept);
     bool keep = w.requires_grad();
     for (const Tensor& p : parts) keep |= p.requires_grad();
-    ctx->save_for_backward({residual ? out[1] : x, norm_weight, kept.norm.rstd, w, keep ? kept.y.bytes : Tensor()});
+    ctx->save_for_backward({residual ? out[1] : x, norm_weight, kept.norm.rstd, w, keep ? kept.y.bytes : Tensor(), kept.norm.left});
     ctx->saved_data["residual"] = residual.has_value();
     ctx->set_materialize_grads(false);   // (the stream's h may have no other reader)
     return out;
@@ -2057,7 +2058,7 @@ struct NormLinear8 : torch::autograd::Function<NormLinear8> {
     const Tensor dy = upstream(g[0]);
     if (wants_norm) {
       const Rounded whole = rounded_up(dy, weight_rows(s[3]));
-      auto [dx, dgamma] = norm_gradients(whole.dy, whole.w, mx8_dense(s[0]), mx8_dense(s[1]), s[2], g[1].defined() ? OptTensor(mx8_dense(g[1])) : std::nullopt);
+      auto [dx, dgamma] = norm_gradients(whole.dy, whole.w, mx8_dense(s[0]), s[5], mx8_dense(s[1]), s[2], g[1].defined() ? OptTensor(mx8_dense(g[1])) : std::nullopt);
       r[0] = dx;
       if (has_residual) r[1] = dx;
       r[2] = dgamma;
@@ -2360,7 +2361,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     check_columns("rmsnorm_mx8_fwd", x);
     const c10::OptionalDeviceGuard device(x.device());
     const Mx8Pair y = mx8_empty(x.sizes(), mx8_rows_of(x), x);
-    NormMx8Out o = rmsnorm_mx8("rmsnorm_mx8_fwd", x, w, eps, residual, true, mx8_of(y));
+    NormMx8Out o = rmsnorm_mx8("rmsnorm_mx8_fwd", x, w, eps, residual, true, false, mx8_of(y));
     return std::make_tuple(y.first, y.second, o.rstd, o.sum.defined() ? OptTensor(o.sum) : std::nullopt);
   }, nogil());
   m.def("linear_8bit", &linear_8bit, nogil());

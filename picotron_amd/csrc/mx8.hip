@@ -159,12 +159,23 @@ __device__ __forceinline__ float scaled(float v, float low, float r, float left,
   return __int_as_float(fabsf(s_left) > 0.f && bits % 2 == 0 ? bits + away : bits);
 }
 
+// What eight values' roundings to bf16 leave, in four bits each: sixteenths of bf16's last place, -8 .. 7.
+__device__ __forceinline__ uint32_t bf16_left(const float (&v)[8]) {
+  uint32_t word = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t bits = __float_as_uint(v[e]), held = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<__bf16>(v[e]))) << 16;
+    word |= static_cast<uint32_t>(min((static_cast<int>(bits - held) + 2048) >> 12, 7) & 15) << (4 * e);
+  }
+  return word;
+}
+
 // A row to a wave (G 64) or to the workgroup (G 256), NV pieces of 16 bytes to a thread, which stay in registers between the sum of squares and the
 // output.  A value in the middle of two codes, or nearly so, takes the other one by an error of 2^-24: the row's sum goes over the lanes in 64 bits, and pieces with such a value are made anew
 // with what the roundings leave.  Of 16 M values 1 then differs from the exact one's code, plainly 12; that costs 4 % ([16384, 2048] 40 -> 42 us).
 template <typename T, int G, int NV>
 __global__ __launch_bounds__(kThreads) void rmsnorm_mx8_kernel(const T* __restrict__ x, const T* __restrict__ w, const pico_mx8 y, float* __restrict__ rstd,
-                                                               const T* __restrict__ res_in, T* __restrict__ res_out, int64_t rows, int hidden, float eps, double inv_hidden) {
+                                                               const T* __restrict__ res_in, T* __restrict__ res_out, uint32_t* __restrict__ res_left, int64_t rows, int hidden, float eps, double inv_hidden) {
   Arguments<0, 64>().arrive();
   constexpr int V = io<T>::kVec;
   constexpr bool kLow = std::is_same_v<T, float>;
@@ -208,6 +219,9 @@ __global__ __launch_bounds__(kThreads) void rmsnorm_mx8_kernel(const T* __restri
         vals[j][e] += r[e];
       }
       if (res_out != nullptr && t + j * G < nvec) store_as<T, true>(res_out + at + piece(j), vals[j]);
+      if constexpr (V == 8) {
+        if (res_left != nullptr && t + j * G < nvec) res_left[row * nvec + t + j * G] = bf16_left(vals[j]);
+      }
     }
     if (t + j * G < nvec) {
       float piece_ss = 0.f;
@@ -250,21 +264,21 @@ __global__ __launch_bounds__(kThreads) void rmsnorm_mx8_kernel(const T* __restri
 }
 
 template <typename T, int G, int NV>
-void launch_norm(const void* x, const void* w, const pico_mx8& y, float* rstd, const void* ri, void* ro, int64_t rows, int hidden, float eps, hipStream_t s) {
+void launch_norm(const void* x, const void* w, const pico_mx8& y, float* rstd, const void* ri, void* ro, uint32_t* left, int64_t rows, int hidden, float eps, hipStream_t s) {
   constexpr int kRows = kThreads / G;
   hipLaunchKernelGGL((rmsnorm_mx8_kernel<T, G, NV>), dim3(static_cast<unsigned>((rows + kRows - 1) / kRows)), dim3(kThreads), 0, s, static_cast<const T*>(x),
-                     static_cast<const T*>(w), y, rstd, static_cast<const T*>(ri), static_cast<T*>(ro), rows, hidden, eps, 1. / hidden);
+                     static_cast<const T*>(w), y, rstd, static_cast<const T*>(ri), static_cast<T*>(ro), left, rows, hidden, eps, 1. / hidden);
 }
 template <typename T>
-void dispatch_norm(const void* x, const void* w, const pico_mx8& y, float* rstd, const void* ri, void* ro, int64_t rows, int hidden, float eps, hipStream_t s) {
+void dispatch_norm(const void* x, const void* w, const pico_mx8& y, float* rstd, const void* ri, void* ro, uint32_t* left, int64_t rows, int hidden, float eps, hipStream_t s) {
   const int nvec = hidden / io<T>::kVec;
-  if (nvec <= 64) return launch_norm<T, 64, 1>(x, w, y, rstd, ri, ro, rows, hidden, eps, s);
-  if (nvec <= 128) return launch_norm<T, 64, 2>(x, w, y, rstd, ri, ro, rows, hidden, eps, s);
-  if (nvec <= 256) return launch_norm<T, 64, 4>(x, w, y, rstd, ri, ro, rows, hidden, eps, s);
-  if (nvec <= 512) return launch_norm<T, 256, 2>(x, w, y, rstd, ri, ro, rows, hidden, eps, s);
-  if (nvec <= 1024) return launch_norm<T, 256, 4>(x, w, y, rstd, ri, ro, rows, hidden, eps, s);
-  if (nvec <= 2048) return launch_norm<T, 256, 8>(x, w, y, rstd, ri, ro, rows, hidden, eps, s);
-  launch_norm<T, 256, 16>(x, w, y, rstd, ri, ro, rows, hidden, eps, s);
+  if (nvec <= 64) return launch_norm<T, 64, 1>(x, w, y, rstd, ri, ro, left, rows, hidden, eps, s);
+  if (nvec <= 128) return launch_norm<T, 64, 2>(x, w, y, rstd, ri, ro, left, rows, hidden, eps, s);
+  if (nvec <= 256) return launch_norm<T, 64, 4>(x, w, y, rstd, ri, ro, left, rows, hidden, eps, s);
+  if (nvec <= 512) return launch_norm<T, 256, 2>(x, w, y, rstd, ri, ro, left, rows, hidden, eps, s);
+  if (nvec <= 1024) return launch_norm<T, 256, 4>(x, w, y, rstd, ri, ro, left, rows, hidden, eps, s);
+  if (nvec <= 2048) return launch_norm<T, 256, 8>(x, w, y, rstd, ri, ro, left, rows, hidden, eps, s);
+  launch_norm<T, 256, 16>(x, w, y, rstd, ri, ro, left, rows, hidden, eps, s);
 }
 
 int vec_of(int dtype) { return dtype == PICO_BF16 ? 8 : 4; }
@@ -328,8 +342,8 @@ extern "C" int pico_mx8_dequantize(const pico_mx8* x, void* y, int64_t rows, int
   return check_launch(fn);
 }
 
-extern "C" int pico_rmsnorm_mx8_fwd(const void* x, const void* weight, const pico_mx8* y, float* rstd, const void* residual_in, void* residual_out, int64_t rows, int64_t hidden,
-                                    float eps, int dtype, void* stream) {
+extern "C" int pico_rmsnorm_mx8_fwd(const void* x, const void* weight, const pico_mx8* y, float* rstd, const void* residual_in, void* residual_out, void* residual_left, int64_t rows,
+                                    int64_t hidden, float eps, int dtype, void* stream) {
   const char* fn = "pico_rmsnorm_mx8_fwd";
   PICO_TRY(check_dtype(fn, dtype));
   PICO_TRY(check_mx8_shape(fn, rows, hidden));
@@ -339,11 +353,12 @@ extern "C" int pico_rmsnorm_mx8_fwd(const void* x, const void* weight, const pic
   PICO_TRY(check_rows(fn, "x", x, hidden, hidden, dtype));
   PICO_TRY(check_rows(fn, "weight", weight, hidden, hidden, dtype));
   PICO_TRY(check_mx8(fn, "y", y));
-  if (residual_out && !residual_in) return fail(PICO_ERR_NULL, "%s: residual_out without residual_in", fn);
-  if (!aligned16(residual_in) || !aligned16(residual_out)) return fail(PICO_ERR_ALIGN, "%s: pointers must be 16-byte aligned", fn);
+  if ((residual_out || residual_left) && !residual_in) return fail(PICO_ERR_NULL, "%s: residual_out or residual_left without residual_in", fn);
+  if (residual_left && dtype != PICO_BF16) return fail(PICO_ERR_DTYPE, "%s: residual_left is bf16's", fn);
+  if (!aligned16(residual_in) || !aligned16(residual_out) || !aligned16(residual_left)) return fail(PICO_ERR_ALIGN, "%s: pointers must be 16-byte aligned", fn);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dtype == PICO_BF16) dispatch_norm<__bf16>(x, weight, *y, rstd, residual_in, residual_out, rows, static_cast<int>(hidden), eps, s);
-  else dispatch_norm<float>(x, weight, *y, rstd, residual_in, residual_out, rows, static_cast<int>(hidden), eps, s);
+  if (dtype == PICO_BF16) dispatch_norm<__bf16>(x, weight, *y, rstd, residual_in, residual_out, static_cast<uint32_t*>(residual_left), rows, static_cast<int>(hidden), eps, s);
+  else dispatch_norm<float>(x, weight, *y, rstd, residual_in, residual_out, static_cast<uint32_t*>(residual_left), rows, static_cast<int>(hidden), eps, s);
   return check_launch(fn);
 }
 

@@ -356,19 +356,24 @@ __global__ __launch_bounds__(NWAVE * kWave) void rmsnorm_bwd_wave_kernel(
 }
 
 // The backward from fp32 gradients that lie in pieces, as a product leaves them: dy = sum over `parts` of sums [parts, rows, hidden].  A dy that was rounded to bf16 on its way, an x that
-// was rounded (the residual stream) and a rounded dweight are three errors of one size in dweight; here the first is left out (dweight's relative 2-norm of the error 2.8e-3 -> 2.4e-3 where
-// the plain form's is 1.7e-3).  bf16 x, w, dres and dx.  Rows to a wave (G 64) or to the
-// workgroup (G 256), dweight's share in registers over all rows of a group.  Bound by memory: 4 parts + 6 bytes an element (two less without dres); [4096, 2048] with dres from one piece
-// 22 us (3.8 TB/s: two waves to a SIMD, two rows each; more would write more shares of dweight).
+// was rounded (the residual stream) and a rounded dweight are three errors of one size in dweight.  The first is left out here, the second where four bits more of x are given (x_left):
+// dweight's error against 64 bits, as relative 2-norms, 2.8e-3, 2.4e-3 without the first, 1.7e-3 without both.  bf16 x, w, dres and dx.  Rows to a wave (G 64) or to the workgroup
+// (G 256), dweight's share in registers over all rows of a group.  Bound by memory: 4 parts + 6.5 bytes an element (two less without dres); [4096, 2048] with dres from one piece 23 us
+// (3.8 TB/s: two waves to a SIMD, two rows each; more would write more shares of dweight).
 constexpr int kSumsThreads = 256;
 template <int G, int NV, bool kRes>
-__global__ __launch_bounds__(kSumsThreads) void rmsnorm_bwd_sums_kernel(const float* __restrict__ sums, int parts, const __bf16* __restrict__ x, const __bf16* __restrict__ w,
+__global__ __launch_bounds__(kSumsThreads) void rmsnorm_bwd_sums_kernel(const float* __restrict__ sums, int parts, const __bf16* __restrict__ x, const uint32_t* __restrict__ x_left, const __bf16* __restrict__ w,
                                                                         const float* __restrict__ rstd, const __bf16* __restrict__ dres, __bf16* __restrict__ dx,
                                                                         float* __restrict__ partial, int64_t rows, int hidden) {
   Arguments<0, 64>().arrive();
   constexpr int V = 8, kGroups = kSumsThreads / G;
   __shared__ float smem[kSumsThreads / kWave];
   extern __shared__ __attribute__((aligned(16))) float dw_lds[];   // [hidden] where there are several groups
+  // (bf16 and four bits more, sixteenths of its last place)
+  auto whole = [](u32x4 raw, uint32_t left, int e) {
+    const uint32_t pair = raw[e / 2];
+    return __uint_as_float((e % 2 ? pair & 0xffff0000u : pair << 16) + (static_cast<uint32_t>(static_cast<int>(left << (28 - 4 * e)) >> 28) << 12));
+  };
   const int t = threadIdx.x % G, nvec = hidden / V;
   const int gid = G == kWave ? __builtin_amdgcn_readfirstlane(threadIdx.x / G) : 0;
   const float inv_h = 1.f / static_cast<float>(hidden);
@@ -385,12 +390,14 @@ __global__ __launch_bounds__(kSumsThreads) void rmsnorm_bwd_sums_kernel(const fl
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + gid; row < rows; row += static_cast<int64_t>(gridDim.x) * kGroups) {
     f32x4 d[NV][2];
     u32x4 xr[NV], rr[kRes ? NV : 1];
+    uint32_t left[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int64_t at = row * hidden + (t + j * G < nvec ? t + j * G : 0) * V;
       d[j][0] = *reinterpret_cast<const f32x4*>(sums + at);
       d[j][1] = *reinterpret_cast<const f32x4*>(sums + at + 4);
       xr[j] = *reinterpret_cast<const u32x4*>(x + at);
+      left[j] = x_left != nullptr ? x_left[at / V] : 0u;
       if constexpr (kRes) rr[j] = *reinterpret_cast<const u32x4*>(dres + at);
     }
     for (int q = 1; q < parts; ++q) {
@@ -408,8 +415,8 @@ __global__ __launch_bounds__(kSumsThreads) void rmsnorm_bwd_sums_kernel(const fl
       if (t + j * G < nvec) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const uint32_t xb = xr[j][e / 2], wb = wp[j][e / 2];
-          const float xh = __uint_as_float(e % 2 ? xb & 0xffff0000u : xb << 16) * r, wv = __uint_as_float(e % 2 ? wb & 0xffff0000u : wb << 16), dv = d[j][e / 4][e % 4];
+          const uint32_t wb = wp[j][e / 2];
+          const float xh = whole(xr[j], left[j], e) * r, wv = __uint_as_float(e % 2 ? wb & 0xffff0000u : wb << 16), dv = d[j][e / 4][e % 4];
           c += dv * wv * xh;
           dw[j][e] += dv * xh;
         }
@@ -431,8 +438,8 @@ __global__ __launch_bounds__(kSumsThreads) void rmsnorm_bwd_sums_kernel(const fl
         float o[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const uint32_t xb = xr[j][e / 2], wb = wp[j][e / 2];
-          const float xv = __uint_as_float(e % 2 ? xb & 0xffff0000u : xb << 16), wv = __uint_as_float(e % 2 ? wb & 0xffff0000u : wb << 16);
+          const uint32_t wb = wp[j][e / 2];
+          const float xv = whole(xr[j], left[j], e), wv = __uint_as_float(e % 2 ? wb & 0xffff0000u : wb << 16);
           o[e] = r * (d[j][e / 4][e % 4] * wv - xv * r * c);
           if constexpr (kRes) o[e] += __uint_as_float(e % 2 ? rr[j][e / 2] & 0xffff0000u : rr[j][e / 2] << 16);
         }
@@ -778,12 +785,12 @@ int64_t bwd_partial_bytes(int64_t rows, int64_t hidden, int dtype) {
 }
 
 // Launches rmsnorm_bwd_sums_kernel: the blocks that it takes.
-int launch_bwd_sums(const float* sums, int parts, const void* x, const void* w, const float* rstd, const void* dres, void* dx, float* partial, int64_t rows, int hidden, hipStream_t s) {
+int launch_bwd_sums(const float* sums, int parts, const void* x, const void* x_left, const void* w, const float* rstd, const void* dres, void* dx, float* partial, int64_t rows, int hidden, hipStream_t s) {
   const int nvec = hidden / 8;
   auto go = [&](auto plain, auto with_residual, int groups) {
     const int blocks = bwd_blocks(rows, groups, hidden);
     hipLaunchKernelGGL(dres ? with_residual : plain, dim3(blocks), dim3(kSumsThreads), groups > 1 ? hidden * sizeof(float) : 0, s, sums, parts, static_cast<const __bf16*>(x),
-                       static_cast<const __bf16*>(w), rstd, static_cast<const __bf16*>(dres), static_cast<__bf16*>(dx), partial, rows, hidden);
+                       static_cast<const uint32_t*>(x_left), static_cast<const __bf16*>(w), rstd, static_cast<const __bf16*>(dres), static_cast<__bf16*>(dx), partial, rows, hidden);
     return blocks;
   };
 #define PICO_SUMS(G, NV) return go(rmsnorm_bwd_sums_kernel<G, NV, false>, rmsnorm_bwd_sums_kernel<G, NV, true>, kSumsThreads / G)
@@ -926,7 +933,7 @@ extern "C" int pico_rmsnorm_bwd_static(const void* dy, const void* x, const void
                           pico_rmsnorm_bwd_static_max_bytes(), rows, hidden, dtype, static_cast<hipStream_t>(stream));
 }
 
-extern "C" int pico_rmsnorm_bwd_sums(const float* dy, int parts, const void* x, const void* weight, const float* rstd, const void* dresidual, void* dx, void* dweight, int dweight_dtype,
+extern "C" int pico_rmsnorm_bwd_sums(const float* dy, int parts, const void* x, const void* x_left, const void* weight, const float* rstd, const void* dresidual, void* dx, void* dweight, int dweight_dtype,
                                      void* workspace, int64_t workspace_bytes, int64_t rows, int64_t hidden, void* stream) {
   const char* fn = "pico_rmsnorm_bwd_sums";
   if (int rc = check_common(fn, rows, hidden, PICO_BF16)) return rc;
@@ -941,10 +948,10 @@ extern "C" int pico_rmsnorm_bwd_sums(const float* dy, int parts, const void* x, 
   if (!dy || !x || !weight || !rstd || !dx || !workspace) return fail(PICO_ERR_NULL, "%s: dy, x, weight, rstd, dx and the workspace are required", fn);
   if (workspace_bytes < pico_rmsnorm_bwd_workspace_bytes(rows, hidden))
     return fail(PICO_ERR_WORKSPACE, "%s: the workspace has %lld bytes, needs %lld", fn, static_cast<long long>(workspace_bytes), static_cast<long long>(pico_rmsnorm_bwd_workspace_bytes(rows, hidden)));
-  if (!aligned16(dy) || !aligned16(x) || !aligned16(weight) || !aligned16(dx) || !aligned16(workspace) || !aligned16(dresidual))
+  if (!aligned16(dy) || !aligned16(x) || !aligned16(weight) || !aligned16(dx) || !aligned16(workspace) || !aligned16(dresidual) || !aligned16(x_left))
     return fail(PICO_ERR_ALIGN, "%s: pointers must be 16-byte aligned", fn);
   if (dx == x || dx == dresidual) return fail(PICO_ERR_NULL, "%s: dx cannot take an input's place", fn);
-  const int blocks = launch_bwd_sums(dy, parts, x, weight, rstd, dresidual, dx, static_cast<float*>(workspace), rows, static_cast<int>(hidden), s);
+  const int blocks = launch_bwd_sums(dy, parts, x, x_left, weight, rstd, dresidual, dx, static_cast<float*>(workspace), rows, static_cast<int>(hidden), s);
   if (int rc = check_launch(fn)) return rc;
   launch_dw_reduce(static_cast<float*>(workspace), dweight, dweight_dtype, blocks, static_cast<int>(hidden), s);
   return check_launch(fn);

@@ -230,23 +230,59 @@ def test_swiglu_linear(device, M, N, K):
 
 
 # ------------------------------------------------------------------------------------------------- the norm's gradient from fp32 pieces
+def in_bf16_and_what_is_left(h):
+    """(bf16(h), h with four bits more than that, the words of these bits) of fp32 h [rows, hidden]."""
+    held = h.to(BF16)
+    bits, first = h.view(torch.int32), held.float().view(torch.int32)
+    left = ((bits - first + 2048) >> 12).clamp(-8, 7)
+    shifts = torch.arange(0, 32, 4, device=h.device)
+    words = ((left.long() & 15).view(h.size(0), -1, 8) << shifts).sum(-1)
+    return held, (first + (left << 12)).view(F32), torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32)
+
+
+@pytest.mark.parametrize("rows,hidden", [(1, 32), (5, 576), (300, 2048), (7, 4128), (3, 16384)])
+def test_what_the_rounding_of_the_stream_leaves(device, rows, hidden):
+    """The words as defined, for values of any size, infinities and zeros; h itself within 2^-12 of bf16's last places more than it."""
+    import ctypes
+    from picotron_amd import _lib
+    lib, g = _lib.lib(), gen(hidden)
+    x, r = (randn(rows, hidden, g=g, dtype=F32) * torch.exp2(torch.randint(-100, 100, (rows, hidden), generator=g, device="cuda").float()) for _ in range(2))
+    x, r = x.to(BF16), torch.where(torch.rand(rows, hidden, generator=g, device="cuda") < 0.5, randn(rows, hidden, g=g).float() * x.abs().float() * 0.1, r).to(BF16)
+    x[0, :4], r[0, :4] = torch.tensor([0.0, -0.0, float("inf"), 1.0], device="cuda"), torch.tensor([0.0, -0.0, 1.0, -1.0], device="cuda")
+    h = x.float() + r.float()
+    out, words = torch.empty_like(x), torch.full((rows * hidden // 8 + 4,), 77, dtype=torch.int32, device="cuda")
+    data, scales = torch.empty(rows, hidden, dtype=torch.uint8, device="cuda"), torch.empty((hidden + 127) // 128, rows, 4, dtype=torch.uint8, device="cuda")
+    p = lambda t: ctypes.c_void_p(t.data_ptr())      # noqa: E731
+    _lib.check(lib.pico_rmsnorm_mx8_fwd(p(x), p(torch.ones_like(x[0])), ctypes.byref(_lib.Mx8(data.data_ptr(), scales.data_ptr())), None, p(r), p(out), p(words), rows, hidden, EPS,
+                                        _lib.PICO_BF16, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))
+    held, whole, want = in_bf16_and_what_is_left(h)
+    assert torch.equal(out, held) and torch.equal(words[:-4].view(rows, -1), want) and (words[-4:] == 77).all()
+    finite = h.isfinite() & (h.abs() >= 2.0 ** -126)
+    assert ((whole - h).abs()[finite] <= 2.0 ** -11 * h.abs()[finite]).all()
+    assert rows == 1 or ((held.float() - h).abs()[finite] > 2.0 ** -11 * h.abs()[finite]).any()
+
+
 @pytest.mark.parametrize("dw_dtype", [BF16, F32])
 @pytest.mark.parametrize("residual", [False, True])
 @pytest.mark.parametrize("rows,hidden,parts", [(1, 8, 1), (3, 96, 2), (33, 576, 1), (257, 2048, 3), (70, 4096, 1), (9, 4104, 2), (5, 8192, 1), (4, 16384, 2), (4500, 264, 1)])
-def test_norm_gradient_of_sums(device, rows, hidden, parts, residual, dw_dtype):
+@pytest.mark.parametrize("left", [False, True])
+def test_norm_gradient_of_sums(device, rows, hidden, parts, residual, dw_dtype, left):
     import ctypes
     from picotron_amd import _lib
     lib, g = _lib.lib(), gen(rows + hidden)
     dy = torch.randn(parts, rows, hidden, generator=g, device="cuda")
-    x, gamma = randn(rows, hidden, g=g), (1 + 0.2 * torch.randn(hidden, generator=g, device="cuda")).to(BF16)
-    rstd = (x.double().pow(2).mean(-1) + EPS).rsqrt().float()
+    h, gamma = randn(rows, hidden, g=g, dtype=F32), (1 + 0.2 * torch.randn(hidden, generator=g, device="cuda")).to(BF16)
+    x, whole, words = in_bf16_and_what_is_left(h)
+    if not left:
+        whole, words = x, None
+    rstd = (whole.double().pow(2).mean(-1) + EPS).rsqrt().float()
     dres = randn(rows, hidden, g=g) if residual else None
     dx, dw = torch.empty_like(x), torch.full((hidden + 8,), 3.0, dtype=dw_dtype, device="cuda")
     ws = torch.empty(lib.pico_rmsnorm_bwd_workspace_bytes(rows, hidden), dtype=torch.uint8, device="cuda")
     p = lambda t: ctypes.c_void_p(t.data_ptr()) if t is not None else None      # noqa: E731
-    _lib.check(lib.pico_rmsnorm_bwd_sums(p(dy), parts, p(x), p(gamma), p(rstd), p(dres), p(dx), p(dw), _lib.PICO_BF16 if dw_dtype == BF16 else _lib.PICO_F32, p(ws), ws.numel(), rows, hidden,
+    _lib.check(lib.pico_rmsnorm_bwd_sums(p(dy), parts, p(x), p(words), p(gamma), p(rstd), p(dres), p(dx), p(dw), _lib.PICO_BF16 if dw_dtype == BF16 else _lib.PICO_F32, p(ws), ws.numel(), rows, hidden,
                                          ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))
-    d, n, w = dy.double().sum(0), x.double() * rstd.double()[:, None], gamma.double()
+    d, n, w = dy.double().sum(0), whole.double() * rstd.double()[:, None], gamma.double()
     q = d * w
     want = rstd.double()[:, None] * (q - n * (q * n).mean(-1, keepdim=True)) + (dres.double() if residual else 0)
     # sums of `rows` (dweight) and `hidden` (the row's mean) products in fp32, 64 side by side at least; one rounding to bf16
@@ -323,7 +359,7 @@ def test_what_is_kept(device):
         y, h = layer(*leaves)
     mine = {t.data_ptr(): t.numel() * t.element_size() for t in kept if not any(t.data_ptr() == p.data_ptr() for p in (*leaves, h))}
     packed = M * K + M * K // 32 + 2 * (M * inner + M * inner // 32)
-    assert sum(mine.values()) == packed + M * 4      # (and rstd)
+    assert sum(mine.values()) == packed + M * 4 + M * K // 2      # (and rstd, and four bits more of h than bf16 holds)
 
 
 def test_upstream_gradients_of_any_layout(device):

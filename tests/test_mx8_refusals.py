@@ -31,7 +31,7 @@ def calls(lib, x=P, y8=None, rows=4, cols=64, ld=None, dtype=0):
     return {
         "quantize": lib.pico_mx8_quantize(x, y8, rows, cols, ld, dtype, None),
         "dequantize": lib.pico_mx8_dequantize(y8, x, rows, cols, ld, dtype, None),
-        "norm": lib.pico_rmsnorm_mx8_fwd(x, P, y8, None, None, None, rows, cols, 1e-5, dtype, None),
+        "norm": lib.pico_rmsnorm_mx8_fwd(x, P, y8, None, None, None, None, rows, cols, 1e-5, dtype, None),
         "swiglu": lib.pico_swiglu_mx8_fwd(x, P, None, y8, None, None, rows, cols, ld, ld, dtype, None),
         "swiglu_bwd": lib.pico_swiglu_mx8_bwd(x, y8, y8, P, P, None, rows, cols, ld, ld, ld, dtype, None),
     }
@@ -61,10 +61,13 @@ def test_pitches(lib):
 def test_what_belongs_together(lib):
     assert lib.pico_swiglu_mx8_fwd(P, P, None, None, packed(), packed(), 4, 64, 64, 64, 0, None) == -1       # no output
     assert lib.pico_swiglu_mx8_fwd(P, P, P, None, packed(), None, 4, 64, 64, 64, 0, None) == -1              # half a checkpoint
-    assert lib.pico_rmsnorm_mx8_fwd(P, P, packed(), None, None, P, 4, 64, 1e-5, 0, None) == -1               # a sum without a residual
-    assert lib.pico_rmsnorm_mx8_fwd(P, P, packed(), None, None, None, 4, 16384 + 32, 1e-5, 0, None) == -3
-    assert lib.pico_rmsnorm_mx8_fwd(P, P, packed(), None, None, None, 1 << 26, 64, 1e-5, 0, None) == -3     # threads of one launch
-    assert lib.pico_rmsnorm_mx8_fwd(P, P, packed(), None, ctypes.c_void_p(BUF + 4), None, 4, 64, 1e-5, 0, None) == -4
+    assert lib.pico_rmsnorm_mx8_fwd(P, P, packed(), None, None, P, None, 4, 64, 1e-5, 0, None) == -1         # a sum without a residual
+    assert lib.pico_rmsnorm_mx8_fwd(P, P, packed(), None, None, None, P, 4, 64, 1e-5, 0, None) == -1         # or what its rounding leaves
+    assert lib.pico_rmsnorm_mx8_fwd(P, P, packed(), None, P, P, P, 4, 64, 1e-5, 1, None) == -2               # fp32 leaves nothing
+    assert lib.pico_rmsnorm_mx8_fwd(P, P, packed(), None, P, P, ctypes.c_void_p(BUF + 8), 4, 64, 1e-5, 0, None) == -4
+    assert lib.pico_rmsnorm_mx8_fwd(P, P, packed(), None, None, None, None, 4, 16384 + 32, 1e-5, 0, None) == -3
+    assert lib.pico_rmsnorm_mx8_fwd(P, P, packed(), None, None, None, None, 1 << 26, 64, 1e-5, 0, None) == -3     # threads of one launch
+    assert lib.pico_rmsnorm_mx8_fwd(P, P, packed(), None, ctypes.c_void_p(BUF + 4), None, None, 4, 64, 1e-5, 0, None) == -4
 
 
 def test_products(lib):
@@ -95,10 +98,11 @@ def test_the_product_that_rounds(lib):
 
 
 def test_the_norms_gradient_from_sums(lib):
-    def call(parts=1, hidden=64, dw=P, dw_dtype=0, dx=P, x=ctypes.c_void_p(BUF + 64), ws=P, bytes_=1 << 30, rows=4):
-        return lib.pico_rmsnorm_bwd_sums(P, parts, x, P, P, None, dx, dw, dw_dtype, ws, bytes_, rows, hidden, None)
+    def call(parts=1, hidden=64, dw=P, dw_dtype=0, dx=P, x=ctypes.c_void_p(BUF + 64), ws=P, bytes_=1 << 30, rows=4, left=None):
+        return lib.pico_rmsnorm_bwd_sums(P, parts, x, left, P, P, None, dx, dw, dw_dtype, ws, bytes_, rows, hidden, None)
     assert call(hidden=12) == -3 and call(hidden=16384 + 8) == -3 and call(rows=-1) == -3 and call(parts=0) == -3 and call(parts=65) == -3
     assert call(dw=None) == -1 and call(ws=None) == -1 and call(x=P) == -1 and call(dw_dtype=4) == -2 and call(bytes_=64) == -6 and call(dx=ctypes.c_void_p(BUF + 8)) == -4
+    assert call(left=ctypes.c_void_p(BUF + 8)) == -4
 
 
 def test_nothing_to_do_is_no_error(lib):
