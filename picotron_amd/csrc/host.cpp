@@ -1887,27 +1887,35 @@ Tensor upstream(const Tensor& given) {
   return plain(m) && m.stride(0) % 8 == 0 ? m : mx8_dense(m);
 }
 Tensor weight_rows(const Tensor& w) { return plain(w) ? w : mx8_dense(w); }   // (as upstream)
-// dy [rows, out] and w [out, in] with zeros up to a multiple of 8 outputs, as the kernels that leave fp32 sums take them.  (The library takes them as they are: there the copies do not pay, us
-// for both gradients without and with them, [4096 x 5003] and [5003 x 2048] 191, 222; [4096 x 15001] and [15001 x 4096] 920, 886.)
+// dy [rows, out] and w [out, in], where it is given, with zeros up to a multiple of 8 outputs, as this package's kernels take them.
 struct Rounded {
   Tensor dy, w;
 };
 Rounded rounded_up(const Tensor& dy, const Tensor& w) {
   const int64_t out = dy.size(1), more = (8 - out % 8) % 8;
   if (more == 0 || dy.size(0) == 0) return {dy, w};
-  return {at::constant_pad_nd(dy, {0, more}), at::constant_pad_nd(w, {0, 0, 0, more})};
+  return {at::constant_pad_nd(dy, {0, more}), w.defined() ? at::constant_pad_nd(w, {0, 0, 0, more}) : w};
 }
+// The same where it pays: the library takes other numbers of outputs as they are, and slower.  us for both gradients so and with the copies, rows x in x out: 422 x 4096 x 16533 323, 216;
+// 16000 x 2048 x 2049 472, 288; 2314 x 2048 x 2439 98, 86; 4096 x 4096 x 15001 857, 828; 4096 x 2048 x 5003 180, 191.  Of few inputs the copy of dy costs more than it saves (9216 x 576 x 2772, the layer's step, 176, 188); small ones are bound by
+// their launches.
+Rounded rounded_up_if_it_pays(const Tensor& dy, const Tensor& w, int64_t in) {
+  return in >= 1024 && dy.size(0) * dy.size(1) * in >= INT64_C(3000000000) ? rounded_up(dy, w) : Rounded{dy, w};
+}
+// the rows of dw [out or more, in] that a weight has
+Tensor outputs_of(const Tensor& dw, int64_t out) { return dw.size(0) == out ? dw : dw.narrow(0, 0, out); }
 // the gradients of x [rows, in] and of the weight, as wanted
 struct WeightGradients {
   Tensor dx, dw;
 };
-WeightGradients weight_gradients(const Tensor& dy, const Tensor& given, bool want_x, bool want_w, const std::function<Tensor()>& x) {
-  const Tensor w = want_x ? weight_rows(given) : Tensor();
+WeightGradients weight_gradients(const Tensor& given_dy, const Tensor& given, int64_t in, bool want_x, bool want_w, const std::function<Tensor()>& x) {
+  const auto [dy, w] = rounded_up_if_it_pays(given_dy, want_x ? weight_rows(given) : Tensor(), in);
+  const int64_t out = given_dy.size(1);
   if (want_x && want_w) {
     const Gradients both = gradients(dy, w, x());
-    return {both.dx, both.dw};
+    return {both.dx, outputs_of(both.dw, out)};
   }
-  return {want_x ? product(dy, w, Product::NN) : Tensor(), want_w ? product(dy, x(), Product::TN) : Tensor()};
+  return {want_x ? product(dy, w, Product::NN) : Tensor(), want_w ? outputs_of(product(dy, x(), Product::TN), out) : Tensor()};
 }
 // dy w in fp32, in pieces to be added, as pico_rmsnorm_bwd_sums takes it; `parts` 0 where no kernel gives that (torch settings ask for another route)
 struct Sums {
@@ -1998,7 +2006,7 @@ struct Linear8 : torch::autograd::Function<Linear8> {
     const auto sizes = ctx->saved_data["sizes"].toIntVector();
     const c10::OptionalDeviceGuard device(g[0].device());
     const Tensor dy = upstream(g[0]);
-    WeightGradients r = weight_gradients(dy, s[0], ctx->needs_input_grad(0), ctx->needs_input_grad(1), [&] { return values(s[1], dy.size(0), sizes.back()); });
+    WeightGradients r = weight_gradients(dy, s[0], sizes.back(), ctx->needs_input_grad(0), ctx->needs_input_grad(1), [&] { return values(s[1], dy.size(0), sizes.back()); });
     return {r.dx.defined() ? r.dx.view(sizes) : Tensor(), r.dw, Tensor()};
   }
 };
@@ -2055,16 +2063,17 @@ struct NormLinear8 : torch::autograd::Function<NormLinear8> {
     const c10::OptionalDeviceGuard device(g[0].device());
     const size_t at_gamma = has_residual ? 2 : 1;   // (among the tensors: eps, packed and a residual that is none do not count)
     const bool wants_norm = needs_any(ctx, 0, at_gamma + 1), wants_w = rows.empty() ? ctx->needs_input_grad(at_gamma + 1) : needs_any(ctx, at_gamma + 2, rows.size());
-    const Tensor dy = upstream(g[0]);
+    Tensor dy = upstream(g[0]);
     if (wants_norm) {
       const Rounded whole = rounded_up(dy, weight_rows(s[3]));
+      dy = whole.dy;
       auto [dx, dgamma] = norm_gradients(whole.dy, whole.w, mx8_dense(s[0]), s[5], mx8_dense(s[1]), s[2], g[1].defined() ? OptTensor(mx8_dense(g[1])) : std::nullopt);
       r[0] = dx;
       if (has_residual) r[1] = dx;
       r[2] = dgamma;
     }
     if (wants_w) {
-      const Tensor dw = product(dy, Linear8::values(s[4], dy.size(0), s[3].size(1)), Product::TN);
+      const Tensor dw = outputs_of(product(dy, Linear8::values(s[4], dy.size(0), s[3].size(1)), Product::TN), s[3].size(0));
       if (rows.empty()) r[4] = dw;
       int64_t at_row = 0;
       for (size_t i = 0; i < rows.size(); ++i, at_row += rows[i - 1]) r[6 + i] = dw.narrow(0, at_row, rows[i]);
@@ -2146,12 +2155,12 @@ struct SwiGLULinear8 : torch::autograd::Function<SwiGLULinear8> {
     refuse_second_order(fn);
     const auto s = ctx->get_saved_variables();
     const c10::OptionalDeviceGuard device(g[0].device());
-    const Tensor dy = upstream(g[0]), w = weight_rows(s[0]);
+    const auto [dy, w] = rounded_up_if_it_pays(upstream(g[0]), weight_rows(s[0]), s[0].size(1));
     variable_list r(3);
     const bool wants_w = ctx->needs_input_grad(1);
     auto [dx, h] = swiglu_mx8_backward(product(dy, w, Product::NN), {s[1], dy.size(0), w.size(1), 2}, ctx->saved_data["sizes"].toIntVector(), at::kBFloat16, wants_w);
     if (ctx->needs_input_grad(0)) r[0] = dx;
-    if (wants_w) r[1] = product(dy, h, Product::TN);
+    if (wants_w) r[1] = outputs_of(product(dy, h, Product::TN), s[0].size(0));
     return r;
   }
 };

@@ -91,7 +91,7 @@ def test_swiglu_extremes(device):
 
 
 # ------------------------------------------------------------------------------------------------- projections
-ROWS = [(1, 64, 32), (1, 2048, 576), (2, 40, 96), (17, 136, 160), (64, 256, 576), (129, 1000, 288), (300, 1728, 576), (512, 512, 1024), (1100, 260, 544), (2050, 2048, 512)]
+ROWS = [(1, 64, 32), (1, 2048, 576), (2, 40, 96), (17, 136, 160), (64, 256, 576), (129, 1000, 288), (300, 1728, 576), (512, 512, 1024), (1100, 260, 544), (2050, 2048, 512), (1100, 1357, 2112)]
 
 
 @pytest.mark.parametrize("M,N,K", ROWS)
