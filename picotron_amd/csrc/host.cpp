@@ -1894,7 +1894,15 @@ struct Rounded {
 Rounded rounded_up(const Tensor& dy, const Tensor& w) {
   const int64_t out = dy.size(1), more = (8 - out % 8) % 8;
   if (more == 0 || dy.size(0) == 0) return {dy, w};
-  return {at::constant_pad_nd(dy, {0, more}), w.defined() ? at::constant_pad_nd(w, {0, 0, 0, more}) : w};
+  auto with_zeros = [&](const Tensor& t, int64_t axis) {
+    auto sizes = t.sizes().vec();
+    sizes[axis] += more;
+    const Tensor y = at::empty(sizes, t.options());
+    y.narrow(axis, 0, out).copy_(t);
+    y.narrow(axis, out, more).zero_();
+    return y;
+  };
+  return {with_zeros(dy, 1), w.defined() ? with_zeros(w, 0) : w};
 }
 // The same where it pays: the library takes other numbers of outputs as they are, and slower.  us for both gradients so and with the copies, rows x in x out: 422 x 4096 x 16533 323, 216;
 // 16000 x 2048 x 2049 472, 288; 2314 x 2048 x 2439 98, 86; 4096 x 4096 x 15001 857, 828; 4096 x 2048 x 5003 180, 191.  Of few inputs the copy of dy costs more than it saves (9216 x 576 x 2772, the layer's step, 176, 188); small ones are bound by

@@ -170,49 +170,45 @@ __device__ __forceinline__ uint32_t bf16_left(const float (&v)[8]) {
   return word;
 }
 
-// A row to a wave (G 64) or to the workgroup (G 256), NV pieces of 16 bytes to a thread, which stay in registers between the sum of squares and the
-// output.  A value in the middle of two codes, or nearly so, takes the other one by an error of 2^-24: the row's sum goes over the lanes in 64 bits, and pieces with such a value are made anew
+// A row to a wave (G 64) or to the workgroup, NV pieces of 16 bytes to a thread, which stay in registers between the sum of squares and the
+// output; four at most, that a row is requested as a whole ([13986, 9984] in bf16 266 us by 256 threads with eight, 197 by 1024 with two).  A value in the middle of two codes, or nearly so, takes the other one by an error of 2^-24: the row's sum goes over the lanes in 64 bits, and pieces with such a value are made anew
 // with what the roundings leave.  Of 16 M values 1 then differs from the exact one's code, plainly 12; that costs 4 % ([16384, 2048] 40 -> 42 us).
+constexpr int norm_threads(int g) { return g < kThreads ? kThreads : g; }
 template <typename T, int G, int NV>
-__global__ __launch_bounds__(kThreads) void rmsnorm_mx8_kernel(const T* __restrict__ x, const T* __restrict__ w, const pico_mx8 y, float* __restrict__ rstd,
+__global__ __launch_bounds__(norm_threads(G)) void rmsnorm_mx8_kernel(const T* __restrict__ x, const T* __restrict__ w, const pico_mx8 y, float* __restrict__ rstd,
                                                                const T* __restrict__ res_in, T* __restrict__ res_out, uint32_t* __restrict__ res_left, int64_t rows, int hidden, float eps, double inv_hidden) {
   Arguments<0, 64>().arrive();
   constexpr int V = io<T>::kVec;
   constexpr bool kLow = std::is_same_v<T, float>;
-  __shared__ double smem[kThreads / kWave];
+  __shared__ double smem[norm_threads(G) / kWave];
   const int t = threadIdx.x % G, nvec = hidden / V;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / G) + threadIdx.x / G;
-  if (row >= rows) return;   // (G 256: uniform over the workgroup, which meets at a barrier below)
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (norm_threads(G) / G) + threadIdx.x / G;
+  if (row >= rows) return;   // (G over 64: uniform over the workgroup, which meets at a barrier below)
   const int64_t at = row * hidden;
   // everything that the row needs is requested before the first of it is used; pieces past the row re-read its first
-  constexpr bool kEarly = NV <= 4;
   auto piece = [&](int j) { return (t + j * G < nvec ? t + j * G : 0) * V; };
-  u32x4 x_raw[kEarly ? NV : 1], r_raw[kEarly ? NV : 1], w_raw[kEarly ? NV : 1];
-  if constexpr (kEarly) {
+  u32x4 x_raw[NV], r_raw[NV], w_raw[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) x_raw[j] = *reinterpret_cast<const u32x4*>(x + at + piece(j));
-    if (res_in != nullptr) {
+  for (int j = 0; j < NV; ++j) x_raw[j] = *reinterpret_cast<const u32x4*>(x + at + piece(j));
+  if (res_in != nullptr) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) r_raw[j] = *reinterpret_cast<const u32x4*>(res_in + at + piece(j));
-    }
-#pragma unroll
-    for (int j = 0; j < NV; ++j) w_raw[j] = *reinterpret_cast<const u32x4*>(w + piece(j));
-    __builtin_amdgcn_sched_barrier(0);
+    for (int j = 0; j < NV; ++j) r_raw[j] = *reinterpret_cast<const u32x4*>(res_in + at + piece(j));
   }
+#pragma unroll
+  for (int j = 0; j < NV; ++j) w_raw[j] = *reinterpret_cast<const u32x4*>(w + piece(j));
+  __builtin_amdgcn_sched_barrier(0);
   float vals[NV][V], low[kLow ? NV : 1][V];   // (the second: what a sum in fp32 leaves)
   double ss = 0.;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    if constexpr (kEarly) io<T>::load(&x_raw[j], vals[j]);
-    else io<T>::load(x + at + piece(j), vals[j]);
+    io<T>::load(&x_raw[j], vals[j]);
     if constexpr (kLow) {
 #pragma unroll
       for (int e = 0; e < V; ++e) low[j][e] = 0.f;
     }
     if (res_in != nullptr) {
       float r[V];
-      if constexpr (kEarly) io<T>::load(&r_raw[j], r);
-      else io<T>::load(res_in + at + piece(j), r);
+      io<T>::load(&r_raw[j], r);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         if constexpr (kLow) low[j][e] = sum_left(vals[j][e], r[e]);
@@ -243,8 +239,7 @@ __global__ __launch_bounds__(kThreads) void rmsnorm_mx8_kernel(const T* __restri
     const int v = t + j * G;
     if (__builtin_amdgcn_readfirstlane(v) >= nvec) break;   // (uniform: whole waves of pieces past the row)
     float wv[V], o[V];
-    if constexpr (kEarly) io<T>::load(&w_raw[j], wv);
-    else io<T>::load(w + piece(j), wv);
+    io<T>::load(&w_raw[j], wv);
 #pragma unroll
     for (int e = 0; e < V; ++e) o[e] = v < nvec ? vals[j][e] * r * wv[e] : 0.f;
     bool near = false;
@@ -265,8 +260,8 @@ __global__ __launch_bounds__(kThreads) void rmsnorm_mx8_kernel(const T* __restri
 
 template <typename T, int G, int NV>
 void launch_norm(const void* x, const void* w, const pico_mx8& y, float* rstd, const void* ri, void* ro, uint32_t* left, int64_t rows, int hidden, float eps, hipStream_t s) {
-  constexpr int kRows = kThreads / G;
-  hipLaunchKernelGGL((rmsnorm_mx8_kernel<T, G, NV>), dim3(static_cast<unsigned>((rows + kRows - 1) / kRows)), dim3(kThreads), 0, s, static_cast<const T*>(x),
+  constexpr int kRows = norm_threads(G) / G;
+  hipLaunchKernelGGL((rmsnorm_mx8_kernel<T, G, NV>), dim3(static_cast<unsigned>((rows + kRows - 1) / kRows)), dim3(norm_threads(G)), 0, s, static_cast<const T*>(x),
                      static_cast<const T*>(w), y, rstd, static_cast<const T*>(ri), static_cast<T*>(ro), left, rows, hidden, eps, 1. / hidden);
 }
 template <typename T>
@@ -277,8 +272,8 @@ void dispatch_norm(const void* x, const void* w, const pico_mx8& y, float* rstd,
   if (nvec <= 256) return launch_norm<T, 64, 4>(x, w, y, rstd, ri, ro, left, rows, hidden, eps, s);
   if (nvec <= 512) return launch_norm<T, 256, 2>(x, w, y, rstd, ri, ro, left, rows, hidden, eps, s);
   if (nvec <= 1024) return launch_norm<T, 256, 4>(x, w, y, rstd, ri, ro, left, rows, hidden, eps, s);
-  if (nvec <= 2048) return launch_norm<T, 256, 8>(x, w, y, rstd, ri, ro, left, rows, hidden, eps, s);
-  launch_norm<T, 256, 16>(x, w, y, rstd, ri, ro, left, rows, hidden, eps, s);
+  if (nvec <= 2048) return launch_norm<T, 1024, 2>(x, w, y, rstd, ri, ro, left, rows, hidden, eps, s);
+  launch_norm<T, 1024, 4>(x, w, y, rstd, ri, ro, left, rows, hidden, eps, s);
 }
 
 int vec_of(int dtype) { return dtype == PICO_BF16 ? 8 : 4; }

@@ -2,6 +2,7 @@
 // accesses, one row is owned by a wave (hidden <= 64*8 vectors) or by a 256-thread block, the row
 // stays in registers between the reduction and the normalisation so HBM is touched once.
 #include "common.h"
+#include <algorithm>
 
 // Scratch of pico_rmsnorm_bwd_static, the entry point that allocates nothing: the per-block partial sums of dweight
 // that pico_rmsnorm_bwd keeps in the caller's workspace.  4 MiB per GPU, held until the process ends.  In host code
@@ -357,17 +358,18 @@ __global__ __launch_bounds__(NWAVE * kWave) void rmsnorm_bwd_wave_kernel(
 
 // The backward from fp32 gradients that lie in pieces, as a product leaves them: dy = sum over `parts` of sums [parts, rows, hidden].  A dy that was rounded to bf16 on its way, an x that
 // was rounded (the residual stream) and a rounded dweight are three errors of one size in dweight.  The first is left out here, the second where four bits more of x are given (x_left):
-// dweight's error against 64 bits, as relative 2-norms, 2.8e-3, 2.4e-3 without the first, 1.7e-3 without both.  bf16 x, w, dres and dx.  Rows to a wave (G 64) or to the workgroup
-// (G 256), dweight's share in registers over all rows of a group.  Bound by memory: 4 parts + 6.5 bytes an element (two less without dres); [4096, 2048] with dres from one piece 23 us
+// dweight's error against 64 bits, as relative 2-norms, 2.8e-3, 2.4e-3 without the first, 1.7e-3 without both.  bf16 x, w, dres and dx.  Rows to a wave (G 64) or to the workgroup,
+// dweight's share in registers over all rows of a group; more than four pieces to a thread leave one wave to a SIMD ([13986, 9984] 534 us by 256 threads with eight and as few workgroups as
+// pico_rmsnorm_bwd takes, 284 by 1024 with two and 512: a copy's rate).  Bound by memory: 4 parts + 6.5 bytes an element (two less without dres); [4096, 2048] with dres from one piece 23 us
 // (3.8 TB/s: two waves to a SIMD, two rows each; more would write more shares of dweight).
-constexpr int kSumsThreads = 256;
+constexpr int sums_threads(int g) { return g < 256 ? 256 : g; }
 template <int G, int NV, bool kRes>
-__global__ __launch_bounds__(kSumsThreads) void rmsnorm_bwd_sums_kernel(const float* __restrict__ sums, int parts, const __bf16* __restrict__ x, const uint32_t* __restrict__ x_left, const __bf16* __restrict__ w,
+__global__ __launch_bounds__(sums_threads(G)) void rmsnorm_bwd_sums_kernel(const float* __restrict__ sums, int parts, const __bf16* __restrict__ x, const uint32_t* __restrict__ x_left, const __bf16* __restrict__ w,
                                                                         const float* __restrict__ rstd, const __bf16* __restrict__ dres, __bf16* __restrict__ dx,
                                                                         float* __restrict__ partial, int64_t rows, int hidden) {
   Arguments<0, 64>().arrive();
-  constexpr int V = 8, kGroups = kSumsThreads / G;
-  __shared__ float smem[kSumsThreads / kWave];
+  constexpr int V = 8, kGroups = sums_threads(G) / G;
+  __shared__ float smem[sums_threads(G) / kWave];
   extern __shared__ __attribute__((aligned(16))) float dw_lds[];   // [hidden] where there are several groups
   // (bf16 and four bits more, sixteenths of its last place)
   auto whole = [](u32x4 raw, uint32_t left, int e) {
@@ -787,19 +789,21 @@ int64_t bwd_partial_bytes(int64_t rows, int64_t hidden, int dtype) {
 // Launches rmsnorm_bwd_sums_kernel: the blocks that it takes.
 int launch_bwd_sums(const float* sums, int parts, const void* x, const void* x_left, const void* w, const float* rstd, const void* dres, void* dx, float* partial, int64_t rows, int hidden, hipStream_t s) {
   const int nvec = hidden / 8;
-  auto go = [&](auto plain, auto with_residual, int groups) {
-    const int blocks = bwd_blocks(rows, groups, hidden);
-    hipLaunchKernelGGL(dres ? with_residual : plain, dim3(blocks), dim3(kSumsThreads), groups > 1 ? hidden * sizeof(float) : 0, s, sums, parts, static_cast<const __bf16*>(x),
+  auto go = [&](auto plain, auto with_residual, int threads, int groups) {
+    // each workgroup writes hidden sums: of long rows a workgroup for 16 at least, where that is more than the CUs
+    const int most = hidden <= 2048 ? kMaxBwdBlocks : static_cast<int>(std::clamp<int64_t>(rows / 16, 256, kMaxBwdBlocks));
+    const int blocks = static_cast<int>(std::min<int64_t>((rows + groups - 1) / groups, most));
+    hipLaunchKernelGGL(dres ? with_residual : plain, dim3(blocks), dim3(threads), groups > 1 ? hidden * sizeof(float) : 0, s, sums, parts, static_cast<const __bf16*>(x),
                        static_cast<const uint32_t*>(x_left), static_cast<const __bf16*>(w), rstd, static_cast<const __bf16*>(dres), static_cast<__bf16*>(dx), partial, rows, hidden);
     return blocks;
   };
-#define PICO_SUMS(G, NV) return go(rmsnorm_bwd_sums_kernel<G, NV, false>, rmsnorm_bwd_sums_kernel<G, NV, true>, kSumsThreads / G)
+#define PICO_SUMS(G, NV) return go(rmsnorm_bwd_sums_kernel<G, NV, false>, rmsnorm_bwd_sums_kernel<G, NV, true>, sums_threads(G), sums_threads(G) / G)
   if (nvec <= 64) PICO_SUMS(64, 1);
   if (nvec <= 128) PICO_SUMS(64, 2);
   if (nvec <= 256) PICO_SUMS(64, 4);
-  if (nvec <= 512) PICO_SUMS(64, 8);
-  if (nvec <= 1024) PICO_SUMS(256, 4);
-  PICO_SUMS(256, 8);
+  if (nvec <= 512) PICO_SUMS(256, 2);
+  if (nvec <= 1024) PICO_SUMS(512, 2);
+  PICO_SUMS(1024, 2);
 #undef PICO_SUMS
 }
 
