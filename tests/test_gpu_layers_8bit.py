@@ -456,6 +456,43 @@ def test_a_captured_step_replays(device):
         assert all(torch.equal(a, b) for a, b in zip(held, want))
 
 
+@pytest.mark.parametrize("tokens", [1, 7, 24])
+def test_a_captured_run_without_gradients_replays(device, tokens):
+    """A few tokens: rows rounded inside the product, contractions in pieces over a workspace, forms of few rows; two graphs that were captured one after the other replay in turn."""
+    from picotron_amd import functional, ops
+    g = gen(tokens)
+    w, v, gamma = randn(1024, 2048, g=g, scale=0.02), randn(2048, 8192, g=g, scale=0.01), randn(2048, g=g)
+    pw, pv = ops.mx8_quantize(w), ops.mx8_quantize(v)
+    x, r, gate_up = randn(tokens, 2048, g=g), randn(tokens, 2048, g=g), randn(tokens, 16384, g=g)
+
+    def run():
+        a = functional.linear_8bit(x, w, packed=pw)
+        b, h = functional.rms_norm_linear_8bit(x, r, gamma, EPS, w, packed=pw)
+        return a, b, h, functional.swiglu_linear_8bit(gate_up, v, packed=pv)
+    with torch.no_grad():
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            run()
+        torch.cuda.current_stream().wait_stream(stream)
+        graphs = []
+        for _ in range(2):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                held = run()
+            graphs.append((graph, held))
+        for turn in range(4):
+            for t in (x, r, gate_up):
+                t.copy_(randn(*t.shape, g=g))
+            want = run()
+            graph, held = graphs[turn % 2]
+            for t in held:
+                t.fill_(float("nan"))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(held, want))
+
+
 def test_other_streams_and_threads(device):
     import threading
     leaves, dy, dh = layer_inputs(M=300, K=320, inner=544)
