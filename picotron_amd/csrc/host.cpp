@@ -268,11 +268,14 @@ struct Rows {
   int64_t rows, cols, pitch;
 };
 bool one_pitch(const Tensor& t) {
-  if (t.dim() == 0 || t.stride(-1) != 1) return false;
-  for (int64_t i = t.dim() - 3; i >= 0; --i)
-    if (t.size(i) != 1 && t.stride(i) != t.stride(i + 1) * t.size(i + 1)) return false;
-  for (int64_t i = t.dim() - 2; i >= 0; --i)   // rows that share memory (an expanded axis, the gradient of a sum) have no pitch that a kernel takes
-    if (t.size(i) != 1) return t.stride(i) >= t.size(-1);
+  if (t.dim() == 0 || (t.stride(-1) != 1 && t.numel() > 0)) return false;
+  int64_t next = 0;   // where the axes behind this one, those of one element aside (whose strides say nothing), end
+  for (int64_t i = t.dim() - 2; i >= 0 && t.numel() > 0; --i) {
+    if (t.size(i) == 1) continue;
+    // rows that share memory (an expanded axis, the gradient of a sum) have no pitch that a kernel takes
+    if (next == 0 ? t.stride(i) < t.size(-1) : t.stride(i) != next) return false;
+    next = t.stride(i) * t.size(i);
+  }
   return true;
 }
 Rows as_rows(const Tensor& t_in) {
