@@ -548,7 +548,7 @@ int pico_linear_log_probs_bwd(const void* x, const void* w, const int64_t* targe
  *   scales  bytes [ceil(cols / 128), rows, 4], 4-byte aligned: byte (t, r, q) is that of columns 128 t + 32 q .. + 31 of row r and stands for
  *           2^(byte - 127); 255: the block is NaN.  Bytes past the last column are written as 0.
  * A block's scale is the smallest 2^e, e >= -127, for which its largest |value| / 2^e is at most 448; values are rounded to the nearest, ties to even.  A block
- * with an infinity or a NaN becomes NaN as a whole.  rows * ceil(cols / 128) stays under 2^27.
+ * with an infinity or a NaN becomes NaN as a whole.  rows * ceil(cols / 128) is 2^27 - 8 at most.
  */
 typedef struct pico_mx8 {
   void* data;
@@ -559,7 +559,7 @@ int pico_mx8_quantize(const void* x, const pico_mx8* y, int64_t rows, int64_t co
 /* The values that x stands for, in `dtype` (both hold them exactly from 2^-126 on; what was rounded up to 2^128 is infinite), with row pitch y_ld. */
 int pico_mx8_dequantize(const pico_mx8* x, void* y, int64_t rows, int64_t cols, int64_t y_ld, int dtype, void* stream);
 /* pico_rmsnorm_fwd (cast_then_scale = 0) whose output is written in 8 bits, from fp32, and in no other form: y [rows, hidden], hidden a multiple of 32
- * up to 16384.  The backward is pico_rmsnorm_bwd, with the gradient of the values that y stands for.  residual_left (bf16, may be NULL): what the rounding of
+ * up to 16384, 2^26 - 4 rows at most.  The backward is pico_rmsnorm_bwd, with the gradient of the values that y stands for.  residual_left (bf16, may be NULL): what the rounding of
  * residual_out leaves, [rows, hidden / 8] words of eight times four bits, sixteenths of the last place, -8 .. 7, the first value's lowest. */
 int pico_rmsnorm_mx8_fwd(const void* x, const void* weight, const pico_mx8* y, float* rstd, const void* residual_in, void* residual_out,
                          void* residual_left, int64_t rows, int64_t hidden, float eps, int dtype, void* stream);

@@ -108,11 +108,11 @@ inline int check_mx8(const char* fn, const char* what, const pico_mx8* t) {
     return fail(PICO_ERR_ALIGN, "%s: %s must have 16-byte aligned data and 4-byte aligned scales", fn, what);
   return PICO_OK;
 }
-// (up to 32 lanes walk a group of 128 columns, and a launch has under 2^32 threads)
-constexpr int64_t kMostGroups = (int64_t{1} << 27) - 1;
+// A launch has under 2^32 threads, in workgroups of 256, and up to 32 lanes walk a group of 128 columns: 2^24 - 1 workgroups of 8 groups.
+constexpr int64_t kMostGroups = (int64_t{1} << 27) - 8;
 inline int check_mx8_shape(const char* fn, int64_t rows, int64_t cols) {
   if (rows < 0 || cols < kBlock || cols % kBlock != 0 || cols > (int64_t{1} << 30) || rows > kMostGroups / ((cols + kGroup - 1) / kGroup))
-    return fail(PICO_ERR_SHAPE, "%s: rows=%lld cols=%lld (cols must be a multiple of %d, rows times groups of %d columns under 2^27)", fn, (long long)rows, (long long)cols,
+    return fail(PICO_ERR_SHAPE, "%s: rows=%lld cols=%lld (cols must be a multiple of %d, rows times groups of %d columns at most 2^27 - 8)", fn, (long long)rows, (long long)cols,
                 kBlock, kGroup);
   return PICO_OK;
 }

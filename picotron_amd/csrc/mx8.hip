@@ -343,7 +343,8 @@ extern "C" int pico_rmsnorm_mx8_fwd(const void* x, const void* weight, const pic
   PICO_TRY(check_dtype(fn, dtype));
   PICO_TRY(check_mx8_shape(fn, rows, hidden));
   if (hidden > 16384) return fail(PICO_ERR_SHAPE, "%s: hidden=%lld (16384 at most)", fn, (long long)hidden);
-  if (rows >= (int64_t{1} << 26)) return fail(PICO_ERR_SHAPE, "%s: rows=%lld (under 2^26)", fn, (long long)rows);   // (up to 64 lanes to a row)
+  // (a launch's threads: 2^24 - 1 workgroups of 256 with a wave to a row; longer rows take more and are fewer by the check above)
+  if (rows > (int64_t{1} << 26) - 4) return fail(PICO_ERR_SHAPE, "%s: rows=%lld (2^26 - 4 at most)", fn, (long long)rows);
   if (rows == 0) return PICO_OK;
   PICO_TRY(check_rows(fn, "x", x, hidden, hidden, dtype));
   PICO_TRY(check_rows(fn, "weight", weight, hidden, hidden, dtype));
