@@ -15,7 +15,6 @@ namespace pico {
 namespace {
 
 constexpr int kBlock = 32, kGroup = 128;   // values under one scale; columns whose four scales lie side by side
-constexpr float kLargestCode = 448.f;
 
 template <int kControl>
 __device__ __forceinline__ uint32_t dpp(uint32_t v) {   // (0 from lanes that are off)
@@ -31,7 +30,7 @@ __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
   return v;
 }
 // The scale of a block whose largest |value| has these bits.  An infinity's bits and a NaN's are larger than any finite value's.  448 is 1.75 * 2^8: a
-// mantissa over 1.75 takes the next power of two.
+// mantissa over 1.75 takes the next power of two (what is added, a quarter of a mantissa less its last bit, carries then).
 __device__ __forceinline__ uint32_t scale_byte(uint32_t largest) {
   const int e = static_cast<int>((largest + 0x1fffffu) >> 23) - 8;
   return largest >= 0x7f800000u ? 255u : static_cast<uint32_t>(max(e, 0));
