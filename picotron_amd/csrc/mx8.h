@@ -76,7 +76,8 @@ __device__ __forceinline__ void decode(const uint32_t (&word)[V / 4], uint32_t b
   const int e = static_cast<int>(byte) - 127;
 #pragma unroll
   for (int w = 0; w < V / 4; ++w) {
-    const auto low = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(word[w]), false), high = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(word[w]), true);
+    const int codes = byte == 255u ? 0x7f7f7f7f : static_cast<int>(word[w]);   // (NaN, whatever codes a block of it has)
+    const auto low = __builtin_amdgcn_cvt_pk_f32_fp8(codes, false), high = __builtin_amdgcn_cvt_pk_f32_fp8(codes, true);
     v[4 * w] = __builtin_amdgcn_ldexpf(low[0], e);
     v[4 * w + 1] = __builtin_amdgcn_ldexpf(low[1], e);
     v[4 * w + 2] = __builtin_amdgcn_ldexpf(high[0], e);
