@@ -558,8 +558,8 @@ typedef struct pico_mx8 {
 int pico_mx8_quantize(const void* x, const pico_mx8* y, int64_t rows, int64_t cols, int64_t x_ld, int dtype, void* stream);
 /* The values that x stands for, in `dtype` (both hold them exactly from 2^-126 on; what was rounded up to 2^128 is infinite), with row pitch y_ld. */
 int pico_mx8_dequantize(const pico_mx8* x, void* y, int64_t rows, int64_t cols, int64_t y_ld, int dtype, void* stream);
-/* pico_rmsnorm_fwd (cast_then_scale = 0) whose output is written in 8 bits, from fp32, and in no other form: y [rows, hidden], hidden a multiple of 32
- * up to 16384, 2^26 - 4 rows at most.  The backward is pico_rmsnorm_bwd, with the gradient of the values that y stands for.  residual_left (bf16, may be NULL): what the rounding of
+/* pico_rmsnorm_fwd (cast_then_scale = 0) whose output is written in 8 bits and in no other form: y [rows, hidden], hidden a multiple of 32
+ * up to 16384, 2^26 - 4 rows at most; its codes are those of the exact values (with residual_out in the place of x or residual_in, of the values in fp32).  The backward is pico_rmsnorm_bwd, with the gradient of the values that y stands for.  residual_left (bf16, may be NULL): what the rounding of
  * residual_out leaves, [rows, hidden / 8] words of eight times four bits, sixteenths of the last place, -8 .. 7, the first value's lowest. */
 int pico_rmsnorm_mx8_fwd(const void* x, const void* weight, const pico_mx8* y, float* rstd, const void* residual_in, void* residual_out,
                          void* residual_left, int64_t rows, int64_t hidden, float eps, int dtype, void* stream);

@@ -143,20 +143,16 @@ __device__ __forceinline__ double group_sum(double v, double* smem) {
   }
 }
 
-// a + b less its rounding
-__device__ __forceinline__ float sum_left(float a, float b) {
-#pragma clang fp contract(off)
-  const float s = a + b, of_b = s - a;
-  return (a - (s - of_b)) + (b - of_b);
-}
-// Whether what this fp32 value stands for, up to 4 of its last places away (three roundings, and that of h in fp32), may lie in the middle of two codes: its last 19 bits are 0 there.
-__device__ __forceinline__ bool may_be_a_middle(float v) { return (__float_as_uint(v) << 13) + (4u << 13) <= 8u << 13; }
-// (v + low) (r + left) w, its last bit 1 where fp32 does not hold it: no such value lies in the middle of two codes
-__device__ __forceinline__ float scaled(float v, float low, float r, float left, float w) {
-#pragma clang fp contract(off)
-  const float n = v * r, n_left = fmaf(low, r, fmaf(v, left, fmaf(v, r, -n))), y = n * w, y_left = fmaf(n_left, w, fmaf(n, w, -y)), s = y + y_left, s_left = y_left - (s - y);
-  const int bits = __float_as_int(s), away = ((__float_as_int(s_left) ^ bits) >> 31) | 1;
-  return __int_as_float(fabsf(s_left) > 0.f && bits % 2 == 0 ? bits + away : bits);
+// Whether what an fp32 value stands for, up to 4 of its last places away (three roundings, and that of h in fp32), may lie in the middle of two codes: its last 19 bits are 0 there.
+// This is under kNearMiddle then.
+constexpr uint32_t kNearMiddle = (8u << 13) + 1;
+__device__ __forceinline__ uint32_t past_a_middle(float v) { return (__float_as_uint(v) << 13) + (4u << 13); }
+// y in 32 bits, the last one 1 where they do not hold it: no such value lies in the middle of two codes
+__device__ __forceinline__ float no_middle(double y) {
+  const float s = static_cast<float>(y);
+  const double left = y - s;
+  const int bits = __float_as_int(s), away = (left < 0.) == (bits < 0) ? 1 : -1;
+  return __int_as_float(fabs(left) > 0. && bits % 2 == 0 ? bits + away : bits);
 }
 
 // What eight values' roundings to bf16 leave, in four bits each: sixteenths of bf16's last place, -8 .. 7.
@@ -170,16 +166,22 @@ __device__ __forceinline__ uint32_t bf16_left(const float (&v)[8]) {
   return word;
 }
 
-// A row to a wave (G 64) or to the workgroup, NV pieces of 16 bytes to a thread, which stay in registers between the sum of squares and the
-// output; four at most, that a row is requested as a whole ([13986, 9984] in bf16 266 us by 256 threads with eight, 197 by 1024 with two).  A value in the middle of two codes, or nearly so, takes the other one by an error of 2^-24: the row's sum goes over the lanes in 64 bits, and pieces with such a value are made anew
-// with what the roundings leave.  Of 16 M values 1 then differs from the exact one's code, plainly 12; that costs 4 % ([16384, 2048] 40 -> 42 us).
+// A row to a wave (G 64) or to the workgroup, NV pieces of 16 bytes to a thread, which stay in registers between the sum of squares and the output; four at most, that a row is
+// requested as a whole ([13986, 9984] in bf16 266 us by 256 threads with eight, 187 by 1024 with two).
+// Every code is that of the exact value.  Beside the middle of two codes an error of 2^-24 would take the other one, so the sum of squares is in 64 bits, with what x + residual loses in 32,
+// and pieces with such a value are made once more in 64 bits and written over ([16384, 2048] with the residual 42 us, as without any of it; 22.8 for 22.3 where there is none).  A
+// kernel for each: without a residual's registers 76 of them, five waves to a SIMD, where one kernel for both takes 98 and 25.2 us.
 constexpr int norm_threads(int g) { return g < kThreads ? kThreads : g; }
-template <typename T, int G, int NV>
+template <typename T>
+__device__ __forceinline__ float value_of(u32x4 raw, int e) {
+  if constexpr (std::is_same_v<T, float>) return __uint_as_float(raw[e]);
+  else return __uint_as_float(e % 2 ? raw[e / 2] & 0xffff0000u : raw[e / 2] << 16);
+}
+template <typename T, int G, int NV, bool kRes>
 __global__ __launch_bounds__(norm_threads(G)) void rmsnorm_mx8_kernel(const T* __restrict__ x, const T* __restrict__ w, const pico_mx8 y, float* __restrict__ rstd,
                                                                const T* __restrict__ res_in, T* __restrict__ res_out, uint32_t* __restrict__ res_left, int64_t rows, int hidden, float eps, double inv_hidden) {
   Arguments<0, 64>().arrive();
   constexpr int V = io<T>::kVec;
-  constexpr bool kLow = std::is_same_v<T, float>;
   __shared__ double smem[norm_threads(G) / kWave];
   const int t = threadIdx.x % G, nvec = hidden / V;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (norm_threads(G) / G) + threadIdx.x / G;
@@ -187,82 +189,108 @@ __global__ __launch_bounds__(norm_threads(G)) void rmsnorm_mx8_kernel(const T* _
   const int64_t at = row * hidden;
   // everything that the row needs is requested before the first of it is used; pieces past the row re-read its first
   auto piece = [&](int j) { return (t + j * G < nvec ? t + j * G : 0) * V; };
-  u32x4 x_raw[NV], r_raw[NV], w_raw[NV];
+  u32x4 x_raw[NV], r_raw[kRes ? NV : 1], w_raw[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) x_raw[j] = *reinterpret_cast<const u32x4*>(x + at + piece(j));
-  if (res_in != nullptr) {
+  if constexpr (kRes) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) r_raw[j] = *reinterpret_cast<const u32x4*>(res_in + at + piece(j));
   }
 #pragma unroll
   for (int j = 0; j < NV; ++j) w_raw[j] = *reinterpret_cast<const u32x4*>(w + piece(j));
   __builtin_amdgcn_sched_barrier(0);
-  float vals[NV][V], low[kLow ? NV : 1][V];   // (the second: what a sum in fp32 leaves)
+  float vals[NV][V];
   double ss = 0.;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    io<T>::load(&x_raw[j], vals[j]);
-    if constexpr (kLow) {
+    const bool live = t + j * G < nvec;
+    double piece_ss = 0.;
 #pragma unroll
-      for (int e = 0; e < V; ++e) low[j][e] = 0.f;
-    }
-    if (res_in != nullptr) {
-      float r[V];
-      io<T>::load(&r_raw[j], r);
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        if constexpr (kLow) low[j][e] = sum_left(vals[j][e], r[e]);
-        vals[j][e] += r[e];
+    for (int e = 0; e < V; ++e) {
+      vals[j][e] = value_of<T>(x_raw[j], e);
+      double h = vals[j][e];
+      if constexpr (kRes) {
+        const float b = value_of<T>(r_raw[j], e);
+        vals[j][e] += b;
+        h += b;   // (with what the sum in 32 bits loses)
       }
-      if (res_out != nullptr && t + j * G < nvec) store_as<T, true>(res_out + at + piece(j), vals[j]);
+      piece_ss += h * h;
+    }
+    asm volatile("" : "+v"(piece_ss));   // (here and now: behind the branch that needs it the operands would take 40 registers more)
+    if (live) ss += piece_ss;
+    if constexpr (kRes) {
+      if (res_out != nullptr && live) store_as<T, true>(res_out + at + piece(j), vals[j]);
       if constexpr (V == 8) {
-        if (res_left != nullptr && t + j * G < nvec) res_left[row * nvec + t + j * G] = bf16_left(vals[j]);
+        if (res_left != nullptr && live) res_left[row * nvec + t + j * G] = bf16_left(vals[j]);
       }
-    }
-    if (t + j * G < nvec) {
-      float piece_ss = 0.f;
-#pragma unroll
-      for (int e = 0; e < V; ++e) piece_ss += vals[j][e] * vals[j][e];
-      ss += piece_ss;
     }
   }
   const double mean = group_sum<G>(ss, smem) * inv_hidden + eps;
-  float r = rsqrtf(static_cast<float>(mean)), left = 0.f;
-  if (r > 0.f && r < __builtin_huge_valf()) {   // (0: a row with an infinity)
-    const double whole = r + 0.5 * r * (1. - mean * r * r);
-    r = static_cast<float>(whole);
-    left = static_cast<float>(whole - r);
-  }
+  float r = rsqrtf(static_cast<float>(mean));
+  double root = r;
+  if (r > 0.f && r < __builtin_huge_valf()) root += 0.5 * r * (1. - mean * r * r);   // (0: a row with an infinity)
+  r = static_cast<float>(root);
   if (rstd != nullptr && t == 0) rstd[row] = r;
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int v = t + j * G;
-    if (__builtin_amdgcn_readfirstlane(v) >= nvec) break;   // (uniform: whole waves of pieces past the row)
-    float wv[V], o[V];
-    io<T>::load(&w_raw[j], wv);
-#pragma unroll
-    for (int e = 0; e < V; ++e) o[e] = v < nvec ? vals[j][e] * r * wv[e] : 0.f;
-    bool near = false;
-#pragma unroll
-    for (int e = 0; e < V; ++e) near |= may_be_a_middle(o[e]);
-    if (__any(near && v < nvec)) {   // (one in a hundred, or two, of a wave's pieces)
-#pragma unroll
-      for (int e = 0; e < V; ++e) o[e] = v < nvec ? scaled(vals[j][e], kLow ? low[j][e] : 0.f, r, left, wv[e]) : 0.f;
-    }
+  auto put = [&](int v, const float (&o)[V]) {
     const Codes<V> c = encode<V>(o);
-    const uint32_t scales = four_scales<V>(c.scale, t);
+    const uint32_t scales = four_scales<V>(v < nvec ? c.scale : 0u, t);
     if (v < nvec) {
       store_codes<V>(static_cast<uint8_t*>(y.data) + at + static_cast<int64_t>(v) * V, c.word);
       if (v % (kGroup / V) == 0) static_cast<uint32_t*>(y.scales)[static_cast<int64_t>(v / (kGroup / V)) * rows + row] = scales;
     }
+  };
+  uint32_t anew = 0;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int v = t + j * G;
+    if (__builtin_amdgcn_readfirstlane(v) >= nvec) break;   // (uniform: whole waves of pieces past the row)
+    float o[V];
+    uint32_t nearest = ~0u;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      o[e] = vals[j][e] * r * value_of<T>(w_raw[j], e);
+      nearest = min(nearest, past_a_middle(o[e]));
+    }
+    if (__any(nearest < kNearMiddle)) {
+      bool near = false;   // (0 is no such value: rows of padding)
+#pragma unroll
+      for (int e = 0; e < V; ++e) near |= past_a_middle(o[e]) < kNearMiddle && o[e] != 0.f;
+      if (__any(near && v < nvec)) anew |= 1u << j;
+    }
+    put(v, o);
+  }
+  // One in a hundred of a wave's pieces, from the operands where they still are (kept in registers until here they would take 90 more).  Where the sum has taken the place of one, the
+  // codes stay those of the values in 32 bits.
+  if (anew == 0 || (kRes && (res_out == res_in || res_out == x))) return;
+  const T *x_again = x, *r_again = res_in;
+  asm volatile("" : "+s"(x_again), "+s"(r_again));   // (loads of their own)
+#pragma unroll 1
+  for (int j = 0; j < NV; ++j) {
+    if ((anew >> j & 1) == 0) continue;
+    const int v = t + j * G;
+    const u32x4 a = *reinterpret_cast<const u32x4*>(x_again + at + piece(j)), gamma = *reinterpret_cast<const u32x4*>(w + piece(j));
+    u32x4 b = {};
+    if constexpr (kRes) b = *reinterpret_cast<const u32x4*>(r_again + at + piece(j));
+    float o[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      double h = value_of<T>(a, e);
+      if constexpr (kRes) h += value_of<T>(b, e);
+      o[e] = no_middle(h * root * value_of<T>(gamma, e));
+    }
+    put(v, o);
   }
 }
 
 template <typename T, int G, int NV>
 void launch_norm(const void* x, const void* w, const pico_mx8& y, float* rstd, const void* ri, void* ro, uint32_t* left, int64_t rows, int hidden, float eps, hipStream_t s) {
   constexpr int kRows = norm_threads(G) / G;
-  hipLaunchKernelGGL((rmsnorm_mx8_kernel<T, G, NV>), dim3(static_cast<unsigned>((rows + kRows - 1) / kRows)), dim3(norm_threads(G)), 0, s, static_cast<const T*>(x),
-                     static_cast<const T*>(w), y, rstd, static_cast<const T*>(ri), static_cast<T*>(ro), left, rows, hidden, eps, 1. / hidden);
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((rows + kRows - 1) / kRows)), dim3(norm_threads(G)), 0, s, static_cast<const T*>(x), static_cast<const T*>(w), y, rstd,
+                       static_cast<const T*>(ri), static_cast<T*>(ro), left, rows, hidden, eps, 1. / hidden);
+  };
+  if (ri != nullptr) go(rmsnorm_mx8_kernel<T, G, NV, true>);
+  else go(rmsnorm_mx8_kernel<T, G, NV, false>);
 }
 template <typename T>
 void dispatch_norm(const void* x, const void* w, const pico_mx8& y, float* rstd, const void* ri, void* ro, uint32_t* left, int64_t rows, int hidden, float eps, hipStream_t s) {
