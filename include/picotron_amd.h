@@ -574,6 +574,9 @@ int pico_swiglu_mx8_fwd(const void* gate, const void* up, void* y, const pico_mx
  * gradient of the weight that it met. */
 int pico_swiglu_mx8_bwd(const void* dy, const pico_mx8* gate8, const pico_mx8* up8, void* dgate, void* dup, void* y, int64_t rows, int64_t cols,
                         int64_t dy_ld, int64_t dgate_ld, int64_t dup_ld, int dtype, void* stream);
+/* The same, of bf16, for a gradient that a product left in fp32, in `parts` (1 .. 64) pieces to be added: dy [parts, rows, cols], contiguous. */
+int pico_swiglu_mx8_bwd_sums(const float* dy, int parts, const pico_mx8* gate8, const pico_mx8* up8, void* dgate, void* dup, void* y, int64_t rows,
+                             int64_t cols, int64_t dgate_ld, int64_t dup_ld, void* stream);
 /* c = a b^T, bf16 [M, N rounded up to a multiple of 8] (the columns from N on are written as 0), contiguous, 16-byte aligned, for a [M, K] and b
  * [N, K].  workspace: pico_mx8_product_workspace_bytes bytes, 16-byte aligned (NULL where that is 0). */
 int64_t pico_mx8_product_workspace_bytes(int64_t M, int64_t N, int64_t K);

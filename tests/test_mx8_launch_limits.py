@@ -43,3 +43,13 @@ def test_the_norm(lib, hidden, last, dtype):
     assert (last + rows_each - 1) // rows_each * threads < 2 ** 32
     for rows, code in ((last, NULL), (last + 1, SHAPE)):
         assert lib.pico_rmsnorm_mx8_fwd(None, P, packed(), None, None, None, None, rows, hidden, 1e-5, dtype, None) == code
+
+
+def test_swiglus_gradient_from_sums(lib):
+    def call(dy=P, parts=1, gate=None, dgate=P, y=None, rows=4, cols=64, ld=64):
+        return lib.pico_swiglu_mx8_bwd_sums(dy, parts, gate or packed(), packed(), dgate, P, y, rows, cols, ld, ld, None)
+    from picotron_amd._lib import Mx8
+    away = ctypes.c_void_p(4096 + 8)
+    assert [call(parts=0), call(parts=65), call(cols=40), call(rows=-1), call(rows=2 ** 27)] == [SHAPE] * 5
+    assert [call(dy=None), call(dgate=None), call(gate=ctypes.byref(Mx8(None, 4096)))] == [NULL] * 3
+    assert [call(dy=away), call(dgate=away), call(y=away), call(ld=68)] == [-4] * 4 and call(ld=56) == -5 and call(rows=0, dy=None) == 0
