@@ -1936,24 +1936,11 @@ struct Sums {
 Sums input_sums(const Tensor& dy, const Tensor& w) {
   if (dy.size(0) == 0 || stays_with_torch(dy, w)) return {Tensor(), 0};
   const ProductSizes n = product_sizes(dy, w, Product::NN);
-  if (!pico_product_mid_takes(n.M, n.N, n.K, n.lda, n.ldb, 0, 1)) return {Tensor(), 0};
-  const ProductRoute r = product_route(Product::NN, n);
-  int tile_m = static_cast<int>(r.tile_m), tile_n = static_cast<int>(r.tile_n), parts = static_cast<int>(r.parts);
-  bool large = r.kernel == ProductRoute::Large;
-  if (r.kernel == ProductRoute::Mid) {   // (tiles under 64 x 96 have no form in fp32)
-    if (tile_m * tile_n <= 64 * 64) tile_m = 64, tile_n = 96;
-    else if (tile_m * tile_n == 96 * 64) tile_m = tile_n = 96;
-    else if (tile_m == 128 && tile_n < 128) tile_n = 128;
-  } else if (!large) {   // what goes to the library, or to the kernel of few rows
-    large = n.M >= 256 && n.N >= 256 && pico_product_large_takes(n.M, n.N, n.K, n.lda, n.ldb, 0, 1, 1);
-    tile_m = large ? 256 : 64;
-    tile_n = large ? 256 : 128;
-    // pieces where the tiles leave CUs idle, 256 of contraction each at least
-    const int64_t tiles = ((n.M + tile_m - 1) / tile_m) * ((n.N + tile_n - 1) / tile_n);
-    parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({256 / tiles, n.K / 256, 8})));
-  }
-  const Sums s = {at::empty({parts, n.M, n.N}, dy.options().dtype(at::kFloat)), parts};
-  check((large ? pico_product_large_sums : pico_product_mid_sums)(ptr(dy), ptr(w), fptr(s.t), n.M, n.N, n.K, n.lda, n.ldb, 0, 1, tile_m, tile_n, parts, stream_now()));
+  const SumsRoute r = sums_route(n);
+  if (r.parts == 0) return {Tensor(), 0};
+  const Sums s = {at::empty({r.parts, n.M, n.N}, dy.options().dtype(at::kFloat)), static_cast<int>(r.parts)};
+  check((r.large ? pico_product_large_sums : pico_product_mid_sums)(ptr(dy), ptr(w), fptr(s.t), n.M, n.N, n.K, n.lda, n.ldb, 0, 1, static_cast<int>(r.tile_m), static_cast<int>(r.tile_n),
+                                                                     s.parts, stream_now()));
   return s;
 }
 // The same in front of a weight [out, half], dy [rows, out] the gradient behind it.  dy w stays in fp32: rounded to bf16 on its way it made d(gate_up) off by 2.35e-3 in the relative 2-norm,
@@ -2334,6 +2321,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   }, pybind11::arg("dy"), pybind11::arg("w"), pybind11::arg("x"));
   // by the rules; tile_n > 0: in pico_product_large; groups > 0: in pico_product; anything else given: in the library, parts 0 and
   // turn -1 by the rules
+  m.def("sums_route", [](const Tensor& a, const Tensor& b) {   // for tests: where a b goes that is to stay in fp32
+    return stays_with_torch(a, b) ? std::string("torch") : route_name(sums_route(product_sizes(a, b, Product::NN)));
+  });
   m.def("product", [=](const Tensor& a, const Tensor& b, const std::string& kind, int64_t parts, int64_t turn, int64_t groups, int64_t tile, int64_t tile_n) {
     const Product k = product_kind(kind);
     if (stays_with_torch(a, b) || (parts == 0 && turn < 0 && groups < 0 && tile_n == 0)) return product(a, b, k);

@@ -434,6 +434,37 @@ std::string route_name(const ProductRoute& r) {
   }
 }
 
+// a b as fp32 sums in pieces that the caller adds (pico_product_large_sums, pico_product_mid_sums): the route's kernel, tiles and pieces where these leave such sums
+struct SumsRoute {
+  bool large = false;
+  int64_t tile_m = 0, tile_n = 0, parts = 0;   // (parts 0: no kernel gives them)
+};
+SumsRoute sums_route(const ProductSizes& n) {
+  if (!pico_product_mid_takes(n.M, n.N, n.K, n.lda, n.ldb, 0, 1)) return {};
+  const ProductRoute r = product_route(Product::NN, n);
+  // Pieces where the tiles leave CUs idle, 512 of contraction each at least: who adds them reads one after the other.  us of norm and projection with gradients in one piece, so, and with 256:
+  // 64 rows of 2048 with 2048 outputs 34.1, 31.8, 36.1; 333 of 576 with 1728 29.2, 26.1, 27.1; 512 of 576 with 1728 31.2, 28.1, 29.3.
+  auto in_pieces = [&](bool large, int64_t tile_m, int64_t tile_n) -> SumsRoute {
+    const int64_t tiles = ((n.M + tile_m - 1) / tile_m) * ((n.N + tile_n - 1) / tile_n);
+    return {large, tile_m, tile_n, std::max<int64_t>(1, std::min<int64_t>({256 / tiles, n.K / 512, 8}))};
+  };
+  if (r.kernel == ProductRoute::Large) return {true, r.tile_m, r.tile_n, r.parts};
+  if (r.kernel == ProductRoute::Mid) {
+    // tiles that have no form in fp32 become the next ones that have, and fewer
+    if (r.tile_m <= 64 && r.tile_n <= 64) return in_pieces(false, 64, 96);
+    if (r.tile_m == 96 && r.tile_n == 64) return in_pieces(false, 96, 96);
+    if (r.tile_m == 128 && r.tile_n < 128) return in_pieces(false, 128, 128);
+    return {false, r.tile_m, r.tile_n, r.parts};
+  }
+  // what goes to the library, or to the kernel of few rows
+  const bool large = n.M >= 256 && n.N >= 256 && pico_product_large_takes(n.M, n.N, n.K, n.lda, n.ldb, 0, 1, 1);
+  return large ? in_pieces(true, 256, 256) : in_pieces(false, 64, 128);
+}
+std::string route_name(const SumsRoute& r) {   // "mid 64x96 in 3", "none"
+  if (r.parts == 0) return "none";
+  return (r.large ? "large " : "mid ") + std::to_string(r.tile_m) + "x" + std::to_string(r.tile_n) + (r.parts > 1 ? " in " + std::to_string(r.parts) : "");
+}
+
 struct GradientTiles {
   MidProduct dx, dw;   // (tile_m 0: apart)
 };
