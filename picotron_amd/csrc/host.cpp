@@ -11,6 +11,7 @@
 #include <ATen/autocast_mode.h>
 #include <c10/hip/HIPStream.h>
 #include <hipblaslt/hipblaslt.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 
 #include <array>
 #include <cstdlib>
@@ -1426,6 +1427,19 @@ void refuse_second_order(const char* fn) {
 void refuse_tangents(const char* fn, std::initializer_list<const Tensor*> inputs) {
   for (const Tensor* t : inputs) TORCH_CHECK(!t->_fw_grad(0).defined(), fn, ": has no forward-mode derivative");
 }
+// Called by a backward pass.  A leaf of which an eager graph, recorded on the default stream, still lives keeps that graph's node for its gradient, and with it its stream: where the pass is
+// being captured the engine would have the default stream wait next, which cannot be captured and ends the process.
+void refuse_capture_beside_eager(const char* fn) {
+  if (capture_now() == 0) return;
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return;
+  for (size_t i = 0; i < node->num_outputs(); ++i) {
+    const auto& next = node->next_edge(i).function;
+    if (!next || !node->task_should_compute_output(i) || !dynamic_cast<torch::autograd::AccumulateGrad*>(next.get())) continue;
+    const auto stream = next->stream();
+    TORCH_CHECK(!stream || stream->id() != 0, fn, ": its backward cannot be captured while an eager graph of the same leaves, recorded on the default stream, lives (release its outputs first)");
+  }
+}
 // d(logits) of `up` times (dlp q + dh H) per row, in `d` where that holds the gradient for a factor of 1 already
 Tensor log_probs_gradient(const TokenRows& r, const float* max_sum, const float* entropy, const pico_values& dlp, const pico_values& dh, const Tensor& up, Tensor d,
                           double temperature, int64_t ignore_index) {
@@ -2014,6 +2028,7 @@ struct Linear8 : torch::autograd::Function<Linear8> {
   static Tensor values(const Tensor& bytes, int64_t rows, int64_t cols) { return mx8_values(Held{bytes, rows, cols, 1}.at(0), {rows, cols}, bytes.options().dtype(at::kBFloat16)); }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
     refuse_second_order(fn);
+    refuse_capture_beside_eager(fn);
     const auto s = ctx->get_saved_variables();
     const auto sizes = ctx->saved_data["sizes"].toIntVector();
     const c10::OptionalDeviceGuard device(g[0].device());
@@ -2063,6 +2078,7 @@ struct NormLinear8 : torch::autograd::Function<NormLinear8> {
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
     refuse_second_order(fn);
+    refuse_capture_beside_eager(fn);
     const auto rows = ctx->saved_data["rows"].toIntVector();
     variable_list r(6 + rows.size());
     const bool has_residual = ctx->saved_data["residual"].toBool();
@@ -2129,6 +2145,7 @@ struct SwiGLU8 : torch::autograd::Function<SwiGLU8> {
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
     refuse_second_order(fn);
+    refuse_capture_beside_eager(fn);
     const Tensor bytes = ctx->get_saved_variables()[0];
     const auto sizes = ctx->saved_data["sizes"].toIntVector();
     const c10::OptionalDeviceGuard device(bytes.device());
@@ -2165,6 +2182,7 @@ struct SwiGLULinear8 : torch::autograd::Function<SwiGLULinear8> {
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
     refuse_second_order(fn);
+    refuse_capture_beside_eager(fn);
     const auto s = ctx->get_saved_variables();
     const c10::OptionalDeviceGuard device(g[0].device());
     const auto [dy, w] = rounded_up(upstream(g[0]), weight_rows(s[0]));
