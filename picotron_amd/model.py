@@ -142,8 +142,17 @@ def _fused_residual() -> bool:
 def _linear_8bit() -> bool:
     """PICO_LINEAR_8BIT=1: the projections behind the layers' norms (q, k and v; gate and up) and behind SwiGLU multiply in 8 bits, and the activations that
     their backward reads are kept in 8 bits.  Weights, gradients and the residual stream stay as they are.  Needs the residual adds inside the norms and the fused
-    projections (both the default), bf16, and sizes that are multiples of 32."""
+    projections (both the default), bf16, and sizes that are multiples of 32.  A layer's norms, attention, MLP and down projection are read, not called: with hooks
+    on them, or another module in their place, it is an error."""
     return os.getenv("PICO_LINEAR_8BIT", "0") == "1"
+
+
+def _check_read(name, module, *types):
+    """An error where reading the module's weights would not do what calling it does."""
+    if type(module) not in types or "forward" in vars(module) or getattr(module, "bias", None) is not None:
+        raise RuntimeError(f"PICO_LINEAR_8BIT=1 reads {name} as a plain {types[0].__name__} without a bias, which {type(module).__name__} is not")
+    if module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks:
+        raise RuntimeError(f"PICO_LINEAR_8BIT=1 reads {name} without calling it, and its hooks would be silent")
 
 
 def _fused_weight(owner, name, linears):
@@ -336,6 +345,11 @@ class DecoderLayer(nn.Module):
         self.cos, self.sin = context_parallel.update_rope_for_context_parallel(self.cos, self.sin)
 
     def forward(self, x, attention_mask=None, position_ids=None):
+        if _linear_8bit():
+            if not _fused_residual():
+                raise RuntimeError("PICO_LINEAR_8BIT=1 needs the residual adds inside the norms (PICO_FUSED_RESIDUAL, FLASH_ATTEN)")
+            branch, x = self.forward_chained_8bit(x, None)
+            return x + branch
         cos, sin = self.cos, self.sin
         x = x + self.attention(self.input_layernorm(x), cos, sin, attention_mask, position_ids)
         x = x + self.mlp(self.post_attention_layernorm(x))
@@ -360,6 +374,11 @@ class DecoderLayer(nn.Module):
         kept for the backward that way."""
         if not _fused_projections() or self.cos.size(0) < branch.size(1):
             raise RuntimeError("PICO_LINEAR_8BIT=1 needs the fused projections (PICO_FUSED_PROJ) and RoPE tables as long as the sequence")
+        for name in ("input_layernorm", "post_attention_layernorm"):
+            _check_read(name, getattr(self, name), TritonRMSNorm)
+        _check_read("attention", self.attention, Attention)
+        _check_read("mlp", self.mlp, MLP)
+        _check_read("mlp.down_proj", self.mlp.down_proj, Linear, nn.Linear)
         norm, (w, parts) = self.input_layernorm, self.attention.qkv_weights()
         qkv, residual = rms_norm_linear_8bit(branch, residual, norm.weight, norm.eps, w, parts=parts)
         a = self.attention.from_qkv(qkv, self.cos, self.sin)
