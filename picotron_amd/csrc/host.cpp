@@ -1971,16 +1971,20 @@ std::pair<Tensor, Tensor> swiglu_mx8_backward(const Tensor& dy, const Tensor& w,
   check(pico_swiglu_mx8_bwd_sums(fptr(s.t), s.parts, &gate8.c, &up8.c, first, first + half * dx.element_size(), ptr(y), kept.rows, half, 2 * half, 2 * half, stream_now()));
   return {dx, y};
 }
-// The gradients of a norm [rows, hidden] in front of a weight, from that of the product, all bf16.
+// The gradients of a norm [rows, hidden] in front of a weight, from that of the product: dx in bf16, the norm's weight's in its own type (by way of fp32 where that is neither of the two).
 std::pair<Tensor, Tensor> norm_gradients(const Tensor& dy, const Tensor& w, const Tensor& x, const Tensor& left, const Tensor& norm_weight, const Tensor& rstd, const OptTensor& dresidual) {
   const Sums s = input_sums(dy, w);
-  if (s.parts == 0) return rmsnorm_backward(product(dy, w, Product::NN).view(x.sizes()), x, norm_weight, rstd, dresidual, norm_weight.scalar_type());
+  const at::ScalarType type = norm_weight.scalar_type(), made = type == at::kBFloat16 ? type : at::kFloat;
+  if (s.parts == 0) {
+    auto [dx, dw] = rmsnorm_backward(product(dy, w, Product::NN).view(x.sizes()), x, norm_weight, rstd, dresidual, made);
+    return {dx, dw.to(type)};
+  }
   const int64_t hidden = x.size(-1), rows = dy.size(0), bytes = pico_rmsnorm_bwd_workspace_bytes(rows, hidden);
   const Tensor weight = norm_weight.to(at::kBFloat16), dres = dresidual ? dresidual->to(at::kBFloat16) : Tensor();
-  const Tensor dx = at::empty(x.sizes(), x.options()), dw = at::empty({hidden}, norm_weight.options()), ws = at::empty({bytes}, x.options().dtype(at::kByte));
+  const Tensor dx = at::empty(x.sizes(), x.options()), dw = at::empty({hidden}, norm_weight.options().dtype(made)), ws = at::empty({bytes}, x.options().dtype(at::kByte));
   check(pico_rmsnorm_bwd_sums(fptr(s.t), s.parts, ptr(x), ptr(left), ptr(weight), fptr(rstd), ptr(dres), ptr(dx), ptr(dw), dtype_code(dw, "rms_norm_linear_8bit: norm_weight"), ptr(ws), bytes, rows, hidden,
                               stream_now()));
-  return {dx, dw};
+  return {dx, dw.to(type)};
 }
 std::vector<int64_t> part_rows(const char* fn, const Tensor& w, at::TensorList parts) {
   std::vector<int64_t> rows;

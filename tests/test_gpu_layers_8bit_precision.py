@@ -99,3 +99,22 @@ def test_swiglus_gradient_from_pieces(device, rows, cols, parts, want_y):
     if want_y:
         h = O.silu(a) * b
         assert ((y[:rows].double() - h).abs() <= (2.0 ** -8 + 40 * u) * h.abs() + 1e-30).all() and (y[rows] == 5).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float64])
+@pytest.mark.parametrize("M", [0, 5, 300])
+def test_norm_weights_of_other_types(device, M, dtype):
+    """Used in bf16, as everywhere; its gradient comes in its own type, and where it is frozen the others' come too."""
+    from picotron_amd import functional
+    g = torch.Generator(device="cuda").manual_seed(M)
+    x, r, w, dy = randn(M, 128, g=g).requires_grad_(), randn(M, 128, g=g), randn(72, 128, g=g, scale=0.1).requires_grad_(), randn(M, 72, g=g)
+    gamma = randn(128, g=g)
+    got = {}
+    for t in (dtype, F32):
+        leaf = gamma.to(t).requires_grad_()
+        y, _ = functional.rms_norm_linear_8bit(x, r, leaf, EPS, w)
+        got[t] = (y.detach(), *torch.autograd.grad(y, (x, w, leaf), dy))
+    assert got[dtype][3].dtype == dtype and torch.equal(got[dtype][3], got[F32][3].to(dtype))
+    assert all(torch.equal(a, b) for a, b in zip(got[dtype][:3], got[F32][:3]))
+    y, _ = functional.rms_norm_linear_8bit(x, r, gamma.to(dtype), EPS, w)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, (x, w), dy), got[F32][1:3]))
