@@ -1898,9 +1898,9 @@ bool needs_any(const AutogradContext* ctx, size_t from, size_t count) {
     if (ctx->needs_input_grad(from + i)) return true;
   return false;
 }
-// an upstream gradient as the products take it, whatever its layout (a bias of one layout's sums against another's would be none of the caller's)
-Tensor upstream(const Tensor& given) {
-  const Tensor g = as_it_is(given), m = g.dim() == 1 ? g.unsqueeze(0) : matrix(g);
+// an upstream gradient as the products take it, [rows, out], whatever its layout (a bias of one layout's sums against another's would be none of the caller's)
+Tensor upstream(const Tensor& given, int64_t rows) {
+  const Tensor g = as_it_is(given), m = g.dim() == 2 ? g : g.reshape({rows, g.size(-1)});
   return plain(m) && m.stride(0) % 8 == 0 ? m : mx8_dense(m);
 }
 Tensor weight_rows(const Tensor& w) { return plain(w) ? w : mx8_dense(w); }   // (as upstream)
@@ -2036,7 +2036,7 @@ struct Linear8 : torch::autograd::Function<Linear8> {
     const auto s = ctx->get_saved_variables();
     const auto sizes = ctx->saved_data["sizes"].toIntVector();
     const c10::OptionalDeviceGuard device(g[0].device());
-    const Tensor dy = upstream(g[0]);
+    const Tensor dy = upstream(g[0], c10::multiply_integers(sizes) / sizes.back());
     WeightGradients r = weight_gradients(dy, s[0], sizes.back(), ctx->needs_input_grad(0), ctx->needs_input_grad(1), [&] { return values(s[1], dy.size(0), sizes.back()); });
     return {r.dx.defined() ? r.dx.view(sizes) : Tensor(), r.dw, Tensor()};
   }
@@ -2095,7 +2095,7 @@ struct NormLinear8 : torch::autograd::Function<NormLinear8> {
     const c10::OptionalDeviceGuard device(g[0].device());
     const size_t at_gamma = has_residual ? 2 : 1;   // (among the tensors: eps, packed and a residual that is none do not count)
     const bool wants_norm = needs_any(ctx, 0, at_gamma + 1), wants_w = rows.empty() ? ctx->needs_input_grad(at_gamma + 1) : needs_any(ctx, at_gamma + 2, rows.size());
-    Tensor dy = upstream(g[0]);
+    Tensor dy = upstream(g[0], mx8_rows_of(s[0]));
     if (wants_norm) {
       const Rounded whole = rounded_up(dy, weight_rows(s[3]));
       dy = whole.dy;
@@ -2189,10 +2189,11 @@ struct SwiGLULinear8 : torch::autograd::Function<SwiGLULinear8> {
     refuse_capture_beside_eager(fn);
     const auto s = ctx->get_saved_variables();
     const c10::OptionalDeviceGuard device(g[0].device());
-    const auto [dy, w] = rounded_up(upstream(g[0]), weight_rows(s[0]));
+    const auto sizes = ctx->saved_data["sizes"].toIntVector();
+    const auto [dy, w] = rounded_up(upstream(g[0], c10::multiply_integers(sizes) / sizes.back()), weight_rows(s[0]));
     variable_list r(3);
     const bool wants_w = ctx->needs_input_grad(1);
-    auto [dx, h] = swiglu_mx8_backward(dy, w, {s[1], dy.size(0), w.size(1), 2}, ctx->saved_data["sizes"].toIntVector(), wants_w);
+    auto [dx, h] = swiglu_mx8_backward(dy, w, {s[1], dy.size(0), w.size(1), 2}, sizes, wants_w);
     if (ctx->needs_input_grad(0)) r[0] = dx;
     if (wants_w) r[1] = outputs_of(product(dy, h, Product::TN), s[0].size(0));
     return r;
