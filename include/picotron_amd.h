@@ -374,6 +374,9 @@ int pico_product_large(const void* a, const void* b, void* c, int64_t M, int64_t
  * for one piece. */
 int pico_product_large_sums(const void* a, const void* b, float* sums, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int a_slow,
                             int b_slow, int tile_m, int tile_n, int parts, void* stream);
+/* a b of pico_product_large in one piece, N a multiple of 16, its fp32 sums rounded to 20 bits (ties away from 0): the first 16 of a sum's bits in c [M, N], the other four in left
+ * [M, N / 8], words of eight values, the first one's lowest. */
+int pico_product_large_bits20(const void* a, const void* b, void* c, void* left, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int tile_m, int tile_n, void* stream);
 int pico_product_mid_sums(const void* a, const void* b, float* sums, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int a_slow,
                           int b_slow, int tile_m, int tile_n, int parts, void* stream);
 
@@ -576,6 +579,9 @@ int pico_swiglu_mx8_bwd(const void* dy, const pico_mx8* gate8, const pico_mx8* u
                         int64_t dy_ld, int64_t dgate_ld, int64_t dup_ld, int dtype, void* stream);
 /* The same, of bf16, for a gradient that a product left in fp32, in `parts` (1 .. 64) pieces to be added: dy [parts, rows, cols], contiguous. */
 int pico_swiglu_mx8_bwd_sums(const float* dy, int parts, const pico_mx8* gate8, const pico_mx8* up8, void* dgate, void* dup, void* y, int64_t rows,
+                             int64_t cols, int64_t dgate_ld, int64_t dup_ld, void* stream);
+/* The same, of bf16, for a gradient in 20 bits as pico_product_large_bits20 leaves it: dy [rows, cols] and dy_left [rows, cols / 8], contiguous. */
+int pico_swiglu_mx8_bwd_bits20(const void* dy, const void* dy_left, const pico_mx8* gate8, const pico_mx8* up8, void* dgate, void* dup, void* y, int64_t rows,
                              int64_t cols, int64_t dgate_ld, int64_t dup_ld, void* stream);
 /* c = a b^T, bf16 [M, N rounded up to a multiple of 8] (the columns from N on are written as 0), contiguous, 16-byte aligned, for a [M, K] and b
  * [N, K].  workspace: pico_mx8_product_workspace_bytes bytes, 16-byte aligned (NULL where that is 0). */

@@ -129,6 +129,8 @@ SIGNATURES = {
     "pico_swiglu_mx8_fwd": (c_int, [_P, _P, _P, _MX8, _MX8, _MX8] + [_I64] * 4 + [c_int, _P]),
     "pico_swiglu_mx8_bwd": (c_int, [_P, _MX8, _MX8, _P, _P, _P] + [_I64] * 5 + [c_int, _P]),
     "pico_swiglu_mx8_bwd_sums": (c_int, [_P, c_int, _MX8, _MX8, _P, _P, _P] + [_I64] * 4 + [_P]),
+    "pico_swiglu_mx8_bwd_bits20": (c_int, [_P, _P, _MX8, _MX8, _P, _P, _P] + [_I64] * 4 + [_P]),
+    "pico_product_large_bits20": (c_int, [_P] * 4 + [_I64] * 5 + [c_int, c_int, _P]),
     "pico_mx8_product_workspace_bytes": (_I64, [_I64] * 3),
     "pico_mx8_product": (c_int, [_MX8, _MX8, _P] + [_I64] * 3 + [_P, _I64, _P]),
     "pico_mx8_product_tiled": (c_int, [_MX8, _MX8, _P] + [_I64] * 3 + [c_int] * 4 + [_P, _I64, _P]),

@@ -35,6 +35,17 @@ __device__ __forceinline__ uint16_t float_to_bf16_bits(float f) {
   __bf16 h = static_cast<__bf16>(f);
   return __builtin_bit_cast(uint16_t, h);
 }
+// An fp32 value rounded to its first 20 bits, which the upper ones of the result are; and back, from the first 16 in their place and a word of eight values' other four.
+__device__ __forceinline__ uint32_t in_bits20(float v) { return __float_as_uint(v) + 0x800u; }
+__device__ __forceinline__ float from_bits20(uint32_t first16, uint32_t word, int e) { return __uint_as_float(first16 | (word >> (4 * e) & 15u) << 12); }
+// What the rounding of a value to bf16 leaves, in four bits: sixteenths of bf16's last place, -8 .. 7; and the value with them (bits of the bf16 one, eight values to a word).
+__device__ __forceinline__ uint32_t bf16_left(float v) {
+  const uint32_t bits = __float_as_uint(v), held = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<__bf16>(v))) << 16;
+  return static_cast<uint32_t>(min((static_cast<int>(bits - held) + 2048) >> 12, 7) & 15);
+}
+__device__ __forceinline__ float with_left(uint32_t held, uint32_t word, int e) {
+  return __uint_as_float(held + (static_cast<uint32_t>(static_cast<int>(word << (28 - 4 * e)) >> 28) << 12));
+}
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   bf16x2 v;
   v[0] = static_cast<__bf16>(lo);

@@ -1957,18 +1957,35 @@ Sums input_sums(const Tensor& dy, const Tensor& w) {
                                                                      s.parts, stream_now()));
   return s;
 }
-// The same in front of a weight [out, half], dy [rows, out] the gradient behind it.  dy w stays in fp32: rounded to bf16 on its way it made d(gate_up) off by 2.35e-3 in the relative 2-norm,
-// where its own rounding is 1.66e-3; the step of [8192 x 11008] and 4096 outputs takes 1712 us for 1657.  y is rounded to bf16, being an operand of the weight's gradient, which is off by
-// 2.35e-3 for that: y as two operands would take another product of its size, 580 us.
+// dy w in 20 bits, where the large product gives it in one piece: 2.5 bytes a value for the 4 of fp32
+struct Bits20 {
+  Tensor t, left;
+};
+Bits20 input_bits20(const Tensor& dy, const Tensor& w) {
+  if (dy.size(0) == 0 || stays_with_torch(dy, w)) return {};
+  const ProductSizes n = product_sizes(dy, w, Product::NN);
+  const SumsRoute r = sums_route(n);
+  if (!r.large || r.parts != 1 || n.N % 16 != 0) return {};
+  const Bits20 o = {at::empty({n.M, n.N}, dy.options()), at::empty({n.M, n.N / 8}, dy.options().dtype(at::kInt))};
+  check(pico_product_large_bits20(ptr(dy), ptr(w), ptr(o.t), ptr(o.left), n.M, n.N, n.K, n.lda, n.ldb, static_cast<int>(r.tile_m), static_cast<int>(r.tile_n), stream_now()));
+  return o;
+}
+// The same in front of a weight [out, half], dy [rows, out] the gradient behind it.  dy w keeps more than bf16 holds: rounded to that on its way it made d(gate_up) off by 2.35e-3 in the
+// relative 2-norm, where its own rounding is 1.66e-3.  The step with all gradients takes, over that, in 20 bits and in fp32, 1.005 and 1.035 of the time at [8192 x 11008] and 4096 outputs,
+// 1.015 and 1.06 at [4096 x 8192] and 2048.  y is rounded to bf16, being an operand of the weight's gradient, which is off by 2.35e-3 for that: y as two operands would take another product of
+// its size, a third more.
 std::pair<Tensor, Tensor> swiglu_mx8_backward(const Tensor& dy, const Tensor& w, const Held& kept, at::IntArrayRef sizes, bool want_y) {
-  const Sums s = input_sums(dy, w);
-  if (s.parts == 0) return swiglu_mx8_backward(product(dy, w, Product::NN), kept, sizes, at::kBFloat16, want_y);
+  const Bits20 more = input_bits20(dy, w);
+  const Sums s = more.t.defined() ? Sums{Tensor(), 0} : input_sums(dy, w);
+  if (!more.t.defined() && s.parts == 0) return swiglu_mx8_backward(product(dy, w, Product::NN), kept, sizes, at::kBFloat16, want_y);
   const int64_t half = kept.cols;
   const auto o = kept.bytes.options().dtype(at::kBFloat16);
   const Tensor dx = at::empty(sizes, o), y = want_y ? at::empty({kept.rows, half}, o) : Tensor();
   const Mx8 gate8 = kept.at(0), up8 = kept.at(1);
   char* first = static_cast<char*>(ptr(dx));
-  check(pico_swiglu_mx8_bwd_sums(fptr(s.t), s.parts, &gate8.c, &up8.c, first, first + half * dx.element_size(), ptr(y), kept.rows, half, 2 * half, 2 * half, stream_now()));
+  void* second = first + half * dx.element_size();
+  check(more.t.defined() ? pico_swiglu_mx8_bwd_bits20(ptr(more.t), ptr(more.left), &gate8.c, &up8.c, first, second, ptr(y), kept.rows, half, 2 * half, 2 * half, stream_now())
+                         : pico_swiglu_mx8_bwd_sums(fptr(s.t), s.parts, &gate8.c, &up8.c, first, second, ptr(y), kept.rows, half, 2 * half, 2 * half, stream_now()));
   return {dx, y};
 }
 // The gradients of a norm [rows, hidden] in front of a weight, from that of the product: dx in bf16, the norm's weight's in its own type (by way of fp32 where that is neither of the two).

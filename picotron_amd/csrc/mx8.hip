@@ -103,10 +103,11 @@ __global__ __launch_bounds__(kThreads) void swiglu_mx8_fwd_kernel(const T* __res
 }
 
 // With g, u what the checkpoint stands for and s = sigmoid(g): dgate = dy u s (1 + g (1 - s)), dup = dy g s; y = g s u again where it is wanted.
-// kSums: dy is fp32, contiguous, in `parts` pieces to be added, as a product leaves it ([8192, 11008] 184 us, 145 from a dy in bf16: a copy's rate both; reading what the product wrote last first, or writing past
-// the caches, is the same).
-template <typename T, bool kSums>
-__global__ __launch_bounds__(kThreads) void swiglu_mx8_bwd_kernel(const std::conditional_t<kSums, float, T>* __restrict__ dy, int parts, const pico_mx8 gate8, const pico_mx8 up8, T* __restrict__ dgate, T* __restrict__ dup,
+// kFrom: dy of rows of pitch dy_ld; or contiguous, in fp32 and in `parts` pieces to be added, as a product leaves it; or contiguous in 20 bits.  [8192, 11008] 145, 184
+// and 154 us, a copy's rate.
+enum class Upstream { Rows, Sums, Bits20 };
+template <typename T, Upstream kFrom>
+__global__ __launch_bounds__(kThreads) void swiglu_mx8_bwd_kernel(const std::conditional_t<kFrom == Upstream::Sums, float, T>* __restrict__ dy, const uint32_t* __restrict__ dy_left, int parts, const pico_mx8 gate8, const pico_mx8 up8, T* __restrict__ dgate, T* __restrict__ dup,
                                                                   T* __restrict__ y, int64_t rows, int cols, int64_t dy_ld, int64_t dgate_ld, int64_t dup_ld, int64_t groups,
                                                                   Divide per_row) {
   constexpr int V = io<T>::kVec;
@@ -115,7 +116,7 @@ __global__ __launch_bounds__(kThreads) void swiglu_mx8_bwd_kernel(const std::con
   float d[V], g[V], u[V], dg[V], du[V], o[V];
   load_block<V>(gate8, p, rows, cols, g);
   load_block<V>(up8, p, rows, cols, u);
-  if constexpr (kSums) {
+  if constexpr (kFrom == Upstream::Sums) {
     const float* from = dy + p.row * cols + p.col;
     f32x4 sum[V / 4];
 #pragma unroll
@@ -127,6 +128,12 @@ __global__ __launch_bounds__(kThreads) void swiglu_mx8_bwd_kernel(const std::con
     }
 #pragma unroll
     for (int e = 0; e < V; ++e) d[e] = sum[e / 4][e % 4];
+  } else if constexpr (kFrom == Upstream::Bits20) {
+    const int64_t at = p.row * cols + p.col;
+    const u32x4 raw = *reinterpret_cast<const u32x4*>(dy + at);
+    const uint32_t word = dy_left[at / 8];
+#pragma unroll
+    for (int e = 0; e < V; ++e) d[e] = from_bits20(e % 2 ? raw[e / 2] & 0xffff0000u : raw[e / 2] << 16, word, e);
   } else {
     io<T>::load(dy + p.row * dy_ld + p.col, d);
   }
@@ -171,14 +178,11 @@ __device__ __forceinline__ float no_middle(double y) {
   return __int_as_float(fabs(left) > 0. && bits % 2 == 0 ? bits + away : bits);
 }
 
-// What eight values' roundings to bf16 leave, in four bits each: sixteenths of bf16's last place, -8 .. 7.
+// of eight values
 __device__ __forceinline__ uint32_t bf16_left(const float (&v)[8]) {
   uint32_t word = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const uint32_t bits = __float_as_uint(v[e]), held = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<__bf16>(v[e]))) << 16;
-    word |= static_cast<uint32_t>(min((static_cast<int>(bits - held) + 2048) >> 12, 7) & 15) << (4 * e);
-  }
+  for (int e = 0; e < 8; ++e) word |= pico::bf16_left(v[e]) << (4 * e);
   return word;
 }
 
@@ -447,28 +451,41 @@ extern "C" int pico_swiglu_mx8_bwd(const void* dy, const pico_mx8* gate8, const 
   hipStream_t s = static_cast<hipStream_t>(stream);
   auto go = [&](auto kernel, auto zero) {
     using T = decltype(zero);
-    hipLaunchKernelGGL(kernel, w.grid, dim3(kThreads), 0, s, static_cast<const T*>(dy), 1, *gate8, *up8, static_cast<T*>(dgate), static_cast<T*>(dup), static_cast<T*>(y), rows,
+    hipLaunchKernelGGL(kernel, w.grid, dim3(kThreads), 0, s, static_cast<const T*>(dy), nullptr, 1, *gate8, *up8, static_cast<T*>(dgate), static_cast<T*>(dup), static_cast<T*>(y), rows,
                        static_cast<int>(cols), dy_ld, dgate_ld, dup_ld, w.groups, w.per_row);
   };
-  if (dtype == PICO_BF16) go(swiglu_mx8_bwd_kernel<__bf16, false>, __bf16());
-  else go(swiglu_mx8_bwd_kernel<float, false>, float());
+  if (dtype == PICO_BF16) go(swiglu_mx8_bwd_kernel<__bf16, Upstream::Rows>, __bf16());
+  else go(swiglu_mx8_bwd_kernel<float, Upstream::Rows>, float());
   return check_launch(fn);
 }
 
-extern "C" int pico_swiglu_mx8_bwd_sums(const float* dy, int parts, const pico_mx8* gate8, const pico_mx8* up8, void* dgate, void* dup, void* y, int64_t rows, int64_t cols, int64_t dgate_ld,
-                                        int64_t dup_ld, void* stream) {
-  const char* fn = "pico_swiglu_mx8_bwd_sums";
+namespace {
+// of bf16, from a contiguous dy that holds more than that
+template <Upstream kFrom, typename From>
+int swiglu_bwd_from(const char* fn, const From* dy, const void* dy_left, int parts, const pico_mx8* gate8, const pico_mx8* up8, void* dgate, void* dup, void* y, int64_t rows, int64_t cols,
+                    int64_t dgate_ld, int64_t dup_ld, void* stream) {
   PICO_TRY(check_mx8_shape(fn, rows, cols));
   if (parts < 1 || parts > 64) return fail(PICO_ERR_SHAPE, "%s: %d pieces (1 .. 64)", fn, parts);
   if (rows == 0) return PICO_OK;
-  PICO_TRY(check_rows(fn, "dy", dy, cols, cols, PICO_F32));
+  PICO_TRY(check_rows(fn, "dy", dy, cols, cols, kFrom == Upstream::Sums ? PICO_F32 : PICO_BF16));
+  if (kFrom == Upstream::Bits20) PICO_TRY(check_rows(fn, "dy_left", dy_left, cols, cols, PICO_F32));
   PICO_TRY(check_mx8(fn, "gate8", gate8));
   PICO_TRY(check_mx8(fn, "up8", up8));
   PICO_TRY(check_rows(fn, "dgate", dgate, cols, dgate_ld, PICO_BF16));
   PICO_TRY(check_rows(fn, "dup", dup, cols, dup_ld, PICO_BF16));
   if (y) PICO_TRY(check_rows(fn, "y", y, cols, cols, PICO_BF16));
   const Walk w = walk(rows, cols, PICO_BF16);
-  hipLaunchKernelGGL((swiglu_mx8_bwd_kernel<__bf16, true>), w.grid, dim3(kThreads), 0, static_cast<hipStream_t>(stream), dy, parts, *gate8, *up8, static_cast<__bf16*>(dgate),
-                     static_cast<__bf16*>(dup), static_cast<__bf16*>(y), rows, static_cast<int>(cols), cols, dgate_ld, dup_ld, w.groups, w.per_row);
+  hipLaunchKernelGGL((swiglu_mx8_bwd_kernel<__bf16, kFrom>), w.grid, dim3(kThreads), 0, static_cast<hipStream_t>(stream), dy, static_cast<const uint32_t*>(dy_left), parts, *gate8, *up8,
+                     static_cast<__bf16*>(dgate), static_cast<__bf16*>(dup), static_cast<__bf16*>(y), rows, static_cast<int>(cols), cols, dgate_ld, dup_ld, w.groups, w.per_row);
   return check_launch(fn);
+}
+}  // namespace
+
+extern "C" int pico_swiglu_mx8_bwd_sums(const float* dy, int parts, const pico_mx8* gate8, const pico_mx8* up8, void* dgate, void* dup, void* y, int64_t rows, int64_t cols, int64_t dgate_ld,
+                                        int64_t dup_ld, void* stream) {
+  return swiglu_bwd_from<Upstream::Sums>("pico_swiglu_mx8_bwd_sums", dy, nullptr, parts, gate8, up8, dgate, dup, y, rows, cols, dgate_ld, dup_ld, stream);
+}
+extern "C" int pico_swiglu_mx8_bwd_bits20(const void* dy, const void* dy_left, const pico_mx8* gate8, const pico_mx8* up8, void* dgate, void* dup, void* y, int64_t rows, int64_t cols,
+                                        int64_t dgate_ld, int64_t dup_ld, void* stream) {
+  return swiglu_bwd_from<Upstream::Bits20>("pico_swiglu_mx8_bwd_bits20", static_cast<const __bf16*>(dy), dy_left, 1, gate8, up8, dgate, dup, y, rows, cols, dgate_ld, dup_ld, stream);
 }

@@ -372,10 +372,7 @@ __global__ __launch_bounds__(sums_threads(G)) void rmsnorm_bwd_sums_kernel(const
   __shared__ float smem[sums_threads(G) / kWave];
   extern __shared__ __attribute__((aligned(16))) float dw_lds[];   // [hidden] where there are several groups
   // (bf16 and four bits more, sixteenths of its last place)
-  auto whole = [](u32x4 raw, uint32_t left, int e) {
-    const uint32_t pair = raw[e / 2];
-    return __uint_as_float((e % 2 ? pair & 0xffff0000u : pair << 16) + (static_cast<uint32_t>(static_cast<int>(left << (28 - 4 * e)) >> 28) << 12));
-  };
+  auto whole = [](u32x4 raw, uint32_t left, int e) { return with_left(e % 2 ? raw[e / 2] & 0xffff0000u : raw[e / 2] << 16, left, e); };
   const int t = threadIdx.x % G, nvec = hidden / V;
   const int gid = G == kWave ? __builtin_amdgcn_readfirstlane(threadIdx.x / G) : 0;
   const float inv_h = 1.f / static_cast<float>(hidden);

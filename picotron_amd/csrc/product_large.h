@@ -71,8 +71,11 @@ struct Shape {
 
 // The tile leaves for c [M, N], rows of pitch ldc, 16 rows and 128 bytes of columns at a time through LDS, as whole lines; what lies past the matrix is
 // dropped by the window.  No wave waits for another here, and the next tile's first steps are on their way.
-template <typename Out, int I, int J>
-__device__ __forceinline__ void store_tile(Out* c, int64_t first_row, int M, int N, int ldc, bool streaming, const Unit& u, int wm, int wn, int lane, unsigned char* rows, const f32x4 (&acc)[I][J]) {
+// kBits20 (N and ldc multiples of 16): the sums rounded to 20 bits (ties away from 0), of which the first 16 go to c and the others to `left`, [M, ldc / 8] words of eight values.  Four
+// operations a value; bf16 and what its rounding leaves took eight, [4096 x 2048] @ [2048 x 8192] 7 us more.
+template <typename Out, int I, int J, bool kBits20 = false>
+__device__ __forceinline__ void store_tile(Out* c, int64_t first_row, int M, int N, int ldc, bool streaming, const Unit& u, int wm, int wn, int lane, unsigned char* rows, const f32x4 (&acc)[I][J],
+                                           uint32_t* left = nullptr) {
   constexpr int kBlocks = 128 / 16 / static_cast<int>(sizeof(Out));   // of 16 columns in 128 bytes
   const int row0 = u.m0 + wm, col0 = u.n0 + wn, cols = N - col0, n = lane % 16, h = lane / 16;
   Out* base = c + (first_row + row0) * ldc + col0;
@@ -91,6 +94,9 @@ __device__ __forceinline__ void store_tile(Out* c, int64_t first_row, int M, int
         unsigned char* to = rows + n * 128;
         if constexpr (sizeof(Out) == 4) {
           *reinterpret_cast<f32x4*>(to + (((j - j0) * 4 + h) ^ (n / 2)) * 16) = acc[i][j];
+        } else if constexpr (kBits20) {
+          const u32x2 v = {__builtin_amdgcn_perm(in_bits20(acc[i][j][1]), in_bits20(acc[i][j][0]), 0x07060302u), __builtin_amdgcn_perm(in_bits20(acc[i][j][3]), in_bits20(acc[i][j][2]), 0x07060302u)};
+          *reinterpret_cast<u32x2*>(to + (((j - j0) * 2 + h / 2) ^ (n / 2)) * 16 + h % 2 * 8) = v;
         } else {
           bf16x4 v;
 #pragma unroll
@@ -109,6 +115,27 @@ __device__ __forceinline__ void store_tile(Out* c, int64_t first_row, int M, int
         if (streaming) __builtin_amdgcn_raw_buffer_store_b128(v, window, to, 0, kStreaming);
         else __builtin_amdgcn_raw_buffer_store_b128(v, window, to, 0, 0);
       }
+      if constexpr (kBits20) {   // 16 rows of 32 bytes, eight of them a lane: the two words of 16 columns
+        static_assert(sizeof(Out) == 2);
+        uint32_t here_lane = lane;
+        asm volatile("" : "+v"(here_lane));   // (what follows from it is made here, and not kept in registers over the products, where none is left)
+        const u32x4 l = resource({reinterpret_cast<uint64_t>(left + ((first_row + row0 + 16 * i) * ldc + col0) / 8),
+                                  live > 0 && cols > 0 ? static_cast<uint32_t>(((live - 1) * static_cast<int64_t>(ldc) + cols) / 2) : 0u});
+        const buffer_rsrc words = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(l[0] | static_cast<uint64_t>(l[1]) << 32), 0, static_cast<int>(l[2]), static_cast<int>(l[3]));
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          if (j < j0 || j >= j0 + kBlocks) continue;
+          __builtin_amdgcn_sched_barrier(0);   // (one after the other: there are no registers for more)
+          uint32_t four = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) four |= (in_bits20(acc[i][j][e]) >> 12 & 15u) << (4 * e);
+          *reinterpret_cast<uint16_t*>(rows + here_lane % 16 * 32 + (j - j0) * 8 + here_lane / 16 * 2) = static_cast<uint16_t>(four);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        const u32x2 v = *reinterpret_cast<const u32x2*>(rows + here_lane * 8);
+        const int block = j0 + static_cast<int>(here_lane % 4), to = static_cast<int>(here_lane / 4) * (ldc / 2) + block * 8;
+        __builtin_amdgcn_raw_buffer_store_b64(v, words, block < J && 16 * block < cols ? to : static_cast<int>(0xfffffff0u), 0, 0);
+      }
     }
   }
 }
@@ -125,6 +152,22 @@ struct StoreTile {
   static __device__ __forceinline__ void tile(const Params& p, const Unit& u, int wm, int wn, int lane, unsigned char* rows, f32x4 (&acc)[I][J]) {
     using Out = std::conditional_t<kParts, float, __bf16>;
     store_tile<Out, I, J>(static_cast<Out*>(p.c), static_cast<int64_t>(u.part) * p.M, p.M, p.N, p.N, p.streaming, u, wm, wn, lane, rows, acc);
+  }
+};
+
+// In 20 bits.
+struct LargeBits20Params : LargeParams {
+  uint32_t* left;   // [M, N / 8]
+};
+struct StoreBits20 {
+  using Params = LargeBits20Params;
+  template <int I, int J> static constexpr int kStores = I * ((J + 3) / 4) * 3;
+  template <int I> static constexpr int kBegun = 0;
+  static constexpr bool kCounted = false;
+  template <int I> static __device__ __forceinline__ void begin(const Params&, const Unit&, int, int, int, uint32_t) {}
+  template <int I, int J>
+  static __device__ __forceinline__ void tile(const Params& p, const Unit& u, int wm, int wn, int lane, unsigned char* rows, f32x4 (&acc)[I][J]) {
+    store_tile<__bf16, I, J, true>(static_cast<__bf16*>(p.c), 0, p.M, p.N, p.N, p.streaming, u, wm, wn, lane, rows, acc, p.left);
   }
 };
 
@@ -294,6 +337,32 @@ __global__ __launch_bounds__(512, 2) void product_large_kernel(const typename Ep
     Epilogue::template tile<I, J>(p, u, wm, wn, lane, rows, acc);
   }
   wait_requests<0>();   // (requests past the work's end still write zeros to LDS)
+}
+
+// On the host: the launch in given tiles.
+template <bool kSlowA, bool kSlowB, int I, int J, typename Epilogue>
+int launch_large(typename Epilogue::Params p, bool pieces, hipStream_t s) {
+  using S = Shape<kSlowA, kSlowB, I, J>;
+  static LdsOnce reserved;
+  if (!reserve_lds_once(reserved, reinterpret_cast<const void*>(&product_large_kernel<kSlowA, kSlowB, I, J, Epilogue>), S::kLds))
+    return fail(PICO_ERR_LAUNCH, "pico_product_large: cannot reserve %d bytes of LDS", S::kLds);
+  p.tiles_m = (p.M + S::TM - 1) / S::TM;
+  p.tiles_n = (p.N + S::TN - 1) / S::TN;
+  const int64_t units = static_cast<int64_t>(p.tiles_m) * p.tiles_n * p.parts;
+  // An output larger than the workgroups' one round of tiles would push the operands out of the caches as it is written: [4096 x
+  // 2048] @ [49152 x 2048]^T 638 -> 570 us, [4096 x 1024] @ [49152 x 1024]^T 358 -> 304.
+  p.streaming = !pieces && units > 256;
+  hipLaunchKernelGGL((product_large_kernel<kSlowA, kSlowB, I, J, Epilogue>), dim3(static_cast<unsigned>(std::min<int64_t>(units, 256))), dim3(S::kThreads), S::kLds, s, p);
+  return check_launch("pico_product_large");
+}
+template <bool kSlowA, bool kSlowB, typename Epilogue>
+int launch_tiles(const typename Epilogue::Params& p, bool pieces, int tile_m, int tile_n, hipStream_t s) {
+  if (tile_m == 256 && tile_n == 256) return launch_large<kSlowA, kSlowB, 8, 4, Epilogue>(p, pieces, s);
+  if (tile_m == 256 && tile_n == 192) return launch_large<kSlowA, kSlowB, 8, 3, Epilogue>(p, pieces, s);
+  if (tile_m == 192 && tile_n == 256) return launch_large<kSlowA, kSlowB, 6, 4, Epilogue>(p, pieces, s);
+  if (tile_m == 256 && tile_n == 128) return launch_large<kSlowA, kSlowB, 8, 2, Epilogue>(p, pieces, s);
+  if (tile_m == 128 && tile_n == 256) return launch_large<kSlowA, kSlowB, 4, 4, Epilogue>(p, pieces, s);
+  return fail(PICO_ERR_SHAPE, "pico_product_large: tiles of %d x %d (256 x 256, or one side 192 or 128)", tile_m, tile_n);
 }
 
 }  // namespace

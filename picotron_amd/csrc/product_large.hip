@@ -23,29 +23,9 @@
 namespace pico {
 namespace {
 
-template <bool kSlowA, bool kSlowB, int I, int J, bool kParts>
-int launch(LargeParams p, hipStream_t s) {
-  using S = Shape<kSlowA, kSlowB, I, J>;
-  static LdsOnce reserved;
-  if (!reserve_lds_once(reserved, reinterpret_cast<const void*>(&product_large_kernel<kSlowA, kSlowB, I, J, StoreTile<kParts>>), S::kLds))
-    return fail(PICO_ERR_LAUNCH, "pico_product_large: cannot reserve %d bytes of LDS", S::kLds);
-  p.tiles_m = (p.M + S::TM - 1) / S::TM;
-  p.tiles_n = (p.N + S::TN - 1) / S::TN;
-  const int64_t units = static_cast<int64_t>(p.tiles_m) * p.tiles_n * p.parts;
-  // An output larger than the workgroups' one round of tiles would push the operands out of the caches as it is written: [4096 x
-  // 2048] @ [49152 x 2048]^T 638 -> 570 us, [4096 x 1024] @ [49152 x 1024]^T 358 -> 304.
-  p.streaming = !kParts && units > 256;
-  hipLaunchKernelGGL((product_large_kernel<kSlowA, kSlowB, I, J, StoreTile<kParts>>), dim3(static_cast<unsigned>(std::min<int64_t>(units, 256))), dim3(S::kThreads), S::kLds, s, p);
-  return check_launch("pico_product_large");
-}
 template <bool kSlowA, bool kSlowB, bool kParts>
 int launch_shape(const LargeParams& p, int tile_m, int tile_n, hipStream_t s) {
-  if (tile_m == 256 && tile_n == 256) return launch<kSlowA, kSlowB, 8, 4, kParts>(p, s);
-  if (tile_m == 256 && tile_n == 192) return launch<kSlowA, kSlowB, 8, 3, kParts>(p, s);
-  if (tile_m == 192 && tile_n == 256) return launch<kSlowA, kSlowB, 6, 4, kParts>(p, s);
-  if (tile_m == 256 && tile_n == 128) return launch<kSlowA, kSlowB, 8, 2, kParts>(p, s);
-  if (tile_m == 128 && tile_n == 256) return launch<kSlowA, kSlowB, 4, 4, kParts>(p, s);
-  return fail(PICO_ERR_SHAPE, "pico_product_large: tiles of %d x %d (256 x 256, or one side 192 or 128)", tile_m, tile_n);
+  return launch_tiles<kSlowA, kSlowB, StoreTile<kParts>>(p, kParts, tile_m, tile_n, s);
 }
 
 }  // namespace

@@ -118,3 +118,49 @@ def test_norm_weights_of_other_types(device, M, dtype):
     assert all(torch.equal(a, b) for a, b in zip(got[dtype][:3], got[F32][:3]))
     y, _ = functional.rms_norm_linear_8bit(x, r, gamma.to(dtype), EPS, w)
     assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, (x, w), dy), got[F32][1:3]))
+
+
+def in_bits20(v):
+    """fp32 v [rows, cols] rounded to 20 bits: (the first 16 as they lie in bf16, the words of eight times the other four, the values)."""
+    bits = v.view(torch.int32) + 0x800
+    words = ((bits >> 12 & 15).long().view(v.size(0), -1, 8) << torch.arange(0, 32, 4, device=v.device)).sum(-1)
+    return (bits >> 16).to(torch.int16).view(BF16), torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32), (bits & ~0xfff).view(F32)
+
+
+@pytest.mark.parametrize("tile", [(256, 256), (256, 192), (192, 256), (256, 128), (128, 256)])
+@pytest.mark.parametrize("M,N,K", [(256, 256, 128), (1, 16, 136), (300, 272, 576), (1000, 1040, 200), (3000, 4112, 320)])
+def test_a_product_in_20_bits(device, M, N, K, tile):
+    """Of the fp32 sums that the same kernel gives; more tiles than workgroups, tiles cut at every side, nothing written beside them."""
+    import ctypes
+    from picotron_amd import _lib
+    lib, g = _lib.lib(), torch.Generator(device="cuda").manual_seed(M)
+    a, b = randn(M, K + 8, g=g)[:, :K], randn(K, N + 24, g=g)[:, :N]
+    sums = torch.empty(M, N, device="cuda")
+    c, left = torch.full((M * N + 64,), 3.0, dtype=BF16, device="cuda"), torch.full((M * N // 8 + 64,), 77, dtype=torch.int32, device="cuda")
+    p = lambda t, off=0: ctypes.c_void_p(t.data_ptr() + off)      # noqa: E731
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    _lib.check(lib.pico_product_large_sums(p(a), p(b), p(sums), M, N, K, K + 8, N + 24, 0, 1, *tile, 1, stream))
+    _lib.check(lib.pico_product_large_bits20(p(a), p(b), p(c, 64), p(left, 128), M, N, K, K + 8, N + 24, *tile, stream))
+    held, words, _ = in_bits20(sums)
+    assert torch.equal(c[32:-32].view(M, N).view(torch.int16), held.view(torch.int16)) and torch.equal(left[32:-32].view(M, -1), words)
+    assert (c[:32] == 3).all() and (c[-32:] == 3).all() and (left[:32] == 77).all() and (left[-32:] == 77).all()
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 32), (33, 576), (70, 4128)])
+@pytest.mark.parametrize("want_y", [False, True])
+def test_swiglus_gradient_from_20_bits(device, rows, cols, want_y):
+    """As from the same values in fp32, which the two hold."""
+    import ctypes
+    from picotron_amd import _lib, ops
+    lib, g = _lib.lib(), torch.Generator(device="cuda").manual_seed(cols)
+    held, words, whole = in_bits20(torch.randn(rows, cols, generator=g, device="cuda"))
+    gate, up = (ops.mx8_quantize(torch.randn(rows, cols, generator=g, device="cuda") * 2) for _ in range(2))
+    p = lambda t: ctypes.c_void_p(t.data_ptr()) if t is not None else None      # noqa: E731
+    m = lambda t: ctypes.byref(_lib.Mx8(t.data.data_ptr(), t.scales.data_ptr()))      # noqa: E731
+    stream, got = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream), []
+    for call in (lambda *o: lib.pico_swiglu_mx8_bwd_bits20(p(held), p(words), m(gate), m(up), *o), lambda *o: lib.pico_swiglu_mx8_bwd_sums(p(whole), 1, m(gate), m(up), *o)):
+        dg, du = (torch.full((rows + 1, cols + 8), 5.0, dtype=BF16, device="cuda") for _ in range(2))
+        y = torch.full((rows + 1, cols), 5.0, dtype=BF16, device="cuda") if want_y else None
+        _lib.check(call(p(dg), p(du), p(y), rows, cols, cols + 8, cols + 8, stream))
+        got.append([t for t in (dg, du, y) if t is not None])
+    assert all(torch.equal(a, b) for a, b in zip(*got)) and (got[0][0][:, cols:] == 5).all() and (got[0][1][rows] == 5).all()

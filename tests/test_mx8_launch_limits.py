@@ -53,3 +53,15 @@ def test_swiglus_gradient_from_sums(lib):
     assert [call(parts=0), call(parts=65), call(cols=40), call(rows=-1), call(rows=2 ** 27)] == [SHAPE] * 5
     assert [call(dy=None), call(dgate=None), call(gate=ctypes.byref(Mx8(None, 4096)))] == [NULL] * 3
     assert [call(dy=away), call(dgate=away), call(y=away), call(ld=68)] == [-4] * 4 and call(ld=56) == -5 and call(rows=0, dy=None) == 0
+
+
+def test_a_product_in_20_bits_and_the_gradient_from_it(lib):
+    away = ctypes.c_void_p(4096 + 8)
+    def product(a=P, left=P, M=64, N=64, K=256, lda=256, tile=(256, 256)):
+        return lib.pico_product_large_bits20(a, P, P, left, M, N, K, lda, N, *tile, None)
+    assert [product(N=72), product(K=250), product(M=0), product(lda=252), product(K=64, lda=64), product(tile=(64, 64))] == [SHAPE] * 6
+    assert [product(a=None), product(left=None)] == [NULL] * 2 and [product(a=away), product(left=away)] == [-4] * 2
+    def swiglu(dy=P, left=P, rows=4, cols=64, ld=64):
+        return lib.pico_swiglu_mx8_bwd_bits20(dy, left, packed(), packed(), P, P, None, rows, cols, ld, ld, None)
+    assert [swiglu(cols=40), swiglu(rows=2 ** 27)] == [SHAPE] * 2 and [swiglu(dy=None), swiglu(left=None)] == [NULL] * 2
+    assert [swiglu(dy=away), swiglu(left=away), swiglu(ld=68)] == [-4] * 3 and swiglu(ld=56) == -5 and swiglu(rows=0, dy=None) == 0
