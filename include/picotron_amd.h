@@ -549,7 +549,7 @@ int pico_linear_log_probs_bwd(const void* x, const void* w, const int64_t* targe
  * No counterpart in the reference.  A row's values as e4m3, every 32 of them under one power-of-two scale:
  *   data    e4m3 [rows, cols], contiguous, 16-byte aligned; cols a multiple of 32
  *   scales  bytes [ceil(cols / 128), rows, 4], 4-byte aligned: byte (t, r, q) is that of columns 128 t + 32 q .. + 31 of row r and stands for
- *           2^(byte - 127); 255: the block is NaN.  Bytes past the last column are written as 0.
+ *           2^(byte - 127); 255: the block is NaN, whatever its codes are.  Bytes past the last column are 0.
  * A block's scale is the smallest 2^e, e >= -127, for which its largest |value| / 2^e is at most 448; values are rounded to the nearest, ties to even.  A block
  * with an infinity or a NaN becomes NaN as a whole.  rows * ceil(cols / 128) is 2^27 - 8 at most.
  */

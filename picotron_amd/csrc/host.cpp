@@ -1921,9 +1921,10 @@ Rounded rounded_up(const Tensor& dy, const Tensor& w) {
   };
   return {with_zeros(dy, 1), w.defined() ? with_zeros(w, 0) : w};
 }
-// The same where it pays: the library takes other numbers of outputs as they are, and slower.  us for both gradients so and with the copies, rows x in x out: 422 x 4096 x 16533 323, 216;
-// 16000 x 2048 x 2049 472, 288; 2314 x 2048 x 2439 98, 86; 4096 x 4096 x 15001 857, 828; 4096 x 2048 x 5003 180, 191.  Of few inputs the copy of dy costs more than it saves (9216 x 576 x 2772, the layer's step, 176, 188); small ones are bound by
-// their launches.
+// The same where it pays: the library takes other numbers of outputs as they are, and slower.  us for both gradients so and with the copies, rows x in x out: 422 x 4096 x 16533 357, 203;
+// 16000 x 2048 x 2049 492, 282; 2314 x 2048 x 2439 101, 86; 4096 x 4096 x 15001 884, 855.  Over 50 drawn sizes that this takes 0.83 of the time in the geometric mean; eight lose, most with 1100 to
+// 2200 inputs and several thousand outputs, where the copy of dy weighs most (4096 x 2048 x 5003 190, 205; 5469 x 1568 x 11557 437, 514: 1.18, the worst).  Of few inputs it costs more than it saves, and small
+// products are bound by their launches (2183 x 1376 x 962 53, 64).
 Rounded rounded_up_if_it_pays(const Tensor& dy, const Tensor& w, int64_t in) {
   return in >= 1024 && dy.size(0) * dy.size(1) * in >= INT64_C(3000000000) ? rounded_up(dy, w) : Rounded{dy, w};
 }
@@ -2114,7 +2115,7 @@ struct NormLinear8 : torch::autograd::Function<NormLinear8> {
     const bool wants_norm = needs_any(ctx, 0, at_gamma + 1), wants_w = rows.empty() ? ctx->needs_input_grad(at_gamma + 1) : needs_any(ctx, at_gamma + 2, rows.size());
     Tensor dy = upstream(g[0], mx8_rows_of(s[0]));
     if (wants_norm) {
-      const Rounded whole = rounded_up(dy, weight_rows(s[3]));
+      const Rounded whole = rounded_up(dy, weight_rows(s[3]));   // (always: what leaves more than bf16 takes nothing else)
       dy = whole.dy;
       auto [dx, dgamma] = norm_gradients(whole.dy, whole.w, mx8_dense(s[0]), s[5], mx8_dense(s[1]), s[2], g[1].defined() ? OptTensor(mx8_dense(g[1])) : std::nullopt);
       r[0] = dx;

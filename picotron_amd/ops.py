@@ -416,7 +416,7 @@ class Mx8:
     """A tensor held in 8 bits: ``data`` float8_e4m3fn [..., cols] and ``scales`` uint8 [ceil(cols / 128), rows, 4], byte (t, r, q) the power of
     two, 2^(byte - 127), of columns 128 t + 32 q .. + 31 of row r.  The scale of 32 values is the smallest power of two under which they fit e4m3
     (448), so nothing saturates and a value is off by at most 2^-4 of itself (2^-10 of the scale where it is under 2^-6 of it); a block that holds an infinity or
-    a NaN is NaN as a whole.  Made by mx8_quantize and rmsnorm_mx8_fwd."""
+    a NaN is NaN as a whole (byte 255, whatever its codes are); bytes past the last column are 0.  Made by mx8_quantize and rmsnorm_mx8_fwd."""
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor):
         self.data, self.scales = data, scales
@@ -446,6 +446,6 @@ def mx8_product(a: Mx8, b: Mx8) -> torch.Tensor:
 
 def rmsnorm_mx8_fwd(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: Optional[torch.Tensor] = None):
     """rmsnorm(h) * weight for h = x + residual (bf16 or fp32, hidden a multiple of 32 up to 16384), written in 8 bits only: returns (Mx8, rstd fp32 [rows], h or
-    None without a residual).  The sum that is normalised is not rounded to x's dtype on the way, h is."""
+    None without a residual).  The sum that is normalised is not rounded on the way, h is: every code is that of the exact value."""
     data, scales, rstd, h = _lib.host().rmsnorm_mx8_fwd(x, weight, eps, residual)
     return Mx8(data, scales), rstd, h
