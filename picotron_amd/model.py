@@ -149,8 +149,9 @@ def _linear_8bit() -> bool:
 
 def _check_read(name, module, *types):
     """An error where reading the module's weights would not do what calling it does."""
-    if type(module) not in types or "forward" in vars(module) or getattr(module, "bias", None) is not None:
-        raise RuntimeError(f"PICO_LINEAR_8BIT=1 reads {name} as a plain {types[0].__name__} without a bias, which {type(module).__name__} is not")
+    plain = isinstance(module, types) and any(type(module).forward is t.forward for t in types) and "forward" not in vars(module)
+    if not plain or getattr(module, "bias", None) is not None:
+        raise RuntimeError(f"PICO_LINEAR_8BIT=1 reads {name} as a plain {types[0].__name__} without a bias, which this {type(module).__name__} is not")
     if module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks:
         raise RuntimeError(f"PICO_LINEAR_8BIT=1 reads {name} without calling it, and its hooks would be silent")
 

@@ -120,3 +120,36 @@ def test_without_the_switch_hooks_and_modules_are_called(layer, calls, monkeypat
         module.register_forward_hook(lambda m, a, out, name=name: seen.append(name))
     layer(X)
     assert seen == ["input_layernorm", "attention", "post_attention_layernorm", "mlp"] and not calls
+
+
+def test_subclasses_count_by_what_they_compute(layer, calls):
+    from picotron_amd import model as M
+
+    class Named(M.MLP):
+        label = "mine"
+
+    class Doubled(M.MLP):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    layer.mlp.__class__ = Named
+    layer(X)
+    assert len(calls) == 3
+    layer.mlp.__class__ = Doubled
+    with pytest.raises(RuntimeError, match="plain MLP"):
+        layer(X)
+
+
+def test_a_parametrized_projection_is_read_through_its_parametrization(layer, calls, monkeypatch):
+    from picotron_amd import model as M
+    got = []
+    monkeypatch.setattr(M, "swiglu_linear_8bit", lambda gate_up, weight, packed=None: (got.append(weight), gate_up[..., :64])[1])
+
+    class Doubled(nn.Module):
+        def forward(self, w):
+            return 2 * w
+
+    plain = layer.mlp.down_proj.weight.detach().clone()
+    nn.utils.parametrize.register_parametrization(layer.mlp.down_proj, "weight", Doubled())
+    layer(X)
+    assert torch.equal(got[0], 2 * plain) and got[0].requires_grad
