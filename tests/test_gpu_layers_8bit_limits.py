@@ -40,3 +40,56 @@ def test_one_row_of_the_smallest_block(device, rows, out):
         assert y.shape == (*rows, out) and torch.equal(y.reshape(1, -1), z)
         a, b = torch.autograd.grad(y, (t, w), dy), torch.autograd.grad(z, (flat, w), dy.reshape(1, -1))
         assert torch.equal(a[0].reshape(1, -1), b[0]) and torch.equal(a[1], b[1]) and a[0].shape == t.shape
+
+
+# rows, outputs, half of gate and up: the product in front of SwiGLU's gradient by fp32 pieces, by whole fp32 sums, in 20 bits
+ROUTES = [(40, 2048, 512), (300, 72, 576), (2500, 520, 4128)]
+
+
+@pytest.mark.parametrize("M,N,K", ROUTES)
+def test_routes_that_these_sizes_stand_for(device, M, N, K):
+    from picotron_amd import _lib
+    route = _lib.host().sums_route(torch.empty(M, N, dtype=BF16, device="cuda"), torch.empty(N, K, dtype=BF16, device="cuda"))
+    assert route.startswith("large") and " in " not in route if M == 2500 else route.startswith("mid") and (" in " in route) == (M == 40), route
+
+
+@pytest.mark.parametrize("M,N,K", ROUTES)
+def test_infinities_in_the_upstream_gradient_stay_in_their_rows(device, M, N, K):
+    from picotron_amd import functional as F
+    wide, w = leaf(M, 2 * K), leaf(N, K)
+    dy = torch.randn(M, N, device="cuda").to(BF16)
+    bad = dy.clone()
+    bad[1, 3], bad[M // 2, 0], bad[M - 1, 5] = float("inf"), float("nan"), -float("inf")
+    want, = torch.autograd.grad(F.swiglu_linear_8bit(wide, w), wide, dy)
+    got, = torch.autograd.grad(F.swiglu_linear_8bit(wide, w), wide, bad)
+    rows = torch.ones(M, dtype=torch.bool, device="cuda")
+    rows[[1, M // 2, M - 1]] = False
+    assert torch.equal(got[rows], want[rows]) and not got[~rows].isfinite().any(1).all() and got[M // 2].isnan().all()
+    for r in (1, M - 1):
+        assert (~got[r].isfinite() | (got[r] == 0)).all()       # (0: a gate or an up of 0, times an infinity, is NaN; a weight of 0 too)
+
+
+@pytest.mark.parametrize("M,N,K", ROUTES)
+def test_a_captured_gradient_by_every_route(device, M, N, K):
+    from picotron_amd import functional as F
+    g = torch.Generator(device="cuda").manual_seed(K)
+    wide, w = (torch.randn(s, generator=g, device="cuda").to(BF16).requires_grad_() for s in ((M, 2 * K), (N, K)))
+    dy = torch.randn(M, N, generator=g, device="cuda").to(BF16)
+    def step():
+        y = F.swiglu_linear_8bit(wide, w)
+        return (y.detach(), *torch.autograd.grad(y, (wide, w), dy))
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for _ in range(3):
+        with torch.no_grad():
+            wide.copy_(torch.randn(M, 2 * K, generator=g, device="cuda"))
+            dy.copy_(torch.randn(M, N, generator=g, device="cuda"))
+        want = step()
+        for t in held:
+            t.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want))
+        del want
