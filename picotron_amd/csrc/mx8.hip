@@ -104,7 +104,7 @@ __global__ __launch_bounds__(kThreads) void swiglu_mx8_fwd_kernel(const T* __res
 
 // With g, u what the checkpoint stands for and s = sigmoid(g): dgate = dy u s (1 + g (1 - s)), dup = dy g s; y = g s u again where it is wanted.
 // kFrom: dy of rows of pitch dy_ld; or contiguous, in fp32 and in `parts` pieces to be added, as a product leaves it; or contiguous in 20 bits.  [8192, 11008] 145, 184
-// and 154 us, a copy's rate.
+// and 150 us, a copy's rate.
 enum class Upstream { Rows, Sums, Bits20 };
 template <typename T, Upstream kFrom>
 __global__ __launch_bounds__(kThreads) void swiglu_mx8_bwd_kernel(const std::conditional_t<kFrom == Upstream::Sums, float, T>* __restrict__ dy, const uint32_t* __restrict__ dy_left, int parts, const pico_mx8 gate8, const pico_mx8 up8, T* __restrict__ dgate, T* __restrict__ dup,

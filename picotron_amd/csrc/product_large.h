@@ -72,7 +72,7 @@ struct Shape {
 // The tile leaves for c [M, N], rows of pitch ldc, 16 rows and 128 bytes of columns at a time through LDS, as whole lines; what lies past the matrix is
 // dropped by the window.  No wave waits for another here, and the next tile's first steps are on their way.
 // kBits20 (N and ldc multiples of 16): the sums rounded to 20 bits (ties away from 0), of which the first 16 go to c and the others to `left`, [M, ldc / 8] words of eight values.  Four
-// operations a value; bf16 and what its rounding leaves took eight, [4096 x 2048] @ [2048 x 8192] 7 us more.
+// operations a value; bf16 and what its rounding leaves took eight, and the step of [4096 x 8192] and 2048 outputs 1.025 of its time with bf16 for 1.015.
 template <typename Out, int I, int J, bool kBits20 = false>
 __device__ __forceinline__ void store_tile(Out* c, int64_t first_row, int M, int N, int ldc, bool streaming, const Unit& u, int wm, int wn, int lane, unsigned char* rows, const f32x4 (&acc)[I][J],
                                            uint32_t* left = nullptr) {
